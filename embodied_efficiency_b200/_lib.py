@@ -5,6 +5,7 @@ The shared library is the only compute path: every entry point here raises
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -80,6 +81,17 @@ SIGNATURES = {
     "ee_expert_head": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int32,
                                  c_int64, c_int64, c_int32, c_void_p]),
     "ee_euler_step": (c_int32, [c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_float, c_int32, c_void_p]),
+    "ee_quantize_tokens": (c_int32, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int32, c_void_p]),
+    "ee_int8_gemm": (c_int32, [c_void_p] * 7 + [c_int64] * 3 + [c_int32] * 3 + [c_void_p]),
+    "ee_int8_linear_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "ee_int8_linear": (c_int32, [c_void_p, c_int64] + [c_void_p] * 6 + [c_size_t] + [c_int64] * 3 + [c_int32] * 3
+                       + [c_void_p]),
+    "ee_rotary": (c_int32, [c_void_p, c_int64, c_int64] * 4 + [c_void_p, c_int64, c_int32, c_void_p, c_int64, c_int32,
+                                                               c_int32, c_int32, c_void_p, c_int32, c_int32, c_int32,
+                                                               c_void_p]),
+    "ee_prompt_attention_workspace_bytes": (c_size_t, [c_int64, c_int64] + [c_int32] * 4),
+    "ee_prompt_attention": (c_int32, [c_void_p, c_int64, c_int64] * 4 + [c_void_p] * 3 + [c_int64, c_int64]
+                            + [c_int32] * 5 + [c_float, c_int32, c_void_p, c_size_t, c_void_p]),
     "ee_flow_sample_traced": (c_int32, [ctypes.POINTER(Expert), c_void_p, c_void_p, c_void_p, c_int32,
                                         c_int32, c_void_p, c_size_t, c_void_p, c_void_p]),
     "ee_flow_sample_phases": (c_int32, [ctypes.POINTER(Expert), c_int32]),
@@ -152,6 +164,29 @@ def require_cuda(*tensors):
         if t is not None and not t.is_cuda:
             raise RuntimeError("embodied_efficiency_b200 kernels need CUDA tensors "
                                f"(got a tensor on {t.device}); there is no CPU path")
+
+
+def on_device(device):
+    """Context in which kernels launch on ``device``: nothing when it is the current one already."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def same_device(*tensors):
+    """The one device of CUDA ``tensors`` (``None`` entries apart)."""
+    require_cuda(*tensors)
+    dev = None
+    for t in tensors:
+        if t is not None:
+            dev = dev or t.device
+            if t.device != dev:
+                raise ValueError(f"tensors on different devices: {dev} and {t.device}")
+    return dev
+
+
+def no_grad_through(what: str, *tensors):
+    """These kernels have no backward pass: an input that asks for one is refused."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() or detach its inputs")
 
 
 def ptr(t) -> int:

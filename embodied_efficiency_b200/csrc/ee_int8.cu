@@ -1,0 +1,273 @@
+// ee_int8.cu -- C ABI: 8-bit integer linears with a scale for each token and
+// each output channel,
+//   y[m][n] = epi( (sum_k xq[m][k] * w[n][k]) * sx[m] * sw[n] + bias[n] ),
+// and the token quantiser xq = rint(x / sx), sx = max(amax |x| / 127, 1e-8).
+#include <atomic>
+
+#include "ee_common.cuh"
+#include "ee_host.h"
+
+namespace ee {
+
+// ---------------------------------------------------------------------------
+// token quantiser
+// ---------------------------------------------------------------------------
+// W warps share a row; a lane keeps its first kQChunks 16-byte chunks in
+// registers between the maximum and the rounding (longer rows read the rest
+// again). The maximum is taken over the 15-bit magnitudes as integers, so an
+// infinity or NaN wins it: such a token gets codes of 0 and a NaN scale.
+constexpr int kQChunks = 8;
+constexpr int kQThreads = 256;
+
+// nearest integer (ties to even) of the fp32 quotient v / s, as the low byte
+// of an int: t = v * (1 / s) is within 1.5 ulp of it, so only a t that close
+// to a tie is divided for
+EE_DEV uint32_t quant_word(const float (&v)[4], float s, float inv) {
+  uint32_t b[4];
+  bool near = false;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float t = v[e] * inv;
+    const float r = t + 12582912.f;  // 1.5 * 2^23: the sum's rounding is rint(t)
+    b[e] = __float_as_uint(r);
+    near |= fabsf(fabsf(t - (r - 12582912.f)) - 0.5f) < 6.103515625e-5f;
+  }
+  if (near) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) b[e] = __float_as_uint(__fdiv_rn(v[e], s) + 12582912.f);
+  }
+  return prmt(prmt(b[0], b[1], 0x0040u), prmt(b[2], b[3], 0x0040u), 0x5410u);
+}
+
+template <typename T, int W>
+__global__ void __launch_bounds__(kQThreads) quantize_tokens_kernel(const T* __restrict__ x, int8_t* __restrict__ xq,
+                                                                    float* __restrict__ sx, long long rows, int cols,
+                                                                    long long ldx) {
+  pdl_entry();
+  constexpr int RPB = kQThreads / (32 * W);  // rows per CTA
+  __shared__ uint32_t part[kQThreads / 32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long row = (long long)blockIdx.x * RPB + warp / W;
+  const bool live = row < rows;
+  const int c0 = (warp % W) * 32 + lane, nch = cols >> 3;
+  const T* xr = x + (live ? row : 0) * ldx;
+  uint4 q[kQChunks];
+  uint32_t mx = 0;
+  auto magnitude = [&](const uint4& w) {
+    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) mx = max(mx, max(ws[e] & 0x7FFFu, (ws[e] >> 16) & 0x7FFFu));
+  };
+#pragma unroll
+  for (int i = 0; i < kQChunks; ++i) {
+    const int c = c0 + i * 32 * W;
+    q[i] = c < nch && live ? *reinterpret_cast<const uint4*>(xr + 8 * c) : make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < kQChunks; ++i) magnitude(q[i]);
+  if (live)
+    for (int c = c0 + kQChunks * 32 * W; c < nch; c += 32 * W) magnitude(*reinterpret_cast<const uint4*>(xr + 8 * c));
+  mx = __reduce_max_sync(0xffffffffu, mx);
+  if (W > 1) {
+    if (lane == 0) part[warp] = mx;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < W; ++i) mx = max(mx, part[warp / W * W + i]);
+  }
+  if (!live) return;
+  const float amax = Act<T>::unpack2(mx).x;
+  const bool finite = amax <= 3.4028234e38f;  // false for infinities and NaN
+  const float s = fmaxf(__fdiv_rn(amax, 127.f), 1e-8f);
+  const float inv = finite ? __frcp_rn(s) : 0.f;
+  if (c0 == 0) sx[row] = finite ? s : __int_as_float(0x7fffffff);
+  int8_t* qr = xq + row * cols;
+  auto store = [&](const uint4& w, int c) {
+    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+    uint32_t o[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float2 f = Act<T>::unpack2(ws[2 * h]), g = Act<T>::unpack2(ws[2 * h + 1]);
+      const float v[4] = {f.x, f.y, g.x, g.y};
+      o[h] = finite ? quant_word(v, s, inv) : 0u;
+    }
+    *reinterpret_cast<uint2*>(qr + 8 * c) = make_uint2(o[0], o[1]);
+  };
+#pragma unroll
+  for (int i = 0; i < kQChunks; ++i) {
+    const int c = c0 + i * 32 * W;
+    if (c < nch) store(q[i], c);
+  }
+  for (int c = c0 + kQChunks * 32 * W; c < nch; c += 32 * W) store(*reinterpret_cast<const uint4*>(xr + 8 * c), c);
+}
+
+template <typename T>
+static int launch_quantize(const T* x, int8_t* xq, float* sx, long long rows, int cols, long long ldx, cudaStream_t s) {
+  // warps per row: few enough that every lane has chunks, enough that a row stays in registers
+  const int per = 32 * kQChunks, nch = cols / 8;
+  const int w = nch <= per ? 1 : (nch <= 2 * per ? 2 : (nch <= 4 * per ? 4 : 8));
+  const long long rpb = kQThreads / (32 * w);
+  const dim3 grid((unsigned)((rows + rpb - 1) / rpb)), blk(kQThreads);
+  cudaError_t e;
+  if (w == 1) e = launch_pdl(quantize_tokens_kernel<T, 1>, grid, blk, 0, s, x, xq, sx, rows, cols, ldx);
+  else if (w == 2) e = launch_pdl(quantize_tokens_kernel<T, 2>, grid, blk, 0, s, x, xq, sx, rows, cols, ldx);
+  else if (w == 4) e = launch_pdl(quantize_tokens_kernel<T, 4>, grid, blk, 0, s, x, xq, sx, rows, cols, ldx);
+  else e = launch_pdl(quantize_tokens_kernel<T, 8>, grid, blk, 0, s, x, xq, sx, rows, cols, ldx);
+  return e == cudaSuccess ? EE_OK : EE_ERR_LAUNCH;
+}
+
+// ---------------------------------------------------------------------------
+// product
+// ---------------------------------------------------------------------------
+struct Int8Args {
+  const int8_t* xq;      // [M][K]
+  const float* sx;       // [M]
+  const int8_t* w;       // [N][K]
+  const void* sw;        // [N] fp32 or fp16
+  const void *bias, *resid;
+  void* out;
+  int M, N, K;
+  int sw_f16, epi;
+};
+enum { I8_BIAS = 1, I8_GELU = 2, I8_RESID = 4 };
+
+EE_DEV float i8_wscale(const Int8Args& a, int n) {
+  return a.sw_f16 ? __half2float(__ldg(reinterpret_cast<const __half*>(a.sw) + n))
+                  : __ldg(reinterpret_cast<const float*>(a.sw) + n);
+}
+// the epilogue of one output in fp32 (one rounding, by the caller)
+template <typename T> EE_DEV float i8_epi(const Int8Args& a, int acc, float sx, float sw, int m, int n) {
+  float y = (float)acc * sx * sw;
+  if (a.epi & I8_BIAS) y += ld_param(reinterpret_cast<const T*>(a.bias) + n);
+  if (a.epi & I8_GELU) y = gelu_erf(y);
+  if (a.epi & I8_RESID) y += ld_param(reinterpret_cast<const T*>(a.resid) + (size_t)m * a.N + n);
+  return y;
+}
+
+// 64 x 64 outputs per CTA, 4 x 4 per thread, 64-byte K steps through shared memory, dp4a
+template <typename T>
+__global__ void __launch_bounds__(256) int8_gemm_kernel(const __grid_constant__ Int8Args a) {
+  pdl_entry();
+  __shared__ int xs[64][17], ws[64][17];
+  const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  int acc[4][4] = {};
+  for (int k0 = 0; k0 < a.K; k0 += 64) {
+    for (int i = threadIdx.x; i < 64 * 16; i += 256) {
+      const int r = i >> 4, c = i & 15, k = k0 + 4 * c;
+      xs[r][c] = (m0 + r < a.M && k < a.K) ? *reinterpret_cast<const int*>(a.xq + (size_t)(m0 + r) * a.K + k) : 0;
+      ws[r][c] = (n0 + r < a.N && k < a.K) ? *reinterpret_cast<const int*>(a.w + (size_t)(n0 + r) * a.K + k) : 0;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < 16; ++c) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(xs[ty + 16 * i][c], ws[tx + 16 * j][c], acc[i][j]);
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
+      if (m < a.M && n < a.N)
+        reinterpret_cast<T*>(a.out)[(size_t)m * a.N + n] = Act<T>::from_f(i8_epi<T>(a, acc[i][j], a.sx[m], i8_wscale(a, n), m, n));
+    }
+}
+
+template <typename T>
+static int launch_int8(const Int8Args& a, cudaStream_t s) {
+  const dim3 grid((a.N + 63) / 64, (a.M + 63) / 64);
+  if (grid.y > 65535) return EE_ERR_SHAPE;
+  return launch_pdl(int8_gemm_kernel<T>, grid, dim3(256), 0, s, a) == cudaSuccess ? EE_OK : EE_ERR_LAUNCH;
+}
+
+static int check_product(const void* weight, const void* w_scales, const void* bias, const void* residual, void* y,
+                         int64_t m, int64_t n, int64_t k, int32_t scale_dtype, int32_t act_dtype, int32_t epilogue) {
+  if (act_dtype != EE_BF16 && act_dtype != EE_F16) return EE_ERR_DTYPE;
+  if (scale_dtype != EE_F32 && scale_dtype != EE_F16) return EE_ERR_DTYPE;
+  if ((epilogue & ~(EE_EPI_BIAS | EE_EPI_GELU | EE_EPI_RESIDUAL)) != 0) return EE_ERR_ARG;
+  if ((epilogue & EE_EPI_GELU) && (epilogue & EE_EPI_RESIDUAL)) return EE_ERR_ARG;
+  // an int32 sum holds 131071 products of two codes (2^31 / 2^14)
+  if (m < 0 || n < 0 || k < 16 || (k % 16) != 0 || k > 131056 || m > 0x7fffff00 || n > 0x7fffff00) return EE_ERR_SHAPE;
+  if (m == 0 || n == 0) return EE_OK;
+  if (!weight || !w_scales || !y) return EE_ERR_ARG;
+  if (((epilogue & EE_EPI_BIAS) && !bias) || ((epilogue & EE_EPI_RESIDUAL) && !residual)) return EE_ERR_ARG;
+  if (!aligned16(weight) || !aligned16(y) || !aligned16(w_scales) || (bias && !aligned16(bias)) ||
+      (residual && !aligned16(residual)))
+    return EE_ERR_ALIGN;
+  return EE_OK;
+}
+
+static int int8_product(const int8_t* xq, const float* sx, const void* weight, const void* w_scales, const void* bias,
+                        const void* residual, void* y, int64_t m, int64_t n, int64_t k, int32_t scale_dtype,
+                        int32_t act_dtype, int32_t epilogue, cudaStream_t s) {
+  Int8Args a{};
+  a.xq = xq; a.sx = sx;
+  a.w = reinterpret_cast<const int8_t*>(weight);
+  a.sw = w_scales;
+  a.bias = bias; a.resid = residual; a.out = y;
+  a.M = (int)m; a.N = (int)n; a.K = (int)k;
+  a.sw_f16 = scale_dtype == EE_F16;
+  a.epi = epilogue;
+  return act_dtype == EE_BF16 ? launch_int8<__nv_bfloat16>(a, s) : launch_int8<__half>(a, s);
+}
+
+}  // namespace ee
+
+using namespace ee;
+
+extern "C" {
+
+int ee_quantize_tokens(const void* x, int64_t ldx, int8_t* xq, float* x_scales, int64_t m, int64_t k,
+                       int32_t act_dtype, ee_stream_t stream) {
+  if (act_dtype != EE_BF16 && act_dtype != EE_F16) return EE_ERR_DTYPE;
+  if (m < 0 || m > 0x7fffff00 || k < 16 || (k % 16) != 0 || k > 131056 || ldx < k || (ldx % 8) != 0)
+    return EE_ERR_SHAPE;
+  if (m == 0) return EE_OK;
+  if (!x || !xq || !x_scales) return EE_ERR_ARG;
+  if (!aligned16(x) || !aligned16(xq) || !aligned16(x_scales)) return EE_ERR_ALIGN;
+  const int rc = check_device();
+  if (rc) return rc;
+  cudaStream_t s = (cudaStream_t)stream;
+  return act_dtype == EE_BF16
+             ? launch_quantize(reinterpret_cast<const __nv_bfloat16*>(x), xq, x_scales, m, (int)k, ldx, s)
+             : launch_quantize(reinterpret_cast<const __half*>(x), xq, x_scales, m, (int)k, ldx, s);
+}
+
+int ee_int8_gemm(const int8_t* xq, const float* x_scales, const void* weight, const void* w_scales, const void* bias,
+                 const void* residual, void* y, int64_t m, int64_t n, int64_t k, int32_t scale_dtype,
+                 int32_t act_dtype, int32_t epilogue, ee_stream_t stream) {
+  int rc = check_product(weight, w_scales, bias, residual, y, m, n, k, scale_dtype, act_dtype, epilogue);
+  if (rc || m == 0 || n == 0) return rc;
+  if (!xq || !x_scales) return EE_ERR_ARG;
+  if (!aligned16(xq) || !aligned16(x_scales)) return EE_ERR_ALIGN;
+  rc = check_device();
+  if (rc) return rc;
+  return int8_product(xq, x_scales, weight, w_scales, bias, residual, y, m, n, k, scale_dtype, act_dtype, epilogue,
+                      (cudaStream_t)stream);
+}
+
+size_t ee_int8_linear_workspace_bytes(int64_t m, int64_t k) {
+  if (m < 0 || k < 0 || m > 0x7fffff00 || k > 131056) return 0;
+  return (((size_t)m * (size_t)k + 15) & ~(size_t)15) + (size_t)m * 4;
+}
+
+int ee_int8_linear(const void* x, int64_t ldx, const void* weight, const void* w_scales, const void* bias,
+                   const void* residual, void* y, void* workspace, size_t workspace_bytes, int64_t m, int64_t n,
+                   int64_t k, int32_t scale_dtype, int32_t act_dtype, int32_t epilogue, ee_stream_t stream) {
+  int rc = check_product(weight, w_scales, bias, residual, y, m, n, k, scale_dtype, act_dtype, epilogue);
+  if (rc || m == 0 || n == 0) return rc;
+  if (!workspace || workspace_bytes < ee_int8_linear_workspace_bytes(m, k)) return EE_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return EE_ERR_ALIGN;
+  int8_t* xq = reinterpret_cast<int8_t*>(workspace);
+  float* sx = reinterpret_cast<float*>(xq + (((size_t)m * (size_t)k + 15) & ~(size_t)15));
+  rc = ee_quantize_tokens(x, ldx, xq, sx, m, k, act_dtype, stream);
+  if (rc) return rc;
+  return int8_product(xq, sx, weight, w_scales, bias, residual, y, m, n, k, scale_dtype, act_dtype, epilogue,
+                      (cudaStream_t)stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,290 @@
+// ee_prompt.cu -- C ABI: attention over packed prompts (causal or full,
+// grouped heads, keys that may reach further back than the queries).
+#include <atomic>
+
+#include "ee_host.h"
+#include "ee_prompt.cuh"
+
+namespace ee {
+
+// ---------------------------------------------------------------------------
+// few query rows per key head
+// ---------------------------------------------------------------------------
+// A row is (token, head of the key head's group), so a key head's whole group
+// shares one read of its keys. A CTA takes 16 RT rows of one sequence and key
+// head; its 8 warps are RT row tiles x 8 / RT key groups, each with its own
+// running maximum and sum over its share of every 128-key stage, merged
+// through shared memory at the end.
+constexpr int kPrKeys = 128;   // keys per stage
+constexpr int kPrStages = 3;
+template <int HD> constexpr int pr_smem() { return kPrStages * 2 * kPrKeys * HD * 2; }
+
+EE_DEV void pr_ldsm(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+EE_DEV void pr_ldsm_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+
+template <typename T, int HD, int RT>
+__global__ void __launch_bounds__(kThreads) prompt_rows_kernel(const __grid_constant__ PromptArgs a) {
+  constexpr int KG = kWarps / RT;        // key groups
+  constexpr int WK = kPrKeys / KG;       // keys of a stage per warp
+  constexpr int RB = HD * 2;             // bytes per key row
+  constexpr int CH = HD / 8;             // 16-byte chunks per key row
+  constexpr int TILE = kPrKeys * RB;
+  extern __shared__ __align__(128) char smem[];
+  __shared__ int sh[kWarps + 2];
+  pdl_entry();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rt = warp % RT, kg = warp / RT, g = lane >> 2, t = lane & 3;
+  const int kvh = blockIdx.y, part = blockIdx.x % a.splits;
+  PromptSeq s;
+  if (!prompt_find(a, blockIdx.x / a.splits, a.group, 16 * RT, kThreads, sh, s)) return;
+  const int rows = s.qlen * a.group, r0 = s.blk * 16 * RT;
+  // keys this CTA's rows see at most, and its part of them in whole stages
+  const int last_tok = (min(r0 + 16 * RT, rows) - 1) / a.group;
+  const int kend = a.causal ? max(min(s.klen, s.klen - s.qlen + last_tok + 1), 0) : s.klen;
+  const int nst = (kend + kPrKeys - 1) / kPrKeys;
+  const int st0 = (int)((long long)nst * part / a.splits), st1 = (int)((long long)nst * (part + 1) / a.splits);
+  const uint32_t sb = smem_u32(smem);
+  auto off = [](int row, int ch) { return row * RB + (((ch) ^ (row & 7)) << 4); };
+  auto load = [&](int st, int buf) {
+    const int k0 = st * kPrKeys, valid = kend - k0;  // keys past the last seen one are zero-filled
+    const char* kb = reinterpret_cast<const char*>(a.k) + ((long long)(s.k0 + k0) * a.k_tok + kvh * a.k_head) * 2;
+    const char* vb = reinterpret_cast<const char*>(a.v) + ((long long)(s.k0 + k0) * a.v_tok + kvh * a.v_head) * 2;
+    const uint32_t d = sb + buf * 2 * TILE;
+#pragma unroll 4
+    for (int i = tid; i < kPrKeys * CH; i += kThreads) {
+      const int row = i / CH, ch = i % CH;
+      const bool ok = row < valid;
+      cp_async16(d + off(row, ch), kb + (ok ? (long long)row * a.k_tok * 2 + ch * 16 : 0), ok);
+      cp_async16(d + TILE + off(row, ch), vb + (ok ? (long long)row * a.v_tok * 2 + ch * 16 : 0), ok);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kPrStages - 1; ++i) {
+    if (st0 + i < st1) load(st0 + i, i);
+    cp_async_commit();
+  }
+  // this warp's query fragments
+  const int ra = r0 + rt * 16 + g, rb = ra + 8;
+  uint32_t qf[HD / 16][4];
+  {
+    auto qrow = [&](int r) {
+      const int tok = r / a.group, h = kvh * a.group + r % a.group;
+      return reinterpret_cast<const char*>(a.q) + ((long long)(s.q0 + tok) * a.q_tok + h * a.q_head) * 2;
+    };
+    const char *pa = qrow(min(ra, rows - 1)), *pb = qrow(min(rb, rows - 1));
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ++ks) {
+      qf[ks][0] = *reinterpret_cast<const uint32_t*>(pa + ks * 32 + t * 4);
+      qf[ks][1] = *reinterpret_cast<const uint32_t*>(pb + ks * 32 + t * 4);
+      qf[ks][2] = *reinterpret_cast<const uint32_t*>(pa + ks * 32 + 16 + t * 4);
+      qf[ks][3] = *reinterpret_cast<const uint32_t*>(pb + ks * 32 + 16 + t * 4);
+    }
+  }
+  // keys below lim are seen by rows ra and rb
+  const int lim0 = a.causal ? min(s.klen, s.klen - s.qlen + ra / a.group + 1) : s.klen;
+  const int lim1 = a.causal ? min(s.klen, s.klen - s.qlen + rb / a.group + 1) : s.klen;
+  float o[HD / 8][4];
+#pragma unroll
+  for (int i = 0; i < HD / 8; ++i)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[i][c] = 0.f;
+  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+  const int mi = lane >> 3;
+  for (int st = st0; st < st1; ++st) {
+    if (st + kPrStages - 1 < st1) load(st + kPrStages - 1, (st - st0 + kPrStages - 1) % kPrStages);
+    cp_async_commit();
+    cp_async_wait<kPrStages - 1>();
+    __syncthreads();
+    const uint32_t kt = sb + ((st - st0) % kPrStages) * 2 * TILE, vt = kt + TILE;
+#pragma unroll
+    for (int k1 = 0; k1 < WK; k1 += 16) {
+      const int kl = kg * WK + k1;             // first of 16 keys, in the stage
+      const int key = st * kPrKeys + kl;       // and in the sequence
+      if (key >= kend) break;
+      float p[2][4] = {};
+#pragma unroll
+      for (int ks = 0; ks < HD / 16; ++ks) {
+        uint32_t b[4];
+        pr_ldsm(kt + off(kl + (mi >> 1) * 8 + (lane & 7), 2 * ks + (mi & 1)), b);
+        mma16816<T>(p[0], qf[ks][0], qf[ks][1], qf[ks][2], qf[ks][3], b[0], b[1]);
+        mma16816<T>(p[1], qf[ks][0], qf[ks][1], qf[ks][2], qf[ks][3], b[2], b[3]);
+      }
+      float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int kk = key + 8 * j + 2 * t + c;
+          p[j][c] = kk < lim0 ? p[j][c] * a.scale_log2 : -INFINITY;
+          p[j][2 + c] = kk < lim1 ? p[j][2 + c] * a.scale_log2 : -INFINITY;
+          x0 = fmaxf(x0, p[j][c]);
+          x1 = fmaxf(x1, p[j][2 + c]);
+        }
+      }
+#pragma unroll
+      for (int d = 1; d < 4; d <<= 1) {
+        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
+        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
+      }
+      const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+      // nothing seen yet: any finite reference will do, exp2(-inf) = 0
+      const float u0 = n0 == -INFINITY ? 0.f : n0, u1 = n1 == -INFINITY ? 0.f : n1;
+      const float c0 = exp2f(m0 - u0), c1 = exp2f(m1 - u1);
+      m0 = n0;
+      m1 = n1;
+      l0 *= c0;
+      l1 *= c1;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          p[j][c] = exp2f(p[j][c] - u0);
+          p[j][2 + c] = exp2f(p[j][2 + c] - u1);
+          l0 += p[j][c];
+          l1 += p[j][2 + c];
+        }
+      }
+      const uint32_t pa0 = Act<T>::pack2(p[0][0], p[0][1]), pa1 = Act<T>::pack2(p[0][2], p[0][3]);
+      const uint32_t pa2 = Act<T>::pack2(p[1][0], p[1][1]), pa3 = Act<T>::pack2(p[1][2], p[1][3]);
+#pragma unroll
+      for (int d = 0; d < HD / 16; ++d) {
+        uint32_t b[4];
+        pr_ldsm_t(vt + off(kl + (mi & 1) * 8 + (lane & 7), 2 * d + (mi >> 1)), b);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          o[2 * d + c][0] *= c0;
+          o[2 * d + c][1] *= c0;
+          o[2 * d + c][2] *= c1;
+          o[2 * d + c][3] *= c1;
+        }
+        mma16816<T>(o[2 * d], pa0, pa1, pa2, pa3, b[0], b[1]);
+        mma16816<T>(o[2 * d + 1], pa0, pa1, pa2, pa3, b[2], b[3]);
+      }
+    }
+    __syncthreads();
+  }
+  cp_async_wait<0>();
+#pragma unroll
+  for (int d = 1; d < 4; d <<= 1) {
+    l0 += __shfl_xor_sync(0xffffffffu, l0, d);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, d);
+  }
+  // merge the key groups: [warp][16 rows][HD + 4] fp32 over the stages
+  constexpr int ML = HD + 4;
+  static_assert(kWarps * 16 * ML * 4 <= kPrStages * 2 * kPrKeys * RB, "the merge fits the stages");
+  float* mg = reinterpret_cast<float*>(smem) + warp * 16 * ML;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < HD / 8; ++i) {
+    *reinterpret_cast<float2*>(mg + g * ML + 8 * i + 2 * t) = make_float2(o[i][0], o[i][1]);
+    *reinterpret_cast<float2*>(mg + (g + 8) * ML + 8 * i + 2 * t) = make_float2(o[i][2], o[i][3]);
+  }
+  if (t == 0) {
+    mg[g * ML + HD] = m0;
+    mg[g * ML + HD + 1] = l0;
+    mg[(g + 8) * ML + HD] = m1;
+    mg[(g + 8) * ML + HD + 1] = l1;
+  }
+  __syncthreads();
+  // 8 threads per row: each sums 1/8 of the row's values over the key groups
+  for (int i = tid; i < 16 * RT * (HD / 4); i += kThreads) {
+    const int r = i / (HD / 4), c = (i % (HD / 4)) * 4;
+    if (r0 + r >= rows) continue;
+    const float* base = reinterpret_cast<const float*>(smem) + ((r >> 4) * 16 + (r & 15)) * ML;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < KG; ++w) m = fmaxf(m, base[w * RT * 16 * ML + HD]);
+    const float u = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < KG; ++w) {
+      const float* p = base + w * RT * 16 * ML;
+      const float f = exp2f(p[HD] - u);
+      const float4 v = *reinterpret_cast<const float4*>(p + c);
+      l += f * p[HD + 1];
+      acc.x += f * v.x;
+      acc.y += f * v.y;
+      acc.z += f * v.z;
+      acc.w += f * v.w;
+    }
+    const int tok = s.q0 + (r0 + r) / a.group, h = kvh * a.group + (r0 + r) % a.group;
+    const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees no key is zero
+    *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + (long long)tok * a.o_tok + h * a.o_head + c) =
+        make_uint2(Act<T>::pack2(acc.x * inv, acc.y * inv), Act<T>::pack2(acc.z * inv, acc.w * inv));
+  }
+}
+
+template <typename T, int HD, int RT>
+static int launch_rows(const PromptArgs& a, cudaStream_t s) {
+  auto fn = prompt_rows_kernel<T, HD, RT>;
+  static std::atomic<int> set[64];
+  allow_max_smem(fn, set);
+  // at most one partial block per sequence beyond the rows' whole blocks
+  const long long units = (long long)a.tq * a.group / (16 * RT) + a.n_seq;
+  if (units * a.splits > 0x7fffffff) return EE_ERR_SHAPE;
+  return launch_pdl(fn, dim3((unsigned)(units * a.splits), a.n_kv), dim3(kThreads), pr_smem<HD>(), s, a) == cudaSuccess
+             ? EE_OK
+             : EE_ERR_LAUNCH;
+}
+
+template <typename T>
+static int launch_prompt(const PromptArgs& a, int hd, cudaStream_t s) {
+  const bool few = (long long)a.tq * a.group <= 16LL * a.n_seq;
+  if (hd == 64) return few ? launch_rows<T, 64, 1>(a, s) : launch_rows<T, 64, 4>(a, s);
+  return few ? launch_rows<T, 128, 1>(a, s) : launch_rows<T, 128, 4>(a, s);
+}
+
+}  // namespace ee
+
+using namespace ee;
+
+extern "C" {
+
+size_t ee_prompt_attention_workspace_bytes(int64_t tq, int64_t tk, int32_t n_seq, int32_t n_q, int32_t n_kv,
+                                           int32_t head_dim) {
+  (void)tq; (void)tk; (void)n_seq; (void)n_q; (void)n_kv; (void)head_dim;
+  return 0;
+}
+
+int ee_prompt_attention(const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok, int64_t k_head,
+                        const void* v, int64_t v_tok, int64_t v_head, void* out, int64_t o_tok, int64_t o_head,
+                        const int32_t* cu_q, const int32_t* cu_k, const int32_t* k_lens, int64_t tq, int64_t tk,
+                        int32_t n_seq, int32_t n_q, int32_t n_kv, int32_t head_dim, int32_t causal, float scale,
+                        int32_t act_dtype, void* workspace, size_t workspace_bytes, ee_stream_t stream) {
+  if (act_dtype != EE_BF16 && act_dtype != EE_F16) return EE_ERR_DTYPE;
+  if (head_dim != 64 && head_dim != 128) return EE_ERR_UNSUPPORTED;
+  if (tq < 0 || tk < 0 || n_seq < 0 || n_q < 1 || n_kv < 1 || n_q % n_kv != 0) return EE_ERR_SHAPE;
+  if (tq > 0x7fffff00 || tk > 0x7fffff00 || n_kv > 65535 || n_q > 65535) return EE_ERR_SHAPE;
+  if (!(scale > 0.f) || scale > 3.0e38f) return EE_ERR_ARG;
+  if (tq == 0 || n_seq == 0) return EE_OK;
+  if (!q || !out || !cu_q || (tk && (!k || !v)) || (!cu_k && tk != tq)) return EE_ERR_ARG;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out)) return EE_ERR_ALIGN;
+  if (((uintptr_t)cu_q | (uintptr_t)cu_k | (uintptr_t)k_lens) & 3) return EE_ERR_ALIGN;
+  if ((q_tok | q_head | k_tok | k_head | v_tok | v_head | o_tok | o_head) % 8 != 0) return EE_ERR_ALIGN;
+  const int rc = check_device();
+  if (rc) return rc;
+  (void)workspace; (void)workspace_bytes;
+  PromptArgs a{};
+  a.q = q; a.k = k; a.v = v; a.out = out;
+  a.cu_q = cu_q;
+  a.cu_k = cu_k ? cu_k : cu_q;
+  a.k_lens = k_lens;
+  a.q_tok = q_tok; a.q_head = q_head; a.k_tok = k_tok; a.k_head = k_head;
+  a.v_tok = v_tok; a.v_head = v_head; a.o_tok = o_tok; a.o_head = o_head;
+  a.tq = (int)tq; a.tk = (int)tk; a.n_seq = n_seq;
+  a.n_q = n_q; a.n_kv = n_kv; a.group = n_q / n_kv;
+  a.causal = causal != 0;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.splits = 1;
+  cudaStream_t s = (cudaStream_t)stream;
+  return act_dtype == EE_BF16 ? launch_prompt<__nv_bfloat16>(a, head_dim, s) : launch_prompt<__half>(a, head_dim, s);
+}
+
+}  // extern "C"

@@ -141,6 +141,124 @@ def wq_linear(x, weight, scales, bias, group_size, bits, zeros=None, gelu=False,
     return y.reshape(*lead, n).to(out_dtype)
 
 
+# ---------------------------------------------------------------------------
+# 8-bit integer linears: a scale for each token and each output channel
+# ---------------------------------------------------------------------------
+def _token_rows(x, k):
+    """x [..., k] as rows of the kernels: a 2-D view where its strides allow one, else a copy."""
+    xf = x.reshape(-1, k)
+    if xf.stride(-1) != 1 or xf.stride(0) % 8 or xf.stride(0) < k or xf.data_ptr() % 16:
+        xf = xf.clone(memory_format=torch.contiguous_format)
+    return xf
+
+
+def _check_int8_operands(weight, scales, bias, residual, k, dtype, out_shape):
+    if weight.dim() != 2 or weight.dtype != torch.int8:
+        raise ValueError(f"weight must be int8 [N, K], got {weight.dtype} {tuple(weight.shape)}")
+    n = weight.shape[0]
+    if weight.shape[1] != k:
+        raise ValueError(f"activations have K={k}, weight has K={weight.shape[1]}")
+    if k < 16 or k % 16 or k > 131056:
+        raise ValueError(f"K must be a multiple of 16, at most 131056 (32-bit sums), got {k}")
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"outputs are bf16 or fp16, not {dtype}")
+    if scales.numel() != n or scales.dtype not in (torch.float32, torch.float16):
+        raise ValueError(f"scales must be {n} float32 or float16 values (one per output channel), "
+                         f"got {scales.dtype} {tuple(scales.shape)}")
+    if bias is not None and bias.numel() != n:
+        raise ValueError(f"bias has {bias.numel()} values, expected {n}")
+    if residual is not None and tuple(residual.shape) != tuple(out_shape):
+        raise ValueError(f"residual has shape {tuple(residual.shape)}, expected {tuple(out_shape)}")
+    return n
+
+
+def _aligned(t):
+    """t contiguous on a 16-byte boundary (a copy where it is not)."""
+    if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _int8_epilogue(scales, bias, gelu, residual, dtype):
+    if gelu and residual is not None:
+        raise ValueError("gelu and residual do not combine")
+    b = _aligned(bias if bias is None or bias.dtype == dtype else bias.to(dtype))
+    r = _aligned(residual if residual is None or residual.dtype == dtype else residual.to(dtype))
+    epi = (_lib.EE_EPI_BIAS if b is not None else 0) | (_lib.EE_EPI_GELU if gelu else 0) | \
+        (_lib.EE_EPI_RESIDUAL if r is not None else 0)
+    return _aligned(scales), b, r, epi
+
+
+def quantize_tokens(x):
+    """int8 codes [..., K] and fp32 scales [..., 1] of bf16 / fp16 activations, one scale per token:
+    ``scale = max(amax |x| / 127, 1e-8)``, ``code = rint(x / scale)`` (``ee_quantize_tokens``). A token that holds an
+    infinity or NaN gets codes of 0 and a NaN scale. K is a multiple of 16."""
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"activations must be bf16 or fp16, not {x.dtype}")
+    k = x.shape[-1]
+    if k < 16 or k % 16 or k > 131056:
+        raise ValueError(f"K must be a multiple of 16, at most 131056, got {k}")
+    dev = _lib.same_device(x)
+    _lib.no_grad_through("quantize_tokens", x)
+    with _lib.on_device(dev):
+        xf = _token_rows(x, k)
+        q = torch.empty(x.shape, dtype=torch.int8, device=dev)
+        s = torch.empty(*x.shape[:-1], 1, dtype=torch.float32, device=dev)
+        _lib.check(_lib.load().ee_quantize_tokens(xf.data_ptr(), xf.stride(0), q.data_ptr(), s.data_ptr(),
+                                                  xf.shape[0], k, _lib.act_code(x.dtype), _lib.stream_ptr(dev)),
+                   "ee_quantize_tokens")
+    return q, s
+
+
+def int8_matmul(xq, x_scale, weight, scales, bias=None, dtype=torch.bfloat16, gelu=False, residual=None):
+    """``(xq @ weight.T) * x_scale * scales + bias`` of int8 codes ``xq`` [..., K] and ``weight`` [N, K], with an exact
+    32-bit integer sum, fp32 after it and one rounding to ``dtype`` (``ee_int8_gemm``). ``x_scale`` holds one fp32 value
+    per token (``quantize_tokens``), ``scales`` one fp32 or fp16 value per output channel. ``gelu`` (exact erf GELU) or
+    ``residual`` are applied in fp32 before that rounding. No backward pass."""
+    k = xq.shape[-1]
+    if xq.dtype != torch.int8:
+        raise ValueError(f"xq must be int8, not {xq.dtype}")
+    out_shape = (*xq.shape[:-1], weight.shape[0])
+    n = _check_int8_operands(weight, scales, bias, residual, k, dtype, out_shape)
+    m = xq.numel() // k
+    if x_scale.dtype != torch.float32 or x_scale.numel() != m:
+        raise ValueError(f"x_scale must hold {m} float32 values (one per token), "
+                         f"got {x_scale.dtype} {tuple(x_scale.shape)}")
+    dev = _lib.same_device(xq, x_scale, weight, scales, bias, residual)
+    _lib.no_grad_through("int8_matmul", x_scale, residual)
+    with _lib.on_device(dev):
+        s, b, r, epi = _int8_epilogue(scales, bias, gelu, residual, dtype)
+        xq, x_scale, weight = _aligned(xq), _aligned(x_scale), _aligned(weight)
+        y = torch.empty(out_shape, dtype=dtype, device=dev)
+        _lib.check(_lib.load().ee_int8_gemm(xq.data_ptr(), x_scale.data_ptr(), weight.data_ptr(), s.data_ptr(),
+                                            _lib.ptr(b), _lib.ptr(r), y.data_ptr(), m, n, k, _lib.scale_code(s.dtype),
+                                            _lib.act_code(dtype), epi, _lib.stream_ptr(dev)), "ee_int8_gemm")
+    return y
+
+
+def int8_linear(x, weight, scales, bias=None, gelu=False, residual=None):
+    """A linear on the 8-bit integer tensor cores: bf16 / fp16 ``x`` [..., K] quantised per token as in
+    ``quantize_tokens``, then ``int8_matmul`` with ``weight`` int8 [N, K] and one scale per output channel, to
+    ``x.dtype`` (``ee_int8_linear``, one call). No backward pass."""
+    k = x.shape[-1]
+    out_shape = (*x.shape[:-1], weight.shape[0])
+    n = _check_int8_operands(weight, scales, bias, residual, k, x.dtype, out_shape)
+    dev = _lib.same_device(x, weight, scales, bias, residual)
+    _lib.no_grad_through("int8_linear", x, residual)
+    with _lib.on_device(dev):
+        xf = _token_rows(x, k)
+        m = xf.shape[0]
+        s, b, r, epi = _int8_epilogue(scales, bias, gelu, residual, x.dtype)
+        weight = _aligned(weight)
+        y = torch.empty(out_shape, dtype=x.dtype, device=dev)
+        ws = torch.empty(m * k + 4 * m, dtype=torch.uint8, device=dev)
+        _lib.check(_lib.load().ee_int8_linear(xf.data_ptr(), xf.stride(0), weight.data_ptr(), s.data_ptr(),
+                                              _lib.ptr(b), _lib.ptr(r), y.data_ptr(), ws.data_ptr(), ws.numel(),
+                                              m, n, k, _lib.scale_code(s.dtype), _lib.act_code(x.dtype), epi,
+                                              _lib.stream_ptr(dev)), "ee_int8_linear")
+    return y
+
+
 def dequant_weight(weight, scales, group_size, bits, dtype, zeros=None):
     """[N, K] ``dtype`` (bf16 / fp16) copy of a packed weight, the values the
     dequant-GEMM multiplies (``ee_dequant_weight``: the exact integer times

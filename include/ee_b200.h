@@ -32,6 +32,9 @@
  *   ee_read_status        device status word of a sampler workspace (new)
  *   ee_encode_kv_maps     TMA descriptors of the cached prefix K/V (new)
  *   ee_barrier_selftest   bounded-wait self-test of the grid barrier (new)
+ *   ee_quantize_tokens / ee_int8_gemm / ee_int8_linear   8-bit integer linears (new)
+ *   ee_rotary             rotary positions with several axes (new)
+ *   ee_prompt_attention   attention over packed prompts (new)
  *   ee_strerror / ee_version / ee_struct_size   (new)
  */
 #ifndef EE_B200_H
@@ -168,6 +171,75 @@ int ee_expert_head(const void* x_act, const void* w_in, const void* b_in, const 
                    ee_stream_t stream);
 int ee_euler_step(void* x, const void* v, void* t, int64_t count, int32_t batch, float dt, int32_t act_dtype,
                   ee_stream_t stream);
+
+/* ---- layers of a packed prompt (new: no counterpart in the reference) ---- */
+/* Integer linears with a scale for each token and each output channel:
+ *   y[m][n] = epi( (sum_k xq[m][k] * weight[n][k]) * x_scales[m] * w_scales[n] )
+ * with an exact int32 sum, the rest in fp32 and one rounding to the act dtype.
+ *   x         [m][k] act dtype, row stride ldx elements (a multiple of 8)
+ *   xq        [m][k] int8, contiguous;  x_scales [m] fp32
+ *   weight    [n][k] int8, contiguous;  w_scales [n] scale_dtype (EE_F32 or EE_F16)
+ *   bias      [n], residual [m][n], y [m][n] act dtype (y may alias residual)
+ * epi: + bias, then GELU(erf) or + residual (EE_EPI_*, as for ee_wq_gemm but
+ * without roundings in between). k % 16 == 0 and k <= 131056 (the sum's 32
+ * bits); m, n >= 0, any.
+ * ee_quantize_tokens: x_scales[m] = max(amax / 127, 1e-8) of row m,
+ * xq = rint(x / x_scales[m]) (true division, ties to even). A row that holds
+ * an infinity or NaN gets codes of 0 and a NaN scale, so its outputs are NaN.
+ * ee_int8_linear is the two in one call, with the codes and scales in a
+ * caller-owned 16-byte aligned workspace. A tensor-core wait that gives up
+ * leaves EE_ERR_TIMEOUT in the status word of ee_wq_gemm_status. */
+int ee_quantize_tokens(const void* x, int64_t ldx, int8_t* xq, float* x_scales, int64_t m, int64_t k,
+                       int32_t act_dtype, ee_stream_t stream);
+int ee_int8_gemm(const int8_t* xq, const float* x_scales, const void* weight, const void* w_scales, const void* bias,
+                 const void* residual, void* y, int64_t m, int64_t n, int64_t k, int32_t scale_dtype,
+                 int32_t act_dtype, int32_t epilogue, ee_stream_t stream);
+size_t ee_int8_linear_workspace_bytes(int64_t m, int64_t k);
+int ee_int8_linear(const void* x, int64_t ldx, const void* weight, const void* w_scales, const void* bias,
+                   const void* residual, void* y, void* workspace, size_t workspace_bytes, int64_t m, int64_t n,
+                   int64_t k, int32_t scale_dtype, int32_t act_dtype, int32_t epilogue, ee_stream_t stream);
+
+/* Rotary positions with up to four axes. Pair i (of head_dim / 2) of every
+ * head of token t turns by positions[axis][t] * freq(i): the first sections[0]
+ * pairs go by axis 0, the next sections[1] by axis 1, ... (the sections sum to
+ * head_dim / 2). Pair i is elements (i, i + head_dim / 2), or (2i, 2i + 1)
+ * when interleaved. freqs[i] = round(freq(i) / (2 pi) * 2^64), a fraction of a
+ * turn: the angle is taken modulo whole turns in integers, so far (and
+ * negative) positions lose nothing. q [tokens][n_q][head_dim] and
+ * k [tokens][n_kv][head_dim] by token / head strides in elements (multiples
+ * of 8; the last dimension contiguous), each to its own output (which may be
+ * the input itself); n_q or n_kv may be 0. positions: int32 or int64
+ * (pos_bits), axes pos_axis elements apart; sections on the HOST.
+ * head_dim 32, 64, 128 or 256. */
+int ee_rotary(const void* q, int64_t q_tok, int64_t q_head, void* q_out, int64_t qo_tok, int64_t qo_head,
+              const void* k, int64_t k_tok, int64_t k_head, void* k_out, int64_t ko_tok, int64_t ko_head,
+              const void* positions, int64_t pos_axis, int32_t pos_bits, const uint64_t* freqs, int64_t tokens,
+              int32_t n_q, int32_t n_kv, int32_t head_dim, const int32_t* sections, int32_t n_axes,
+              int32_t interleaved, int32_t act_dtype, ee_stream_t stream);
+
+/* Attention over n_seq packed sequences: queries cu_q[b] .. cu_q[b + 1] of q
+ * [tq][n_q][head_dim] against keys cu_k[b] .. cu_k[b + 1] of k / v
+ * [tk][n_kv][head_dim] (the first k_lens[b] of them when k_lens is given: a
+ * cache with room to grow). cu_k NULL: the queries' own offsets (tk == tq).
+ * Head h reads key head h / (n_q / n_kv). causal: a sequence's last query sees
+ * its last key, query i keys 0 .. klen - qlen + i; a query that sees no key
+ * gives zeros. Offsets and lengths live on the device (int32) and are cut to
+ * tq / tk; rows of `out` that belong to no sequence stay as they were.
+ * Sequences may have no queries or no keys. Strides in elements, multiples of
+ * 8; the last dimension contiguous. head_dim 64 or 128; scale > 0 (finite).
+ * Keys a sequence does not have are never read into a result, whatever they
+ * hold; inside a sequence, values under the causal mask have to be finite (a
+ * masked weight is a product with 0). fp32 statistics and sums, weights
+ * rounded to the act dtype for the product with v, one rounding of the result.
+ * workspace: ee_prompt_attention_workspace_bytes() bytes, 16-byte aligned (may
+ * be NULL when that is 0); calls that may overlap need one each. */
+size_t ee_prompt_attention_workspace_bytes(int64_t tq, int64_t tk, int32_t n_seq, int32_t n_q, int32_t n_kv,
+                                           int32_t head_dim);
+int ee_prompt_attention(const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok, int64_t k_head,
+                        const void* v, int64_t v_tok, int64_t v_head, void* out, int64_t o_tok, int64_t o_head,
+                        const int32_t* cu_q, const int32_t* cu_k, const int32_t* k_lens, int64_t tq, int64_t tk,
+                        int32_t n_seq, int32_t n_q, int32_t n_kv, int32_t head_dim, int32_t causal, float scale,
+                        int32_t act_dtype, void* workspace, size_t workspace_bytes, ee_stream_t stream);
 
 /* ---- fused flow-matching sampler --------------------------------------- */
 typedef struct ee_linear {
