@@ -4,8 +4,8 @@
 // and the token quantiser xq = rint(x / sx), sx = max(amax |x| / 127, 1e-8).
 #include <atomic>
 
-#include "ee_common.cuh"
 #include "ee_host.h"
+#include "ee_int8_tc.cuh"
 
 namespace ee {
 
@@ -118,70 +118,94 @@ static int launch_quantize(const T* x, int8_t* xq, float* sx, long long rows, in
 // ---------------------------------------------------------------------------
 // product
 // ---------------------------------------------------------------------------
-struct Int8Args {
-  const int8_t* xq;      // [M][K]
-  const float* sx;       // [M]
-  const int8_t* w;       // [N][K]
-  const void* sw;        // [N] fp32 or fp16
-  const void *bias, *resid;
-  void* out;
-  int M, N, K;
-  int sw_f16, epi;
-};
-enum { I8_BIAS = 1, I8_GELU = 2, I8_RESID = 4 };
+constexpr unsigned long long kI8TimeoutNs = 1000000000ull;
 
-EE_DEV float i8_wscale(const Int8Args& a, int n) {
-  return a.sw_f16 ? __half2float(__ldg(reinterpret_cast<const __half*>(a.sw) + n))
-                  : __ldg(reinterpret_cast<const float*>(a.sw) + n);
-}
-// the epilogue of one output in fp32 (one rounding, by the caller)
-template <typename T> EE_DEV float i8_epi(const Int8Args& a, int acc, float sx, float sw, int m, int n) {
-  float y = (float)acc * sx * sw;
-  if (a.epi & I8_BIAS) y += ld_param(reinterpret_cast<const T*>(a.bias) + n);
-  if (a.epi & I8_GELU) y = gelu_erf(y);
-  if (a.epi & I8_RESID) y += ld_param(reinterpret_cast<const T*>(a.resid) + (size_t)m * a.N + n);
-  return y;
+int* gemm_status_ptr();  // ee_ops.cu: the status word of the GEMM kernels on the current device
+
+template <typename T, bool GELU>
+static int launch_pair(Int8Args a, const int8_t* xq, const int8_t* w, cudaStream_t s) {
+  auto fn = int8_pair_kernel<T, GELU>;
+  static std::atomic<int> set[64];
+  allow_max_smem(fn, set);
+  const DevProps* dp = device_props();
+  if (!dp) return EE_ERR_DEVICE;
+  CUtensorMap tx, tw, ty{};
+  if (!make_tmap_2d(&tx, xq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.K, a.M, a.K, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !make_tmap_2d(&tw, w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.K, a.N, a.K, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      (a.vec && !make_tmap_2d(&ty, a.out, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, a.N, a.M, (uint64_t)a.N * 2, 64, 32,
+                              CU_TENSOR_MAP_SWIZZLE_128B)))
+    return EE_ERR_LAUNCH;
+  a.tiles_m = (a.M + 255) / 256;
+  a.tiles_n = (a.N + 255) / 256;
+  const long long tiles = (long long)a.tiles_m * a.tiles_n;
+  if (tiles > 0x7fffffff) return EE_ERR_SHAPE;
+  const int pairs = (int)(tiles < dp->sms / 2 ? tiles : dp->sms / 2);
+  return launch_pdl(fn, dim3(2 * pairs), dim3(kI8PairThreads), kI8PairSmem, s, tx, tw, ty, a) == cudaSuccess
+             ? EE_OK
+             : EE_ERR_LAUNCH;
 }
 
-// 64 x 64 outputs per CTA, 4 x 4 per thread, 64-byte K steps through shared memory, dp4a
-template <typename T>
-__global__ void __launch_bounds__(256) int8_gemm_kernel(const __grid_constant__ Int8Args a) {
-  pdl_entry();
-  __shared__ int xs[64][17], ws[64][17];
-  const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  int acc[4][4] = {};
-  for (int k0 = 0; k0 < a.K; k0 += 64) {
-    for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-      const int r = i >> 4, c = i & 15, k = k0 + 4 * c;
-      xs[r][c] = (m0 + r < a.M && k < a.K) ? *reinterpret_cast<const int*>(a.xq + (size_t)(m0 + r) * a.K + k) : 0;
-      ws[r][c] = (n0 + r < a.N && k < a.K) ? *reinterpret_cast<const int*>(a.w + (size_t)(n0 + r) * a.K + k) : 0;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int c = 0; c < 16; ++c) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(xs[ty + 16 * i][c], ws[tx + 16 * j][c], acc[i][j]);
-    }
-    __syncthreads();
+template <typename T, int NT, bool GELU>
+static int launch_few(Int8Args a, const int8_t* xq, const int8_t* w, int split, cudaStream_t s) {
+  auto fn = int8_few_kernel<T, NT, GELU>;
+  static std::atomic<int> set[64];
+  allow_max_smem(fn, set);
+  CUtensorMap tx, tw;
+  if (!make_tmap_2d(&tx, xq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.K, a.M, a.K, 128, NT, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !make_tmap_2d(&tw, w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.K, a.N, a.K, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B))
+    return EE_ERR_LAUNCH;
+  const int nkb = (a.K + 127) / 128, kbc = (nkb + split - 1) / split;
+  const int fit = (int)((200 * 1024) / i8_few_stage<NT>());
+  a.split = split;
+  a.ns = kbc < fit ? kbc : fit;
+  uint32_t ring = a.ns * i8_few_stage<NT>();
+  if (ring < i8_few_part<NT>()) ring = i8_few_part<NT>();
+  const size_t smem = 1024 + ring + 16 * a.ns + 16;
+  const long long units = (long long)((a.N + 127) / 128) * ((a.M + NT - 1) / NT);
+  if (units * split > 0x7fffffff) return EE_ERR_SHAPE;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(units * split));
+  cfg.blockDim = dim3(kI8FewThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = split;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  unsigned int n = 1;
+  add_pdl_attr(attr, n);
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  return cudaLaunchKernelEx(&cfg, fn, tx, tw, a) == cudaSuccess ? EE_OK : EE_ERR_LAUNCH;
+}
+
+// Which kernel: the token tile NT (0: the pair kernel) and the K split.
+struct Int8Plan { int nt, split; };
+static Int8Plan int8_plan(int m, int n, int k, int sms) {
+  const int nkb = (k + 127) / 128;
+  const int nt = m <= 16 ? 16 : (m <= 32 ? 32 : (m <= 64 ? 64 : 128));
+  const long long units = (long long)((n + 127) / 128) * ((m + nt - 1) / nt);
+  if (m > 128 && units > 2 * sms) return {0, 1};
+  int split = 1;
+  while (split < 8 && units * split * 2 <= sms && split * 2 <= nkb) split *= 2;
+  return {nt, split};
+}
+
+template <typename T, bool GELU>
+static int launch_int8_g(const Int8Args& a, const int8_t* xq, const int8_t* w, cudaStream_t s) {
+  const Int8Plan p = int8_plan(a.M, a.N, a.K, device_sms());
+  switch (p.nt) {
+    case 16: return launch_few<T, 16, GELU>(a, xq, w, p.split, s);
+    case 32: return launch_few<T, 32, GELU>(a, xq, w, p.split, s);
+    case 64: return launch_few<T, 64, GELU>(a, xq, w, p.split, s);
+    case 128: return launch_few<T, 128, GELU>(a, xq, w, p.split, s);
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-      if (m < a.M && n < a.N)
-        reinterpret_cast<T*>(a.out)[(size_t)m * a.N + n] = Act<T>::from_f(i8_epi<T>(a, acc[i][j], a.sx[m], i8_wscale(a, n), m, n));
-    }
+  return launch_pair<T, GELU>(a, xq, w, s);
 }
-
 template <typename T>
-static int launch_int8(const Int8Args& a, cudaStream_t s) {
-  const dim3 grid((a.N + 63) / 64, (a.M + 63) / 64);
-  if (grid.y > 65535) return EE_ERR_SHAPE;
-  return launch_pdl(int8_gemm_kernel<T>, grid, dim3(256), 0, s, a) == cudaSuccess ? EE_OK : EE_ERR_LAUNCH;
+static int launch_int8(const Int8Args& a, const int8_t* xq, const int8_t* w, cudaStream_t s) {
+  return (a.epi & I8_GELU) ? launch_int8_g<T, true>(a, xq, w, s) : launch_int8_g<T, false>(a, xq, w, s);
 }
 
 static int check_product(const void* weight, const void* w_scales, const void* bias, const void* residual, void* y,
@@ -205,14 +229,18 @@ static int int8_product(const int8_t* xq, const float* sx, const void* weight, c
                         const void* residual, void* y, int64_t m, int64_t n, int64_t k, int32_t scale_dtype,
                         int32_t act_dtype, int32_t epilogue, cudaStream_t s) {
   Int8Args a{};
-  a.xq = xq; a.sx = sx;
-  a.w = reinterpret_cast<const int8_t*>(weight);
+  a.sx = sx;
   a.sw = w_scales;
   a.bias = bias; a.resid = residual; a.out = y;
   a.M = (int)m; a.N = (int)n; a.K = (int)k;
   a.sw_f16 = scale_dtype == EE_F16;
   a.epi = epilogue;
-  return act_dtype == EE_BF16 ? launch_int8<__nv_bfloat16>(a, s) : launch_int8<__half>(a, s);
+  a.vec = n % 8 == 0;
+  a.status = gemm_status_ptr();
+  a.timeout_ns = kI8TimeoutNs;
+  if (!a.status) return EE_ERR_DEVICE;
+  const int8_t* w = reinterpret_cast<const int8_t*>(weight);
+  return act_dtype == EE_BF16 ? launch_int8<__nv_bfloat16>(a, xq, w, s) : launch_int8<__half>(a, xq, w, s);
 }
 
 }  // namespace ee

@@ -114,7 +114,7 @@ constexpr int kStreamMaxM = EE_STREAM_MAX_M;
 // Status word of the GEMM kernels (first error since the last reset).
 static __device__ int g_gemm_status;
 
-static int* gemm_status_ptr() {
+int* gemm_status_ptr() {
   static std::mutex mu;
   static int* addr[64] = {};
   int dev = 0;
