@@ -4,6 +4,7 @@
 
 #include "ee_host.h"
 #include "ee_prompt.cuh"
+#include "ee_prompt_tc.cuh"
 
 namespace ee {
 
@@ -234,9 +235,53 @@ static int launch_rows(const PromptArgs& a, cudaStream_t s) {
              : EE_ERR_LAUNCH;
 }
 
+int* gemm_status_ptr();  // ee_ops.cu: the status word of the tensor-core kernels on the current device
+
+// [tokens][heads][hd] by strides, read in boxes of 64 columns of one head and 128 tokens
+static bool make_head_map(CUtensorMap* map, const void* base, int hd, int heads, long long tokens, long long head,
+                          long long tok) {
+  auto enc = tmap_encoder();
+  if (!enc) return false;
+  if (heads == 1) head = hd;   // strides of dimensions of one entry mean nothing
+  if (tokens == 1) tok = (long long)hd * heads;
+  const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)heads, (cuuint64_t)tokens};
+  const cuuint64_t strides[2] = {(cuuint64_t)head * 2, (cuuint64_t)tok * 2};
+  const cuuint32_t box[3] = {64, 1, 128}, estr[3] = {1, 1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int HD>
+static int launch_tc(const PromptArgs& p, cudaStream_t s) {
+  auto fn = prompt_tc_kernel<T, HD>;
+  static std::atomic<int> set[64];
+  allow_max_smem(fn, set);
+  CUtensorMap mq, mk, mv;
+  if (!make_head_map(&mq, p.q, HD, p.n_q, p.tq, p.q_head, p.q_tok) ||
+      !make_head_map(&mk, p.k, HD, p.n_kv, p.tk, p.k_head, p.k_tok) ||
+      !make_head_map(&mv, p.v, HD, p.n_kv, p.tk, p.v_head, p.v_tok))
+    return EE_ERR_SHAPE;  // a stride the loads cannot address
+  PromptTcArgs a{};
+  a.p = p;
+  a.pair_heads = p.group % 2 == 0;
+  a.head_items = a.pair_heads ? p.n_q / 2 : p.n_q;
+  a.status = gemm_status_ptr();
+  a.timeout_ns = 1000000000ull;
+  if (!a.status) return EE_ERR_DEVICE;
+  const long long units = (long long)p.tq / (a.pair_heads ? 128 : 256) + p.n_seq;
+  if (units * a.head_items > 0x7fffffff) return EE_ERR_SHAPE;
+  return launch_pdl(fn, dim3((unsigned)(units * a.head_items)), dim3(kPtThreads), pt_smem<HD>(), s, mq, mk, mv, a) ==
+                 cudaSuccess
+             ? EE_OK
+             : EE_ERR_LAUNCH;
+}
+
 template <typename T>
 static int launch_prompt(const PromptArgs& a, int hd, cudaStream_t s) {
-  const bool few = (long long)a.tq * a.group <= 16LL * a.n_seq;
+  const long long rows = (long long)a.tq * a.group;  // per key head, of all sequences
+  if (rows > 64LL * a.n_seq && a.tk > 0) return hd == 64 ? launch_tc<T, 64>(a, s) : launch_tc<T, 128>(a, s);
+  const bool few = rows <= 16LL * a.n_seq;
   if (hd == 64) return few ? launch_rows<T, 64, 1>(a, s) : launch_rows<T, 64, 4>(a, s);
   return few ? launch_rows<T, 128, 1>(a, s) : launch_rows<T, 128, 4>(a, s);
 }
