@@ -13,12 +13,16 @@ namespace ee {
 // ---------------------------------------------------------------------------
 // A row is (token, head of the key head's group), so a key head's whole group
 // shares one read of its keys. A CTA takes 16 RT rows of one sequence and key
-// head; its 8 warps are RT row tiles x 8 / RT key groups, each with its own
-// running maximum and sum over its share of every 128-key stage, merged
-// through shared memory at the end.
-constexpr int kPrKeys = 128;   // keys per stage
-constexpr int kPrStages = 3;
-template <int HD> constexpr int pr_smem() { return kPrStages * 2 * kPrKeys * HD * 2; }
+// head and, where the units alone would not fill the GPU, one of `splits`
+// parts of their keys (prompt_combine_kernel joins the parts); its warps are
+// RT row tiles x KG key groups, each with its own running maximum and sum over
+// its share of every 64-key stage, merged through shared memory at the end.
+// HBM-bound on the keys and values; the ring holds three or four stages, and
+// two or three CTAs share an SM.
+constexpr int kPrKeys = 64;   // keys per stage
+template <int RT> constexpr int pr_warps() { return RT == 1 ? 4 : 8; }
+template <int HD> constexpr int pr_stages() { return HD == 128 ? 3 : 4; }
+template <int HD> constexpr int pr_smem() { return pr_stages<HD>() * 2 * kPrKeys * HD * 2; }
 
 EE_DEV void pr_ldsm(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -30,20 +34,21 @@ EE_DEV void pr_ldsm_t(uint32_t addr, uint32_t (&r)[4]) {
 }
 
 template <typename T, int HD, int RT>
-__global__ void __launch_bounds__(kThreads) prompt_rows_kernel(const __grid_constant__ PromptArgs a) {
-  constexpr int KG = kWarps / RT;        // key groups
+__global__ void __launch_bounds__(32 * pr_warps<RT>()) prompt_rows_kernel(const __grid_constant__ PromptArgs a) {
+  constexpr int NW = pr_warps<RT>(), NT = 32 * NW, NS = pr_stages<HD>();
+  constexpr int KG = NW / RT;            // key groups
   constexpr int WK = kPrKeys / KG;       // keys of a stage per warp
   constexpr int RB = HD * 2;             // bytes per key row
   constexpr int CH = HD / 8;             // 16-byte chunks per key row
   constexpr int TILE = kPrKeys * RB;
   extern __shared__ __align__(128) char smem[];
-  __shared__ int sh[kWarps + 2];
+  __shared__ int sh[NW + 2];
   pdl_entry();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rt = warp % RT, kg = warp / RT, g = lane >> 2, t = lane & 3;
   const int kvh = blockIdx.y, part = blockIdx.x % a.splits;
   PromptSeq s;
-  if (!prompt_find(a, blockIdx.x / a.splits, a.group, 16 * RT, kThreads, sh, s)) return;
+  if (!prompt_find(a, blockIdx.x / a.splits, a.group, 16 * RT, NT, sh, s)) return;
   const int rows = s.qlen * a.group, r0 = s.blk * 16 * RT;
   // keys this CTA's rows see at most, and its part of them in whole stages
   const int last_tok = (min(r0 + 16 * RT, rows) - 1) / a.group;
@@ -58,7 +63,7 @@ __global__ void __launch_bounds__(kThreads) prompt_rows_kernel(const __grid_cons
     const char* vb = reinterpret_cast<const char*>(a.v) + ((long long)(s.k0 + k0) * a.v_tok + kvh * a.v_head) * 2;
     const uint32_t d = sb + buf * 2 * TILE;
 #pragma unroll 4
-    for (int i = tid; i < kPrKeys * CH; i += kThreads) {
+    for (int i = tid; i < kPrKeys * CH; i += NT) {
       const int row = i / CH, ch = i % CH;
       const bool ok = row < valid;
       cp_async16(d + off(row, ch), kb + (ok ? (long long)row * a.k_tok * 2 + ch * 16 : 0), ok);
@@ -66,7 +71,7 @@ __global__ void __launch_bounds__(kThreads) prompt_rows_kernel(const __grid_cons
     }
   };
 #pragma unroll
-  for (int i = 0; i < kPrStages - 1; ++i) {
+  for (int i = 0; i < NS - 1; ++i) {
     if (st0 + i < st1) load(st0 + i, i);
     cp_async_commit();
   }
@@ -98,11 +103,11 @@ __global__ void __launch_bounds__(kThreads) prompt_rows_kernel(const __grid_cons
   float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
   const int mi = lane >> 3;
   for (int st = st0; st < st1; ++st) {
-    if (st + kPrStages - 1 < st1) load(st + kPrStages - 1, (st - st0 + kPrStages - 1) % kPrStages);
+    if (st + NS - 1 < st1) load(st + NS - 1, (st - st0 + NS - 1) % NS);
     cp_async_commit();
-    cp_async_wait<kPrStages - 1>();
+    cp_async_wait<NS - 1>();
     __syncthreads();
-    const uint32_t kt = sb + ((st - st0) % kPrStages) * 2 * TILE, vt = kt + TILE;
+    const uint32_t kt = sb + ((st - st0) % NS) * 2 * TILE, vt = kt + TILE;
 #pragma unroll
     for (int k1 = 0; k1 < WK; k1 += 16) {
       const int kl = kg * WK + k1;             // first of 16 keys, in the stage
@@ -178,7 +183,7 @@ __global__ void __launch_bounds__(kThreads) prompt_rows_kernel(const __grid_cons
   }
   // merge the key groups: [warp][16 rows][HD + 4] fp32 over the stages
   constexpr int ML = HD + 4;
-  static_assert(kWarps * 16 * ML * 4 <= kPrStages * 2 * kPrKeys * RB, "the merge fits the stages");
+  static_assert(NW * 16 * ML * 4 <= NS * 2 * kPrKeys * RB, "the merge fits the stages");
   float* mg = reinterpret_cast<float*>(smem) + warp * 16 * ML;
   __syncthreads();
 #pragma unroll
@@ -193,8 +198,7 @@ __global__ void __launch_bounds__(kThreads) prompt_rows_kernel(const __grid_cons
     mg[(g + 8) * ML + HD + 1] = l1;
   }
   __syncthreads();
-  // 8 threads per row: each sums 1/8 of the row's values over the key groups
-  for (int i = tid; i < 16 * RT * (HD / 4); i += kThreads) {
+  for (int i = tid; i < 16 * RT * (HD / 4); i += NT) {  // 4 values of a row over the key groups
     const int r = i / (HD / 4), c = (i % (HD / 4)) * 4;
     if (r0 + r >= rows) continue;
     const float* base = reinterpret_cast<const float*>(smem) + ((r >> 4) * 16 + (r & 15)) * ML;
@@ -216,10 +220,120 @@ __global__ void __launch_bounds__(kThreads) prompt_rows_kernel(const __grid_cons
       acc.w += f * v.w;
     }
     const int tok = s.q0 + (r0 + r) / a.group, h = kvh * a.group + (r0 + r) % a.group;
+    if (a.splits > 1) {  // this part's sums, relative to its maximum
+      const long long at = ((long long)part * a.tq + tok) * a.n_q + h;
+      if (c == 0) *reinterpret_cast<float2*>(a.stat + 2 * at) = make_float2(m, l);
+      if (l != 0.f) *reinterpret_cast<float4*>(a.part + at * HD + c) = acc;
+      continue;
+    }
     const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees no key is zero
     *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + (long long)tok * a.o_tok + h * a.o_head + c) =
         make_uint2(Act<T>::pack2(acc.x * inv, acc.y * inv), Act<T>::pack2(acc.z * inv, acc.w * inv));
   }
+}
+
+// Joins the parts of every (token, head), one CTA each: first a thread per
+// part for the common maximum and the parts' weights, then hd / 4 threads
+// across the values and the rest across the parts, so that both passes have
+// their loads in flight together.
+constexpr int kPrCombine = 256, kPrMaxSplits = 512;
+template <typename T, int HD>
+__global__ void __launch_bounds__(kPrCombine) prompt_combine_kernel(const __grid_constant__ PromptArgs a) {
+  constexpr int LANES = HD / 4, GROUPS = kPrCombine / LANES;
+  __shared__ float wt[kPrMaxSplits];
+  __shared__ float4 sv[GROUPS][LANES];
+  __shared__ float red[2][kPrCombine / 32];
+  pdl_entry();
+  const int tok = blockIdx.x, h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // rows outside the sequences have no parts and stay as they were
+  if (tok < __ldg(a.cu_q) || tok >= __ldg(a.cu_q + a.n_seq)) return;
+  const long long step = (long long)a.tq * a.n_q, at = (long long)tok * a.n_q + h;
+  float2 st[kPrMaxSplits / kPrCombine];
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kPrMaxSplits / kPrCombine; ++i) {
+    const int sp = threadIdx.x + i * kPrCombine;
+    st[i] = sp < a.splits ? __ldg(reinterpret_cast<const float2*>(a.stat) + at + sp * step) : make_float2(-INFINITY, 0.f);
+    m = fmaxf(m, st[i].x);
+  }
+  m = warp_max(m);
+  if (lane == 0) red[0][warp] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kPrCombine / 32; ++i) m = fmaxf(m, red[0][i]);
+  const float u = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPrMaxSplits / kPrCombine; ++i) {
+    const float f = st[i].y == 0.f ? 0.f : exp2f(st[i].x - u);  // weight 0: no key seen, its sums were not written
+    wt[threadIdx.x + i * kPrCombine] = f;
+    l += f * st[i].y;
+  }
+  l = warp_sum(l);
+  if (lane == 0) red[1][warp] = l;
+  __syncthreads();
+  const int c = threadIdx.x % LANES, grp = threadIdx.x / LANES;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = grp; i < a.splits; i += GROUPS) {
+    const float f = wt[i];
+    if (f != 0.f) {
+      const float4 v = __ldg(reinterpret_cast<const float4*>(a.part + (at + i * step) * HD) + c);
+      acc.x += f * v.x;
+      acc.y += f * v.y;
+      acc.z += f * v.z;
+      acc.w += f * v.w;
+    }
+  }
+  sv[grp][c] = acc;
+  __syncthreads();
+  if (grp) return;
+  l = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPrCombine / 32; ++i) l += red[1][i];
+#pragma unroll
+  for (int g = 1; g < GROUPS; ++g) {
+    const float4 v = sv[g][c];
+    acc.x += v.x;
+    acc.y += v.y;
+    acc.z += v.z;
+    acc.w += v.w;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + (long long)tok * a.o_tok + h * a.o_head + 4 * c) =
+      make_uint2(Act<T>::pack2(acc.x * inv, acc.y * inv), Act<T>::pack2(acc.z * inv, acc.w * inv));
+}
+
+// How a call runs, by what the host knows of it: rows (queries x group) per
+// sequence and key head, and keys per sequence, on average.
+//   tc      more than 64 rows: the tensor-core kernel's 128-row tiles
+//   rt      16-row tiles per CTA of the rows kernel
+//   splits  parts of the keys: enough CTAs for four an SM, of 128 keys or more
+#ifndef EE_PROMPT_TC_ROWS
+#define EE_PROMPT_TC_ROWS 64
+#endif
+#ifndef EE_PROMPT_WANT
+#define EE_PROMPT_WANT 4LL
+#endif
+#ifndef EE_PROMPT_MINK
+#define EE_PROMPT_MINK 128
+#endif
+struct PromptPlan { bool tc; int rt, splits; };
+static PromptPlan prompt_plan(long long tq, long long tk, int n_seq, int n_q, int n_kv) {
+  PromptPlan pl{};
+  const long long rows = tq * (n_q / n_kv);
+  pl.tc = rows > (long long)EE_PROMPT_TC_ROWS * n_seq && tk > 0;
+  pl.rt = rows <= 16LL * n_seq ? 1 : 4;
+  pl.splits = 1;
+  if (pl.tc || n_seq < 1) return pl;
+  const long long units = (rows / (16 * pl.rt) > n_seq ? rows / (16 * pl.rt) : n_seq) * n_kv;
+  const long long want = (EE_PROMPT_WANT * device_sms() + units - 1) / units, most = (tk / n_seq + EE_PROMPT_MINK - 1) / EE_PROMPT_MINK;
+  const long long s = want < most ? want : most;
+  pl.splits = s < 1 ? 1 : (int)(s < kPrMaxSplits ? s : kPrMaxSplits);
+  return pl;
+}
+static size_t prompt_ws_bytes(const PromptPlan& pl, long long tq, int n_q, int hd) {
+  return pl.splits > 1 ? (size_t)pl.splits * tq * n_q * (hd + 2) * 4 : 0;
 }
 
 template <typename T, int HD, int RT>
@@ -230,7 +344,11 @@ static int launch_rows(const PromptArgs& a, cudaStream_t s) {
   // at most one partial block per sequence beyond the rows' whole blocks
   const long long units = (long long)a.tq * a.group / (16 * RT) + a.n_seq;
   if (units * a.splits > 0x7fffffff) return EE_ERR_SHAPE;
-  return launch_pdl(fn, dim3((unsigned)(units * a.splits), a.n_kv), dim3(kThreads), pr_smem<HD>(), s, a) == cudaSuccess
+  if (launch_pdl(fn, dim3((unsigned)(units * a.splits), a.n_kv), dim3(32 * pr_warps<RT>()), pr_smem<HD>(), s, a) !=
+      cudaSuccess)
+    return EE_ERR_LAUNCH;
+  if (a.splits == 1) return EE_OK;
+  return launch_pdl(prompt_combine_kernel<T, HD>, dim3((unsigned)a.tq, a.n_q), dim3(kPrCombine), 0, s, a) == cudaSuccess
              ? EE_OK
              : EE_ERR_LAUNCH;
 }
@@ -278,12 +396,10 @@ static int launch_tc(const PromptArgs& p, cudaStream_t s) {
 }
 
 template <typename T>
-static int launch_prompt(const PromptArgs& a, int hd, cudaStream_t s) {
-  const long long rows = (long long)a.tq * a.group;  // per key head, of all sequences
-  if (rows > 64LL * a.n_seq && a.tk > 0) return hd == 64 ? launch_tc<T, 64>(a, s) : launch_tc<T, 128>(a, s);
-  const bool few = rows <= 16LL * a.n_seq;
-  if (hd == 64) return few ? launch_rows<T, 64, 1>(a, s) : launch_rows<T, 64, 4>(a, s);
-  return few ? launch_rows<T, 128, 1>(a, s) : launch_rows<T, 128, 4>(a, s);
+static int launch_prompt(const PromptArgs& a, const PromptPlan& pl, int hd, cudaStream_t s) {
+  if (pl.tc) return hd == 64 ? launch_tc<T, 64>(a, s) : launch_tc<T, 128>(a, s);
+  if (hd == 64) return pl.rt == 1 ? launch_rows<T, 64, 1>(a, s) : launch_rows<T, 64, 4>(a, s);
+  return pl.rt == 1 ? launch_rows<T, 128, 1>(a, s) : launch_rows<T, 128, 4>(a, s);
 }
 
 }  // namespace ee
@@ -294,8 +410,8 @@ extern "C" {
 
 size_t ee_prompt_attention_workspace_bytes(int64_t tq, int64_t tk, int32_t n_seq, int32_t n_q, int32_t n_kv,
                                            int32_t head_dim) {
-  (void)tq; (void)tk; (void)n_seq; (void)n_q; (void)n_kv; (void)head_dim;
-  return 0;
+  if (tq < 0 || tk < 0 || n_seq < 0 || n_q < 1 || n_kv < 1 || n_q % n_kv || tq > 0x7fffff00 || tk > 0x7fffff00) return 0;
+  return prompt_ws_bytes(prompt_plan(tq, tk, n_seq, n_q, n_kv), tq, n_q, head_dim);
 }
 
 int ee_prompt_attention(const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok, int64_t k_head,
@@ -315,7 +431,10 @@ int ee_prompt_attention(const void* q, int64_t q_tok, int64_t q_head, const void
   if ((q_tok | q_head | k_tok | k_head | v_tok | v_head | o_tok | o_head) % 8 != 0) return EE_ERR_ALIGN;
   const int rc = check_device();
   if (rc) return rc;
-  (void)workspace; (void)workspace_bytes;
+  const PromptPlan pl = prompt_plan(tq, tk, n_seq, n_q, n_kv);
+  const size_t need = prompt_ws_bytes(pl, tq, n_q, head_dim);
+  if (need && (!workspace || workspace_bytes < need)) return EE_ERR_WORKSPACE;
+  if (need && !aligned16(workspace)) return EE_ERR_ALIGN;
   PromptArgs a{};
   a.q = q; a.k = k; a.v = v; a.out = out;
   a.cu_q = cu_q;
@@ -327,9 +446,12 @@ int ee_prompt_attention(const void* q, int64_t q_tok, int64_t q_head, const void
   a.n_q = n_q; a.n_kv = n_kv; a.group = n_q / n_kv;
   a.causal = causal != 0;
   a.scale_log2 = scale * 1.4426950408889634f;
-  a.splits = 1;
+  a.splits = pl.splits;
+  a.part = reinterpret_cast<float*>(workspace);
+  a.stat = a.part + (size_t)pl.splits * tq * n_q * head_dim;
   cudaStream_t s = (cudaStream_t)stream;
-  return act_dtype == EE_BF16 ? launch_prompt<__nv_bfloat16>(a, head_dim, s) : launch_prompt<__half>(a, head_dim, s);
+  return act_dtype == EE_BF16 ? launch_prompt<__nv_bfloat16>(a, pl, head_dim, s)
+                               : launch_prompt<__half>(a, pl, head_dim, s);
 }
 
 }  // extern "C"
