@@ -310,7 +310,10 @@ __global__ void __launch_bounds__(kPrCombine) prompt_combine_kernel(const __grid
 //   rt      16-row tiles per CTA of the rows kernel
 //   splits  parts of the keys: enough CTAs for four an SM, of 128 keys or more
 #ifndef EE_PROMPT_TC_ROWS
-#define EE_PROMPT_TC_ROWS 64
+#define EE_PROMPT_TC_ROWS 16
+#endif
+#ifndef EE_PROMPT_TC_MINK
+#define EE_PROMPT_TC_MINK 512
 #endif
 #ifndef EE_PROMPT_WANT
 #define EE_PROMPT_WANT 4LL
@@ -322,10 +325,18 @@ struct PromptPlan { bool tc; int rt, splits; };
 static PromptPlan prompt_plan(long long tq, long long tk, int n_seq, int n_q, int n_kv) {
   PromptPlan pl{};
   const long long rows = tq * (n_q / n_kv);
-  pl.tc = rows > (long long)EE_PROMPT_TC_ROWS * n_seq && tk > 0;
+  pl.tc = rows > (long long)EE_PROMPT_TC_ROWS * n_seq && tk > 0 && n_q / n_kv <= 128;
   pl.rt = rows <= 16LL * n_seq ? 1 : 4;
   pl.splits = 1;
-  if (pl.tc || n_seq < 1) return pl;
+  if (n_seq < 1) return pl;
+  if (pl.tc) {
+    const long long per = 256 / (n_q / n_kv) * (n_q / n_kv);
+    const long long items = (rows / per > n_seq ? rows / per : n_seq) * n_kv;
+    const long long want = device_sms() / items, most = tk / n_seq / EE_PROMPT_TC_MINK;
+    const long long s = want < most ? want : most;
+    pl.splits = s < 1 ? 1 : (int)s;
+    return pl;
+  }
   const long long units = (rows / (16 * pl.rt) > n_seq ? rows / (16 * pl.rt) : n_seq) * n_kv;
   const long long want = (EE_PROMPT_WANT * device_sms() + units - 1) / units, most = (tk / n_seq + EE_PROMPT_MINK - 1) / EE_PROMPT_MINK;
   const long long s = want < most ? want : most;
@@ -334,6 +345,14 @@ static PromptPlan prompt_plan(long long tq, long long tk, int n_seq, int n_q, in
 }
 static size_t prompt_ws_bytes(const PromptPlan& pl, long long tq, int n_q, int hd) {
   return pl.splits > 1 ? (size_t)pl.splits * tq * n_q * (hd + 2) * 4 : 0;
+}
+
+template <typename T, int HD>
+static int launch_combine(const PromptArgs& a, cudaStream_t s) {
+  if (a.splits == 1) return EE_OK;
+  return launch_pdl(prompt_combine_kernel<T, HD>, dim3((unsigned)a.tq, a.n_q), dim3(kPrCombine), 0, s, a) == cudaSuccess
+             ? EE_OK
+             : EE_ERR_LAUNCH;
 }
 
 template <typename T, int HD, int RT>
@@ -347,24 +366,21 @@ static int launch_rows(const PromptArgs& a, cudaStream_t s) {
   if (launch_pdl(fn, dim3((unsigned)(units * a.splits), a.n_kv), dim3(32 * pr_warps<RT>()), pr_smem<HD>(), s, a) !=
       cudaSuccess)
     return EE_ERR_LAUNCH;
-  if (a.splits == 1) return EE_OK;
-  return launch_pdl(prompt_combine_kernel<T, HD>, dim3((unsigned)a.tq, a.n_q), dim3(kPrCombine), 0, s, a) == cudaSuccess
-             ? EE_OK
-             : EE_ERR_LAUNCH;
+  return launch_combine<T, HD>(a, s);
 }
 
 int* gemm_status_ptr();  // ee_ops.cu: the status word of the tensor-core kernels on the current device
 
-// [tokens][heads][hd] by strides, read in boxes of 64 columns of one head and 128 tokens
+// [tokens][heads][hd] by strides, read in boxes of 64 columns of bh heads and bt tokens
 static bool make_head_map(CUtensorMap* map, const void* base, int hd, int heads, long long tokens, long long head,
-                          long long tok) {
+                          long long tok, int bh, int bt) {
   auto enc = tmap_encoder();
   if (!enc) return false;
   if (heads == 1) head = hd;   // strides of dimensions of one entry mean nothing
   if (tokens == 1) tok = (long long)hd * heads;
   const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)heads, (cuuint64_t)tokens};
   const cuuint64_t strides[2] = {(cuuint64_t)head * 2, (cuuint64_t)tok * 2};
-  const cuuint32_t box[3] = {64, 1, 128}, estr[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {64, (cuuint32_t)bh, (cuuint32_t)bt}, estr[3] = {1, 1, 1};
   return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), dims, strides, box, estr,
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -375,24 +391,25 @@ static int launch_tc(const PromptArgs& p, cudaStream_t s) {
   auto fn = prompt_tc_kernel<T, HD>;
   static std::atomic<int> set[64];
   allow_max_smem(fn, set);
-  CUtensorMap mq, mk, mv;
-  if (!make_head_map(&mq, p.q, HD, p.n_q, p.tq, p.q_head, p.q_tok) ||
-      !make_head_map(&mk, p.k, HD, p.n_kv, p.tk, p.k_head, p.k_tok) ||
-      !make_head_map(&mv, p.v, HD, p.n_kv, p.tk, p.v_head, p.v_tok))
-    return EE_ERR_SHAPE;  // a stride the loads cannot address
+  const DevProps* dp = device_props();
+  if (!dp) return EE_ERR_DEVICE;
   PromptTcArgs a{};
   a.p = p;
-  a.pair_heads = p.group % 2 == 0;
-  a.head_items = a.pair_heads ? p.n_q / 2 : p.n_q;
+  a.tpt = 128 / p.group;
   a.status = gemm_status_ptr();
   a.timeout_ns = 1000000000ull;
   if (!a.status) return EE_ERR_DEVICE;
-  const long long units = (long long)p.tq / (a.pair_heads ? 128 : 256) + p.n_seq;
-  if (units * a.head_items > 0x7fffffff) return EE_ERR_SHAPE;
-  return launch_pdl(fn, dim3((unsigned)(units * a.head_items)), dim3(kPtThreads), pt_smem<HD>(), s, mq, mk, mv, a) ==
-                 cudaSuccess
-             ? EE_OK
-             : EE_ERR_LAUNCH;
+  CUtensorMap mq, mk, mv;
+  if (!make_head_map(&mq, p.q, HD, p.n_q, p.tq, p.q_head, p.q_tok, p.group, a.tpt) ||
+      !make_head_map(&mk, p.k, HD, p.n_kv, p.tk, p.k_head, p.k_tok, 1, 128) ||
+      !make_head_map(&mv, p.v, HD, p.n_kv, p.tk, p.v_head, p.v_tok, 1, 128))
+    return EE_ERR_SHAPE;  // a stride the loads cannot address
+  // at most one partial unit per sequence beyond the rows' whole units
+  const long long items = ((long long)p.tq / (2 * a.tpt) + p.n_seq) * p.n_kv * p.splits;
+  if (items > 0x7fffffff) return EE_ERR_SHAPE;
+  const unsigned grid = (unsigned)(items < dp->sms ? items : dp->sms);
+  if (launch_pdl(fn, dim3(grid), dim3(kPtThreads), pt_smem<HD>(), s, mq, mk, mv, a) != cudaSuccess) return EE_ERR_LAUNCH;
+  return launch_combine<T, HD>(p, s);
 }
 
 template <typename T>
