@@ -31,6 +31,8 @@
 // timeout leaves EE_ERR_TIMEOUT in the GEMM status word.
 #pragma once
 
+#include <type_traits>
+
 #include "ee_prompt.cuh"
 #include "ee_tma.cuh"
 #include "ee_umma.cuh"
@@ -44,18 +46,24 @@ struct PromptTcArgs {
   unsigned long long timeout_ns;
 };
 
+#ifndef EE_PT_POLY64
+#define EE_PT_POLY64 0xA4
+#endif
+#ifndef EE_PT_POLY128
+#define EE_PT_POLY128 0x88
+#endif
 constexpr int kPtThreads = 384;
 // registers: 384 threads launch with 168 each; the four warps of loads and MMAs
 // give theirs up to 88 and the softmax warps take 208 (256 x 208 + 128 x 88 =
 // 384 x 168), so that a whole row of S stays in registers
 constexpr int kPtRegsLaunch = 168, kPtRegsSoft = 208, kPtRegsRest = 88;
 static_assert(256 * kPtRegsSoft + 128 * kPtRegsRest <= kPtThreads * kPtRegsLaunch, "the register shares fit the launch");
-constexpr int kPtKeys = 128, kPtInfo = 4;  // keys per block; items published ahead
+constexpr int kPtKeys = 128, kPtInfo = 4, kPtLoads = 8;  // keys per block; items published, loads of K / V ahead
 template <int HD> constexpr int pt_slots() { return HD == 128 ? 5 : 8; }
 template <int HD> constexpr uint32_t pt_tile() { return 128u * HD * 2; }
 template <int HD> constexpr uint32_t pt_off_bar() { return (2 + pt_slots<HD>()) * pt_tile<HD>(); }
-// barriers: full / empty per slot, Q full / empty, S / P / O / O free per tile, V to fix / fixed, item full / empty
-template <int HD> constexpr uint32_t pt_off_info() { return pt_off_bar<HD>() + 8 * (2 * pt_slots<HD>() + 12 + 2 * kPtInfo) + 8; }
+// barriers: full / empty per load of K / V, Q full / empty, S / P (two halves) / S free / O / O free per tile, V to fix / fixed, item full / empty
+template <int HD> constexpr uint32_t pt_off_info() { return pt_off_bar<HD>() + 8 * (2 * kPtLoads + 16 + 2 * kPtInfo) + 8; }
 template <int HD> constexpr uint32_t pt_smem() { return pt_off_info<HD>() + kPtInfo * 64 + 1024; }
 
 // One published item (16 words)
@@ -145,21 +153,89 @@ EE_DEV bool prompt_item(const PromptTcArgs& a, int idx, int units, PromptItem& i
   return true;
 }
 
+// Packed pairs of fp32 (one instruction for two values)
+EE_DEV uint64_t pack64(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+EE_DEV void unpack64(uint64_t v, uint32_t& lo, uint32_t& hi) { asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v)); }
+EE_DEV uint64_t both(float x) { return pack64(__float_as_uint(x), __float_as_uint(x)); }
+EE_DEV uint64_t fma2f(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+EE_DEV uint64_t add2f(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+EE_DEV uint64_t mul2f(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+EE_DEV float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+EE_DEV uint32_t max_nan(uint32_t a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(__uint_as_float(a)), "f"(b));
+  return __float_as_uint(r);
+}
+// 2^x of a pair on the FMA pipe, for x <= 2^8 (below -126: 2^-126, NaN stays):
+// x = n + f with n the nearest integer (the low bits of x + 1.5 * 2^23), 2^f by
+// a minimax polynomial fitted here -- degree 3 for bf16 (relative error 7.5e-5,
+// against 2^-9 of the weights' rounding), degree 4 for fp16 (2.6e-6, 2^-12).
+template <typename T>
+EE_DEV uint64_t exp2_pair(uint64_t x) {
+  uint32_t a, b;
+  unpack64(x, a, b);
+  x = pack64(max_nan(a, -126.f), max_nan(b, -126.f));
+  const uint64_t t = add2f(x, both(12582912.f));
+  const uint64_t f = add2f(x, mul2f(add2f(t, both(-12582912.f)), both(-1.f)));
+  uint64_t p;
+  if (sizeof(T) == 2 && Act<T>::kInt4Base == 128.f) {  // bf16
+    p = fma2f(f, both(0.05517134f), both(0.24261117f));
+    p = fma2f(f, p, both(0.69326103f));
+    p = fma2f(f, p, both(0.99992807f));
+  } else {
+    p = fma2f(f, both(0.00957005f), both(0.05591786f));
+    p = fma2f(f, p, both(0.24024746f));
+    p = fma2f(f, p, both(0.69312182f));
+    p = fma2f(f, p, both(0.99999926f));
+  }
+  unpack64(t, a, b);  // 2^n: n << 23 added to the bits of 1 (1.5 * 2^23 shifts out)
+  return mul2f(p, pack64(a * 8388608u + 0x3f800000u, b * 8388608u + 0x3f800000u));
+}
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(kPtThreads, 1)
     prompt_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                      const __grid_constant__ CUtensorMap mv, const __grid_constant__ PromptTcArgs a) {
-  constexpr int NS = pt_slots<HD>();
+  constexpr int NS = pt_slots<HD>(), NP = kPtLoads;
+  static_assert(NS <= NP, "a barrier per load that the slots can hold");
   constexpr uint32_t TILE = pt_tile<HD>(), PANEL = 128 * 128;  // a panel: 64 columns of 128 rows
   constexpr int PANELS = HD / 64;
+  // hd 64 leaves TMEM for P beside S, so the next scores are computed during the softmax
+  constexpr bool SEP = HD == 64;
+#ifndef EE_PT_PARTS
+#define EE_PT_PARTS 2
+#endif
+  constexpr int PARTS = EE_PT_PARTS;  // pieces in which a block's weights are handed over
+  // pairs of every eight whose exponentials run on the FMA pipe (a bit each): 2 for hd 128, 3 for hd 64
+  constexpr uint32_t kPoly = HD == 64 ? EE_PT_POLY64 : EE_PT_POLY128;
   extern __shared__ __align__(1024) char smem_raw[];
   const uint32_t base0 = smem_u32(smem_raw);
   const uint32_t sb = (base0 + 1023u) & ~1023u;
   char* smem = smem_raw + (sb - base0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t sQ = sb, sKV = sb + 2 * TILE;
-  const uint32_t b_full = sb + pt_off_bar<HD>(), b_empty = b_full + 8 * NS;
-  const uint32_t b_qf = b_empty + 8 * NS, b_qe = b_qf + 8, b_s = b_qe + 8, b_p = b_s + 16, b_o = b_p + 16;
+  const uint32_t b_full = sb + pt_off_bar<HD>(), b_empty = b_full + 8 * NP;
+  const uint32_t b_qf = b_empty + 8 * NP, b_qe = b_qf + 8, b_s = b_qe + 8, b_p = b_s + 16, b_sf = b_p + 32, b_o = b_sf + 16;
   const uint32_t b_of = b_o + 16, b_req = b_of + 16, b_fix = b_req + 8, b_if = b_fix + 8, b_ie = b_if + 8 * kPtInfo;
   const uint32_t off_tm = b_ie + 8 * kPtInfo - sb;
   volatile PromptItem* ring = reinterpret_cast<volatile PromptItem*>(smem + pt_off_info<HD>());
@@ -168,7 +244,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     tma_prefetch_map(&mq);
     tma_prefetch_map(&mk);
     tma_prefetch_map(&mv);
-    for (int s = 0; s < NS; ++s) {
+    for (int s = 0; s < NP; ++s) {
       mbar_init(b_full + 8 * s, 1);
       mbar_init(b_empty + 8 * s, 1);
     }
@@ -179,6 +255,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     for (int t = 0; t < 2; ++t) {
       mbar_init(b_s + 8 * t, 1);
       mbar_init(b_p + 8 * t, 4);
+      mbar_init(b_p + 16 + 8 * t, 4);
+      mbar_init(b_sf + 8 * t, 4);
       mbar_init(b_o + 8 * t, 1);
       mbar_init(b_of + 8 * t, 4);
     }
@@ -197,7 +275,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + off_tm);
-  // TMEM columns: S (P over its first half) of tile t at 128 t, O at 256 + 128 t
+  // TMEM columns: S of tile t at 128 t, O at 256 + 128 t (SEP: 256 + 64 t), P over S (SEP: at 384 + 64 t)
+  constexpr uint32_t OC = SEP ? 64 : 128;
   // The consumers' view of the item ring: wait for item i, read it; release when done with it.
   auto item_wait = [&](int i) { return mbar_wait(b_if + 8 * (i % kPtInfo), (uint32_t)((i / kPtInfo) & 1), a.timeout_ns); };
   auto item_done = [&](int i) { mbar_arrive(b_ie + 8 * (i % kPtInfo)); };
@@ -207,7 +286,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     if (warp == 8) {
       // ---------------- items and loads ----------------
       bool ok = true;
-      int units = 0, n = 0, nq = 0;  // K / V tiles and Q loads issued so far
+      int units = 0, n = 0, nq = 0, sl = 0;  // K / V tiles and Q loads issued so far, next slot
+      uint32_t g = 0, slot_load[NS];         // loads (barrier phases) of K / V so far, and each slot's last one
       for (int b = lane; b < p.n_seq; b += 32) units += (prompt_seq(p, b).qlen + 2 * a.tpt - 1) / (2 * a.tpt);
       units = __reduce_add_sync(0xffffffffu, units);
       const uint32_t qbytes = (uint32_t)(p.group * a.tpt) * 128u * PANELS;
@@ -224,20 +304,26 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           r->n[0] = it.n[0]; r->n[1] = it.n[1]; r->tail = it.tail;
           r->nbm = more && ok ? it.nbm : -1;
           mbar_arrive(b_if + 8 * (i % kPtInfo));
-          auto load_kv = [&](int w) {  // tile w of the item: K(0) V(0) K(1) V(1) ...
-            const int sl = n % NS;
-            if (n >= NS && !mbar_wait(b_empty + 8 * sl, (uint32_t)((n / NS - 1) & 1), a.timeout_ns)) {
-              ok = false;
-              return;
+          // tile w of the item (K(0) V(0) K(1) V(1) ...) into the next slot, on the load's barrier
+          auto load_kv = [&](int w) {
+            if (n >= NS) {  // the load that used the slot before has been consumed
+              const uint32_t was = slot_load[sl];
+              if (!mbar_wait(b_empty + 8 * (was % NP), (was / NP) & 1, a.timeout_ns)) {
+                ok = false;
+                return;
+              }
             }
-            mbar_arrive_expect_tx(b_full + 8 * sl, TILE);
+            slot_load[sl] = g;
             for (int c = 0; c < PANELS; ++c)
               tma_load_3d(sKV + sl * TILE + c * PANEL, (w & 1) ? &mv : &mk, 64 * c, it.kvh,
-                          it.k0 + it.key0 + (w >> 1) * kPtKeys, b_full + 8 * sl);
+                          it.k0 + it.key0 + (w >> 1) * kPtKeys, b_full + 8 * (g % NP));
             ++n;
+            if (++sl == NS) sl = 0;
           };
           if (more && ok && it.nbm > 0) {
+            mbar_arrive_expect_tx(b_full + 8 * (g % NP), TILE);
             load_kv(0);
+            ++g;
             // Q: its buffers are free when the last scores of the previous item are done
             if (ok && nq > 0 && !mbar_wait(b_qe, (uint32_t)((nq - 1) & 1), a.timeout_ns)) ok = false;
             if (ok) {
@@ -248,7 +334,11 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                     tma_load_3d(sQ + t * TILE + c * PANEL, &mq, 64 * c, it.kvh * p.group, it.q0 + it.tok + t * a.tpt, b_qf);
               ++nq;
             }
-            for (int w = 1; w < 2 * it.nbm && ok; ++w) load_kv(w);
+            for (int j = 0; j < it.nbm && ok; ++j, ++g) {  // V(j) and K(j + 1)
+              mbar_arrive_expect_tx(b_full + 8 * (g % NP), j + 1 < it.nbm ? 2 * TILE : TILE);
+              load_kv(2 * j + 1);
+              if (j + 1 < it.nbm && ok) load_kv(2 * j + 2);
+            }
           }
         }
         ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
@@ -256,95 +346,117 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       }
       // everything issued lands before the CTA may exit
       if (lane == 0) {
-        for (int g = max(n - NS, 0); g < n; ++g)
-          if (!mbar_wait(b_full + 8 * (g % NS), (uint32_t)((g / NS) & 1), a.timeout_ns)) ok = false;
-        if (nq > 0 && !mbar_wait(b_qf, (uint32_t)((nq - 1) & 1), a.timeout_ns)) ok = false;
+        if (ok)
+          for (uint32_t e = g > NP ? g - NP : 0; e < g; ++e)
+            if (!mbar_wait(b_full + 8 * (e % NP), (e / NP) & 1, a.timeout_ns)) ok = false;
+        if (ok && nq > 0 && !mbar_wait(b_qf, (uint32_t)((nq - 1) & 1), a.timeout_ns)) ok = false;
         if (!ok) atomicCAS(a.status, 0, (int)EE_ERR_TIMEOUT);
       }
       __syncwarp();
     } else if (warp == 9) {
-      // ---------------- MMA issue ----------------
-      if (lane == 0) {
-        constexpr uint32_t id_s = umma_idesc<T>(128, 128), id_o = umma_idesc<T>(128, HD) | kIdescBMajorMN;
-        bool ok = true;
-        int n = 0, nq = 0, nfix = 0;   // K / V tiles, Q loads and fixed tails consumed so far
-        int np[2] = {0, 0}, no[2] = {0, 0};  // P blocks and outputs of each tile so far
-        auto wait_slot = [&](int g) { return mbar_wait(b_full + 8 * (g % NS), (uint32_t)((g / NS) & 1), a.timeout_ns); };
-        auto scores = [&](int t, int g) {  // S_t = Q_t K^T, K in ring tile g
-          const uint64_t qd = umma_desc_sw128(sQ + t * TILE), kd = umma_desc_sw128(sKV + (uint32_t)(g % NS) * TILE);
+      // ---------------- MMA issue (all lanes run the loops, see elect_one) ----------------
+      // The tensor cores queue about two MMAs beyond the running one and a wait costs 100 cycles or more even when
+      // it is over, so the issuer's waits are few: one for V(j) and K(j + 1) together, then the weights.
+      constexpr uint32_t id_s = umma_idesc<T>(128, 128), id_o = umma_idesc<T>(128, HD) | kIdescBMajorMN;
+      const uint64_t q_desc = umma_desc_sw128(sQ), k_desc = umma_desc_sw128(sKV), v_desc = umma_desc_mn128(sKV, PANEL);
+      auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, a.timeout_ns)); };
+      bool ok = true;
+      int sl = 0;                         // slot of the next K / V tile
+      uint32_t g = 0, nq = 0, nfix = 0;   // loads of K / V, Q loads and fixed tails so far
+      uint32_t np[2] = {0, 0}, no[2] = {0, 0};  // P blocks and outputs of each tile so far
+      auto scores = [&](int t, int slot) {      // S_t = Q_t K^T
+        const uint64_t qd = q_desc + (uint64_t)(t * (TILE >> 4)), kd = k_desc + (uint64_t)(slot * (TILE >> 4));
+        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk) {
             const uint64_t o = (uint64_t)(((kk >> 2) * PANEL + (kk & 3) * 32) >> 4);
             umma_f16(tmem + 128 * t, qd + o, kd + o, id_s, kk ? 1u : 0u);
           }
           umma_commit(b_s + 8 * t);
-        };
-        for (int i = 0; ok; ++i) {
-          if (!item_wait(i)) {
-            ok = false;
-            break;
-          }
-          const volatile PromptItem* r = ring + i % kPtInfo;
-          const int nbm = r->nbm, n0 = r->n[0], n1 = r->n[1], tail = r->tail;
-          item_done(i);
-          if (nbm < 0) break;
-          if (nbm == 0) continue;
-          ok = mbar_wait(b_qf, (uint32_t)(nq & 1), a.timeout_ns) && wait_slot(n);
-          if (!ok) break;
-          ++nq;
-          tc_fence_after();
-          if (n0 > 0) scores(0, n);
-          if (n1 > 0) scores(1, n);
-          umma_commit(b_empty + 8 * (n % NS));
+        }
+        __syncwarp();
+      };
+      for (int i = 0; ok; ++i) {
+        ok = __all_sync(0xffffffffu, item_wait(i));
+        if (!ok) break;
+        const volatile PromptItem* r = ring + i % kPtInfo;
+        const int nbm = __shfl_sync(0xffffffffu, r->nbm, 0), n0 = __shfl_sync(0xffffffffu, r->n[0], 0);
+        const int n1 = __shfl_sync(0xffffffffu, r->n[1], 0), tail = __shfl_sync(0xffffffffu, r->tail, 0);
+        if (lane == 0) item_done(i);
+        __syncwarp();
+        if (nbm < 0) break;
+        if (nbm == 0) continue;
+        ok = wait(b_qf, nq & 1) && wait(b_full + 8 * (g % NP), (g / NP) & 1);
+        if (!ok) break;
+        ++nq;
+        tc_fence_after();
+        if (n0 > 0) scores(0, sl);
+        if (n1 > 0) scores(1, sl);
+        if (elect_one()) {
+          umma_commit(b_empty + 8 * (g % NP));
           if (nbm == 1) umma_commit(b_qe);
-          for (int j = 0; j < nbm && ok; ++j) {
-            const int vg = n + 2 * j + 1, vs = vg % NS;
-            ok = wait_slot(vg);
-            if (ok && j + 1 < nbm) ok = wait_slot(vg + 1);
-            const bool fix = j + 1 == nbm && tail < kPtKeys;
-            if (ok && fix) mbar_arrive(b_req);
-            int fixed = fix ? 0 : 1;
-            const uint64_t vd = umma_desc_mn128(sKV + (uint32_t)vs * TILE, PANEL);
+        }
+        __syncwarp();
+        ++g;
+        for (int j = 0; j < nbm; ++j, ++g) {
+          const int vs = sl + 1 == NS ? 0 : sl + 1, ks = vs + 1 == NS ? 0 : vs + 1;  // V(j) and K(j + 1)
+          ok = wait(b_full + 8 * (g % NP), (g / NP) & 1);
+          if (!ok) break;
+          bool fix = j + 1 == nbm && tail < kPtKeys;
+          if (fix && lane == 0) mbar_arrive(b_req);
+          __syncwarp();
+          const uint64_t vd = v_desc + (uint64_t)(vs * (TILE >> 4));
+          if (SEP) {
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-              const int nt = t ? n1 : n0;
-              if (!ok || j >= nt) continue;
-              // O of the tile's previous item has been read
-              if (j == 0 && no[t] > 0) ok = mbar_wait(b_of + 8 * t, (uint32_t)((no[t] - 1) & 1), a.timeout_ns);
-              ok = ok && mbar_wait(b_p + 8 * t, (uint32_t)(np[t] & 1), a.timeout_ns);
-              if (ok && !fixed) {
-                ok = mbar_wait(b_fix, (uint32_t)(nfix & 1), a.timeout_ns);
-                ++nfix;
-                fixed = 1;
-              }
-              if (!ok) continue;
-              ++np[t];
+              if (!ok || j + 1 >= (t ? n1 : n0)) continue;
+              ok = wait(b_sf + 8 * t, np[t] & 1);  // S(j) is in the softmax's registers
               tc_fence_after();
-#pragma unroll
-              for (int kk = 0; kk < kPtKeys / 16; ++kk)  // O_t += P_t V(j), 16 keys at a time
-                umma_f16_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * kk, vd + (uint64_t)((kk * 2048) >> 4), id_o,
-                            (j | kk) ? 1u : 0u);
-              if (j + 1 < nt) {
-                scores(t, vg + 1);
-              } else {
-                umma_commit(b_o + 8 * t);
-                ++no[t];
-              }
-            }
-            if (ok) {
-              umma_commit(b_empty + 8 * vs);
-              if (j + 1 < nbm) umma_commit(b_empty + 8 * ((vg + 1) % NS));
-              if (j + 2 == nbm) umma_commit(b_qe);
+              if (ok) scores(t, ks);
             }
           }
-          n += 2 * nbm;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const int nt = t ? n1 : n0;
+            if (!ok || j >= nt) continue;
+            // O of the tile's previous item has been read
+            if (j == 0 && no[t] > 0) ok = wait(b_of + 8 * t, (no[t] - 1) & 1);
+            if (ok && fix) {
+              ok = wait(b_fix, nfix & 1);
+              ++nfix;
+              fix = false;
+            }
+#pragma unroll
+            for (int h = 0; h < PARTS; ++h) {  // O_t += P_t V(j)
+              ok = ok && wait(b_p + 16 * h + 8 * t, np[t] & 1);
+              tc_fence_after();
+              if (ok && elect_one()) {
+#pragma unroll
+                for (int kk = 8 / PARTS * h; kk < 8 / PARTS * (h + 1); ++kk)
+                  umma_f16_ts(tmem + 256 + OC * t, tmem + (SEP ? 384 + 64 * t : 128 * t) + 8 * kk,
+                              vd + (uint64_t)((kk * 2048) >> 4), id_o, (j | kk) ? 1u : 0u);
+                if (h == PARTS - 1 && (SEP || j + 1 == nt)) umma_commit(b_o + 8 * t);
+              }
+              __syncwarp();
+            }
+            ++np[t];
+            if (ok && !SEP && j + 1 < nt) scores(t, ks);
+            if (j + 1 == nt) ++no[t];
+          }
+          if (!ok) break;
+          if (elect_one()) {
+            umma_commit(b_empty + 8 * (g % NP));
+            if (j + 2 == nbm) umma_commit(b_qe);
+          }
+          __syncwarp();
+          sl = ks;
         }
-        if (!ok) atomicCAS(a.status, 0, (int)EE_ERR_TIMEOUT);
       }
-      __syncwarp();
+      if (!ok && lane == 0) atomicCAS(a.status, 0, (int)EE_ERR_TIMEOUT);
     } else if (warp == 10) {
       // ---------------- V rows past the sequence's end ----------------
       int n = 0, nfix = 0;
+      uint32_t g = 0;
       for (int i = 0;; ++i) {
         bool ok = item_wait(i);
         const volatile PromptItem* r = ring + i % kPtInfo;
@@ -352,14 +464,15 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         __syncwarp();
         if (lane == 0) item_done(i);
         if (!__all_sync(0xffffffffu, ok) || nbm < 0) break;
+        if (nbm == 0) continue;
         n += 2 * nbm;
-        if (nbm == 0 || tail == kPtKeys) continue;
-        // not before the MMA warp has come to the block: earlier, the slot's parity may be an older load's
-        const int g = n - 1;
+        g += nbm + 1;
+        if (tail == kPtKeys) continue;
+        // not before the MMA warp has come to the block: earlier, the barrier's parity may be an older load's
         ok = mbar_wait(b_req, (uint32_t)(nfix++ & 1), a.timeout_ns) &&
-             mbar_wait(b_full + 8 * (g % NS), (uint32_t)((g / NS) & 1), a.timeout_ns);
+             mbar_wait(b_full + 8 * ((g - 1) % NP), ((g - 1) / NP) & 1, a.timeout_ns);
         if (!__all_sync(0xffffffffu, ok)) break;
-        const uint32_t v = sKV + (uint32_t)(g % NS) * TILE;
+        const uint32_t v = sKV + (uint32_t)((n - 1) % NS) * TILE;
         for (int e = lane; e < (kPtKeys - tail) * 8 * PANELS; e += 32) {
           const int row = tail + e / (8 * PANELS), c = e % (8 * PANELS);
           asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v + (c >> 3) * PANEL + row * 128 + (c & 7) * 16),
@@ -376,8 +489,9 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPtRegsSoft));
     const int t = warp >> 2, q4 = warp & 3, r = 32 * q4 + lane;
     const int rtok = r / p.group, rhead = r - rtok * p.group;
-    const uint32_t ts = tmem + 128 * t + ((uint32_t)(32 * q4) << 16), to = tmem + 256 + 128 * t + ((uint32_t)(32 * q4) << 16);
-    int ns = 0, no = 0;  // score blocks and outputs so far
+    const uint32_t ts = tmem + 128 * t + ((uint32_t)(32 * q4) << 16), to = tmem + 256 + OC * t + ((uint32_t)(32 * q4) << 16);
+    const uint32_t tp = SEP ? tmem + 384 + 64 * t + ((uint32_t)(32 * q4) << 16) : ts;
+    int ns = 0, no = 0;  // score blocks and commits of O (per block when SEP, else per item) so far
     bool ok = true;
     for (int i = 0; ok; ++i) {
       ok = __all_sync(0xffffffffu, item_wait(i));
@@ -402,8 +516,14 @@ __global__ void __launch_bounds__(kPtThreads, 1)
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, v[c]);
         tmem_wait_ld();
+        if (SEP) {  // the whole of S is in registers: the next scores may be written
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(b_sf + 8 * t);
+        }
         const int left = lim - j * kPtKeys;
-        if (__any_sync(0xffffffffu, left < kPtKeys)) {
+        const bool masked = __any_sync(0xffffffffu, left < kPtKeys);
+        if (masked) {
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -413,17 +533,24 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         float x[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          x[c] = __uint_as_float(v[c][0]);
+          x[c] = fmaxf(__uint_as_float(v[c][0]), __uint_as_float(v[c][1]));
 #pragma unroll
-          for (int e = 1; e < 32; ++e) x[c] = fmaxf(x[c], __uint_as_float(v[c][e]));
+          for (int e = 2; e < 32; e += 2) x[c] = max3(x[c], __uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1]));
         }
-        const float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * p.scale_log2;
+        const float mx = fmaxf(max3(x[0], x[1], x[2]), x[3]) * p.scale_log2;
         float f = 1.f;
         if (mx > m + 8.f) {  // also from -inf, with f = 0: nothing to rescale yet
           f = ex2(m - mx);
           m = mx;
         }
-        if (__any_sync(0xffffffffu, f != 1.f) && j > 0) {
+        const bool rescale = __any_sync(0xffffffffu, f != 1.f) && j > 0;
+        if (SEP && j > 0) {  // O += P(j-1) V(j-1) is done: P may be written, O rescaled
+          ok = __all_sync(0xffffffffu, mbar_wait(b_o + 8 * t, (uint32_t)((no - 1) & 1), a.timeout_ns));
+          if (!ok) break;
+          tc_fence_after();
+        }
+        if (SEP) ++no;
+        if (rescale) {
 #pragma unroll 1
           for (int c = 0; c < HD / 16; ++c) {
             uint32_t o[16];
@@ -436,29 +563,51 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           tmem_wait_st();
         }
         const float neg = m == -INFINITY ? 0.f : -m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint64_t sc2 = both(p.scale_log2), neg2 = both(neg);
+        uint64_t sum[4] = {0, 0, 0, 0};
+        // weights of the block, 64 keys at a time: the products with the first half start under the second
+        auto weights = [&](auto mixed) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+          for (int c = 0; c < 4; ++c) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float p0 = ex2(fmaf(__uint_as_float(v[c][e]), p.scale_log2, neg));
-            const float p1 = ex2(fmaf(__uint_as_float(v[c][e + 1]), p.scale_log2, neg));
-            sum[c] += p0 + p1;
-            v[c >> 1][(c & 1) * 16 + e / 2] = Act<T>::pack2(p0, p1);
+            for (int e = 0; e < 32; e += 2) {
+              uint64_t y = fma2f(pack64(v[c][e], v[c][e + 1]), sc2, neg2);
+              if (decltype(mixed)::value && kPoly >> ((e >> 1) & 7) & 1) {
+                y = exp2_pair<T>(y);
+              } else {
+                uint32_t y0, y1;
+                unpack64(y, y0, y1);
+                y = pack64(__float_as_uint(ex2(__uint_as_float(y0))), __float_as_uint(ex2(__uint_as_float(y1))));
+              }
+              sum[c] = add2f(sum[c], y);
+              uint32_t y0, y1;
+              unpack64(y, y0, y1);
+              v[c >> 1][(c & 1) * 16 + e / 2] = Act<T>::pack2(__uint_as_float(y0), __uint_as_float(y1));
+            }
+            if (c & 1) tmem_st32(tp + 32 * (c >> 1), v[c >> 1]);
+            if (c == 3 || (PARTS == 2 && c == 1)) {
+              tmem_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(b_p + 16 * (PARTS - 1 ? c >> 1 : 0) + 8 * t);
+            }
           }
-          if (c & 1) tmem_st32(ts + 32 * (c >> 1), v[c >> 1]);
+        };
+        // exact zeros where keys are masked or nothing has been seen
+        if (masked || __any_sync(0xffffffffu, m == -INFINITY)) weights(std::false_type{});
+        else weights(std::true_type{});
+        {
+          const uint64_t s2 = add2f(add2f(sum[0], sum[1]), add2f(sum[2], sum[3]));
+          uint32_t s0, s1;
+          unpack64(s2, s0, s1);
+          l = l * f + (__uint_as_float(s0) + __uint_as_float(s1));
         }
-        l = l * f + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(b_p + 8 * t);
       }
       if (!ok) break;
       if (nt > 0) {
-        ok = __all_sync(0xffffffffu, mbar_wait(b_o + 8 * t, (uint32_t)(no & 1), a.timeout_ns));
+        if (!SEP) ++no;
+        ok = __all_sync(0xffffffffu, mbar_wait(b_o + 8 * t, (uint32_t)((no - 1) & 1), a.timeout_ns));
         if (!ok) break;
-        ++no;
       }
       tc_fence_after();
       const bool whole = p.splits == 1;

@@ -32,6 +32,17 @@ EE_DEV void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" 
 // generic-proxy shared-memory writes -> visible to the async proxy (MMA reads)
 EE_DEV void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// One lane of a converged warp. A warp that issues MMAs runs its loops with all
+// lanes, so that descriptors and addresses are warp-uniform values (what the
+// MMA instruction takes), and only the issue itself is under this predicate:
+// issued from code that one lane has branched into, a 128 x 128 x 16 MMA
+// costs about 90 cycles of operand moves, more than it takes to execute.
+EE_DEV bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+
 // ---- descriptors ------------------------------------------------------------
 // Shared-memory matrix descriptor of a K-major, 128-byte-swizzled tile whose
 // first row starts at `saddr` (inside a 1024-byte aligned swizzle atom):
