@@ -12,15 +12,15 @@ namespace ee {
 // few query rows per key head
 // ---------------------------------------------------------------------------
 // A row is (token, head of the key head's group), so a key head's whole group
-// shares one read of its keys. A CTA takes 16 RT rows of one sequence and key
+// shares one read of its keys. A CTA takes 16 rows of one sequence and key
 // head and, where the units alone would not fill the GPU, one of `splits`
-// parts of their keys (prompt_combine_kernel joins the parts); its warps are
-// RT row tiles x KG key groups, each with its own running maximum and sum over
-// its share of every 64-key stage, merged through shared memory at the end.
+// parts of their keys (prompt_combine_kernel joins the parts); each of its
+// warps has its own running maximum and sum over its 16 keys of every 64-key
+// stage, merged through shared memory at the end.
 // HBM-bound on the keys and values; the ring holds three or four stages, and
 // two or three CTAs share an SM.
 constexpr int kPrKeys = 64;   // keys per stage
-template <int RT> constexpr int pr_warps() { return RT == 1 ? 4 : 8; }
+constexpr int kPrWarps = 4;
 template <int HD> constexpr int pr_stages() { return HD == 128 ? 3 : 4; }
 template <int HD> constexpr int pr_smem() { return pr_stages<HD>() * 2 * kPrKeys * HD * 2; }
 
@@ -33,11 +33,10 @@ EE_DEV void pr_ldsm_t(uint32_t addr, uint32_t (&r)[4]) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
 
-template <typename T, int HD, int RT>
-__global__ void __launch_bounds__(32 * pr_warps<RT>()) prompt_rows_kernel(const __grid_constant__ PromptArgs a) {
-  constexpr int NW = pr_warps<RT>(), NT = 32 * NW, NS = pr_stages<HD>();
-  constexpr int KG = NW / RT;            // key groups
-  constexpr int WK = kPrKeys / KG;       // keys of a stage per warp
+template <typename T, int HD>
+__global__ void __launch_bounds__(32 * kPrWarps) prompt_rows_kernel(const __grid_constant__ PromptArgs a) {
+  constexpr int NW = kPrWarps, NT = 32 * NW, NS = pr_stages<HD>();
+  constexpr int WK = kPrKeys / NW;       // keys of a stage per warp
   constexpr int RB = HD * 2;             // bytes per key row
   constexpr int CH = HD / 8;             // 16-byte chunks per key row
   constexpr int TILE = kPrKeys * RB;
@@ -45,13 +44,13 @@ __global__ void __launch_bounds__(32 * pr_warps<RT>()) prompt_rows_kernel(const 
   __shared__ int sh[NW + 2];
   pdl_entry();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int rt = warp % RT, kg = warp / RT, g = lane >> 2, t = lane & 3;
+  const int g = lane >> 2, t = lane & 3;
   const int kvh = blockIdx.y, part = blockIdx.x % a.splits;
   PromptSeq s;
-  if (!prompt_find(a, blockIdx.x / a.splits, a.group, 16 * RT, NT, sh, s)) return;
-  const int rows = s.qlen * a.group, r0 = s.blk * 16 * RT;
+  if (!prompt_find(a, blockIdx.x / a.splits, a.group, 16, NT, sh, s)) return;
+  const int rows = s.qlen * a.group, r0 = s.blk * 16;
   // keys this CTA's rows see at most, and its part of them in whole stages
-  const int last_tok = (min(r0 + 16 * RT, rows) - 1) / a.group;
+  const int last_tok = (min(r0 + 16, rows) - 1) / a.group;
   const int kend = a.causal ? max(min(s.klen, s.klen - s.qlen + last_tok + 1), 0) : s.klen;
   const int nst = (kend + kPrKeys - 1) / kPrKeys;
   const int st0 = (int)((long long)nst * part / a.splits), st1 = (int)((long long)nst * (part + 1) / a.splits);
@@ -76,7 +75,7 @@ __global__ void __launch_bounds__(32 * pr_warps<RT>()) prompt_rows_kernel(const 
     cp_async_commit();
   }
   // this warp's query fragments
-  const int ra = r0 + rt * 16 + g, rb = ra + 8;
+  const int ra = r0 + g, rb = ra + 8;
   uint32_t qf[HD / 16][4];
   {
     auto qrow = [&](int r) {
@@ -110,7 +109,7 @@ __global__ void __launch_bounds__(32 * pr_warps<RT>()) prompt_rows_kernel(const 
     const uint32_t kt = sb + ((st - st0) % NS) * 2 * TILE, vt = kt + TILE;
 #pragma unroll
     for (int k1 = 0; k1 < WK; k1 += 16) {
-      const int kl = kg * WK + k1;             // first of 16 keys, in the stage
+      const int kl = warp * WK + k1;            // first of 16 keys, in the stage
       const int key = st * kPrKeys + kl;       // and in the sequence
       if (key >= kend) break;
       float p[2][4] = {};
@@ -181,7 +180,7 @@ __global__ void __launch_bounds__(32 * pr_warps<RT>()) prompt_rows_kernel(const 
     l0 += __shfl_xor_sync(0xffffffffu, l0, d);
     l1 += __shfl_xor_sync(0xffffffffu, l1, d);
   }
-  // merge the key groups: [warp][16 rows][HD + 4] fp32 over the stages
+  // merge the warps: [warp][16 rows][HD + 4] fp32 over the stages
   constexpr int ML = HD + 4;
   static_assert(NW * 16 * ML * 4 <= NS * 2 * kPrKeys * RB, "the merge fits the stages");
   float* mg = reinterpret_cast<float*>(smem) + warp * 16 * ML;
@@ -198,19 +197,19 @@ __global__ void __launch_bounds__(32 * pr_warps<RT>()) prompt_rows_kernel(const 
     mg[(g + 8) * ML + HD + 1] = l1;
   }
   __syncthreads();
-  for (int i = tid; i < 16 * RT * (HD / 4); i += NT) {  // 4 values of a row over the key groups
+  for (int i = tid; i < 16 * (HD / 4); i += NT) {  // 4 values of a row over the warps
     const int r = i / (HD / 4), c = (i % (HD / 4)) * 4;
     if (r0 + r >= rows) continue;
-    const float* base = reinterpret_cast<const float*>(smem) + ((r >> 4) * 16 + (r & 15)) * ML;
+    const float* base = reinterpret_cast<const float*>(smem) + r * ML;
     float m = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < KG; ++w) m = fmaxf(m, base[w * RT * 16 * ML + HD]);
+    for (int w = 0; w < NW; ++w) m = fmaxf(m, base[w * 16 * ML + HD]);
     const float u = m == -INFINITY ? 0.f : m;
     float l = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < KG; ++w) {
-      const float* p = base + w * RT * 16 * ML;
+    for (int w = 0; w < NW; ++w) {
+      const float* p = base + w * 16 * ML;
       const float f = exp2f(p[HD] - u);
       const float4 v = *reinterpret_cast<const float4*>(p + c);
       l += f * p[HD + 1];
@@ -306,39 +305,27 @@ __global__ void __launch_bounds__(kPrCombine) prompt_combine_kernel(const __grid
 
 // How a call runs, by what the host knows of it: rows (queries x group) per
 // sequence and key head, and keys per sequence, on average.
-//   tc      more than 64 rows: the tensor-core kernel's 128-row tiles
-//   rt      16-row tiles per CTA of the rows kernel
-//   splits  parts of the keys: enough CTAs for four an SM, of 128 keys or more
-#ifndef EE_PROMPT_TC_ROWS
-#define EE_PROMPT_TC_ROWS 16
-#endif
-#ifndef EE_PROMPT_TC_MINK
-#define EE_PROMPT_TC_MINK 512
-#endif
-#ifndef EE_PROMPT_WANT
-#define EE_PROMPT_WANT 4LL
-#endif
-#ifndef EE_PROMPT_MINK
-#define EE_PROMPT_MINK 128
-#endif
-struct PromptPlan { bool tc; int rt, splits; };
+//   tc      more than 16 rows: the tensor-core kernel's 128-row tiles (8 x 50
+//           new tokens behind 816, 16 heads of 128: 27 us, 68 with 64-row warp
+//           MMA units), 16 or fewer: the rows kernel's single MMA row tile
+//   splits  parts of the keys, joined by a second launch. Rows kernel: enough
+//           CTAs for four an SM, of 128 keys or more each (two or eight an SM
+//           measured within 10 % or slower: 8 x 4096 keys, 32 / 8 heads of 128:
+//           53 / 47 / 49 us for 2 / 4 / 8). Tensor-core kernel: where the items
+//           would leave SMs idle, parts of 512 keys or more.
+constexpr long long kPrRows = 16, kPrCtasPerSm = 4, kPrMinKeys = 128, kPtMinKeys = 512;
+struct PromptPlan { bool tc; int splits; };
 static PromptPlan prompt_plan(long long tq, long long tk, int n_seq, int n_q, int n_kv) {
-  PromptPlan pl{};
-  const long long rows = tq * (n_q / n_kv);
-  pl.tc = rows > (long long)EE_PROMPT_TC_ROWS * n_seq && tk > 0 && n_q / n_kv <= 128;
-  pl.rt = rows <= 16LL * n_seq ? 1 : 4;
-  pl.splits = 1;
+  PromptPlan pl{false, 1};
   if (n_seq < 1) return pl;
-  if (pl.tc) {
-    const long long per = 256 / (n_q / n_kv) * (n_q / n_kv);
-    const long long items = (rows / per > n_seq ? rows / per : n_seq) * n_kv;
-    const long long want = device_sms() / items, most = tk / n_seq / EE_PROMPT_TC_MINK;
-    const long long s = want < most ? want : most;
-    pl.splits = s < 1 ? 1 : (int)s;
-    return pl;
-  }
-  const long long units = (rows / (16 * pl.rt) > n_seq ? rows / (16 * pl.rt) : n_seq) * n_kv;
-  const long long want = (EE_PROMPT_WANT * device_sms() + units - 1) / units, most = (tk / n_seq + EE_PROMPT_MINK - 1) / EE_PROMPT_MINK;
+  const int group = n_q / n_kv;
+  const long long rows = tq * group;
+  pl.tc = rows > kPrRows * n_seq && tk > 0 && group <= 128;
+  // rows of a unit: two tiles of whole tokens, or one MMA tile
+  const long long per = pl.tc ? 2 * (128 / group) * group : kPrRows;
+  const long long units = (rows / per > n_seq ? rows / per : n_seq) * n_kv;
+  const long long want = pl.tc ? device_sms() / units : (kPrCtasPerSm * device_sms() + units - 1) / units;
+  const long long most = pl.tc ? tk / n_seq / kPtMinKeys : (tk / n_seq + kPrMinKeys - 1) / kPrMinKeys;
   const long long s = want < most ? want : most;
   pl.splits = s < 1 ? 1 : (int)(s < kPrMaxSplits ? s : kPrMaxSplits);
   return pl;
@@ -355,15 +342,15 @@ static int launch_combine(const PromptArgs& a, cudaStream_t s) {
              : EE_ERR_LAUNCH;
 }
 
-template <typename T, int HD, int RT>
+template <typename T, int HD>
 static int launch_rows(const PromptArgs& a, cudaStream_t s) {
-  auto fn = prompt_rows_kernel<T, HD, RT>;
+  auto fn = prompt_rows_kernel<T, HD>;
   static std::atomic<int> set[64];
   allow_max_smem(fn, set);
   // at most one partial block per sequence beyond the rows' whole blocks
-  const long long units = (long long)a.tq * a.group / (16 * RT) + a.n_seq;
+  const long long units = (long long)a.tq * a.group / 16 + a.n_seq;
   if (units * a.splits > 0x7fffffff) return EE_ERR_SHAPE;
-  if (launch_pdl(fn, dim3((unsigned)(units * a.splits), a.n_kv), dim3(32 * pr_warps<RT>()), pr_smem<HD>(), s, a) !=
+  if (launch_pdl(fn, dim3((unsigned)(units * a.splits), a.n_kv), dim3(32 * kPrWarps), pr_smem<HD>(), s, a) !=
       cudaSuccess)
     return EE_ERR_LAUNCH;
   return launch_combine<T, HD>(a, s);
@@ -415,8 +402,7 @@ static int launch_tc(const PromptArgs& p, cudaStream_t s) {
 template <typename T>
 static int launch_prompt(const PromptArgs& a, const PromptPlan& pl, int hd, cudaStream_t s) {
   if (pl.tc) return hd == 64 ? launch_tc<T, 64>(a, s) : launch_tc<T, 128>(a, s);
-  if (hd == 64) return pl.rt == 1 ? launch_rows<T, 64, 1>(a, s) : launch_rows<T, 64, 4>(a, s);
-  return pl.rt == 1 ? launch_rows<T, 128, 1>(a, s) : launch_rows<T, 128, 4>(a, s);
+  return hd == 64 ? launch_rows<T, 64>(a, s) : launch_rows<T, 128>(a, s);
 }
 
 }  // namespace ee

@@ -13,7 +13,13 @@
 // While one tile's threads are in the softmax, the tensor cores run the other
 // tile's two products: per 128 x 128 block and tile 2 x 128^2 hd MACs (1024
 // cycles at hd 128) against 128^2 exponentials (1024 cycles of the MUFU), so
-// both are near their limit at hd 128 and the exponentials lead at hd 64.
+// both are near their limit at hd 128 and the exponentials lead at hd 64. (A
+// share of the exponentials as polynomials on the FMA pipe was slower at every
+// share: 411 -> 428 / 472 / 530 us at hd 64 for 1/8, 1/4, 1/2 of them.)
+//
+// Measured: 8192 causal tokens, 16 / 4 heads of 128: 242 us, 1137 TFLOP/s,
+// 0.70 of the measured GEMM rate; 16 / 4 heads of 64 without a mask: 411 us,
+// the MUFU 74 % busy while an SM has work.
 //
 // The running maximum m is a reference, not the exact maximum: it moves only
 // when a row's maximum exceeds it by more than 2^8, so O is rarely rescaled
@@ -31,8 +37,6 @@
 // timeout leaves EE_ERR_TIMEOUT in the GEMM status word.
 #pragma once
 
-#include <type_traits>
-
 #include "ee_prompt.cuh"
 #include "ee_tma.cuh"
 #include "ee_umma.cuh"
@@ -46,12 +50,6 @@ struct PromptTcArgs {
   unsigned long long timeout_ns;
 };
 
-#ifndef EE_PT_POLY64
-#define EE_PT_POLY64 0xA4
-#endif
-#ifndef EE_PT_POLY128
-#define EE_PT_POLY128 0x88
-#endif
 constexpr int kPtThreads = 384;
 // registers: 384 threads launch with 168 each; the four warps of loads and MMAs
 // give theirs up to 88 and the softmax warps take 208 (256 x 208 + 128 x 88 =
@@ -171,45 +169,10 @@ EE_DEV uint64_t add2f(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-EE_DEV uint64_t mul2f(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 EE_DEV float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
-}
-EE_DEV uint32_t max_nan(uint32_t a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(__uint_as_float(a)), "f"(b));
-  return __float_as_uint(r);
-}
-// 2^x of a pair on the FMA pipe, for x <= 2^8 (below -126: 2^-126, NaN stays):
-// x = n + f with n the nearest integer (the low bits of x + 1.5 * 2^23), 2^f by
-// a minimax polynomial fitted here -- degree 3 for bf16 (relative error 7.5e-5,
-// against 2^-9 of the weights' rounding), degree 4 for fp16 (2.6e-6, 2^-12).
-template <typename T>
-EE_DEV uint64_t exp2_pair(uint64_t x) {
-  uint32_t a, b;
-  unpack64(x, a, b);
-  x = pack64(max_nan(a, -126.f), max_nan(b, -126.f));
-  const uint64_t t = add2f(x, both(12582912.f));
-  const uint64_t f = add2f(x, mul2f(add2f(t, both(-12582912.f)), both(-1.f)));
-  uint64_t p;
-  if (sizeof(T) == 2 && Act<T>::kInt4Base == 128.f) {  // bf16
-    p = fma2f(f, both(0.05517134f), both(0.24261117f));
-    p = fma2f(f, p, both(0.69326103f));
-    p = fma2f(f, p, both(0.99992807f));
-  } else {
-    p = fma2f(f, both(0.00957005f), both(0.05591786f));
-    p = fma2f(f, p, both(0.24024746f));
-    p = fma2f(f, p, both(0.69312182f));
-    p = fma2f(f, p, both(0.99999926f));
-  }
-  unpack64(t, a, b);  // 2^n: n << 23 added to the bits of 1 (1.5 * 2^23 shifts out)
-  return mul2f(p, pack64(a * 8388608u + 0x3f800000u, b * 8388608u + 0x3f800000u));
 }
 
 template <typename T, int HD>
@@ -222,12 +185,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   constexpr int PANELS = HD / 64;
   // hd 64 leaves TMEM for P beside S, so the next scores are computed during the softmax
   constexpr bool SEP = HD == 64;
-#ifndef EE_PT_PARTS
-#define EE_PT_PARTS 2
-#endif
-  constexpr int PARTS = EE_PT_PARTS;  // pieces in which a block's weights are handed over
-  // pairs of every eight whose exponentials run on the FMA pipe (a bit each): 2 for hd 128, 3 for hd 64
-  constexpr uint32_t kPoly = HD == 64 ? EE_PT_POLY64 : EE_PT_POLY128;
+  // pieces in which a block's weights are handed over (1 at hd 64: 501 instead of 411 us for 8192 tokens)
+  constexpr int PARTS = 2;
   extern __shared__ __align__(1024) char smem_raw[];
   const uint32_t base0 = smem_u32(smem_raw);
   const uint32_t sb = (base0 + 1023u) & ~1023u;
@@ -522,8 +481,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           if (lane == 0) mbar_arrive(b_sf + 8 * t);
         }
         const int left = lim - j * kPtKeys;
-        const bool masked = __any_sync(0xffffffffu, left < kPtKeys);
-        if (masked) {
+        if (__any_sync(0xffffffffu, left < kPtKeys)) {
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -566,36 +524,24 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         const uint64_t sc2 = both(p.scale_log2), neg2 = both(neg);
         uint64_t sum[4] = {0, 0, 0, 0};
         // weights of the block, 64 keys at a time: the products with the first half start under the second
-        auto weights = [&](auto mixed) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 4; ++c) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              uint64_t y = fma2f(pack64(v[c][e], v[c][e + 1]), sc2, neg2);
-              if (decltype(mixed)::value && kPoly >> ((e >> 1) & 7) & 1) {
-                y = exp2_pair<T>(y);
-              } else {
-                uint32_t y0, y1;
-                unpack64(y, y0, y1);
-                y = pack64(__float_as_uint(ex2(__uint_as_float(y0))), __float_as_uint(ex2(__uint_as_float(y1))));
-              }
-              sum[c] = add2f(sum[c], y);
-              uint32_t y0, y1;
-              unpack64(y, y0, y1);
-              v[c >> 1][(c & 1) * 16 + e / 2] = Act<T>::pack2(__uint_as_float(y0), __uint_as_float(y1));
-            }
-            if (c & 1) tmem_st32(tp + 32 * (c >> 1), v[c >> 1]);
-            if (c == 3 || (PARTS == 2 && c == 1)) {
-              tmem_wait_st();
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(b_p + 16 * (PARTS - 1 ? c >> 1 : 0) + 8 * t);
-            }
+          for (int e = 0; e < 32; e += 2) {
+            uint32_t y0, y1;
+            unpack64(fma2f(pack64(v[c][e], v[c][e + 1]), sc2, neg2), y0, y1);
+            const float w0 = ex2(__uint_as_float(y0)), w1 = ex2(__uint_as_float(y1));
+            sum[c] = add2f(sum[c], pack64(__float_as_uint(w0), __float_as_uint(w1)));
+            v[c >> 1][(c & 1) * 16 + e / 2] = Act<T>::pack2(w0, w1);
           }
-        };
-        // exact zeros where keys are masked or nothing has been seen
-        if (masked || __any_sync(0xffffffffu, m == -INFINITY)) weights(std::false_type{});
-        else weights(std::true_type{});
+          if (c & 1) tmem_st32(tp + 32 * (c >> 1), v[c >> 1]);
+          if (c == 3 || (PARTS == 2 && c == 1)) {
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(b_p + 16 * (PARTS - 1 ? c >> 1 : 0) + 8 * t);
+          }
+        }
         {
           const uint64_t s2 = add2f(add2f(sum[0], sum[1]), add2f(sum[2], sum[3]));
           uint32_t s0, s1;
