@@ -140,7 +140,9 @@ def check(rc: int, what: str):
 
 
 def stream_ptr(device=None) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    if device is None or device.index is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)  # the same handle without a Stream object
 
 
 def act_code(dtype) -> int:
@@ -166,27 +168,35 @@ def require_cuda(*tensors):
                                f"(got a tensor on {t.device}); there is no CPU path")
 
 
+_HERE = contextlib.nullcontext()
+
+
 def on_device(device):
     """Context in which kernels launch on ``device``: nothing when it is the current one already."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def same_device(*tensors):
     """The one device of CUDA ``tensors`` (``None`` entries apart)."""
-    require_cuda(*tensors)
     dev = None
     for t in tensors:
         if t is not None:
-            dev = dev or t.device
-            if t.device != dev:
-                raise ValueError(f"tensors on different devices: {dev} and {t.device}")
+            if not t.is_cuda:
+                require_cuda(t)
+            d = t.device
+            if dev is None:
+                dev = d
+            elif d != dev:
+                raise ValueError(f"tensors on different devices: {dev} and {d}")
     return dev
 
 
 def no_grad_through(what: str, *tensors):
     """These kernels have no backward pass: an input that asks for one is refused."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() or detach its inputs")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() or detach its inputs")
 
 
 def ptr(t) -> int:

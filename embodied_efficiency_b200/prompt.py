@@ -21,27 +21,32 @@ from . import _lib
 
 
 def _heads(t, name):
-    """Checks of a [tokens, heads, head_dim] operand; a copy where a stride or the base is not on 16 bytes."""
+    """A [tokens, heads, head_dim] operand and its strides; a copy where a stride or the base is not on 16 bytes."""
     if t.dim() != 3:
         raise ValueError(f"{name} must be [tokens, heads, head_dim], got {tuple(t.shape)}")
-    if t.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"{name} must be bf16 or fp16, not {t.dtype}")
     s = t.stride()
     if s[2] != 1 or s[0] % 8 or s[1] % 8 or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
-    return t
+        s = t.stride()
+    return t, s
 
 
 def _out(out, like, name):
-    """An output to fill: ``out`` after checks, or a new contiguous tensor."""
+    """An output to fill and its strides: ``out`` after checks, or a new contiguous tensor."""
     if out is None:
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
-    s = out.stride()
+        out = torch.empty_like(like) if like.is_contiguous() else like.new_empty(like.shape)
+        return out, out.stride()
     if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
         raise ValueError(f"{name} must be {like.dtype} {tuple(like.shape)} on {like.device}")
-    if out.dim() != 3 or s[2] != 1 or s[0] % 8 or s[1] % 8 or out.data_ptr() % 16:
+    s = out.stride()
+    if s[2] != 1 or s[0] % 8 or s[1] % 8 or out.data_ptr() % 16:
         raise ValueError(f"{name} needs a contiguous last dimension, strides of 8 elements and a 16-byte boundary")
-    return out
+    return out, s
+
+
+def _act_dtype(t, name):
+    if t.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"{name} must be bf16 or fp16, not {t.dtype}")
 
 
 _TURNS: dict = {}
@@ -59,7 +64,10 @@ def _turns(device, half: int, base: float) -> torch.Tensor:
 
 
 @functools.lru_cache(maxsize=64)
-def _section_array(sections):
+def _sections(sections, half: int):
+    """The axes' pair counts as the ABI takes them, after checks."""
+    if not 1 <= len(sections) <= 4 or min(sections) < 0 or sum(sections) != half:
+        raise ValueError(f"sections {sections} must be one to four counts that sum to head_dim / 2 = {half}")
     return (ctypes.c_int32 * len(sections))(*sections)
 
 
@@ -71,47 +79,50 @@ def rotary_embed(q, k, positions, sections, base: float = 10000.0, interleaved: 
     ``positions`` is int32 or int64 [axes, T] ([T] for one axis); angles stay exact to the last bits of fp32 at any
     position. Returns (q, k) turned, as new tensors or in ``out`` = (q_out, k_out), which may be the inputs
     themselves. head_dim 32, 64, 128 or 256; bf16 / fp16."""
-    sections = tuple(int(s) for s in sections)
-    pos = positions.unsqueeze(0) if positions.dim() == 1 else positions
     one = q if q is not None else k
     if one is None:
         raise ValueError("rotary_embed needs q or k")
     t, hd = one.shape[0], one.shape[-1]
-    if not 1 <= len(sections) <= 4 or min(sections) < 0 or sum(sections) != hd // 2:
-        raise ValueError(f"sections {sections} must be one to four counts that sum to head_dim / 2 = {hd // 2}")
-    if pos.dim() != 2 or tuple(pos.shape) != (len(sections), t):
+    if type(sections) is not tuple:
+        sections = tuple(sections)
+    sec = _sections(sections, hd // 2)
+    pshape = positions.shape if positions.dim() != 1 else (1, positions.shape[0])
+    if len(pshape) != 2 or pshape[0] != len(sections) or pshape[1] != t:
         raise ValueError(f"positions have shape {tuple(positions.shape)}, expected {(len(sections), t)}")
-    if pos.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"positions must be int32 or int64, not {pos.dtype}")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"positions must be int32 or int64, not {positions.dtype}")
     if hd not in (32, 64, 128, 256):
         raise ValueError(f"head_dim must be 32, 64, 128 or 256, got {hd}")
-    if not base > 1.0 or math.isinf(base):
+    if not 1.0 < base < math.inf:
         raise ValueError(f"base must be finite and above 1, got {base}")
+    _act_dtype(one, "q and k")
     if q is not None and k is not None and (k.shape[0] != t or k.shape[-1] != hd or k.dtype != q.dtype):
         raise ValueError(f"q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} do not belong together")
-    dev = _lib.same_device(q, k, pos)
+    dev = _lib.same_device(q, k, positions)
     _lib.no_grad_through("rotary_embed", q, k)
+    qo, ko = out if out is not None else (None, None)
+    qs = ks = qp = kp = qop = kop = nq = nk = 0
+    none = (0, 0)
     with _lib.on_device(dev):
-        qo, ko = out if out is not None else (None, None)
-        args, res, keep = [], [], []
-        for x, o, name in ((q, qo, "q"), (k, ko, "k")):
-            if x is None:
-                args += [0, 0, 0, 0, 0, 0]
-                res.append(None)
-                continue
-            xs = _heads(x, name)
-            o = _out(o, x, f"out for {name}")
-            args += [xs.data_ptr(), xs.stride(0), xs.stride(1), o.data_ptr(), o.stride(0), o.stride(1)]
-            res.append(o)
-            keep.append(xs)
-        if pos.stride(1) != 1:
-            pos = pos.contiguous()
-        _lib.check(_lib.load().ee_rotary(*args, pos.data_ptr(), pos.stride(0), 32 if pos.dtype == torch.int32 else 64,
-                                         _turns(dev, hd // 2, float(base)).data_ptr(), t,
-                                         0 if q is None else q.shape[1], 0 if k is None else k.shape[1], hd,
-                                         _section_array(sections), len(sections), 1 if interleaved else 0,
-                                         _lib.act_code(one.dtype), _lib.stream_ptr(dev)), "ee_rotary")
-    return res[0], res[1]
+        if q is not None:
+            (q, qs), (qo, qos), nq = _heads(q, "q"), _out(qo, q, "out for q"), q.shape[1]
+            qp, qop = q.data_ptr(), qo.data_ptr()
+        else:
+            qo, qs, qos = None, none, none
+        if k is not None:
+            (k, ks), (ko, kos), nk = _heads(k, "k"), _out(ko, k, "out for k"), k.shape[1]
+            kp, kop = k.data_ptr(), ko.data_ptr()
+        else:
+            ko, ks, kos = None, none, none
+        if positions.stride(-1) != 1:
+            positions = positions.contiguous()
+        rc = _lib.load().ee_rotary(qp, qs[0], qs[1], qop, qos[0], qos[1], kp, ks[0], ks[1], kop, kos[0], kos[1],
+                                   positions.data_ptr(), positions.stride(0) if positions.dim() == 2 else t,
+                                   32 if positions.dtype == torch.int32 else 64, _turns(dev, hd // 2, base).data_ptr(),
+                                   t, nq, nk, hd, sec, len(sections), 1 if interleaved else 0,
+                                   _lib.act_code(one.dtype), _lib.stream_ptr(dev))
+    _lib.check(rc, "ee_rotary")
+    return qo, ko
 
 
 def _offsets(t, n, name):
@@ -134,8 +145,9 @@ def prompt_attention(q, k, v, cu_q, cu_k=None, k_lens=None, causal: bool = True,
         raise ValueError(f"q {q.dtype}, k {k.dtype} {tuple(k.shape)} and v {v.dtype} {tuple(v.shape)} do not match")
     if q.dim() != 3 or k.dim() != 3 or q.shape[2] != k.shape[2]:
         raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} must be [tokens, heads, head_dim]")
+    _act_dtype(q, "q, k and v")
     tq, hq, hd = q.shape
-    tk, hk = k.shape[0], k.shape[1]
+    tk, hk, _ = k.shape
     if hd not in (64, 128):
         raise ValueError(f"head_dim must be 64 or 128, got {hd}")
     if hk < 1 or hq < 1 or hq % hk:
@@ -153,15 +165,14 @@ def prompt_attention(q, k, v, cu_q, cu_k=None, k_lens=None, causal: bool = True,
     k_lens = None if k_lens is None else _offsets(k_lens, n, "k_lens")
     dev = _lib.same_device(q, k, v, cu_q, cu_k, k_lens)
     _lib.no_grad_through("prompt_attention", q, k, v)
+    lib = _lib.load()
     with _lib.on_device(dev):
-        qs, ks, vs = _heads(q, "q"), _heads(k, "k"), _heads(v, "v")
-        o = _out(out, q, "out")
-        lib = _lib.load()
+        (qc, qs), (k, ks), (v, vs), (out, os_) = _heads(q, "q"), _heads(k, "k"), _heads(v, "v"), _out(out, q, "out")
         nb = lib.ee_prompt_attention_workspace_bytes(tq, tk, n, hq, hk, hd)
         ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
-        _lib.check(lib.ee_prompt_attention(
-            qs.data_ptr(), qs.stride(0), qs.stride(1), ks.data_ptr(), ks.stride(0), ks.stride(1), vs.data_ptr(),
-            vs.stride(0), vs.stride(1), o.data_ptr(), o.stride(0), o.stride(1), cu_q.data_ptr(), _lib.ptr(cu_k),
-            _lib.ptr(k_lens), tq, tk, n, hq, hk, hd, 1 if causal else 0, scale, _lib.act_code(q.dtype), _lib.ptr(ws),
-            nb, _lib.stream_ptr(dev)), "ee_prompt_attention")
-    return o
+        rc = lib.ee_prompt_attention(
+            qc.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], out.data_ptr(),
+            os_[0], os_[1], cu_q.data_ptr(), _lib.ptr(cu_k), _lib.ptr(k_lens), tq, tk, n, hq, hk, hd,
+            1 if causal else 0, scale, _lib.act_code(q.dtype), _lib.ptr(ws), nb, _lib.stream_ptr(dev))
+    _lib.check(rc, "ee_prompt_attention")
+    return out

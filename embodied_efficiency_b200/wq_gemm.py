@@ -145,11 +145,12 @@ def wq_linear(x, weight, scales, bias, group_size, bits, zeros=None, gelu=False,
 # 8-bit integer linears: a scale for each token and each output channel
 # ---------------------------------------------------------------------------
 def _token_rows(x, k):
-    """x [..., k] as rows of the kernels: a 2-D view where its strides allow one, else a copy."""
-    xf = x.reshape(-1, k)
-    if xf.stride(-1) != 1 or xf.stride(0) % 8 or xf.stride(0) < k or xf.data_ptr() % 16:
-        xf = xf.clone(memory_format=torch.contiguous_format)
-    return xf
+    """x [..., k] as rows of the kernels and their stride: a 2-D view where its strides allow one, else a copy."""
+    xf = x if x.dim() == 2 else x.reshape(-1, k)
+    ld, one = xf.stride()
+    if one != 1 or ld % 8 or ld < k or x.data_ptr() % 16:
+        xf, ld = xf.clone(memory_format=torch.contiguous_format), k
+    return xf, ld
 
 
 def _check_int8_operands(weight, scales, bias, residual, k, dtype, out_shape):
@@ -201,12 +202,12 @@ def quantize_tokens(x):
     dev = _lib.same_device(x)
     _lib.no_grad_through("quantize_tokens", x)
     with _lib.on_device(dev):
-        xf = _token_rows(x, k)
+        xf, ld = _token_rows(x, k)
         q = torch.empty(x.shape, dtype=torch.int8, device=dev)
-        s = torch.empty(*x.shape[:-1], 1, dtype=torch.float32, device=dev)
-        _lib.check(_lib.load().ee_quantize_tokens(xf.data_ptr(), xf.stride(0), q.data_ptr(), s.data_ptr(),
-                                                  xf.shape[0], k, _lib.act_code(x.dtype), _lib.stream_ptr(dev)),
-                   "ee_quantize_tokens")
+        s = torch.empty((*x.shape[:-1], 1), dtype=torch.float32, device=dev)
+        rc = _lib.load().ee_quantize_tokens(xf.data_ptr(), ld, q.data_ptr(), s.data_ptr(), xf.shape[0], k,
+                                            _lib.act_code(x.dtype), _lib.stream_ptr(dev))
+    _lib.check(rc, "ee_quantize_tokens")
     return q, s
 
 
@@ -230,9 +231,10 @@ def int8_matmul(xq, x_scale, weight, scales, bias=None, dtype=torch.bfloat16, ge
         s, b, r, epi = _int8_epilogue(scales, bias, gelu, residual, dtype)
         xq, x_scale, weight = _aligned(xq), _aligned(x_scale), _aligned(weight)
         y = torch.empty(out_shape, dtype=dtype, device=dev)
-        _lib.check(_lib.load().ee_int8_gemm(xq.data_ptr(), x_scale.data_ptr(), weight.data_ptr(), s.data_ptr(),
-                                            _lib.ptr(b), _lib.ptr(r), y.data_ptr(), m, n, k, _lib.scale_code(s.dtype),
-                                            _lib.act_code(dtype), epi, _lib.stream_ptr(dev)), "ee_int8_gemm")
+        rc = _lib.load().ee_int8_gemm(xq.data_ptr(), x_scale.data_ptr(), weight.data_ptr(), s.data_ptr(), _lib.ptr(b),
+                                      _lib.ptr(r), y.data_ptr(), m, n, k, _lib.scale_code(s.dtype),
+                                      _lib.act_code(dtype), epi, _lib.stream_ptr(dev))
+    _lib.check(rc, "ee_int8_gemm")
     return y
 
 
@@ -241,21 +243,22 @@ def int8_linear(x, weight, scales, bias=None, gelu=False, residual=None):
     ``quantize_tokens``, then ``int8_matmul`` with ``weight`` int8 [N, K] and one scale per output channel, to
     ``x.dtype`` (``ee_int8_linear``, one call). No backward pass."""
     k = x.shape[-1]
-    out_shape = (*x.shape[:-1], weight.shape[0])
+    out_shape = (x.shape[0], weight.shape[0]) if x.dim() == 2 else (*x.shape[:-1], weight.shape[0])
     n = _check_int8_operands(weight, scales, bias, residual, k, x.dtype, out_shape)
     dev = _lib.same_device(x, weight, scales, bias, residual)
     _lib.no_grad_through("int8_linear", x, residual)
     with _lib.on_device(dev):
-        xf = _token_rows(x, k)
+        xf, ld = _token_rows(x, k)
         m = xf.shape[0]
         s, b, r, epi = _int8_epilogue(scales, bias, gelu, residual, x.dtype)
         weight = _aligned(weight)
-        y = torch.empty(out_shape, dtype=x.dtype, device=dev)
-        ws = torch.empty(m * k + 4 * m, dtype=torch.uint8, device=dev)
-        _lib.check(_lib.load().ee_int8_linear(xf.data_ptr(), xf.stride(0), weight.data_ptr(), s.data_ptr(),
-                                              _lib.ptr(b), _lib.ptr(r), y.data_ptr(), ws.data_ptr(), ws.numel(),
-                                              m, n, k, _lib.scale_code(s.dtype), _lib.act_code(x.dtype), epi,
-                                              _lib.stream_ptr(dev)), "ee_int8_linear")
+        y = x.new_empty(out_shape)
+        need = m * k + 4 * m  # ee_int8_linear_workspace_bytes: codes and scales
+        ws = weight.new_empty(need)
+        rc = _lib.load().ee_int8_linear(xf.data_ptr(), ld, weight.data_ptr(), s.data_ptr(), _lib.ptr(b), _lib.ptr(r),
+                                        y.data_ptr(), ws.data_ptr(), need, m, n, k, _lib.scale_code(s.dtype),
+                                        _lib.act_code(x.dtype), epi, _lib.stream_ptr(dev))
+    _lib.check(rc, "ee_int8_linear")
     return y
 
 
