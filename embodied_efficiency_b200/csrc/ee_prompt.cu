@@ -14,13 +14,13 @@ namespace ee {
 // A row is (token, head of the key head's group), so a key head's whole group
 // shares one read of its keys. A CTA takes 16 rows of one sequence and key
 // head and, where the units alone would not fill the GPU, one of `splits`
-// parts of their keys (prompt_combine_kernel joins the parts); each of its
-// warps has its own running maximum and sum over its 16 keys of every 64-key
-// stage, merged through shared memory at the end.
-// HBM-bound on the keys and values; the ring holds three or four stages, and
-// two or three CTAs share an SM.
-constexpr int kPrKeys = 64;   // keys per stage
-constexpr int kPrWarps = 4;
+// parts of their keys. Its four warps each stream 16 keys of every 64 through
+// a ring of their own (cp.async, no barrier between warps) with their own
+// running maximum and sum; they are merged through shared memory at the end,
+// and the parts through distributed shared memory when they are a cluster (up
+// to 8), else by prompt_combine_kernel. HBM-bound on the keys and values: two
+// or three CTAs share an SM, 128 KB of loads in flight.
+constexpr int kPrWarps = 4, kPrKeys = 64;   // keys per step of the CTA
 template <int HD> constexpr int pr_stages() { return HD == 128 ? 3 : 4; }
 template <int HD> constexpr int pr_smem() { return pr_stages<HD>() * 2 * kPrKeys * HD * 2; }
 
@@ -36,45 +36,49 @@ EE_DEV void pr_ldsm_t(uint32_t addr, uint32_t (&r)[4]) {
 template <typename T, int HD>
 __global__ void __launch_bounds__(32 * kPrWarps) prompt_rows_kernel(const __grid_constant__ PromptArgs a) {
   constexpr int NW = kPrWarps, NT = 32 * NW, NS = pr_stages<HD>();
-  constexpr int WK = kPrKeys / NW;       // keys of a stage per warp
   constexpr int RB = HD * 2;             // bytes per key row
   constexpr int CH = HD / 8;             // 16-byte chunks per key row
-  constexpr int TILE = kPrKeys * RB;
+  constexpr int TILE = 16 * RB;          // a warp's 16 keys
   extern __shared__ __align__(128) char smem[];
-  __shared__ int sh[NW + 2];
+  __shared__ PromptFind<NT> sh;
   pdl_entry();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
   const int kvh = blockIdx.y, part = blockIdx.x % a.splits;
   PromptSeq s;
-  if (!prompt_find(a, blockIdx.x / a.splits, a.group, 16, NT, sh, s)) return;
+  if (!prompt_find<NT>(a, blockIdx.x / a.splits, a.group, 16, &sh, s)) return;  // the same for a whole cluster
   const int rows = s.qlen * a.group, r0 = s.blk * 16;
-  // keys this CTA's rows see at most, and its part of them in whole stages
+  // keys this CTA's rows see at most, and its part of them in steps of 64
   const int last_tok = (min(r0 + 16, rows) - 1) / a.group;
   const int kend = a.causal ? max(min(s.klen, s.klen - s.qlen + last_tok + 1), 0) : s.klen;
   const int nst = (kend + kPrKeys - 1) / kPrKeys;
   const int st0 = (int)((long long)nst * part / a.splits), st1 = (int)((long long)nst * (part + 1) / a.splits);
-  const uint32_t sb = smem_u32(smem);
-  auto off = [](int row, int ch) { return row * RB + (((ch) ^ (row & 7)) << 4); };
+  const uint32_t ring = smem_u32(smem) + warp * NS * 2 * TILE;
+  auto off = [](int row, int ch) { return row * RB + ((ch ^ (row & 7)) << 4); };
+  // keys 64 st + 16 warp ..: K, then V; those past the last seen one are zero-filled
+  const char* kp = reinterpret_cast<const char*>(a.k) + ((long long)(s.k0 + 16 * warp) * a.k_tok + kvh * a.k_head) * 2;
+  const char* vp = reinterpret_cast<const char*>(a.v) + ((long long)(s.k0 + 16 * warp) * a.v_tok + kvh * a.v_head) * 2;
+  const int lrow = lane / CH, lch = lane % CH;  // this lane's row and chunk of every 32 / CH rows
   auto load = [&](int st, int buf) {
-    const int k0 = st * kPrKeys, valid = kend - k0;  // keys past the last seen one are zero-filled
-    const char* kb = reinterpret_cast<const char*>(a.k) + ((long long)(s.k0 + k0) * a.k_tok + kvh * a.k_head) * 2;
-    const char* vb = reinterpret_cast<const char*>(a.v) + ((long long)(s.k0 + k0) * a.v_tok + kvh * a.v_head) * 2;
-    const uint32_t d = sb + buf * 2 * TILE;
-#pragma unroll 4
-    for (int i = tid; i < kPrKeys * CH; i += NT) {
-      const int row = i / CH, ch = i % CH;
+    const long long k0 = (long long)st * kPrKeys;
+    const int valid = kend - (int)k0 - 16 * warp;
+    const uint32_t d = ring + buf * 2 * TILE;
+#pragma unroll
+    for (int i = 0; i < 16 * CH / 32; ++i) {
+      const int row = lrow + i * (32 / CH);
       const bool ok = row < valid;
-      cp_async16(d + off(row, ch), kb + (ok ? (long long)row * a.k_tok * 2 + ch * 16 : 0), ok);
-      cp_async16(d + TILE + off(row, ch), vb + (ok ? (long long)row * a.v_tok * 2 + ch * 16 : 0), ok);
+      cp_async16(d + off(row, lch), kp + (ok ? (k0 + row) * a.k_tok * 2 + lch * 16 : 0), ok);
+      cp_async16(d + TILE + off(row, lch), vp + (ok ? (k0 + row) * a.v_tok * 2 + lch * 16 : 0), ok);
     }
   };
+  // an address to hand to a load that reads nothing
+  if (s.k0 + 16 * warp >= a.tk) kp = reinterpret_cast<const char*>(a.k), vp = reinterpret_cast<const char*>(a.v);
 #pragma unroll
   for (int i = 0; i < NS - 1; ++i) {
     if (st0 + i < st1) load(st0 + i, i);
     cp_async_commit();
   }
-  // this warp's query fragments
+  // the query fragments
   const int ra = r0 + g, rb = ra + 8;
   uint32_t qf[HD / 16][4];
   {
@@ -101,22 +105,20 @@ __global__ void __launch_bounds__(32 * kPrWarps) prompt_rows_kernel(const __grid
     for (int c = 0; c < 4; ++c) o[i][c] = 0.f;
   float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
   const int mi = lane >> 3;
+  int buf = 0;
   for (int st = st0; st < st1; ++st) {
-    if (st + NS - 1 < st1) load(st + NS - 1, (st - st0 + NS - 1) % NS);
+    if (st + NS - 1 < st1) load(st + NS - 1, buf == 0 ? NS - 1 : buf - 1);
     cp_async_commit();
     cp_async_wait<NS - 1>();
-    __syncthreads();
-    const uint32_t kt = sb + ((st - st0) % NS) * 2 * TILE, vt = kt + TILE;
-#pragma unroll
-    for (int k1 = 0; k1 < WK; k1 += 16) {
-      const int kl = warp * WK + k1;            // first of 16 keys, in the stage
-      const int key = st * kPrKeys + kl;       // and in the sequence
-      if (key >= kend) break;
+    __syncwarp();
+    const uint32_t kt = ring + buf * 2 * TILE, vt = kt + TILE;
+    const int key = st * kPrKeys + 16 * warp;  // first of the warp's 16 keys
+    if (key < kend) {
       float p[2][4] = {};
 #pragma unroll
       for (int ks = 0; ks < HD / 16; ++ks) {
         uint32_t b[4];
-        pr_ldsm(kt + off(kl + (mi >> 1) * 8 + (lane & 7), 2 * ks + (mi & 1)), b);
+        pr_ldsm(kt + off((mi >> 1) * 8 + (lane & 7), 2 * ks + (mi & 1)), b);
         mma16816<T>(p[0], qf[ks][0], qf[ks][1], qf[ks][2], qf[ks][3], b[0], b[1]);
         mma16816<T>(p[1], qf[ks][0], qf[ks][1], qf[ks][2], qf[ks][3], b[2], b[3]);
       }
@@ -140,11 +142,20 @@ __global__ void __launch_bounds__(32 * kPrWarps) prompt_rows_kernel(const __grid
       const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
       // nothing seen yet: any finite reference will do, exp2(-inf) = 0
       const float u0 = n0 == -INFINITY ? 0.f : n0, u1 = n1 == -INFINITY ? 0.f : n1;
-      const float c0 = exp2f(m0 - u0), c1 = exp2f(m1 - u1);
-      m0 = n0;
-      m1 = n1;
-      l0 *= c0;
-      l1 *= c1;
+      if (__any_sync(0xffffffffu, n0 != m0 || n1 != m1)) {
+        const float c0 = exp2f(m0 - u0), c1 = exp2f(m1 - u1);
+        m0 = n0;
+        m1 = n1;
+        l0 *= c0;
+        l1 *= c1;
+#pragma unroll
+        for (int i = 0; i < HD / 8; ++i) {
+          o[i][0] *= c0;
+          o[i][1] *= c0;
+          o[i][2] *= c1;
+          o[i][3] *= c1;
+        }
+      }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
 #pragma unroll
@@ -160,19 +171,13 @@ __global__ void __launch_bounds__(32 * kPrWarps) prompt_rows_kernel(const __grid
 #pragma unroll
       for (int d = 0; d < HD / 16; ++d) {
         uint32_t b[4];
-        pr_ldsm_t(vt + off(kl + (mi & 1) * 8 + (lane & 7), 2 * d + (mi >> 1)), b);
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          o[2 * d + c][0] *= c0;
-          o[2 * d + c][1] *= c0;
-          o[2 * d + c][2] *= c1;
-          o[2 * d + c][3] *= c1;
-        }
+        pr_ldsm_t(vt + off((mi & 1) * 8 + (lane & 7), 2 * d + (mi >> 1)), b);
         mma16816<T>(o[2 * d], pa0, pa1, pa2, pa3, b[0], b[1]);
         mma16816<T>(o[2 * d + 1], pa0, pa1, pa2, pa3, b[2], b[3]);
       }
     }
-    __syncthreads();
+    __syncwarp();  // every lane has read the stage before it is loaded again
+    if (++buf == NS) buf = 0;
   }
   cp_async_wait<0>();
 #pragma unroll
@@ -180,9 +185,9 @@ __global__ void __launch_bounds__(32 * kPrWarps) prompt_rows_kernel(const __grid
     l0 += __shfl_xor_sync(0xffffffffu, l0, d);
     l1 += __shfl_xor_sync(0xffffffffu, l1, d);
   }
-  // merge the warps: [warp][16 rows][HD + 4] fp32 over the stages
+  // merge the warps: [warp][16 rows][HD + 4] fp32 over the rings; this CTA's sums behind them
   constexpr int ML = HD + 4;
-  static_assert(NW * 16 * ML * 4 <= NS * 2 * kPrKeys * RB, "the merge fits the stages");
+  static_assert((NW + 1) * 16 * ML * 4 <= pr_smem<HD>(), "the merge fits the rings");
   float* mg = reinterpret_cast<float*>(smem) + warp * 16 * ML;
   __syncthreads();
 #pragma unroll
@@ -191,43 +196,72 @@ __global__ void __launch_bounds__(32 * kPrWarps) prompt_rows_kernel(const __grid
     *reinterpret_cast<float2*>(mg + (g + 8) * ML + 8 * i + 2 * t) = make_float2(o[i][2], o[i][3]);
   }
   if (t == 0) {
-    mg[g * ML + HD] = m0;
-    mg[g * ML + HD + 1] = l0;
-    mg[(g + 8) * ML + HD] = m1;
-    mg[(g + 8) * ML + HD + 1] = l1;
+    *reinterpret_cast<float2*>(mg + g * ML + HD) = make_float2(m0, l0);
+    *reinterpret_cast<float2*>(mg + (g + 8) * ML + HD) = make_float2(m1, l1);
   }
   __syncthreads();
-  for (int i = tid; i < 16 * (HD / 4); i += NT) {  // 4 values of a row over the warps
-    const int r = i / (HD / 4), c = (i % (HD / 4)) * 4;
-    if (r0 + r >= rows) continue;
-    const float* base = reinterpret_cast<const float*>(smem) + r * ML;
-    float m = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) m = fmaxf(m, base[w * 16 * ML + HD]);
+  // n partial sums of row r's values c .. c + 3, `at(i)` giving (maximum, weight) and the values
+  auto merge = [&](int n, auto stat, auto vals, float& m, float& l) {
+    m = -INFINITY;
+    for (int w = 0; w < n; ++w) m = fmaxf(m, stat(w).x);
     const float u = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
+    l = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const float* p = base + w * 16 * ML;
-      const float f = exp2f(p[HD] - u);
-      const float4 v = *reinterpret_cast<const float4*>(p + c);
-      l += f * p[HD + 1];
+    for (int w = 0; w < n; ++w) {
+      const float2 st = stat(w);
+      const float f = exp2f(st.x - u);
+      const float4 v = vals(w);
+      l += f * st.y;
       acc.x += f * v.x;
       acc.y += f * v.y;
       acc.z += f * v.z;
       acc.w += f * v.w;
     }
+    return acc;
+  };
+  auto write = [&](int r, int c, float4 acc, float l) {
     const int tok = s.q0 + (r0 + r) / a.group, h = kvh * a.group + (r0 + r) % a.group;
-    if (a.splits > 1) {  // this part's sums, relative to its maximum
-      const long long at = ((long long)part * a.tq + tok) * a.n_q + h;
-      if (c == 0) *reinterpret_cast<float2*>(a.stat + 2 * at) = make_float2(m, l);
-      if (l != 0.f) *reinterpret_cast<float4*>(a.part + at * HD + c) = acc;
-      continue;
-    }
     const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees no key is zero
     *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + (long long)tok * a.o_tok + h * a.o_head + c) =
         make_uint2(Act<T>::pack2(acc.x * inv, acc.y * inv), Act<T>::pack2(acc.z * inv, acc.w * inv));
+  };
+  const int live = min(16, rows - r0) * (HD / 4);
+  float* own = reinterpret_cast<float*>(smem) + NW * 16 * ML;
+  for (int i = tid; i < live; i += NT) {  // 4 values of a row over the warps
+    const int r = i / (HD / 4), c = (i % (HD / 4)) * 4;
+    const float* base = reinterpret_cast<const float*>(smem) + r * ML;
+    float m, l;
+    const float4 acc = merge(
+        NW, [&](int w) { return *reinterpret_cast<const float2*>(base + w * 16 * ML + HD); },
+        [&](int w) { return *reinterpret_cast<const float4*>(base + w * 16 * ML + c); }, m, l);
+    if (a.splits == 1) {
+      write(r, c, acc, l);
+    } else if (a.clustered) {
+      *reinterpret_cast<float4*>(own + r * ML + c) = acc;
+      if (c == 0) *reinterpret_cast<float2*>(own + r * ML + HD) = make_float2(m, l);
+    } else {  // this part's sums, relative to its maximum
+      const int tok = s.q0 + (r0 + r) / a.group, h = kvh * a.group + (r0 + r) % a.group;
+      const long long at = ((long long)part * a.tq + tok) * a.n_q + h;
+      if (c == 0) *reinterpret_cast<float2*>(a.stat + 2 * at) = make_float2(m, l);
+      if (l != 0.f) *reinterpret_cast<float4*>(a.part + at * HD + c) = acc;
+    }
+  }
+  if (a.splits > 1 && a.clustered) {
+    cluster_sync();
+    const uint32_t base = smem_u32(own);
+    for (int i = tid + part * NT; i < live; i += NT * a.splits) {
+      const int r = i / (HD / 4), c = (i % (HD / 4)) * 4;
+      float m, l;
+      const float4 acc = merge(
+          a.splits,
+          [&](int w) {
+            const uint32_t at = mapa(base + (r * ML + HD) * 4, w);
+            return make_float2(ld_dsmem_f32(at), ld_dsmem_f32(at + 4));
+          },
+          [&](int w) { return ld_dsmem_f4(mapa(base + (r * ML + c) * 4, w)); }, m, l);
+      write(r, c, acc, l);
+    }
+    cluster_sync();  // the sums stay until the whole cluster has read them
   }
 }
 
@@ -313,10 +347,16 @@ __global__ void __launch_bounds__(kPrCombine) prompt_combine_kernel(const __grid
 //           measured within 10 % or slower: 8 x 4096 keys, 32 / 8 heads of 128:
 //           53 / 47 / 49 us for 2 / 4 / 8). Tensor-core kernel: where the items
 //           would leave SMs idle, parts of 512 keys or more.
-constexpr long long kPrRows = 16, kPrCtasPerSm = 4, kPrMinKeys = 128, kPtMinKeys = 512;
-struct PromptPlan { bool tc; int splits; };
+#ifndef EE_PR_PER_SM
+#define EE_PR_PER_SM 4
+#endif
+#ifndef EE_PR_CLUSTER
+#define EE_PR_CLUSTER 8
+#endif
+constexpr long long kPrRows = 16, kPrCtasPerSm = EE_PR_PER_SM, kPrMinKeys = 128, kPtMinKeys = 512;
+struct PromptPlan { bool tc; int splits; bool clustered; };
 static PromptPlan prompt_plan(long long tq, long long tk, int n_seq, int n_q, int n_kv) {
-  PromptPlan pl{false, 1};
+  PromptPlan pl{false, 1, false};
   if (n_seq < 1) return pl;
   const int group = n_q / n_kv;
   const long long rows = tq * group;
@@ -328,15 +368,16 @@ static PromptPlan prompt_plan(long long tq, long long tk, int n_seq, int n_q, in
   const long long most = pl.tc ? tk / n_seq / kPtMinKeys : (tk / n_seq + kPrMinKeys - 1) / kPrMinKeys;
   const long long s = want < most ? want : most;
   pl.splits = s < 1 ? 1 : (int)(s < kPrMaxSplits ? s : kPrMaxSplits);
+  pl.clustered = !pl.tc && pl.splits > 1 && pl.splits <= EE_PR_CLUSTER;
   return pl;
 }
 static size_t prompt_ws_bytes(const PromptPlan& pl, long long tq, int n_q, int hd) {
-  return pl.splits > 1 ? (size_t)pl.splits * tq * n_q * (hd + 2) * 4 : 0;
+  return pl.splits > 1 && !pl.clustered ? (size_t)pl.splits * tq * n_q * (hd + 2) * 4 : 0;
 }
 
 template <typename T, int HD>
 static int launch_combine(const PromptArgs& a, cudaStream_t s) {
-  if (a.splits == 1) return EE_OK;
+  if (a.splits == 1 || a.clustered) return EE_OK;
   return launch_pdl(prompt_combine_kernel<T, HD>, dim3((unsigned)a.tq, a.n_q), dim3(kPrCombine), 0, s, a) == cudaSuccess
              ? EE_OK
              : EE_ERR_LAUNCH;
@@ -350,9 +391,23 @@ static int launch_rows(const PromptArgs& a, cudaStream_t s) {
   // at most one partial block per sequence beyond the rows' whole blocks
   const long long units = (long long)a.tq * a.group / 16 + a.n_seq;
   if (units * a.splits > 0x7fffffff) return EE_ERR_SHAPE;
-  if (launch_pdl(fn, dim3((unsigned)(units * a.splits), a.n_kv), dim3(32 * kPrWarps), pr_smem<HD>(), s, a) !=
-      cudaSuccess)
-    return EE_ERR_LAUNCH;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(units * a.splits), a.n_kv);
+  cfg.blockDim = dim3(32 * kPrWarps);
+  cfg.dynamicSmemBytes = pr_smem<HD>();
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  unsigned int n = 0;
+  add_pdl_attr(attr, n);
+  if (a.clustered) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = a.splits;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  if (cudaLaunchKernelEx(&cfg, fn, a) != cudaSuccess) return EE_ERR_LAUNCH;
   return launch_combine<T, HD>(a, s);
 }
 
@@ -450,6 +505,7 @@ int ee_prompt_attention(const void* q, int64_t q_tok, int64_t q_head, const void
   a.causal = causal != 0;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.splits = pl.splits;
+  a.clustered = pl.clustered;
   a.part = reinterpret_cast<float*>(workspace);
   a.stat = a.part + (size_t)pl.splits * tq * n_q * head_dim;
   cudaStream_t s = (cudaStream_t)stream;

@@ -21,9 +21,10 @@ struct PromptArgs {
   long long q_tok, q_head, k_tok, k_head, v_tok, v_head, o_tok, o_head;  // strides, elements
   int tq, tk, n_seq, n_q, n_kv, group, causal;
   float scale_log2;  // scale * log2(e)
-  float* part;       // [splits][tq][n_q][hd] and [splits][tq][n_q][2]: partial results, when splits > 1
+  int splits;        // parts of the keys
+  int clustered;     // the parts are a cluster's CTAs, joined there; else through part and stat
+  float* part;       // [splits][tq][n_q][hd] sums of a part and [splits][tq][n_q][2] their maximum and weight
   float* stat;
-  int splits;
 };
 
 struct PromptSeq {
@@ -44,41 +45,46 @@ EE_DEV PromptSeq prompt_seq(const PromptArgs& a, int b) {
 
 // The sequence and block of unit `u`, the sequences' query rows (times `mul`)
 // being cut into blocks of `rows`; false when there is no such unit. All
-// `threads` threads of the CTA call it; `sh` has threads / 32 + 2 words.
-EE_DEV bool prompt_find(const PromptArgs& a, int u, int mul, int rows, int threads, int* sh, PromptSeq& out) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = threads >> 5;
+// THREADS threads of the CTA call it, each with a sequence of its own whose
+// whole record it reads at once, so a call of up to THREADS sequences waits
+// for global memory once.
+template <int THREADS>
+struct PromptFind {
+  int sums[THREADS / 32], hit;
+  PromptSeq seq;
+};
+template <int THREADS>
+EE_DEV bool prompt_find(const PromptArgs& a, int u, int mul, int rows, PromptFind<THREADS>* sh, PromptSeq& out) {
+  constexpr int NW = THREADS / 32;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int before = 0;
-  for (int b0 = 0; b0 < a.n_seq; b0 += threads) {
-    const int b = b0 + tid;
-    int nb = 0;
-    if (b < a.n_seq) {
-      const int q0 = min(max(__ldg(a.cu_q + b), 0), a.tq);
-      const int ql = min(max(__ldg(a.cu_q + b + 1), q0), a.tq) - q0;
-      nb = (int)(((long long)ql * mul + rows - 1) / rows);
-    }
+  for (int b0 = 0; b0 < a.n_seq; b0 += THREADS) {
+    PromptSeq s{};
+    if (b0 + tid < a.n_seq) s = prompt_seq(a, b0 + tid);
+    const int nb = (int)(((long long)s.qlen * mul + rows - 1) / rows);
     int inc = nb;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int t = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += t;
     }
-    if (tid == 0) sh[nw] = -1;
-    if (lane == 31) sh[warp] = inc;
+    if (tid == 0) sh->hit = 0;
+    if (lane == 31) sh->sums[warp] = inc;
     __syncthreads();
     int base = before, total = before;
-    for (int w = 0; w < nw; ++w) {
-      if (w < warp) base += sh[w];
-      total += sh[w];
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      if (w < warp) base += sh->sums[w];
+      total += sh->sums[w];
     }
-    if (nb > 0 && u >= base + inc - nb && u < base + inc) {
-      sh[nw] = b;
-      sh[nw + 1] = u - (base + inc - nb);
+    if (u >= base + inc - nb && u < base + inc) {
+      s.blk = u - (base + inc - nb);
+      sh->seq = s;
+      sh->hit = 1;
     }
     __syncthreads();
-    const int found = sh[nw];
-    if (found >= 0) {
-      out = prompt_seq(a, found);
-      out.blk = sh[nw + 1];
+    if (sh->hit) {
+      out = sh->seq;
       return true;
     }
     before = total;
