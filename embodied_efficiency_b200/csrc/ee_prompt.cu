@@ -12,17 +12,75 @@ namespace ee {
 // few query rows per key head
 // ---------------------------------------------------------------------------
 // A row is (token, head of the key head's group), so a key head's whole group
-// shares one read of its keys. A CTA takes 16 rows of one sequence and key
-// head and, where the units alone would not fill the GPU, one of `splits`
-// parts of their keys. Its four warps each stream 16 keys of every 64 through
-// a ring of their own (cp.async, no barrier between warps) with their own
-// running maximum and sum; they are merged through shared memory at the end,
-// and the parts through distributed shared memory when they are a cluster (up
-// to 8), else by prompt_combine_kernel. HBM-bound on the keys and values: two
-// or three CTAs share an SM, 128 KB of loads in flight.
-constexpr int kPrWarps = 4, kPrKeys = 64;   // keys per step of the CTA
-template <int HD> constexpr int pr_stages() { return HD == 128 ? 3 : 4; }
-template <int HD> constexpr int pr_smem() { return pr_stages<HD>() * 2 * kPrKeys * HD * 2; }
+// shares one read of its keys; an item is 16 rows of one sequence and key head
+// against the sequence's keys, cut into steps of 16 keys. All items' steps
+// form one list, and every warp of the grid takes an equal, contiguous share
+// of it whatever the sequences' lengths: each warp is on its own, streaming
+// its steps' keys and values through a ring (cp.async, no barrier between
+// warps, the next item's loads under the current one's last steps) with a
+// running maximum and sum. An item that lies in one share is written at once;
+// of an item cut by a border each warp leaves its sums in the workspace, at
+// most one at either end of its share, and prompt_join_kernel adds them up.
+// HBM-bound on the keys and values, with 128 KB of loads in flight per
+// SM. (One CTA per item and part of its keys, joined in a cluster or by a
+// second launch, left SMs idle for 27 % of the time on 64 sequences of 1 to
+// 1632 keys and waited for each CTA's first loads again: 36 us.)
+constexpr int kPrStep = 16, kPrMinSteps = 8;   // keys of a step; steps that are worth a warp
+template <int HD> constexpr int pr_warps() { return HD == 128 ? 8 : 16; }
+constexpr int kPrStages = 3;
+template <int HD> constexpr int pr_stage() { return 2 * kPrStep * HD * 2; }  // K and V of a step
+template <int HD> constexpr int pr_smem() { return pr_warps<HD>() * kPrStages * pr_stage<HD>(); }
+
+// steps of sequence b's items (all its row blocks and key heads), and of one item
+EE_DEV long long pr_steps(const PromptArgs& a, const PromptSeq& s, int& per_item) {
+  per_item = (s.klen + kPrStep - 1) / kPrStep;
+  return (long long)((s.qlen * a.group + 15) / 16) * a.n_kv * per_item;
+}
+
+// The list of steps: its length, and for every thread the steps before its
+// share of the sequences (`per` each, consecutive). All threads of the CTA.
+template <int THREADS>
+struct PrList {
+  long long before[THREADS];
+  long long warp_sum[THREADS / 32];
+};
+template <int THREADS, typename Visit>
+EE_DEV long long pr_list(const PromptArgs& a, PrList<THREADS>* sh, int per, Visit visit) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  long long mine = 0;
+  for (int b = tid * per; b < min((tid + 1) * per, a.n_seq); ++b) {
+    int n;
+    const PromptSeq s = prompt_seq(a, b);
+    visit(s, mine);  // the sequence and the steps of the thread's own before it
+    mine += pr_steps(a, s, n);
+  }
+  long long inc = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long t = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += t;
+  }
+  if (lane == 31) sh->warp_sum[warp] = inc;
+  __syncthreads();
+  long long base = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) base += sh->warp_sum[w];
+    total += sh->warp_sum[w];
+  }
+  sh->before[tid] = base + inc - mine;
+  __syncthreads();
+  return total;
+}
+// Steps in a warp's share of a list of `total`, for `most` warps: warp w takes
+// steps w * share .., so step x belongs to warp x / share.
+EE_DEV long long pr_div(long long a, long long b) {  // of values >= 0, mostly below 2^32
+  return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
+}
+EE_DEV long long pr_share(long long total, int most) {
+  const long long q = pr_div(total + most - 1, most);
+  return q < kPrMinSteps ? kPrMinSteps : q;
+}
 
 EE_DEV void pr_ldsm(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -33,352 +91,467 @@ EE_DEV void pr_ldsm_t(uint32_t addr, uint32_t (&r)[4]) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
 
+// A place in the list: a step of an item of a sequence.
+struct PrAt {
+  int b, step, per_item, item, items;  // sequence; step of the item; steps per item; item of the sequence (row block
+  PromptSeq s;                         // x key heads + key head) and their number
+  EE_DEV void enter(const PromptArgs& a, int seq) {  // sequence `seq` or the next one that has steps
+    for (b = seq; b < a.n_seq; ++b) {
+      s = prompt_seq(a, b);
+      const long long n = pr_steps(a, s, per_item);
+      if (n > 0) {
+        items = (s.qlen * a.group + 15) / 16 * a.n_kv;
+        break;
+      }
+    }
+    item = step = 0;
+  }
+  EE_DEV void next(const PromptArgs& a) {
+    if (++step < per_item) return;
+    step = 0;
+    if (++item == items) enter(a, b + 1);
+  }
+};
+
 template <typename T, int HD>
-__global__ void __launch_bounds__(32 * kPrWarps) prompt_rows_kernel(const __grid_constant__ PromptArgs a) {
-  constexpr int NW = kPrWarps, NT = 32 * NW, NS = pr_stages<HD>();
+__global__ void __launch_bounds__(32 * pr_warps<HD>(), 1) prompt_rows_kernel(const __grid_constant__ PromptArgs a) {
+  constexpr int NW = pr_warps<HD>(), NT = 32 * NW, NS = kPrStages;
   constexpr int RB = HD * 2;             // bytes per key row
   constexpr int CH = HD / 8;             // 16-byte chunks per key row
-  constexpr int TILE = 16 * RB;          // a warp's 16 keys
+  constexpr int TILE = kPrStep * RB;
   extern __shared__ __align__(128) char smem[];
-  __shared__ PromptFind<NT> sh;
+  __shared__ PrList<NT> sh;
   pdl_entry();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int g = lane >> 2, t = lane & 3;
-  const int kvh = blockIdx.y, part = blockIdx.x % a.splits;
-  PromptSeq s;
-  if (!prompt_find<NT>(a, blockIdx.x / a.splits, a.group, 16, &sh, s)) return;  // the same for a whole cluster
-  const int rows = s.qlen * a.group, r0 = s.blk * 16;
-  // keys this CTA's rows see at most, and its part of them in steps of 64
-  const int last_tok = (min(r0 + 16, rows) - 1) / a.group;
-  const int kend = a.causal ? max(min(s.klen, s.klen - s.qlen + last_tok + 1), 0) : s.klen;
-  const int nst = (kend + kPrKeys - 1) / kPrKeys;
-  const int st0 = (int)((long long)nst * part / a.splits), st1 = (int)((long long)nst * (part + 1) / a.splits);
+  const int g = lane >> 2, t = lane & 3, mi = lane >> 3;
+  const int per = (a.n_seq + NT - 1) / NT;
+  const long long total = pr_list<NT>(a, &sh, per, [](const PromptSeq&, long long) {});
+  const long long share = pr_share(total, (int)gridDim.x * NW);
+  const long long me = (long long)warp * gridDim.x + blockIdx.x;  // neighbours in the list on different SMs
+  const long long first = me * share;
+  if (first >= total) return;
+  int left = (int)(total - first < share ? total - first : share);  // steps to go
+  // where the share starts: the last thread whose sequences begin at or before it, then along its sequences
+  PrAt ld{};
+  {
+    int lo = 0;
+#pragma unroll
+    for (int o = NT / 2; o > 0; o >>= 1)
+      if (sh.before[lo + o] <= first) lo += o;
+    long long at = first - sh.before[lo];
+    ld.enter(a, lo * per);
+    while (ld.b < a.n_seq) {
+      const long long n = (long long)ld.items * ld.per_item;
+      if (at < n) break;
+      at -= n;
+      ld.enter(a, ld.b + 1);
+    }
+    if (ld.b >= a.n_seq) return;  // the lengths have changed meanwhile
+    ld.item = (int)pr_div(at, ld.per_item);
+    ld.step = (int)(at - (long long)ld.item * ld.per_item);
+  }
+  PrAt at = ld;
   const uint32_t ring = smem_u32(smem) + warp * NS * 2 * TILE;
   auto off = [](int row, int ch) { return row * RB + ((ch ^ (row & 7)) << 4); };
-  // keys 64 st + 16 warp ..: K, then V; those past the last seen one are zero-filled
-  const char* kp = reinterpret_cast<const char*>(a.k) + ((long long)(s.k0 + 16 * warp) * a.k_tok + kvh * a.k_head) * 2;
-  const char* vp = reinterpret_cast<const char*>(a.v) + ((long long)(s.k0 + 16 * warp) * a.v_tok + kvh * a.v_head) * 2;
   const int lrow = lane / CH, lch = lane % CH;  // this lane's row and chunk of every 32 / CH rows
-  auto load = [&](int st, int buf) {
-    const long long k0 = (long long)st * kPrKeys;
-    const int valid = kend - (int)k0 - 16 * warp;
+  // the keys and values of step `ld`, those past the sequence's end zero-filled; then on to the next step
+  auto load = [&](int buf) {
+    const int kvh = ld.item % a.n_kv, valid = ld.s.klen - ld.step * kPrStep;
+    const long long k0 = ld.s.k0 + (long long)ld.step * kPrStep;
+    const char* kb = reinterpret_cast<const char*>(a.k) + (k0 * a.k_tok + kvh * a.k_head) * 2 + lch * 16;
+    const char* vb = reinterpret_cast<const char*>(a.v) + (k0 * a.v_tok + kvh * a.v_head) * 2 + lch * 16;
     const uint32_t d = ring + buf * 2 * TILE;
 #pragma unroll
-    for (int i = 0; i < 16 * CH / 32; ++i) {
+    for (int i = 0; i < kPrStep * CH / 32; ++i) {
       const int row = lrow + i * (32 / CH);
-      const bool ok = row < valid;
-      cp_async16(d + off(row, lch), kp + (ok ? (k0 + row) * a.k_tok * 2 + lch * 16 : 0), ok);
-      cp_async16(d + TILE + off(row, lch), vp + (ok ? (k0 + row) * a.v_tok * 2 + lch * 16 : 0), ok);
+      const bool ok = row < valid;  // row 0 always is: the address of the others
+      cp_async16(d + off(row, lch), kb + (ok ? row * a.k_tok * 2 : 0), ok);
+      cp_async16(d + TILE + off(row, lch), vb + (ok ? row * a.v_tok * 2 : 0), ok);
     }
+    ld.next(a);
   };
-  // an address to hand to a load that reads nothing
-  if (s.k0 + 16 * warp >= a.tk) kp = reinterpret_cast<const char*>(a.k), vp = reinterpret_cast<const char*>(a.v);
+  int ahead = 0;  // steps loaded beyond the current one
 #pragma unroll
   for (int i = 0; i < NS - 1; ++i) {
-    if (st0 + i < st1) load(st0 + i, i);
+    if (i < left && ld.b < a.n_seq) {
+      load(i);
+      ++ahead;
+    }
     cp_async_commit();
   }
-  // the query fragments
-  const int ra = r0 + g, rb = ra + 8;
   uint32_t qf[HD / 16][4];
-  {
-    auto qrow = [&](int r) {
-      const int tok = r / a.group, h = kvh * a.group + r % a.group;
-      return reinterpret_cast<const char*>(a.q) + ((long long)(s.q0 + tok) * a.q_tok + h * a.q_head) * 2;
-    };
-    const char *pa = qrow(min(ra, rows - 1)), *pb = qrow(min(rb, rows - 1));
-#pragma unroll
-    for (int ks = 0; ks < HD / 16; ++ks) {
-      qf[ks][0] = *reinterpret_cast<const uint32_t*>(pa + ks * 32 + t * 4);
-      qf[ks][1] = *reinterpret_cast<const uint32_t*>(pb + ks * 32 + t * 4);
-      qf[ks][2] = *reinterpret_cast<const uint32_t*>(pa + ks * 32 + 16 + t * 4);
-      qf[ks][3] = *reinterpret_cast<const uint32_t*>(pb + ks * 32 + 16 + t * 4);
-    }
-  }
-  // keys below lim are seen by rows ra and rb
-  const int lim0 = a.causal ? min(s.klen, s.klen - s.qlen + ra / a.group + 1) : s.klen;
-  const int lim1 = a.causal ? min(s.klen, s.klen - s.qlen + rb / a.group + 1) : s.klen;
   float o[HD / 8][4];
-#pragma unroll
-  for (int i = 0; i < HD / 8; ++i)
-#pragma unroll
-    for (int c = 0; c < 4; ++c) o[i][c] = 0.f;
-  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-  const int mi = lane >> 3;
+  float m0 = 0.f, m1 = 0.f, l0 = 0.f, l1 = 0.f;
+  int rows = 0, r0 = 0, kvh = 0, lim0 = 0, lim1 = 0;
+  bool fresh = true;      // the item's first step of this share
+  int from = 0;           // that step
+  bool head = true;       // no item of the share has been finished yet
   int buf = 0;
-  for (int st = st0; st < st1; ++st) {
-    if (st + NS - 1 < st1) load(st + NS - 1, buf == 0 ? NS - 1 : buf - 1);
+  for (; left > 0 && ahead > 0; --left, --ahead) {
+    if (fresh) {
+      fresh = false;
+      from = at.step;
+      rows = at.s.qlen * a.group;
+      r0 = at.item / a.n_kv * 16;
+      kvh = at.item % a.n_kv;
+      const int ra = min(r0 + g, rows - 1), rb = min(r0 + g + 8, rows - 1);
+      auto qrow = [&](int r) {
+        const int tok = r / a.group, h = kvh * a.group + r % a.group;
+        return reinterpret_cast<const char*>(a.q) + ((long long)(at.s.q0 + tok) * a.q_tok + h * a.q_head) * 2;
+      };
+      const char *pa = qrow(ra), *pb = qrow(rb);
+#pragma unroll
+      for (int ks = 0; ks < HD / 16; ++ks) {
+        qf[ks][0] = *reinterpret_cast<const uint32_t*>(pa + ks * 32 + t * 4);
+        qf[ks][1] = *reinterpret_cast<const uint32_t*>(pb + ks * 32 + t * 4);
+        qf[ks][2] = *reinterpret_cast<const uint32_t*>(pa + ks * 32 + 16 + t * 4);
+        qf[ks][3] = *reinterpret_cast<const uint32_t*>(pb + ks * 32 + 16 + t * 4);
+      }
+      // keys below lim are seen by rows ra and rb
+      lim0 = a.causal ? min(at.s.klen, at.s.klen - at.s.qlen + ra / a.group + 1) : at.s.klen;
+      lim1 = a.causal ? min(at.s.klen, at.s.klen - at.s.qlen + rb / a.group + 1) : at.s.klen;
+#pragma unroll
+      for (int i = 0; i < HD / 8; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[i][c] = 0.f;
+      m0 = m1 = -INFINITY;
+      l0 = l1 = 0.f;
+    }
+    if (left > NS - 1 && ld.b < a.n_seq) {
+      load(buf == 0 ? NS - 1 : buf - 1);
+      ++ahead;
+    }
     cp_async_commit();
     cp_async_wait<NS - 1>();
     __syncwarp();
     const uint32_t kt = ring + buf * 2 * TILE, vt = kt + TILE;
-    const int key = st * kPrKeys + 16 * warp;  // first of the warp's 16 keys
-    if (key < kend) {
-      float p[2][4] = {};
+    const int key = at.step * kPrStep;
+    float p[2][4] = {};
 #pragma unroll
-      for (int ks = 0; ks < HD / 16; ++ks) {
-        uint32_t b[4];
-        pr_ldsm(kt + off((mi >> 1) * 8 + (lane & 7), 2 * ks + (mi & 1)), b);
-        mma16816<T>(p[0], qf[ks][0], qf[ks][1], qf[ks][2], qf[ks][3], b[0], b[1]);
-        mma16816<T>(p[1], qf[ks][0], qf[ks][1], qf[ks][2], qf[ks][3], b[2], b[3]);
+    for (int ks = 0; ks < HD / 16; ++ks) {
+      uint32_t b[4];
+      pr_ldsm(kt + off((mi >> 1) * 8 + (lane & 7), 2 * ks + (mi & 1)), b);
+      mma16816<T>(p[0], qf[ks][0], qf[ks][1], qf[ks][2], qf[ks][3], b[0], b[1]);
+      mma16816<T>(p[1], qf[ks][0], qf[ks][1], qf[ks][2], qf[ks][3], b[2], b[3]);
+    }
+    float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int kk = key + 8 * j + 2 * t + c;
+        p[j][c] = kk < lim0 ? p[j][c] * a.scale_log2 : -INFINITY;
+        p[j][2 + c] = kk < lim1 ? p[j][2 + c] * a.scale_log2 : -INFINITY;
+        x0 = fmaxf(x0, p[j][c]);
+        x1 = fmaxf(x1, p[j][2 + c]);
       }
-      float x0 = -INFINITY, x1 = -INFINITY;
+    }
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+    for (int d = 1; d < 4; d <<= 1) {
+      x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
+      x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
+    }
+    const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+    // nothing seen yet: any finite reference will do, exp2(-inf) = 0
+    const float u0 = n0 == -INFINITY ? 0.f : n0, u1 = n1 == -INFINITY ? 0.f : n1;
+    if (__any_sync(0xffffffffu, n0 != m0 || n1 != m1)) {
+      const float c0 = exp2f(m0 - u0), c1 = exp2f(m1 - u1);
+      m0 = n0;
+      m1 = n1;
+      l0 *= c0;
+      l1 *= c1;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int kk = key + 8 * j + 2 * t + c;
-          p[j][c] = kk < lim0 ? p[j][c] * a.scale_log2 : -INFINITY;
-          p[j][2 + c] = kk < lim1 ? p[j][2 + c] * a.scale_log2 : -INFINITY;
-          x0 = fmaxf(x0, p[j][c]);
-          x1 = fmaxf(x1, p[j][2 + c]);
-        }
+      for (int i = 0; i < HD / 8; ++i) {
+        o[i][0] *= c0;
+        o[i][1] *= c0;
+        o[i][2] *= c1;
+        o[i][3] *= c1;
       }
+    }
 #pragma unroll
-      for (int d = 1; d < 4; d <<= 1) {
-        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
-        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        p[j][c] = exp2f(p[j][c] - u0);
+        p[j][2 + c] = exp2f(p[j][2 + c] - u1);
+        l0 += p[j][c];
+        l1 += p[j][2 + c];
       }
-      const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
-      // nothing seen yet: any finite reference will do, exp2(-inf) = 0
-      const float u0 = n0 == -INFINITY ? 0.f : n0, u1 = n1 == -INFINITY ? 0.f : n1;
-      if (__any_sync(0xffffffffu, n0 != m0 || n1 != m1)) {
-        const float c0 = exp2f(m0 - u0), c1 = exp2f(m1 - u1);
-        m0 = n0;
-        m1 = n1;
-        l0 *= c0;
-        l1 *= c1;
+    }
+    const uint32_t pa0 = Act<T>::pack2(p[0][0], p[0][1]), pa1 = Act<T>::pack2(p[0][2], p[0][3]);
+    const uint32_t pa2 = Act<T>::pack2(p[1][0], p[1][1]), pa3 = Act<T>::pack2(p[1][2], p[1][3]);
 #pragma unroll
-        for (int i = 0; i < HD / 8; ++i) {
-          o[i][0] *= c0;
-          o[i][1] *= c0;
-          o[i][2] *= c1;
-          o[i][3] *= c1;
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          p[j][c] = exp2f(p[j][c] - u0);
-          p[j][2 + c] = exp2f(p[j][2 + c] - u1);
-          l0 += p[j][c];
-          l1 += p[j][2 + c];
-        }
-      }
-      const uint32_t pa0 = Act<T>::pack2(p[0][0], p[0][1]), pa1 = Act<T>::pack2(p[0][2], p[0][3]);
-      const uint32_t pa2 = Act<T>::pack2(p[1][0], p[1][1]), pa3 = Act<T>::pack2(p[1][2], p[1][3]);
-#pragma unroll
-      for (int d = 0; d < HD / 16; ++d) {
-        uint32_t b[4];
-        pr_ldsm_t(vt + off((mi & 1) * 8 + (lane & 7), 2 * d + (mi >> 1)), b);
-        mma16816<T>(o[2 * d], pa0, pa1, pa2, pa3, b[0], b[1]);
-        mma16816<T>(o[2 * d + 1], pa0, pa1, pa2, pa3, b[2], b[3]);
-      }
+    for (int d = 0; d < HD / 16; ++d) {
+      uint32_t b[4];
+      pr_ldsm_t(vt + off((mi & 1) * 8 + (lane & 7), 2 * d + (mi >> 1)), b);
+      mma16816<T>(o[2 * d], pa0, pa1, pa2, pa3, b[0], b[1]);
+      mma16816<T>(o[2 * d + 1], pa0, pa1, pa2, pa3, b[2], b[3]);
     }
     __syncwarp();  // every lane has read the stage before it is loaded again
     if (++buf == NS) buf = 0;
+    const bool end = at.step + 1 == at.per_item;
+    if (end || left == 1) {
+#pragma unroll
+      for (int d = 1; d < 4; d <<= 1) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, d);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, d);
+      }
+      const bool whole = end && from == 0;
+#pragma unroll
+      for (int hr = 0; hr < 2; ++hr) {
+        const int rr = g + 8 * hr, r = r0 + rr;
+        if (r >= rows) continue;
+        const float m = hr ? m1 : m0, l = hr ? l1 : l0;
+        if (whole) {
+          const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees no key is zero
+          T* out = reinterpret_cast<T*>(a.out) + (long long)(at.s.q0 + r / a.group) * a.o_tok +
+                   (kvh * a.group + r % a.group) * a.o_head;
+#pragma unroll
+          for (int i = 0; i < HD / 8; ++i)
+            *reinterpret_cast<uint32_t*>(out + 8 * i + 2 * t) = Act<T>::pack2(o[i][2 * hr] * inv, o[i][2 * hr + 1] * inv);
+        } else {
+          const long long slot = (me * 2 + (head ? 0 : 1)) * 16 + rr;  // at the share's front, or its end
+#pragma unroll
+          for (int i = 0; i < HD / 8; ++i)
+            *reinterpret_cast<float2*>(a.part + slot * HD + 8 * i + 2 * t) = make_float2(o[i][2 * hr], o[i][2 * hr + 1]);
+          if (t == 0) *reinterpret_cast<float2*>(a.stat + 2 * slot) = make_float2(m, l);
+        }
+      }
+      fresh = true;
+      head = false;
+    }
+    at.next(a);
   }
   cp_async_wait<0>();
-#pragma unroll
-  for (int d = 1; d < 4; d <<= 1) {
-    l0 += __shfl_xor_sync(0xffffffffu, l0, d);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, d);
-  }
-  // merge the warps: [warp][16 rows][HD + 4] fp32 over the rings; this CTA's sums behind them
-  constexpr int ML = HD + 4;
-  static_assert((NW + 1) * 16 * ML * 4 <= pr_smem<HD>(), "the merge fits the rings");
-  float* mg = reinterpret_cast<float*>(smem) + warp * 16 * ML;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < HD / 8; ++i) {
-    *reinterpret_cast<float2*>(mg + g * ML + 8 * i + 2 * t) = make_float2(o[i][0], o[i][1]);
-    *reinterpret_cast<float2*>(mg + (g + 8) * ML + 8 * i + 2 * t) = make_float2(o[i][2], o[i][3]);
-  }
-  if (t == 0) {
-    *reinterpret_cast<float2*>(mg + g * ML + HD) = make_float2(m0, l0);
-    *reinterpret_cast<float2*>(mg + (g + 8) * ML + HD) = make_float2(m1, l1);
-  }
-  __syncthreads();
-  // n partial sums of row r's values c .. c + 3, `at(i)` giving (maximum, weight) and the values
-  auto merge = [&](int n, auto stat, auto vals, float& m, float& l) {
-    m = -INFINITY;
-    for (int w = 0; w < n; ++w) m = fmaxf(m, stat(w).x);
-    const float u = m == -INFINITY ? 0.f : m;
-    l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int w = 0; w < n; ++w) {
-      const float2 st = stat(w);
-      const float f = exp2f(st.x - u);
-      const float4 v = vals(w);
-      l += f * st.y;
-      acc.x += f * v.x;
-      acc.y += f * v.y;
-      acc.z += f * v.z;
-      acc.w += f * v.w;
-    }
-    return acc;
-  };
-  auto write = [&](int r, int c, float4 acc, float l) {
-    const int tok = s.q0 + (r0 + r) / a.group, h = kvh * a.group + (r0 + r) % a.group;
-    const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees no key is zero
-    *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + (long long)tok * a.o_tok + h * a.o_head + c) =
-        make_uint2(Act<T>::pack2(acc.x * inv, acc.y * inv), Act<T>::pack2(acc.z * inv, acc.w * inv));
-  };
-  const int live = min(16, rows - r0) * (HD / 4);
-  float* own = reinterpret_cast<float*>(smem) + NW * 16 * ML;
-  for (int i = tid; i < live; i += NT) {  // 4 values of a row over the warps
-    const int r = i / (HD / 4), c = (i % (HD / 4)) * 4;
-    const float* base = reinterpret_cast<const float*>(smem) + r * ML;
-    float m, l;
-    const float4 acc = merge(
-        NW, [&](int w) { return *reinterpret_cast<const float2*>(base + w * 16 * ML + HD); },
-        [&](int w) { return *reinterpret_cast<const float4*>(base + w * 16 * ML + c); }, m, l);
-    if (a.splits == 1) {
-      write(r, c, acc, l);
-    } else if (a.clustered) {
-      *reinterpret_cast<float4*>(own + r * ML + c) = acc;
-      if (c == 0) *reinterpret_cast<float2*>(own + r * ML + HD) = make_float2(m, l);
-    } else {  // this part's sums, relative to its maximum
-      const int tok = s.q0 + (r0 + r) / a.group, h = kvh * a.group + (r0 + r) % a.group;
-      const long long at = ((long long)part * a.tq + tok) * a.n_q + h;
-      if (c == 0) *reinterpret_cast<float2*>(a.stat + 2 * at) = make_float2(m, l);
-      if (l != 0.f) *reinterpret_cast<float4*>(a.part + at * HD + c) = acc;
-    }
-  }
-  if (a.splits > 1 && a.clustered) {
-    cluster_sync();
-    const uint32_t base = smem_u32(own);
-    for (int i = tid + part * NT; i < live; i += NT * a.splits) {
-      const int r = i / (HD / 4), c = (i % (HD / 4)) * 4;
-      float m, l;
-      const float4 acc = merge(
-          a.splits,
-          [&](int w) {
-            const uint32_t at = mapa(base + (r * ML + HD) * 4, w);
-            return make_float2(ld_dsmem_f32(at), ld_dsmem_f32(at + 4));
-          },
-          [&](int w) { return ld_dsmem_f4(mapa(base + (r * ML + c) * 4, w)); }, m, l);
-      write(r, c, acc, l);
-    }
-    cluster_sync();  // the sums stay until the whole cluster has read them
-  }
 }
 
-// Joins the parts of every (token, head), one CTA each: first a thread per
-// part for the common maximum and the parts' weights, then hd / 4 threads
-// across the values and the rest across the parts, so that both passes have
-// their loads in flight together.
-constexpr int kPrCombine = 256, kPrMaxSplits = 512;
-template <typename T, int HD>
-__global__ void __launch_bounds__(kPrCombine) prompt_combine_kernel(const __grid_constant__ PromptArgs a) {
-  constexpr int LANES = HD / 4, GROUPS = kPrCombine / LANES;
-  __shared__ float wt[kPrMaxSplits];
-  __shared__ float4 sv[GROUPS][LANES];
-  __shared__ float red[2][kPrCombine / 32];
-  pdl_entry();
-  const int tok = blockIdx.x, h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // rows outside the sequences have no parts and stay as they were
-  if (tok < __ldg(a.cu_q) || tok >= __ldg(a.cu_q + a.n_seq)) return;
-  const long long step = (long long)a.tq * a.n_q, at = (long long)tok * a.n_q + h;
-  float2 st[kPrMaxSplits / kPrCombine];
-  float m = -INFINITY;
+// Joins the partial rows of one (token, head) by one CTA: `n` of them at
+// slot(i) of part / stat, 1024 at a time with a running maximum. A thread per
+// part for the weights, then hd / 4 threads across the values and the rest
+// across the parts, so that both passes have their loads in flight together.
+constexpr int kPrJoin = 256, kPrChunk = 4 * kPrJoin;
+template <int HD>
+struct JoinSmem {
+  float wt[kPrChunk], red[2][kPrJoin / 32];
+  float4 sv[4 * kPrJoin / HD][HD / 4];
+};
+template <typename T, int HD, typename Slot>
+EE_DEV void join_row(const PromptArgs& a, long long n, Slot slot, T* out, JoinSmem<HD>* sh) {
+  constexpr int LANES = HD / 4, GROUPS = kPrJoin / LANES;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, c = tid % LANES, grp = tid / LANES;
+  const float2* stat = reinterpret_cast<const float2*>(a.stat);
+  float m = -INFINITY, l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (long long i0 = 0; i0 < n; i0 += kPrChunk) {
+    const int here = (int)(n - i0 < kPrChunk ? n - i0 : kPrChunk);
+    float2 st[kPrChunk / kPrJoin];
+    float x = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < kPrMaxSplits / kPrCombine; ++i) {
-    const int sp = threadIdx.x + i * kPrCombine;
-    st[i] = sp < a.splits ? __ldg(reinterpret_cast<const float2*>(a.stat) + at + sp * step) : make_float2(-INFINITY, 0.f);
-    m = fmaxf(m, st[i].x);
-  }
-  m = warp_max(m);
-  if (lane == 0) red[0][warp] = m;
-  __syncthreads();
+    for (int j = 0; j < kPrChunk / kPrJoin; ++j) {
+      const int i = tid + j * kPrJoin;
+      st[j] = i < here ? __ldg(stat + slot(i0 + i)) : make_float2(-INFINITY, 0.f);
+      x = fmaxf(x, st[j].x);
+    }
+    x = warp_max(x);
+    if (lane == 0) sh->red[0][warp] = x;
+    __syncthreads();
+    float top = m;
 #pragma unroll
-  for (int i = 0; i < kPrCombine / 32; ++i) m = fmaxf(m, red[0][i]);
-  const float u = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
+    for (int i = 0; i < kPrJoin / 32; ++i) top = fmaxf(top, sh->red[0][i]);
+    const float u = top == -INFINITY ? 0.f : top, old = exp2f(m - u);
+    m = top;
+    l *= old;
+    acc = make_float4(acc.x * old, acc.y * old, acc.z * old, acc.w * old);
 #pragma unroll
-  for (int i = 0; i < kPrMaxSplits / kPrCombine; ++i) {
-    const float f = st[i].y == 0.f ? 0.f : exp2f(st[i].x - u);  // weight 0: no key seen, its sums were not written
-    wt[threadIdx.x + i * kPrCombine] = f;
-    l += f * st[i].y;
+    for (int j = 0; j < kPrChunk / kPrJoin; ++j) {
+      // weight 0: the part has seen no key, its sums need not have been written
+      const float f = st[j].y == 0.f ? 0.f : exp2f(st[j].x - u);
+      l += f * st[j].y;
+      sh->wt[tid + j * kPrJoin] = f;
+    }
+    __syncthreads();
+    for (int i = grp; i < here; i += 8 * GROUPS) {  // loads first: none waits for another's weight
+      float4 v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        v[k] = __ldg(reinterpret_cast<const float4*>(a.part + slot(i0 + min(i + k * GROUPS, here - 1)) * HD) + c);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float w = i + k * GROUPS < here ? sh->wt[i + k * GROUPS] : 0.f;
+        if (w != 0.f) {
+          acc.x += w * v[k].x;
+          acc.y += w * v[k].y;
+          acc.z += w * v[k].z;
+          acc.w += w * v[k].w;
+        }
+      }
+    }
+    __syncthreads();
   }
   l = warp_sum(l);
-  if (lane == 0) red[1][warp] = l;
-  __syncthreads();
-  const int c = threadIdx.x % LANES, grp = threadIdx.x / LANES;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int i = grp; i < a.splits; i += GROUPS) {
-    const float f = wt[i];
-    if (f != 0.f) {
-      const float4 v = __ldg(reinterpret_cast<const float4*>(a.part + (at + i * step) * HD) + c);
-      acc.x += f * v.x;
-      acc.y += f * v.y;
-      acc.z += f * v.z;
-      acc.w += f * v.w;
-    }
-  }
-  sv[grp][c] = acc;
+  if (lane == 0) sh->red[1][warp] = l;
+  sh->sv[grp][c] = acc;
   __syncthreads();
   if (grp) return;
   l = 0.f;
 #pragma unroll
-  for (int i = 0; i < kPrCombine / 32; ++i) l += red[1][i];
+  for (int i = 0; i < kPrJoin / 32; ++i) l += sh->red[1][i];
 #pragma unroll
   for (int g = 1; g < GROUPS; ++g) {
-    const float4 v = sv[g][c];
+    const float4 v = sh->sv[g][c];
     acc.x += v.x;
     acc.y += v.y;
     acc.z += v.z;
     acc.w += v.w;
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + (long long)tok * a.o_tok + h * a.o_head + 4 * c) =
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees no key is zero
+  *reinterpret_cast<uint2*>(out + 4 * c) =
       make_uint2(Act<T>::pack2(acc.x * inv, acc.y * inv), Act<T>::pack2(acc.z * inv, acc.w * inv));
+}
+
+// The parts of the tensor-core kernel's keys, by (part, token, head).
+template <typename T, int HD>
+__global__ void __launch_bounds__(kPrJoin) prompt_combine_kernel(const __grid_constant__ PromptArgs a) {
+  __shared__ JoinSmem<HD> sh;
+  pdl_entry();
+  const int tok = blockIdx.x, h = blockIdx.y;
+  // rows outside the sequences have no parts and stay as they were
+  if (tok < __ldg(a.cu_q) || tok >= __ldg(a.cu_q + a.n_seq)) return;
+  const long long step = (long long)a.tq * a.n_q, at = (long long)tok * a.n_q + h;
+  join_row<T, HD>(a, a.splits, [&](long long i) { return at + i * step; },
+                  reinterpret_cast<T*>(a.out) + (long long)tok * a.o_tok + h * a.o_head, &sh);
+}
+
+// The same by one warp, 32 parts at a time, hd / 32 values a lane: for items of
+// few parts, where a CTA's barriers cost more than its width saves.
+template <typename T, int HD, typename Slot>
+EE_DEV void join_row_warp(const PromptArgs& a, long long n, Slot slot, T* out) {
+  constexpr int V = HD / 32;
+  const int lane = threadIdx.x & 31;
+  float m = -INFINITY, l = 0.f, v[V] = {};
+  for (long long i0 = 0; i0 < n; i0 += 32) {
+    const int here = (int)(n - i0 < 32 ? n - i0 : 32);
+    const float2 st = lane < here ? __ldg(reinterpret_cast<const float2*>(a.stat) + slot(i0 + lane))
+                                  : make_float2(-INFINITY, 0.f);
+    const float top = fmaxf(m, warp_max(st.x));
+    const float u = top == -INFINITY ? 0.f : top, old = exp2f(m - u);
+    m = top;
+    const float f = st.y == 0.f ? 0.f : exp2f(st.x - u);
+    l = l * old + f * st.y;
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] *= old;
+    for (int i = 0; i < here; i += 8) {  // loads first: none waits for another's weight
+      float2 x[8][V / 2];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int e = 0; e < V / 2; ++e)
+          x[k][e] = __ldg(reinterpret_cast<const float2*>(a.part + slot(i0 + min(i + k, here - 1)) * HD + lane * V) + e);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float w = __shfl_sync(0xffffffffu, f, (i + k) & 31);  // 0 past the last part
+        if (w != 0.f) {
+#pragma unroll
+          for (int e = 0; e < V / 2; ++e) {
+            v[2 * e] += w * x[k][e].x;
+            v[2 * e + 1] += w * x[k][e].y;
+          }
+        }
+      }
+    }
+  }
+  l = warp_sum(l);
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees no key is zero
+#pragma unroll
+  for (int e = 0; e < V; e += 2)
+    *reinterpret_cast<uint32_t*>(out + lane * V + e) = Act<T>::pack2(v[e] * inv, v[e + 1] * inv);
+}
+
+// The rows of the kernel for few rows whose item was cut, and rows without
+// keys. MANY: a CTA per (token, head); else a warp.
+template <typename T, int HD, bool MANY>
+__global__ void __launch_bounds__(kPrJoin) prompt_join_kernel(const __grid_constant__ PromptArgs a, int most) {
+  __shared__ PrList<kPrJoin> list;
+  __shared__ JoinSmem<HD> sh;
+  __shared__ PromptSeq seq;
+  __shared__ long long seq_first;
+  __shared__ int found;
+  pdl_entry();
+  const int tok = blockIdx.x;
+  if (threadIdx.x == 0) found = 0;
+  const int per = (a.n_seq + kPrJoin - 1) / kPrJoin;
+  PromptSeq hit{};
+  long long hit_at = -1;  // steps of the thread's own sequences before the token's
+  const long long total = pr_list<kPrJoin>(a, &list, per, [&](const PromptSeq& s, long long before) {
+    if (tok >= s.q0 && tok < s.q0 + s.qlen) {
+      hit = s;
+      hit_at = before;
+    }
+  });
+  if (hit_at >= 0) {
+    seq = hit;
+    seq_first = list.before[threadIdx.x] + hit_at;
+    found = 1;
+  }
+  __syncthreads();
+  if (!found) return;  // rows outside the sequences stay as they were
+  const PromptSeq s = seq;
+  int steps;
+  pr_steps(a, s, steps);
+  const long long share = pr_share(total, most);
+  const int h = MANY ? blockIdx.y : blockIdx.y * (kPrJoin / 32) + (threadIdx.x >> 5);
+  if (h < a.n_q) {
+    const int kvh = h / a.group, r = (tok - s.q0) * a.group + h % a.group;
+    long long w0 = 0, n = 0, front = 0;
+    if (steps > 0) {
+      const long long first = seq_first + (long long)(r / 16 * a.n_kv + kvh) * steps;
+      w0 = pr_div(first, share);
+      n = pr_div(first + steps - 1, share) - w0 + 1;
+      if (n == 1) return;  // in one share: written already
+      front = w0 * share == first ? 0 : 16;  // else the first part is at its share's end
+    }
+    auto slot = [&](long long i) { return (w0 + i) * 32 + (i == 0 ? front : 0) + r % 16; };
+    T* out = reinterpret_cast<T*>(a.out) + (long long)tok * a.o_tok + h * a.o_head;
+    if (MANY) join_row<T, HD>(a, n, slot, out, &sh);
+    else join_row_warp<T, HD>(a, n, slot, out);
+  }
 }
 
 // How a call runs, by what the host knows of it: rows (queries x group) per
 // sequence and key head, and keys per sequence, on average.
 //   tc      more than 16 rows: the tensor-core kernel's 128-row tiles (8 x 50
 //           new tokens behind 816, 16 heads of 128: 27 us, 68 with 64-row warp
-//           MMA units), 16 or fewer: the rows kernel's single MMA row tile
-//   splits  parts of the keys, joined by a second launch. Rows kernel: enough
-//           CTAs for four an SM, of 128 keys or more each (two or eight an SM
-//           measured within 10 % or slower: 8 x 4096 keys, 32 / 8 heads of 128:
-//           53 / 47 / 49 us for 2 / 4 / 8). Tensor-core kernel: where the items
-//           would leave SMs idle, parts of 512 keys or more.
-#ifndef EE_PR_PER_SM
-#define EE_PR_PER_SM 4
-#endif
-#ifndef EE_PR_CLUSTER
-#define EE_PR_CLUSTER 8
-#endif
-constexpr long long kPrRows = 16, kPrCtasPerSm = EE_PR_PER_SM, kPrMinKeys = 128, kPtMinKeys = 512;
-struct PromptPlan { bool tc; int splits; bool clustered; };
+//           MMA units), 16 or fewer: the kernel for few rows' single MMA tile
+//   splits  of the tensor-core kernel: where its items would leave SMs idle,
+//           parts of 512 keys or more, joined by a second launch
+constexpr long long kPrRows = 16, kPtMinKeys = 512;
+struct PromptPlan { bool tc; int splits; };
 static PromptPlan prompt_plan(long long tq, long long tk, int n_seq, int n_q, int n_kv) {
-  PromptPlan pl{false, 1, false};
+  PromptPlan pl{false, 1};
   if (n_seq < 1) return pl;
   const int group = n_q / n_kv;
   const long long rows = tq * group;
   pl.tc = rows > kPrRows * n_seq && tk > 0 && group <= 128;
-  // rows of a unit: two tiles of whole tokens, or one MMA tile
-  const long long per = pl.tc ? 2 * (128 / group) * group : kPrRows;
-  const long long units = (rows / per > n_seq ? rows / per : n_seq) * n_kv;
-  const long long want = pl.tc ? device_sms() / units : (kPrCtasPerSm * device_sms() + units - 1) / units;
-  const long long most = pl.tc ? tk / n_seq / kPtMinKeys : (tk / n_seq + kPrMinKeys - 1) / kPrMinKeys;
+  if (!pl.tc) return pl;
+  const long long per = 2 * (128 / group) * group;  // rows of an item: two tiles of whole tokens
+  const long long items = (rows / per > n_seq ? rows / per : n_seq) * n_kv;
+  const long long want = device_sms() / items, most = tk / n_seq / kPtMinKeys;
   const long long s = want < most ? want : most;
-  pl.splits = s < 1 ? 1 : (int)(s < kPrMaxSplits ? s : kPrMaxSplits);
-  pl.clustered = !pl.tc && pl.splits > 1 && pl.splits <= EE_PR_CLUSTER;
+  pl.splits = s < 1 ? 1 : (int)s;
   return pl;
 }
+static long long prompt_partials(const PromptPlan& pl, long long tq, int n_q, int hd) {  // partial rows
+  if (pl.tc) return pl.splits > 1 ? pl.splits * tq * n_q : 0;
+  return (long long)device_sms() * (hd == 128 ? pr_warps<128>() : pr_warps<64>()) * 32;
+}
 static size_t prompt_ws_bytes(const PromptPlan& pl, long long tq, int n_q, int hd) {
-  return pl.splits > 1 && !pl.clustered ? (size_t)pl.splits * tq * n_q * (hd + 2) * 4 : 0;
+  return (size_t)prompt_partials(pl, tq, n_q, hd) * (hd + 2) * 4;
 }
 
 template <typename T, int HD>
 static int launch_combine(const PromptArgs& a, cudaStream_t s) {
-  if (a.splits == 1 || a.clustered) return EE_OK;
-  return launch_pdl(prompt_combine_kernel<T, HD>, dim3((unsigned)a.tq, a.n_q), dim3(kPrCombine), 0, s, a) == cudaSuccess
+  if (a.splits == 1) return EE_OK;
+  return launch_pdl(prompt_combine_kernel<T, HD>, dim3((unsigned)a.tq, a.n_q), dim3(kPrJoin), 0, s, a) == cudaSuccess
              ? EE_OK
              : EE_ERR_LAUNCH;
 }
@@ -388,27 +561,17 @@ static int launch_rows(const PromptArgs& a, cudaStream_t s) {
   auto fn = prompt_rows_kernel<T, HD>;
   static std::atomic<int> set[64];
   allow_max_smem(fn, set);
-  // at most one partial block per sequence beyond the rows' whole blocks
-  const long long units = (long long)a.tq * a.group / 16 + a.n_seq;
-  if (units * a.splits > 0x7fffffff) return EE_ERR_SHAPE;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(units * a.splits), a.n_kv);
-  cfg.blockDim = dim3(32 * kPrWarps);
-  cfg.dynamicSmemBytes = pr_smem<HD>();
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  unsigned int n = 0;
-  add_pdl_attr(attr, n);
-  if (a.clustered) {
-    attr[n].id = cudaLaunchAttributeClusterDimension;
-    attr[n].val.clusterDim.x = a.splits;
-    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
-    ++n;
-  }
-  cfg.attrs = attr;
-  cfg.numAttrs = n;
-  if (cudaLaunchKernelEx(&cfg, fn, a) != cudaSuccess) return EE_ERR_LAUNCH;
-  return launch_combine<T, HD>(a, s);
+  const int sms = device_sms();
+  if (launch_pdl(fn, dim3(sms), dim3(32 * pr_warps<HD>()), pr_smem<HD>(), s, a) != cudaSuccess) return EE_ERR_LAUNCH;
+  // parts of an item, on average: a CTA per row from 16 on
+  const long long items = (((long long)a.tq * a.group / 16 > a.n_seq ? (long long)a.tq * a.group / 16 : a.n_seq)) * a.n_kv;
+  const int most = sms * pr_warps<HD>();
+  const cudaError_t e =
+      most > 16 * items
+          ? launch_pdl(prompt_join_kernel<T, HD, true>, dim3((unsigned)a.tq, a.n_q), dim3(kPrJoin), 0, s, a, most)
+          : launch_pdl(prompt_join_kernel<T, HD, false>, dim3((unsigned)a.tq, (a.n_q + kPrJoin / 32 - 1) / (kPrJoin / 32)),
+                       dim3(kPrJoin), 0, s, a, most);
+  return e == cudaSuccess ? EE_OK : EE_ERR_LAUNCH;
 }
 
 int* gemm_status_ptr();  // ee_ops.cu: the status word of the tensor-core kernels on the current device
@@ -505,9 +668,8 @@ int ee_prompt_attention(const void* q, int64_t q_tok, int64_t q_head, const void
   a.causal = causal != 0;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.splits = pl.splits;
-  a.clustered = pl.clustered;
   a.part = reinterpret_cast<float*>(workspace);
-  a.stat = a.part + (size_t)pl.splits * tq * n_q * head_dim;
+  a.stat = a.part + (size_t)prompt_partials(pl, tq, n_q, head_dim) * head_dim;
   cudaStream_t s = (cudaStream_t)stream;
   return act_dtype == EE_BF16 ? launch_prompt<__nv_bfloat16>(a, pl, head_dim, s)
                                : launch_prompt<__half>(a, pl, head_dim, s);

@@ -21,10 +21,9 @@ struct PromptArgs {
   long long q_tok, q_head, k_tok, k_head, v_tok, v_head, o_tok, o_head;  // strides, elements
   int tq, tk, n_seq, n_q, n_kv, group, causal;
   float scale_log2;  // scale * log2(e)
-  int splits;        // parts of the keys
-  int clustered;     // the parts are a cluster's CTAs, joined there; else through part and stat
-  float* part;       // [splits][tq][n_q][hd] sums of a part and [splits][tq][n_q][2] their maximum and weight
-  float* stat;
+  int splits;        // tensor-core kernel: parts of the keys
+  float* part;       // sums of partial rows and, in stat, their maximum and weight: [splits][tq][n_q][hd], or by
+  float* stat;       // worker ([workers][2][16][hd]) in the kernel for few rows
 };
 
 struct PromptSeq {
@@ -41,55 +40,6 @@ EE_DEV PromptSeq prompt_seq(const PromptArgs& a, int b) {
   s.klen = min(max(end, s.k0), a.tk) - s.k0;
   s.blk = 0;
   return s;
-}
-
-// The sequence and block of unit `u`, the sequences' query rows (times `mul`)
-// being cut into blocks of `rows`; false when there is no such unit. All
-// THREADS threads of the CTA call it, each with a sequence of its own whose
-// whole record it reads at once, so a call of up to THREADS sequences waits
-// for global memory once.
-template <int THREADS>
-struct PromptFind {
-  int sums[THREADS / 32], hit;
-  PromptSeq seq;
-};
-template <int THREADS>
-EE_DEV bool prompt_find(const PromptArgs& a, int u, int mul, int rows, PromptFind<THREADS>* sh, PromptSeq& out) {
-  constexpr int NW = THREADS / 32;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int before = 0;
-  for (int b0 = 0; b0 < a.n_seq; b0 += THREADS) {
-    PromptSeq s{};
-    if (b0 + tid < a.n_seq) s = prompt_seq(a, b0 + tid);
-    const int nb = (int)(((long long)s.qlen * mul + rows - 1) / rows);
-    int inc = nb;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int t = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += t;
-    }
-    if (tid == 0) sh->hit = 0;
-    if (lane == 31) sh->sums[warp] = inc;
-    __syncthreads();
-    int base = before, total = before;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      if (w < warp) base += sh->sums[w];
-      total += sh->sums[w];
-    }
-    if (u >= base + inc - nb && u < base + inc) {
-      s.blk = u - (base + inc - nb);
-      sh->seq = s;
-      sh->hit = 1;
-    }
-    __syncthreads();
-    if (sh->hit) {
-      out = sh->seq;
-      return true;
-    }
-    before = total;
-  }
-  return false;
 }
 
 }  // namespace ee
