@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import importlib.util
 import os
 import threading
 
@@ -128,6 +129,24 @@ def load():
                 fn.argtypes = args
             _lib = lib
     return _lib
+
+
+_native = None
+
+
+def native():
+    """The extension module ``lib/ee_torch.so``: the usual calls of the prompt-layer operators without the
+    interpreter. Its functions return None for any other call (see csrc/ee_torch.cpp)."""
+    global _native
+    if _native is None:
+        load()
+        path = _build.TORCH_LIB
+        if not os.path.exists(path):
+            raise RuntimeError(f"{path} is missing: build it with `python -m embodied_efficiency_b200.build`")
+        spec = importlib.util.spec_from_file_location("ee_torch", path)
+        _native = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(_native)
+    return _native
 
 
 def strerror(code: int) -> str:

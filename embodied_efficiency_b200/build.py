@@ -1,4 +1,5 @@
-"""Build the sm_100a shared library ``lib/libee_b200.so`` from ``csrc/`` with nvcc.
+"""Build the sm_100a shared library ``lib/libee_b200.so`` from ``csrc/`` with nvcc, and the extension module
+``lib/ee_torch.so`` (the native host side of the prompt-layer operators) with g++.
 
 The library is built in-tree so that it travels with the source checkout;
 ``python -m embodied_efficiency_b200.build`` (or ``__graft_entry__.build()``)
@@ -15,6 +16,8 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 LIBDIR = os.path.join(PKG, "lib")
 LIB = os.path.join(LIBDIR, "libee_b200.so")
+TORCH_SRC = os.path.join(CSRC, "ee_torch.cpp")       # native host side of the prompt-layer operators
+TORCH_LIB = os.path.join(LIBDIR, "ee_torch.so")      # a Python extension module linked against LIB
 INCLUDE = os.path.join(os.path.dirname(PKG), "include")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -39,10 +42,30 @@ def _deps() -> list:
 
 
 def up_to_date() -> bool:
-    if not os.path.exists(LIB):
+    if not os.path.exists(LIB) or not os.path.exists(TORCH_LIB):
         return False
-    t = os.path.getmtime(LIB)
+    t = min(os.path.getmtime(LIB), os.path.getmtime(TORCH_LIB))
     return all(os.path.getmtime(f) <= t for f in _deps())
+
+
+def _build_torch() -> str:
+    """Compile ``TORCH_SRC`` with g++ against this interpreter's torch."""
+    import sysconfig
+
+    import torch
+    tdir = os.path.join(os.path.dirname(torch.__file__))
+    cuda = os.path.dirname(os.path.dirname(nvcc())) if os.path.sep in nvcc() else "/usr/local/cuda"
+    tmp = TORCH_LIB + ".tmp"
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-isystem", os.path.join(tdir, "include"), "-isystem", os.path.join(tdir, "include/torch/csrc/api/include"),
+           "-isystem", sysconfig.get_paths()["include"], "-isystem", os.path.join(cuda, "include"), "-I", INCLUDE,
+           TORCH_SRC, "-o", tmp, "-L", LIBDIR, "-l:libee_b200.so", "-L", os.path.join(tdir, "lib"), "-ltorch_python",
+           "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on {TORCH_SRC}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, TORCH_LIB)
+    return TORCH_LIB
 
 
 def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> str:
@@ -73,6 +96,7 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) 
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB)
+    _build_torch()
     return LIB
 
 

@@ -30,6 +30,7 @@ struct Int8Args {
   int vec;               // N % 8 == 0: rows of 16-byte pieces
   int tiles_m, tiles_n;  // pair kernel: 256 x 256 output tiles
   int split, ns;         // few kernel: CTAs per cluster (K slices), ring stages
+  int early;             // launched behind the call's own quantiser: the weights may be read before it has finished
   int* status;
   unsigned long long timeout_ns;
 };
@@ -66,20 +67,30 @@ EE_DEV float i8_wscale(const Int8Args& a, int n) {
 // GELU(z) = max(z, 0) - |z| Phi(-|z|), with Phi(-a) = e^(-a^2/2) t P(t),
 // t = 1 / (1 + 0.35 a): Hastings' form, its degree-7 polynomial fitted here
 // by weighted minimax (|error| of Phi below 4e-8, relative below 4e-6). About
-// 16 instructions, where erff costs twice that: the epilogue of a 256 x 256
-// tile has to keep up with the tensor cores.
-EE_DEV float i8_gelu(float z) {
-  const float a = fabsf(z);
-  float t, e;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(0.35f, a, 1.f)));
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * z * -0.72134752f));
-  float p = fmaf(t, 0.044615f, -0.18442732f);
-  p = fmaf(t, p, 0.21107948f);
-  p = fmaf(t, p, 0.00892954f);
-  p = fmaf(t, p, 0.14315536f);
-  p = fmaf(t, p, 0.13687154f);
-  p = fmaf(t, p, 0.13977644f);
-  return fmaf(-fminf(a, 3.0e38f), p * t * e, fmaxf(z, 0.f));  // the fminf: 0 instead of inf * 0
+// 11 instructions a value in packed pairs, where erff costs 30: the epilogue
+// of a 256 x 256 tile has to keep up with the tensor cores.
+EE_DEV uint64_t i8_gelu2(uint64_t z) {
+  uint32_t z0, z1, d0, d1, e0, e1;
+  unpack64(z, z0, z1);
+  const uint64_t a = pack64(z0 & 0x7FFFFFFFu, z1 & 0x7FFFFFFFu);
+  unpack64(fma2f(a, both(0.35f), both(1.f)), d0, d1);
+  unpack64(mul2f(mul2f(z, z), both(-0.72134752f)), e0, e1);
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+r"(d0));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+r"(d1));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+r"(e0));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+r"(e1));
+  const uint64_t t = pack64(d0, d1);
+  uint64_t p = fma2f(t, both(-0.044615f), both(0.18442732f));  // -P: the final product is subtracted
+  p = fma2f(t, p, both(-0.21107948f));
+  p = fma2f(t, p, both(-0.00892954f));
+  p = fma2f(t, p, both(-0.14315536f));
+  p = fma2f(t, p, both(-0.13687154f));
+  p = fma2f(t, p, both(-0.13977644f));
+  p = mul2f(mul2f(p, t), pack64(e0, e1));
+  unpack64(a, d0, d1);
+  // the fminf: 0 instead of inf * 0
+  return fma2f(pack64(__float_as_uint(fminf(__uint_as_float(d0), 3.0e38f)), __float_as_uint(fminf(__uint_as_float(d1), 3.0e38f))),
+               p, pack64(__float_as_uint(fmaxf(__uint_as_float(z0), 0.f)), __float_as_uint(fmaxf(__uint_as_float(z1), 0.f))));
 }
 
 // ---------------------------------------------------------------------------
@@ -137,12 +148,13 @@ EE_DEV void sts16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d)
 // warps. Two accumulators of 256 TMEM columns, so a tile's epilogue runs under
 // the next tile's MMAs. Outputs are staged as swizzled [32 rows][64 columns]
 // blocks and stored by TMA.
-constexpr int kI8Stages = 5;
-constexpr int kI8EpiWarps = 8;
+// (16 epilogue warps and a stage less were slower with the GELU: 677 us
+// instead of 654 for 52224 x 8192 x 2048.)
+constexpr int kI8Stages = 5, kI8EpiWarps = 8;
 constexpr int kI8PairThreads = 32 * (2 + kI8EpiWarps);
 constexpr uint32_t kI8Stage = 32768;
-constexpr uint32_t kI8OffEpi = kI8Stages * kI8Stage;              // 4 KB per epilogue warp
-constexpr uint32_t kI8OffCol = kI8OffEpi + kI8EpiWarps * 4096;    // [2][256] scales and biases
+constexpr uint32_t kI8OffEpi = kI8Stages * kI8Stage;            // 4 KB per epilogue warp
+constexpr uint32_t kI8OffCol = kI8OffEpi + kI8EpiWarps * 4096;  // [2][256] scales and biases
 constexpr uint32_t kI8OffBar = kI8OffCol + 2 * 2 * 256 * 4;
 constexpr uint32_t kI8PairSmem = kI8OffBar + 8 * (2 * kI8Stages + 4) + 16 + 1024;
 
@@ -150,6 +162,8 @@ template <typename T, bool GELU>
 __global__ void __launch_bounds__(kI8PairThreads, 1) __cluster_dims__(2, 1, 1)
     int8_pair_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw,
                      const __grid_constant__ CUtensorMap ty, const __grid_constant__ Int8Args a) {
+  constexpr int NS = kI8Stages, EW = kI8EpiWarps;
+  constexpr uint32_t OFF_BAR = kI8OffBar;
   extern __shared__ __align__(1024) char smem_raw[];
   const uint32_t base0 = smem_u32(smem_raw);
   const uint32_t sb = (base0 + 1023u) & ~1023u;
@@ -158,29 +172,29 @@ __global__ void __launch_bounds__(kI8PairThreads, 1) __cluster_dims__(2, 1, 1)
   const uint32_t rank = cl_rank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const int tiles = a.tiles_m * a.tiles_n, nkb = (a.K + 127) / 128;
-  const uint32_t bar_full = sb + kI8OffBar, bar_empty = bar_full + 8 * kI8Stages;
-  const uint32_t bar_accf = bar_empty + 8 * kI8Stages, bar_acce = bar_accf + 16;
+  const uint32_t bar_full = sb + OFF_BAR, bar_empty = bar_full + 8 * NS;
+  const uint32_t bar_accf = bar_empty + 8 * NS, bar_acce = bar_accf + 16;
   if (warp == 0 && lane == 0) {
     tma_prefetch_map(&tx);
     tma_prefetch_map(&tw);
     tma_prefetch_map(&ty);
-    for (int s = 0; s < kI8Stages; ++s) {
+    for (int s = 0; s < NS; ++s) {
       mbar_init(bar_full + 8 * s, 1);
       mbar_init(bar_empty + 8 * s, 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(bar_accf + 8 * b, 1);
-      mbar_init(bar_acce + 8 * b, 2 * kI8EpiWarps);
+      mbar_init(bar_acce + 8 * b, 2 * EW);
     }
     mbar_fence_init();
   }
-  pdl_entry();
-  if (warp == 1) tmem_alloc2(sb + kI8OffBar + 8 * (2 * kI8Stages + 4), 512);
+  if (!a.early) pdl_entry();
+  if (warp == 1) tmem_alloc2(sb + OFF_BAR + 8 * (2 * NS + 4), 512);
   __syncwarp();
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + kI8OffBar + 8 * (2 * kI8Stages + 4));
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + OFF_BAR + 8 * (2 * NS + 4));
   // tiles in bands of 8 token tiles, so that the tiles in flight share rows of both operands in L2
   auto tile_at = [&](int t, int& tm, int& tn) {
     const int band = t / (8 * a.tiles_n), in = t - band * 8 * a.tiles_n;
@@ -189,9 +203,22 @@ __global__ void __launch_bounds__(kI8PairThreads, 1) __cluster_dims__(2, 1, 1)
     tm = band * 8 + in - tn * h;
   };
 
+  const uint32_t lead_full = mapa(bar_full, 0);
+  int pre = 0;  // stages whose weights are on their way before the tokens are ready
+  if (a.early) {
+    if (warp == 0 && lane == 0 && pair < tiles) {
+      int tm, tn;
+      tile_at(pair, tm, tn);
+      for (; pre < NS && pre < nkb; ++pre) {
+        if (rank == 0) mbar_arrive_expect_tx(bar_full + 8 * pre, 2 * kI8Stage);
+        tma_load_2d_pair(sb + pre * kI8Stage + 16384, &tw, pre * 128, tn * 256 + 128 * (int)rank, lead_full + 8 * pre);
+      }
+    }
+    __syncwarp();
+    pdl_entry();
+  }
   if (warp == 0) {
     if (lane == 0) {
-      const uint32_t lead_full = mapa(bar_full, 0);
       int s = 0, issued = 0;
       uint32_t ph = 0;
       bool ok = true;
@@ -200,21 +227,23 @@ __global__ void __launch_bounds__(kI8PairThreads, 1) __cluster_dims__(2, 1, 1)
         tile_at(t, tm, tn);
         const int m0 = tm * 256 + 128 * (int)rank, n0 = tn * 256 + 128 * (int)rank;
         for (int kb = 0; kb < nkb; ++kb) {
-          if (issued >= kI8Stages && !mbar_wait(bar_empty + 8 * s, ph ^ 1, a.timeout_ns)) {
+          if (issued >= NS && !mbar_wait(bar_empty + 8 * s, ph ^ 1, a.timeout_ns)) {
             ok = false;
             break;
           }
           const uint32_t st = sb + s * kI8Stage;
-          if (rank == 0) mbar_arrive_expect_tx(bar_full + 8 * s, 2 * kI8Stage);
+          if (issued >= pre) {
+            if (rank == 0) mbar_arrive_expect_tx(bar_full + 8 * s, 2 * kI8Stage);
+            tma_load_2d_pair(st + 16384, &tw, kb * 128, n0, lead_full + 8 * s);
+          }
           tma_load_2d_pair(st, &tx, kb * 128, m0, lead_full + 8 * s);
-          tma_load_2d_pair(st + 16384, &tw, kb * 128, n0, lead_full + 8 * s);
           ++issued;
-          if (++s == kI8Stages) { s = 0; ph ^= 1; }
+          if (++s == NS) { s = 0; ph ^= 1; }
         }
       }
       // the last stages have been read (so have landed) before the CTA may exit
-      for (int g = max(issued - kI8Stages, 0); g < issued; ++g)
-        if (!mbar_wait(bar_empty + 8 * (g % kI8Stages), (uint32_t)((g / kI8Stages) & 1), a.timeout_ns)) ok = false;
+      for (int g = max(issued - NS, 0); g < issued; ++g)
+        if (!mbar_wait(bar_empty + 8 * (g % NS), (uint32_t)((g / NS) & 1), a.timeout_ns)) ok = false;
       if (!ok) atomicCAS(a.status, 0, (int)EE_ERR_TIMEOUT);
     }
     __syncwarp();
@@ -243,7 +272,7 @@ __global__ void __launch_bounds__(kI8PairThreads, 1) __cluster_dims__(2, 1, 1)
           for (int kk = 0; kk < 4; ++kk)
             umma_i8<2>(tmem + buf * 256, ad + 2 * kk, bd + 2 * kk, idesc, (kb | kk) != 0 ? 1u : 0u);
           umma_commit2(bar_empty + 8 * s);
-          if (++s == kI8Stages) { s = 0; ph ^= 1; }
+          if (++s == NS) { s = 0; ph ^= 1; }
         }
         if (ok) umma_commit2(bar_accf + 8 * buf);
       }
@@ -251,7 +280,8 @@ __global__ void __launch_bounds__(kI8PairThreads, 1) __cluster_dims__(2, 1, 1)
     }
     __syncwarp();
   } else {
-    const int ew = warp - 2, q4 = warp & 3, half = ew >> 2;  // lanes 32 q4 .. of TMEM, columns 128 half ..
+    constexpr int CW = 256 / (EW / 4);  // columns per epilogue warp
+    const int ew = warp - 2, q4 = warp & 3, cbeg = (ew >> 2) * CW;  // lanes 32 q4 .. of TMEM, columns cbeg ..
     const uint32_t stg = sb + kI8OffEpi + ew * 4096;
     const uint32_t acce = mapa(bar_acce, 0);
     int i = 0;
@@ -263,66 +293,78 @@ __global__ void __launch_bounds__(kI8PairThreads, 1) __cluster_dims__(2, 1, 1)
       const int m = m0 + lane;
       // the tile's column scales and biases, staged while the MMAs run
       float* col = reinterpret_cast<float*>(smem + kI8OffCol) + buf * 512;
-      {
-        const int c = ew * 32 + lane, n = n0 + c;
-        col[c] = n < a.N ? i8_wscale(a, n) : 0.f;
-        col[256 + c] = (n < a.N && (a.epi & I8_BIAS)) ? ld_param(reinterpret_cast<const T*>(a.bias) + n) : 0.f;
+      for (int c = ew * 32 + lane; c < 512; c += 32 * EW) {
+        const int n = n0 + (c & 255);
+        float w = 0.f;
+        if (n < a.N) {
+          if (c < 256) w = i8_wscale(a, n);
+          else if (a.epi & I8_BIAS) w = ld_param(reinterpret_cast<const T*>(a.bias) + n);
+        }
+        col[c] = w;
       }
       const float sx = m < a.M ? __ldg(a.sx + m) : 0.f;
-      named_sync(1, 32 * kI8EpiWarps);
+      named_sync(1, 32 * EW);
       if (ok && !mbar_wait(bar_accf + 8 * buf, (uint32_t)((i >> 1) & 1), a.timeout_ns)) {
         if (lane == 0) atomicCAS(a.status, 0, (int)EE_ERR_TIMEOUT);
         ok = false;
       }
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
+      const uint64_t sx2 = both(sx);
 #pragma unroll 1
-      for (int c0 = half * 128; c0 < half * 128 + 128 && ok; c0 += 64) {
-        uint32_t v[2][32];
-        tmem_ld32(tmem + buf * 256 + ((uint32_t)(32 * q4) << 16) + c0, v[0]);
-        tmem_ld32(tmem + buf * 256 + ((uint32_t)(32 * q4) << 16) + c0 + 32, v[1]);
-        tmem_wait_ld();
-        if (c0 == half * 128 + 64) {  // this warp's last read of the buffer
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(acce + 8 * buf);
-        }
+      for (int c0 = cbeg; c0 < cbeg + CW && ok; c0 += 64) {
         if (lane == 0) bulk_wait_read();  // the previous block has left the staging buffer
         __syncwarp();
         const T* res = reinterpret_cast<const T*>(a.resid) + (size_t)m * a.N + n0 + c0;
+        const bool rv = !GELU && (a.epi & I8_RESID) && m < a.M;
 #pragma unroll
-        for (int g = 0; g < 8; ++g) {  // 8 columns: one 16-byte piece of the row
-          uint4 rq = make_uint4(0, 0, 0, 0);
-          const bool rv = !GELU && (a.epi & I8_RESID) && m < a.M;
-          if (rv && a.vec && n0 + c0 + 8 * g < a.N) rq = *reinterpret_cast<const uint4*>(res + 8 * g);
-          const uint32_t rw[4] = {rq.x, rq.y, rq.z, rq.w};
-          float wv[8], bv[8];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            *reinterpret_cast<float4*>(wv + 4 * e) = *reinterpret_cast<const float4*>(col + c0 + 8 * g + 4 * e);
-            *reinterpret_cast<float4*>(bv + 4 * e) = *reinterpret_cast<const float4*>(col + 256 + c0 + 8 * g + 4 * e);
+        for (int h = 0; h < 2; ++h) {
+          uint32_t v[32];
+          tmem_ld32(tmem + buf * 256 + ((uint32_t)(32 * q4) << 16) + c0 + 32 * h, v);
+          tmem_wait_ld();
+          if (h == 1 && c0 + 64 == cbeg + CW) {  // this warp's last read of the buffer
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(acce + 8 * buf);
           }
-          uint32_t o[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int c = 8 * g + 2 * e;
-            float y0 = fmaf((float)(int)v[c >> 5][c & 31] * sx, wv[2 * e], bv[2 * e]);
-            float y1 = fmaf((float)(int)v[c >> 5][(c & 31) + 1] * sx, wv[2 * e + 1], bv[2 * e + 1]);
-            if (GELU) {
-              y0 = i8_gelu(y0);
-              y1 = i8_gelu(y1);
-            } else if (rv) {
-              float2 r = Act<T>::unpack2(rw[e]);
-              if (!a.vec) {
-                r.x = n0 + c0 + c < a.N ? ld_param(res + c) : 0.f;
-                r.y = n0 + c0 + c + 1 < a.N ? ld_param(res + c + 1) : 0.f;
-              }
-              y0 += r.x;
-              y1 += r.y;
+          for (int g = 0; g < 4; ++g) {  // 8 columns: one 16-byte piece of the row
+            const int c = 32 * h + 8 * g;
+            uint4 rq = make_uint4(0, 0, 0, 0);
+            if (rv && a.vec && n0 + c0 + c < a.N) rq = *reinterpret_cast<const uint4*>(res + c);
+            const uint32_t rw[4] = {rq.x, rq.y, rq.z, rq.w};
+            uint4 w4[2], b4[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              w4[e] = *reinterpret_cast<const uint4*>(col + c0 + c + 4 * e);
+              b4[e] = *reinterpret_cast<const uint4*>(col + 256 + c0 + c + 4 * e);
             }
-            o[e] = Act<T>::pack2(y0, y1);
+            uint32_t o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint4 wq = w4[e >> 1], bq = b4[e >> 1];
+              const uint64_t w2 = (e & 1) ? pack64(wq.z, wq.w) : pack64(wq.x, wq.y);
+              const uint64_t b2 = (e & 1) ? pack64(bq.z, bq.w) : pack64(bq.x, bq.y);
+              const uint64_t s2 = pack64(__float_as_uint((float)(int)v[8 * g + 2 * e]),
+                                         __float_as_uint((float)(int)v[8 * g + 2 * e + 1]));
+              uint64_t y = fma2f(mul2f(s2, sx2), w2, b2);
+              if (GELU) y = i8_gelu2(y);
+              uint32_t y0, y1;
+              unpack64(y, y0, y1);
+              float f0 = __uint_as_float(y0), f1 = __uint_as_float(y1);
+              if (rv) {
+                float2 r = Act<T>::unpack2(rw[e]);
+                if (!a.vec) {
+                  r.x = n0 + c0 + c + 2 * e < a.N ? ld_param(res + c + 2 * e) : 0.f;
+                  r.y = n0 + c0 + c + 2 * e + 1 < a.N ? ld_param(res + c + 2 * e + 1) : 0.f;
+                }
+                f0 += r.x;
+                f1 += r.y;
+              }
+              o[e] = Act<T>::pack2(f0, f1);
+            }
+            sts16(stg + sw128(lane, 4 * h + g), o[0], o[1], o[2], o[3]);
           }
-          sts16(stg + sw128(lane, g), o[0], o[1], o[2], o[3]);
         }
         if (a.vec) {
           fence_proxy_async_smem();
@@ -361,11 +403,11 @@ __global__ void __launch_bounds__(kI8PairThreads, 1) __cluster_dims__(2, 1, 1)
 // ---------------------------------------------------------------------------
 // One cluster per 128 features x NT tokens, its CTAs each a slice of K: the
 // weights are the MMA's 128 lanes (A), the tokens its N, so a call of one
-// token wastes lanes of nothing but the tensor core. Six warps: TMA producer,
-// MMA issuer, four that move the int32 partial sums to shared memory as
-// [token][feature]; then every CTA adds its share of the features over the
+// token wastes lanes of nothing but the tensor core. TMA producer, MMA issuer,
+// four warps that move the int32 partial sums to shared memory as
+// [token][feature]; then all warps of every CTA adds its share of the features over the
 // cluster's partials (integers: exact in any order) and writes them.
-constexpr int kI8FewThreads = 192;
+constexpr int kI8FewThreads = 256;
 template <int NT> constexpr uint32_t i8_few_stage() { return 16384u + NT * 128u; }
 template <int NT> constexpr uint32_t i8_few_part() { return NT * 128u * 4u; }
 
@@ -400,7 +442,7 @@ __global__ void __launch_bounds__(kI8FewThreads)
     mbar_init(bar_acc, 1);
     mbar_fence_init();
   }
-  pdl_entry();
+  if (!a.early) pdl_entry();
   if (warp == 1) {
     tmem_alloc(sb + off_tm, COLS);
     tmem_relinquish();
@@ -409,6 +451,17 @@ __global__ void __launch_bounds__(kI8FewThreads)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + off_tm);
+  int pre = 0;  // stages whose weights are on their way before the tokens are ready
+  if (a.early) {
+    if (warp == 0 && lane == 0) {
+      for (; pre < a.ns && kb0 + pre < kb1; ++pre) {
+        mbar_arrive_expect_tx(bar_full + 8 * pre, STAGE);
+        tma_load_2d(sb + pre * STAGE, &tw, (kb0 + pre) * 128, n0, bar_full + 8 * pre);
+      }
+    }
+    __syncwarp();
+    pdl_entry();
+  }
   if (warp == 0) {
     if (lane == 0) {
       bool ok = true;
@@ -420,8 +473,10 @@ __global__ void __launch_bounds__(kI8FewThreads)
           break;
         }
         const uint32_t st = sb + s * STAGE, fb = bar_full + 8 * s;
-        mbar_arrive_expect_tx(fb, STAGE);
-        tma_load_2d(st, &tw, kb * 128, n0, fb);
+        if (issued >= pre) {
+          mbar_arrive_expect_tx(fb, STAGE);
+          tma_load_2d(st, &tw, kb * 128, n0, fb);
+        }
         tma_load_2d(st + 16384, &tx, kb * 128, m0, fb);
         ++issued;
         if (++s == a.ns) { s = 0; ph ^= 1; }
@@ -461,7 +516,7 @@ __global__ void __launch_bounds__(kI8FewThreads)
   if (!done && lane == 0) atomicCAS(a.status, 0, (int)EE_ERR_TIMEOUT);
   __syncthreads();
   tc_fence_after();
-  if (warp >= 2) {
+  if (warp >= 4) {
     const int q4 = warp & 3;
 #pragma unroll
     for (int c0 = 0; c0 < NT; c0 += 16) {
@@ -479,16 +534,25 @@ __global__ void __launch_bounds__(kI8FewThreads)
     tc_fence_after();
     tmem_dealloc(tmem, COLS);
   }
-  // this CTA's features rank * (128 / S) ..: groups of 4 of one token
-  const int fg = 32 / S;  // feature groups of 4 per CTA
-  for (int i = threadIdx.x; i < NT * fg && done; i += kI8FewThreads) {
-    const int tok = i / fg, f = ((int)rank * fg + i % fg) * 4;
-    const int m = m0 + tok, n = n0 + f;
-    if (m >= a.M || n >= a.N) continue;
+  // this CTA's features rank * (128 / S) ..: 4 of one token at a time, the same 4 for all of a thread's tokens
+  const int fg = 32 / S;
+  static_assert(kI8FewThreads % 32 == 0, "a thread's features do not change");
+  const int f = ((int)rank * fg + (int)threadIdx.x % fg) * 4, n = n0 + f;
+  float sw[4], bias[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    sw[e] = n + e < a.N ? i8_wscale(a, n + e) : 0.f;
+    bias[e] = n + e < a.N && (a.epi & I8_BIAS) ? ld_param(reinterpret_cast<const T*>(a.bias) + n + e) : 0.f;
+  }
+#pragma unroll 2
+  for (int tok = threadIdx.x / fg; tok < NT; tok += kI8FewThreads / fg) {
+    const int m = m0 + tok;
+    if (m >= a.M || n >= a.N || !done) break;
+    const float sx = __ldg(a.sx + m);
     int4 acc = make_int4(0, 0, 0, 0);
     const uint32_t at = sb + (tok * 128 + f) * 4;
     if (S > 1) {
-#pragma unroll 4
+#pragma unroll 8
       for (int r = 0; r < S; ++r) {
         const float4 p = ld_dsmem_f4(mapa(at, r));
         acc.x += __float_as_int(p.x);
@@ -499,26 +563,35 @@ __global__ void __launch_bounds__(kI8FewThreads)
     } else {
       acc = *reinterpret_cast<const int4*>(smem + (at - sb));
     }
-    const float sx = __ldg(a.sx + m);
-    const int s4[4] = {acc.x, acc.y, acc.z, acc.w};
-    float y[4];
+    float y[4] = {(float)acc.x, (float)acc.y, (float)acc.z, (float)acc.w};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      y[e] = 0.f;
-      if (n + e < a.N) {
-        const float b = (a.epi & I8_BIAS) ? ld_param(reinterpret_cast<const T*>(a.bias) + n + e) : 0.f;
-        y[e] = fmaf((float)s4[e] * sx, i8_wscale(a, n + e), b);
-        if (GELU) y[e] = i8_gelu(y[e]);
-        else if (a.epi & I8_RESID) y[e] += ld_param(reinterpret_cast<const T*>(a.resid) + (size_t)m * a.N + n + e);
+    for (int e = 0; e < 4; ++e) y[e] = fmaf(y[e] * sx, sw[e], bias[e]);
+    if (GELU) {
+#pragma unroll
+      for (int e = 0; e < 4; e += 2) {
+        uint32_t g0, g1;
+        unpack64(i8_gelu2(pack64(__float_as_uint(y[e]), __float_as_uint(y[e + 1]))), g0, g1);
+        y[e] = __uint_as_float(g0);
+        y[e + 1] = __uint_as_float(g1);
       }
     }
-    T* out = reinterpret_cast<T*>(a.out) + (size_t)m * a.N + n;
+    const size_t o = (size_t)m * a.N + n;
+    const T* res = reinterpret_cast<const T*>(a.resid) + o;
+    T* out = reinterpret_cast<T*>(a.out) + o;
     if (a.vec) {
+      if (!GELU && (a.epi & I8_RESID)) {
+        const uint2 r = *reinterpret_cast<const uint2*>(res);
+        const float2 r0 = Act<T>::unpack2(r.x), r1 = Act<T>::unpack2(r.y);
+        y[0] += r0.x; y[1] += r0.y; y[2] += r1.x; y[3] += r1.y;
+      }
       *reinterpret_cast<uint2*>(out) = make_uint2(Act<T>::pack2(y[0], y[1]), Act<T>::pack2(y[2], y[3]));
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (n + e < a.N) out[e] = Act<T>::from_f(y[e]);
+        if (n + e < a.N) {
+          if (!GELU && (a.epi & I8_RESID)) y[e] += ld_param(res + e);
+          out[e] = Act<T>::from_f(y[e]);
+        }
     }
   }
   if (S > 1) cluster_sync();  // the partials stay until every CTA of the cluster has read them

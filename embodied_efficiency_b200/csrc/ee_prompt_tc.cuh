@@ -151,24 +151,6 @@ EE_DEV bool prompt_item(const PromptTcArgs& a, int idx, int units, PromptItem& i
   return true;
 }
 
-// Packed pairs of fp32 (one instruction for two values)
-EE_DEV uint64_t pack64(uint32_t lo, uint32_t hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
-  return r;
-}
-EE_DEV void unpack64(uint64_t v, uint32_t& lo, uint32_t& hi) { asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v)); }
-EE_DEV uint64_t both(float x) { return pack64(__float_as_uint(x), __float_as_uint(x)); }
-EE_DEV uint64_t fma2f(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-EE_DEV uint64_t add2f(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 EE_DEV float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));

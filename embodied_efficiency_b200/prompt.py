@@ -79,6 +79,12 @@ def rotary_embed(q, k, positions, sections, base: float = 10000.0, interleaved: 
     ``positions`` is int32 or int64 [axes, T] ([T] for one axis); angles stay exact to the last bits of fp32 at any
     position. Returns (q, k) turned, as new tensors or in ``out`` = (q_out, k_out), which may be the inputs
     themselves. head_dim 32, 64, 128 or 256; bf16 / fp16."""
+    if out is None and q is not None and k is not None:
+        tab = _TURNS.get((q.device, q.shape[-1] // 2, base))
+        if tab is not None:
+            done = (_lib._native or _lib.native()).rotary_embed(q, k, positions, sections, tab, interleaved)
+            if done is not None:
+                return done
     one = q if q is not None else k
     if one is None:
         raise ValueError("rotary_embed needs q or k")
@@ -141,6 +147,10 @@ def prompt_attention(q, k, v, cu_q, cu_k=None, k_lens=None, causal: bool = True,
     head_dim^-0.5. Offsets are int32 on the device, not decreasing; what they claim beyond the tensors is cut off.
     Returns [Tq, heads, head_dim], new or ``out``; rows that belong to no sequence are not written.
     head_dim 64 or 128; bf16 / fp16."""
+    if out is None:
+        done = (_lib._native or _lib.native()).prompt_attention(q, k, v, cu_q, cu_k, k_lens, causal, scale)
+        if done is not None:
+            return done
     if k.shape != v.shape or q.dtype != k.dtype or q.dtype != v.dtype:
         raise ValueError(f"q {q.dtype}, k {k.dtype} {tuple(k.shape)} and v {v.dtype} {tuple(v.shape)} do not match")
     if q.dim() != 3 or k.dim() != 3 or q.shape[2] != k.shape[2]:

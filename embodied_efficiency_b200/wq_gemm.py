@@ -194,6 +194,9 @@ def quantize_tokens(x):
     """int8 codes [..., K] and fp32 scales [..., 1] of bf16 / fp16 activations, one scale per token:
     ``scale = max(amax |x| / 127, 1e-8)``, ``code = rint(x / scale)`` (``ee_quantize_tokens``). A token that holds an
     infinity or NaN gets codes of 0 and a NaN scale. K is a multiple of 16."""
+    done = (_lib._native or _lib.native()).quantize_tokens(x)
+    if done is not None:
+        return done
     if x.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError(f"activations must be bf16 or fp16, not {x.dtype}")
     k = x.shape[-1]
@@ -216,6 +219,9 @@ def int8_matmul(xq, x_scale, weight, scales, bias=None, dtype=torch.bfloat16, ge
     32-bit integer sum, fp32 after it and one rounding to ``dtype`` (``ee_int8_gemm``). ``x_scale`` holds one fp32 value
     per token (``quantize_tokens``), ``scales`` one fp32 or fp16 value per output channel. ``gelu`` (exact erf GELU) or
     ``residual`` are applied in fp32 before that rounding. No backward pass."""
+    y = (_lib._native or _lib.native()).int8_matmul(xq, x_scale, weight, scales, bias, gelu, residual, dtype)
+    if y is not None:
+        return y
     k = xq.shape[-1]
     if xq.dtype != torch.int8:
         raise ValueError(f"xq must be int8, not {xq.dtype}")
@@ -242,6 +248,9 @@ def int8_linear(x, weight, scales, bias=None, gelu=False, residual=None):
     """A linear on the 8-bit integer tensor cores: bf16 / fp16 ``x`` [..., K] quantised per token as in
     ``quantize_tokens``, then ``int8_matmul`` with ``weight`` int8 [N, K] and one scale per output channel, to
     ``x.dtype`` (``ee_int8_linear``, one call). No backward pass."""
+    y = (_lib._native or _lib.native()).int8_linear(x, weight, scales, bias, gelu, residual)
+    if y is not None:
+        return y
     k = x.shape[-1]
     out_shape = (x.shape[0], weight.shape[0]) if x.dim() == 2 else (*x.shape[:-1], weight.shape[0])
     n = _check_int8_operands(weight, scales, bias, residual, k, x.dtype, out_shape)
