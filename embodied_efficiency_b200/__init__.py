@@ -18,7 +18,7 @@ The compute lives in lib/libee_b200.so (C ABI: include/ee_b200.h).
 from .quant import dequantize_weight, quantize_weight, quantize_weight_asym4
 from .wq_gemm import (TritonQuantLinear, _pack_int4, _unpack_int4, correctness_check, int8_linear, int8_matmul,
                       quantize_model_triton, quantize_tokens, wq_linear)
-from .expert import ActionExpert, ActionExpertConfig, Block, flow_sample, sample, timestep_embedding
+from .expert import ActionExpert, ActionExpertConfig, Block, PackedKV, flow_sample, sample, timestep_embedding
 from .graphed import GraphedSampler
 from .prompt import prompt_attention, rotary_embed
 
@@ -26,4 +26,4 @@ __all__ = ["quantize_weight", "dequantize_weight", "quantize_weight_asym4", "Tri
            "_pack_int4", "_unpack_int4", "wq_linear", "quantize_model_triton", "correctness_check",
            "ActionExpert", "ActionExpertConfig", "Block", "flow_sample", "sample",
            "timestep_embedding", "GraphedSampler", "quantize_tokens", "int8_matmul", "int8_linear",
-           "rotary_embed", "prompt_attention"]
+           "rotary_embed", "prompt_attention", "PackedKV"]

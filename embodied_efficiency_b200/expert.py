@@ -21,6 +21,7 @@ import torch.nn.functional as F
 
 from . import _lib
 from . import fused as _fused
+from .prompt import prompt_attention
 from .wq_gemm import wq_linear
 
 
@@ -185,6 +186,27 @@ def _apply_linear(mod, x, gelu: bool = False, residual=None):
     return y if residual is None else residual + y
 
 
+class PackedKV:
+    """One block's K / V of prefixes of different lengths, one behind another without padding: ``k`` and ``v``
+    [tokens, heads, head_dim], views of one kv_c output, and the int32 offsets ``cu`` [batch + 1] of their first rows."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor):
+        self.k, self.v, self.cu = k, v, cu
+        self._cu_q = None
+
+    def queries(self, b: int, n: int) -> torch.Tensor:
+        """Offsets of ``n`` action tokens per prefix."""
+        if b != self.cu.numel() - 1:
+            raise ValueError(f"{self.cu.numel() - 1} packed prefixes for a batch of {b}")
+        if self._cu_q is None or self._cu_q[0] != n:
+            self._cu_q = (n, torch.arange(0, (b + 1) * n, n, dtype=torch.int32, device=self.cu.device))
+        return self._cu_q[1]
+
+
+def _is_packed(prefix_kv) -> bool:
+    return len(prefix_kv) > 0 and isinstance(prefix_kv[0], PackedKV)
+
+
 class Block(nn.Module):
     """kernel/flow_expert.py:51-95: pre-norm self-attention over the action chunk
     (optional), cross-attention to the cached prefix, GELU MLP."""
@@ -223,6 +245,12 @@ class Block(nn.Module):
         k, v = _apply_linear(self.kv_c, prefix).chunk(2, dim=-1)
         return self._split(k), self._split(v)
 
+    def precompute_kv_packed(self, prefix: torch.Tensor, cu: torch.Tensor) -> PackedKV:
+        """The same for packed prefixes [tokens, D] with offsets ``cu``."""
+        _lib.require_cuda(prefix)
+        k, v = _apply_linear(self.kv_c, prefix).chunk(2, dim=-1)
+        return PackedKV(k.unflatten(-1, (self.h, self.hd)), v.unflatten(-1, (self.h, self.hd)), cu)
+
     def forward(self, x: torch.Tensor, kv_c):
         """Eager GPU composition (used only where the fused launch does not apply)."""
         _lib.require_cuda(x)
@@ -238,6 +266,11 @@ class Block(nn.Module):
                 a = self._merge(F.scaled_dot_product_attention(self._split(q), self._split(k), self._split(v)))
             x = _apply_linear(self.proj, a, residual=x)
         qc = _apply_linear(self.q_c, _apply_norm(self.nx, x))
+        if isinstance(kv_c, PackedKV):
+            a = prompt_attention(qc.reshape(b * n, self.h, hd), kv_c.k, kv_c.v, kv_c.queries(b, n), kv_c.cu,
+                                 causal=False).view(b, n, d)
+            x = _apply_linear(self.out_c, a, residual=x)
+            return _apply_linear(self.mlp[2], _apply_linear(self.mlp[0], _apply_norm(self.n2, x), gelu=True), residual=x)
         k, v = kv_c
         a = None
         p = k.shape[2]
@@ -277,6 +310,13 @@ class ActionExpert(nn.Module):
         prefix = prefix.to(self.out_norm.weight.dtype)
         return [blk.precompute_kv(prefix) for blk in self.blocks]
 
+    def encode_packed(self, prefix: torch.Tensor, cu: torch.Tensor):
+        """Per-layer K/V of prefixes of different lengths: packed rows [tokens, d] and their int32 offsets
+        ``cu`` [batch + 1] on the device. ``flow_sample`` and ``GraphedSampler`` take the result in place of
+        ``encode``'s and run layer by layer, the cross-attention on ``prompt_attention``."""
+        prefix = prefix.to(self.out_norm.weight.dtype)
+        return [blk.precompute_kv_packed(prefix, cu) for blk in self.blocks]
+
     def plan(self, batch: int, prefix_kv):
         """The fused-launch plan for this batch and prefix K/V (built once, cached)."""
         return get_plan(self, batch, prefix_kv)
@@ -285,7 +325,7 @@ class ActionExpert(nn.Module):
         """kernel/flow_expert.py:117-124: velocity for x_act [B,H,A] at times t [B]."""
         _lib.require_cuda(x_act)
         b = x_act.shape[0]
-        if _fused.preferred(self, b, FUSED_MAX_TOKENS):
+        if not _is_packed(prefix_kv) and _fused.preferred(self, b, FUSED_MAX_TOKENS):
             v = self.plan(b, prefix_kv).run(x_act, 1, t0=t, mode=_lib.EE_MODE_VELOCITY)
             return v.to(x_act.dtype)
         return self.forward_layers(x_act, t, prefix_kv)
@@ -350,7 +390,7 @@ def flow_sample(expert, x_init: torch.Tensor, n_steps: int, prefix_kv, path: str
     """
     _lib.require_cuda(x_init)
     b = x_init.shape[0]
-    fused_ok = _fused.supports(expert, b)
+    fused_ok = not _is_packed(prefix_kv) and _fused.supports(expert, b)
     if path == "fused" and not fused_ok:
         raise ValueError("the fused launch does not cover this expert / batch")
     use_fused = fused_ok and (path == "fused" or (path == "auto" and _fused.preferred(expert, b, FUSED_MAX_TOKENS)))

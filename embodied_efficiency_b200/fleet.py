@@ -50,7 +50,9 @@ class FleetShard:
 class FleetSampler:
     """Runs this rank's block of a fleet of ``n_requests`` sampler requests.
 
-    ``request_fn(i)`` returns request i's (prefix [1, P, d], noise [1, H, A])
+    ``request_fn(i)`` returns request i's (prefix [1, P, d], noise [1, H, A]);
+    with an ``expert``, P may differ between the requests of a chunk, whose
+    prefixes are then packed without padding (``ActionExpert.encode_packed``)
     (the caller decides where requests come from; ``synth.fleet_request``
     gives the seeded synthetic fleet). With an
     ``expert`` the chunks run through ``flow_sample`` (one fused launch per
@@ -77,7 +79,9 @@ class FleetSampler:
         staged = []
         for a, b in chunk_bounds(self.lo, self.hi, self.chunk):
             reqs = [request_fn(i) for i in range(a, b)]
-            pre = torch.cat([r[0] for r in reqs], 0)
+            lens = [r[0].shape[1] for r in reqs]
+            packed = self.expert is not None and len(set(lens)) > 1  # prompts of different lengths
+            pre = torch.cat([r[0][0] if packed else r[0] for r in reqs], 0)
             x0 = torch.cat([r[1] for r in reqs], 0)
             if self.device is not None:
                 pre, x0 = pre.to(self.device), x0.to(self.device)
@@ -85,7 +89,11 @@ class FleetSampler:
             if self.expert is not None:
                 dt = self.expert.out_norm.weight.dtype
                 pre, x0 = pre.to(dt), x0.to(dt)
-                kv = self.expert.encode(pre)
+                if packed:
+                    cu = torch.tensor([0] + lens, device=pre.device).cumsum(0).to(torch.int32)
+                    kv = self.expert.encode_packed(pre, cu)
+                else:
+                    kv = self.expert.encode(pre)
             staged.append((a, b, pre, x0, kv))
         self._inputs = staged
         self._graphs = None

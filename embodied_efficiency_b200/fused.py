@@ -55,6 +55,10 @@ def supports(expert, batch: int) -> bool:
             for m in mods:
                 if not (isinstance(m, nn.Linear) or _is_quant_linear(m) or _is_ref_quantlinear(m)):
                     return False
+                if getattr(m, "act_bits", 16) != 16:  # the launch multiplies 16-bit activations
+                    return False
+        if getattr(expert.t_proj, "act_bits", 16) != 16:
+            return False
         return isinstance(expert.in_proj, nn.Linear) and isinstance(expert.out_proj, nn.Linear)
     except AttributeError:
         return False
@@ -201,6 +205,8 @@ class FusedPlan:
         r = _lib.Linear()
         bias = getattr(m, "bias", None)
         r.bias = self._act_tensor(bias.detach()).data_ptr() if bias is not None else 0
+        if getattr(m, "act_bits", 16) != 16:
+            raise ValueError("the fused launch does not cover linears with 8-bit activations")
         if _is_quant_linear(m):
             r.weight = self._own(m.weight.contiguous()).data_ptr()
             r.scales = self._own(m.scales.float().contiguous()).data_ptr()

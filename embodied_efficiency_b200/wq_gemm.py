@@ -321,11 +321,25 @@ class TritonQuantLinear(nn.Module):
     ``bias``, ``bits``, ``group_size``, ``in_features``, ``out_features``) so
     that callers such as ``compiler._weight_mb`` see the same module; the
     forward runs the sm_100a dequant-GEMM.
+
+    ``act_bits=8`` (with ``bits=8``; not in the reference) quantises the
+    activations too, one scale per token, and multiplies on the integer tensor
+    cores (``int8_linear``): the weights then have one scale per output
+    channel, whatever ``group_size`` says, and no dense copy is ever made.
+    Buffers and ``state_dict`` are those of a per-channel int8 module.
     """
 
-    def __init__(self, lin: nn.Linear, bits: int = 8, group_size: int = 128):
+    def __init__(self, lin: nn.Linear, bits: int = 8, group_size: int = 128, act_bits: int = 16):
         super().__init__()
         assert bits in (4, 8)
+        if act_bits not in (8, 16):
+            raise ValueError(f"act_bits must be 8 or 16, got {act_bits}")
+        if act_bits == 8:
+            if bits != 8 or lin.in_features % 16 or lin.in_features > 131056:
+                raise ValueError("act_bits=8 needs bits=8 and in_features a multiple of 16, at most 131056, "
+                                 f"got bits={bits}, in_features={lin.in_features}")
+            group_size = lin.in_features
+        self.act_bits = act_bits
         q3, scale3, gs = quantize_weight(lin.weight.data.float(), bits, group_size)
         out, ng, g = q3.shape
         q2d = q3.reshape(out, ng * g).to(torch.int8)
@@ -362,7 +376,12 @@ class TritonQuantLinear(nn.Module):
         """``wq_linear`` with this module's buffers (and the fused epilogues);
         from ``DENSE_MIN_TOKENS`` bf16 / fp16 tokens on, on the dense copy of
         the weight -- the same products, so the same results up to the
-        GEMM's accumulation order. Never builds the copy during stream capture."""
+        GEMM's accumulation order. Never builds the copy during stream capture.
+        With ``act_bits=8`` every call is ``int8_linear`` (fp32 activations in bf16, as ``wq_linear`` takes them)."""
+        if self.act_bits == 8:
+            act = x.dtype if x.dtype in (torch.bfloat16, torch.float16) else torch.bfloat16
+            r = None if residual is None else residual.detach().to(act)
+            return int8_linear(x.detach().to(act), self.weight, self.scales, self.bias, gelu, r).to(x.dtype)
         m = x.numel() // self.in_features if self.in_features else 0
         if (DENSE_MIN_TOKENS is not None and x.is_cuda and x.dtype in (torch.bfloat16, torch.float16)
                 and m >= DENSE_MIN_TOKENS
@@ -380,19 +399,21 @@ class TritonQuantLinear(nn.Module):
         return self.out_features * self.in_features * self.bits / 8.0 + self.scales.numel() * 2
 
     def extra_repr(self):
-        return f"in={self.in_features}, out={self.out_features}, bits={self.bits}, group={self.group_size}"
+        act = "" if self.act_bits == 16 else f", act_bits={self.act_bits}"
+        return f"in={self.in_features}, out={self.out_features}, bits={self.bits}, group={self.group_size}{act}"
 
 
-def quantize_model_triton(model, bits=8, group_size=128, skip=("in_proj", "out_proj")):
+def quantize_model_triton(model, bits=8, group_size=128, skip=("in_proj", "out_proj"), act_bits=16):
     """kernel/triton_gemm.py:187-195: swap every nn.Linear except ``skip`` for
-    ``TritonQuantLinear``, recursively; returns the mutated model."""
+    ``TritonQuantLinear``, recursively; returns the mutated model. With
+    ``act_bits=8`` the activations are quantised too (see there)."""
     for name, mod in list(model.named_children()):
         if name in skip:
             continue
         if isinstance(mod, nn.Linear):
-            setattr(model, name, TritonQuantLinear(mod, bits, group_size))
+            setattr(model, name, TritonQuantLinear(mod, bits, group_size, act_bits))
         else:
-            quantize_model_triton(mod, bits, group_size, skip)
+            quantize_model_triton(mod, bits, group_size, skip, act_bits)
     return model
 
 
