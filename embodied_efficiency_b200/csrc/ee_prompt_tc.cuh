@@ -57,9 +57,10 @@ constexpr int kPtThreads = 384;
 constexpr int kPtRegsLaunch = 168, kPtRegsSoft = 208, kPtRegsRest = 88;
 static_assert(256 * kPtRegsSoft + 128 * kPtRegsRest <= kPtThreads * kPtRegsLaunch, "the register shares fit the launch");
 constexpr int kPtKeys = 128, kPtInfo = 4, kPtLoads = 8;  // keys per block; items published, loads of K / V ahead
-template <int HD> constexpr int pt_slots() { return HD == 128 ? 5 : 8; }
+template <int HD> constexpr int pt_slots() { return HD == 128 ? 4 : 8; }
 template <int HD> constexpr uint32_t pt_tile() { return 128u * HD * 2; }
-template <int HD> constexpr uint32_t pt_off_bar() { return (2 + pt_slots<HD>()) * pt_tile<HD>(); }
+template <int HD> constexpr uint32_t pt_off_out() { return (2 + pt_slots<HD>()) * pt_tile<HD>(); }  // 4 KB per softmax warp
+template <int HD> constexpr uint32_t pt_off_bar() { return pt_off_out<HD>() + 8 * 4096; }
 // barriers: full / empty per load of K / V, Q full / empty, S / P (two halves) / S free / O / O free per tile, V to fix / fixed, item full / empty
 template <int HD> constexpr uint32_t pt_off_info() { return pt_off_bar<HD>() + 8 * (2 * kPtLoads + 16 + 2 * kPtInfo) + 8; }
 template <int HD> constexpr uint32_t pt_smem() { return pt_off_info<HD>() + kPtInfo * 64 + 1024; }
@@ -441,7 +442,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       if (it->nbm < 0) break;
       const int nt = it->n[t], qlen = it->qlen, klen = it->klen, key0 = it->key0;
       const int tok = it->tok + t * a.tpt + rtok, head = it->kvh * p.group + rhead;
-      const long long out_row = (long long)it->q0 + tok;
+      const int out_row = it->q0 + tok;
       const int part = it->part;
       __syncwarp();
       if (lane == 0) item_done(i);
@@ -540,35 +541,56 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       tc_fence_after();
       const bool whole = p.splits == 1;
       const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees no key is zero
-      T* out = reinterpret_cast<T*>(p.out) + out_row * p.o_tok + head * p.o_head;
       const long long at = ((long long)part * p.tq + out_row) * p.n_q + head;
       if (!whole && mine) *reinterpret_cast<float2*>(p.stat + 2 * at) = make_float2(m, l);
+      // the element a lane's row starts at, -1 for a row that is not there
+      const long long row_at = mine ? (long long)out_row * p.o_tok + head * p.o_head : -1;
+      const uint32_t stg = sb + pt_off_out<HD>() + warp * 4096;
 #pragma unroll
-      for (int c = 0; c < HD / 32; ++c) {
-        uint32_t o[32];
-        if (nt > 0) {
-          tmem_ld32(to + 32 * c, o);
-          tmem_wait_ld();
-          if (c == HD / 32 - 1) {  // O has been read: the next item may start over
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(b_of + 8 * t);
+      for (int c = 0; c < HD / 64; ++c) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t o[32];
+          if (nt > 0) {
+            tmem_ld32(to + 64 * c + 32 * h, o);
+            tmem_wait_ld();
+            if (c == HD / 64 - 1 && h == 1) {  // O has been read: the next item may start over
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(b_of + 8 * t);
+            }
+          }
+          if (whole) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              uint32_t w[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                w[k] = l == 0.f ? 0u
+                                : Act<T>::pack2(__uint_as_float(o[8 * e + 2 * k]) * inv,
+                                                __uint_as_float(o[8 * e + 2 * k + 1]) * inv);
+              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(stg + sw128(lane, 4 * h + e)), "r"(w[0]),
+                           "r"(w[1]), "r"(w[2]), "r"(w[3])
+                           : "memory");
+            }
+          } else if (mine && l != 0.f) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<uint4*>(p.part + at * HD + 64 * c + 32 * h + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
           }
         }
-        if (mine && whole) {
+        if (whole) {
+          // 64 columns of the warp's rows from shared memory: a lane's own row would be 16 bytes of 32 lines a store
+          __syncwarp();
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            uint32_t w[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              w[k] = l == 0.f ? 0u
-                              : Act<T>::pack2(__uint_as_float(o[e + 2 * k]) * inv, __uint_as_float(o[e + 2 * k + 1]) * inv);
-            *reinterpret_cast<uint4*>(out + 32 * c + e) = make_uint4(w[0], w[1], w[2], w[3]);
+          for (int e = 0; e < 8; ++e) {
+            const int rr = 4 * e + (lane >> 3);
+            const long long base = __shfl_sync(0xffffffffu, row_at, rr);
+            if (base >= 0)
+              *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + base + 64 * c + 8 * (lane & 7)) =
+                  lds16(stg + sw128(rr, lane & 7));
           }
-        } else if (mine && l != 0.f) {
-#pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            *reinterpret_cast<uint4*>(p.part + at * HD + 32 * c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          __syncwarp();
         }
       }
     }
