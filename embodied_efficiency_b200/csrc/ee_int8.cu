@@ -3,6 +3,7 @@
 //   y[m][n] = epi( (sum_k xq[m][k] * w[n][k]) * sx[m] * sw[n] + bias[n] ),
 // and the token quantiser xq = rint(x / sx), sx = max(amax |x| / 127, 1e-8).
 #include <atomic>
+#include <cmath>
 
 #include "ee_host.h"
 #include "ee_int8_tc.cuh"
@@ -185,16 +186,32 @@ static int launch_few(Int8Args a, const int8_t* xq, const int8_t* w, int split, 
   return cudaLaunchKernelEx(&cfg, fn, tx, tw, a) == cudaSuccess ? EE_OK : EE_ERR_LAUNCH;
 }
 
-// Which kernel: the token tile NT (0: the pair kernel) and the K split.
+// Which kernel: the token tile NT (0: the pair kernel) and the K split, by a
+// cost in microseconds fitted to measurements of both kernels: a fixed part
+// (launch, first loads, epilogue) and, per wave of CTAs and 128-byte k-block,
+// the time its operands take to arrive. It tells 18 from 34 us (1000 x 4096 x
+// 4096: pairs, few), 10 from 12 (1600 x 1024 x 1024: pairs, few), 16 from 10
+// (512 x 1024 x 4096: pairs, few over 4 slices of K) and 10 from 9 (1023 x
+// 1000 x 1040: 128-token tiles, 64-token tiles).
 struct Int8Plan { int nt, split; };
 static Int8Plan int8_plan(int m, int n, int k, int sms) {
-  const int nkb = (k + 127) / 128;
-  const int nt = m <= 16 ? 16 : (m <= 32 ? 32 : (m <= 64 ? 64 : 128));
-  const long long units = (long long)((n + 127) / 128) * ((m + nt - 1) / nt);
-  if (m > 128 && units > 2 * sms) return {0, 1};
-  int split = 1;
-  while (split < 8 && units * split * 2 <= sms && split * 2 <= nkb) split *= 2;
-  return {nt, split};
+  const int nkb = (k + 127) / 128, tiles_n = (n + 127) / 128;
+  auto waves = [](double items, double slots) { return std::ceil(items / slots); };
+  Int8Plan best{0, 1};
+  double cost = 7.4 + 0.275 * nkb * waves(std::ceil(m / 256.0) * std::ceil(n / 256.0), sms / 2);
+  if (m <= 64) cost = 1e30;  // a quarter of a pair's tokens or fewer: the other kernel's tiles fit
+  static const struct { int nt; double fixed; } tiles[4] = {{16, 5.4}, {32, 6.3}, {64, 7.2}, {128, 8.3}};
+  for (const auto& t : tiles) {
+    const double units = (double)tiles_n * std::ceil(m / (double)t.nt), per = 0.28 * (16 + t.nt / 8.0) / 32;
+    for (int s = 1; s <= 8 && s <= nkb && (s == 1 || units * s <= sms); s *= 2) {
+      const double c = t.fixed + (s > 1 ? 0.4 : 0.0) + per * waves(units * s, sms) * ((nkb + s - 1) / s);
+      if (c < cost) {
+        cost = c;
+        best = {t.nt, s};
+      }
+    }
+  }
+  return best;
 }
 
 template <typename T, bool GELU>
