@@ -98,43 +98,51 @@ EE_DEV float ex2(float x) {
   return y;
 }
 
-// Item `idx` (unit-major from the last unit down, key heads and parts inside):
-// the whole warp searches, 32 sequences at a time. False past the last item.
-EE_DEV bool prompt_item(const PromptTcArgs& a, int idx, int units, PromptItem& it) {
+// The 32 sequences in which the last item was found: a CTA's items come in
+// order of descending units, so the search only ever moves down from there.
+struct PromptWindow {
+  int base, before;  // first sequence; units before it
+};
+// The window's sequences, one a lane, and the units up to and including each.
+EE_DEV int prompt_window(const PromptTcArgs& a, const PromptWindow& w, PromptSeq& s, int& nu) {
+  const int lane = threadIdx.x & 31, b = w.base + lane;
+  s = PromptSeq{};
+  if (b < a.p.n_seq) s = prompt_seq(a.p, b);
+  nu = (s.qlen + 2 * a.tpt - 1) / (2 * a.tpt);
+  int inc = nu;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += t;
+  }
+  return inc;
+}
+
+// Item `idx` (unit-major from the last unit down, key heads and parts inside),
+// by the whole warp. False past the last item.
+EE_DEV bool prompt_item(const PromptTcArgs& a, int idx, int units, PromptWindow& w, PromptItem& it) {
   const PromptArgs& p = a.p;
-  const int lane = threadIdx.x & 31, per = p.n_kv * p.splits;
+  const int per = p.n_kv * p.splits;
   const int unit = units - 1 - idx / per;
   if (unit < 0) return false;
   it.kvh = idx % per / p.splits;
   it.part = idx % p.splits;
-  int before = 0;
-  for (int b0 = 0; b0 < p.n_seq; b0 += 32) {
-    const int b = b0 + lane;
-    PromptSeq s{};
-    int nu = 0;
-    if (b < p.n_seq) {
-      s = prompt_seq(p, b);
-      nu = (s.qlen + 2 * a.tpt - 1) / (2 * a.tpt);
-    }
-    int inc = nu;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int t = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += t;
-    }
-    inc += before;
-    const unsigned hit = __ballot_sync(0xffffffffu, unit >= inc - nu && unit < inc);
-    if (hit) {
-      const int src = __ffs(hit) - 1;
-      it.q0 = __shfl_sync(0xffffffffu, s.q0, src);
-      it.qlen = __shfl_sync(0xffffffffu, s.qlen, src);
-      it.k0 = __shfl_sync(0xffffffffu, s.k0, src);
-      it.klen = __shfl_sync(0xffffffffu, s.klen, src);
-      it.tok = (unit - __shfl_sync(0xffffffffu, inc - nu, src)) * 2 * a.tpt;
-      break;
-    }
-    before = __shfl_sync(0xffffffffu, inc, 31);
+  PromptSeq s;
+  int nu, inc = prompt_window(a, w, s, nu);
+  while (unit < w.before && w.base > 0) {
+    w.base -= 32;
+    inc = prompt_window(a, w, s, nu);
+    w.before -= __shfl_sync(0xffffffffu, inc, 31);
   }
+  inc += w.before;
+  const unsigned hit = __ballot_sync(0xffffffffu, unit >= inc - nu && unit < inc);
+  if (!hit) return false;  // the offsets have changed meanwhile
+  const int src = __ffs(hit) - 1;
+  it.q0 = __shfl_sync(0xffffffffu, s.q0, src);
+  it.qlen = __shfl_sync(0xffffffffu, s.qlen, src);
+  it.k0 = __shfl_sync(0xffffffffu, s.k0, src);
+  it.klen = __shfl_sync(0xffffffffu, s.klen, src);
+  it.tok = (unit - __shfl_sync(0xffffffffu, inc - nu, src)) * 2 * a.tpt;
   int nb[2];
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
@@ -230,13 +238,20 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       bool ok = true;
       int units = 0, n = 0, nq = 0, sl = 0;  // K / V tiles and Q loads issued so far, next slot
       uint32_t g = 0, slot_load[NS];         // loads (barrier phases) of K / V so far, and each slot's last one
+#pragma unroll 4
       for (int b = lane; b < p.n_seq; b += 32) units += (prompt_seq(p, b).qlen + 2 * a.tpt - 1) / (2 * a.tpt);
       units = __reduce_add_sync(0xffffffffu, units);
+      PromptWindow window{(p.n_seq - 1) / 32 * 32, 0};
+      {
+        PromptSeq s;
+        int nu;
+        window.before = units - __shfl_sync(0xffffffffu, prompt_window(a, window, s, nu), 31);
+      }
       const uint32_t qbytes = (uint32_t)(p.group * a.tpt) * 128u * PANELS;
       for (int i = 0;; ++i) {
         const long long idx = (long long)i * gridDim.x + ((i & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
         PromptItem it{};
-        const bool more = ok && idx < (long long)units * p.n_kv * p.splits && prompt_item(a, (int)idx, units, it);
+        const bool more = ok && idx < (long long)units * p.n_kv * p.splits && prompt_item(a, (int)idx, units, window, it);
         if (lane == 0) {
           if (i >= kPtInfo && ok && !mbar_wait(b_ie + 8 * (i % kPtInfo), (uint32_t)((i / kPtInfo - 1) & 1), a.timeout_ns))
             ok = false;

@@ -79,8 +79,8 @@ class FleetSampler:
         staged = []
         for a, b in chunk_bounds(self.lo, self.hi, self.chunk):
             reqs = [request_fn(i) for i in range(a, b)]
-            lens = [r[0].shape[1] for r in reqs]
-            packed = self.expert is not None and len(set(lens)) > 1  # prompts of different lengths
+            lens = [r[0].shape[1] for r in reqs] if self.expert is not None else []
+            packed = len(set(lens)) > 1  # prompts of different lengths
             pre = torch.cat([r[0][0] if packed else r[0] for r in reqs], 0)
             x0 = torch.cat([r[1] for r in reqs], 0)
             if self.device is not None:

@@ -57,6 +57,9 @@ def _turns(device, half: int, base: float) -> torch.Tensor:
     key = (device, half, base)
     tab = _TURNS.get(key)
     if tab is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"rotary_embed copies its frequencies (head_dim {2 * half}, base {base}) to the device on "
+                               "first use: call it once before the stream capture")
         vals = [int(round(math.ldexp(base ** (-i / half) / (2.0 * math.pi), 64))) & (2 ** 64 - 1) for i in range(half)]
         host = torch.tensor([v - 2 ** 64 if v >= 2 ** 63 else v for v in vals], dtype=torch.int64)
         tab = _TURNS[key] = host.to(device)
@@ -78,7 +81,8 @@ def rotary_embed(q, k, positions, sections, base: float = 10000.0, interleaved: 
     ``sections[1]`` by axis 1 and so on. Pairs are (i, i + head_dim / 2), or (2i, 2i + 1) when ``interleaved``.
     ``positions`` is int32 or int64 [axes, T] ([T] for one axis); angles stay exact to the last bits of fp32 at any
     position. Returns (q, k) turned, as new tensors or in ``out`` = (q_out, k_out), which may be the inputs
-    themselves. head_dim 32, 64, 128 or 256; bf16 / fp16."""
+    themselves. head_dim 32, 64, 128 or 256; bf16 / fp16. The first call for a head_dim and base on a device copies a
+    small table to it and has to come before a stream capture."""
     if out is None and q is not None and k is not None:
         tab = _TURNS.get((q.device, q.shape[-1] // 2, base))
         if tab is not None:

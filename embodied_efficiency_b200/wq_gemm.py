@@ -329,6 +329,8 @@ class TritonQuantLinear(nn.Module):
     Buffers and ``state_dict`` are those of a per-channel int8 module.
     """
 
+    act_bits = 16  # modules pickled before there was a choice
+
     def __init__(self, lin: nn.Linear, bits: int = 8, group_size: int = 128, act_bits: int = 16):
         super().__init__()
         assert bits in (4, 8)

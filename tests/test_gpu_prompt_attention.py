@@ -1,4 +1,6 @@
 """GPU parity of attention over packed prompts (ee_prompt_attention) against its definition in 64 bits."""
+import random
+
 import pytest
 import torch
 
@@ -64,6 +66,32 @@ def test_prompts(cuda, dtype, hq, hk, hd, lens, causal):
     out = prompt_attention(q, k, v, _cu(lens, cuda), causal=causal)
     assert out.shape == q.shape and out.dtype == dtype
     _check(out, q, k, v, lens, lens, causal, hd ** -0.5)
+
+
+@pytest.mark.parametrize("hq,hk,hd", [(8, 8, 64), (4, 2, 128), (12, 4, 64)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_more_items_than_sms(cuda, hq, hk, hd, causal):
+    """Several items per CTA, one after another: lengths on both sides of the tiles, sequences without queries or
+    without keys among them."""
+    from embodied_efficiency_b200 import prompt_attention
+    r = random.Random(hq)
+    q_len = [r.choice([0, 1, 20, 64, 127, 128, 129, 200, 256, 257, 300]) for _ in range(90)]
+    k_len = [n if r.random() < 0.7 else r.choice([0, 1, n + 5, n + 128, max(n - 3, 0)]) for n in q_len]
+    q, k, v = _inputs(cuda, torch.bfloat16, sum(q_len), sum(k_len), hq, hk, hd, 5)
+    out = prompt_attention(q, k, v, _cu(q_len, cuda), _cu(k_len, cuda), causal=causal)
+    _check(out, q, k, v, q_len, k_len, causal, hd ** -0.5)
+
+
+@pytest.mark.parametrize("longest", [3, 40])
+def test_many_short_sequences(cuda, longest):
+    """More sequences than a CTA has threads, most of them tiny or empty."""
+    from embodied_efficiency_b200 import prompt_attention
+    r = random.Random(longest)
+    q_len = [0 if r.random() < 0.2 else r.randint(0 if longest < 9 else 20, longest) for _ in range(1300)]
+    k_len = [n + r.choice([0, 0, 1, 17, 70]) for n in q_len]
+    q, k, v = _inputs(cuda, torch.float16, sum(q_len), sum(k_len), 4, 2, 64, 6)
+    out = prompt_attention(q, k, v, _cu(q_len, cuda), _cu(k_len, cuda))
+    _check(out, q, k, v, q_len, k_len, True, 0.125)
 
 
 CACHED = [([1], [1]), ([1], [777]), ([1] * 5, [1, 128, 129, 4000, 0]), ([1] * 64, list(range(1, 1300, 20))[:64]),

@@ -85,3 +85,22 @@ def test_views_in_place_and_empty(cuda):
         again = rotary_embed(keep[:, :hq * hd].view(t, hq, hd), None, pos, (32,))[0]
     torch.cuda.synchronize()
     assert torch.equal(again, q2)
+
+
+def test_captured(cuda):
+    """The table of frequencies has to be there before a capture; replays follow the buffers."""
+    from embodied_efficiency_b200 import rotary_embed
+    q, pos = torch.randn(3, 2, 64, device=cuda).half(), torch.arange(3, device=cuda, dtype=torch.int32)
+    want = rotary_embed(q, q, pos, (32,))[0]
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        got = rotary_embed(q, q, pos, (32,))
+        with pytest.raises(RuntimeError, match="before the stream capture"):
+            rotary_embed(q, q, pos, (32,), base=77.0)
+    gr.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want) and torch.equal(got[1], want)
+    pos.add_(5)
+    gr.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], rotary_embed(q, q, pos, (32,))[0]) and not torch.equal(got[0], want)
