@@ -481,10 +481,15 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         const int left = lim - j * kPtKeys;
         if (__any_sync(0xffffffffu, left < kPtKeys)) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < 4; ++c) {
+            const int n = left - 32 * c;
+            if (__any_sync(0xffffffffu, n < 32)) {  // a bit per key: one predicated move a value instead of a comparison too
+              const uint32_t seen = n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u);
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (32 * c + e >= left) v[c][e] = 0xff800000u;
+              for (int e = 0; e < 32; ++e)
+                if (!(seen >> e & 1u)) v[c][e] = 0xff800000u;
+            }
+          }
         }
         float x[4];
 #pragma unroll
@@ -597,14 +602,18 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         if (whole) {
           // 64 columns of the warp's rows from shared memory: a lane's own row would be 16 bytes of 32 lines a store
           __syncwarp();
+          long long base[8];
+          uint4 line[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const int rr = 4 * e + (lane >> 3);
-            const long long base = __shfl_sync(0xffffffffu, row_at, rr);
-            if (base >= 0)
-              *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + base + 64 * c + 8 * (lane & 7)) =
-                  lds16(stg + sw128(rr, lane & 7));
+            base[e] = __shfl_sync(0xffffffffu, row_at, rr);
+            line[e] = lds16(stg + sw128(rr, lane & 7));
           }
+          T* out = reinterpret_cast<T*>(p.out) + 64 * c + 8 * (lane & 7);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (base[e] >= 0) *reinterpret_cast<uint4*>(out + base[e]) = line[e];
           __syncwarp();
         }
       }
