@@ -20,22 +20,29 @@ namespace ee {
 constexpr int kQChunks = 8;
 constexpr int kQThreads = 256;
 
-// nearest integer (ties to even) of the fp32 quotient v / s, as the low byte
-// of an int: t = v * (1 / s) is within 1.5 ulp of it, so only a t that close
-// to a tie is divided for
-EE_DEV uint32_t quant_word(const float (&v)[4], float s, float inv) {
-  uint32_t b[4];
-  bool near = false;
+// nearest integers (ties to even) of the fp32 quotients v / s of four values,
+// one byte each: t = v * (1 / s) is within 1.5 ulp of the quotient, so only a t
+// that close to a tie is divided for. In packed pairs, as the instructions per
+// value, not the bytes, bound a long row otherwise.
+EE_DEV uint32_t quant_word(uint64_t v01, uint64_t v23, float s, uint64_t inv2) {
+  const uint64_t magic = both(12582912.f), back = both(-12582912.f);  // 1.5 * 2^23: the sum's rounding is rint(t)
+  const uint64_t t01 = mul2f(v01, inv2), t23 = mul2f(v23, inv2);
+  uint64_t r01 = add2f(t01, magic), r23 = add2f(t23, magic);
+  // rint(t) - t, exact and at most 1/2
+  const uint64_t d01 = fma2f(t01, both(-1.f), add2f(r01, back)), d23 = fma2f(t23, both(-1.f), add2f(r23, back));
+  uint32_t d[4], b[4];
+  unpack64(d01, d[0], d[1]);
+  unpack64(d23, d[2], d[3]);
+  const float far = fmaxf(fmaxf(fabsf(__uint_as_float(d[0])), fabsf(__uint_as_float(d[1]))),
+                          fmaxf(fabsf(__uint_as_float(d[2])), fabsf(__uint_as_float(d[3]))));
+  unpack64(r01, b[0], b[1]);
+  unpack64(r23, b[2], b[3]);
+  if (far > 0.49993896484375f) {  // 1/2 - 2^-14
+    uint32_t v[4];
+    unpack64(v01, v[0], v[1]);
+    unpack64(v23, v[2], v[3]);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float t = v[e] * inv;
-    const float r = t + 12582912.f;  // 1.5 * 2^23: the sum's rounding is rint(t)
-    b[e] = __float_as_uint(r);
-    near |= fabsf(fabsf(t - (r - 12582912.f)) - 0.5f) < 6.103515625e-5f;
-  }
-  if (near) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) b[e] = __float_as_uint(__fdiv_rn(v[e], s) + 12582912.f);
+    for (int e = 0; e < 4; ++e) b[e] = __float_as_uint(__fdiv_rn(__uint_as_float(v[e]), s) + 12582912.f);
   }
   return prmt(prmt(b[0], b[1], 0x0040u), prmt(b[2], b[3], 0x0040u), 0x5410u);
 }
@@ -55,9 +62,8 @@ __global__ void __launch_bounds__(kQThreads) quantize_tokens_kernel(const T* __r
   uint4 q[kQChunks];
   uint32_t mx = 0;
   auto magnitude = [&](const uint4& w) {
-    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) mx = max(mx, max(ws[e] & 0x7FFFu, (ws[e] >> 16) & 0x7FFFu));
+    mx = __vmaxu2(mx, __vmaxu2(__vmaxu2(w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu),
+                               __vmaxu2(w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu)));  // of the two halves by themselves
   };
 #pragma unroll
   for (int i = 0; i < kQChunks; ++i) {
@@ -68,7 +74,7 @@ __global__ void __launch_bounds__(kQThreads) quantize_tokens_kernel(const T* __r
   for (int i = 0; i < kQChunks; ++i) magnitude(q[i]);
   if (live)
     for (int c = c0 + kQChunks * 32 * W; c < nch; c += 32 * W) magnitude(*reinterpret_cast<const uint4*>(xr + 8 * c));
-  mx = __reduce_max_sync(0xffffffffu, mx);
+  mx = __reduce_max_sync(0xffffffffu, max(mx & 0xFFFFu, mx >> 16));
   if (W > 1) {
     if (lane == 0) part[warp] = mx;
     __syncthreads();
@@ -79,7 +85,7 @@ __global__ void __launch_bounds__(kQThreads) quantize_tokens_kernel(const T* __r
   const float amax = Act<T>::unpack2(mx).x;
   const bool finite = amax <= 3.4028234e38f;  // false for infinities and NaN
   const float s = fmaxf(__fdiv_rn(amax, 127.f), 1e-8f);
-  const float inv = finite ? __frcp_rn(s) : 0.f;
+  const uint64_t inv2 = both(finite ? __frcp_rn(s) : 0.f);
   if (c0 == 0) sx[row] = finite ? s : __int_as_float(0x7fffffff);
   int8_t* qr = xq + row * cols;
   auto store = [&](const uint4& w, int c) {
@@ -88,8 +94,9 @@ __global__ void __launch_bounds__(kQThreads) quantize_tokens_kernel(const T* __r
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const float2 f = Act<T>::unpack2(ws[2 * h]), g = Act<T>::unpack2(ws[2 * h + 1]);
-      const float v[4] = {f.x, f.y, g.x, g.y};
-      o[h] = finite ? quant_word(v, s, inv) : 0u;
+      o[h] = finite ? quant_word(pack64(__float_as_uint(f.x), __float_as_uint(f.y)),
+                                 pack64(__float_as_uint(g.x), __float_as_uint(g.y)), s, inv2)
+                    : 0u;
     }
     *reinterpret_cast<uint2*>(qr + 8 * c) = make_uint2(o[0], o[1]);
   };
