@@ -25,7 +25,7 @@ namespace ee {
 // SM. (One CTA per item and part of its keys, joined in a cluster or by a
 // second launch, left SMs idle for 27 % of the time on 64 sequences of 1 to
 // 1632 keys and waited for each CTA's first loads again: 36 us.)
-constexpr int kPrStep = 16, kPrMinSteps = 8;   // keys of a step; steps that are worth a warp
+constexpr int kPrStep = 16, kPrMinSteps = 6;   // keys of a step; steps that are worth a warp
 template <int HD> constexpr int pr_warps() { return HD == 128 ? 8 : 16; }
 constexpr int kPrStages = 3;
 template <int HD> constexpr int pr_stage() { return 2 * kPrStep * HD * 2; }  // K and V of a step
@@ -234,28 +234,29 @@ __global__ void __launch_bounds__(32 * pr_warps<HD>(), 1) prompt_rows_kernel(con
       mma16816<T>(p[0], qf[ks][0], qf[ks][1], qf[ks][2], qf[ks][3], b[0], b[1]);
       mma16816<T>(p[1], qf[ks][0], qf[ks][1], qf[ks][2], qf[ks][3], b[2], b[3]);
     }
-    float x0 = -INFINITY, x1 = -INFINITY;
+    if (__any_sync(0xffffffffu, key + kPrStep > min(lim0, lim1))) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < 2; ++j) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int kk = key + 8 * j + 2 * t + c;
-        p[j][c] = kk < lim0 ? p[j][c] * a.scale_log2 : -INFINITY;
-        p[j][2 + c] = kk < lim1 ? p[j][2 + c] * a.scale_log2 : -INFINITY;
-        x0 = fmaxf(x0, p[j][c]);
-        x1 = fmaxf(x1, p[j][2 + c]);
+        for (int c = 0; c < 2; ++c) {
+          const int kk = key + 8 * j + 2 * t + c;
+          if (kk >= lim0) p[j][c] = -INFINITY;
+          if (kk >= lim1) p[j][2 + c] = -INFINITY;
+        }
       }
     }
+    float x0 = fmaxf(fmaxf(p[0][0], p[0][1]), fmaxf(p[1][0], p[1][1]));
+    float x1 = fmaxf(fmaxf(p[0][2], p[0][3]), fmaxf(p[1][2], p[1][3]));
 #pragma unroll
     for (int d = 1; d < 4; d <<= 1) {
       x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
       x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
     }
-    const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
-    // nothing seen yet: any finite reference will do, exp2(-inf) = 0
+    const float n0 = fmaxf(m0, x0 * a.scale_log2), n1 = fmaxf(m1, x1 * a.scale_log2);
+    // nothing seen yet: any finite reference will do, 2^-inf = 0
     const float u0 = n0 == -INFINITY ? 0.f : n0, u1 = n1 == -INFINITY ? 0.f : n1;
     if (__any_sync(0xffffffffu, n0 != m0 || n1 != m1)) {
-      const float c0 = exp2f(m0 - u0), c1 = exp2f(m1 - u1);
+      const float c0 = ex2(m0 - u0), c1 = ex2(m1 - u1);
       m0 = n0;
       m1 = n1;
       l0 *= c0;
@@ -272,8 +273,8 @@ __global__ void __launch_bounds__(32 * pr_warps<HD>(), 1) prompt_rows_kernel(con
     for (int j = 0; j < 2; ++j) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        p[j][c] = exp2f(p[j][c] - u0);
-        p[j][2 + c] = exp2f(p[j][2 + c] - u1);
+        p[j][c] = ex2(fmaf(p[j][c], a.scale_log2, -u0));
+        p[j][2 + c] = ex2(fmaf(p[j][2 + c], a.scale_log2, -u1));
         l0 += p[j][c];
         l1 += p[j][2 + c];
       }
