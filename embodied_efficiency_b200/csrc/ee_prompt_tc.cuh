@@ -17,12 +17,14 @@
 // share of the exponentials as polynomials on the FMA pipe was slower at every
 // share: 411 -> 428 / 472 / 530 us at hd 64 for 1/8, 1/4, 1/2 of them.)
 //
-// Measured: 8192 causal tokens, 16 / 4 heads of 128: 242 us, 1137 TFLOP/s,
-// 0.70 of the measured GEMM rate; 16 / 4 heads of 64 without a mask: 411 us,
-// the MUFU 74 % busy while an SM has work.
+// Measured: 8192 causal tokens, 16 / 4 heads of 128: 225 us, 1220 TFLOP/s,
+// 0.76 of the measured GEMM rate; 16 / 4 heads of 64 without a mask: 410 us,
+// the MUFU 74 % busy while an SM has work. What bounds it is one thread's row:
+// 3000 cycles per pair of blocks at hd 64 where the MUFU needs 2048. (Two
+// threads a row need 130 registers and have 104: 470 -> 720 us at hd 128.)
 //
 // The running maximum m is a reference, not the exact maximum: it moves only
-// when a row's maximum exceeds it by more than 2^8, so O is rarely rescaled
+// when a row's maximum exceeds it by more than 8 (a factor of 2^8), so O is rarely rescaled
 // (the weights stay below 2^8 and the result O / l does not depend on m). S(j)
 // of a tile is issued after its O += P(j-1) V(j-1), so the wait for S(j) also
 // says that O may be rescaled.
@@ -176,7 +178,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   constexpr int PANELS = HD / 64;
   // hd 64 leaves TMEM for P beside S, so the next scores are computed during the softmax
   constexpr bool SEP = HD == 64;
-  // pieces in which a block's weights are handed over (1 at hd 64: 501 instead of 411 us for 8192 tokens)
+  // pieces in which a block's weights are handed over (in one piece, hd 64: 501 instead of 411 us for 8192 tokens)
   constexpr int PARTS = 2;
   extern __shared__ __align__(1024) char smem_raw[];
   const uint32_t base0 = smem_u32(smem_raw);
