@@ -471,7 +471,9 @@ EE_DEV void join_row_warp(const PromptArgs& a, long long n, Slot slot, T* out) {
 }
 
 // The rows of the kernel for few rows whose item was cut, and rows without
-// keys. MANY: a CTA per (token, head); else a warp.
+// keys. MANY: a CTA per (token, head); else a warp. The search reads only the
+// offsets, which are final -- the kernel before this one has waited for them --
+// so it runs under that kernel's end.
 template <typename T, int HD, bool MANY>
 __global__ void __launch_bounds__(kPrJoin) prompt_join_kernel(const __grid_constant__ PromptArgs a, int most) {
   __shared__ PrList<kPrJoin> list;
@@ -479,7 +481,6 @@ __global__ void __launch_bounds__(kPrJoin) prompt_join_kernel(const __grid_const
   __shared__ PromptSeq seq;
   __shared__ long long seq_first;
   __shared__ int found;
-  pdl_entry();
   const int tok = blockIdx.x;
   if (threadIdx.x == 0) found = 0;
   const int per = (a.n_seq + kPrJoin - 1) / kPrJoin;
@@ -497,6 +498,7 @@ __global__ void __launch_bounds__(kPrJoin) prompt_join_kernel(const __grid_const
     found = 1;
   }
   __syncthreads();
+  pdl_entry();          // by every thread, the ones that return too: this grid must not end before the one it follows
   if (!found) return;  // rows outside the sequences stay as they were
   const PromptSeq s = seq;
   int steps;
