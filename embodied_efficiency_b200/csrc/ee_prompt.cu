@@ -156,21 +156,41 @@ __global__ void __launch_bounds__(32 * pr_warps<HD>(), 1) prompt_rows_kernel(con
   const uint32_t ring = smem_u32(smem) + warp * NS * 2 * TILE;
   auto off = [](int row, int ch) { return row * RB + ((ch ^ (row & 7)) << 4); };
   const int lrow = lane / CH, lch = lane % CH;  // this lane's row and chunk of every 32 / CH rows
+  // where this lane reads step `ld` from, and the keys that the sequence has from there on
+  const char *kp = nullptr, *vp = nullptr;
+  int valid = 0;
+  const long long k_row = a.k_tok * 2, v_row = a.v_tok * 2;
+  auto aim = [&]() {
+    const int kvh = ld.item % a.n_kv;
+    const long long k0 = ld.s.k0 + (long long)ld.step * kPrStep + lrow;
+    kp = reinterpret_cast<const char*>(a.k) + k0 * k_row + kvh * a.k_head * 2 + lch * 16;
+    vp = reinterpret_cast<const char*>(a.v) + k0 * v_row + kvh * a.v_head * 2 + lch * 16;
+    valid = ld.s.klen - ld.step * kPrStep - lrow;
+  };
+  aim();
   // the keys and values of step `ld`, those past the sequence's end zero-filled; then on to the next step
   auto load = [&](int buf) {
-    const int kvh = ld.item % a.n_kv, valid = ld.s.klen - ld.step * kPrStep;
-    const long long k0 = ld.s.k0 + (long long)ld.step * kPrStep;
-    const char* kb = reinterpret_cast<const char*>(a.k) + (k0 * a.k_tok + kvh * a.k_head) * 2 + lch * 16;
-    const char* vb = reinterpret_cast<const char*>(a.v) + (k0 * a.v_tok + kvh * a.v_head) * 2 + lch * 16;
     const uint32_t d = ring + buf * 2 * TILE;
+    const char *kr = kp, *vr = vp;
 #pragma unroll
     for (int i = 0; i < kPrStep * CH / 32; ++i) {
       const int row = lrow + i * (32 / CH);
-      const bool ok = row < valid;  // row 0 always is: the address of the others
-      cp_async16(d + off(row, lch), kb + (ok ? row * a.k_tok * 2 : 0), ok);
-      cp_async16(d + TILE + off(row, lch), vb + (ok ? row * a.v_tok * 2 : 0), ok);
+      const bool ok = i * (32 / CH) < valid;
+      // a copy of nothing reads nothing: any address will do
+      cp_async16(d + off(row, lch), ok ? kr : reinterpret_cast<const char*>(a.k), ok);
+      cp_async16(d + TILE + off(row, lch), ok ? vr : reinterpret_cast<const char*>(a.v), ok);
+      kr += 32 / CH * k_row;
+      vr += 32 / CH * v_row;
     }
-    ld.next(a);
+    if (ld.step + 1 < ld.per_item) {
+      ++ld.step;
+      kp += kPrStep * k_row;
+      vp += kPrStep * v_row;
+      valid -= kPrStep;
+    } else {
+      ld.next(a);
+      if (ld.b < a.n_seq) aim();
+    }
   };
   int ahead = 0;  // steps loaded beyond the current one
 #pragma unroll
