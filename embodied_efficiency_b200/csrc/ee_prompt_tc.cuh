@@ -22,6 +22,9 @@
 // the MUFU 74 % busy while an SM has work. What bounds it is one thread's row:
 // 3000 cycles per pair of blocks at hd 64 where the MUFU needs 2048. (Two
 // threads a row need 130 registers and have 104: 470 -> 720 us at hd 128.)
+// A last tile without a neighbour leaves its item's second half idle; halving
+// its keys over both halves and joining the sums was slower (128 prompts of
+// 257 to 816 tokens, hd 64: 395 -> 415 us).
 //
 // The running maximum m is a reference, not the exact maximum: it moves only
 // when a row's maximum exceeds it by more than 8 (a factor of 2^8), so O is rarely rescaled

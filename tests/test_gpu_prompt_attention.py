@@ -82,6 +82,37 @@ def test_more_items_than_sms(cuda, hq, hk, hd, causal):
     _check(out, q, k, v, q_len, k_len, causal, hd ** -0.5)
 
 
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("hq,hk", [(5, 5), (8, 2)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_last_tiles_that_have_no_neighbour(cuda, dtype, hq, hk, causal):
+    """Heads of 64, sequences whose last query tile stands alone against one to nine blocks of keys, many of them per
+    CTA and between whole pairs; rows that see nothing of the later blocks; NaN behind every sequence's keys; and
+    scores whose largest lies in the first or in the last block."""
+    from embodied_efficiency_b200 import prompt_attention
+    r = random.Random(hq)
+    tile = 128 * hk // hq
+    q_len = [r.choice([tile, tile - 1, tile // 2, 2 * tile, 2 * tile + 1, 3 * tile, 3 * tile - 5]) for _ in range(150)]
+    k_len = [max(n + r.choice([0, 0, 1, 100]), r.choice([1, 128, 129, 255, 256, 257, 384, 511, 640, 1100])) for n in q_len]
+    room = [n + r.choice([0, 3, 200]) for n in k_len]
+    q, k, v = _inputs(cuda, dtype, sum(q_len), sum(room), hq, hk, 64, 11)
+    start, at = [0], 0
+    for i, (n, w) in enumerate(zip(k_len, room)):
+        if i % 3:  # a slope along the keys, up or down
+            k[at:at + n, :, 0] += (torch.arange(n, device=cuda, dtype=dtype) * (0.125 if i % 3 == 1 else -0.125))[:, None]
+        k[at + n:at + w], v[at + n:at + w] = float("nan"), float("nan")
+        at += w
+        start.append(at)
+    q[:, :, 0] = 4.0
+    used = torch.tensor(k_len, device=cuda, dtype=torch.int32)
+    out = prompt_attention(q, k, v, _cu(q_len, cuda), torch.tensor(start, device=cuda, dtype=torch.int32), used,
+                           causal=causal)
+    keep = torch.cat([torch.arange(a, a + n) for a, n in zip(start, k_len)]).to(cuda)
+    _check(out, q, k[keep], v[keep], q_len, k_len, causal, 0.125)
+    assert torch.equal(out, prompt_attention(q, k, v, _cu(q_len, cuda), torch.tensor(start, device=cuda, dtype=torch.int32),
+                                             used, causal=causal))
+
+
 @pytest.mark.parametrize("longest", [3, 40])
 def test_many_short_sequences(cuda, longest):
     """More sequences than a CTA has threads, most of them tiny or empty."""
