@@ -149,6 +149,8 @@ def prompt_attention(q, k, v, cu_q, cu_k=None, k_lens=None, causal: bool = True,
     ``h // (heads // kv_heads)``. With ``causal`` a sequence's last query sees its last key, so queries may be the new
     tokens (or the one new token) behind a cached prompt; a query that sees no key gives zeros. ``scale`` defaults to
     head_dim^-0.5. Offsets are int32 on the device, not decreasing; what they claim beyond the tensors is cut off.
+    A masked key counts with weight 0, so ``k`` may hold anything there, while ``v`` has to be finite on the keys of a
+    sequence (0 * inf is NaN); beyond them, nothing is used.
     Returns [Tq, heads, head_dim], new or ``out``; rows that belong to no sequence are not written.
     head_dim 64 or 128; bf16 / fp16."""
     if out is None:
