@@ -234,6 +234,19 @@ def test_views_of_a_fused_projection_graphs_and_streams(cuda, lens):
     assert all(torch.equal(o, want) for o in outs)
 
 
+@pytest.mark.parametrize("t", [3, 300])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_broadcast_and_head_major_views(cuda, t, hd):
+    """Strides of 0 (heads or tokens that share their memory) and heads that lie behind one another."""
+    from embodied_efficiency_b200 import prompt_attention
+    q, k, v = _inputs(cuda, torch.bfloat16, t, t, 8, 1, hd, 21)
+    major = q.transpose(0, 1).contiguous().transpose(0, 1)
+    cu = _cu([t], cuda)
+    for qq, kk, vv in ((q, k.expand(t, 4, hd), v.expand(t, 4, hd)), (q, k[:1].expand(t, 1, hd), v[:1].expand(t, 1, hd)),
+                       (q[:, :1].expand(t, 8, hd), k, v), (q[:1, :1].expand(t, 8, hd), k, v), (major, k, v)):
+        _check(prompt_attention(qq, kk, vv, cu), qq, kk, vv, [t], [t], True, hd ** -0.5)
+
+
 def test_offsets_beyond_the_tensors_are_cut(cuda):
     """Tables that claim rows the tensors do not have read and write nothing outside them."""
     from embodied_efficiency_b200 import prompt_attention
