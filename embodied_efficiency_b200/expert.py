@@ -192,15 +192,19 @@ class PackedKV:
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor):
         self.k, self.v, self.cu = k, v, cu
-        self._cu_q = None
+        self._cu_q = {}
 
     def queries(self, b: int, n: int) -> torch.Tensor:
         """Offsets of ``n`` action tokens per prefix."""
         if b != self.cu.numel() - 1:
             raise ValueError(f"{self.cu.numel() - 1} packed prefixes for a batch of {b}")
-        if self._cu_q is None or self._cu_q[0] != n:
-            self._cu_q = (n, torch.arange(0, (b + 1) * n, n, dtype=torch.int32, device=self.cu.device))
-        return self._cu_q[1]
+        cu_q = self._cu_q.get(n)
+        if cu_q is None:
+            if self.cu.is_cuda and torch.cuda.is_current_stream_capturing():  # theirs are the graph's, filled by its replays
+                return torch.arange(0, (b + 1) * n, n, dtype=torch.int32, device=self.cu.device)
+            # copied from the host, which waits for it: there for every stream; kept, as captured calls may read it
+            cu_q = self._cu_q[n] = torch.arange(0, (b + 1) * n, n, dtype=torch.int32).to(self.cu.device)
+        return cu_q
 
 
 def _is_packed(prefix_kv) -> bool:

@@ -158,3 +158,28 @@ def test_fleet_of_different_prompts(cuda):
     for i, (pre, x0) in enumerate(reqs):
         ref = flow_sample(m, x0.to(cuda).bfloat16(), 3, m.encode(pre.to(cuda)), path="layers").float().cpu()
         assert float((acts[i] - ref[0]).abs().max()) <= 3e-2 * float(ref.abs().max())
+
+
+def test_offsets_first_asked_for_in_a_capture(cuda):
+    """A graph's own memory holds nothing before its replay: what a capture computes is not kept for eager calls, and
+    what eager calls keep serves captures and other streams."""
+    from embodied_efficiency_b200.expert import PackedKV
+    kv = torch.zeros(9, 2, 64, device=cuda, dtype=torch.bfloat16)
+    packed = PackedKV(kv, kv, torch.tensor([0, 2, 5, 9], device=cuda, dtype=torch.int32))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        inside = packed.queries(3, 4) + 0
+    eager = packed.queries(3, 4)
+    assert eager.tolist() == [0, 4, 8, 12]
+    graph.replay()
+    assert inside.tolist() == [0, 4, 8, 12]
+    again = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(again):
+        assert packed.queries(3, 4) is eager
+        keep = eager + 0
+    assert packed.queries(3, 5).tolist() == [0, 5, 10, 15]
+    assert packed.queries(3, 4) is eager  # still there for the capture
+    again.replay()
+    assert keep.tolist() == [0, 4, 8, 12]
+    with pytest.raises(ValueError):
+        packed.queries(4, 4)
