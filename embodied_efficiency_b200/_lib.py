@@ -85,6 +85,8 @@ SIGNATURES = {
     "ee_quantize_tokens": (c_int32, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int32, c_void_p]),
     "ee_int8_gemm": (c_int32, [c_void_p] * 7 + [c_int64] * 3 + [c_int32] * 3 + [c_void_p]),
     "ee_int8_linear_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "ee_int8_plan": (c_int32, [c_int64] * 3 + [c_int32, ctypes.POINTER(c_int32), ctypes.POINTER(c_int32),
+                                              ctypes.POINTER(c_size_t)]),
     "ee_int8_linear": (c_int32, [c_void_p, c_int64] + [c_void_p] * 6 + [c_size_t] + [c_int64] * 3 + [c_int32] * 3
                        + [c_void_p]),
     "ee_rotary": (c_int32, [c_void_p, c_int64, c_int64] * 4 + [c_void_p, c_int64, c_int32, c_void_p, c_int64, c_int32,

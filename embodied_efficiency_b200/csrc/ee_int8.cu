@@ -157,6 +157,17 @@ static int launch_pair(Int8Args a, const int8_t* xq, const int8_t* w, cudaStream
              : EE_ERR_LAUNCH;
 }
 
+// Ring stages of a CTA that takes kbc k-blocks. Clusters of 4 or 8 find room on
+// the GPU at once when two CTAs share an SM (50 x 2048 x 8192: 19 us with rings
+// of 200 KB, 10 with 100); alone or in pairs, CTAs are better off with the
+// deeper ring (2000 x 1024 x 4096: 27 and 25)
+template <int NT>
+static int few_stages(int k, int split) {
+  const int nkb = (k + 127) / 128, kbc = (nkb + split - 1) / split;
+  const int fit = (int)((split >= 4 ? 100u : 200u) * 1024u / i8_few_stage<NT>());
+  return kbc < fit ? kbc : fit;
+}
+
 template <typename T, int NT, bool GELU>
 static int launch_few(Int8Args a, const int8_t* xq, const int8_t* w, int split, cudaStream_t s) {
   auto fn = int8_few_kernel<T, NT, GELU>;
@@ -166,15 +177,9 @@ static int launch_few(Int8Args a, const int8_t* xq, const int8_t* w, int split, 
   if (!make_tmap_2d(&tx, xq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.K, a.M, a.K, 128, NT, CU_TENSOR_MAP_SWIZZLE_128B) ||
       !make_tmap_2d(&tw, w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.K, a.N, a.K, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B))
     return EE_ERR_LAUNCH;
-  const int nkb = (a.K + 127) / 128, kbc = (nkb + split - 1) / split;
-  // clusters of 4 or 8 find room on the GPU at once when two CTAs share an SM (50 x 2048 x 8192: 19 us with rings of
-  // 200 KB, 10 with 100); alone or in pairs, CTAs are better off with the deeper ring (2000 x 1024 x 4096: 27 and 25)
-  const int fit = (int)((split >= 4 ? 100u : 200u) * 1024u / i8_few_stage<NT>());
   a.split = split;
-  a.ns = kbc < fit ? kbc : fit;
-  uint32_t ring = a.ns * i8_few_stage<NT>();
-  if (ring < i8_few_part<NT>()) ring = i8_few_part<NT>();
-  const size_t smem = 1024 + ring + 16 * a.ns + 16;
+  a.ns = few_stages<NT>(a.K, split);
+  const size_t smem = i8_few_smem<NT>(a.ns);
   const long long units = (long long)((a.N + 127) / 128) * ((a.M + NT - 1) / NT);
   if (units * split > 0x7fffffff) return EE_ERR_SHAPE;
   cudaLaunchConfig_t cfg{};
@@ -220,6 +225,17 @@ static Int8Plan int8_plan(int m, int n, int k, int sms) {
     }
   }
   return best;
+}
+
+// shared memory that a CTA of the plan asks for
+static size_t int8_plan_smem(const Int8Plan& p, int k) {
+  switch (p.nt) {
+    case 16: return i8_few_smem<16>(few_stages<16>(k, p.split));
+    case 32: return i8_few_smem<32>(few_stages<32>(k, p.split));
+    case 64: return i8_few_smem<64>(few_stages<64>(k, p.split));
+    case 128: return i8_few_smem<128>(few_stages<128>(k, p.split));
+  }
+  return kI8PairSmem;
 }
 
 template <typename T, bool GELU>
@@ -307,6 +323,16 @@ int ee_int8_gemm(const int8_t* xq, const float* x_scales, const void* weight, co
   if (rc) return rc;
   return int8_product(xq, x_scales, weight, w_scales, bias, residual, y, m, n, k, scale_dtype, act_dtype, epilogue,
                       false, (cudaStream_t)stream);
+}
+
+int ee_int8_plan(int64_t m, int64_t n, int64_t k, int32_t sms, int32_t* tokens, int32_t* ctas, size_t* smem_bytes) {
+  if (!tokens || !ctas || !smem_bytes || sms < 2) return EE_ERR_ARG;
+  if (m < 1 || n < 1 || k < 16 || (k % 16) != 0 || k > 131056 || m > 0x7fffff00 || n > 0x7fffff00) return EE_ERR_SHAPE;
+  const Int8Plan p = int8_plan((int)m, (int)n, (int)k, sms);
+  *tokens = p.nt ? p.nt : 256;
+  *ctas = p.nt ? p.split : 2;
+  *smem_bytes = int8_plan_smem(p, (int)k);
+  return EE_OK;
 }
 
 size_t ee_int8_linear_workspace_bytes(int64_t m, int64_t k) {

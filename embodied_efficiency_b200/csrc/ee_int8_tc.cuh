@@ -157,7 +157,28 @@ constexpr uint32_t kI8Stage = 32768;
 constexpr uint32_t kI8OffEpi = kI8Stages * kI8Stage;            // 4 KB per epilogue warp
 constexpr uint32_t kI8OffCol = kI8OffEpi + kI8EpiWarps * 4096;  // [2][256] scales and biases
 constexpr uint32_t kI8OffBar = kI8OffCol + 2 * 2 * 256 * 4;
-constexpr uint32_t kI8PairSmem = kI8OffBar + 8 * (2 * kI8Stages + 4) + 16 + 1024;
+constexpr uint32_t kI8PairUsed = kI8OffBar + 8 * (2 * kI8Stages + 4) + 16 + 1024;
+
+// The other kernel's CTAs: a ring of stages (128 weight rows and NT tokens of
+// a k-block) that the partial sums take over, two barriers a stage, one for the
+// sums, the TMEM address.
+template <int NT> constexpr uint32_t i8_few_stage() { return 16384u + NT * 128u; }
+template <int NT> constexpr uint32_t i8_few_part() { return NT * 128u * 4u; }
+template <int NT> constexpr uint32_t i8_few_ring(int ns) {
+  return ns * i8_few_stage<NT>() > i8_few_part<NT>() ? ns * i8_few_stage<NT>() : i8_few_part<NT>();
+}
+template <int NT> constexpr uint32_t i8_few_smem(int ns) { return 1024u + i8_few_ring<NT>(ns) + 16u * ns + 16u; }
+
+// A pair takes all TMEM columns of two SMs, and one of its CTAs can have its
+// columns while the other waits for a CTA of another stream's launch. So that
+// none which waits for a CTA elsewhere can be that one, no CTA of a cluster of
+// int8_few_kernel fits beside a pair's: the pair asks for more shared memory
+// than it uses. (All of an SM's would keep every other stream's kernels out.)
+constexpr uint32_t kSmShared = 228 * 1024, kCtaReserve = 1024;  // of an SM; per CTA, beside what it asks for
+constexpr uint32_t kI8PairAlone = (kSmShared - 2 * kCtaReserve - i8_few_smem<16>(1)) / 1024 * 1024 + 1024;
+constexpr uint32_t kI8PairSmem = kI8PairUsed > kI8PairAlone ? kI8PairUsed : kI8PairAlone;
+static_assert(kI8PairSmem + kCtaReserve <= kSmShared, "a pair's CTA fits");
+static_assert(kI8PairSmem + i8_few_smem<16>(1) + 2 * kCtaReserve > kSmShared, "and nothing of the other kernel beside it");
 
 template <typename T, bool GELU>
 __global__ void __launch_bounds__(kI8PairThreads, 1) __cluster_dims__(2, 1, 1)
@@ -406,11 +427,11 @@ __global__ void __launch_bounds__(kI8PairThreads, 1) __cluster_dims__(2, 1, 1)
 // weights are the MMA's 128 lanes (A), the tokens its N, so a call of one
 // token wastes lanes of nothing but the tensor core. TMA producer, MMA issuer,
 // four warps that move the int32 partial sums to shared memory as
-// [token][feature]; then all warps of every CTA adds its share of the features over the
+// [token][feature]; then all warps of every CTA add its share of the features over the
 // cluster's partials (integers: exact in any order) and writes them.
+// TMEM is given back before the CTA waits for its cluster: a CTA that holds
+// columns waits for its own loads only, so whoever waits for them gets them.
 constexpr int kI8FewThreads = 256;
-template <int NT> constexpr uint32_t i8_few_stage() { return 16384u + NT * 128u; }
-template <int NT> constexpr uint32_t i8_few_part() { return NT * 128u * 4u; }
 
 template <typename T, int NT, bool GELU>
 __global__ void __launch_bounds__(kI8FewThreads)
@@ -429,9 +450,7 @@ __global__ void __launch_bounds__(kI8FewThreads)
   const int n0 = (unit % n_units) * 128, m0 = (unit / n_units) * NT;
   const int nkb = (a.K + 127) / 128;
   const int kb0 = nkb * (int)rank / S, kb1 = nkb * ((int)rank + 1) / S;
-  uint32_t ring = a.ns * STAGE;
-  if (ring < i8_few_part<NT>()) ring = i8_few_part<NT>();
-  const uint32_t bar_full = sb + ring, bar_empty = bar_full + 8 * a.ns, bar_acc = bar_empty + 8 * a.ns;
+  const uint32_t bar_full = sb + i8_few_ring<NT>(a.ns), bar_empty = bar_full + 8 * a.ns, bar_acc = bar_empty + 8 * a.ns;
   const uint32_t off_tm = bar_acc + 8 - sb;
   if (warp == 0 && lane == 0) {
     tma_prefetch_map(&tx);
@@ -528,13 +547,14 @@ __global__ void __launch_bounds__(kI8FewThreads)
       for (int e = 0; e < 16; ++e)
         *reinterpret_cast<uint32_t*>(smem + ((c0 + e) * 128 + 32 * q4 + lane) * 4) = v[e];
     }
+    tc_fence_before();
   }
-  tc_fence_before();
-  if (S > 1) cluster_sync(); else __syncthreads();
+  if (warp == 1 || warp >= 4) named_sync(1, 32 * 5);  // the sums are out of TMEM
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, COLS);
   }
+  if (S > 1) cluster_sync(); else __syncthreads();
   // this CTA's features rank * (128 / S) ..: 4 of one token at a time, the same 4 for all of a thread's tokens
   const int fg = 32 / S;
   static_assert(kI8FewThreads % 32 == 0, "a thread's features do not change");

@@ -32,7 +32,8 @@
  *   ee_read_status        device status word of a sampler workspace (new)
  *   ee_encode_kv_maps     TMA descriptors of the cached prefix K/V (new)
  *   ee_barrier_selftest   bounded-wait self-test of the grid barrier (new)
- *   ee_quantize_tokens / ee_int8_gemm / ee_int8_linear   8-bit integer linears (new)
+ *   ee_quantize_tokens / ee_int8_gemm / ee_int8_linear / ee_int8_plan
+ *                         8-bit integer linears (new)
  *   ee_rotary             rotary positions with several axes (new)
  *   ee_prompt_attention   attention over packed prompts (new)
  *   ee_strerror / ee_version / ee_struct_size   (new)
@@ -195,6 +196,10 @@ int ee_int8_gemm(const int8_t* xq, const float* x_scales, const void* weight, co
                  const void* residual, void* y, int64_t m, int64_t n, int64_t k, int32_t scale_dtype,
                  int32_t act_dtype, int32_t epilogue, ee_stream_t stream);
 size_t ee_int8_linear_workspace_bytes(int64_t m, int64_t k);
+/* The product's launch for these sizes on a GPU of `sms` multiprocessors (no
+ * device call): tokens per tile (256: CTA pairs), CTAs per cluster, shared
+ * memory that a CTA asks for. */
+int ee_int8_plan(int64_t m, int64_t n, int64_t k, int32_t sms, int32_t* tokens, int32_t* ctas, size_t* smem_bytes);
 int ee_int8_linear(const void* x, int64_t ldx, const void* weight, const void* w_scales, const void* bias,
                    const void* residual, void* y, void* workspace, size_t workspace_bytes, int64_t m, int64_t n,
                    int64_t k, int32_t scale_dtype, int32_t act_dtype, int32_t epilogue, ee_stream_t stream);
