@@ -95,6 +95,7 @@ SIGNATURES = {
     "ee_prompt_attention_workspace_bytes": (c_size_t, [c_int64, c_int64] + [c_int32] * 4),
     "ee_prompt_attention": (c_int32, [c_void_p, c_int64, c_int64] * 4 + [c_void_p] * 3 + [c_int64, c_int64]
                             + [c_int32] * 5 + [c_float, c_int32, c_void_p, c_size_t, c_void_p]),
+    "ee_prompt_attention_wait_limit": (c_int32, [ctypes.c_uint64]),
     "ee_flow_sample_traced": (c_int32, [ctypes.POINTER(Expert), c_void_p, c_void_p, c_void_p, c_int32,
                                         c_int32, c_void_p, c_size_t, c_void_p, c_void_p]),
     "ee_flow_sample_phases": (c_int32, [ctypes.POINTER(Expert), c_int32]),

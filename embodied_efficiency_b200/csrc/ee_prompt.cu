@@ -616,6 +616,9 @@ static bool make_head_map(CUtensorMap* map, const void* base, int hd, int heads,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+constexpr unsigned long long kPtWaitNs = 1000000000ull;
+static std::atomic<unsigned long long> g_wait_limit{kPtWaitNs};
+
 template <typename T, int HD>
 static int launch_tc(const PromptArgs& p, cudaStream_t s) {
   auto fn = prompt_tc_kernel<T, HD>;
@@ -627,7 +630,7 @@ static int launch_tc(const PromptArgs& p, cudaStream_t s) {
   a.p = p;
   a.tpt = 128 / p.group;
   a.status = gemm_status_ptr();
-  a.timeout_ns = 1000000000ull;
+  a.timeout_ns = g_wait_limit.load(std::memory_order_relaxed);
   if (!a.status) return EE_ERR_DEVICE;
   CUtensorMap mq, mk, mv;
   if (!make_head_map(&mq, p.q, HD, p.n_q, p.tq, p.q_head, p.q_tok, p.group, a.tpt) ||
@@ -658,6 +661,11 @@ size_t ee_prompt_attention_workspace_bytes(int64_t tq, int64_t tk, int32_t n_seq
                                            int32_t head_dim) {
   if (tq < 0 || tk < 0 || n_seq < 0 || n_q < 1 || n_kv < 1 || n_q % n_kv || tq > 0x7fffff00 || tk > 0x7fffff00) return 0;
   return prompt_ws_bytes(prompt_plan(tq, tk, n_seq, n_q, n_kv), tq, n_q, head_dim);
+}
+
+int ee_prompt_attention_wait_limit(uint64_t ns) {
+  g_wait_limit.store(ns ? ns : kPtWaitNs, std::memory_order_relaxed);
+  return EE_OK;
 }
 
 int ee_prompt_attention(const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok, int64_t k_head,

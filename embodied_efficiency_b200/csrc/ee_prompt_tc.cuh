@@ -38,8 +38,13 @@
 // 4-7: softmax and output of tile 0 and 1; warp 8: finds the items, publishes
 // them in a shared-memory ring and loads Q, K and V by TMA; warp 9: MMA issue;
 // warp 10: zeroes V's rows past a sequence's end (their weights are 0, but
-// 0 * NaN is not); warp 11 only fills the warpgroup. Waits are bounded; a
-// timeout leaves EE_ERR_TIMEOUT in the GEMM status word.
+// 0 * NaN is not); warp 11 only fills the warpgroup.
+//
+// Waits are bounded, each by what it waits for: a block's loads, scores,
+// weights or products by timeout_ns, an item's whole walk by timeout_ns without
+// a block started (wait_walk). A wait that gives up leaves EE_ERR_TIMEOUT in
+// the GEMM status word and ends its role; the others then give up too, every
+// load lands and every MMA completes before the CTA returns its memory.
 #pragma once
 
 #include "ee_prompt.cuh"
@@ -62,13 +67,15 @@ constexpr int kPtThreads = 384;
 constexpr int kPtRegsLaunch = 168, kPtRegsSoft = 208, kPtRegsRest = 88;
 static_assert(256 * kPtRegsSoft + 128 * kPtRegsRest <= kPtThreads * kPtRegsLaunch, "the register shares fit the launch");
 constexpr int kPtKeys = 128, kPtInfo = 4, kPtLoads = 8;  // keys per block; items published, loads of K / V ahead
+constexpr unsigned long long kPtDrainNs = 1000000000ull;  // for loads and MMAs already issued, whatever timeout_ns is
 template <int HD> constexpr int pt_slots() { return HD == 128 ? 4 : 8; }
 template <int HD> constexpr uint32_t pt_tile() { return 128u * HD * 2; }
 template <int HD> constexpr uint32_t pt_off_out() { return (2 + pt_slots<HD>()) * pt_tile<HD>(); }  // 4 KB per softmax warp
 template <int HD> constexpr uint32_t pt_off_bar() { return pt_off_out<HD>() + 8 * 4096; }
-// barriers: full / empty per load of K / V, Q full / empty, S / P (two halves) / S free / O / O free per tile, V to fix / fixed, item full / empty
-template <int HD> constexpr uint32_t pt_off_info() { return pt_off_bar<HD>() + 8 * (2 * kPtLoads + 16 + 2 * kPtInfo) + 8; }
-template <int HD> constexpr uint32_t pt_smem() { return pt_off_info<HD>() + kPtInfo * 64 + 1024; }
+// barriers: full / empty per load of K / V, Q full / empty, S / P (two halves) / S free / O / O free per tile, V to fix / fixed, item full / empty, MMAs done after a failure
+template <int HD> constexpr uint32_t pt_off_info() { return pt_off_bar<HD>() + 8 * (2 * kPtLoads + 17 + 2 * kPtInfo) + 8; }
+template <int HD> constexpr uint32_t pt_off_beat() { return pt_off_info<HD>() + kPtInfo * 64; }  // blocks the MMA warp has come to
+template <int HD> constexpr uint32_t pt_smem() { return pt_off_beat<HD>() + 16 + 1024; }
 
 // One published item (16 words)
 struct PromptItem {
@@ -192,8 +199,9 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   const uint32_t b_full = sb + pt_off_bar<HD>(), b_empty = b_full + 8 * NP;
   const uint32_t b_qf = b_empty + 8 * NP, b_qe = b_qf + 8, b_s = b_qe + 8, b_p = b_s + 16, b_sf = b_p + 32, b_o = b_sf + 16;
   const uint32_t b_of = b_o + 16, b_req = b_of + 16, b_fix = b_req + 8, b_if = b_fix + 8, b_ie = b_if + 8 * kPtInfo;
-  const uint32_t off_tm = b_ie + 8 * kPtInfo - sb;
+  const uint32_t b_end = b_ie + 8 * kPtInfo, off_tm = b_end + 8 - sb;
   volatile PromptItem* ring = reinterpret_cast<volatile PromptItem*>(smem + pt_off_info<HD>());
+  volatile uint32_t* beat = reinterpret_cast<volatile uint32_t*>(smem + pt_off_beat<HD>());
   const PromptArgs& p = a.p;
   if (warp == 8 && lane == 0) {
     tma_prefetch_map(&mq);
@@ -207,6 +215,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     mbar_init(b_fix, 1);
     mbar_init(b_qf, 1);
     mbar_init(b_qe, 1);
+    mbar_init(b_end, 1);
+    *beat = 0;
     for (int t = 0; t < 2; ++t) {
       mbar_init(b_s + 8 * t, 1);
       mbar_init(b_p + 8 * t, 4);
@@ -232,8 +242,19 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + off_tm);
   // TMEM columns: S of tile t at 128 t, O at 256 + 128 t (SEP: 256 + 64 t), P over S (SEP: at 384 + 64 t)
   constexpr uint32_t OC = SEP ? 64 : 128;
-  // The consumers' view of the item ring: wait for item i, read it; release when done with it.
-  auto item_wait = [&](int i) { return mbar_wait(b_if + 8 * (i % kPtInfo), (uint32_t)((i / kPtInfo) & 1), a.timeout_ns); };
+  // A wait that may take an item's walk over its keys: given up when timeout_ns pass without a block begun.
+  auto wait_walk = [&](uint32_t bar, uint32_t parity) {
+    uint32_t seen = *beat;
+    while (!mbar_wait(bar, parity, a.timeout_ns)) {
+      const uint32_t now = *beat;
+      if (now == seen) return false;
+      seen = now;
+    }
+    return true;
+  };
+  // The consumers' view of the item ring: wait for item i, read it; release when done with it. A tile that has no
+  // blocks of the item before comes here while the other one walks them.
+  auto item_wait = [&](int i) { return wait_walk(b_if + 8 * (i % kPtInfo), (uint32_t)((i / kPtInfo) & 1)); };
   auto item_done = [&](int i) { mbar_arrive(b_ie + 8 * (i % kPtInfo)); };
 
   if (warp >= 8) {
@@ -257,16 +278,17 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         const long long idx = (long long)i * gridDim.x + ((i & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
         PromptItem it{};
         const bool more = ok && idx < (long long)units * p.n_kv * p.splits && prompt_item(a, (int)idx, units, window, it);
-        if (lane == 0) {
-          if (i >= kPtInfo && ok && !mbar_wait(b_ie + 8 * (i % kPtInfo), (uint32_t)((i / kPtInfo - 1) & 1), a.timeout_ns))
-            ok = false;
+        if (lane == 0 && i >= kPtInfo)  // the slot's item has been read by all; if not, it stays as it is
+          ok = mbar_wait(b_ie + 8 * (i % kPtInfo), (uint32_t)((i / kPtInfo - 1) & 1), a.timeout_ns);
+        if (lane == 0 && ok) {
           volatile PromptItem* r = ring + i % kPtInfo;
           r->q0 = it.q0; r->qlen = it.qlen; r->klen = it.klen;
           r->tok = it.tok; r->kvh = it.kvh; r->part = it.part; r->key0 = it.key0;
           r->n[0] = it.n[0]; r->n[1] = it.n[1]; r->tail = it.tail;
-          r->nbm = more && ok ? it.nbm : -1;
+          r->nbm = more ? it.nbm : -1;
           mbar_arrive(b_if + 8 * (i % kPtInfo));
-          // tile w of the item (K(0) V(0) K(1) V(1) ...) into the next slot, on the load's barrier
+          // tile w of the item (K(0) V(0) K(1) V(1) ...) into the next slot, on the load's barrier, which expects
+          // what has been issued and no more: `loaded` ends its phase, after a failure too
           auto load_kv = [&](int w) {
             if (n >= NS) {  // the load that used the slot before has been consumed
               const uint32_t was = slot_load[sl];
@@ -276,16 +298,20 @@ __global__ void __launch_bounds__(kPtThreads, 1)
               }
             }
             slot_load[sl] = g;
+            mbar_expect_tx(b_full + 8 * (g % NP), TILE);
             for (int c = 0; c < PANELS; ++c)
               tma_load_3d(sKV + sl * TILE + c * PANEL, (w & 1) ? &mv : &mk, 64 * c, it.kvh,
                           it.k0 + it.key0 + (w >> 1) * kPtKeys, b_full + 8 * (g % NP));
             ++n;
             if (++sl == NS) sl = 0;
           };
-          if (more && ok && it.nbm > 0) {
-            mbar_arrive_expect_tx(b_full + 8 * (g % NP), TILE);
-            load_kv(0);
+          auto loaded = [&]() {
+            mbar_arrive(b_full + 8 * (g % NP));
             ++g;
+          };
+          if (more && it.nbm > 0) {
+            load_kv(0);
+            loaded();
             // Q: its buffers are free when the last scores of the previous item are done
             if (ok && nq > 0 && !mbar_wait(b_qe, (uint32_t)((nq - 1) & 1), a.timeout_ns)) ok = false;
             if (ok) {
@@ -296,22 +322,26 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                     tma_load_3d(sQ + t * TILE + c * PANEL, &mq, 64 * c, it.kvh * p.group, it.q0 + it.tok + t * a.tpt, b_qf);
               ++nq;
             }
-            for (int j = 0; j < it.nbm && ok; ++j, ++g) {  // V(j) and K(j + 1)
-              mbar_arrive_expect_tx(b_full + 8 * (g % NP), j + 1 < it.nbm ? 2 * TILE : TILE);
+            for (int j = 0; j < it.nbm && ok; ++j) {  // V(j) and K(j + 1)
               load_kv(2 * j + 1);
               if (j + 1 < it.nbm && ok) load_kv(2 * j + 2);
+              loaded();
             }
           }
         }
         ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
         if (!more || !ok) break;
       }
-      // everything issued lands before the CTA may exit
+      // everything issued lands before the CTA may exit, whatever has failed; if nothing has, it is used too, and the
+      // MMA warp's arrivals that say so have come
       if (lane == 0) {
-        if (ok)
-          for (uint32_t e = g > NP ? g - NP : 0; e < g; ++e)
-            if (!mbar_wait(b_full + 8 * (e % NP), (e / NP) & 1, a.timeout_ns)) ok = false;
-        if (ok && nq > 0 && !mbar_wait(b_qf, (uint32_t)((nq - 1) & 1), a.timeout_ns)) ok = false;
+        const uint32_t e0 = g > NP ? g - NP : 0;
+        bool landed = true;
+        for (uint32_t e = e0; e < g; ++e) landed &= mbar_wait(b_full + 8 * (e % NP), (e / NP) & 1, kPtDrainNs);
+        if (nq > 0) landed &= mbar_wait(b_qf, (uint32_t)((nq - 1) & 1), kPtDrainNs);
+        ok = ok && landed;
+        for (uint32_t e = e0; e < g && ok; ++e) ok = mbar_wait(b_empty + 8 * (e % NP), (e / NP) & 1, a.timeout_ns);
+        if (ok && nq > 0) ok = mbar_wait(b_qe, (uint32_t)((nq - 1) & 1), a.timeout_ns);
         if (!ok) atomicCAS(a.status, 0, (int)EE_ERR_TIMEOUT);
       }
       __syncwarp();
@@ -364,6 +394,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           const int vs = sl + 1 == NS ? 0 : sl + 1, ks = vs + 1 == NS ? 0 : vs + 1;  // V(j) and K(j + 1)
           ok = wait(b_full + 8 * (g % NP), (g / NP) & 1);
           if (!ok) break;
+          if (lane == 0) *beat = g;
           bool fix = j + 1 == nbm && tail < kPtKeys;
           if (fix && lane == 0) mbar_arrive(b_req);
           __syncwarp();
@@ -414,7 +445,13 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           sl = ks;
         }
       }
-      if (!ok && lane == 0) atomicCAS(a.status, 0, (int)EE_ERR_TIMEOUT);
+      if (!ok) {  // what has been issued completes before the memory it works on is given back
+        if (lane == 0) atomicCAS(a.status, 0, (int)EE_ERR_TIMEOUT);
+        __syncwarp();
+        if (elect_one()) umma_commit(b_end);
+        mbar_wait(b_end, 0, kPtDrainNs);
+        __syncwarp();
+      }
     } else if (warp == 10) {
       // ---------------- V rows past the sequence's end ----------------
       int n = 0, nfix = 0;
@@ -431,7 +468,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         g += nbm + 1;
         if (tail == kPtKeys) continue;
         // not before the MMA warp has come to the block: earlier, the barrier's parity may be an older load's
-        ok = mbar_wait(b_req, (uint32_t)(nfix++ & 1), a.timeout_ns) &&
+        ok = wait_walk(b_req, (uint32_t)(nfix++ & 1)) &&
              mbar_wait(b_full + 8 * ((g - 1) % NP), ((g - 1) / NP) & 1, a.timeout_ns);
         if (!__all_sync(0xffffffffu, ok)) break;
         const uint32_t v = sKV + (uint32_t)((n - 1) % NS) * TILE;
@@ -626,7 +663,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     if (!ok && lane == 0) atomicCAS(a.status, 0, (int)EE_ERR_TIMEOUT);
   }
   tc_fence_before();
-  __syncthreads();  // every MMA has completed (the outputs waited for them) and every TMEM read is done
+  __syncthreads();  // every MMA has completed (the outputs or the MMA warp waited for them) and every TMEM read is done
   if (warp == 9) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);

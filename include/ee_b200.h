@@ -245,6 +245,11 @@ int ee_prompt_attention(const void* q, int64_t q_tok, int64_t q_head, const void
                         const int32_t* cu_q, const int32_t* cu_k, const int32_t* k_lens, int64_t tq, int64_t tk,
                         int32_t n_seq, int32_t n_q, int32_t n_kv, int32_t head_dim, int32_t causal, float scale,
                         int32_t act_dtype, void* workspace, size_t workspace_bytes, ee_stream_t stream);
+/* Limit of the waits inside the tensor-core attention kernel from the next
+ * launch on, for the whole process: a wait without progress for `ns` (0: the
+ * default, 1 s) gives up, the launch ends with its outputs unfinished and
+ * EE_ERR_TIMEOUT in the status word of ee_wq_gemm_status. */
+int ee_prompt_attention_wait_limit(uint64_t ns);
 
 /* ---- fused flow-matching sampler --------------------------------------- */
 typedef struct ee_linear {
