@@ -4,9 +4,11 @@
 // Pair i of a head (elements i and i + hd/2, or 2i and 2i + 1 interleaved)
 // turns by pos[axis(i)][token] * base^(-2i / hd). The table holds each
 // frequency as a 64-bit fraction of a turn, F = round(freq / 2 pi * 2^64), so
-// pos * F modulo 2^64 is the angle's fraction of a turn with an error below
-// |pos| * 2^-65 turns: whole turns drop out in the integer multiply instead of
-// costing the float angle its low bits at far positions.
+// pos * F modulo 2^64 is the angle's fraction of a turn, at most |pos| * 2^-65
+// turns off if F is the rounded value (more digits than a double has): whole
+// turns drop out in the integer multiply instead of costing the float angle its
+// low bits at far positions. Its top 32 bits, as an fp32 value of [-1, 1) half
+// turns, add 2^-25 of those.
 //
 // HBM-bound: every value is read and written once (4 bytes), the angles are
 // hd/2 sine / cosine pairs per token shared by all its heads. One warp per

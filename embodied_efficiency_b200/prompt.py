@@ -12,6 +12,7 @@ forward only.
 from __future__ import annotations
 
 import ctypes
+import decimal
 import functools
 import math
 
@@ -50,18 +51,27 @@ def _act_dtype(t, name):
 
 
 _TURNS: dict = {}
+_PI = decimal.Decimal("3.14159265358979323846264338327950288419716939937510582097494459")
+
+
+def _turn_fractions(half: int, base: float) -> list:
+    """round(base^(-i / half) / 2 pi * 2^64) for i < half. In 50 digits: in double, whose 53 bits end 11 short of the
+    table's, a position of 2^40 would turn 2^-15 of a turn too far."""
+    with decimal.localcontext() as ctx:
+        ctx.prec = 50
+        log, scale = decimal.Decimal(float(base)).ln(), decimal.Decimal(2 ** 64) / (2 * _PI)
+        return [int((scale * (log * -i / half).exp()).to_integral_value()) for i in range(half)]
 
 
 def _turns(device, half: int, base: float) -> torch.Tensor:
-    """base^(-i / half) / 2 pi as 64-bit fractions of a turn (int64 bits), a constant table per device."""
+    """``_turn_fractions`` as int64 bits, a constant table per device."""
     key = (device, half, base)
     tab = _TURNS.get(key)
     if tab is None:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError(f"rotary_embed copies its frequencies (head_dim {2 * half}, base {base}) to the device on "
                                "first use: call it once before the stream capture")
-        vals = [int(round(math.ldexp(base ** (-i / half) / (2.0 * math.pi), 64))) & (2 ** 64 - 1) for i in range(half)]
-        host = torch.tensor([v - 2 ** 64 if v >= 2 ** 63 else v for v in vals], dtype=torch.int64)
+        host = torch.tensor(_turn_fractions(half, base), dtype=torch.int64)  # at most 2^64 / 2 pi < 2^63
         tab = _TURNS[key] = host.to(device)
     return tab
 
@@ -79,8 +89,8 @@ def rotary_embed(q, k, positions, sections, base: float = 10000.0, interleaved: 
     [T, kv_heads, head_dim] (either may be None): pair i of the head_dim / 2 pairs turns by
     ``positions[axis][t] * base^(-2i / head_dim)``, the first ``sections[0]`` pairs by axis 0, the next
     ``sections[1]`` by axis 1 and so on. Pairs are (i, i + head_dim / 2), or (2i, 2i + 1) when ``interleaved``.
-    ``positions`` is int32 or int64 [axes, T] ([T] for one axis); angles stay exact to the last bits of fp32 at any
-    position. Returns (q, k) turned, as new tensors or in ``out`` = (q_out, k_out), which may be the inputs
+    ``positions`` is int32 or int64 [axes, T] ([T] for one axis); an angle is off by less than 2^-22 (fp32's rounding of
+    angle, sine and cosine) and ``|position| * 2^-62``: as much again only from 2^40 on. Returns (q, k) turned, as new tensors or in ``out`` = (q_out, k_out), which may be the inputs
     themselves. head_dim 32, 64, 128 or 256; bf16 / fp16. The first call for a head_dim and base on a device copies a
     small table to it and has to come before a stream capture."""
     if out is None and q is not None and k is not None:

@@ -209,8 +209,9 @@ int ee_int8_linear(const void* x, int64_t ldx, const void* weight, const void* w
  * pairs go by axis 0, the next sections[1] by axis 1, ... (the sections sum to
  * head_dim / 2). Pair i is elements (i, i + head_dim / 2), or (2i, 2i + 1)
  * when interleaved. freqs[i] = round(freq(i) / (2 pi) * 2^64), a fraction of a
- * turn: the angle is taken modulo whole turns in integers, so far (and
- * negative) positions lose nothing. q [tokens][n_q][head_dim] and
+ * turn: the angle is taken modulo whole turns in integers, so at a far (or
+ * negative) position only the table's own rounding counts: |position| * 2^-65
+ * turns for entries that are rounded from more than a double's 53 bits. q [tokens][n_q][head_dim] and
  * k [tokens][n_kv][head_dim] by token / head strides in elements (multiples
  * of 8; the last dimension contiguous), each to its own output (which may be
  * the input itself); n_q or n_kv may be 0. positions: int32 or int64
