@@ -41,12 +41,6 @@ struct Call {
     if (!t.is_cuda() || t.get_device() != dev || (grad && t.requires_grad())) return fail();
     return &t;
   }
-  const Tensor* param(PyObject* o) {  // the same for a module's parameter (a bias), which may ask for one
-    if (!ok || !THPVariable_Check(o)) return fail();
-    const Tensor& t = THPVariable_Unpack(o);
-    if (!t.is_cuda() || t.get_device() != dev) return fail();
-    return &t;
-  }
   const Tensor* fail() {
     ok = false;
     return nullptr;
@@ -73,7 +67,7 @@ struct Linear {
 };
 // weight, scales, bias, gelu, residual of a product with outputs of `type` and shape [..., n]
 bool linear(Call& c, PyObject* const* a, ScalarType type, int64_t m, at::IntArrayRef lead, Linear& l) {
-  const Tensor *w = c.param(a[0]), *s = c.param(a[1]);
+  const Tensor *w = c.get(a[0]), *s = c.get(a[1]);
   if (!c.need(w && s && w->dim() == 2 && w->scalar_type() == at::kChar && w->is_contiguous() && aligned(*w))) return false;
   l.n = w->size(0);
   l.k = w->size(1);
@@ -85,7 +79,7 @@ bool linear(Call& c, PyObject* const* a, ScalarType type, int64_t m, at::IntArra
   l.scales = s->data_ptr();
   l.scale_dtype = f32 ? EE_F32 : EE_F16;
   if (a[2] != Py_None) {
-    const Tensor* b = c.param(a[2]);
+    const Tensor* b = c.get(a[2]);
     if (!c.need(b && b->scalar_type() == type && b->numel() == l.n && b->is_contiguous() && aligned(*b))) return false;
     l.bias = b->data_ptr();
     l.epilogue |= EE_EPI_BIAS;

@@ -218,7 +218,8 @@ def int8_matmul(xq, x_scale, weight, scales, bias=None, dtype=torch.bfloat16, ge
     """``(xq @ weight.T) * x_scale * scales + bias`` of int8 codes ``xq`` [..., K] and ``weight`` [N, K], with an exact
     32-bit integer sum, fp32 after it and one rounding to ``dtype`` (``ee_int8_gemm``). ``x_scale`` holds one fp32 value
     per token (``quantize_tokens``), ``scales`` one fp32 or fp16 value per output channel. ``gelu`` (exact erf GELU) or
-    ``residual`` are applied in fp32 before that rounding. No backward pass."""
+    ``residual`` are applied in fp32 before that rounding. No backward pass: operands that ask for a gradient are
+    refused while gradients are enabled."""
     y = (_lib._native or _lib.native()).int8_matmul(xq, x_scale, weight, scales, bias, gelu, residual, dtype)
     if y is not None:
         return y
@@ -232,7 +233,7 @@ def int8_matmul(xq, x_scale, weight, scales, bias=None, dtype=torch.bfloat16, ge
         raise ValueError(f"x_scale must hold {m} float32 values (one per token), "
                          f"got {x_scale.dtype} {tuple(x_scale.shape)}")
     dev = _lib.same_device(xq, x_scale, weight, scales, bias, residual)
-    _lib.no_grad_through("int8_matmul", x_scale, residual)
+    _lib.no_grad_through("int8_matmul", x_scale, scales, bias, residual)
     with _lib.on_device(dev):
         s, b, r, epi = _int8_epilogue(scales, bias, gelu, residual, dtype)
         xq, x_scale, weight = _aligned(xq), _aligned(x_scale), _aligned(weight)
@@ -247,7 +248,8 @@ def int8_matmul(xq, x_scale, weight, scales, bias=None, dtype=torch.bfloat16, ge
 def int8_linear(x, weight, scales, bias=None, gelu=False, residual=None):
     """A linear on the 8-bit integer tensor cores: bf16 / fp16 ``x`` [..., K] quantised per token as in
     ``quantize_tokens``, then ``int8_matmul`` with ``weight`` int8 [N, K] and one scale per output channel, to
-    ``x.dtype`` (``ee_int8_linear``, one call). No backward pass."""
+    ``x.dtype`` (``ee_int8_linear``, one call). No backward pass: operands that ask for a gradient (a bias that is a
+    module's parameter, say) are refused while gradients are enabled."""
     y = (_lib._native or _lib.native()).int8_linear(x, weight, scales, bias, gelu, residual)
     if y is not None:
         return y
@@ -255,7 +257,7 @@ def int8_linear(x, weight, scales, bias=None, gelu=False, residual=None):
     out_shape = (x.shape[0], weight.shape[0]) if x.dim() == 2 else (*x.shape[:-1], weight.shape[0])
     n = _check_int8_operands(weight, scales, bias, residual, k, x.dtype, out_shape)
     dev = _lib.same_device(x, weight, scales, bias, residual)
-    _lib.no_grad_through("int8_linear", x, residual)
+    _lib.no_grad_through("int8_linear", x, scales, bias, residual)
     with _lib.on_device(dev):
         xf, ld = _token_rows(x, k)
         m = xf.shape[0]
@@ -379,11 +381,14 @@ class TritonQuantLinear(nn.Module):
         from ``DENSE_MIN_TOKENS`` bf16 / fp16 tokens on, on the dense copy of
         the weight -- the same products, so the same results up to the
         GEMM's accumulation order. Never builds the copy during stream capture.
-        With ``act_bits=8`` every call is ``int8_linear`` (fp32 activations in bf16, as ``wq_linear`` takes them)."""
+        With ``act_bits=8`` every call is ``int8_linear`` (fp32 activations in bf16, as ``wq_linear`` takes them).
+        None of these has a backward pass: inputs and parameters count as constants, and the result asks for no
+        gradient whatever they ask for."""
         if self.act_bits == 8:
             act = x.dtype if x.dtype in (torch.bfloat16, torch.float16) else torch.bfloat16
+            b = None if self.bias is None else self.bias.detach()
             r = None if residual is None else residual.detach().to(act)
-            return int8_linear(x.detach().to(act), self.weight, self.scales, self.bias, gelu, r).to(x.dtype)
+            return int8_linear(x.detach().to(act), self.weight, self.scales.detach(), b, gelu, r).to(x.dtype)
         m = x.numel() // self.in_features if self.in_features else 0
         if (DENSE_MIN_TOKENS is not None and x.is_cuda and x.dtype in (torch.bfloat16, torch.float16)
                 and m >= DENSE_MIN_TOKENS
