@@ -12,6 +12,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 from . import build as _build
 
@@ -214,11 +215,15 @@ def same_device(*tensors):
 
 
 def no_grad_through(what: str, *tensors):
-    """These kernels have no backward pass: an input that asks for one is refused."""
+    """These kernels have no derivatives: an input that asks for a gradient, or carries a tangent, is refused."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() or detach its inputs")
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} has no forward-mode derivative: give it the primal values")
 
 
 def ptr(t) -> int:

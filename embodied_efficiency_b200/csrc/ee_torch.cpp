@@ -35,10 +35,10 @@ struct Call {
   int dev = c10::cuda::current_device();
   const bool grad = at::GradMode::is_enabled();
 
-  const Tensor* get(PyObject* o) {  // a CUDA tensor of the current device that asks for no gradient
+  const Tensor* get(PyObject* o) {  // a CUDA tensor of the current device that asks for no gradient of either mode
     if (!ok || !THPVariable_Check(o)) return fail();
     const Tensor& t = THPVariable_Unpack(o);
-    if (!t.is_cuda() || t.get_device() != dev || (grad && t.requires_grad())) return fail();
+    if (!t.is_cuda() || t.get_device() != dev || (grad && t.requires_grad()) || t._fw_grad(0).defined()) return fail();
     return &t;
   }
   const Tensor* fail() {
