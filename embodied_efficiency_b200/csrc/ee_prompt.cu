@@ -274,7 +274,9 @@ __global__ void __launch_bounds__(32 * pr_warps<HD>(), 1) prompt_rows_kernel(con
       x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
       x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
     }
-    const float n0 = fmaxf(m0, x0 * a.scale_log2), n1 = fmaxf(m1, x1 * a.scale_log2);
+    // fp16: weights up to 2^15
+    const float n0 = fmaxf(m0, prompt_reference<T, 15>(x0 * a.scale_log2));
+    const float n1 = fmaxf(m1, prompt_reference<T, 15>(x1 * a.scale_log2));
     // nothing seen yet: any finite reference will do, 2^-inf = 0
     const float u0 = n0 == -INFINITY ? 0.f : n0, u1 = n1 == -INFINITY ? 0.f : n1;
     if (__any_sync(0xffffffffu, n0 != m0 || n1 != m1)) {

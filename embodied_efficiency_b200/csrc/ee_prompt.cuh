@@ -10,9 +10,24 @@
 // read or write outside the tensors.
 #pragma once
 
+#include <type_traits>
+
 #include "ee_common.cuh"
 
 namespace ee {
+
+// What a row's weights 2^(x - reference) are taken relative to, given its
+// largest scaled score x. Weights are rounded to 16 bits for their product with
+// v, and fp16 ends at 2^-24: beside a largest weight of 1, keys 17 nats below
+// it would be lost however many they are. So for fp16 the reference lies BITS
+// below x and the weights are that much larger; their sum is too, and the
+// division drops the factor. (Not from 2^20 on, where fp32 no longer takes
+// BITS off exactly enough; bf16 has fp32's range.)
+template <typename T, int BITS>
+EE_DEV float prompt_reference(float x) {
+  if (!std::is_same<T, __half>::value) return x;
+  return fabsf(x) < 1048576.f ? x - (float)BITS : x;
+}
 
 struct PromptArgs {
   const void *q, *k, *v;

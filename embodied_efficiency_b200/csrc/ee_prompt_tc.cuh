@@ -27,8 +27,8 @@
 // 257 to 816 tokens, hd 64: 395 -> 415 us).
 //
 // The running maximum m is a reference, not the exact maximum: it moves only
-// when a row's maximum exceeds it by more than 8 (a factor of 2^8), so O is rarely rescaled
-// (the weights stay below 2^8 and the result O / l does not depend on m). S(j)
+// when a row's maximum exceeds the one it was set by by more than 8 (a factor of 2^8), so O is rarely rescaled
+// (the weights stay below 2^8, 2^15 for fp16, see prompt_reference, and the result O / l does not depend on m). S(j)
 // of a tile is issued after its O += P(j-1) V(j-1), so the wait for S(j) also
 // says that O may be rescaled.
 //
@@ -505,7 +505,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       if (lane == 0) item_done(i);
       const bool mine = rtok < a.tpt && tok < qlen;
       const int lim = (p.causal ? min(klen, klen - qlen + tok + 1) : klen) - key0;  // keys of this part the row sees
-      float m = -INFINITY, l = 0.f;
+      float m = -INFINITY, top = -INFINITY, l = 0.f;  // top: the score at which m moves
       for (int j = 0; j < nt; ++j) {
         ok = __all_sync(0xffffffffu, mbar_wait(b_s + 8 * t, (uint32_t)(ns & 1), a.timeout_ns));
         if (!ok) break;
@@ -542,9 +542,11 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         }
         const float mx = fmaxf(max3(x[0], x[1], x[2]), x[3]) * p.scale_log2;
         float f = 1.f;
-        if (mx > m + 8.f) {  // also from -inf, with f = 0: nothing to rescale yet
-          f = ex2(m - mx);
-          m = mx;
+        if (mx > top) {  // also from -inf, with f = 0: nothing to rescale yet
+          const float to = prompt_reference<T, 7>(mx);
+          f = ex2(m - to);
+          m = to;
+          top = mx + 8.f;
         }
         const bool rescale = __any_sync(0xffffffffu, f != 1.f) && j > 0;
         if (SEP && j > 0) {  // O += P(j-1) V(j-1) is done: P may be written, O rescaled
