@@ -49,8 +49,29 @@ struct Call {
   void* stream() const { return c10::cuda::getCurrentCUDAStream(dev).stream(); }
 };
 
+// Lets the interpreter's other threads run while a call allocates and
+// launches: both may wait for the GPU (an allocation that needs a
+// synchronisation, a launch queue that is full). Taken once the operands have
+// been looked at; results become Python objects after its end.
+class NoGil {
+  PyThreadState* state_ = PyEval_SaveThread();
+
+ public:
+  NoGil() = default;
+  NoGil(const NoGil&) = delete;
+  ~NoGil() { PyEval_RestoreThread(state_); }
+};
+
 PyObject* none() { Py_RETURN_NONE; }
 PyObject* give(int rc, const Tensor& t) { return rc == EE_OK ? THPVariable_Wrap(t) : none(); }
+PyObject* give(int rc, const Tensor& t, const Tensor& u) {
+  if (rc != EE_OK) return none();
+  PyObject* r = PyTuple_New(2);
+  if (!r) return nullptr;
+  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(t));
+  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(u));
+  return r;
+}
 
 bool heads_ok(const Tensor& t) {
   return t.dim() == 3 && act_type(t.scalar_type()) && t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
@@ -112,12 +133,17 @@ PyObject* int8_linear(PyObject*, PyObject* const* a, Py_ssize_t argc) {
   const auto lead = x->sizes().slice(0, x->dim() - 1);
   Linear l;
   if (!linear(c, a + 1, x->scalar_type(), m, lead, l) || !c.need(l.k == k)) return none();
-  const Tensor y = output(*x, lead, l.n, x->scalar_type());
-  const size_t need = ee_int8_linear_workspace_bytes(m, k);
-  const Tensor ws = at::empty({(int64_t)need}, x->options().dtype(at::kChar));
-  return give(ee_int8_linear(x->data_ptr(), k, l.weight, l.scales, l.bias, l.residual, y.data_ptr(), ws.data_ptr(), need,
-                             m, l.n, k, l.scale_dtype, act_code(x->scalar_type()), l.epilogue, c.stream()),
-              y);
+  Tensor y;
+  int rc;
+  {
+    NoGil others;
+    y = output(*x, lead, l.n, x->scalar_type());
+    const size_t need = ee_int8_linear_workspace_bytes(m, k);
+    const Tensor ws = at::empty({(int64_t)need}, x->options().dtype(at::kChar));
+    rc = ee_int8_linear(x->data_ptr(), k, l.weight, l.scales, l.bias, l.residual, y.data_ptr(), ws.data_ptr(), need, m,
+                        l.n, k, l.scale_dtype, act_code(x->scalar_type()), l.epilogue, c.stream());
+  }
+  return give(rc, y);
 }
 
 // int8_matmul(xq, x_scale, weight, scales, bias, gelu, residual, dtype)
@@ -135,11 +161,16 @@ PyObject* int8_matmul(PyObject*, PyObject* const* a, Py_ssize_t argc) {
   if (!linear(c, a + 2, type, m, lead, l) ||
       !c.need(l.k == k && sx->scalar_type() == at::kFloat && sx->numel() == m && sx->is_contiguous() && aligned(*sx)))
     return none();
-  const Tensor y = output(*x, lead, l.n, type);
-  return give(ee_int8_gemm(static_cast<const int8_t*>(x->data_ptr()), static_cast<const float*>(sx->data_ptr()), l.weight,
-                           l.scales, l.bias, l.residual, y.data_ptr(), m, l.n, k, l.scale_dtype, act_code(type),
-                           l.epilogue, c.stream()),
-              y);
+  Tensor y;
+  int rc;
+  {
+    NoGil others;
+    y = output(*x, lead, l.n, type);
+    rc = ee_int8_gemm(static_cast<const int8_t*>(x->data_ptr()), static_cast<const float*>(sx->data_ptr()), l.weight,
+                      l.scales, l.bias, l.residual, y.data_ptr(), m, l.n, k, l.scale_dtype, act_code(type), l.epilogue,
+                      c.stream());
+  }
+  return give(rc, y);
 }
 
 // quantize_tokens(x) -> (codes, scales)
@@ -151,15 +182,16 @@ PyObject* quantize_tokens(PyObject*, PyObject* const* a, Py_ssize_t argc) {
   const int64_t k = x->size(-1);
   if (!c.need(k >= 16 && k % 16 == 0 && k <= 131056 && x->numel() > 0)) return none();
   const auto lead = x->sizes().slice(0, x->dim() - 1);
-  const Tensor q = at::empty(x->sizes(), x->options().dtype(at::kChar)), s = output(*x, lead, 1, at::kFloat);
-  if (ee_quantize_tokens(x->data_ptr(), k, static_cast<int8_t*>(q.data_ptr()), static_cast<float*>(s.data_ptr()),
-                         x->numel() / k, k, act_code(x->scalar_type()), c.stream()) != EE_OK)
-    return none();
-  PyObject* t = PyTuple_New(2);
-  if (!t) return nullptr;
-  PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(q));
-  PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(s));
-  return t;
+  Tensor q, s;
+  int rc;
+  {
+    NoGil others;
+    q = at::empty(x->sizes(), x->options().dtype(at::kChar));
+    s = output(*x, lead, 1, at::kFloat);
+    rc = ee_quantize_tokens(x->data_ptr(), k, static_cast<int8_t*>(q.data_ptr()), static_cast<float*>(s.data_ptr()),
+                            x->numel() / k, k, act_code(x->scalar_type()), c.stream());
+  }
+  return give(rc, q, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -193,17 +225,20 @@ PyObject* rotary_embed(PyObject*, PyObject* const* a, Py_ssize_t argc) {
               (pos->dim() == 2 ? pos->size(0) == axes && pos->size(1) == t : pos->dim() == 1 && axes == 1 && pos->size(0) == t) &&
               tab->scalar_type() == at::kLong && tab->numel() == hd / 2 && tab->is_contiguous()))
     return none();
-  const Tensor qo = at::empty(q->sizes(), q->options()), ko = at::empty(k->sizes(), k->options());
-  if (ee_rotary(q->data_ptr(), q->stride(0), q->stride(1), qo.data_ptr(), qo.stride(0), qo.stride(1), k->data_ptr(),
-                k->stride(0), k->stride(1), ko.data_ptr(), ko.stride(0), ko.stride(1), pos->data_ptr(), t, p64 ? 64 : 32,
-                static_cast<const uint64_t*>(tab->data_ptr()), t, (int32_t)q->size(1), (int32_t)k->size(1), (int32_t)hd,
-                sections, (int32_t)axes, a[5] == Py_True, act_code(q->scalar_type()), c.stream()) != EE_OK)
-    return none();
-  PyObject* r = PyTuple_New(2);
-  if (!r) return nullptr;
-  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(qo));
-  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(ko));
-  return r;
+  const bool interleaved = a[5] == Py_True;
+  Tensor qo, ko;
+  int rc;
+  {
+    NoGil others;
+    qo = at::empty(q->sizes(), q->options());
+    ko = at::empty(k->sizes(), k->options());
+    rc = ee_rotary(q->data_ptr(), q->stride(0), q->stride(1), qo.data_ptr(), qo.stride(0), qo.stride(1), k->data_ptr(),
+                   k->stride(0), k->stride(1), ko.data_ptr(), ko.stride(0), ko.stride(1), pos->data_ptr(), t,
+                   p64 ? 64 : 32, static_cast<const uint64_t*>(tab->data_ptr()), t, (int32_t)q->size(1),
+                   (int32_t)k->size(1), (int32_t)hd, sections, (int32_t)axes, interleaved, act_code(q->scalar_type()),
+                   c.stream());
+  }
+  return give(rc, qo, ko);
 }
 
 // ---------------------------------------------------------------------------
@@ -232,18 +267,24 @@ PyObject* prompt_attention(PyObject*, PyObject* const* a, Py_ssize_t argc) {
               table(kl, n) && (ck || tk == tq) && tq < (1 << 30) && tk < (1 << 30) && hq < 65536 && n < (1 << 30) &&
               scale > 0.f && scale < 3.0e38f && (hd == 64 || hd == 128)))
     return none();
-  const Tensor out = at::empty(q->sizes(), q->options());
-  const size_t need = ee_prompt_attention_workspace_bytes(tq, tk, (int32_t)n, (int32_t)hq, (int32_t)hk, (int32_t)hd);
-  Tensor ws;
-  if (need) ws = at::empty({(int64_t)need}, q->options().dtype(at::kByte));
-  return give(ee_prompt_attention(q->data_ptr(), q->stride(0), q->stride(1), k->data_ptr(), k->stride(0), k->stride(1),
-                                  v->data_ptr(), v->stride(0), v->stride(1), out.data_ptr(), out.stride(0), out.stride(1),
-                                  static_cast<const int32_t*>(cq->data_ptr()),
-                                  ck ? static_cast<const int32_t*>(ck->data_ptr()) : nullptr,
-                                  kl ? static_cast<const int32_t*>(kl->data_ptr()) : nullptr, tq, tk, (int32_t)n,
-                                  (int32_t)hq, (int32_t)hk, (int32_t)hd, a[6] == Py_True, scale,
-                                  act_code(q->scalar_type()), need ? ws.data_ptr() : nullptr, need, c.stream()),
-              out);
+  const bool causal = a[6] == Py_True;
+  Tensor out;
+  int rc;
+  {
+    NoGil others;
+    out = at::empty(q->sizes(), q->options());
+    const size_t need = ee_prompt_attention_workspace_bytes(tq, tk, (int32_t)n, (int32_t)hq, (int32_t)hk, (int32_t)hd);
+    Tensor ws;
+    if (need) ws = at::empty({(int64_t)need}, q->options().dtype(at::kByte));
+    rc = ee_prompt_attention(q->data_ptr(), q->stride(0), q->stride(1), k->data_ptr(), k->stride(0), k->stride(1),
+                             v->data_ptr(), v->stride(0), v->stride(1), out.data_ptr(), out.stride(0), out.stride(1),
+                             static_cast<const int32_t*>(cq->data_ptr()),
+                             ck ? static_cast<const int32_t*>(ck->data_ptr()) : nullptr,
+                             kl ? static_cast<const int32_t*>(kl->data_ptr()) : nullptr, tq, tk, (int32_t)n,
+                             (int32_t)hq, (int32_t)hk, (int32_t)hd, causal, scale, act_code(q->scalar_type()),
+                             need ? ws.data_ptr() : nullptr, need, c.stream());
+  }
+  return give(rc, out);
 }
 
 // C++ exceptions (out of memory in an allocation) become Python's: the Python
