@@ -42,6 +42,12 @@ def _out(out, like, name):
     s = out.stride()
     if s[2] != 1 or s[0] % 8 or s[1] % 8 or out.data_ptr() % 16:
         raise ValueError(f"{name} needs a contiguous last dimension, strides of 8 elements and a 16-byte boundary")
+    reach = out.shape[2]  # elements that the dimensions of smaller strides cover
+    for stride, size in sorted(zip(s[:2], out.shape[:2])):
+        if size > 1 and out.numel():
+            if stride < reach:
+                raise ValueError(f"elements of {name} overlap in memory (strides {s}): it cannot be written")
+            reach += stride * (size - 1)
     return out, s
 
 
@@ -90,9 +96,10 @@ def rotary_embed(q, k, positions, sections, base: float = 10000.0, interleaved: 
     ``positions[axis][t] * base^(-2i / head_dim)``, the first ``sections[0]`` pairs by axis 0, the next
     ``sections[1]`` by axis 1 and so on. Pairs are (i, i + head_dim / 2), or (2i, 2i + 1) when ``interleaved``.
     ``positions`` is int32 or int64 [axes, T] ([T] for one axis); an angle is off by less than 2^-22 (fp32's rounding of
-    angle, sine and cosine) and ``|position| * 2^-62``: as much again only from 2^40 on. Returns (q, k) turned, as new tensors or in ``out`` = (q_out, k_out), which may be the inputs
-    themselves. head_dim 32, 64, 128 or 256; bf16 / fp16. The first call for a head_dim and base on a device copies a
-    small table to it and has to come before a stream capture."""
+    angle, sine and cosine) and ``|position| * 2^-62``: as much again only from 2^40 on. Returns (q, k) turned, as new
+    tensors or in ``out`` = (q_out, k_out), which may be the inputs themselves but not overlap them, or one another, in
+    any other way. head_dim 32, 64, 128 or 256; bf16 / fp16. The first call for a head_dim and base on a device copies
+    a small table to it and has to come before a stream capture."""
     if out is None and q is not None and k is not None:
         tab = _TURNS.get((q.device, q.shape[-1] // 2, base))
         if tab is not None:
@@ -161,7 +168,7 @@ def prompt_attention(q, k, v, cu_q, cu_k=None, k_lens=None, causal: bool = True,
     head_dim^-0.5. Offsets are int32 on the device, not decreasing; what they claim beyond the tensors is cut off.
     A masked key counts with weight 0, so ``k`` may hold anything there, while ``v`` has to be finite on the keys of a
     sequence (0 * inf is NaN); beyond them, nothing is used.
-    Returns [Tq, heads, head_dim], new or ``out``; rows that belong to no sequence are not written.
+    Returns [Tq, heads, head_dim], new or ``out`` (which shares no memory with the inputs); rows that belong to no sequence are not written.
     head_dim 64 or 128; bf16 / fp16."""
     if out is None:
         done = (_lib._native or _lib.native()).prompt_attention(q, k, v, cu_q, cu_k, k_lens, causal, scale)
