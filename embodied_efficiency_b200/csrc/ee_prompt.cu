@@ -41,6 +41,8 @@ EE_DEV long long pr_steps(const PromptArgs& a, const PromptSeq& s, int& per_item
 
 // The list of steps: its length, and for every thread the steps before its
 // share of the sequences (`per` each, consecutive). All threads of the CTA.
+// visit(b, s, before): each of the thread's sequences and the steps of its own
+// ones before it.
 template <int THREADS>
 struct PrList {
   long long before[THREADS];
@@ -53,7 +55,7 @@ EE_DEV long long pr_list(const PromptArgs& a, PrList<THREADS>* sh, int per, Visi
   for (int b = tid * per; b < min((tid + 1) * per, a.n_seq); ++b) {
     int n;
     const PromptSeq s = prompt_seq(a, b);
-    visit(s, mine);  // the sequence and the steps of the thread's own before it
+    visit(b, s, mine);
     mine += pr_steps(a, s, n);
   }
   long long inc = mine;
@@ -127,7 +129,7 @@ __global__ void __launch_bounds__(32 * pr_warps<HD>(), 1) prompt_rows_kernel(con
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3, mi = lane >> 3;
   const int per = (a.n_seq + NT - 1) / NT;
-  const long long total = pr_list<NT>(a, &sh, per, [](const PromptSeq&, long long) {});
+  const long long total = pr_list<NT>(a, &sh, per, [](int, const PromptSeq&, long long) {});
   const long long share = pr_share(total, (int)gridDim.x * NW);
   const long long me = (long long)warp * gridDim.x + blockIdx.x;  // neighbours in the list on different SMs
   const long long first = me * share;
@@ -502,26 +504,29 @@ __global__ void __launch_bounds__(kPrJoin) prompt_join_kernel(const __grid_const
   __shared__ JoinSmem<HD> sh;
   __shared__ PromptSeq seq;
   __shared__ long long seq_first;
-  __shared__ int found;
+  __shared__ int found;  // the token's sequence: the first that claims it, should a table that decreases have several
   const int tok = blockIdx.x;
-  if (threadIdx.x == 0) found = 0;
+  if (threadIdx.x == 0) found = 0x7fffffff;
+  __syncthreads();
   const int per = (a.n_seq + kPrJoin - 1) / kPrJoin;
   PromptSeq hit{};
-  long long hit_at = -1;  // steps of the thread's own sequences before the token's
-  const long long total = pr_list<kPrJoin>(a, &list, per, [&](const PromptSeq& s, long long before) {
-    if (tok >= s.q0 && tok < s.q0 + s.qlen) {
+  int hit_b = -1;
+  long long hit_at = 0;  // steps of the thread's own sequences before the token's
+  const long long total = pr_list<kPrJoin>(a, &list, per, [&](int b, const PromptSeq& s, long long before) {
+    if (hit_b < 0 && tok >= s.q0 && tok < s.q0 + s.qlen) {
       hit = s;
+      hit_b = b;
       hit_at = before;
+      atomicMin(&found, b);
     }
   });
-  if (hit_at >= 0) {
+  if (hit_b >= 0 && hit_b == found) {
     seq = hit;
     seq_first = list.before[threadIdx.x] + hit_at;
-    found = 1;
   }
   __syncthreads();
-  pdl_entry();          // by every thread, the ones that return too: this grid must not end before the one it follows
-  if (!found) return;  // rows outside the sequences stay as they were
+  pdl_entry();  // by every thread, the ones that return too: this grid must not end before the one it follows
+  if (found == 0x7fffffff) return;  // rows outside the sequences stay as they were
   const PromptSeq s = seq;
   int steps;
   pr_steps(a, s, steps);
