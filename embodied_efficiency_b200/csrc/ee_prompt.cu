@@ -1,6 +1,7 @@
 // ee_prompt.cu -- C ABI: attention over packed prompts (causal or full,
 // grouped heads, keys that may reach further back than the queries).
 #include <atomic>
+#include <cfloat>
 
 #include "ee_host.h"
 #include "ee_prompt.cuh"
@@ -684,7 +685,8 @@ int ee_prompt_attention(const void* q, int64_t q_tok, int64_t q_head, const void
   if (head_dim != 64 && head_dim != 128) return EE_ERR_UNSUPPORTED;
   if (tq < 0 || tk < 0 || n_seq < 0 || n_q < 1 || n_kv < 1 || n_q % n_kv != 0) return EE_ERR_SHAPE;
   if (tq > 0x7fffff00 || tk > 0x7fffff00 || n_kv > 65535 || n_q > 65535) return EE_ERR_SHAPE;
-  if (!(scale > 0.f) || scale > 3.0e38f) return EE_ERR_ARG;
+  const float scale_log2 = scale * 1.4426950408889634f;
+  if (!(scale > 0.f) || !(scale_log2 <= FLT_MAX)) return EE_ERR_ARG;
   if (tq == 0 || n_seq == 0) return EE_OK;
   if (!q || !out || !cu_q || (tk && (!k || !v)) || (!cu_k && tk != tq)) return EE_ERR_ARG;
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out)) return EE_ERR_ALIGN;
@@ -706,7 +708,7 @@ int ee_prompt_attention(const void* q, int64_t q_tok, int64_t q_head, const void
   a.tq = (int)tq; a.tk = (int)tk; a.n_seq = n_seq;
   a.n_q = n_q; a.n_kv = n_kv; a.group = n_q / n_kv;
   a.causal = causal != 0;
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.scale_log2 = scale_log2;
   a.splits = pl.splits;
   a.part = reinterpret_cast<float*>(workspace);
   a.stat = a.part + (size_t)prompt_partials(pl, tq, n_q, head_dim) * head_dim;

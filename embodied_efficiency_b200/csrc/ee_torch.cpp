@@ -265,7 +265,7 @@ PyObject* prompt_attention(PyObject*, PyObject* const* a, Py_ssize_t argc) {
   if (!c.need(k->sizes() == v->sizes() && k->scalar_type() == q->scalar_type() && v->scalar_type() == q->scalar_type() &&
               k->size(2) == hd && tq > 0 && n >= 1 && hk >= 1 && hq % hk == 0 && table(cq, n + 1) && table(ck, n + 1) &&
               table(kl, n) && (ck || tk == tq) && tq < (1 << 30) && tk < (1 << 30) && hq < 65536 && n < (1 << 30) &&
-              scale > 0.f && scale < 3.0e38f && (hd == 64 || hd == 128)))
+              scale > 0.f && scale < 2.0e38f && (hd == 64 || hd == 128)))
     return none();
   const bool causal = a[6] == Py_True;
   Tensor out;

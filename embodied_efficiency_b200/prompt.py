@@ -158,6 +158,9 @@ def _offsets(t, n, name):
     return t if t.is_contiguous() else t.contiguous()
 
 
+_MAX_SCALE = 2.0 ** 128 / 1.4427  # scale * log2(e) is an fp32 value
+
+
 def prompt_attention(q, k, v, cu_q, cu_k=None, k_lens=None, causal: bool = True, scale: float | None = None, out=None):
     """Attention over packed prompts (``ee_prompt_attention``): sequence b's queries, rows ``cu_q[b]`` to
     ``cu_q[b + 1]`` of ``q`` [Tq, heads, head_dim], against its keys, rows ``cu_k[b]`` to ``cu_k[b + 1]`` of ``k`` and
@@ -191,8 +194,8 @@ def prompt_attention(q, k, v, cu_q, cu_k=None, k_lens=None, causal: bool = True,
     if cu_k is None and tk != tq:
         raise ValueError(f"{tk} keys for {tq} queries need offsets of their own (cu_k)")
     scale = hd ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < math.inf:
-        raise ValueError(f"scale must be finite and above 0, got {scale}")
+    if not 2.0 ** -126 <= scale <= _MAX_SCALE:
+        raise ValueError(f"scale must be finite and above 0 (fp32, 2^-126 to {_MAX_SCALE:.4g}), got {scale}")
     cu_q = _offsets(cu_q, n + 1, "cu_q")
     cu_k = None if cu_k is None else _offsets(cu_k, n + 1, "cu_k")
     k_lens = None if k_lens is None else _offsets(k_lens, n, "k_lens")

@@ -232,7 +232,8 @@ int ee_rotary(const void* q, int64_t q_tok, int64_t q_head, void* q_out, int64_t
  * gives zeros. Offsets and lengths live on the device (int32) and are cut to
  * tq / tk; rows of `out` that belong to no sequence stay as they were.
  * Sequences may have no queries or no keys. Strides in elements, multiples of
- * 8; the last dimension contiguous. head_dim 64 or 128; scale > 0 (finite).
+ * 8; the last dimension contiguous. head_dim 64 or 128; scale > 0, and
+ * scale * log2(e) finite in fp32.
  * Keys a sequence does not have are never read into a result, whatever they
  * hold; inside a sequence, values under the causal mask have to be finite (a
  * masked weight is a product with 0). fp32 statistics and sums, weights
