@@ -10,6 +10,7 @@ import ctypes
 import importlib.util
 import os
 import threading
+import warnings
 
 import torch
 from torch.autograd import forward_ad
@@ -138,19 +139,39 @@ def load():
 _native = None
 
 
+class _NoNative:
+    """Takes no call: stands where the extension module cannot."""
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
 def native():
     """The extension module ``lib/ee_torch.so``: the usual calls of the prompt-layer operators without the
-    interpreter. Its functions return None for any other call (see csrc/ee_torch.cpp)."""
+    interpreter. Its functions return None for any other call (see csrc/ee_torch.cpp), which the Python functions then
+    make through ctypes on the same kernels; so they do, after a warning, where the module is missing or was built for
+    another torch."""
     global _native
     if _native is None:
         load()
-        path = _build.TORCH_LIB
-        if not os.path.exists(path):
-            raise RuntimeError(f"{path} is missing: build it with `python -m embodied_efficiency_b200.build`")
-        spec = importlib.util.spec_from_file_location("ee_torch", path)
-        _native = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(_native)
+        _native = _load_native(_build.TORCH_LIB)
     return _native
+
+
+def _load_native(path):
+    try:
+        with open(path, "rb"):
+            pass
+        spec = importlib.util.spec_from_file_location("ee_torch", path)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        if mod.torch_version != _build.torch_version():
+            raise ImportError(f"built for {mod.torch_version}, this is {_build.torch_version()}")
+        return mod
+    except (ImportError, OSError, AttributeError) as e:
+        warnings.warn(f"{path} is not used, calls go through the interpreter ({e}): build it with "
+                      "`python -m embodied_efficiency_b200.build`", RuntimeWarning, stacklevel=3)
+        return _NoNative()
 
 
 def strerror(code: int) -> str:

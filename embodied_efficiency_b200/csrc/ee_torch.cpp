@@ -306,4 +306,11 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "ee_torch", nullptr, -1, methods, n
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit_ee_torch() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit_ee_torch() {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "torch_version", EE_TORCH_VERSION) < 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}
