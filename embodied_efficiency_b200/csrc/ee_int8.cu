@@ -110,10 +110,10 @@ __global__ void __launch_bounds__(kQThreads) quantize_tokens_kernel(const T* __r
 
 template <typename T>
 static int launch_quantize(const T* x, int8_t* xq, float* sx, long long rows, int cols, long long ldx, cudaStream_t s) {
-  // warps per row: enough that a row stays in registers (52224 x 2048: 56 us, 5.7 TB/s, with one;
-  // a fifth more with two), and while the rows
-  // alone leave the GPU empty more of them, as long as each lane has a chunk (one row of 2048: 3.6 us with one, 1.9
-  // with four)
+  // warps per row: enough that a row stays in registers (52224 x 2048: 54 us, 6.0 TB/s, with one; a fifth more with
+  // two), and while the rows alone leave the GPU empty more of them, as long as each lane has a chunk (one row of 2048:
+  // 3.6 us with one, 1.9 with four). In between a warp has one row and stops: 6528 x 2048 takes 10.4 us for 40 MB, 816
+  // CTAs in 592 places with no next row in flight
   const int per = 32 * kQChunks, nch = cols / 8;
   int w = nch <= per ? 1 : (nch <= 2 * per ? 2 : (nch <= 4 * per ? 4 : 8));
   while (w < 8 && rows * w <= 8 * device_sms() && nch > 32 * w) w *= 2;

@@ -148,7 +148,8 @@ EE_DEV void sts16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d)
 // warps. Two accumulators of 256 TMEM columns, so a tile's epilogue runs under
 // the next tile's MMAs. Outputs are staged as swizzled [32 rows][64 columns]
 // blocks and stored by TMA.
-// Measured: 52224 x 8192 x 2048: 582 us, 3.0 POP/s (with the GELU 650), 8192^3:
+// Measured, single passes after a pause: 52224 x 8192 x 2048: 582 us, 3.0 POP/s
+// (with the GELU 650; back to back, at the power limit's clocks, 790), 8192^3:
 // 333 us, 3.3 POP/s, twice the measured 16-bit GEMM rate. (16 epilogue warps and
 // a stage less were slower with the GELU: 677 us.)
 constexpr int kI8Stages = 5, kI8EpiWarps = 8;

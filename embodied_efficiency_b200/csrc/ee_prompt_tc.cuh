@@ -17,9 +17,14 @@
 // share of the exponentials as polynomials on the FMA pipe was slower at every
 // share: 411 -> 428 / 472 / 530 us at hd 64 for 1/8, 1/4, 1/2 of them.)
 //
-// Measured: 8192 causal tokens, 16 / 4 heads of 128: 225 us, 1220 TFLOP/s,
-// 0.76 of the measured GEMM rate; 16 / 4 heads of 64 without a mask: 410 us,
-// the MUFU 74 % busy while an SM has work. What bounds it is one thread's row:
+// P is rounded to 16 bits, as the product takes it, while the sum l keeps the
+// unrounded weights: half a step each, in either direction, which over many
+// keys leaves 1.3 times the error of a plain fp32 form (fp16, heads of 64:
+// 2.8e-4 to 2.1e-4 relative); a second product for the low bits would double P V.
+//
+// Measured: 8192 causal tokens, 16 / 4 heads of 128: 225 us in a single pass
+// after a pause, 1220 TFLOP/s, 0.76 of the measured GEMM rate (back to back, at
+// lower clocks, 257); 16 / 4 heads of 64 without a mask: 410 us, the MUFU 74 % busy while an SM has work. What bounds it is one thread's row:
 // 3000 cycles per pair of blocks at hd 64 where the MUFU needs 2048. (Two
 // threads a row need 130 registers and have 104: 470 -> 720 us at hd 128.)
 // A last tile without a neighbour leaves its item's second half idle; halving

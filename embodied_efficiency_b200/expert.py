@@ -317,7 +317,8 @@ class ActionExpert(nn.Module):
     def encode_packed(self, prefix: torch.Tensor, cu: torch.Tensor):
         """Per-layer K/V of prefixes of different lengths: packed rows [tokens, d] and their int32 offsets
         ``cu`` [batch + 1] on the device. ``flow_sample`` and ``GraphedSampler`` take the result in place of
-        ``encode``'s and run layer by layer, the cross-attention on ``prompt_attention``."""
+        ``encode``'s and run layer by layer, the cross-attention on ``prompt_attention`` (so heads of 64 or 128, in bf16
+        or fp16)."""
         prefix = prefix.to(self.out_norm.weight.dtype)
         return [blk.precompute_kv_packed(prefix, cu) for blk in self.blocks]
 

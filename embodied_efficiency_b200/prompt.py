@@ -171,6 +171,8 @@ def prompt_attention(q, k, v, cu_q, cu_k=None, k_lens=None, causal: bool = True,
     head_dim^-0.5. Offsets are int32 on the device, not decreasing; what they claim beyond the tensors is cut off.
     A masked key counts with weight 0, so ``k`` may hold anything there, while ``v`` has to be finite on the keys of a
     sequence (0 * inf is NaN); beyond them, nothing is used.
+    One kernel serves the whole call, chosen by the mean of queries per sequence and key head: long prompts are faster
+    in a call of their own than beside many single tokens.
     Returns [Tq, heads, head_dim], new or ``out`` (which shares no memory with the inputs); rows that belong to no sequence are not written.
     head_dim 64 or 128; bf16 / fp16."""
     if out is None:
