@@ -63,8 +63,7 @@ _PI = decimal.Decimal("3.1415926535897932384626433832795028841971693993751058209
 def _turn_fractions(half: int, base: float) -> list:
     """round(base^(-i / half) / 2 pi * 2^64) for i < half. In 50 digits: in double, whose 53 bits end 11 short of the
     table's, a position of 2^40 would turn 2^-15 of a turn too far."""
-    with decimal.localcontext() as ctx:
-        ctx.prec = 50
+    with decimal.localcontext(decimal.Context(prec=50)):  # of its own: a caller's may trap inexact results
         log, scale = decimal.Decimal(float(base)).ln(), decimal.Decimal(2 ** 64) / (2 * _PI)
         return [int((scale * (log * -i / half).exp()).to_integral_value()) for i in range(half)]
 

@@ -49,6 +49,14 @@ def test_table_is_the_rounded_frequency(half, base):
         assert 0 < have < 2 ** 63 and abs(have - want * 2 ** 64) <= Fraction(1, 2) + Fraction(1, 10 ** 20)
 
 
+def test_table_in_another_decimal_context():
+    import decimal
+    from embodied_efficiency_b200.prompt import _turn_fractions
+    want = _turn_fractions(16, 10000.0)
+    with decimal.localcontext(decimal.Context(prec=5, rounding=decimal.ROUND_UP, traps=[decimal.Inexact])):
+        assert _turn_fractions(16, 10000.0) == want
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("base", [10000.0, 500000.0])
 @pytest.mark.parametrize("interleaved", [False, True])
