@@ -10,7 +10,7 @@ pytestmark = pytest.mark.gpu
 
 
 def test_a_launch_that_waits_lets_other_threads_run(cuda):
-    """A stream that is held up for half a second by a host function (libc's usleep: it needs no interpreter) takes
+    """A stream that is held up for 0.9 seconds by a host function (libc's usleep: it needs no interpreter) takes
     about a thousand launches; the next launch waits for it on the host. Other Python threads go on meanwhile."""
     from embodied_efficiency_b200 import quantize_tokens
     cudart, libc = ctypes.CDLL("libcudart.so.12"), ctypes.CDLL(None)
@@ -35,7 +35,7 @@ def test_a_launch_that_waits_lets_other_threads_run(cuda):
     try:
         with torch.cuda.stream(side):
             start = time.perf_counter()
-            assert launch(side.cuda_stream, ctypes.cast(libc.usleep, ctypes.c_void_p), 500_000) == 0
+            assert launch(side.cuda_stream, ctypes.cast(libc.usleep, ctypes.c_void_p), 900_000) == 0
             for _ in range(5000):
                 got = quantize_tokens(x)[0]
             took = time.perf_counter() - start
@@ -44,5 +44,5 @@ def test_a_launch_that_waits_lets_other_threads_run(cuda):
         other.join()
     torch.cuda.synchronize()
     assert torch.equal(got, want)
-    assert took > 0.3, "no launch had to wait: nothing is shown"
-    assert max(gaps) < 0.15, max(gaps)
+    assert took > 0.6, "no launch had to wait: nothing is shown"
+    assert max(gaps) < 0.3, max(gaps)

@@ -22,12 +22,12 @@ def short_waits(cuda):
 
 @pytest.mark.parametrize("hd", [64, 128])
 def test_a_walk_longer_than_the_limit(short_waits, cuda, hd):
-    """One item per SM that walks 626 blocks of keys, a millisecond or more: its second tile is empty, and the last
+    """One item per SM that walks 1251 blocks of keys, a millisecond or more: its second tile is empty, and the last
     block has one key, so that two roles wait for the whole walk. Weights' and result's rounding to 16 bits, fp32 sums
     of nk / 16 steps (2^-24 each), scores to 2^-22 of sum |q k|, which moves a weight twice."""
     from embodied_efficiency_b200 import prompt_attention
     from embodied_efficiency_b200.wq_gemm import gemm_status
-    nq, nk, heads = 100, 80001, torch.cuda.get_device_properties(cuda).multi_processor_count
+    nq, nk, heads = 100, 160001, torch.cuda.get_device_properties(cuda).multi_processor_count
     g = torch.Generator(device=cuda).manual_seed(hd)
     q = (torch.randn(nq, heads, hd, generator=g, device=cuda) * 1.5).bfloat16()
     k, v = (torch.randn(nk, 1, hd, generator=g, device=cuda).bfloat16() for _ in range(2))
