@@ -24,18 +24,20 @@
 //
 // Measured: 8192 causal tokens, 16 / 4 heads of 128: 225 us in a single pass
 // after a pause, 1220 TFLOP/s, 0.76 of the measured GEMM rate (back to back, at
-// lower clocks, 257); 16 / 4 heads of 64 without a mask: 410 us, the MUFU 74 % busy while an SM has work. What bounds it is one thread's row:
-// 3000 cycles per pair of blocks at hd 64 where the MUFU needs 2048. (Two
-// threads a row need 130 registers and have 104: 470 -> 720 us at hd 128.)
+// lower clocks, 257); 16 / 4 heads of 64 without a mask: 410 us, the MUFU 74 %
+// busy while an SM has work. What bounds it is one thread's row: 3000 cycles
+// per pair of blocks at hd 64 where the MUFU needs 2048. (Two threads a row
+// need 130 registers and have 104: 470 -> 720 us at hd 128.)
 // A last tile without a neighbour leaves its item's second half idle; halving
 // its keys over both halves and joining the sums was slower (128 prompts of
 // 257 to 816 tokens, hd 64: 395 -> 415 us).
 //
 // The running maximum m is a reference, not the exact maximum: it moves only
-// when a row's maximum exceeds the one it was set by by more than 8 (a factor of 2^8), so O is rarely rescaled
-// (the weights stay below 2^8, 2^15 for fp16, see prompt_reference, and the result O / l does not depend on m). S(j)
-// of a tile is issued after its O += P(j-1) V(j-1), so the wait for S(j) also
-// says that O may be rescaled.
+// when a row's maximum exceeds the one that set it by more than 8 (a factor of
+// 2^8), so O is rarely rescaled (the weights stay below 2^8, for fp16 2^15, see
+// prompt_reference, and the result O / l does not depend on m). S(j) of a tile
+// is issued after its O += P(j-1) V(j-1), so the wait for S(j) also says that O
+// may be rescaled.
 //
 // Persistent: one CTA per SM takes items c, 2G - 1 - c, 2G + c, ... of the G
 // CTAs (a snake, longest items first), and the next item's loads and first
@@ -77,7 +79,8 @@ template <int HD> constexpr int pt_slots() { return HD == 128 ? 4 : 8; }
 template <int HD> constexpr uint32_t pt_tile() { return 128u * HD * 2; }
 template <int HD> constexpr uint32_t pt_off_out() { return (2 + pt_slots<HD>()) * pt_tile<HD>(); }  // 4 KB per softmax warp
 template <int HD> constexpr uint32_t pt_off_bar() { return pt_off_out<HD>() + 8 * 4096; }
-// barriers: full / empty per load of K / V, Q full / empty, S / P (two halves) / S free / O / O free per tile, V to fix / fixed, item full / empty, MMAs done after a failure
+// barriers: full / empty per load of K / V, Q full / empty, S / P (two halves) / S free / O / O free per tile, V to fix /
+// fixed, item full / empty, MMAs done after a failure
 template <int HD> constexpr uint32_t pt_off_info() { return pt_off_bar<HD>() + 8 * (2 * kPtLoads + 17 + 2 * kPtInfo) + 8; }
 template <int HD> constexpr uint32_t pt_off_beat() { return pt_off_info<HD>() + kPtInfo * 64; }  // blocks the MMA warp has come to
 template <int HD> constexpr uint32_t pt_smem() { return pt_off_beat<HD>() + 16 + 1024; }
