@@ -8,7 +8,8 @@ Modules (reference counterpart in brackets):
              quantize_tokens, int8_matmul, int8_linear (8-bit activations too)
   expert     ActionExpertConfig, Block, ActionExpert, timestep_embedding,
              flow_sample, sample                                 [kernel/flow_expert.py]
-  prompt     rotary_embed, prompt_attention (a prompt's layers)
+  prompt     rotary_embed, norm_rotary_embed, prompt_attention (a prompt's layers)
+  cache      KVCache, cache_write, cache_read (paged, 8- or 4-bit keys and values)
   graphed    GraphedSampler, eval_all                            [kernel/cudagraph.py]
   fused      plan of the single-launch sampler (ee_flow_sample)
   fleet      batch-of-robots mode over several GPUs
@@ -20,10 +21,12 @@ from .wq_gemm import (TritonQuantLinear, _pack_int4, _unpack_int4, correctness_c
                       quantize_model_triton, quantize_tokens, wq_linear)
 from .expert import ActionExpert, ActionExpertConfig, Block, PackedKV, flow_sample, sample, timestep_embedding
 from .graphed import GraphedSampler
-from .prompt import prompt_attention, rotary_embed
+from .prompt import norm_rotary_embed, prompt_attention, rotary_embed
+from .cache import KVCache, cache_read, cache_write
 
 __all__ = ["quantize_weight", "dequantize_weight", "quantize_weight_asym4", "TritonQuantLinear",
            "_pack_int4", "_unpack_int4", "wq_linear", "quantize_model_triton", "correctness_check",
            "ActionExpert", "ActionExpertConfig", "Block", "flow_sample", "sample",
            "timestep_embedding", "GraphedSampler", "quantize_tokens", "int8_matmul", "int8_linear",
-           "rotary_embed", "prompt_attention", "PackedKV"]
+           "rotary_embed", "norm_rotary_embed", "prompt_attention", "PackedKV", "KVCache",
+           "cache_write", "cache_read"]

@@ -56,6 +56,12 @@ class Expert(ctypes.Structure):
                 ("out_norm", Norm), ("blocks", c_void_p), ("kv_maps", c_void_p)]
 
 
+class Cache(ctypes.Structure):
+    _fields_ = [("k_codes", c_void_p), ("v_codes", c_void_p), ("k_steps", c_void_p), ("v_steps", c_void_p),
+                ("pages", c_int32), ("kv_heads", c_int32), ("page_size", c_int32), ("head_dim", c_int32),
+                ("bits", c_int32), ("reserved", c_int32)]
+
+
 # name -> (restype, argtypes); every symbol include/ee_b200.h declares
 SIGNATURES = {
     "ee_strerror": (ctypes.c_char_p, [c_int32]),
@@ -94,6 +100,14 @@ SIGNATURES = {
     "ee_rotary": (c_int32, [c_void_p, c_int64, c_int64] * 4 + [c_void_p, c_int64, c_int32, c_void_p, c_int64, c_int32,
                                                                c_int32, c_int32, c_void_p, c_int32, c_int32, c_int32,
                                                                c_void_p]),
+    "ee_norm_rotary": (c_int32, [c_void_p, c_int64, c_int64] * 4 + [c_void_p, c_void_p, c_int32, c_float, c_void_p,
+                                                                    c_int64, c_int32, c_void_p, c_int64, c_int32,
+                                                                    c_int32, c_int32, c_void_p, c_int32, c_int32,
+                                                                    c_int32, c_void_p]),
+    "ee_cache_write": (c_int32, [ctypes.POINTER(Cache)] + [c_void_p, c_int64, c_int64] * 2
+                       + [c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_int32, c_int32, c_void_p]),
+    "ee_cache_read": (c_int32, [ctypes.POINTER(Cache)] + [c_void_p, c_int64, c_int64] * 2
+                      + [c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_int32, c_int32, c_void_p]),
     "ee_prompt_attention_workspace_bytes": (c_size_t, [c_int64, c_int64] + [c_int32] * 4),
     "ee_prompt_attention": (c_int32, [c_void_p, c_int64, c_int64] * 4 + [c_void_p] * 3 + [c_int64, c_int64]
                             + [c_int32] * 5 + [c_float, c_int32, c_void_p, c_size_t, c_void_p]),

@@ -1,5 +1,6 @@
 // ee_rotary.cu -- C ABI: rotary positions with up to four axes (time, height,
-// width, ...) applied to the query and key heads of packed tokens.
+// width, ...) applied to the query and key heads of packed tokens, by
+// themselves (ee_rotary) or after an RMS norm of each head (ee_norm_rotary).
 //
 // Pair i of a head (elements i and i + hd/2, or 2i and 2i + 1 interleaved)
 // turns by pos[axis(i)][token] * base^(-2i / hd). The table holds each
@@ -18,6 +19,11 @@
 // registers leave 5 CTAs an SM and 71 us instead of 65 for the case below).
 // Measured: 65537 tokens, 16 + 8 heads of 64: 65 us, 6.2 TB/s, 0.94 of the
 // copy rate; 6528 tokens, 16 + 16 heads of 128: 17 us.
+//
+// The norm, y = w x / sqrt(mean(x^2) + eps), is taken in fp32 on the 16 values
+// that a lane holds of a head anyway, their squares summed over the head's hd /
+// 16 lanes by shuffles: one rounding, at the end, and no pass of its own.
+#include <cfloat>
 #include <type_traits>
 
 #include "ee_common.cuh"
@@ -35,11 +41,34 @@ struct RotaryArgs {
   int n_q, n_kv;
   int end0, end1, end2;                // pairs below end0: axis 0, below end1: axis 1, ...
   int pos64, interleaved;
+  const void *qw, *kw;                 // norm: weights [hd] of the query and key heads
+  int w32;                             // they are fp32, not of the act dtype
+  float eps;
 };
 
 constexpr int kRotWarps = 4;
 
-template <typename T, int HD>
+// eight weights as fp32
+template <typename T>
+EE_DEV void norm_weights(const void* w, int w32, int at, float (&r)[8]) {
+  if (w32) {
+    const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(w) + at);
+    const float4 x = __ldg(p), y = __ldg(p + 1);
+    r[0] = x.x; r[1] = x.y; r[2] = x.z; r[3] = x.w;
+    r[4] = y.x; r[5] = y.y; r[6] = y.z; r[7] = y.w;
+  } else {
+    const uint4 x = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(w) + at));
+    const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = Act<T>::unpack2(xw[e]);
+      r[2 * e] = f.x;
+      r[2 * e + 1] = f.y;
+    }
+  }
+}
+
+template <typename T, int HD, bool NORM>
 __global__ void __launch_bounds__(kRotWarps * 32) rotary_kernel(const __grid_constant__ RotaryArgs a) {
   constexpr int HALF = HD / 2, CH = HALF / 8;  // 8-pair chunks per head
   constexpr int HL = 32 / CH;                  // heads a warp turns at once
@@ -79,14 +108,16 @@ __global__ void __launch_bounds__(kRotWarps * 32) rotary_kernel(const __grid_con
     }
   }
   const int lo = a.interleaved ? 16 * c : 8 * c, hi = a.interleaved ? lo + 8 : lo + HALF;
-  const int heads = a.n_q + a.n_kv;
-  auto turn_heads = [&](int h0, auto un) {
+  float wl[NORM ? 8 : 1], wh[NORM ? 8 : 1];  // this lane's weights
+  // heads h0, h0 + HL, ... below `heads`; with a norm all of the queries or all of the keys, by the whole warp
+  auto turn_heads = [&](int h0, int heads, auto un) {
     constexpr int UN = decltype(un)::value;
     uint4 x[UN], y[UN];
     T* dst[UN];
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
       const int h = h0 + u * HL;
+      if (NORM) x[u] = y[u] = make_uint4(0, 0, 0, 0);
       if (h < heads) {
         const bool isq = h < a.n_q;
         const T* src = isq ? reinterpret_cast<const T*>(a.q) + t * a.q_tok + h * a.q_head
@@ -99,10 +130,40 @@ __global__ void __launch_bounds__(kRotWarps * 32) rotary_kernel(const __grid_con
     }
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
-      if (h0 + u * HL >= heads) continue;
+      if (!NORM && h0 + u * HL >= heads) continue;
       const uint32_t xw[4] = {x[u].x, x[u].y, x[u].z, x[u].w}, yw[4] = {y[u].x, y[u].y, y[u].z, y[u].w};
       uint32_t xo[4], yo[4];
-      if (a.interleaved) {
+      if constexpr (NORM) {
+        float f[8], g[8], sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 p = Act<T>::unpack2(xw[e]), q = Act<T>::unpack2(yw[e]);
+          f[2 * e] = p.x; f[2 * e + 1] = p.y;
+          g[2 * e] = q.x; g[2 * e + 1] = q.y;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = fmaf(f[e], f[e], fmaf(g[e], g[e], sum));
+#pragma unroll
+        for (int o = 1; o < CH; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (h0 + u * HL >= heads) continue;
+        const float r = rsqrtf(fmaf(sum, 1.f / HD, a.eps));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          f[e] *= r * wl[e];
+          g[e] *= r * wh[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          if (a.interleaved) {
+            xo[e / 2] = Act<T>::pack2(f[e] * cv[e / 2] - f[e + 1] * sv[e / 2], f[e] * sv[e / 2] + f[e + 1] * cv[e / 2]);
+            yo[e / 2] = Act<T>::pack2(g[e] * cv[4 + e / 2] - g[e + 1] * sv[4 + e / 2],
+                                      g[e] * sv[4 + e / 2] + g[e + 1] * cv[4 + e / 2]);
+          } else {
+            xo[e / 2] = Act<T>::pack2(f[e] * cv[e] - g[e] * sv[e], f[e + 1] * cv[e + 1] - g[e + 1] * sv[e + 1]);
+            yo[e / 2] = Act<T>::pack2(f[e] * sv[e] + g[e] * cv[e], f[e + 1] * sv[e + 1] + g[e + 1] * cv[e + 1]);
+          }
+        }
+      } else      if (a.interleaved) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float2 f = Act<T>::unpack2(xw[e]), g = Act<T>::unpack2(yw[e]);
@@ -121,18 +182,30 @@ __global__ void __launch_bounds__(kRotWarps * 32) rotary_kernel(const __grid_con
       *reinterpret_cast<uint4*>(dst[u] + hi) = make_uint4(yo[0], yo[1], yo[2], yo[3]);
     }
   };
-  for (int h0 = lane / CH; h0 < heads; h0 += 3 * HL) turn_heads(h0, std::integral_constant<int, 3>{});
+  if constexpr (NORM) {
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {  // queries, keys
+      const int first = part ? a.n_q : 0, end = part ? a.n_q + a.n_kv : a.n_q;
+      if (first == end) continue;
+      norm_weights<T>(part ? a.kw : a.qw, a.w32, lo, wl);
+      norm_weights<T>(part ? a.kw : a.qw, a.w32, hi, wh);
+      for (int h = first; h < end; h += 3 * HL) turn_heads(h + lane / CH, end, std::integral_constant<int, 3>{});
+    }
+  } else {
+    const int heads = a.n_q + a.n_kv;
+    for (int h0 = lane / CH; h0 < heads; h0 += 3 * HL) turn_heads(h0, heads, std::integral_constant<int, 3>{});
+  }
 }
 
-template <typename T>
+template <typename T, bool NORM>
 static int launch_rotary(const RotaryArgs& a, int hd, cudaStream_t s) {
   const unsigned grid = (unsigned)((a.tokens + kRotWarps - 1) / kRotWarps);
   cudaError_t e = cudaErrorInvalidValue;
   switch (hd) {
-    case 32: e = launch_pdl(rotary_kernel<T, 32>, dim3(grid), dim3(kRotWarps * 32), 0, s, a); break;
-    case 64: e = launch_pdl(rotary_kernel<T, 64>, dim3(grid), dim3(kRotWarps * 32), 0, s, a); break;
-    case 128: e = launch_pdl(rotary_kernel<T, 128>, dim3(grid), dim3(kRotWarps * 32), 0, s, a); break;
-    case 256: e = launch_pdl(rotary_kernel<T, 256>, dim3(grid), dim3(kRotWarps * 32), 0, s, a); break;
+    case 32: e = launch_pdl(rotary_kernel<T, 32, NORM>, dim3(grid), dim3(kRotWarps * 32), 0, s, a); break;
+    case 64: e = launch_pdl(rotary_kernel<T, 64, NORM>, dim3(grid), dim3(kRotWarps * 32), 0, s, a); break;
+    case 128: e = launch_pdl(rotary_kernel<T, 128, NORM>, dim3(grid), dim3(kRotWarps * 32), 0, s, a); break;
+    case 256: e = launch_pdl(rotary_kernel<T, 256, NORM>, dim3(grid), dim3(kRotWarps * 32), 0, s, a); break;
   }
   return e == cudaSuccess ? EE_OK : EE_ERR_LAUNCH;
 }
@@ -141,11 +214,12 @@ static int launch_rotary(const RotaryArgs& a, int hd, cudaStream_t s) {
 
 using namespace ee;
 
-extern "C" int ee_rotary(const void* q, int64_t q_tok, int64_t q_head, void* q_out, int64_t qo_tok, int64_t qo_head,
-                         const void* k, int64_t k_tok, int64_t k_head, void* k_out, int64_t ko_tok, int64_t ko_head,
-                         const void* positions, int64_t pos_axis, int32_t pos_bits, const uint64_t* freqs,
-                         int64_t tokens, int32_t n_q, int32_t n_kv, int32_t head_dim, const int32_t* sections,
-                         int32_t n_axes, int32_t interleaved, int32_t act_dtype, ee_stream_t stream) {
+static int rotary(const void* q, int64_t q_tok, int64_t q_head, void* q_out, int64_t qo_tok, int64_t qo_head,
+                  const void* k, int64_t k_tok, int64_t k_head, void* k_out, int64_t ko_tok, int64_t ko_head,
+                  const void* positions, int64_t pos_axis, int32_t pos_bits, const uint64_t* freqs, int64_t tokens,
+                  int32_t n_q, int32_t n_kv, int32_t head_dim, const int32_t* sections, int32_t n_axes,
+                  int32_t interleaved, int32_t act_dtype, bool norm, const void* q_weight, const void* k_weight,
+                  int32_t weight_dtype, float eps, cudaStream_t s) {
   if (!sections || n_axes < 1 || n_axes > 4 || tokens < 0 || n_q < 0 || n_kv < 0) return EE_ERR_ARG;
   if (pos_bits != 32 && pos_bits != 64) return EE_ERR_ARG;
   if (act_dtype != EE_BF16 && act_dtype != EE_F16) return EE_ERR_DTYPE;
@@ -162,6 +236,12 @@ extern "C" int ee_rotary(const void* q, int64_t q_tok, int64_t q_head, void* q_o
   if ((n_q && (!aligned16(q) || !aligned16(q_out))) || (n_kv && (!aligned16(k) || !aligned16(k_out))))
     return EE_ERR_ALIGN;
   if (((uintptr_t)positions & (pos_bits / 8 - 1)) || ((uintptr_t)freqs & 7)) return EE_ERR_ALIGN;
+  if (norm) {
+    if (weight_dtype != EE_F32 && weight_dtype != act_dtype) return EE_ERR_DTYPE;
+    if (!(eps >= FLT_MIN) || !(eps <= FLT_MAX)) return EE_ERR_ARG;
+    if ((n_q && !q_weight) || (n_kv && !k_weight)) return EE_ERR_ARG;
+    if ((n_q && !aligned16(q_weight)) || (n_kv && !aligned16(k_weight))) return EE_ERR_ALIGN;
+  }
   const int64_t strides[8] = {q_tok, q_head, qo_tok, qo_head, k_tok, k_head, ko_tok, ko_head};
   for (int i = 0; i < 8; ++i)
     if ((i < 4 ? n_q : n_kv) && (strides[i] % 8) != 0) return EE_ERR_ALIGN;
@@ -182,6 +262,38 @@ extern "C" int ee_rotary(const void* q, int64_t q_tok, int64_t q_head, void* q_o
   if (n_axes == 1) a.end0 = 0x7fffffff;
   a.pos64 = pos_bits == 64;
   a.interleaved = interleaved != 0;
-  cudaStream_t s = (cudaStream_t)stream;
-  return act_dtype == EE_BF16 ? launch_rotary<__nv_bfloat16>(a, head_dim, s) : launch_rotary<__half>(a, head_dim, s);
+  if (norm) {
+    a.qw = q_weight; a.kw = k_weight;
+    a.w32 = weight_dtype == EE_F32;
+    a.eps = eps;
+    return act_dtype == EE_BF16 ? launch_rotary<__nv_bfloat16, true>(a, head_dim, s)
+                                : launch_rotary<__half, true>(a, head_dim, s);
+  }
+  return act_dtype == EE_BF16 ? launch_rotary<__nv_bfloat16, false>(a, head_dim, s)
+                              : launch_rotary<__half, false>(a, head_dim, s);
 }
+
+extern "C" {
+
+int ee_rotary(const void* q, int64_t q_tok, int64_t q_head, void* q_out, int64_t qo_tok, int64_t qo_head, const void* k,
+              int64_t k_tok, int64_t k_head, void* k_out, int64_t ko_tok, int64_t ko_head, const void* positions,
+              int64_t pos_axis, int32_t pos_bits, const uint64_t* freqs, int64_t tokens, int32_t n_q, int32_t n_kv,
+              int32_t head_dim, const int32_t* sections, int32_t n_axes, int32_t interleaved, int32_t act_dtype,
+              ee_stream_t stream) {
+  return rotary(q, q_tok, q_head, q_out, qo_tok, qo_head, k, k_tok, k_head, k_out, ko_tok, ko_head, positions, pos_axis,
+                pos_bits, freqs, tokens, n_q, n_kv, head_dim, sections, n_axes, interleaved, act_dtype, false, nullptr,
+                nullptr, 0, 0.f, (cudaStream_t)stream);
+}
+
+int ee_norm_rotary(const void* q, int64_t q_tok, int64_t q_head, void* q_out, int64_t qo_tok, int64_t qo_head,
+                   const void* k, int64_t k_tok, int64_t k_head, void* k_out, int64_t ko_tok, int64_t ko_head,
+                   const void* q_weight, const void* k_weight, int32_t weight_dtype, float eps, const void* positions,
+                   int64_t pos_axis, int32_t pos_bits, const uint64_t* freqs, int64_t tokens, int32_t n_q, int32_t n_kv,
+                   int32_t head_dim, const int32_t* sections, int32_t n_axes, int32_t interleaved, int32_t act_dtype,
+                   ee_stream_t stream) {
+  return rotary(q, q_tok, q_head, q_out, qo_tok, qo_head, k, k_tok, k_head, k_out, ko_tok, ko_head, positions, pos_axis,
+                pos_bits, freqs, tokens, n_q, n_kv, head_dim, sections, n_axes, interleaved, act_dtype, true, q_weight,
+                k_weight, weight_dtype, eps, (cudaStream_t)stream);
+}
+
+}  // extern "C"

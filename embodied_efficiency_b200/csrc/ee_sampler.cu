@@ -212,6 +212,7 @@ size_t ee_struct_size(int32_t which) {
     case 1: return sizeof(ee_norm);
     case 2: return sizeof(ee_block);
     case 3: return sizeof(ee_expert);
+    case 4: return sizeof(ee_cache);
   }
   return 0;
 }

@@ -1,6 +1,7 @@
 // ee_torch.cpp -- native host side of the prompt-layer operators: what a call
-// of rotary_embed, prompt_attention, int8_linear, int8_matmul and
-// quantize_tokens does on the host, without the interpreter. A call of few
+// of rotary_embed, norm_rotary_embed, prompt_attention, int8_linear,
+// int8_matmul, quantize_tokens and the operators of a cache does on the host,
+// without the interpreter. A call of few
 // tokens takes the GPU 3 to 8 us; checks, allocations and argument conversion
 // in Python took 13 to 17 us around it.
 //
@@ -10,6 +11,8 @@
 // the Python function of the same name then makes the copies or raises the
 // error. So nothing here reports an argument error itself.
 #include <Python.h>
+
+#include <cfloat>
 
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
@@ -197,10 +200,9 @@ PyObject* quantize_tokens(PyObject*, PyObject* const* a, Py_ssize_t argc) {
 // ---------------------------------------------------------------------------
 // rotary positions
 // ---------------------------------------------------------------------------
-// rotary_embed(q, k, positions, sections, turns, interleaved); turns: the
-// table of hd / 2 frequencies on the device
-PyObject* rotary_embed(PyObject*, PyObject* const* a, Py_ssize_t argc) {
-  if (argc != 6) return none();
+// q, k, positions, sections, turns, interleaved; turns: the table of hd / 2
+// frequencies on the device. w: q_weight, k_weight, eps, or nothing
+PyObject* rotary(PyObject* const* a, PyObject* const* w) {
   Call c;
   const Tensor *q = c.get(a[0]), *k = c.get(a[1]), *pos = c.get(a[2]), *tab = c.get(a[4]);
   if (!c.need(q && k && pos && tab && heads_ok(*q) && heads_ok(*k) && PyTuple_Check(a[3]) && PyBool_Check(a[5])))
@@ -226,19 +228,126 @@ PyObject* rotary_embed(PyObject*, PyObject* const* a, Py_ssize_t argc) {
               tab->scalar_type() == at::kLong && tab->numel() == hd / 2 && tab->is_contiguous()))
     return none();
   const bool interleaved = a[5] == Py_True;
+  const Tensor *qw = nullptr, *kw = nullptr;
+  float eps = 0.f;
+  if (w) {
+    qw = c.get(w[0]);
+    kw = c.get(w[1]);
+    eps = PyFloat_Check(w[2]) ? (float)PyFloat_AS_DOUBLE(w[2]) : 0.f;
+    auto vector = [&](const Tensor* t) {
+      return t->dim() == 1 && t->numel() == hd && t->is_contiguous() && aligned(*t) &&
+             (t->scalar_type() == at::kFloat || t->scalar_type() == q->scalar_type());
+    };
+    if (!c.need(qw && kw && vector(qw) && vector(kw) && qw->scalar_type() == kw->scalar_type() && eps >= FLT_MIN &&
+                eps <= FLT_MAX))
+      return none();
+  }
   Tensor qo, ko;
   int rc;
   {
     NoGil others;
     qo = at::empty(q->sizes(), q->options());
     ko = at::empty(k->sizes(), k->options());
-    rc = ee_rotary(q->data_ptr(), q->stride(0), q->stride(1), qo.data_ptr(), qo.stride(0), qo.stride(1), k->data_ptr(),
-                   k->stride(0), k->stride(1), ko.data_ptr(), ko.stride(0), ko.stride(1), pos->data_ptr(), t,
-                   p64 ? 64 : 32, static_cast<const uint64_t*>(tab->data_ptr()), t, (int32_t)q->size(1),
-                   (int32_t)k->size(1), (int32_t)hd, sections, (int32_t)axes, interleaved, act_code(q->scalar_type()),
-                   c.stream());
+    const auto *turns = static_cast<const uint64_t*>(tab->data_ptr());
+    const int32_t nq = (int32_t)q->size(1), nk = (int32_t)k->size(1), act = act_code(q->scalar_type());
+    if (w)
+      rc = ee_norm_rotary(q->data_ptr(), q->stride(0), q->stride(1), qo.data_ptr(), qo.stride(0), qo.stride(1),
+                          k->data_ptr(), k->stride(0), k->stride(1), ko.data_ptr(), ko.stride(0), ko.stride(1),
+                          qw->data_ptr(), kw->data_ptr(), qw->scalar_type() == at::kFloat ? EE_F32 : act, eps,
+                          pos->data_ptr(), t, p64 ? 64 : 32, turns, t, nq, nk, (int32_t)hd, sections, (int32_t)axes,
+                          interleaved, act, c.stream());
+    else
+      rc = ee_rotary(q->data_ptr(), q->stride(0), q->stride(1), qo.data_ptr(), qo.stride(0), qo.stride(1), k->data_ptr(),
+                     k->stride(0), k->stride(1), ko.data_ptr(), ko.stride(0), ko.stride(1), pos->data_ptr(), t,
+                     p64 ? 64 : 32, turns, t, nq, nk, (int32_t)hd, sections, (int32_t)axes, interleaved, act, c.stream());
   }
   return give(rc, qo, ko);
+}
+PyObject* rotary_embed(PyObject*, PyObject* const* a, Py_ssize_t argc) { return argc == 6 ? rotary(a, nullptr) : none(); }
+
+// norm_rotary_embed(q, k, q_weight, k_weight, positions, sections, turns, interleaved, eps)
+PyObject* norm_rotary_embed(PyObject*, PyObject* const* a, Py_ssize_t argc) {
+  if (argc != 9) return none();
+  PyObject* const heads[6] = {a[0], a[1], a[4], a[5], a[6], a[7]};
+  PyObject* const norm[3] = {a[2], a[3], a[8]};
+  return rotary(heads, norm);
+}
+
+// ---------------------------------------------------------------------------
+// cache
+// ---------------------------------------------------------------------------
+// The cache's keys, the address of its ee_cache (made and checked by KVCache,
+// whose tensors the record describes), offsets, table and lengths of a call.
+struct Places {
+  const ee_cache* cache;
+  const int32_t *cu, *table, *k_lens;
+  int64_t table_row, width, n;
+};
+bool places(Call& c, PyObject* keys, PyObject* record, PyObject* cu_o, PyObject* table_o, PyObject* lens_o, Places& p) {
+  const Tensor *k = c.get(keys), *cu = c.get(cu_o), *table = c.get(table_o), *lens = c.get(lens_o);
+  if (!c.need(k && cu && table && lens && PyLong_Check(record))) return false;
+  p.cache = static_cast<const ee_cache*>(PyLong_AsVoidPtr(record));
+  p.n = cu->numel() - 1;
+  if (!c.need(p.cache && p.cache->k_codes == k->data_ptr() && cu->dim() == 1 && cu->scalar_type() == at::kInt && cu->is_contiguous() && p.n >= 1 &&
+              p.n < (1 << 30) && lens->dim() == 1 && lens->scalar_type() == at::kInt && lens->numel() == p.n &&
+              lens->is_contiguous() && table->dim() == 2 && table->scalar_type() == at::kInt && table->size(0) == p.n &&
+              table->size(1) >= 1 && table->stride(1) == 1 && table->size(1) <= 0x7fffffff / p.cache->page_size))
+    return false;
+  p.cu = static_cast<const int32_t*>(cu->data_ptr());
+  p.table = static_cast<const int32_t*>(table->data_ptr());
+  p.k_lens = static_cast<const int32_t*>(lens->data_ptr());
+  p.table_row = table->stride(0);
+  p.width = table->size(1);
+  return true;
+}
+bool cache_heads(const Tensor& t, const ee_cache& c) {
+  return heads_ok(t) && t.size(0) > 0 && t.size(0) < (1 << 30) && t.size(1) == c.kv_heads && t.size(2) == c.head_dim;
+}
+
+// cache_write(keys, record, k, v, cu, table, k_lens) -> True
+PyObject* cache_write(PyObject*, PyObject* const* a, Py_ssize_t argc) {
+  if (argc != 7) return none();
+  Call c;
+  Places p;
+  if (!places(c, a[0], a[1], a[4], a[5], a[6], p)) return none();
+  const Tensor *k = c.get(a[2]), *v = c.get(a[3]);
+  if (!c.need(k && v && cache_heads(*k, *p.cache) && cache_heads(*v, *p.cache) && k->size(0) == v->size(0) &&
+              k->scalar_type() == v->scalar_type()))
+    return none();
+  int rc;
+  {
+    NoGil others;
+    rc = ee_cache_write(p.cache, k->data_ptr(), k->stride(0), k->stride(1), v->data_ptr(), v->stride(0), v->stride(1),
+                        p.cu, p.table, p.table_row, (int32_t)p.width, p.k_lens, k->size(0), (int32_t)p.n,
+                        act_code(k->scalar_type()), c.stream());
+  }
+  if (rc != EE_OK) return none();
+  Py_RETURN_TRUE;
+}
+
+// cache_read(keys, record, cu, table, k_lens, tokens, dtype) -> (k, v)
+PyObject* cache_read(PyObject*, PyObject* const* a, Py_ssize_t argc) {
+  if (argc != 7 || !PyLong_Check(a[5]) || !THPDtype_Check(a[6])) return none();
+  const ScalarType type = reinterpret_cast<THPDtype*>(a[6])->scalar_type;
+  const int64_t tokens = PyLong_AsLongLong(a[5]);
+  if (tokens < 1 || tokens >= (1 << 30) || !act_type(type)) {
+    PyErr_Clear();
+    return none();
+  }
+  Call c;
+  Places p;
+  if (!places(c, a[0], a[1], a[2], a[3], a[4], p)) return none();
+  const Tensor& keys = THPVariable_Unpack(a[0]);
+  Tensor k, v;
+  int rc;
+  {
+    NoGil others;
+    k = at::empty({tokens, p.cache->kv_heads, p.cache->head_dim}, keys.options().dtype(type));
+    v = at::empty({tokens, p.cache->kv_heads, p.cache->head_dim}, keys.options().dtype(type));
+    rc = ee_cache_read(p.cache, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), p.cu,
+                       p.table, p.table_row, (int32_t)p.width, p.k_lens, tokens, (int32_t)p.n, act_code(type), c.stream());
+  }
+  return give(rc, k, v);
 }
 
 // ---------------------------------------------------------------------------
@@ -301,7 +410,8 @@ PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t n) {
 #define EE_METHOD(name) \
   {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&guarded<name>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {EE_METHOD(int8_linear),  EE_METHOD(int8_matmul),      EE_METHOD(quantize_tokens),
-                         EE_METHOD(rotary_embed), EE_METHOD(prompt_attention), {nullptr, nullptr, 0, nullptr}};
+                         EE_METHOD(rotary_embed), EE_METHOD(norm_rotary_embed), EE_METHOD(prompt_attention),
+                         EE_METHOD(cache_write),  EE_METHOD(cache_read),        {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "ee_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

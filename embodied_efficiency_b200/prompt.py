@@ -1,5 +1,5 @@
-"""Attention layers of packed prompts: rotary positions with several axes and
-causal or full attention with grouped heads, on the sm_100a kernels of
+"""Attention layers of packed prompts: rotary positions with several axes (alone or
+behind a norm of each head) and causal or full attention with grouped heads, on the sm_100a kernels of
 ``libee_b200.so``.
 
 A prompt's queries, keys and values are rows of token-major tensors
@@ -51,6 +51,13 @@ def _out(out, like, name):
     return out, s
 
 
+def _vector(t):
+    """A contiguous vector on a 16-byte boundary; a copy where it is not."""
+    if t is not None and (t.stride(0) != 1 or t.data_ptr() % 16):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
 def _act_dtype(t, name):
     if t.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError(f"{name} must be bf16 or fp16, not {t.dtype}")
@@ -68,13 +75,13 @@ def _turn_fractions(half: int, base: float) -> list:
         return [int((scale * (log * -i / half).exp()).to_integral_value()) for i in range(half)]
 
 
-def _turns(device, half: int, base: float) -> torch.Tensor:
+def _turns(device, half: int, base: float, name: str = "rotary_embed") -> torch.Tensor:
     """``_turn_fractions`` as int64 bits, a constant table per device."""
     key = (device, half, base)
     tab = _TURNS.get(key)
     if tab is None:
         if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError(f"rotary_embed copies its frequencies (head_dim {2 * half}, base {base}) to the device on "
+            raise RuntimeError(f"{name} copies its frequencies (head_dim {2 * half}, base {base}) to the device on "
                                "first use: call it once before the stream capture")
         host = torch.tensor(_turn_fractions(half, base), dtype=torch.int64)  # at most 2^64 / 2 pi < 2^63
         tab = _TURNS[key] = host.to(device)
@@ -105,9 +112,36 @@ def rotary_embed(q, k, positions, sections, base: float = 10000.0, interleaved: 
             done = (_lib._native or _lib.native()).rotary_embed(q, k, positions, sections, tab, interleaved)
             if done is not None:
                 return done
+    return _rotary("rotary_embed", q, k, positions, sections, base, interleaved, out)
+
+
+def norm_rotary_embed(q, k, q_weight, k_weight, positions, sections, eps: float = 1e-6, base: float = 10000.0,
+                      interleaved: bool = False, out=None):
+    """``rotary_embed`` of heads that are normalised first, in one pass (``ee_norm_rotary``): every head x of ``q``
+    becomes ``q_weight * x / sqrt(mean(x^2) + eps)`` before it turns, every head of ``k`` the same with ``k_weight``
+    ([head_dim], fp32 or of the heads' type, both the same; None for heads that are None). Squares and sums in fp32, one
+    rounding at the end. ``eps`` at least 2^-126. Everything else as for ``rotary_embed``."""
+    if out is None and q is not None and k is not None:
+        tab = _TURNS.get((q.device, q.shape[-1] // 2, base))
+        if tab is not None:
+            done = (_lib._native or _lib.native()).norm_rotary_embed(q, k, q_weight, k_weight, positions, sections, tab,
+                                                                     interleaved, eps)
+            if done is not None:
+                return done
+    return _rotary("norm_rotary_embed", q, k, positions, sections, base, interleaved, out, (q_weight, k_weight, eps))
+
+
+def _norm_weight(w, x, name):
+    if w is None or w.dim() != 1 or w.numel() != x.shape[-1]:
+        raise ValueError(f"{name} must be [{x.shape[-1]}], got {None if w is None else tuple(w.shape)}")
+    if w.dtype not in (torch.float32, x.dtype):
+        raise ValueError(f"{name} must be fp32 or {x.dtype}, not {w.dtype}")
+
+
+def _rotary(name, q, k, positions, sections, base, interleaved, out, norm=None):
     one = q if q is not None else k
     if one is None:
-        raise ValueError("rotary_embed needs q or k")
+        raise ValueError(f"{name} needs q or k")
     t, hd = one.shape[0], one.shape[-1]
     if type(sections) is not tuple:
         sections = tuple(sections)
@@ -124,8 +158,20 @@ def rotary_embed(q, k, positions, sections, base: float = 10000.0, interleaved: 
     _act_dtype(one, "q and k")
     if q is not None and k is not None and (k.shape[0] != t or k.shape[-1] != hd or k.dtype != q.dtype):
         raise ValueError(f"q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} do not belong together")
-    dev = _lib.same_device(q, k, positions)
-    _lib.no_grad_through("rotary_embed", q, k)
+    if norm is not None:
+        qw, kw, eps = norm
+        qw, kw = (None if q is None else qw), (None if k is None else kw)
+        for w, x, n in ((qw, q, "q_weight"), (kw, k, "k_weight")):
+            if x is not None:
+                _norm_weight(w, x, n)
+        if qw is not None and kw is not None and qw.dtype != kw.dtype:
+            raise ValueError(f"q_weight is {qw.dtype}, k_weight {kw.dtype}")
+        if not 2.0 ** -126 <= eps <= 3.4e38:
+            raise ValueError(f"eps must be finite and at least 2^-126, got {eps}")
+    else:
+        qw = kw = None
+    dev = _lib.same_device(q, k, positions, qw, kw)
+    _lib.no_grad_through(name, q, k, qw, kw)
     qo, ko = out if out is not None else (None, None)
     qs = ks = qp = kp = qop = kop = nq = nk = 0
     none = (0, 0)
@@ -142,12 +188,17 @@ def rotary_embed(q, k, positions, sections, base: float = 10000.0, interleaved: 
             ko, ks, kos = None, none, none
         if positions.stride(-1) != 1:
             positions = positions.contiguous()
-        rc = _lib.load().ee_rotary(qp, qs[0], qs[1], qop, qos[0], qos[1], kp, ks[0], ks[1], kop, kos[0], kos[1],
-                                   positions.data_ptr(), positions.stride(0) if positions.dim() == 2 else t,
-                                   32 if positions.dtype == torch.int32 else 64, _turns(dev, hd // 2, base).data_ptr(),
-                                   t, nq, nk, hd, sec, len(sections), 1 if interleaved else 0,
-                                   _lib.act_code(one.dtype), _lib.stream_ptr(dev))
-    _lib.check(rc, "ee_rotary")
+        heads = (qp, qs[0], qs[1], qop, qos[0], qos[1], kp, ks[0], ks[1], kop, kos[0], kos[1])
+        rest = (positions.data_ptr(), positions.stride(0) if positions.dim() == 2 else t,
+                32 if positions.dtype == torch.int32 else 64, _turns(dev, hd // 2, base, name).data_ptr(), t, nq, nk, hd,
+                sec, len(sections), 1 if interleaved else 0, _lib.act_code(one.dtype), _lib.stream_ptr(dev))
+        if norm is None:
+            rc = _lib.load().ee_rotary(*heads, *rest)
+        else:
+            qw, kw = _vector(qw), _vector(kw)
+            code = _lib.EE_F32 if (kw if qw is None else qw).dtype == torch.float32 else _lib.act_code(one.dtype)
+            rc = _lib.load().ee_norm_rotary(*heads, _lib.ptr(qw), _lib.ptr(kw), code, eps, *rest)
+    _lib.check(rc, "ee_rotary" if norm is None else "ee_norm_rotary")
     return qo, ko
 
 

@@ -35,7 +35,10 @@
  *   ee_quantize_tokens / ee_int8_gemm / ee_int8_linear / ee_int8_plan
  *                         8-bit integer linears (new)
  *   ee_rotary             rotary positions with several axes (new)
+ *   ee_norm_rotary        the same behind an RMS norm of each head (new)
  *   ee_prompt_attention   attention over packed prompts (new)
+ *   ee_cache_write / ee_cache_read / ee_cache_attention
+ *                         paged cache of quantised keys and values (new)
  *   ee_strerror / ee_version / ee_struct_size   (new)
  */
 #ifndef EE_B200_H
@@ -223,6 +226,18 @@ int ee_rotary(const void* q, int64_t q_tok, int64_t q_head, void* q_out, int64_t
               int32_t n_q, int32_t n_kv, int32_t head_dim, const int32_t* sections, int32_t n_axes,
               int32_t interleaved, int32_t act_dtype, ee_stream_t stream);
 
+/* ee_rotary of heads that are normalised first: every query head of values x
+ * becomes weight * x / sqrt(mean(x^2) + eps) before it turns, with q_weight
+ * [head_dim], every key head with k_weight (EE_F32 or the act dtype, 16-byte
+ * aligned; NULL where there are no such heads). Squares, sums and turns in
+ * fp32, one rounding. eps >= 2^-126. Everything else as for ee_rotary. */
+int ee_norm_rotary(const void* q, int64_t q_tok, int64_t q_head, void* q_out, int64_t qo_tok, int64_t qo_head,
+                   const void* k, int64_t k_tok, int64_t k_head, void* k_out, int64_t ko_tok, int64_t ko_head,
+                   const void* q_weight, const void* k_weight, int32_t weight_dtype, float eps, const void* positions,
+                   int64_t pos_axis, int32_t pos_bits, const uint64_t* freqs, int64_t tokens, int32_t n_q, int32_t n_kv,
+                   int32_t head_dim, const int32_t* sections, int32_t n_axes, int32_t interleaved, int32_t act_dtype,
+                   ee_stream_t stream);
+
 /* Attention over n_seq packed sequences: queries cu_q[b] .. cu_q[b + 1] of q
  * [tq][n_q][head_dim] against keys cu_k[b] .. cu_k[b + 1] of k / v
  * [tk][n_kv][head_dim] (the first k_lens[b] of them when k_lens is given: a
@@ -252,6 +267,40 @@ int ee_prompt_attention(const void* q, int64_t q_tok, int64_t q_head, const void
  * default, 1 s) gives up, the launch ends with its outputs unfinished and
  * EE_ERR_TIMEOUT in the status word of ee_wq_gemm_status. */
 int ee_prompt_attention_wait_limit(uint64_t ns);
+
+/* ---- paged cache of quantised keys and values (new) ----------------------- */
+/* `pages` pages of page_size tokens (32, 64, 128 or 256): codes
+ * [pages][kv_heads][page_size][head_dim] of 8 bits (int8), or of 4 (two's
+ * complement, two a byte, the even one in the low half), and fp32 steps
+ * [pages][kv_heads][page_size]; a value is code * step. All contiguous.
+ * head_dim 64 or 128; pages * kv_heads * page_size < 2^31.
+ *
+ * A sequence's key i lies in row i % page_size of page table[b][i / page_size]
+ * (`table`: int32, rows table_row elements apart, `width` entries each, on the
+ * device, like the offsets and lengths). A place that the table does not name,
+ * or names with a page number outside 0 .. pages - 1, holds no key: it is not
+ * written, not read and masked. */
+typedef struct ee_cache {
+  void *k_codes, *v_codes;
+  float *k_steps, *v_steps;
+  int32_t pages, kv_heads, page_size, head_dim, bits, reserved;
+} ee_cache;
+
+/* The tokens of sequence b, rows cu[b] .. cu[b + 1] of k / v [tokens][kv_heads]
+ * [head_dim] (strides in elements, multiples of 8), are its last ones before
+ * k_lens[b]: with n of them, row cu[b] + i is key k_lens[b] - n + i.
+ * ee_cache_write quantises them into the cache: per token and head step =
+ * max(amax / (127 or 7), 1e-8), codes rint(x / step) (true division, ties to
+ * even); a head that holds an infinity or NaN gets codes of 0 and a NaN step.
+ * A place that two tokens of a call claim is left with either's or a mixture.
+ * ee_cache_read gives code * step, rounded once to the act dtype. Rows whose
+ * key is before 0 or whose place holds no key stay as they were. */
+int ee_cache_write(const ee_cache* cache, const void* k, int64_t k_tok, int64_t k_head, const void* v, int64_t v_tok,
+                   int64_t v_head, const int32_t* cu, const int32_t* table, int64_t table_row, int32_t width,
+                   const int32_t* k_lens, int64_t tokens, int32_t n_seq, int32_t act_dtype, ee_stream_t stream);
+int ee_cache_read(const ee_cache* cache, void* k, int64_t k_tok, int64_t k_head, void* v, int64_t v_tok, int64_t v_head,
+                  const int32_t* cu, const int32_t* table, int64_t table_row, int32_t width, const int32_t* k_lens,
+                  int64_t tokens, int32_t n_seq, int32_t act_dtype, ee_stream_t stream);
 
 /* ---- fused flow-matching sampler --------------------------------------- */
 typedef struct ee_linear {
