@@ -9,7 +9,8 @@ Modules (reference counterpart in brackets):
   expert     ActionExpertConfig, Block, ActionExpert, timestep_embedding,
              flow_sample, sample                                 [kernel/flow_expert.py]
   prompt     rotary_embed, norm_rotary_embed, prompt_attention (a prompt's layers)
-  cache      KVCache, cache_write, cache_read (paged, 8- or 4-bit keys and values)
+  cache      KVCache, cache_write, cache_read, cache_attention
+             (paged, 8- or 4-bit keys and values)
   graphed    GraphedSampler, eval_all                            [kernel/cudagraph.py]
   fused      plan of the single-launch sampler (ee_flow_sample)
   fleet      batch-of-robots mode over several GPUs
@@ -22,11 +23,11 @@ from .wq_gemm import (TritonQuantLinear, _pack_int4, _unpack_int4, correctness_c
 from .expert import ActionExpert, ActionExpertConfig, Block, PackedKV, flow_sample, sample, timestep_embedding
 from .graphed import GraphedSampler
 from .prompt import norm_rotary_embed, prompt_attention, rotary_embed
-from .cache import KVCache, cache_read, cache_write
+from .cache import KVCache, cache_attention, cache_read, cache_write
 
 __all__ = ["quantize_weight", "dequantize_weight", "quantize_weight_asym4", "TritonQuantLinear",
            "_pack_int4", "_unpack_int4", "wq_linear", "quantize_model_triton", "correctness_check",
            "ActionExpert", "ActionExpertConfig", "Block", "flow_sample", "sample",
            "timestep_embedding", "GraphedSampler", "quantize_tokens", "int8_matmul", "int8_linear",
            "rotary_embed", "norm_rotary_embed", "prompt_attention", "PackedKV", "KVCache",
-           "cache_write", "cache_read"]
+           "cache_write", "cache_read", "cache_attention"]

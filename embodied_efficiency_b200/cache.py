@@ -15,7 +15,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .prompt import _act_dtype, _heads, _offsets, _out
+from .prompt import _MAX_SCALE, _act_dtype, _heads, _offsets, _out
 
 PAGE_SIZES = (32, 64, 128, 256)
 
@@ -151,3 +151,58 @@ def cache_read(cache: KVCache, cu, table, k_lens, tokens: int, dtype=torch.bfloa
                                        k_lens.data_ptr(), tokens, n, _lib.act_code(dtype), _lib.stream_ptr(dev))
     _lib.check(rc, "ee_cache_read")
     return k, v
+
+
+def cache_attention(q, cache: KVCache, cu_q, table, k_lens, causal: bool = True, scale: float | None = None, prefix=None,
+                    out=None):
+    """Attention over the cache (``ee_cache_attention``): sequence b's queries, rows ``cu_q[b]`` to ``cu_q[b + 1]`` of
+    ``q`` [tokens, heads, head_dim], against its first ``k_lens[b]`` keys (at most what its row of the table covers).
+    ``prefix`` = (k, v) [P, kv_heads, head_dim] in q's type are keys and values before those that every sequence shares
+    and every query sees: they are read once for the whole call. heads is a multiple of kv_heads: head h reads key head
+    ``h // (heads // kv_heads)``; at most 128 heads a key head with a prefix. With ``causal`` a sequence's last query
+    sees its last key; a query that sees no key gives zeros. ``scale`` defaults to head_dim^-0.5. Keys past a
+    sequence's length, under the mask or on pages that the cache does not have count with weight 0, whatever is there.
+    One kernel serves the whole call, chosen by the mean of queries per sequence and key head. Returns [tokens, heads,
+    head_dim], new or ``out`` (which shares no memory with the inputs); rows that belong to no sequence are not
+    written. bf16 / fp16."""
+    if out is None and type(cache) is KVCache:
+        done = (_lib._native or _lib.native()).cache_attention(cache.k, cache._at, q, cu_q, table, k_lens, causal, scale,
+                                                               prefix)
+        if done is not None:
+            return done
+    cu_q, table, k_lens, n = _places(cache, cu_q, table, k_lens, "cu_q")
+    hd, hk = cache.head_dim, cache.kv_heads
+    _act_dtype(q, "q")
+    if q.dim() != 3 or q.shape[2] != hd:
+        raise ValueError(f"q {tuple(q.shape)} must be [tokens, heads, {hd}]")
+    tq, hq = q.shape[:2]
+    if hq < 1 or hq % hk:
+        raise ValueError(f"{hq} heads are not a multiple of {hk} key heads")
+    scale = hd ** -0.5 if scale is None else float(scale)
+    if not 2.0 ** -126 <= scale <= _MAX_SCALE:
+        raise ValueError(f"scale must be finite and above 0 (fp32, 2^-126 to {_MAX_SCALE:.4g}), got {scale}")
+    pk = pv = None
+    if prefix is not None:
+        pk, pv = prefix
+        if pk.dim() != 3 or pk.shape != pv.shape or pk.dtype != q.dtype or pv.dtype != q.dtype or pk.shape[1:] != (hk, hd):
+            raise ValueError(f"prefix k {pk.dtype} {tuple(pk.shape)} and v {pv.dtype} {tuple(pv.shape)} must be "
+                             f"{q.dtype} [P, {hk}, {hd}]")
+        if pk.shape[0] and hq // hk > 128:
+            raise ValueError(f"{hq // hk} heads a key head: at most 128 with a prefix")
+    dev = _lib.same_device(cache.k, q, pk, pv, cu_q, table, k_lens)
+    _lib.no_grad_through("cache_attention", q, pk, pv)
+    lib = _lib.load()
+    with _lib.on_device(dev):
+        (qc, qs), (out, os_) = _heads(q, "q"), _out(out, q, "out")
+        p_len, pks, pvs = 0, (0, 0), (0, 0)
+        if pk is not None and pk.shape[0]:
+            (pk, pks), (pv, pvs), p_len = _heads(pk, "prefix k"), _heads(pv, "prefix v"), pk.shape[0]
+        nb = lib.ee_cache_attention_workspace_bytes(tq, n, hq, hk, hd, cache.bits, p_len)
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+        rc = lib.ee_cache_attention(
+            ctypes.byref(cache._c), qc.data_ptr(), qs[0], qs[1], out.data_ptr(), os_[0], os_[1], cu_q.data_ptr(),
+            table.data_ptr(), table.stride(0), table.shape[1], k_lens.data_ptr(), _lib.ptr(pk), pks[0], pks[1],
+            _lib.ptr(pv), pvs[0], pvs[1], p_len, tq, n, hq, 1 if causal else 0, scale, _lib.act_code(q.dtype),
+            _lib.ptr(ws), nb, _lib.stream_ptr(dev))
+    _lib.check(rc, "ee_cache_attention")
+    return out

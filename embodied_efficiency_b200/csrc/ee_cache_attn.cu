@@ -1,0 +1,135 @@
+// ee_cache_attn.cu -- C ABI: attention over a paged cache of quantised keys and
+// values, behind a prefix in 16 bits that the sequences share.
+#include <cfloat>
+
+#include "ee_cache_attn.cuh"
+#include "ee_prompt.cuh"
+
+namespace ee {
+
+int* gemm_status_ptr();  // ee_ops.cu: the status word of the tensor-core kernels on the current device
+int cache_view(const ee_cache* c, const int32_t* table, int64_t table_row, int32_t width, const int32_t* k_lens,
+               int32_t n_seq, CacheView* v);                       // ee_cache.cu
+int prompt_sums_splits(long long tq, long long tk, int n_q, int n_kv);                         // ee_prompt.cu
+int launch_prompt_sums(const PromptArgs& a, int head_dim, int act_dtype, cudaStream_t s);
+
+constexpr unsigned long long kCacheWaitNs = 1000000000ull;
+
+// How a call runs, by its mean of rows (queries x group) per sequence and key
+// head: up to 8, one MMA column tile a warp; up to 16, two; above, four warps of
+// two tiles share a ring of keys.
+static CachePlan cache_plan(long long tq, int n_seq, int group) {
+  const long long rows = tq * group;
+  if (rows <= 8ll * n_seq) return CachePlan{1, 1};
+  if (rows <= 16ll * n_seq) return CachePlan{2, 1};
+  return CachePlan{2, 4};
+}
+static int plan_rows(const CachePlan& p) { return 8 * p.nt * p.w; }
+template <int HD, int BITS>
+static int plan_workers_b(const CachePlan& p) {
+  return p.w > 1 ? CaShape<HD, BITS, 2, 4>::WORKERS : p.nt > 1 ? CaShape<HD, BITS, 2, 1>::WORKERS : CaShape<HD, BITS, 1, 1>::WORKERS;
+}
+static int plan_workers(const CachePlan& p, int hd, int bits) {
+  if (hd == 64) return bits == 8 ? plan_workers_b<64, 8>(p) : plan_workers_b<64, 4>(p);
+  return bits == 8 ? plan_workers_b<128, 8>(p) : plan_workers_b<128, 4>(p);
+}
+static long long own_partials(const CachePlan& p, int hd, int bits) {  // partial rows
+  return (long long)device_sms() * plan_workers(p, hd, bits) * 2 * plan_rows(p);
+}
+
+}  // namespace ee
+
+using namespace ee;
+
+extern "C" {
+
+size_t ee_cache_attention_workspace_bytes(int64_t tq, int32_t n_seq, int32_t n_q, int32_t n_kv, int32_t head_dim,
+                                          int32_t bits, int64_t prefix_len) {
+  if (tq < 1 || n_seq < 1 || n_q < 1 || n_kv < 1 || n_q % n_kv || prefix_len < 0 || tq > 0x7fffff00 / n_q) return 0;
+  if ((head_dim != 64 && head_dim != 128) || (bits != 8 && bits != 4)) return 0;
+  long long rows = own_partials(cache_plan(tq, n_seq, n_q / n_kv), head_dim, bits);
+  if (prefix_len) rows += prompt_sums_splits(tq, prefix_len, n_q, n_kv) * tq * n_q;
+  return (size_t)rows * (head_dim + 2) * 4;
+}
+
+int ee_cache_attention(const ee_cache* cache, const void* q, int64_t q_tok, int64_t q_head, void* out, int64_t o_tok,
+                       int64_t o_head, const int32_t* cu_q, const int32_t* table, int64_t table_row, int32_t width,
+                       const int32_t* k_lens, const void* prefix_k, int64_t pk_tok, int64_t pk_head,
+                       const void* prefix_v, int64_t pv_tok, int64_t pv_head, int64_t prefix_len, int64_t tq,
+                       int32_t n_seq, int32_t n_q, int32_t causal, float scale, int32_t act_dtype, void* workspace,
+                       size_t workspace_bytes, ee_stream_t stream) {
+  if (act_dtype != EE_BF16 && act_dtype != EE_F16) return EE_ERR_DTYPE;
+  CacheAttnArgs a{};
+  int rc = cache_view(cache, table, table_row, width, k_lens, n_seq, &a.c);
+  if (rc) return rc;
+  const int n_kv = cache->kv_heads, hd = cache->head_dim;
+  if (tq < 0 || n_q < 1 || n_q > 65535 || n_q % n_kv != 0 || prefix_len < 0 || prefix_len > 0x7fffff00) return EE_ERR_SHAPE;
+  if (tq > 0x7fffff00 / n_q) return EE_ERR_SHAPE;  // rows are 31-bit numbers
+  if (prefix_len && n_q / n_kv > 128) return EE_ERR_UNSUPPORTED;
+  const float scale_log2 = scale * 1.4426950408889634f;
+  if (!(scale > 0.f) || !(scale_log2 <= FLT_MAX)) return EE_ERR_ARG;
+  if (tq == 0 || n_seq == 0) return EE_OK;
+  if (!q || !out || !cu_q || (prefix_len && (!prefix_k || !prefix_v))) return EE_ERR_ARG;
+  if (!aligned16(q) || !aligned16(out) || ((uintptr_t)cu_q & 3)) return EE_ERR_ALIGN;
+  if ((q_tok | q_head | o_tok | o_head) % 8 != 0) return EE_ERR_ALIGN;
+  if (prefix_len && (!aligned16(prefix_k) || !aligned16(prefix_v) || (pk_tok | pk_head | pv_tok | pv_head) % 8 != 0))
+    return EE_ERR_ALIGN;
+  rc = check_device();
+  if (rc) return rc;
+  const CachePlan plan = cache_plan(tq, n_seq, n_q / n_kv);
+  const size_t need = ee_cache_attention_workspace_bytes(tq, n_seq, n_q, n_kv, hd, cache->bits, prefix_len);
+  if (!workspace || workspace_bytes < need) return EE_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return EE_ERR_ALIGN;
+  cudaStream_t s = (cudaStream_t)stream;
+  a.q = q; a.out = out;
+  a.cu_q = cu_q;
+  a.q_tok = q_tok; a.q_head = q_head; a.o_tok = o_tok; a.o_head = o_head;
+  a.tq = (int)tq; a.n_q = n_q; a.group = n_q / n_kv;
+  a.causal = causal != 0;
+  a.rows = plan_rows(plan);
+  a.scale_log2 = scale_log2;
+  a.k_steps = cache->k_steps; a.v_steps = cache->v_steps;
+  a.timeout_ns = kCacheWaitNs;
+  a.status = gemm_status_ptr();
+  if (!a.status) return EE_ERR_DEVICE;
+  const long long own = own_partials(plan, hd, cache->bits);
+  a.part = reinterpret_cast<float*>(workspace);
+  float* pre = a.part + own * hd;
+  if (prefix_len) {
+    PromptArgs p{};
+    p.q = q; p.k = prefix_k; p.v = prefix_v;
+    p.q_tok = q_tok; p.q_head = q_head; p.k_tok = pk_tok; p.k_head = pk_head; p.v_tok = pv_tok; p.v_head = pv_head;
+    p.tq = (int)tq; p.tk = (int)prefix_len; p.n_seq = 1;
+    p.n_q = n_q; p.n_kv = n_kv; p.group = a.group;
+    p.scale_log2 = scale_log2;
+    p.splits = a.pre_splits = prompt_sums_splits(tq, prefix_len, n_q, n_kv);
+    p.sums = 1;
+    p.part = pre;
+    a.stat = pre + (long long)a.pre_splits * tq * n_q * hd;
+    p.stat = a.stat + own * 2;
+    a.pre_part = p.part; a.pre_stat = p.stat;
+    rc = launch_prompt_sums(p, hd, act_dtype, s);
+    if (rc) return rc;
+  } else {
+    a.stat = pre;
+  }
+  CacheMaps m;
+  if (a.c.width == 0 || a.c.pages == 0) {  // no keys but the prefix's: the maps are not used
+    a.c.width = 0;
+    m = CacheMaps{};
+  } else {
+    const int rb = hd * cache->bits / 8;
+    const uint64_t rows = (uint64_t)cache->pages * n_kv * cache->page_size;
+    const auto sw = rb == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : rb == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
+    if (!make_tmap_2d(&m.k, cache->k_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, rb, rows, rb, rb, kCaKeys, sw) ||
+        !make_tmap_2d(&m.v, cache->v_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, rb, rows, rb, rb, kCaKeys, sw))
+      return EE_ERR_SHAPE;
+  }
+  if (act_dtype == EE_BF16)
+    return hd == 64 ? launch_cache_attn<__nv_bfloat16, 64>(m, a, plan, cache->bits, s)
+                    : launch_cache_attn<__nv_bfloat16, 128>(m, a, plan, cache->bits, s);
+  return hd == 64 ? launch_cache_attn<__half, 64>(m, a, plan, cache->bits, s)
+                  : launch_cache_attn<__half, 128>(m, a, plan, cache->bits, s);
+}
+
+}  // extern "C"

@@ -5,6 +5,7 @@
 
 #include "ee_host.h"
 #include "ee_prompt.cuh"
+#include "ee_prompt_list.cuh"
 #include "ee_prompt_tc.cuh"
 
 namespace ee {
@@ -35,65 +36,10 @@ template <int HD> constexpr int pr_stage() { return 2 * kPrStep * HD * 2; }  // 
 template <int HD> constexpr int pr_smem() { return pr_warps<HD>() * kPrStages * pr_stage<HD>(); }
 
 // steps of sequence b's items (all its row blocks and key heads), and of one item
-EE_DEV long long pr_steps(const PromptArgs& a, const PromptSeq& s, int& per_item) {
+EE_DEV PromptSeq list_seq(const PromptArgs& a, int b) { return prompt_seq(a, b); }
+EE_DEV long long list_steps(const PromptArgs& a, const PromptSeq& s, int& per_item) {
   per_item = (s.klen + kPrStep - 1) / kPrStep;
   return (long long)((s.qlen * a.group + 15) / 16) * a.n_kv * per_item;
-}
-
-// The list of steps: its length, and for every thread the steps before its
-// share of the sequences (`per` each, consecutive). All threads of the CTA.
-// visit(b, s, before): each of the thread's sequences and the steps of its own
-// ones before it.
-template <int THREADS>
-struct PrList {
-  long long before[THREADS];
-  long long warp_sum[THREADS / 32];
-};
-template <int THREADS, typename Visit>
-EE_DEV long long pr_list(const PromptArgs& a, PrList<THREADS>* sh, int per, Visit visit) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  long long mine = 0;
-  for (int b = tid * per; b < min((tid + 1) * per, a.n_seq); ++b) {
-    int n;
-    const PromptSeq s = prompt_seq(a, b);
-    visit(b, s, mine);
-    mine += pr_steps(a, s, n);
-  }
-  long long inc = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long t = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += t;
-  }
-  if (lane == 31) sh->warp_sum[warp] = inc;
-  __syncthreads();
-  long long base = 0, total = 0;
-#pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) {
-    if (w < warp) base += sh->warp_sum[w];
-    total += sh->warp_sum[w];
-  }
-  sh->before[tid] = base + inc - mine;
-  __syncthreads();
-  return total;
-}
-// Steps in a warp's share of a list of `total`, for `most` warps: warp w takes
-// steps w * share .., so step x belongs to warp x / share.
-EE_DEV long long pr_div(long long a, long long b) {  // of values >= 0, mostly below 2^32
-  return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
-}
-EE_DEV long long pr_share(long long total, int most) {
-  const long long q = pr_div(total + most - 1, most);
-  return q < kPrMinSteps ? kPrMinSteps : q;
-}
-
-EE_DEV void pr_ldsm(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
-}
-EE_DEV void pr_ldsm_t(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
 
 // A place in the list: a step of an item of a sequence.
@@ -103,7 +49,7 @@ struct PrAt {
   EE_DEV void enter(const PromptArgs& a, int seq) {  // sequence `seq` or the next one that has steps
     for (b = seq; b < a.n_seq; ++b) {
       s = prompt_seq(a, b);
-      const long long n = pr_steps(a, s, per_item);
+      const long long n = list_steps(a, s, per_item);
       if (n > 0) {
         items = (s.qlen * a.group + 15) / 16 * a.n_kv;
         break;
@@ -130,8 +76,8 @@ __global__ void __launch_bounds__(32 * pr_warps<HD>(), 1) prompt_rows_kernel(con
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3, mi = lane >> 3;
   const int per = (a.n_seq + NT - 1) / NT;
-  const long long total = pr_list<NT>(a, &sh, per, [](int, const PromptSeq&, long long) {});
-  const long long share = pr_share(total, (int)gridDim.x * NW);
+  const long long total = pr_list<NT>(a, &sh, per, a.n_seq, [](int, const PromptSeq&, long long) {});
+  const long long share = pr_share(total, (int)gridDim.x * NW, kPrMinSteps);
   const long long me = (long long)warp * gridDim.x + blockIdx.x;  // neighbours in the list on different SMs
   const long long first = me * share;
   if (first >= total) return;
@@ -355,90 +301,6 @@ __global__ void __launch_bounds__(32 * pr_warps<HD>(), 1) prompt_rows_kernel(con
   cp_async_wait<0>();
 }
 
-// Joins the partial rows of one (token, head) by one CTA: `n` of them at
-// slot(i) of part / stat, 1024 at a time with a running maximum. A thread per
-// part for the weights, then hd / 4 threads across the values and the rest
-// across the parts, so that both passes have their loads in flight together.
-constexpr int kPrJoin = 256, kPrChunk = 4 * kPrJoin;
-template <int HD>
-struct JoinSmem {
-  float wt[kPrChunk], red[2][kPrJoin / 32];
-  float4 sv[4 * kPrJoin / HD][HD / 4];
-};
-template <typename T, int HD, typename Slot>
-EE_DEV void join_row(const PromptArgs& a, long long n, Slot slot, T* out, JoinSmem<HD>* sh) {
-  constexpr int LANES = HD / 4, GROUPS = kPrJoin / LANES;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, c = tid % LANES, grp = tid / LANES;
-  const float2* stat = reinterpret_cast<const float2*>(a.stat);
-  float m = -INFINITY, l = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (long long i0 = 0; i0 < n; i0 += kPrChunk) {
-    const int here = (int)(n - i0 < kPrChunk ? n - i0 : kPrChunk);
-    float2 st[kPrChunk / kPrJoin];
-    float x = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < kPrChunk / kPrJoin; ++j) {
-      const int i = tid + j * kPrJoin;
-      st[j] = i < here ? __ldg(stat + slot(i0 + i)) : make_float2(-INFINITY, 0.f);
-      x = fmaxf(x, st[j].x);
-    }
-    x = warp_max(x);
-    if (lane == 0) sh->red[0][warp] = x;
-    __syncthreads();
-    float top = m;
-#pragma unroll
-    for (int i = 0; i < kPrJoin / 32; ++i) top = fmaxf(top, sh->red[0][i]);
-    const float u = top == -INFINITY ? 0.f : top, old = exp2f(m - u);
-    m = top;
-    l *= old;
-    acc = make_float4(acc.x * old, acc.y * old, acc.z * old, acc.w * old);
-#pragma unroll
-    for (int j = 0; j < kPrChunk / kPrJoin; ++j) {
-      // weight 0: the part has seen no key, its sums need not have been written
-      const float f = st[j].y == 0.f ? 0.f : exp2f(st[j].x - u);
-      l += f * st[j].y;
-      sh->wt[tid + j * kPrJoin] = f;
-    }
-    __syncthreads();
-    for (int i = grp; i < here; i += 8 * GROUPS) {  // loads first: none waits for another's weight
-      float4 v[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        v[k] = __ldg(reinterpret_cast<const float4*>(a.part + slot(i0 + min(i + k * GROUPS, here - 1)) * HD) + c);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float w = i + k * GROUPS < here ? sh->wt[i + k * GROUPS] : 0.f;
-        if (w != 0.f) {
-          acc.x += w * v[k].x;
-          acc.y += w * v[k].y;
-          acc.z += w * v[k].z;
-          acc.w += w * v[k].w;
-        }
-      }
-    }
-    __syncthreads();
-  }
-  l = warp_sum(l);
-  if (lane == 0) sh->red[1][warp] = l;
-  sh->sv[grp][c] = acc;
-  __syncthreads();
-  if (grp) return;
-  l = 0.f;
-#pragma unroll
-  for (int i = 0; i < kPrJoin / 32; ++i) l += sh->red[1][i];
-#pragma unroll
-  for (int g = 1; g < GROUPS; ++g) {
-    const float4 v = sh->sv[g][c];
-    acc.x += v.x;
-    acc.y += v.y;
-    acc.z += v.z;
-    acc.w += v.w;
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees no key is zero
-  *reinterpret_cast<uint2*>(out + 4 * c) =
-      make_uint2(Act<T>::pack2(acc.x * inv, acc.y * inv), Act<T>::pack2(acc.z * inv, acc.w * inv));
-}
-
 // The parts of the tensor-core kernel's keys, by (part, token, head).
 template <typename T, int HD>
 __global__ void __launch_bounds__(kPrJoin) prompt_combine_kernel(const __grid_constant__ PromptArgs a) {
@@ -448,53 +310,8 @@ __global__ void __launch_bounds__(kPrJoin) prompt_combine_kernel(const __grid_co
   // rows outside the sequences have no parts and stay as they were
   if (tok < __ldg(a.cu_q) || tok >= __ldg(a.cu_q + a.n_seq)) return;
   const long long step = (long long)a.tq * a.n_q, at = (long long)tok * a.n_q + h;
-  join_row<T, HD>(a, a.splits, [&](long long i) { return at + i * step; },
+  join_row<T, HD>(a.part, a.stat, a.splits, [&](long long i) { return at + i * step; },
                   reinterpret_cast<T*>(a.out) + (long long)tok * a.o_tok + h * a.o_head, &sh);
-}
-
-// The same by one warp, 32 parts at a time, hd / 32 values a lane: for items of
-// few parts, where a CTA's barriers cost more than its width saves.
-template <typename T, int HD, typename Slot>
-EE_DEV void join_row_warp(const PromptArgs& a, long long n, Slot slot, T* out) {
-  constexpr int V = HD / 32;
-  const int lane = threadIdx.x & 31;
-  float m = -INFINITY, l = 0.f, v[V] = {};
-  for (long long i0 = 0; i0 < n; i0 += 32) {
-    const int here = (int)(n - i0 < 32 ? n - i0 : 32);
-    const float2 st = lane < here ? __ldg(reinterpret_cast<const float2*>(a.stat) + slot(i0 + lane))
-                                  : make_float2(-INFINITY, 0.f);
-    const float top = fmaxf(m, warp_max(st.x));
-    const float u = top == -INFINITY ? 0.f : top, old = exp2f(m - u);
-    m = top;
-    const float f = st.y == 0.f ? 0.f : exp2f(st.x - u);
-    l = l * old + f * st.y;
-#pragma unroll
-    for (int e = 0; e < V; ++e) v[e] *= old;
-    for (int i = 0; i < here; i += 8) {  // loads first: none waits for another's weight
-      float2 x[8][V / 2];
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-#pragma unroll
-        for (int e = 0; e < V / 2; ++e)
-          x[k][e] = __ldg(reinterpret_cast<const float2*>(a.part + slot(i0 + min(i + k, here - 1)) * HD + lane * V) + e);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float w = __shfl_sync(0xffffffffu, f, (i + k) & 31);  // 0 past the last part
-        if (w != 0.f) {
-#pragma unroll
-          for (int e = 0; e < V / 2; ++e) {
-            v[2 * e] += w * x[k][e].x;
-            v[2 * e + 1] += w * x[k][e].y;
-          }
-        }
-      }
-    }
-  }
-  l = warp_sum(l);
-  const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees no key is zero
-#pragma unroll
-  for (int e = 0; e < V; e += 2)
-    *reinterpret_cast<uint32_t*>(out + lane * V + e) = Act<T>::pack2(v[e] * inv, v[e + 1] * inv);
 }
 
 // The rows of the kernel for few rows whose item was cut, and rows without
@@ -515,7 +332,7 @@ __global__ void __launch_bounds__(kPrJoin) prompt_join_kernel(const __grid_const
   PromptSeq hit{};
   int hit_b = -1;
   long long hit_at = 0;  // steps of the thread's own sequences before the token's
-  const long long total = pr_list<kPrJoin>(a, &list, per, [&](int b, const PromptSeq& s, long long before) {
+  const long long total = pr_list<kPrJoin>(a, &list, per, a.n_seq, [&](int b, const PromptSeq& s, long long before) {
     if (hit_b < 0 && tok >= s.q0 && tok < s.q0 + s.qlen) {
       hit = s;
       hit_b = b;
@@ -532,8 +349,8 @@ __global__ void __launch_bounds__(kPrJoin) prompt_join_kernel(const __grid_const
   if (found == 0x7fffffff) return;  // rows outside the sequences stay as they were
   const PromptSeq s = seq;
   int steps;
-  pr_steps(a, s, steps);
-  const long long share = pr_share(total, most);
+  list_steps(a, s, steps);
+  const long long share = pr_share(total, most, kPrMinSteps);
   const int h = MANY ? blockIdx.y : blockIdx.y * (kPrJoin / 32) + (threadIdx.x >> 5);
   if (h < a.n_q) {
     const int kvh = h / a.group, r = (tok - s.q0) * a.group + h % a.group;
@@ -547,8 +364,8 @@ __global__ void __launch_bounds__(kPrJoin) prompt_join_kernel(const __grid_const
     }
     auto slot = [&](long long i) { return (w0 + i) * 32 + (i == 0 ? front : 0) + r % 16; };
     T* out = reinterpret_cast<T*>(a.out) + (long long)tok * a.o_tok + h * a.o_head;
-    if (MANY) join_row<T, HD>(a, n, slot, out, &sh);
-    else join_row_warp<T, HD>(a, n, slot, out);
+    if (MANY) join_row<T, HD>(a.part, a.stat, n, slot, out, &sh);
+    else join_row_warp<T, HD>(a.part, a.stat, n, slot, out);
   }
 }
 
@@ -588,7 +405,7 @@ static size_t prompt_ws_bytes(const PromptPlan& pl, long long tq, int n_q, int h
 
 template <typename T, int HD>
 static int launch_combine(const PromptArgs& a, cudaStream_t s) {
-  if (a.splits == 1) return EE_OK;
+  if (a.splits == 1 || a.sums) return EE_OK;
   return launch_pdl(prompt_combine_kernel<T, HD>, dim3((unsigned)a.tq, a.n_q), dim3(kPrJoin), 0, s, a) == cudaSuccess
              ? EE_OK
              : EE_ERR_LAUNCH;
@@ -662,6 +479,20 @@ template <typename T>
 static int launch_prompt(const PromptArgs& a, const PromptPlan& pl, int hd, cudaStream_t s) {
   if (pl.tc) return hd == 64 ? launch_tc<T, 64>(a, s) : launch_tc<T, 128>(a, s);
   return hd == 64 ? launch_rows<T, 64>(a, s) : launch_rows<T, 128>(a, s);
+}
+
+// The sums of all tq rows as one sequence over all tk keys, left unfinished in
+// a.part and a.stat: what a caller joins with the keys of its own. The parts of
+// the keys are those that leave no SM idle, of 512 keys or more.
+int prompt_sums_splits(long long tq, long long tk, int n_q, int n_kv) {
+  const int group = n_q / n_kv, tpt = 128 / group;
+  const long long items = (tq + 2 * tpt - 1) / (2 * tpt) * n_kv, want = device_sms() / items, most = tk / kPtMinKeys;
+  const long long s = want < most ? want : most;
+  return s < 1 ? 1 : (int)s;
+}
+int launch_prompt_sums(const PromptArgs& a, int hd, int act_dtype, cudaStream_t s) {
+  if (act_dtype == EE_BF16) return hd == 64 ? launch_tc<__nv_bfloat16, 64>(a, s) : launch_tc<__nv_bfloat16, 128>(a, s);
+  return hd == 64 ? launch_tc<__half, 64>(a, s) : launch_tc<__half, 128>(a, s);
 }
 
 }  // namespace ee

@@ -37,6 +37,7 @@ struct PromptArgs {
   int tq, tk, n_seq, n_q, n_kv, group, causal;
   float scale_log2;  // scale * log2(e)
   int splits;        // tensor-core kernel: parts of the keys
+  int sums;          // it leaves its sums in part and stat whatever the number of parts
   float* part;       // sums of partial rows and, in stat, their maximum and weight: [splits][tq][n_q][hd], or by
   float* stat;       // worker ([workers][2][16][hd]) in the kernel for few rows
 };
@@ -47,6 +48,7 @@ struct PromptSeq {
 
 EE_DEV PromptSeq prompt_seq(const PromptArgs& a, int b) {
   PromptSeq s;
+  if (!a.cu_q) return PromptSeq{0, a.tq, 0, a.tk, 0};  // one sequence of all rows
   s.q0 = min(max(__ldg(a.cu_q + b), 0), a.tq);
   s.qlen = min(max(__ldg(a.cu_q + b + 1), s.q0), a.tq) - s.q0;
   s.k0 = min(max(__ldg(a.cu_k + b), 0), a.tk);

@@ -611,7 +611,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         if (!ok) break;
       }
       tc_fence_after();
-      const bool whole = p.splits == 1;
+      const bool whole = p.splits == 1 && !p.sums;
       const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees no key is zero
       const long long at = ((long long)part * p.tq + out_row) * p.n_q + head;
       if (!whole && mine) *reinterpret_cast<float2*>(p.stat + 2 * at) = make_float2(m, l);

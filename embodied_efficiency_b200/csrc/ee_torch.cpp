@@ -396,6 +396,54 @@ PyObject* prompt_attention(PyObject*, PyObject* const* a, Py_ssize_t argc) {
   return give(rc, out);
 }
 
+// cache_attention(keys, record, q, cu_q, table, k_lens, causal, scale, prefix)
+PyObject* cache_attention(PyObject*, PyObject* const* a, Py_ssize_t argc) {
+  if (argc != 9 || !PyBool_Check(a[6])) return none();
+  Call c;
+  Places p;
+  if (!places(c, a[0], a[1], a[3], a[4], a[5], p)) return none();
+  const Tensor *q = c.get(a[2]), *pk = nullptr, *pv = nullptr;
+  const int64_t hk = p.cache->kv_heads, hd = p.cache->head_dim;
+  if (!c.need(q && heads_ok(*q) && q->size(0) > 0 && q->size(2) == hd && q->size(1) >= 1 && q->size(1) < 65536 &&
+              q->size(1) % hk == 0 && q->size(0) <= 0x7fffff00 / q->size(1)))
+    return none();
+  const int64_t tq = q->size(0), hq = q->size(1);
+  if (a[8] != Py_None) {
+    if (!c.need(PyTuple_Check(a[8]) && PyTuple_GET_SIZE(a[8]) == 2)) return none();
+    pk = c.get(PyTuple_GET_ITEM(a[8], 0));
+    pv = c.get(PyTuple_GET_ITEM(a[8], 1));
+    if (!c.need(pk && pv && heads_ok(*pk) && heads_ok(*pv) && pk->sizes() == pv->sizes() && pk->size(0) > 0 &&
+                pk->size(0) < (1 << 30) && pk->size(1) == hk && pk->size(2) == hd &&
+                pk->scalar_type() == q->scalar_type() && pv->scalar_type() == q->scalar_type() && hq / hk <= 128))
+      return none();
+  }
+  float scale = 0.f;
+  if (a[7] == Py_None) {
+    scale = (float)(1.0 / std::sqrt((double)hd));
+  } else if (PyFloat_Check(a[7])) {
+    scale = (float)PyFloat_AS_DOUBLE(a[7]);
+  }
+  if (!c.need(scale > 0.f && scale < 2.0e38f)) return none();
+  const bool causal = a[6] == Py_True;
+  const int64_t plen = pk ? pk->size(0) : 0;
+  Tensor out;
+  int rc;
+  {
+    NoGil others;
+    out = at::empty(q->sizes(), q->options());
+    const size_t need = ee_cache_attention_workspace_bytes(tq, (int32_t)p.n, (int32_t)hq, (int32_t)hk, (int32_t)hd,
+                                                           p.cache->bits, plen);
+    const Tensor ws = at::empty({(int64_t)need}, q->options().dtype(at::kByte));
+    rc = ee_cache_attention(p.cache, q->data_ptr(), q->stride(0), q->stride(1), out.data_ptr(), out.stride(0),
+                            out.stride(1), p.cu, p.table, p.table_row, (int32_t)p.width, p.k_lens,
+                            pk ? pk->data_ptr() : nullptr, pk ? pk->stride(0) : 0, pk ? pk->stride(1) : 0,
+                            pv ? pv->data_ptr() : nullptr, pv ? pv->stride(0) : 0, pv ? pv->stride(1) : 0, plen, tq,
+                            (int32_t)p.n, (int32_t)hq, causal, scale, act_code(q->scalar_type()), ws.data_ptr(), need,
+                            c.stream());
+  }
+  return give(rc, out);
+}
+
 // C++ exceptions (out of memory in an allocation) become Python's: the Python
 // function then meets the same condition and raises torch's own error.
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
@@ -411,7 +459,8 @@ PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&guarded<name>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {EE_METHOD(int8_linear),  EE_METHOD(int8_matmul),      EE_METHOD(quantize_tokens),
                          EE_METHOD(rotary_embed), EE_METHOD(norm_rotary_embed), EE_METHOD(prompt_attention),
-                         EE_METHOD(cache_write),  EE_METHOD(cache_read),        {nullptr, nullptr, 0, nullptr}};
+                         EE_METHOD(cache_write),  EE_METHOD(cache_read),        EE_METHOD(cache_attention),
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "ee_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

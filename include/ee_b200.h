@@ -302,6 +302,30 @@ int ee_cache_read(const ee_cache* cache, void* k, int64_t k_tok, int64_t k_head,
                   const int32_t* cu, const int32_t* table, int64_t table_row, int32_t width, const int32_t* k_lens,
                   int64_t tokens, int32_t n_seq, int32_t act_dtype, ee_stream_t stream);
 
+/* Attention of queries cu_q[b] .. cu_q[b + 1] of q [tq][n_q][head_dim] over
+ * sequence b's first k_lens[b] keys of the cache (at most what a row of the
+ * table covers) and, before those, over prefix_len keys prefix_k / prefix_v
+ * [prefix_len][kv_heads][head_dim] in the act dtype that every sequence shares
+ * (0: none; n_q / kv_heads at most 128 with one). Head h reads key head
+ * h / (n_q / kv_heads). causal: a sequence's last query sees its last key, query
+ * i keys 0 .. k_lens[b] - n + i and the prefix. A query that sees no key gives
+ * zeros; rows of `out` that belong to no sequence stay as they were. A key's
+ * code * step counts as it is (NaN where its head held an infinity or NaN), with
+ * fp32 statistics and sums; weights are rounded to 16 bits (fp16: twice) for
+ * the product with the values. Strides in elements, multiples of 8. tq * n_q <
+ * 2^31 - 255. scale as for ee_prompt_attention.
+ * workspace: ee_cache_attention_workspace_bytes() bytes, 16-byte aligned; calls
+ * that may overlap need one each. A wait that gives up after a second leaves
+ * EE_ERR_TIMEOUT in the status word of ee_wq_gemm_status. */
+size_t ee_cache_attention_workspace_bytes(int64_t tq, int32_t n_seq, int32_t n_q, int32_t n_kv, int32_t head_dim,
+                                          int32_t bits, int64_t prefix_len);
+int ee_cache_attention(const ee_cache* cache, const void* q, int64_t q_tok, int64_t q_head, void* out, int64_t o_tok,
+                       int64_t o_head, const int32_t* cu_q, const int32_t* table, int64_t table_row, int32_t width,
+                       const int32_t* k_lens, const void* prefix_k, int64_t pk_tok, int64_t pk_head,
+                       const void* prefix_v, int64_t pv_tok, int64_t pv_head, int64_t prefix_len, int64_t tq,
+                       int32_t n_seq, int32_t n_q, int32_t causal, float scale, int32_t act_dtype, void* workspace,
+                       size_t workspace_bytes, ee_stream_t stream);
+
 /* ---- fused flow-matching sampler --------------------------------------- */
 typedef struct ee_linear {
   const void* weight; /* see EE_W_*                                       */

@@ -100,6 +100,32 @@ def test_cache_arguments(cache):
             call()
 
 
+def test_attention_arguments(cache):
+    from embodied_efficiency_b200 import cache_attention
+    q, cu = torch.zeros(5, 4, 64, dtype=BF), torch.tensor([0, 5], dtype=torch.int32)
+    tab, kl, p = torch.zeros(1, 4, dtype=torch.int32), torch.tensor([9], dtype=torch.int32), torch.zeros(7, 2, 64, dtype=BF)
+    many = torch.zeros(5, 258, 64, dtype=BF)
+    for match, call in (
+            ("must be a KVCache", lambda: cache_attention(q, p, cu, tab, kl)),
+            ("cu_q must be int32", lambda: cache_attention(q, cache, cu.long(), tab, kl)),
+            ("cu_q needs at least one", lambda: cache_attention(q, cache, cu[:0], tab, kl)),
+            ("k_lens must be int32 \\[1\\]", lambda: cache_attention(q, cache, cu, tab, cu)),
+            ("table must be int32", lambda: cache_attention(q, cache, cu, tab.float(), kl)),
+            ("q must be bf16 or fp16", lambda: cache_attention(q.float(), cache, cu, tab, kl)),
+            ("must be \\[tokens, heads, 64\\]", lambda: cache_attention(q[..., :32], cache, cu, tab, kl)),
+            ("not a multiple of 2", lambda: cache_attention(q[:, :3], cache, cu, tab, kl)),
+            ("scale must be", lambda: cache_attention(q, cache, cu, tab, kl, scale=-1.0)),
+            ("scale must be", lambda: cache_attention(q, cache, cu, tab, kl, scale=float("nan"))),
+            ("prefix k", lambda: cache_attention(q, cache, cu, tab, kl, prefix=(p, p[:6]))),
+            ("prefix k", lambda: cache_attention(q, cache, cu, tab, kl, prefix=(p.half(), p.half()))),
+            ("prefix k", lambda: cache_attention(q, cache, cu, tab, kl, prefix=(p[:, :1], p[:, :1]))),
+            ("at most 128", lambda: cache_attention(many, cache, cu, tab, kl, prefix=(p, p)))):
+        with pytest.raises(ValueError, match=match):
+            call()
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        cache_attention(q, cache, cu, tab, kl, prefix=(p, p))
+
+
 def test_abi_codes(lib):
     from embodied_efficiency_b200 import _lib
     assert lib.ee_struct_size(4) == ctypes.sizeof(_lib.Cache)
@@ -129,3 +155,23 @@ def test_abi_codes(lib):
             assert fn(c, *(args[:i] + [v] + args[i + 1:])) == rc, (i, v)
         for i in (9, 11, 12):
             assert fn(c, *(args[:i] + [0] + args[i + 1:])) == 0  # nothing to do
+    # ee_cache_attention(cache, q, tok, head, out, tok, head, cu_q, table, table_row, width, k_lens, prefix_k, tok, head,
+    #                    prefix_v, tok, head, prefix_len, tq, n_seq, n_q, causal, scale, act, workspace, bytes, stream)
+    ca = [16, 256, 64, 16, 256, 64, 16, 16, 4, 4, 16, 16, 128, 64, 16, 128, 64, 7, 5, 1, 4, 1, 0.125, _lib.EE_BF16, 0, 0,
+          None]
+    fn = lib.ee_cache_attention
+    for f, v, rc in (("bits", 16, 9), ("head_dim", 96, 9), ("page_size", 16, 9), ("k_codes", 0, 1), ("v_codes", 24, 3)):
+        assert fn(ctypes.byref(_lib.Cache(**{**good, f: v})), *ca) == rc, (f, v)
+    assert fn(None, *ca) == 1
+    for i, v, rc in ((0, 0, 1), (3, 0, 1), (6, 0, 1), (7, 0, 1), (10, 0, 1), (11, 0, 1), (14, 0, 1), (0, 8, 3), (3, 8, 3),
+                     (1, 4, 3), (5, 12, 3), (6, 2, 3), (11, 8, 3), (13, 4, 3), (9, -1, 2), (17, -1, 2), (17, 1 << 31, 2),
+                     (18, -1, 2), (18, 1 << 30, 2), (19, -1, 2), (20, 3, 2), (20, 0, 2), (20, 260, 9), (22, 0.0, 1),
+                     (22, float("nan"), 1), (22, 3e38, 1), (23, 2, 4)):
+        assert fn(c, *(ca[:i] + [v] + ca[i + 1:])) == rc, (i, v)
+    for i in (18, 19):
+        assert fn(c, *(ca[:i] + [0] + ca[i + 1:])) == 0
+    need = lib.ee_cache_attention_workspace_bytes
+    assert need(5, 1, 4, 2, 64, 8, 0) > 0 and need(5, 1, 4, 2, 64, 8, 100) > need(5, 1, 4, 2, 64, 8, 0)
+    for bad in ((0, 1, 4, 2, 64, 8, 0), (5, 1, 3, 2, 64, 8, 0), (5, 1, 4, 2, 96, 8, 0), (5, 1, 4, 2, 64, 16, 0),
+                (1 << 30, 1, 4, 2, 64, 8, 0), (5, 1, 4, 2, 64, 8, -1)):
+        assert need(*bad) == 0
