@@ -108,7 +108,7 @@ SIGNATURES = {
                        + [c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_int32, c_int32, c_void_p]),
     "ee_cache_read": (c_int32, [ctypes.POINTER(Cache)] + [c_void_p, c_int64, c_int64] * 2
                       + [c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_int32, c_int32, c_void_p]),
-    "ee_cache_attention_workspace_bytes": (c_size_t, [c_int64] + [c_int32] * 5 + [c_int64]),
+    "ee_cache_attention_workspace_bytes": (c_size_t, [c_int64] + [c_int32] * 5 + [c_int64] * 2),
     "ee_cache_attention": (c_int32, [ctypes.POINTER(Cache)] + [c_void_p, c_int64, c_int64] * 2
                            + [c_void_p, c_void_p, c_int64, c_int32, c_void_p] + [c_void_p, c_int64, c_int64] * 2
                            + [c_int64, c_int64] + [c_int32] * 3 + [c_float, c_int32, c_void_p, c_size_t, c_void_p]),

@@ -88,8 +88,8 @@ def _places(cache, cu, table, k_lens, name):
     cu, k_lens = _offsets(cu, n + 1, name), _offsets(k_lens, n, "k_lens")
     if table.dim() != 2 or table.dtype != torch.int32 or table.shape[0] != n:
         raise ValueError(f"table must be int32 [{n}, pages], got {table.dtype} {tuple(table.shape)}")
-    if table.shape[1] > 0x7fffffff // cache.page_size:
-        raise ValueError(f"table names {table.shape[1]} pages a sequence: at most {0x7fffffff // cache.page_size}")
+    if table.shape[1] > 0x7fff0000 // cache.page_size:
+        raise ValueError(f"table names {table.shape[1]} pages a sequence: at most {0x7fff0000 // cache.page_size}")
     if table.stride(1) != 1 and table.shape[1] > 1:
         table = table.contiguous()
     return cu, table, k_lens, n
@@ -197,7 +197,7 @@ def cache_attention(q, cache: KVCache, cu_q, table, k_lens, causal: bool = True,
         p_len, pks, pvs = 0, (0, 0), (0, 0)
         if pk is not None and pk.shape[0]:
             (pk, pks), (pv, pvs), p_len = _heads(pk, "prefix k"), _heads(pv, "prefix v"), pk.shape[0]
-        nb = lib.ee_cache_attention_workspace_bytes(tq, n, hq, hk, hd, cache.bits, p_len)
+        nb = lib.ee_cache_attention_workspace_bytes(tq, n, hq, hk, hd, cache.bits, table.shape[1] * cache.page_size, p_len)
         ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
         rc = lib.ee_cache_attention(
             ctypes.byref(cache._c), qc.data_ptr(), qs[0], qs[1], out.data_ptr(), os_[0], os_[1], cu_q.data_ptr(),

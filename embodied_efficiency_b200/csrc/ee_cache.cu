@@ -168,7 +168,7 @@ int cache_view(const ee_cache* c, const int32_t* table, int64_t table_row, int32
   if (c->page_size != 32 && c->page_size != 64 && c->page_size != 128 && c->page_size != 256) return EE_ERR_UNSUPPORTED;
   if (c->pages < 0 || c->kv_heads < 1 || c->kv_heads > 65535 || n_seq < 0 || width < 0) return EE_ERR_SHAPE;
   if ((int64_t)c->pages * c->kv_heads > 0x7fffffff / c->page_size) return EE_ERR_SHAPE;  // rows are 31-bit numbers
-  if ((int64_t)width > 0x7fffffff / c->page_size) return EE_ERR_SHAPE;
+  if ((int64_t)width > 0x7fff0000 / c->page_size) return EE_ERR_SHAPE;  // so are keys, and a tile past the last
   if (c->pages && (!c->k_codes || !c->v_codes || !c->k_steps || !c->v_steps)) return EE_ERR_ARG;
   if (n_seq && (!k_lens || (width && !table))) return EE_ERR_ARG;
   if (((uintptr_t)c->k_codes | (uintptr_t)c->v_codes | (uintptr_t)c->k_steps | (uintptr_t)c->v_steps) & 15)

@@ -3,38 +3,51 @@
 #include <cfloat>
 
 #include "ee_cache_attn.cuh"
-#include "ee_prompt.cuh"
 
 namespace ee {
 
 int* gemm_status_ptr();  // ee_ops.cu: the status word of the tensor-core kernels on the current device
 int cache_view(const ee_cache* c, const int32_t* table, int64_t table_row, int32_t width, const int32_t* k_lens,
                int32_t n_seq, CacheView* v);                       // ee_cache.cu
-int prompt_sums_splits(long long tq, long long tk, int n_q, int n_kv);                         // ee_prompt.cu
+// ee_prompt.cu
+int prompt_sums_splits(long long tq, long long tk, int n_q, int n_kv);
+int prompt_parts(long long tq, int n_seq, int n_q, int n_kv, long long keys);
 int launch_prompt_sums(const PromptArgs& a, int head_dim, int act_dtype, cudaStream_t s);
+int launch_prompt_combine(const PromptArgs& a, int head_dim, int act_dtype, cudaStream_t s);
 
 constexpr unsigned long long kCacheWaitNs = 1000000000ull;
 
 // How a call runs, by its mean of rows (queries x group) per sequence and key
-// head: up to 8, one MMA column tile a warp; up to 16, two; above, four warps of
-// two tiles share a ring of keys.
-static CachePlan cache_plan(long long tq, int n_seq, int group) {
+// head: up to 8, one MMA column tile a warp; up to 16, two; above, the
+// tensor-core kernel's 128-row tiles (64 x 50 rows behind 257..816, 16 heads of
+// 128: the kernel for few rows in 64-row items took 239 us).
+static CachePlan cache_plan(long long tq, int n_seq, int n_q, int n_kv, long long keys) {
+  const int group = n_q / n_kv;
   const long long rows = tq * group;
   if (rows <= 8ll * n_seq) return CachePlan{1, 1};
-  if (rows <= 16ll * n_seq) return CachePlan{2, 1};
-  return CachePlan{2, 4};
+  if (rows <= 16ll * n_seq || group > 128) return CachePlan{2, 1};
+  return CachePlan{0, prompt_parts(tq, n_seq, n_q, n_kv, keys)};
 }
-static int plan_rows(const CachePlan& p) { return 8 * p.nt * p.w; }
 template <int HD, int BITS>
 static int plan_workers_b(const CachePlan& p) {
-  return p.w > 1 ? CaShape<HD, BITS, 2, 4>::WORKERS : p.nt > 1 ? CaShape<HD, BITS, 2, 1>::WORKERS : CaShape<HD, BITS, 1, 1>::WORKERS;
+  return p.nt > 1 ? CaShape<HD, BITS, 2>::WORKERS : CaShape<HD, BITS, 1>::WORKERS;
 }
 static int plan_workers(const CachePlan& p, int hd, int bits) {
   if (hd == 64) return bits == 8 ? plan_workers_b<64, 8>(p) : plan_workers_b<64, 4>(p);
   return bits == 8 ? plan_workers_b<128, 8>(p) : plan_workers_b<128, 4>(p);
 }
-static long long own_partials(const CachePlan& p, int hd, int bits) {  // partial rows
-  return (long long)device_sms() * plan_workers(p, hd, bits) * 2 * plan_rows(p);
+// Partial rows: of the prefix, of the call's own keys in its layout.
+struct CacheParts {
+  long long own, pre;
+  int pre_splits;
+};
+static CacheParts cache_parts(const CachePlan& p, long long tq, int n_q, int n_kv, int hd, int bits, long long prefix_len) {
+  CacheParts c{0, 0, 0};
+  if (prefix_len) c.pre_splits = prompt_sums_splits(tq, prefix_len, n_q, n_kv);
+  c.pre = c.pre_splits * tq * n_q;
+  if (p.nt == 0) c.own = p.splits > 1 || prefix_len ? p.splits * tq * n_q : 0;
+  else c.own = (long long)device_sms() * plan_workers(p, hd, bits) * 2 * 8 * p.nt + (prefix_len ? tq * n_q : 0);
+  return c;
 }
 
 }  // namespace ee
@@ -44,12 +57,11 @@ using namespace ee;
 extern "C" {
 
 size_t ee_cache_attention_workspace_bytes(int64_t tq, int32_t n_seq, int32_t n_q, int32_t n_kv, int32_t head_dim,
-                                          int32_t bits, int64_t prefix_len) {
-  if (tq < 1 || n_seq < 1 || n_q < 1 || n_kv < 1 || n_q % n_kv || prefix_len < 0 || tq > 0x7fffff00 / n_q) return 0;
+                                          int32_t bits, int64_t keys, int64_t prefix_len) {
+  if (tq < 1 || n_seq < 1 || n_q < 1 || n_kv < 1 || n_q % n_kv || keys < 0 || prefix_len < 0 || tq > 0x7fffff00 / n_q) return 0;
   if ((head_dim != 64 && head_dim != 128) || (bits != 8 && bits != 4)) return 0;
-  long long rows = own_partials(cache_plan(tq, n_seq, n_q / n_kv), head_dim, bits);
-  if (prefix_len) rows += prompt_sums_splits(tq, prefix_len, n_q, n_kv) * tq * n_q;
-  return (size_t)rows * (head_dim + 2) * 4;
+  const CacheParts c = cache_parts(cache_plan(tq, n_seq, n_q, n_kv, keys), tq, n_q, n_kv, head_dim, bits, prefix_len);
+  return (size_t)(c.own + c.pre) * (head_dim + 2) * 4;
 }
 
 int ee_cache_attention(const ee_cache* cache, const void* q, int64_t q_tok, int64_t q_head, void* out, int64_t o_tok,
@@ -76,60 +88,99 @@ int ee_cache_attention(const ee_cache* cache, const void* q, int64_t q_tok, int6
     return EE_ERR_ALIGN;
   rc = check_device();
   if (rc) return rc;
-  const CachePlan plan = cache_plan(tq, n_seq, n_q / n_kv);
-  const size_t need = ee_cache_attention_workspace_bytes(tq, n_seq, n_q, n_kv, hd, cache->bits, prefix_len);
-  if (!workspace || workspace_bytes < need) return EE_ERR_WORKSPACE;
+  const long long keys = (long long)width * cache->page_size;
+  const CachePlan plan = cache_plan(tq, n_seq, n_q, n_kv, keys);
+  const CacheParts cp = cache_parts(plan, tq, n_q, n_kv, hd, cache->bits, prefix_len);
+  const size_t need = ee_cache_attention_workspace_bytes(tq, n_seq, n_q, n_kv, hd, cache->bits, keys, prefix_len);
+  if (need && (!workspace || workspace_bytes < need)) return EE_ERR_WORKSPACE;
   if (!aligned16(workspace)) return EE_ERR_ALIGN;
   cudaStream_t s = (cudaStream_t)stream;
-  a.q = q; a.out = out;
-  a.cu_q = cu_q;
-  a.q_tok = q_tok; a.q_head = q_head; a.o_tok = o_tok; a.o_head = o_head;
-  a.tq = (int)tq; a.n_q = n_q; a.group = n_q / n_kv;
-  a.causal = causal != 0;
-  a.rows = plan_rows(plan);
-  a.scale_log2 = scale_log2;
-  a.k_steps = cache->k_steps; a.v_steps = cache->v_steps;
-  a.timeout_ns = kCacheWaitNs;
-  a.status = gemm_status_ptr();
-  if (!a.status) return EE_ERR_DEVICE;
-  const long long own = own_partials(plan, hd, cache->bits);
-  a.part = reinterpret_cast<float*>(workspace);
-  float* pre = a.part + own * hd;
-  if (prefix_len) {
-    PromptArgs p{};
-    p.q = q; p.k = prefix_k; p.v = prefix_v;
-    p.q_tok = q_tok; p.q_head = q_head; p.k_tok = pk_tok; p.k_head = pk_head; p.v_tok = pv_tok; p.v_head = pv_head;
-    p.tq = (int)tq; p.tk = (int)prefix_len; p.n_seq = 1;
-    p.n_q = n_q; p.n_kv = n_kv; p.group = a.group;
-    p.scale_log2 = scale_log2;
-    p.splits = a.pre_splits = prompt_sums_splits(tq, prefix_len, n_q, n_kv);
-    p.sums = 1;
-    p.part = pre;
-    a.stat = pre + (long long)a.pre_splits * tq * n_q * hd;
-    p.stat = a.stat + own * 2;
-    a.pre_part = p.part; a.pre_stat = p.stat;
-    rc = launch_prompt_sums(p, hd, act_dtype, s);
-    if (rc) return rc;
-  } else {
-    a.stat = pre;
-  }
-  CacheMaps m;
-  if (a.c.width == 0 || a.c.pages == 0) {  // no keys but the prefix's: the maps are not used
-    a.c.width = 0;
-    m = CacheMaps{};
-  } else {
+  int* status = gemm_status_ptr();
+  if (!status) return EE_ERR_DEVICE;
+  if (cache->pages == 0) a.c.width = 0;  // no keys but the prefix's: the maps are not used
+  CacheMaps m{};
+  if (a.c.width > 0) {
     const int rb = hd * cache->bits / 8;
     const uint64_t rows = (uint64_t)cache->pages * n_kv * cache->page_size;
-    const auto sw = rb == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : rb == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
-    if (!make_tmap_2d(&m.k, cache->k_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, rb, rows, rb, rb, kCaKeys, sw) ||
-        !make_tmap_2d(&m.v, cache->v_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, rb, rows, rb, rb, kCaKeys, sw))
+    const auto sw = plan.nt == 0 ? CU_TENSOR_MAP_SWIZZLE_NONE
+                    : rb == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                    : rb == 64   ? CU_TENSOR_MAP_SWIZZLE_64B
+                                 : CU_TENSOR_MAP_SWIZZLE_32B;
+    const int box = plan.nt ? kCaKeys : cache->page_size < 128 ? cache->page_size : 128;
+    if (!make_tmap_2d(&m.k, cache->k_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, rb, rows, rb, rb, box, sw) ||
+        !make_tmap_2d(&m.v, cache->v_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, rb, rows, rb, rb, box, sw))
       return EE_ERR_SHAPE;
   }
+  float* part = reinterpret_cast<float*>(workspace);
+  float* stat = part + (cp.own + cp.pre) * hd;
+  // of the prefix: behind the parts of the call's own keys in the kernel for few rows, before them in the other
+  const long long pre_at = plan.nt ? cp.own : 0;
+  PromptArgs p{};
+  p.q = q;
+  p.q_tok = q_tok; p.q_head = q_head;
+  p.tq = (int)tq;
+  p.n_q = n_q; p.n_kv = n_kv; p.group = n_q / n_kv;
+  p.scale_log2 = scale_log2;
+  if (prefix_len) {
+    PromptArgs x = p;
+    x.k = prefix_k; x.v = prefix_v;
+    x.k_tok = pk_tok; x.k_head = pk_head; x.v_tok = pv_tok; x.v_head = pv_head;
+    x.tk = (int)prefix_len;
+    x.n_seq = 1;
+    x.splits = cp.pre_splits;
+    x.sums = 1;
+    x.part = part + pre_at * hd;
+    x.stat = stat + pre_at * 2;
+    rc = launch_prompt_sums(x, hd, act_dtype, s);
+    if (rc) return rc;
+  }
+  if (plan.nt) {
+    a.q = q; a.out = out;
+    a.cu_q = cu_q;
+    a.q_tok = q_tok; a.q_head = q_head; a.o_tok = o_tok; a.o_head = o_head;
+    a.tq = (int)tq; a.n_q = n_q; a.group = n_q / n_kv;
+    a.causal = causal != 0;
+    a.rows = 8 * plan.nt;
+    a.scale_log2 = scale_log2;
+    a.k_steps = cache->k_steps; a.v_steps = cache->v_steps;
+    a.part = part; a.stat = stat;
+    a.pre_splits = cp.pre_splits;
+    a.status = status;
+    a.timeout_ns = kCacheWaitNs;
+    if (act_dtype == EE_BF16)
+      return hd == 64 ? launch_cache_few<__nv_bfloat16, 64>(m, a, plan, cache->bits, s)
+                      : launch_cache_few<__nv_bfloat16, 128>(m, a, plan, cache->bits, s);
+    return hd == 64 ? launch_cache_few<__half, 64>(m, a, plan, cache->bits, s)
+                    : launch_cache_few<__half, 128>(m, a, plan, cache->bits, s);
+  }
+  PromptTcArgs t{};
+  p.out = out;
+  p.o_tok = o_tok; p.o_head = o_head;
+  p.cu_q = cu_q;
+  p.k_lens = k_lens;
+  p.tk = a.c.width << a.c.shift;
+  p.n_seq = n_seq;
+  p.causal = causal != 0;
+  p.splits = plan.splits;
+  p.sums = prefix_len > 0;
+  p.part = part + cp.pre * hd;
+  p.stat = stat + cp.pre * 2;
+  t.p = p;
+  t.tpt = 128 / p.group;
+  t.status = status;
+  t.timeout_ns = kCacheWaitNs;
+  t.c = a.c;
+  t.k_steps = cache->k_steps; t.v_steps = cache->v_steps;
   if (act_dtype == EE_BF16)
-    return hd == 64 ? launch_cache_attn<__nv_bfloat16, 64>(m, a, plan, cache->bits, s)
-                    : launch_cache_attn<__nv_bfloat16, 128>(m, a, plan, cache->bits, s);
-  return hd == 64 ? launch_cache_attn<__half, 64>(m, a, plan, cache->bits, s)
-                  : launch_cache_attn<__half, 128>(m, a, plan, cache->bits, s);
+    rc = hd == 64 ? launch_cache_many<__nv_bfloat16, 64>(m, t, cache->bits, s)
+                  : launch_cache_many<__nv_bfloat16, 128>(m, t, cache->bits, s);
+  else
+    rc = hd == 64 ? launch_cache_many<__half, 64>(m, t, cache->bits, s) : launch_cache_many<__half, 128>(m, t, cache->bits, s);
+  if (rc || (!prefix_len && plan.splits == 1)) return rc;
+  p.splits = cp.pre_splits + plan.splits;
+  p.part = part;
+  p.stat = stat;
+  return launch_prompt_combine(p, hd, act_dtype, s);
 }
 
 }  // extern "C"

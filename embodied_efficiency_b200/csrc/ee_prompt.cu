@@ -381,18 +381,14 @@ __global__ void __launch_bounds__(kPrJoin) prompt_join_kernel(const __grid_const
 //           parts of 512 keys or more, joined by a second launch
 constexpr long long kPrRows = 16, kPtMinKeys = 512;
 struct PromptPlan { bool tc; int splits; };
+int prompt_parts(long long tq, int n_seq, int n_q, int n_kv, long long keys);
 static PromptPlan prompt_plan(long long tq, long long tk, int n_seq, int n_q, int n_kv) {
   PromptPlan pl{false, 1};
   if (n_seq < 1) return pl;
   const int group = n_q / n_kv;
   const long long rows = tq * group;
   pl.tc = rows > kPrRows * n_seq && tk > 0 && group <= 128;
-  if (!pl.tc) return pl;
-  const long long per = 2 * (128 / group) * group;  // rows of an item: two tiles of whole tokens
-  const long long items = (rows / per > n_seq ? rows / per : n_seq) * n_kv;
-  const long long want = device_sms() / items, most = tk / n_seq / kPtMinKeys;
-  const long long s = want < most ? want : most;
-  pl.splits = s < 1 ? 1 : (int)s;
+  if (pl.tc) pl.splits = prompt_parts(tq, n_seq, n_q, n_kv, tk / n_seq);
   return pl;
 }
 static long long prompt_partials(const PromptPlan& pl, long long tq, int n_q, int hd) {  // partial rows
@@ -404,11 +400,14 @@ static size_t prompt_ws_bytes(const PromptPlan& pl, long long tq, int n_q, int h
 }
 
 template <typename T, int HD>
-static int launch_combine(const PromptArgs& a, cudaStream_t s) {
-  if (a.splits == 1 || a.sums) return EE_OK;
+static int launch_parts(const PromptArgs& a, cudaStream_t s) {
   return launch_pdl(prompt_combine_kernel<T, HD>, dim3((unsigned)a.tq, a.n_q), dim3(kPrJoin), 0, s, a) == cudaSuccess
              ? EE_OK
              : EE_ERR_LAUNCH;
+}
+template <typename T, int HD>
+static int launch_combine(const PromptArgs& a, cudaStream_t s) {
+  return a.splits == 1 || a.sums ? EE_OK : launch_parts<T, HD>(a, s);
 }
 
 template <typename T, int HD>
@@ -432,8 +431,8 @@ static int launch_rows(const PromptArgs& a, cudaStream_t s) {
 int* gemm_status_ptr();  // ee_ops.cu: the status word of the tensor-core kernels on the current device
 
 // [tokens][heads][hd] by strides, read in boxes of 64 columns of bh heads and bt tokens
-static bool make_head_map(CUtensorMap* map, const void* base, int hd, int heads, long long tokens, long long head,
-                          long long tok, int bh, int bt) {
+bool prompt_head_map(CUtensorMap* map, const void* base, int hd, int heads, long long tokens, long long head, long long tok,
+                     int bh, int bt) {
   auto enc = tmap_encoder();
   if (!enc) return false;
   if (heads == 1) head = hd;   // strides of dimensions of one entry mean nothing
@@ -463,15 +462,15 @@ static int launch_tc(const PromptArgs& p, cudaStream_t s) {
   a.timeout_ns = g_wait_limit.load(std::memory_order_relaxed);
   if (!a.status) return EE_ERR_DEVICE;
   CUtensorMap mq, mk, mv;
-  if (!make_head_map(&mq, p.q, HD, p.n_q, p.tq, p.q_head, p.q_tok, p.group, a.tpt) ||
-      !make_head_map(&mk, p.k, HD, p.n_kv, p.tk, p.k_head, p.k_tok, 1, 128) ||
-      !make_head_map(&mv, p.v, HD, p.n_kv, p.tk, p.v_head, p.v_tok, 1, 128))
+  if (!prompt_head_map(&mq, p.q, HD, p.n_q, p.tq, p.q_head, p.q_tok, p.group, a.tpt) ||
+      !prompt_head_map(&mk, p.k, HD, p.n_kv, p.tk, p.k_head, p.k_tok, 1, 128) ||
+      !prompt_head_map(&mv, p.v, HD, p.n_kv, p.tk, p.v_head, p.v_tok, 1, 128))
     return EE_ERR_SHAPE;  // a stride the loads cannot address
   // at most one partial unit per sequence beyond the rows' whole units
   const long long items = ((long long)p.tq / (2 * a.tpt) + p.n_seq) * p.n_kv * p.splits;
   if (items > 0x7fffffff) return EE_ERR_SHAPE;
   const unsigned grid = (unsigned)(items < dp->sms ? items : dp->sms);
-  if (launch_pdl(fn, dim3(grid), dim3(kPtThreads), pt_smem<HD>(), s, mq, mk, mv, a) != cudaSuccess) return EE_ERR_LAUNCH;
+  if (launch_pdl(fn, dim3(grid), dim3(kPtThreads), pt_smem<HD, 0>(), s, mq, mk, mv, a) != cudaSuccess) return EE_ERR_LAUNCH;
   return launch_combine<T, HD>(p, s);
 }
 
@@ -489,6 +488,22 @@ int prompt_sums_splits(long long tq, long long tk, int n_q, int n_kv) {
   const long long items = (tq + 2 * tpt - 1) / (2 * tpt) * n_kv, want = device_sms() / items, most = tk / kPtMinKeys;
   const long long s = want < most ? want : most;
   return s < 1 ? 1 : (int)s;
+}
+// Parts of the keys for items that would leave SMs idle, at most one per 512 of
+// `keys` a sequence.
+int prompt_parts(long long tq, int n_seq, int n_q, int n_kv, long long keys) {
+  const int group = n_q / n_kv;
+  const long long rows = tq * group, per = 2 * (128 / group) * group;  // of an item: two tiles of whole tokens
+  const long long items = (rows / per > n_seq ? rows / per : n_seq) * n_kv;
+  const long long want = device_sms() / items, most = keys / kPtMinKeys;
+  const long long s = want < most ? want : most;
+  return s < 1 ? 1 : (int)s;
+}
+// Joins a.splits parts of every row of a sequence.
+int launch_prompt_combine(const PromptArgs& a, int hd, int act_dtype, cudaStream_t s) {
+  if (act_dtype == EE_BF16)
+    return hd == 64 ? launch_parts<__nv_bfloat16, 64>(a, s) : launch_parts<__nv_bfloat16, 128>(a, s);
+  return hd == 64 ? launch_parts<__half, 64>(a, s) : launch_parts<__half, 128>(a, s);
 }
 int launch_prompt_sums(const PromptArgs& a, int hd, int act_dtype, cudaStream_t s) {
   if (act_dtype == EE_BF16) return hd == 64 ? launch_tc<__nv_bfloat16, 64>(a, s) : launch_tc<__nv_bfloat16, 128>(a, s);

@@ -51,11 +51,16 @@ EE_DEV PromptSeq prompt_seq(const PromptArgs& a, int b) {
   if (!a.cu_q) return PromptSeq{0, a.tq, 0, a.tk, 0};  // one sequence of all rows
   s.q0 = min(max(__ldg(a.cu_q + b), 0), a.tq);
   s.qlen = min(max(__ldg(a.cu_q + b + 1), s.q0), a.tq) - s.q0;
+  s.blk = 0;
+  if (!a.cu_k) {  // a cache: the sequence is found by its table, at most tk keys
+    s.k0 = b;
+    s.klen = min(max(__ldg(a.k_lens + b), 0), a.tk);
+    return s;
+  }
   s.k0 = min(max(__ldg(a.cu_k + b), 0), a.tk);
   int end = __ldg(a.cu_k + b + 1);
   if (a.k_lens) end = min(end, s.k0 + min(max(__ldg(a.k_lens + b), 0), a.tk - s.k0));
   s.klen = min(max(end, s.k0), a.tk) - s.k0;
-  s.blk = 0;
   return s;
 }
 

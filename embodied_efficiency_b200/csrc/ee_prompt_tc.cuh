@@ -54,6 +54,7 @@
 // load lands and every MMA completes before the CTA returns its memory.
 #pragma once
 
+#include "ee_cache.cuh"
 #include "ee_prompt.cuh"
 #include "ee_tma.cuh"
 #include "ee_umma.cuh"
@@ -65,6 +66,8 @@ struct PromptTcArgs {
   int tpt;  // tokens per tile: 128 / group
   int* status;
   unsigned long long timeout_ns;
+  CacheView c;  // keys and values in a cache
+  const float *k_steps, *v_steps;
 };
 
 constexpr int kPtThreads = 384;
@@ -75,15 +78,31 @@ constexpr int kPtRegsLaunch = 168, kPtRegsSoft = 208, kPtRegsRest = 88;
 static_assert(256 * kPtRegsSoft + 128 * kPtRegsRest <= kPtThreads * kPtRegsLaunch, "the register shares fit the launch");
 constexpr int kPtKeys = 128, kPtInfo = 4, kPtLoads = 8;  // keys per block; items published, loads of K / V ahead
 constexpr unsigned long long kPtDrainNs = 1000000000ull;  // for loads and MMAs already issued, whatever timeout_ns is
-template <int HD> constexpr int pt_slots() { return HD == 128 ? 4 : 8; }
+// Shared memory: Q of both tiles, the slots of K / V, output staging of every
+// softmax warp, barriers, published items; for a cache also the ring of codes
+// as they come, and the steps of the blocks.
+template <int HD, int BITS> constexpr int pt_slots() { return BITS ? (HD == 128 ? 3 : 6) : (HD == 128 ? 4 : 8); }
 template <int HD> constexpr uint32_t pt_tile() { return 128u * HD * 2; }
-template <int HD> constexpr uint32_t pt_off_out() { return (2 + pt_slots<HD>()) * pt_tile<HD>(); }  // 4 KB per softmax warp
-template <int HD> constexpr uint32_t pt_off_bar() { return pt_off_out<HD>() + 8 * 4096; }
+template <int BITS> constexpr uint32_t pt_stage() { return BITS ? 2048u : 4096u; }  // bytes of a warp's output staging
+template <int HD, int BITS> constexpr uint32_t pt_raw() { return 128u * HD * BITS / 8; }  // codes of a tile
+template <int HD, int BITS> constexpr int pt_raws() { return BITS ? (int)(32768u / (128u * HD * (BITS ? BITS : 8) / 8)) : 0; }
+constexpr int kPtSteps = 4;  // blocks whose steps are held
+template <int HD, int BITS> constexpr uint32_t pt_off_raw() { return (2 + pt_slots<HD, BITS>()) * pt_tile<HD>(); }
+template <int HD, int BITS> constexpr uint32_t pt_off_out() { return pt_off_raw<HD, BITS>() + (BITS ? 32768u : 0u); }
+template <int HD, int BITS> constexpr uint32_t pt_off_rawsteps() { return pt_off_out<HD, BITS>() + 8 * pt_stage<BITS>(); }
+template <int HD, int BITS> constexpr uint32_t pt_off_steps() { return pt_off_rawsteps<HD, BITS>() + pt_raws<HD, BITS>() * 1024u; }
+template <int HD, int BITS> constexpr uint32_t pt_off_bar() { return pt_off_steps<HD, BITS>() + (BITS ? kPtSteps * 1024u : 0u); }
 // barriers: full / empty per load of K / V, Q full / empty, S / P (two halves) / S free / O / O free per tile, V to fix /
-// fixed, item full / empty, MMAs done after a failure
-template <int HD> constexpr uint32_t pt_off_info() { return pt_off_bar<HD>() + 8 * (2 * kPtLoads + 17 + 2 * kPtInfo) + 8; }
-template <int HD> constexpr uint32_t pt_off_beat() { return pt_off_info<HD>() + kPtInfo * 64; }  // blocks the MMA warp has come to
-template <int HD> constexpr uint32_t pt_smem() { return pt_off_beat<HD>() + 16 + 1024; }
+// fixed, item full / empty, MMAs done after a failure, codes full / empty
+template <int HD, int BITS> constexpr uint32_t pt_off_info() {
+  return pt_off_bar<HD, BITS>() + 8 * (2 * kPtLoads + 17 + 2 * kPtInfo + 2 * pt_raws<HD, BITS>()) + 8;
+}
+template <int HD, int BITS> constexpr uint32_t pt_off_beat() { return pt_off_info<HD, BITS>() + kPtInfo * 64; }  // blocks the MMA warp has come to
+// which keys of a block are there (4 words a block), which pieces of a tile of codes
+template <int HD, int BITS> constexpr uint32_t pt_off_there() { return pt_off_beat<HD, BITS>() + 16; }
+template <int HD, int BITS> constexpr uint32_t pt_smem() {
+  return pt_off_there<HD, BITS>() + (BITS ? kPtSteps * 16 + pt_raws<HD, BITS>() * 4 : 0) + 1024;
+}
 
 // One published item (16 words)
 struct PromptItem {
@@ -186,11 +205,35 @@ EE_DEV float max3(float a, float b, float c) {
   return r;
 }
 
-template <typename T, int HD>
+// Two signed 4-bit codes of a word, byte `p`, or two 8-bit ones of bytes 2p and
+// 2p + 1, as 16-bit values: exact, for 8 bits in bf16 a 64th of it (bf16's
+// numbers below 2^-126 take a byte as it is, times 2^-133; one multiplication by
+// 2^127 and the sum take it to where it belongs, where an exponent OR-ed above
+// it has seven bits only and takes three instructions).
+template <typename T> EE_DEV uint32_t code_pair8(uint32_t flipped, int p);  // of a word with its sign bits flipped
+template <> EE_DEV uint32_t code_pair8<__half>(uint32_t w, int p) {
+  return fma2<__half>(prmt(w, 0x64u, p ? 0x4342u : 0x4140u), 0x3C003C00u, 0xE480E480u);
+}
+template <> EE_DEV uint32_t code_pair8<__nv_bfloat16>(uint32_t w, int p) {
+  return fma2<__nv_bfloat16>(prmt(w, 0u, p ? 0x4342u : 0x4140u), 0x7F007F00u, 0xC000C000u);
+}
+template <typename T> EE_DEV uint32_t code_pair4(uint32_t w, uint32_t w_shr4, int p) {
+  return fma2<T>(nib_pair<T>(w, w_shr4, p, 0x00080008u), Act<T>::kOne2, std::is_same<T, __half>::value ? 0xE408E408u : 0xC308C308u);
+}
+// what code_pair8 leaves out
+template <typename T, int BITS> EE_DEV constexpr float code_unit() { return BITS == 8 && !std::is_same<T, __half>::value ? 64.f : 1.f; }
+
+// BITS 0: K and V of 16 bits. 8 or 4: codes from a paged cache. TMA brings them
+// into a ring, 128 keys at a time; warps 10 and 11 turn them into 16-bit tiles in
+// the slots, exactly, and hand on the steps: a key's step multiplies its column
+// of S, a value's step its column of P after the sum is taken (so the weights
+// that P V rounds to bf16 are the products). fp16 has no room for weights times
+// steps: there the values are multiplied and rounded once more, to fp16.
+template <typename T, int HD, int BITS = 0>
 __global__ void __launch_bounds__(kPtThreads, 1)
     prompt_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                      const __grid_constant__ CUtensorMap mv, const __grid_constant__ PromptTcArgs a) {
-  constexpr int NS = pt_slots<HD>(), NP = kPtLoads;
+  constexpr int NS = pt_slots<HD, BITS>(), NP = kPtLoads, NR = pt_raws<HD, BITS>();
   static_assert(NS <= NP, "a barrier per load that the slots can hold");
   constexpr uint32_t TILE = pt_tile<HD>(), PANEL = 128 * 128;  // a panel: 64 columns of 128 rows
   constexpr int PANELS = HD / 64;
@@ -198,26 +241,31 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   constexpr bool SEP = HD == 64;
   // pieces in which a block's weights are handed over (in one piece, hd 64: 501 instead of 411 us for 8192 tokens)
   constexpr int PARTS = 2;
+  constexpr bool VSCALE = BITS && !std::is_same<T, __half>::value;  // P takes the values' steps
   extern __shared__ __align__(1024) char smem_raw[];
   const uint32_t base0 = smem_u32(smem_raw);
   const uint32_t sb = (base0 + 1023u) & ~1023u;
   char* smem = smem_raw + (sb - base0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t sQ = sb, sKV = sb + 2 * TILE;
-  const uint32_t b_full = sb + pt_off_bar<HD>(), b_empty = b_full + 8 * NP;
+  const uint32_t b_full = sb + pt_off_bar<HD, BITS>(), b_empty = b_full + 8 * NP;
   const uint32_t b_qf = b_empty + 8 * NP, b_qe = b_qf + 8, b_s = b_qe + 8, b_p = b_s + 16, b_sf = b_p + 32, b_o = b_sf + 16;
   const uint32_t b_of = b_o + 16, b_req = b_of + 16, b_fix = b_req + 8, b_if = b_fix + 8, b_ie = b_if + 8 * kPtInfo;
-  const uint32_t b_end = b_ie + 8 * kPtInfo, off_tm = b_end + 8 - sb;
-  volatile PromptItem* ring = reinterpret_cast<volatile PromptItem*>(smem + pt_off_info<HD>());
-  volatile uint32_t* beat = reinterpret_cast<volatile uint32_t*>(smem + pt_off_beat<HD>());
+  const uint32_t b_end = b_ie + 8 * kPtInfo, b_rf = b_end + 8, b_re = b_rf + 8 * NR, off_tm = b_re + 8 * NR - sb;
+  volatile PromptItem* ring = reinterpret_cast<volatile PromptItem*>(smem + pt_off_info<HD, BITS>());
+  volatile uint32_t* beat = reinterpret_cast<volatile uint32_t*>(smem + pt_off_beat<HD, BITS>());
   const PromptArgs& p = a.p;
   if (warp == 8 && lane == 0) {
     tma_prefetch_map(&mq);
     tma_prefetch_map(&mk);
     tma_prefetch_map(&mv);
     for (int s = 0; s < NP; ++s) {
-      mbar_init(b_full + 8 * s, 1);
+      mbar_init(b_full + 8 * s, BITS ? 2 : 1);
       mbar_init(b_empty + 8 * s, 1);
+    }
+    for (int s = 0; s < NR; ++s) {
+      mbar_init(b_rf + 8 * s, 1);
+      mbar_init(b_re + 8 * s, 2);
     }
     mbar_init(b_req, 1);
     mbar_init(b_fix, 1);
@@ -235,7 +283,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     }
     for (int i = 0; i < kPtInfo; ++i) {
       mbar_init(b_if + 8 * i, 1);
-      mbar_init(b_ie + 8 * i, 10);  // 8 softmax warps, the MMA warp, the fixing warp
+      mbar_init(b_ie + 8 * i, BITS ? 11 : 10);  // 8 softmax warps, the MMA warp, the fixing or decoding warps
     }
     mbar_fence_init();
   }
@@ -317,7 +365,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             mbar_arrive(b_full + 8 * (g % NP));
             ++g;
           };
-          if (more && it.nbm > 0) {
+          if (BITS == 0 && more && it.nbm > 0) {
             load_kv(0);
             loaded();
             // Q: its buffers are free when the last scores of the previous item are done
@@ -339,10 +387,74 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         }
         ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
         if (!more || !ok) break;
+        if constexpr (BITS > 0) {
+          // the tiles' codes, K(0) V(0) K(1) ..., in pieces of a page; a block's steps come with its K. A lane per piece
+          // looks its page up, a block ahead.
+          const int shift = min(a.c.shift, 7), pieces = kPtKeys >> shift;
+          constexpr uint32_t RB = HD * BITS / 8;
+          auto rows_of = [&](int j) {  // this lane's piece of block j: its first row in the cache, -1 for none
+            const int key = it.key0 + j * kPtKeys + (lane << shift);
+            if (lane >= pieces || j >= it.nbm || key >= it.klen) return -1;
+            const int page = __ldg(a.c.table + (long long)it.k0 * a.c.table_row + (key >> a.c.shift));
+            if ((unsigned)page >= (unsigned)a.c.pages) return -1;
+            return ((page * a.c.n_kv + it.kvh) << a.c.shift) + (key & ((1 << a.c.shift) - 1));
+          };
+          int row = rows_of(0);
+          for (int j = 0; j < it.nbm && ok; ++j) {
+            const int next = rows_of(j + 1);
+            const uint32_t there = __ballot_sync(0xffffffffu, row >= 0);
+            for (int w = 0; w < 2 && ok; ++w) {
+              if (w == 1 && j == 0) {
+                // Q: its buffers are free when the last scores of the previous item are done
+                if (lane == 0 && nq > 0) ok = mbar_wait(b_qe, (uint32_t)((nq - 1) & 1), a.timeout_ns);
+                ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+                if (!ok) break;
+                if (lane == 0) {
+                  mbar_arrive_expect_tx(b_qf, (it.n[0] > 0 ? qbytes : 0) + (it.n[1] > 0 ? qbytes : 0));
+                  for (int t = 0; t < 2; ++t)
+                    if (it.n[t] > 0)
+                      for (int c = 0; c < PANELS; ++c)
+                        tma_load_3d(sQ + t * TILE + c * PANEL, &mq, 64 * c, it.kvh * p.group, it.q0 + it.tok + t * a.tpt, b_qf);
+                }
+                ++nq;
+              }
+              const uint32_t slot = g % NR;
+              if (lane == 0 && g >= (uint32_t)NR) ok = mbar_wait(b_re + 8 * slot, (g / NR - 1) & 1, a.timeout_ns);
+              ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+              if (!ok) break;
+              const uint32_t bar = b_rf + 8 * slot, dst = sb + pt_off_raw<HD, BITS>() + slot * pt_raw<HD, BITS>();
+              const uint32_t steps = sb + pt_off_rawsteps<HD, BITS>() + slot * 1024;
+              if (lane == 0) {
+                *reinterpret_cast<volatile uint32_t*>(smem + pt_off_there<HD, BITS>() + kPtSteps * 16 + slot * 4) = there;
+                mbar_arrive_expect_tx(bar, __popc(there) * ((RB << shift) + (w == 0 ? 8u << shift : 0u)));
+              }
+              __syncwarp();
+              if (row >= 0) {
+                tma_load_2d(dst + lane * (RB << shift), w ? &mv : &mk, 0, row, bar);
+                if (w == 0) {
+                  bulk_load(steps + lane * (4 << shift), a.k_steps + row, 4 << shift, bar);
+                  bulk_load(steps + 512 + lane * (4 << shift), a.v_steps + row, 4 << shift, bar);
+                }
+              }
+              __syncwarp();
+              ++g;
+            }
+            row = next;
+          }
+          if (!ok) break;
+        }
       }
       // everything issued lands before the CTA may exit, whatever has failed; if nothing has, it is used too, and the
       // MMA warp's arrivals that say so have come
-      if (lane == 0) {
+      if (BITS && lane == 0) {
+        bool landed = true;
+        for (uint32_t e = g > (uint32_t)NR ? g - NR : 0; e < g; ++e) landed &= mbar_wait(b_rf + 8 * (e % NR), (e / NR) & 1, kPtDrainNs);
+        if (nq > 0) landed &= mbar_wait(b_qf, (uint32_t)((nq - 1) & 1), kPtDrainNs);
+        ok = ok && landed;
+        if (ok && nq > 0) ok = mbar_wait(b_qe, (uint32_t)((nq - 1) & 1), a.timeout_ns);
+        if (!ok) atomicCAS(a.status, 0, (int)EE_ERR_TIMEOUT);
+      }
+      if (BITS == 0 && lane == 0) {
         const uint32_t e0 = g > NP ? g - NP : 0;
         bool landed = true;
         for (uint32_t e = e0; e < g; ++e) landed &= mbar_wait(b_full + 8 * (e % NP), (e / NP) & 1, kPtDrainNs);
@@ -403,7 +515,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           ok = wait(b_full + 8 * (g % NP), (g / NP) & 1);
           if (!ok) break;
           if (lane == 0) *beat = g;
-          bool fix = j + 1 == nbm && tail < kPtKeys;
+          bool fix = BITS == 0 && j + 1 == nbm && tail < kPtKeys;
           if (fix && lane == 0) mbar_arrive(b_req);
           __syncwarp();
           const uint64_t vd = v_desc + (uint64_t)(vs * (TILE >> 4));
@@ -460,6 +572,111 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         mbar_wait(b_end, 0, kPtDrainNs);
         __syncwarp();
       }
+    } else if (BITS > 0) {
+      // ---------------- codes into 16-bit tiles, 64 keys of each by either warp ----------------
+      if constexpr (BITS > 0) {
+      constexpr int RB = HD * BITS / 8, CPR = RB / 16;  // 16-byte pieces of a row
+      const int half = warp - 10;
+      uint32_t g = 0, rt = 0, blk = 0, slot_load[NS];  // loads of K / V, tiles of codes and blocks so far, each slot's last load
+      int n = 0, sl = 0;                               // K / V tiles so far, next slot
+      bool ok = true;
+      for (int i = 0;; ++i) {
+        ok = __all_sync(0xffffffffu, item_wait(i));
+        if (!ok) break;
+        const volatile PromptItem* r = ring + i % kPtInfo;
+        const int nbm = r->nbm, klen = r->klen, key0 = r->key0;
+        __syncwarp();
+        if (lane == 0) item_done(i);
+        if (nbm < 0) break;
+        for (int w = 0; w < 2 * nbm && ok; ++w) {
+          const uint32_t rs = rt % NR;
+          ok = mbar_wait(b_rf + 8 * rs, (rt / NR) & 1, a.timeout_ns);
+          if (ok && n >= NS) {
+            const uint32_t was = slot_load[sl];  // the load that used the slot before has been consumed
+            ok = mbar_wait(b_empty + 8 * (was % NP), (was / NP) & 1, a.timeout_ns);
+          }
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          slot_load[sl] = g;
+          const uint32_t raw = sb + pt_off_raw<HD, BITS>() + rs * pt_raw<HD, BITS>(), dst = sKV + sl * TILE;
+          const float* raw_steps = reinterpret_cast<const float*>(smem + pt_off_rawsteps<HD, BITS>() + rs * 1024);
+          float* steps = reinterpret_cast<float*>(smem + pt_off_steps<HD, BITS>() + (blk % kPtSteps) * 1024);
+          if ((w & 1) == 0) {
+            const uint32_t there = *reinterpret_cast<volatile uint32_t*>(smem + pt_off_there<HD, BITS>() + kPtSteps * 16 + rs * 4);
+            const int shift = min(a.c.shift, 7);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int key = 64 * half + 32 * h + lane;
+              const bool have = key0 + (w >> 1) * kPtKeys + key < klen && (there >> (key >> shift) & 1);
+              float ks = have ? raw_steps[key] : 0.f, vs = have ? raw_steps[128 + key] : 0.f;
+              // a value's step that is no number must reach the rows that see it and no others: as its key's
+              if (!(fabsf(vs) <= 3.4028234e38f)) {
+                ks = __int_as_float(0x7fffffff);
+                vs = 0.f;
+              }
+              steps[key] = ks * (p.scale_log2 * code_unit<T, BITS>());
+              steps[128 + key] = vs * code_unit<T, BITS>();
+              const uint32_t all = __ballot_sync(0xffffffffu, have);
+              if (lane == 0)
+                *reinterpret_cast<volatile uint32_t*>(smem + pt_off_there<HD, BITS>() + (blk % kPtSteps) * 16 + (2 * half + h) * 4) = all;
+            }
+            __syncwarp();
+          }
+          const bool isv = w & 1;
+#pragma unroll 2
+          for (int e = lane; e < 64 * CPR; e += 32) {
+            const int row = 64 * half + e / CPR, q = e % CPR;
+            const uint4 x = lds16(raw + row * RB + q * 16);
+            const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
+            uint32_t o[64 / BITS];  // pairs
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if (BITS == 8) {
+                const uint32_t f = xw[k] ^ 0x80808080u;
+                o[2 * k] = code_pair8<T>(f, 0);
+                o[2 * k + 1] = code_pair8<T>(f, 1);
+              } else {
+#pragma unroll
+                for (int b = 0; b < 4; ++b) o[4 * k + b] = code_pair4<T>(xw[k], xw[k] >> 4, b);
+              }
+            }
+            if (!VSCALE && isv) {
+              const float s = steps[128 + row];
+#pragma unroll
+              for (int k = 0; k < 64 / BITS; ++k) {
+                const float2 f = Act<T>::unpack2(o[k]);
+                o[k] = Act<T>::pack2(f.x * s, f.y * s);
+              }
+            }
+#pragma unroll
+            for (int k = 0; k < 16 / BITS; ++k) {
+              const int c = q * (16 / BITS) + k;  // 16-byte piece of the 16-bit row
+              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (c >> 3) * PANEL + sw128(row, c & 7)),
+                           "r"(o[4 * k]), "r"(o[4 * k + 1]), "r"(o[4 * k + 2]), "r"(o[4 * k + 3])
+                           : "memory");
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(b_re + 8 * rs);
+          ++rt;
+          ++n;
+          if (++sl == NS) sl = 0;
+          if (isv) ++blk;
+          if (w == 0 || (isv ? w + 1 == 2 * nbm : true)) {  // K(0) alone; V(j) with K(j + 1); the last V alone
+            if (lane == 0) mbar_arrive(b_full + 8 * (g % NP));
+            ++g;
+          }
+        }
+        if (!ok) break;
+      }
+      // the MMA warp's arrivals that say the tiles are used have come
+      if (half == 0 && lane == 0) {
+        for (uint32_t e = g > (uint32_t)NP ? g - NP : 0; e < g && ok; ++e) ok = mbar_wait(b_empty + 8 * (e % NP), (e / NP) & 1, a.timeout_ns);
+      }
+      if (!ok && lane == 0) atomicCAS(a.status, 0, (int)EE_ERR_TIMEOUT);
+      __syncwarp();
+      }
     } else if (warp == 10) {
       // ---------------- V rows past the sequence's end ----------------
       int n = 0, nfix = 0;
@@ -499,13 +716,14 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     const uint32_t ts = tmem + 128 * t + ((uint32_t)(32 * q4) << 16), to = tmem + 256 + OC * t + ((uint32_t)(32 * q4) << 16);
     const uint32_t tp = SEP ? tmem + 384 + 64 * t + ((uint32_t)(32 * q4) << 16) : ts;
     int ns = 0, no = 0;  // score blocks and commits of O (per block when SEP, else per item) so far
+    uint32_t gs = 0, bs = 0;  // loads of K / V and blocks of the items before (cache)
     bool ok = true;
     for (int i = 0; ok; ++i) {
       ok = __all_sync(0xffffffffu, item_wait(i));
       if (!ok) break;
       const volatile PromptItem* it = ring + i % kPtInfo;
       if (it->nbm < 0) break;
-      const int nt = it->n[t], qlen = it->qlen, klen = it->klen, key0 = it->key0;
+      const int nt = it->n[t], qlen = it->qlen, klen = it->klen, key0 = it->key0, nbm = it->nbm;
       const int tok = it->tok + t * a.tpt + rtok, head = it->kvh * p.group + rhead;
       const int out_row = it->q0 + tok;
       const int part = it->part;
@@ -529,12 +747,36 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           if (lane == 0) mbar_arrive(b_sf + 8 * t);
         }
         const int left = lim - j * kPtKeys;
-        if (__any_sync(0xffffffffu, left < kPtKeys)) {
+        const float4* steps = reinterpret_cast<const float4*>(smem + pt_off_steps<HD, BITS>() + ((bs + j) % kPtSteps) * 1024);
+        uint32_t there[4];
+        bool gaps = false;
+        if constexpr (BITS > 0) {
+          // K(j) is in its slot, or S would not be there; this wait makes the block's steps visible here
+          const uint32_t gk = gs + j;
+          ok = __all_sync(0xffffffffu, mbar_wait(b_full + 8 * (gk % NP), (gk / NP) & 1, a.timeout_ns));
+          if (!ok) break;
+          const volatile uint32_t* tw =
+              reinterpret_cast<volatile uint32_t*>(smem + pt_off_there<HD, BITS>() + ((bs + j) % kPtSteps) * 16);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) there[c] = tw[c];
+          gaps = (there[0] & there[1] & there[2] & there[3]) != 0xffffffffu;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              const float4 k = steps[8 * c + e / 4];
+              unpack64(mul2f(pack64(v[c][e], v[c][e + 1]), pack64(__float_as_uint(k.x), __float_as_uint(k.y))), v[c][e], v[c][e + 1]);
+              unpack64(mul2f(pack64(v[c][e + 2], v[c][e + 3]), pack64(__float_as_uint(k.z), __float_as_uint(k.w))), v[c][e + 2],
+                       v[c][e + 3]);
+            }
+        }
+        if (gaps || __any_sync(0xffffffffu, left < kPtKeys)) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const int n = left - 32 * c;
-            if (__any_sync(0xffffffffu, n < 32)) {  // a bit per key: one predicated move a value instead of a comparison too
-              const uint32_t seen = n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u);
+            if (gaps || __any_sync(0xffffffffu, n < 32)) {  // a bit per key: one predicated move a value instead of a comparison too
+              uint32_t seen = n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u);
+              if (BITS) seen &= there[c];
 #pragma unroll
               for (int e = 0; e < 32; ++e)
                 if (!(seen >> e & 1u)) v[c][e] = 0xff800000u;
@@ -548,7 +790,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
 #pragma unroll
           for (int e = 2; e < 32; e += 2) x[c] = max3(x[c], __uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1]));
         }
-        const float mx = fmaxf(max3(x[0], x[1], x[2]), x[3]) * p.scale_log2;
+        const float mx = fmaxf(max3(x[0], x[1], x[2]), x[3]) * (BITS ? 1.f : p.scale_log2);  // a cache's steps have it in them
         float f = 1.f;
         if (mx > top) {  // also from -inf, with f = 0: nothing to rescale yet
           const float to = prompt_reference<T, 7>(mx);
@@ -584,9 +826,15 @@ __global__ void __launch_bounds__(kPtThreads, 1)
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
             uint32_t y0, y1;
-            unpack64(fma2f(pack64(v[c][e], v[c][e + 1]), sc2, neg2), y0, y1);
-            const float w0 = ex2(__uint_as_float(y0)), w1 = ex2(__uint_as_float(y1));
+            const uint64_t x2 = pack64(v[c][e], v[c][e + 1]);
+            unpack64(BITS ? add2f(x2, neg2) : fma2f(x2, sc2, neg2), y0, y1);
+            float w0 = ex2(__uint_as_float(y0)), w1 = ex2(__uint_as_float(y1));
             sum[c] = add2f(sum[c], pack64(__float_as_uint(w0), __float_as_uint(w1)));
+            if (VSCALE) {
+              const float2 s2 = reinterpret_cast<const float2*>(steps + 32)[16 * c + e / 2];
+              w0 *= s2.x;
+              w1 *= s2.y;
+            }
             v[c >> 1][(c & 1) * 16 + e / 2] = Act<T>::pack2(w0, w1);
           }
           if (c & 1) tmem_st32(tp + 32 * (c >> 1), v[c >> 1]);
@@ -605,6 +853,10 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         }
       }
       if (!ok) break;
+      if (BITS) {
+        gs += nbm > 0 ? nbm + 1 : 0;
+        bs += nbm;
+      }
       if (nt > 0) {
         if (!SEP) ++no;
         ok = __all_sync(0xffffffffu, mbar_wait(b_o + 8 * t, (uint32_t)((no - 1) & 1), a.timeout_ns));
@@ -617,7 +869,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       if (!whole && mine) *reinterpret_cast<float2*>(p.stat + 2 * at) = make_float2(m, l);
       // the element a lane's row starts at, -1 for a row that is not there
       const long long row_at = mine ? (long long)out_row * p.o_tok + head * p.o_head : -1;
-      const uint32_t stg = sb + pt_off_out<HD>() + warp * 4096;
+      const uint32_t stg = sb + pt_off_out<HD, BITS>() + warp * pt_stage<BITS>();
 #pragma unroll
       for (int c = 0; c < HD / 64; ++c) {
 #pragma unroll
@@ -641,7 +893,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                 w[k] = l == 0.f ? 0u
                                 : Act<T>::pack2(__uint_as_float(o[8 * e + 2 * k]) * inv,
                                                 __uint_as_float(o[8 * e + 2 * k + 1]) * inv);
-              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(stg + sw128(lane, 4 * h + e)), "r"(w[0]),
+              const uint32_t to_row = BITS ? lane * 64 + ((e ^ ((lane >> 1) & 3)) << 4) : sw128(lane, 4 * h + e);
+              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(stg + to_row), "r"(w[0]),
                            "r"(w[1]), "r"(w[2]), "r"(w[3])
                            : "memory");
             }
@@ -650,8 +903,24 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             for (int e = 0; e < 32; e += 4)
               *reinterpret_cast<uint4*>(p.part + at * HD + 64 * c + 32 * h + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
           }
+          if (BITS && whole) {  // 32 columns at a time: the ring of codes has taken the room for more
+            __syncwarp();
+            long long base[4];
+            uint4 line[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int rr = 8 * e + (lane >> 2);
+              base[e] = __shfl_sync(0xffffffffu, row_at, rr);
+              line[e] = lds16(stg + rr * 64 + (((lane & 3) ^ ((rr >> 1) & 3)) << 4));
+            }
+            T* out = reinterpret_cast<T*>(p.out) + 64 * c + 32 * h + 8 * (lane & 3);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (base[e] >= 0) *reinterpret_cast<uint4*>(out + base[e]) = line[e];
+            __syncwarp();
+          }
         }
-        if (whole) {
+        if (BITS == 0 && whole) {
           // 64 columns of the warp's rows from shared memory: a lane's own row would be 16 bytes of 32 lines a store
           __syncwarp();
           long long base[8];

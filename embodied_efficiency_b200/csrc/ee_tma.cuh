@@ -81,6 +81,14 @@ EE_DEV void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint
       : "memory");
 }
 
+// Untiled copy of `bytes` (a multiple of 16, as both addresses) into shared
+// memory, completing them on `bar`.
+EE_DEV void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
 // Pull a tensor map (kernel parameter) into the descriptor cache early.
 EE_DEV void tma_prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");

@@ -291,7 +291,7 @@ bool places(Call& c, PyObject* keys, PyObject* record, PyObject* cu_o, PyObject*
   if (!c.need(p.cache && p.cache->k_codes == k->data_ptr() && cu->dim() == 1 && cu->scalar_type() == at::kInt && cu->is_contiguous() && p.n >= 1 &&
               p.n < (1 << 30) && lens->dim() == 1 && lens->scalar_type() == at::kInt && lens->numel() == p.n &&
               lens->is_contiguous() && table->dim() == 2 && table->scalar_type() == at::kInt && table->size(0) == p.n &&
-              table->size(1) >= 1 && table->stride(1) == 1 && table->size(1) <= 0x7fffffff / p.cache->page_size))
+              table->size(1) >= 1 && table->stride(1) == 1 && table->size(1) <= 0x7fff0000 / p.cache->page_size))
     return false;
   p.cu = static_cast<const int32_t*>(cu->data_ptr());
   p.table = static_cast<const int32_t*>(table->data_ptr());
@@ -432,14 +432,15 @@ PyObject* cache_attention(PyObject*, PyObject* const* a, Py_ssize_t argc) {
     NoGil others;
     out = at::empty(q->sizes(), q->options());
     const size_t need = ee_cache_attention_workspace_bytes(tq, (int32_t)p.n, (int32_t)hq, (int32_t)hk, (int32_t)hd,
-                                                           p.cache->bits, plen);
-    const Tensor ws = at::empty({(int64_t)need}, q->options().dtype(at::kByte));
+                                                           p.cache->bits, p.width * p.cache->page_size, plen);
+    Tensor ws;
+    if (need) ws = at::empty({(int64_t)need}, q->options().dtype(at::kByte));
     rc = ee_cache_attention(p.cache, q->data_ptr(), q->stride(0), q->stride(1), out.data_ptr(), out.stride(0),
                             out.stride(1), p.cu, p.table, p.table_row, (int32_t)p.width, p.k_lens,
                             pk ? pk->data_ptr() : nullptr, pk ? pk->stride(0) : 0, pk ? pk->stride(1) : 0,
                             pv ? pv->data_ptr() : nullptr, pv ? pv->stride(0) : 0, pv ? pv->stride(1) : 0, plen, tq,
-                            (int32_t)p.n, (int32_t)hq, causal, scale, act_code(q->scalar_type()), ws.data_ptr(), need,
-                            c.stream());
+                            (int32_t)p.n, (int32_t)hq, causal, scale, act_code(q->scalar_type()),
+                            need ? ws.data_ptr() : nullptr, need, c.stream());
   }
   return give(rc, out);
 }

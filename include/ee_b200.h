@@ -314,11 +314,12 @@ int ee_cache_read(const ee_cache* cache, void* k, int64_t k_tok, int64_t k_head,
  * fp32 statistics and sums; weights are rounded to 16 bits (fp16: twice) for
  * the product with the values. Strides in elements, multiples of 8. tq * n_q <
  * 2^31 - 255. scale as for ee_prompt_attention.
- * workspace: ee_cache_attention_workspace_bytes() bytes, 16-byte aligned; calls
+ * workspace: ee_cache_attention_workspace_bytes() bytes (keys = width *
+ * page_size), 16-byte aligned (may be NULL when that is 0); calls
  * that may overlap need one each. A wait that gives up after a second leaves
  * EE_ERR_TIMEOUT in the status word of ee_wq_gemm_status. */
 size_t ee_cache_attention_workspace_bytes(int64_t tq, int32_t n_seq, int32_t n_q, int32_t n_kv, int32_t head_dim,
-                                          int32_t bits, int64_t prefix_len);
+                                          int32_t bits, int64_t keys, int64_t prefix_len);
 int ee_cache_attention(const ee_cache* cache, const void* q, int64_t q_tok, int64_t q_head, void* out, int64_t o_tok,
                        int64_t o_head, const int32_t* cu_q, const int32_t* table, int64_t table_row, int32_t width,
                        const int32_t* k_lens, const void* prefix_k, int64_t pk_tok, int64_t pk_head,

@@ -171,7 +171,8 @@ def test_abi_codes(lib):
     for i in (18, 19):
         assert fn(c, *(ca[:i] + [0] + ca[i + 1:])) == 0
     need = lib.ee_cache_attention_workspace_bytes
-    assert need(5, 1, 4, 2, 64, 8, 0) > 0 and need(5, 1, 4, 2, 64, 8, 100) > need(5, 1, 4, 2, 64, 8, 0)
-    for bad in ((0, 1, 4, 2, 64, 8, 0), (5, 1, 3, 2, 64, 8, 0), (5, 1, 4, 2, 96, 8, 0), (5, 1, 4, 2, 64, 16, 0),
-                (1 << 30, 1, 4, 2, 64, 8, 0), (5, 1, 4, 2, 64, 8, -1)):
+    assert need(5, 1, 4, 2, 64, 8, 128, 0) > 0 and need(5, 1, 4, 2, 64, 8, 128, 100) > need(5, 1, 4, 2, 64, 8, 128, 0)
+    for bad in ((0, 1, 4, 2, 64, 8, 128, 0), (5, 1, 3, 2, 64, 8, 128, 0), (5, 1, 4, 2, 96, 8, 128, 0),
+                (5, 1, 4, 2, 64, 16, 128, 0), (1 << 30, 1, 4, 2, 64, 8, 128, 0), (5, 1, 4, 2, 64, 8, 128, -1),
+                (5, 1, 4, 2, 64, 8, -1, 0)):
         assert need(*bad) == 0
