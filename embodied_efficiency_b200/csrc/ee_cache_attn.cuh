@@ -620,7 +620,7 @@ int launch_cache_tc(const CacheMaps& m, const PromptTcArgs& a, cudaStream_t s) {
   const long long items = ((long long)a.p.tq / (2 * a.tpt) + a.p.n_seq) * a.p.n_kv * a.p.splits;
   if (items > 0x7fffffff) return EE_ERR_SHAPE;
   const int sms = device_sms();
-  return launch_pdl(fn, dim3((unsigned)(items < sms ? items : sms)), dim3(kPtThreads), pt_smem<HD, BITS>(), s, mq, m.k, m.v,
+  return launch_pdl(fn, dim3((unsigned)(items < sms ? items : sms)), dim3(PtThreads<BITS>::N), pt_smem<HD, BITS>(), s, mq, m.k, m.v,
                     a) == cudaSuccess
              ? EE_OK
              : EE_ERR_LAUNCH;

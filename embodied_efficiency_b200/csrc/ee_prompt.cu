@@ -470,7 +470,7 @@ static int launch_tc(const PromptArgs& p, cudaStream_t s) {
   const long long items = ((long long)p.tq / (2 * a.tpt) + p.n_seq) * p.n_kv * p.splits;
   if (items > 0x7fffffff) return EE_ERR_SHAPE;
   const unsigned grid = (unsigned)(items < dp->sms ? items : dp->sms);
-  if (launch_pdl(fn, dim3(grid), dim3(kPtThreads), pt_smem<HD, 0>(), s, mq, mk, mv, a) != cudaSuccess) return EE_ERR_LAUNCH;
+  if (launch_pdl(fn, dim3(grid), dim3(PtThreads<0>::N), pt_smem<HD, 0>(), s, mq, mk, mv, a) != cudaSuccess) return EE_ERR_LAUNCH;
   return launch_combine<T, HD>(p, s);
 }
 

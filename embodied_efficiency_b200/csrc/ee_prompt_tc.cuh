@@ -68,41 +68,51 @@ struct PromptTcArgs {
   unsigned long long timeout_ns;
   CacheView c;  // keys and values in a cache
   const float *k_steps, *v_steps;
+  const float *pre_part, *pre_stat;  // sums over a prefix ([pre_splits][tq][n_q]), to be added to whole rows
+  int pre_splits;
 };
 
-constexpr int kPtThreads = 384;
 // registers: 384 threads launch with 168 each; the four warps of loads and MMAs
 // give theirs up to 88 and the softmax warps take 208 (256 x 208 + 128 x 88 =
-// 384 x 168), so that a whole row of S stays in registers
-constexpr int kPtRegsLaunch = 168, kPtRegsSoft = 208, kPtRegsRest = 88;
-static_assert(256 * kPtRegsSoft + 128 * kPtRegsRest <= kPtThreads * kPtRegsLaunch, "the register shares fit the launch");
+// 384 x 168), so that a whole row of S stays in registers. With four more warps
+// that decode a cache's codes 512 threads launch with 128, and the shares are
+// 200, 72 and 40.
+template <int BITS> struct PtThreads {
+  static constexpr int N = BITS ? 512 : 384, LAUNCH = BITS ? 128 : 168;
+  static constexpr int SOFT = BITS ? 200 : 208, REST = BITS ? 72 : 88, DECODE = BITS ? 40 : 0;
+  static_assert(256 * SOFT + 128 * REST + 128 * DECODE <= N * LAUNCH, "the register shares fit the launch");
+};
 constexpr int kPtKeys = 128, kPtInfo = 4, kPtLoads = 8;  // keys per block; items published, loads of K / V ahead
 constexpr unsigned long long kPtDrainNs = 1000000000ull;  // for loads and MMAs already issued, whatever timeout_ns is
 // Shared memory: Q of both tiles, the slots of K / V, output staging of every
 // softmax warp, barriers, published items; for a cache also the ring of codes
 // as they come, and the steps of the blocks.
-template <int HD, int BITS> constexpr int pt_slots() { return BITS ? (HD == 128 ? 3 : 6) : (HD == 128 ? 4 : 8); }
+template <int HD, int BITS> constexpr int pt_slots() { return BITS ? (HD == 128 ? 3 : 4) : (HD == 128 ? 4 : 8); }
+constexpr int kPtSlotsK = 2;  // of a cache's: K, the others V
 template <int HD> constexpr uint32_t pt_tile() { return 128u * HD * 2; }
-template <int BITS> constexpr uint32_t pt_stage() { return BITS ? 2048u : 4096u; }  // bytes of a warp's output staging
+template <int BITS> constexpr uint32_t pt_stage() { return BITS ? 0u : 4096u; }  // bytes of a warp's output staging
 template <int HD, int BITS> constexpr uint32_t pt_raw() { return 128u * HD * BITS / 8; }  // codes of a tile
-template <int HD, int BITS> constexpr int pt_raws() { return BITS ? (int)(32768u / (128u * HD * (BITS ? BITS : 8) / 8)) : 0; }
+// tiles of codes on their way: 40 to 48 KB where they are large (with 32 KB an SM waited for them)
+template <int HD, int BITS> constexpr int pt_raws() { return !BITS ? 0 : HD * BITS == 1024 ? 3 : HD * BITS == 512 ? 5 : 6; }
 constexpr int kPtSteps = 4;  // blocks whose steps are held
 template <int HD, int BITS> constexpr uint32_t pt_off_raw() { return (2 + pt_slots<HD, BITS>()) * pt_tile<HD>(); }
-template <int HD, int BITS> constexpr uint32_t pt_off_out() { return pt_off_raw<HD, BITS>() + (BITS ? 32768u : 0u); }
+template <int HD, int BITS> constexpr uint32_t pt_off_out() { return pt_off_raw<HD, BITS>() + pt_raws<HD, BITS>() * pt_raw<HD, BITS>(); }
 template <int HD, int BITS> constexpr uint32_t pt_off_rawsteps() { return pt_off_out<HD, BITS>() + 8 * pt_stage<BITS>(); }
 template <int HD, int BITS> constexpr uint32_t pt_off_steps() { return pt_off_rawsteps<HD, BITS>() + pt_raws<HD, BITS>() * 1024u; }
 template <int HD, int BITS> constexpr uint32_t pt_off_bar() { return pt_off_steps<HD, BITS>() + (BITS ? kPtSteps * 1024u : 0u); }
 // barriers: full / empty per load of K / V, Q full / empty, S / P (two halves) / S free / O / O free per tile, V to fix /
-// fixed, item full / empty, MMAs done after a failure, codes full / empty
+// fixed, item full / empty, MMAs done after a failure; of a cache tile 1's sums, steps full, codes full / empty. (There full
+// / empty are a slot's, K and V by themselves.)
 template <int HD, int BITS> constexpr uint32_t pt_off_info() {
-  return pt_off_bar<HD, BITS>() + 8 * (2 * kPtLoads + 17 + 2 * kPtInfo + 2 * pt_raws<HD, BITS>()) + 8;
+  return pt_off_bar<HD, BITS>() + 8 * (2 * kPtLoads + 18 + kPtSteps + 2 * kPtInfo + 2 * pt_raws<HD, BITS>()) + 8;
 }
 template <int HD, int BITS> constexpr uint32_t pt_off_beat() { return pt_off_info<HD, BITS>() + kPtInfo * 64; }  // blocks the MMA warp has come to
 // which keys of a block are there (4 words a block), which pieces of a tile of codes
 template <int HD, int BITS> constexpr uint32_t pt_off_there() { return pt_off_beat<HD, BITS>() + 16; }
-template <int HD, int BITS> constexpr uint32_t pt_smem() {
-  return pt_off_there<HD, BITS>() + (BITS ? kPtSteps * 16 + pt_raws<HD, BITS>() * 4 : 0) + 1024;
+template <int HD, int BITS> constexpr uint32_t pt_off_alt() {  // tile 1's maxima and sums for tile 0
+  return pt_off_there<HD, BITS>() + (BITS ? kPtSteps * 16 + (pt_raws<HD, BITS>() * 4 + 15) / 16 * 16 : 0);
 }
+template <int HD, int BITS> constexpr uint32_t pt_smem() { return pt_off_alt<HD, BITS>() + (BITS ? 1024 : 0) + 1024; }
 
 // One published item (16 words)
 struct PromptItem {
@@ -111,8 +121,9 @@ struct PromptItem {
   int key0;                // first key of this part
   int n[2];                // key blocks of the tiles in this part
   int tail;                // valid keys of the part's last block (128: all)
-  int nbm;                 // max(n[0], n[1]); -1: no more items
-  int pad[4];
+  int nbm;                 // blocks of keys: max(n[0], n[1]), or their sum where the tiles alternate; -1: no more items
+  int alt;                 // the item has rows for one tile only: both take them, tile t the blocks j = t mod 2
+  int pad[3];
 };
 
 EE_DEV void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
@@ -159,6 +170,7 @@ EE_DEV int prompt_window(const PromptTcArgs& a, const PromptWindow& w, PromptSeq
 
 // Item `idx` (unit-major from the last unit down, key heads and parts inside),
 // by the whole warp. False past the last item.
+template <int BITS>
 EE_DEV bool prompt_item(const PromptTcArgs& a, int idx, int units, PromptWindow& w, PromptItem& it) {
   const PromptArgs& p = a.p;
   const int per = p.n_kv * p.splits;
@@ -195,6 +207,11 @@ EE_DEV bool prompt_item(const PromptTcArgs& a, int idx, int units, PromptWindow&
   it.n[0] = max(min(nb[0], j1) - j0, 0);
   it.n[1] = max(min(nb[1], j1) - j0, 0);
   it.nbm = max(it.n[0], it.n[1]);
+  it.alt = BITS > 0 && it.n[1] == 0 && it.tok + a.tpt >= it.qlen && it.nbm > 1;
+  if (it.alt) {
+    it.n[0] = (it.nbm + 1) / 2;
+    it.n[1] = it.nbm / 2;
+  }
   it.tail = it.nbm > 0 ? min(it.klen - (j0 + it.nbm - 1) * kPtKeys, kPtKeys) : kPtKeys;
   return true;
 }
@@ -230,11 +247,12 @@ template <typename T, int BITS> EE_DEV constexpr float code_unit() { return BITS
 // that P V rounds to bf16 are the products). fp16 has no room for weights times
 // steps: there the values are multiplied and rounded once more, to fp16.
 template <typename T, int HD, int BITS = 0>
-__global__ void __launch_bounds__(kPtThreads, 1)
+__global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
     prompt_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                      const __grid_constant__ CUtensorMap mv, const __grid_constant__ PromptTcArgs a) {
-  constexpr int NS = pt_slots<HD, BITS>(), NP = kPtLoads, NR = pt_raws<HD, BITS>();
+  constexpr int NS = pt_slots<HD, BITS>(), NP = kPtLoads, NR = pt_raws<HD, BITS>(), KS = kPtSlotsK, VS = NS - KS;
   static_assert(NS <= NP, "a barrier per load that the slots can hold");
+  static_assert(pt_smem<HD, BITS>() <= 227 * 1024, "an SM's shared memory");
   constexpr uint32_t TILE = pt_tile<HD>(), PANEL = 128 * 128;  // a panel: 64 columns of 128 rows
   constexpr int PANELS = HD / 64;
   // hd 64 leaves TMEM for P beside S, so the next scores are computed during the softmax
@@ -251,7 +269,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   const uint32_t b_full = sb + pt_off_bar<HD, BITS>(), b_empty = b_full + 8 * NP;
   const uint32_t b_qf = b_empty + 8 * NP, b_qe = b_qf + 8, b_s = b_qe + 8, b_p = b_s + 16, b_sf = b_p + 32, b_o = b_sf + 16;
   const uint32_t b_of = b_o + 16, b_req = b_of + 16, b_fix = b_req + 8, b_if = b_fix + 8, b_ie = b_if + 8 * kPtInfo;
-  const uint32_t b_end = b_ie + 8 * kPtInfo, b_rf = b_end + 8, b_re = b_rf + 8 * NR, off_tm = b_re + 8 * NR - sb;
+  const uint32_t b_end = b_ie + 8 * kPtInfo, b_alt = b_end + 8, b_st = b_alt + 8, b_rf = b_st + 8 * kPtSteps, b_re = b_rf + 8 * NR, off_tm = b_re + 8 * NR - sb;
   volatile PromptItem* ring = reinterpret_cast<volatile PromptItem*>(smem + pt_off_info<HD, BITS>());
   volatile uint32_t* beat = reinterpret_cast<volatile uint32_t*>(smem + pt_off_beat<HD, BITS>());
   const PromptArgs& p = a.p;
@@ -260,18 +278,20 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     tma_prefetch_map(&mk);
     tma_prefetch_map(&mv);
     for (int s = 0; s < NP; ++s) {
-      mbar_init(b_full + 8 * s, BITS ? 2 : 1);
+      mbar_init(b_full + 8 * s, BITS ? 4 : 1);
       mbar_init(b_empty + 8 * s, 1);
     }
     for (int s = 0; s < NR; ++s) {
       mbar_init(b_rf + 8 * s, 1);
-      mbar_init(b_re + 8 * s, 2);
+      mbar_init(b_re + 8 * s, 4);
     }
     mbar_init(b_req, 1);
     mbar_init(b_fix, 1);
     mbar_init(b_qf, 1);
     mbar_init(b_qe, 1);
     mbar_init(b_end, 1);
+    mbar_init(b_alt, 4);
+    for (int i = 0; i < kPtSteps; ++i) mbar_init(b_st + 8 * i, 4);
     *beat = 0;
     for (int t = 0; t < 2; ++t) {
       mbar_init(b_s + 8 * t, 1);
@@ -283,7 +303,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     }
     for (int i = 0; i < kPtInfo; ++i) {
       mbar_init(b_if + 8 * i, 1);
-      mbar_init(b_ie + 8 * i, BITS ? 11 : 10);  // 8 softmax warps, the MMA warp, the fixing or decoding warps
+      mbar_init(b_ie + 8 * i, BITS ? 13 : 10);  // 8 softmax warps, the MMA warp, the fixing warp or four decoding ones
     }
     mbar_fence_init();
   }
@@ -313,8 +333,119 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   auto item_wait = [&](int i) { return wait_walk(b_if + 8 * (i % kPtInfo), (uint32_t)((i / kPtInfo) & 1)); };
   auto item_done = [&](int i) { mbar_arrive(b_ie + 8 * (i % kPtInfo)); };
 
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPtRegsRest));
+  if (BITS > 0 && warp >= 12) {
+    if constexpr (BITS > 0) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PtThreads<BITS>::DECODE));
+      // ---------------- codes into 16-bit tiles, 32 keys of each by a warp ----------------
+      constexpr int RB = HD * BITS / 8, CPR = RB / 16;  // 16-byte pieces of a row
+      const int quarter = warp - 12;
+      uint32_t rt = 0, count[2] = {0, 0};  // tiles of codes, of K and of V so far
+      bool ok = true;
+      for (int i = 0;; ++i) {
+        ok = __all_sync(0xffffffffu, item_wait(i));
+        if (!ok) break;
+        const volatile PromptItem* r = ring + i % kPtInfo;
+        const int nbm = r->nbm, klen = r->klen, key0 = r->key0;
+        __syncwarp();
+        if (lane == 0) item_done(i);
+        if (nbm < 0) break;
+        for (int x = 0; x < 2 * nbm && ok; ++x) {  // K(0) K(1) V(0) K(2) V(1) ... V(nbm - 1)
+          const bool isv = x == 2 * nbm - 1 || (x > 0 && (x & 1) == 0);
+          const int j = isv ? (x == 2 * nbm - 1 ? nbm - 1 : x / 2 - 1) : (x + 1) / 2;
+          const uint32_t rs = rt % NR, blk = isv ? count[1] : count[0], slots = isv ? VS : KS, slot = blk % slots;
+          const int at = (isv ? KS : 0) + slot;
+          ok = mbar_wait(b_rf + 8 * rs, (rt / NR) & 1, a.timeout_ns);
+          // the products of the tile that used the slot before are done
+          if (ok && blk >= slots) ok = mbar_wait(b_empty + 8 * at, (blk / slots - 1) & 1, a.timeout_ns);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const uint32_t raw = sb + pt_off_raw<HD, BITS>() + rs * pt_raw<HD, BITS>(), dst = sKV + at * TILE;
+          float* steps = reinterpret_cast<float*>(smem + pt_off_steps<HD, BITS>() + (blk % kPtSteps) * 1024);
+          if (!isv) {
+            const float* raw_steps = reinterpret_cast<const float*>(smem + pt_off_rawsteps<HD, BITS>() + rs * 1024);
+            const uint32_t there = *reinterpret_cast<volatile uint32_t*>(smem + pt_off_there<HD, BITS>() + kPtSteps * 16 + rs * 4);
+            const int shift = min(a.c.shift, 7), key = 32 * quarter + lane;
+            const bool have = key0 + j * kPtKeys + key < klen && (there >> (key >> shift) & 1);
+            float ks = have ? raw_steps[key] : 0.f, vs = have ? raw_steps[128 + key] : 0.f;
+            // a value's step that is no number must reach the rows that see it and no others: as its key's
+            if (!(fabsf(vs) <= 3.4028234e38f)) {
+              ks = __int_as_float(0x7fffffff);
+              vs = 0.f;
+            }
+            steps[key] = ks * (p.scale_log2 * code_unit<T, BITS>());
+            steps[128 + key] = vs * code_unit<T, BITS>();
+            const uint32_t all = __ballot_sync(0xffffffffu, have);
+            if (lane == 0)
+              *reinterpret_cast<volatile uint32_t*>(smem + pt_off_there<HD, BITS>() + (blk % kPtSteps) * 16 + quarter * 4) = all;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(b_st + 8 * (blk % kPtSteps));
+          }
+          constexpr int BATCH = CPR < 4 ? CPR : 4;  // pieces of a lane under way at once
+  #pragma unroll 1
+          for (int e0 = lane; e0 < 32 * CPR; e0 += 32 * BATCH) {
+            uint4 x[BATCH];
+  #pragma unroll
+            for (int u = 0; u < BATCH; ++u) x[u] = lds16(raw + 32 * quarter * RB + (e0 + 32 * u) * 16);
+  #pragma unroll
+            for (int u = 0; u < BATCH; ++u) {
+              const int e = e0 + 32 * u, row = 32 * quarter + e / CPR, q = e % CPR;
+              // heads of 128 in bytes: the upper half's lanes write their two pieces in the other order, so that the eight
+              // lanes of a row reach all banks
+              const int flip = HD * BITS == 1024 ? (q >> 2) & 1 : 0;
+              const uint32_t xw[4] = {flip ? x[u].z : x[u].x, flip ? x[u].w : x[u].y, flip ? x[u].x : x[u].z, flip ? x[u].y : x[u].w};
+              uint32_t o[64 / BITS];  // pairs
+  #pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                if (BITS == 8) {
+                  const uint32_t f = xw[k] ^ 0x80808080u;
+                  o[2 * k] = code_pair8<T>(f, 0);
+                  o[2 * k + 1] = code_pair8<T>(f, 1);
+                } else {
+  #pragma unroll
+                  for (int b = 0; b < 4; ++b) o[4 * k + b] = code_pair4<T>(xw[k], xw[k] >> 4, b);
+                }
+              }
+              if (!VSCALE && isv) {
+                const float s = steps[128 + row];
+  #pragma unroll
+                for (int k = 0; k < 64 / BITS; ++k) {
+                  const float2 f = Act<T>::unpack2(o[k]);
+                  o[k] = Act<T>::pack2(f.x * s, f.y * s);
+                }
+              }
+  #pragma unroll
+              for (int k = 0; k < 16 / BITS; ++k) {
+                const int c = q * (16 / BITS) + (HD * BITS == 1024 ? k ^ flip : k);  // 16-byte piece of the 16-bit row
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (c >> 3) * PANEL + sw128(row, c & 7)),
+                             "r"(o[4 * k]), "r"(o[4 * k + 1]), "r"(o[4 * k + 2]), "r"(o[4 * k + 3])
+                             : "memory");
+              }
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(b_re + 8 * rs);
+            mbar_arrive(b_full + 8 * at);
+          }
+          ++rt;
+          if (isv) ++count[1]; else ++count[0];
+        }
+        if (!ok) break;
+      }
+      // the MMA warp's arrivals that say the tiles are used have come
+      if (quarter == 0 && lane == 0) {
+        for (int v = 0; v < 2; ++v) {
+          const uint32_t slots = v ? VS : KS, n = v ? count[1] : count[0];
+          for (uint32_t e = n > slots ? n - slots : 0; e < n && ok; ++e)
+            ok = mbar_wait(b_empty + 8 * ((v ? KS : 0) + e % slots), (e / slots) & 1, a.timeout_ns);
+        }
+      }
+      if (!ok && lane == 0) atomicCAS(a.status, 0, (int)EE_ERR_TIMEOUT);
+      __syncwarp();
+    }
+  } else if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PtThreads<BITS>::REST));
     if (warp == 8) {
       // ---------------- items and loads ----------------
       bool ok = true;
@@ -333,7 +464,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       for (int i = 0;; ++i) {
         const long long idx = (long long)i * gridDim.x + ((i & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
         PromptItem it{};
-        const bool more = ok && idx < (long long)units * p.n_kv * p.splits && prompt_item(a, (int)idx, units, window, it);
+        const bool more = ok && idx < (long long)units * p.n_kv * p.splits && prompt_item<BITS>(a, (int)idx, units, window, it);
         if (lane == 0 && i >= kPtInfo)  // the slot's item has been read by all; if not, it stays as it is
           ok = mbar_wait(b_ie + 8 * (i % kPtInfo), (uint32_t)((i / kPtInfo - 1) & 1), a.timeout_ns);
         if (lane == 0 && ok) {
@@ -341,6 +472,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           r->q0 = it.q0; r->qlen = it.qlen; r->klen = it.klen;
           r->tok = it.tok; r->kvh = it.kvh; r->part = it.part; r->key0 = it.key0;
           r->n[0] = it.n[0]; r->n[1] = it.n[1]; r->tail = it.tail;
+          r->alt = it.alt;
           r->nbm = more ? it.nbm : -1;
           mbar_arrive(b_if + 8 * (i % kPtInfo));
           // tile w of the item (K(0) V(0) K(1) V(1) ...) into the next slot, on the load's barrier, which expects
@@ -388,58 +520,63 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
         if (!more || !ok) break;
         if constexpr (BITS > 0) {
-          // the tiles' codes, K(0) V(0) K(1) ..., in pieces of a page; a block's steps come with its K. A lane per piece
-          // looks its page up, a block ahead.
+          // the tiles' codes, K(0) K(1) V(0) K(2) V(1) ..., in pieces of a page; a block's steps come with its K. A lane per
+          // piece looks its page up, two blocks ahead.
           const int shift = min(a.c.shift, 7), pieces = kPtKeys >> shift;
           constexpr uint32_t RB = HD * BITS / 8;
-          auto rows_of = [&](int j) {  // this lane's piece of block j: its first row in the cache, -1 for none
+          auto page_of = [&](int j) {  // of this lane's piece of block j, -1 for none
             const int key = it.key0 + j * kPtKeys + (lane << shift);
             if (lane >= pieces || j >= it.nbm || key >= it.klen) return -1;
-            const int page = __ldg(a.c.table + (long long)it.k0 * a.c.table_row + (key >> a.c.shift));
-            if ((unsigned)page >= (unsigned)a.c.pages) return -1;
-            return ((page * a.c.n_kv + it.kvh) << a.c.shift) + (key & ((1 << a.c.shift) - 1));
+            return __ldg(a.c.table + (long long)it.k0 * a.c.table_row + (key >> a.c.shift));
           };
-          int row = rows_of(0);
-          for (int j = 0; j < it.nbm && ok; ++j) {
-            const int next = rows_of(j + 1);
-            const uint32_t there = __ballot_sync(0xffffffffu, row >= 0);
-            for (int w = 0; w < 2 && ok; ++w) {
-              if (w == 1 && j == 0) {
-                // Q: its buffers are free when the last scores of the previous item are done
-                if (lane == 0 && nq > 0) ok = mbar_wait(b_qe, (uint32_t)((nq - 1) & 1), a.timeout_ns);
-                ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-                if (!ok) break;
-                if (lane == 0) {
-                  mbar_arrive_expect_tx(b_qf, (it.n[0] > 0 ? qbytes : 0) + (it.n[1] > 0 ? qbytes : 0));
-                  for (int t = 0; t < 2; ++t)
-                    if (it.n[t] > 0)
-                      for (int c = 0; c < PANELS; ++c)
-                        tma_load_3d(sQ + t * TILE + c * PANEL, &mq, 64 * c, it.kvh * p.group, it.q0 + it.tok + t * a.tpt, b_qf);
-                }
-                ++nq;
-              }
-              const uint32_t slot = g % NR;
-              if (lane == 0 && g >= (uint32_t)NR) ok = mbar_wait(b_re + 8 * slot, (g / NR - 1) & 1, a.timeout_ns);
-              ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-              if (!ok) break;
-              const uint32_t bar = b_rf + 8 * slot, dst = sb + pt_off_raw<HD, BITS>() + slot * pt_raw<HD, BITS>();
-              const uint32_t steps = sb + pt_off_rawsteps<HD, BITS>() + slot * 1024;
-              if (lane == 0) {
-                *reinterpret_cast<volatile uint32_t*>(smem + pt_off_there<HD, BITS>() + kPtSteps * 16 + slot * 4) = there;
-                mbar_arrive_expect_tx(bar, __popc(there) * ((RB << shift) + (w == 0 ? 8u << shift : 0u)));
-              }
-              __syncwarp();
-              if (row >= 0) {
-                tma_load_2d(dst + lane * (RB << shift), w ? &mv : &mk, 0, row, bar);
-                if (w == 0) {
-                  bulk_load(steps + lane * (4 << shift), a.k_steps + row, 4 << shift, bar);
-                  bulk_load(steps + 512 + lane * (4 << shift), a.v_steps + row, 4 << shift, bar);
-                }
-              }
-              __syncwarp();
-              ++g;
+          auto codes = [&](int w, int j, int page) {  // K (w = 0) or V of block j
+            const bool there = (unsigned)page < (unsigned)a.c.pages;
+            const uint32_t mask = __ballot_sync(0xffffffffu, there), slot = g % NR;
+            if (lane == 0 && g >= (uint32_t)NR) ok = mbar_wait(b_re + 8 * slot, (g / NR - 1) & 1, a.timeout_ns);
+            ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+            if (!ok) return;
+            const uint32_t bar = b_rf + 8 * slot, dst = sb + pt_off_raw<HD, BITS>() + slot * pt_raw<HD, BITS>();
+            const uint32_t steps = sb + pt_off_rawsteps<HD, BITS>() + slot * 1024;
+            if (lane == 0) {
+              *reinterpret_cast<volatile uint32_t*>(smem + pt_off_there<HD, BITS>() + kPtSteps * 16 + slot * 4) = mask;
+              mbar_arrive_expect_tx(bar, __popc(mask) * ((RB << shift) + (w == 0 ? 8u << shift : 0u)));
             }
-            row = next;
+            __syncwarp();
+            if (there) {
+              const int key = it.key0 + j * kPtKeys + (lane << shift);
+              const int row = ((page * a.c.n_kv + it.kvh) << a.c.shift) + (key & ((1 << a.c.shift) - 1));
+              tma_load_2d(dst + lane * (RB << shift), w ? &mv : &mk, 0, row, bar);
+              if (w == 0) {
+                bulk_load(steps + lane * (4 << shift), a.k_steps + row, 4 << shift, bar);
+                bulk_load(steps + 512 + lane * (4 << shift), a.v_steps + row, 4 << shift, bar);
+              }
+            }
+            __syncwarp();
+            ++g;
+          };
+          if (it.nbm > 0) {
+            int page = page_of(0), next = page_of(1);
+            codes(0, 0, page);
+            // Q: its buffers are free when the last scores of the previous item are done
+            if (ok && lane == 0 && nq > 0) ok = mbar_wait(b_qe, (uint32_t)((nq - 1) & 1), a.timeout_ns);
+            ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+            if (!ok) break;
+            if (lane == 0) {
+              const bool two = it.n[1] > 0 && !it.alt;
+              mbar_arrive_expect_tx(b_qf, (it.n[0] > 0 ? qbytes : 0) + (two ? qbytes : 0));
+              for (int t = 0; t < 2; ++t)
+                if (t ? two : it.n[0] > 0)
+                  for (int c = 0; c < PANELS; ++c)
+                    tma_load_3d(sQ + t * TILE + c * PANEL, &mq, 64 * c, it.kvh * p.group, it.q0 + it.tok + t * a.tpt, b_qf);
+            }
+            ++nq;
+            for (int j = 0; j < it.nbm && ok; ++j) {
+              const int after = page_of(j + 2);
+              if (j + 1 < it.nbm) codes(0, j + 1, next);
+              if (ok) codes(1, j, page);
+              page = next;
+              next = after;
+            }
           }
           if (!ok) break;
         }
@@ -475,9 +612,10 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       bool ok = true;
       int sl = 0;                         // slot of the next K / V tile
       uint32_t g = 0, nq = 0, nfix = 0;   // loads of K / V, Q loads and fixed tails so far
+      uint32_t nk = 0, nv = 0;            // tiles of K and of V (cache)
       uint32_t np[2] = {0, 0}, no[2] = {0, 0};  // P blocks and outputs of each tile so far
-      auto scores = [&](int t, int slot) {      // S_t = Q_t K^T
-        const uint64_t qd = q_desc + (uint64_t)(t * (TILE >> 4)), kd = k_desc + (uint64_t)(slot * (TILE >> 4));
+      auto scores = [&](int t, int slot, int tq) {  // S_t = Q_tq K^T
+        const uint64_t qd = q_desc + (uint64_t)(tq * (TILE >> 4)), kd = k_desc + (uint64_t)(slot * (TILE >> 4));
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk) {
@@ -494,16 +632,95 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         const volatile PromptItem* r = ring + i % kPtInfo;
         const int nbm = __shfl_sync(0xffffffffu, r->nbm, 0), n0 = __shfl_sync(0xffffffffu, r->n[0], 0);
         const int n1 = __shfl_sync(0xffffffffu, r->n[1], 0), tail = __shfl_sync(0xffffffffu, r->tail, 0);
+        const bool alt = BITS > 0 && __shfl_sync(0xffffffffu, r->alt, 0) != 0;
         if (lane == 0) item_done(i);
         __syncwarp();
         if (nbm < 0) break;
         if (nbm == 0) continue;
+        if constexpr (BITS > 0) {
+          auto product = [&](int t, bool first, bool last) {  // O_t += P_t V, V in the next slot
+            const uint32_t outs = t ? no[1] : no[0], ps = t ? np[1] : np[0];
+            if (first && outs > 0) ok = wait(b_of + 8 * t, (outs - 1) & 1);  // O of the tile's previous item has been read
+            const uint64_t vd = v_desc + (uint64_t)((KS + nv % VS) * (TILE >> 4));
+#pragma unroll
+            for (int h = 0; h < PARTS; ++h) {
+              ok = ok && wait(b_p + 16 * h + 8 * t, ps & 1);
+              tc_fence_after();
+              if (ok && elect_one()) {
+#pragma unroll
+                for (int kk = 8 / PARTS * h; kk < 8 / PARTS * (h + 1); ++kk)
+                  umma_f16_ts(tmem + 256 + OC * t, tmem + (SEP ? 384 + 64 * t : 128 * t) + 8 * kk,
+                              vd + (uint64_t)((kk * 2048) >> 4), id_o, (!first || kk) ? 1u : 0u);
+                if (h == PARTS - 1 && (SEP || last)) umma_commit(b_o + 8 * t);
+              }
+              __syncwarp();
+            }
+            if (t) ++np[1]; else ++np[0];
+            if (last) {
+              if (t) ++no[1]; else ++no[0];
+            }
+          };
+          auto k_there = [&]() {
+            ok = ok && wait(b_full + 8 * (nk % KS), (nk / KS) & 1);
+            tc_fence_after();
+          };
+          auto k_used = [&](bool end) {  // the next K's slot is free when its scores are there; the item's last ones free Q
+            if (elect_one()) {
+              umma_commit(b_empty + 8 * (nk % KS));
+              if (end) umma_commit(b_qe);
+            }
+            __syncwarp();
+            ++nk;
+          };
+          ok = wait(b_qf, nq & 1);
+          ++nq;
+          // Scores of block j + 1 (of block 0 for j = -1) by tile: tiles that alternate take the other one's columns, and the
+          // scores and their softmax run before P(j) is there (P(j - 1) has been waited for, so S(j - 1) has been read)
+          for (int j = -1; j < nbm; ++j) {
+            const bool more = j + 1 < nbm;
+            if (lane == 0) *beat = *beat + 1;
+            __syncwarp();
+            // heads of 128: P lies over S, so a tile's next scores come after its product
+            const bool early = j < 0 || alt || SEP;
+            if (more) k_there();
+            if (more && early) {
+#pragma unroll 1
+              for (int t = 0; t < 2; ++t) {
+                if (!ok || (alt ? t != ((j + 1) & 1) : j + 1 >= (t ? n1 : n0))) continue;
+                if (SEP && !alt && j >= 0) {  // S(j) is in the softmax's registers
+                  ok = wait(b_sf + 8 * t, (t ? np[1] : np[0]) & 1);
+                  tc_fence_after();
+                }
+                if (ok) scores(t, nk % KS, alt ? 0 : t);
+              }
+              if (ok) k_used(j + 2 == nbm);
+            }
+            if (!ok) break;
+            if (j < 0) continue;
+            ok = wait(b_full + 8 * (KS + nv % VS), (nv / VS) & 1);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int t = 0; t < 2; ++t) {
+              const int nt = t ? n1 : n0;
+              if (!ok || (alt ? t != (j & 1) : j >= nt)) continue;
+              product(t, alt ? j < 2 : j == 0, alt ? j + 2 >= nbm : j + 1 == nt);
+              if (ok && !early && j + 1 < nt) scores(t, nk % KS, t);
+            }
+            if (ok && more && !early) k_used(j + 2 == nbm);
+            if (!ok) break;
+            if (elect_one()) umma_commit(b_empty + 8 * (KS + nv % VS));
+            __syncwarp();
+            ++nv;
+          }
+          continue;
+        }
         ok = wait(b_qf, nq & 1) && wait(b_full + 8 * (g % NP), (g / NP) & 1);
         if (!ok) break;
         ++nq;
         tc_fence_after();
-        if (n0 > 0) scores(0, sl);
-        if (n1 > 0) scores(1, sl);
+        if (n0 > 0) scores(0, sl, 0);
+        if (n1 > 0) scores(1, sl, 1);
         if (elect_one()) {
           umma_commit(b_empty + 8 * (g % NP));
           if (nbm == 1) umma_commit(b_qe);
@@ -515,7 +732,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           ok = wait(b_full + 8 * (g % NP), (g / NP) & 1);
           if (!ok) break;
           if (lane == 0) *beat = g;
-          bool fix = BITS == 0 && j + 1 == nbm && tail < kPtKeys;
+          bool fix = j + 1 == nbm && tail < kPtKeys;
           if (fix && lane == 0) mbar_arrive(b_req);
           __syncwarp();
           const uint64_t vd = v_desc + (uint64_t)(vs * (TILE >> 4));
@@ -525,7 +742,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
               if (!ok || j + 1 >= (t ? n1 : n0)) continue;
               ok = wait(b_sf + 8 * t, np[t] & 1);  // S(j) is in the softmax's registers
               tc_fence_after();
-              if (ok) scores(t, ks);
+              if (ok) scores(t, ks, t);
             }
           }
 #pragma unroll
@@ -553,7 +770,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
               __syncwarp();
             }
             ++np[t];
-            if (ok && !SEP && j + 1 < nt) scores(t, ks);
+            if (ok && !SEP && j + 1 < nt) scores(t, ks, t);
             if (j + 1 == nt) ++no[t];
           }
           if (!ok) break;
@@ -572,112 +789,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         mbar_wait(b_end, 0, kPtDrainNs);
         __syncwarp();
       }
-    } else if (BITS > 0) {
-      // ---------------- codes into 16-bit tiles, 64 keys of each by either warp ----------------
-      if constexpr (BITS > 0) {
-      constexpr int RB = HD * BITS / 8, CPR = RB / 16;  // 16-byte pieces of a row
-      const int half = warp - 10;
-      uint32_t g = 0, rt = 0, blk = 0, slot_load[NS];  // loads of K / V, tiles of codes and blocks so far, each slot's last load
-      int n = 0, sl = 0;                               // K / V tiles so far, next slot
-      bool ok = true;
-      for (int i = 0;; ++i) {
-        ok = __all_sync(0xffffffffu, item_wait(i));
-        if (!ok) break;
-        const volatile PromptItem* r = ring + i % kPtInfo;
-        const int nbm = r->nbm, klen = r->klen, key0 = r->key0;
-        __syncwarp();
-        if (lane == 0) item_done(i);
-        if (nbm < 0) break;
-        for (int w = 0; w < 2 * nbm && ok; ++w) {
-          const uint32_t rs = rt % NR;
-          ok = mbar_wait(b_rf + 8 * rs, (rt / NR) & 1, a.timeout_ns);
-          if (ok && n >= NS) {
-            const uint32_t was = slot_load[sl];  // the load that used the slot before has been consumed
-            ok = mbar_wait(b_empty + 8 * (was % NP), (was / NP) & 1, a.timeout_ns);
-          }
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          slot_load[sl] = g;
-          const uint32_t raw = sb + pt_off_raw<HD, BITS>() + rs * pt_raw<HD, BITS>(), dst = sKV + sl * TILE;
-          const float* raw_steps = reinterpret_cast<const float*>(smem + pt_off_rawsteps<HD, BITS>() + rs * 1024);
-          float* steps = reinterpret_cast<float*>(smem + pt_off_steps<HD, BITS>() + (blk % kPtSteps) * 1024);
-          if ((w & 1) == 0) {
-            const uint32_t there = *reinterpret_cast<volatile uint32_t*>(smem + pt_off_there<HD, BITS>() + kPtSteps * 16 + rs * 4);
-            const int shift = min(a.c.shift, 7);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int key = 64 * half + 32 * h + lane;
-              const bool have = key0 + (w >> 1) * kPtKeys + key < klen && (there >> (key >> shift) & 1);
-              float ks = have ? raw_steps[key] : 0.f, vs = have ? raw_steps[128 + key] : 0.f;
-              // a value's step that is no number must reach the rows that see it and no others: as its key's
-              if (!(fabsf(vs) <= 3.4028234e38f)) {
-                ks = __int_as_float(0x7fffffff);
-                vs = 0.f;
-              }
-              steps[key] = ks * (p.scale_log2 * code_unit<T, BITS>());
-              steps[128 + key] = vs * code_unit<T, BITS>();
-              const uint32_t all = __ballot_sync(0xffffffffu, have);
-              if (lane == 0)
-                *reinterpret_cast<volatile uint32_t*>(smem + pt_off_there<HD, BITS>() + (blk % kPtSteps) * 16 + (2 * half + h) * 4) = all;
-            }
-            __syncwarp();
-          }
-          const bool isv = w & 1;
-#pragma unroll 2
-          for (int e = lane; e < 64 * CPR; e += 32) {
-            const int row = 64 * half + e / CPR, q = e % CPR;
-            const uint4 x = lds16(raw + row * RB + q * 16);
-            const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
-            uint32_t o[64 / BITS];  // pairs
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              if (BITS == 8) {
-                const uint32_t f = xw[k] ^ 0x80808080u;
-                o[2 * k] = code_pair8<T>(f, 0);
-                o[2 * k + 1] = code_pair8<T>(f, 1);
-              } else {
-#pragma unroll
-                for (int b = 0; b < 4; ++b) o[4 * k + b] = code_pair4<T>(xw[k], xw[k] >> 4, b);
-              }
-            }
-            if (!VSCALE && isv) {
-              const float s = steps[128 + row];
-#pragma unroll
-              for (int k = 0; k < 64 / BITS; ++k) {
-                const float2 f = Act<T>::unpack2(o[k]);
-                o[k] = Act<T>::pack2(f.x * s, f.y * s);
-              }
-            }
-#pragma unroll
-            for (int k = 0; k < 16 / BITS; ++k) {
-              const int c = q * (16 / BITS) + k;  // 16-byte piece of the 16-bit row
-              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (c >> 3) * PANEL + sw128(row, c & 7)),
-                           "r"(o[4 * k]), "r"(o[4 * k + 1]), "r"(o[4 * k + 2]), "r"(o[4 * k + 3])
-                           : "memory");
-            }
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(b_re + 8 * rs);
-          ++rt;
-          ++n;
-          if (++sl == NS) sl = 0;
-          if (isv) ++blk;
-          if (w == 0 || (isv ? w + 1 == 2 * nbm : true)) {  // K(0) alone; V(j) with K(j + 1); the last V alone
-            if (lane == 0) mbar_arrive(b_full + 8 * (g % NP));
-            ++g;
-          }
-        }
-        if (!ok) break;
-      }
-      // the MMA warp's arrivals that say the tiles are used have come
-      if (half == 0 && lane == 0) {
-        for (uint32_t e = g > (uint32_t)NP ? g - NP : 0; e < g && ok; ++e) ok = mbar_wait(b_empty + 8 * (e % NP), (e / NP) & 1, a.timeout_ns);
-      }
-      if (!ok && lane == 0) atomicCAS(a.status, 0, (int)EE_ERR_TIMEOUT);
-      __syncwarp();
-      }
-    } else if (warp == 10) {
+    } else if (BITS == 0 && warp == 10) {
       // ---------------- V rows past the sequence's end ----------------
       int n = 0, nfix = 0;
       uint32_t g = 0;
@@ -710,13 +822,13 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     }
   } else {
     // ---------------- softmax and output ----------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPtRegsSoft));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PtThreads<BITS>::SOFT));
     const int t = warp >> 2, q4 = warp & 3, r = 32 * q4 + lane;
     const int rtok = r / p.group, rhead = r - rtok * p.group;
     const uint32_t ts = tmem + 128 * t + ((uint32_t)(32 * q4) << 16), to = tmem + 256 + OC * t + ((uint32_t)(32 * q4) << 16);
     const uint32_t tp = SEP ? tmem + 384 + 64 * t + ((uint32_t)(32 * q4) << 16) : ts;
     int ns = 0, no = 0;  // score blocks and commits of O (per block when SEP, else per item) so far
-    uint32_t gs = 0, bs = 0;  // loads of K / V and blocks of the items before (cache)
+    uint32_t bs = 0, nalt = 0;  // blocks and items shared by the tiles so far (cache)
     bool ok = true;
     for (int i = 0; ok; ++i) {
       ok = __all_sync(0xffffffffu, item_wait(i));
@@ -724,7 +836,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       const volatile PromptItem* it = ring + i % kPtInfo;
       if (it->nbm < 0) break;
       const int nt = it->n[t], qlen = it->qlen, klen = it->klen, key0 = it->key0, nbm = it->nbm;
-      const int tok = it->tok + t * a.tpt + rtok, head = it->kvh * p.group + rhead;
+      const bool alt = BITS > 0 && it->alt != 0;
+      const int tok = it->tok + (alt ? 0 : t) * a.tpt + rtok, head = it->kvh * p.group + rhead;
       const int out_row = it->q0 + tok;
       const int part = it->part;
       __syncwarp();
@@ -732,7 +845,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       const bool mine = rtok < a.tpt && tok < qlen;
       const int lim = (p.causal ? min(klen, klen - qlen + tok + 1) : klen) - key0;  // keys of this part the row sees
       float m = -INFINITY, top = -INFINITY, l = 0.f;  // top: the score at which m moves
-      for (int j = 0; j < nt; ++j) {
+      for (int i = 0; i < nt; ++i) {
+        const int j = alt ? 2 * i + t : i;
         ok = __all_sync(0xffffffffu, mbar_wait(b_s + 8 * t, (uint32_t)(ns & 1), a.timeout_ns));
         if (!ok) break;
         ++ns;
@@ -751,9 +865,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         uint32_t there[4];
         bool gaps = false;
         if constexpr (BITS > 0) {
-          // K(j) is in its slot, or S would not be there; this wait makes the block's steps visible here
-          const uint32_t gk = gs + j;
-          ok = __all_sync(0xffffffffu, mbar_wait(b_full + 8 * (gk % NP), (gk / NP) & 1, a.timeout_ns));
+          // the block's steps came before its K; four blocks on there are others
+          ok = __all_sync(0xffffffffu, mbar_wait(b_st + 8 * ((bs + j) % kPtSteps), ((bs + j) / kPtSteps) & 1, a.timeout_ns));
           if (!ok) break;
           const volatile uint32_t* tw =
               reinterpret_cast<volatile uint32_t*>(smem + pt_off_there<HD, BITS>() + ((bs + j) % kPtSteps) * 16);
@@ -798,8 +911,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           m = to;
           top = mx + 8.f;
         }
-        const bool rescale = __any_sync(0xffffffffu, f != 1.f) && j > 0;
-        if (SEP && j > 0) {  // O += P(j-1) V(j-1) is done: P may be written, O rescaled
+        const bool rescale = __any_sync(0xffffffffu, f != 1.f) && i > 0;
+        if (SEP && i > 0) {  // O += P(j-1) V(j-1) is done: P may be written, O rescaled
           ok = __all_sync(0xffffffffu, mbar_wait(b_o + 8 * t, (uint32_t)((no - 1) & 1), a.timeout_ns));
           if (!ok) break;
           tc_fence_after();
@@ -820,6 +933,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         const float neg = m == -INFINITY ? 0.f : -m;
         const uint64_t sc2 = both(p.scale_log2), neg2 = both(neg);
         uint64_t sum[4] = {0, 0, 0, 0};
+        float4 vs4;
         // weights of the block, 64 keys at a time: the products with the first half start under the second
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -831,9 +945,14 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             float w0 = ex2(__uint_as_float(y0)), w1 = ex2(__uint_as_float(y1));
             sum[c] = add2f(sum[c], pack64(__float_as_uint(w0), __float_as_uint(w1)));
             if (VSCALE) {
-              const float2 s2 = reinterpret_cast<const float2*>(steps + 32)[16 * c + e / 2];
-              w0 *= s2.x;
-              w1 *= s2.y;
+              if (e % 4 == 0) vs4 = steps[32 + 8 * c + e / 4];
+              uint32_t u0, u1;
+              unpack64(mul2f(pack64(__float_as_uint(w0), __float_as_uint(w1)),
+                             e % 4 == 0 ? pack64(__float_as_uint(vs4.x), __float_as_uint(vs4.y))
+                                        : pack64(__float_as_uint(vs4.z), __float_as_uint(vs4.w))),
+                       u0, u1);
+              w0 = __uint_as_float(u0);
+              w1 = __uint_as_float(u1);
             }
             v[c >> 1][(c & 1) * 16 + e / 2] = Act<T>::pack2(w0, w1);
           }
@@ -853,10 +972,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         }
       }
       if (!ok) break;
-      if (BITS) {
-        gs += nbm > 0 ? nbm + 1 : 0;
-        bs += nbm;
-      }
+      if (BITS) bs += nbm;
       if (nt > 0) {
         if (!SEP) ++no;
         ok = __all_sync(0xffffffffu, mbar_wait(b_o + 8 * t, (uint32_t)((no - 1) & 1), a.timeout_ns));
@@ -864,6 +980,47 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       }
       tc_fence_after();
       const bool whole = p.splits == 1 && !p.sums;
+      if (BITS && alt && t == 1) {  // its sums and O, in the same lanes of tensor memory, are tile 0's to finish
+        *reinterpret_cast<volatile float*>(smem + pt_off_alt<HD, BITS>() + 8 * r) = m;
+        *reinterpret_cast<volatile float*>(smem + pt_off_alt<HD, BITS>() + 8 * r + 4) = l;
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(b_alt);
+        continue;
+      }
+      float own = 1.f, own1 = 0.f;  // what O (and tile 1's) is multiplied by before the division
+      bool merge = false;
+      const long long row0 = (long long)out_row * p.n_q + head, hop = (long long)p.tq * p.n_q;
+      const float2* pre_stat = reinterpret_cast<const float2*>(a.pre_stat) + row0;
+      float ref = m;
+      if (BITS && alt) {
+        ok = __all_sync(0xffffffffu, mbar_wait(b_alt, (uint32_t)(nalt & 1), a.timeout_ns));
+        if (!ok) break;
+        ++nalt;
+        tc_fence_after();
+        const float m1 = *reinterpret_cast<volatile float*>(smem + pt_off_alt<HD, BITS>() + 8 * r);
+        const float l1 = *reinterpret_cast<volatile float*>(smem + pt_off_alt<HD, BITS>() + 8 * r + 4);
+        ref = fmaxf(m, m1);
+        merge = true;
+        own = m == -INFINITY ? 0.f : ex2(m - ref);
+        own1 = m1 == -INFINITY ? 0.f : ex2(m1 - ref);
+        l = l * own + l1 * own1;
+        m = ref;
+      }
+      if (BITS && a.pre_splits && mine) {
+        for (int i = 0; i < a.pre_splits; ++i) {
+          const float2 x = __ldg(pre_stat + i * hop);
+          if (x.y != 0.f) ref = fmaxf(ref, x.x);
+        }
+        const float f = m == -INFINITY ? 0.f : ex2(m - ref);
+        l *= f;
+        own *= f;
+        own1 *= f;
+        for (int i = 0; i < a.pre_splits; ++i) {
+          const float2 x = __ldg(pre_stat + i * hop);
+          if (x.y != 0.f) l += ex2(x.x - ref) * x.y;
+        }
+      }
       const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees no key is zero
       const long long at = ((long long)part * p.tq + out_row) * p.n_q + head;
       if (!whole && mine) *reinterpret_cast<float2*>(p.stat + 2 * at) = make_float2(m, l);
@@ -877,11 +1034,42 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           uint32_t o[32];
           if (nt > 0) {
             tmem_ld32(to + 64 * c + 32 * h, o);
-            tmem_wait_ld();
+            if (BITS && merge) {
+              uint32_t x[32];
+              tmem_ld32(to + OC + 64 * c + 32 * h, x);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * own + __uint_as_float(x[e]) * own1);
+            } else {
+              tmem_wait_ld();
+            }
             if (c == HD / 64 - 1 && h == 1) {  // O has been read: the next item may start over
               tc_fence_before();
               __syncwarp();
-              if (lane == 0) mbar_arrive(b_of + 8 * t);
+              if (lane == 0) {
+                mbar_arrive(b_of + 8 * t);
+                if (BITS && merge) mbar_arrive(b_of + 8);
+              }
+            }
+          }
+          if (BITS && a.pre_splits && mine) {
+            if (!merge) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = nt > 0 ? __float_as_uint(__uint_as_float(o[e]) * own) : 0u;
+            }
+            for (int i = 0; i < a.pre_splits; ++i) {
+              const float2 x = __ldg(pre_stat + i * hop);
+              if (x.y == 0.f) continue;
+              const float f = ex2(x.x - ref);
+              const float4* src = reinterpret_cast<const float4*>(a.pre_part + (row0 + i * hop) * HD + 64 * c + 32 * h);
+#pragma unroll
+              for (int e = 0; e < 32; e += 4) {
+                const float4 y = __ldg(src + e / 4);
+                o[e] = __float_as_uint(fmaf(f, y.x, __uint_as_float(o[e])));
+                o[e + 1] = __float_as_uint(fmaf(f, y.y, __uint_as_float(o[e + 1])));
+                o[e + 2] = __float_as_uint(fmaf(f, y.z, __uint_as_float(o[e + 2])));
+                o[e + 3] = __float_as_uint(fmaf(f, y.w, __uint_as_float(o[e + 3])));
+              }
             }
           }
           if (whole) {
@@ -893,31 +1081,20 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                 w[k] = l == 0.f ? 0u
                                 : Act<T>::pack2(__uint_as_float(o[8 * e + 2 * k]) * inv,
                                                 __uint_as_float(o[8 * e + 2 * k + 1]) * inv);
-              const uint32_t to_row = BITS ? lane * 64 + ((e ^ ((lane >> 1) & 3)) << 4) : sw128(lane, 4 * h + e);
-              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(stg + to_row), "r"(w[0]),
-                           "r"(w[1]), "r"(w[2]), "r"(w[3])
-                           : "memory");
+              if (BITS) {  // 16 bytes of a lane's own row: the ring of codes has taken the room to gather lines in
+                if (mine)
+                  *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + row_at + 64 * c + 32 * h + 8 * e) =
+                      make_uint4(w[0], w[1], w[2], w[3]);
+              } else {
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(stg + sw128(lane, 4 * h + e)), "r"(w[0]),
+                             "r"(w[1]), "r"(w[2]), "r"(w[3])
+                             : "memory");
+              }
             }
           } else if (mine && l != 0.f) {
 #pragma unroll
             for (int e = 0; e < 32; e += 4)
               *reinterpret_cast<uint4*>(p.part + at * HD + 64 * c + 32 * h + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-          }
-          if (BITS && whole) {  // 32 columns at a time: the ring of codes has taken the room for more
-            __syncwarp();
-            long long base[4];
-            uint4 line[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int rr = 8 * e + (lane >> 2);
-              base[e] = __shfl_sync(0xffffffffu, row_at, rr);
-              line[e] = lds16(stg + rr * 64 + (((lane & 3) ^ ((rr >> 1) & 3)) << 4));
-            }
-            T* out = reinterpret_cast<T*>(p.out) + 64 * c + 32 * h + 8 * (lane & 3);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (base[e] >= 0) *reinterpret_cast<uint4*>(out + base[e]) = line[e];
-            __syncwarp();
           }
         }
         if (BITS == 0 && whole) {
