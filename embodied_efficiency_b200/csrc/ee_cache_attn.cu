@@ -11,7 +11,7 @@ int cache_view(const ee_cache* c, const int32_t* table, int64_t table_row, int32
                int32_t n_seq, CacheView* v);                       // ee_cache.cu
 // ee_prompt.cu
 int prompt_sums_splits(long long tq, long long tk, int n_q, int n_kv);
-int prompt_parts(long long tq, int n_seq, int n_q, int n_kv, long long keys);
+int prompt_parts(long long tq, int n_seq, int n_q, int n_kv, long long keys, int tiles);
 int launch_prompt_sums(const PromptArgs& a, int head_dim, int act_dtype, cudaStream_t s);
 int launch_prompt_combine(const PromptArgs& a, int head_dim, int act_dtype, cudaStream_t s);
 
@@ -26,7 +26,7 @@ static CachePlan cache_plan(long long tq, int n_seq, int n_q, int n_kv, long lon
   const long long rows = tq * group;
   if (rows <= 8ll * n_seq) return CachePlan{1, 1};
   if (rows <= 16ll * n_seq || group > 128) return CachePlan{2, 1};
-  return CachePlan{0, prompt_parts(tq, n_seq, n_q, n_kv, keys)};
+  return CachePlan{0, prompt_parts(tq, n_seq, n_q, n_kv, keys, 1)};
 }
 template <int HD, int BITS>
 static int plan_workers_b(const CachePlan& p) {

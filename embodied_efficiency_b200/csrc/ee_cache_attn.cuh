@@ -616,8 +616,8 @@ int launch_cache_tc(const CacheMaps& m, const PromptTcArgs& a, cudaStream_t s) {
   allow_max_smem(fn, set);
   CUtensorMap mq;
   if (!prompt_head_map(&mq, a.p.q, HD, a.p.n_q, a.p.tq, a.p.q_head, a.p.q_tok, a.p.group, a.tpt)) return EE_ERR_SHAPE;
-  // at most one partial unit per sequence beyond the rows' whole units
-  const long long items = ((long long)a.p.tq / (2 * a.tpt) + a.p.n_seq) * a.p.n_kv * a.p.splits;
+  // at most one partial tile per sequence beyond the rows' whole tiles
+  const long long items = ((long long)a.p.tq / a.tpt + a.p.n_seq) * a.p.n_kv * a.p.splits;
   if (items > 0x7fffffff) return EE_ERR_SHAPE;
   const int sms = device_sms();
   return launch_pdl(fn, dim3((unsigned)(items < sms ? items : sms)), dim3(PtThreads<BITS>::N), pt_smem<HD, BITS>(), s, mq, m.k, m.v,

@@ -381,14 +381,14 @@ __global__ void __launch_bounds__(kPrJoin) prompt_join_kernel(const __grid_const
 //           parts of 512 keys or more, joined by a second launch
 constexpr long long kPrRows = 16, kPtMinKeys = 512;
 struct PromptPlan { bool tc; int splits; };
-int prompt_parts(long long tq, int n_seq, int n_q, int n_kv, long long keys);
+int prompt_parts(long long tq, int n_seq, int n_q, int n_kv, long long keys, int tiles);
 static PromptPlan prompt_plan(long long tq, long long tk, int n_seq, int n_q, int n_kv) {
   PromptPlan pl{false, 1};
   if (n_seq < 1) return pl;
   const int group = n_q / n_kv;
   const long long rows = tq * group;
   pl.tc = rows > kPrRows * n_seq && tk > 0 && group <= 128;
-  if (pl.tc) pl.splits = prompt_parts(tq, n_seq, n_q, n_kv, tk / n_seq);
+  if (pl.tc) pl.splits = prompt_parts(tq, n_seq, n_q, n_kv, tk / n_seq, 2);
   return pl;
 }
 static long long prompt_partials(const PromptPlan& pl, long long tq, int n_q, int hd) {  // partial rows
@@ -491,9 +491,9 @@ int prompt_sums_splits(long long tq, long long tk, int n_q, int n_kv) {
 }
 // Parts of the keys for items that would leave SMs idle, at most one per 512 of
 // `keys` a sequence.
-int prompt_parts(long long tq, int n_seq, int n_q, int n_kv, long long keys) {
+int prompt_parts(long long tq, int n_seq, int n_q, int n_kv, long long keys, int tiles) {
   const int group = n_q / n_kv;
-  const long long rows = tq * group, per = 2 * (128 / group) * group;  // of an item: two tiles of whole tokens
+  const long long rows = tq * group, per = tiles * (128 / group) * group;  // of an item: tiles of whole tokens
   const long long items = (rows / per > n_seq ? rows / per : n_seq) * n_kv;
   const long long want = device_sms() / items, most = keys / kPtMinKeys;
   const long long s = want < most ? want : most;

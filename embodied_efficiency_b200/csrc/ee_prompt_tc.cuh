@@ -87,32 +87,33 @@ constexpr unsigned long long kPtDrainNs = 1000000000ull;  // for loads and MMAs 
 // Shared memory: Q of both tiles, the slots of K / V, output staging of every
 // softmax warp, barriers, published items; for a cache also the ring of codes
 // as they come, and the steps of the blocks.
-template <int HD, int BITS> constexpr int pt_slots() { return BITS ? (HD == 128 ? 3 : 4) : (HD == 128 ? 4 : 8); }
+template <int HD, int BITS> constexpr int pt_slots() { return BITS ? 4 : (HD == 128 ? 4 : 8); }
 constexpr int kPtSlotsK = 2;  // of a cache's: K, the others V
+template <int BITS> constexpr int pt_tiles() { return BITS ? 1 : 2; }  // tiles of rows in an item
 template <int HD> constexpr uint32_t pt_tile() { return 128u * HD * 2; }
 template <int BITS> constexpr uint32_t pt_stage() { return BITS ? 0u : 4096u; }  // bytes of a warp's output staging
 template <int HD, int BITS> constexpr uint32_t pt_raw() { return 128u * HD * BITS / 8; }  // codes of a tile
 // tiles of codes on their way: 40 to 48 KB where they are large (with 32 KB an SM waited for them)
 template <int HD, int BITS> constexpr int pt_raws() { return !BITS ? 0 : HD * BITS == 1024 ? 3 : HD * BITS == 512 ? 5 : 6; }
 constexpr int kPtSteps = 4;  // blocks whose steps are held
-template <int HD, int BITS> constexpr uint32_t pt_off_raw() { return (2 + pt_slots<HD, BITS>()) * pt_tile<HD>(); }
+template <int HD, int BITS> constexpr uint32_t pt_off_raw() { return (pt_tiles<BITS>() + pt_slots<HD, BITS>()) * pt_tile<HD>(); }
 template <int HD, int BITS> constexpr uint32_t pt_off_out() { return pt_off_raw<HD, BITS>() + pt_raws<HD, BITS>() * pt_raw<HD, BITS>(); }
 template <int HD, int BITS> constexpr uint32_t pt_off_rawsteps() { return pt_off_out<HD, BITS>() + 8 * pt_stage<BITS>(); }
 template <int HD, int BITS> constexpr uint32_t pt_off_steps() { return pt_off_rawsteps<HD, BITS>() + pt_raws<HD, BITS>() * 1024u; }
 template <int HD, int BITS> constexpr uint32_t pt_off_bar() { return pt_off_steps<HD, BITS>() + (BITS ? kPtSteps * 1024u : 0u); }
 // barriers: full / empty per load of K / V, Q full / empty, S / P (two halves) / S free / O / O free per tile, V to fix /
-// fixed, item full / empty, MMAs done after a failure; of a cache tile 1's sums, steps full, codes full / empty. (There full
-// / empty are a slot's, K and V by themselves.)
+// fixed, item full / empty, MMAs done after a failure; of a cache the other half's sums (twice), steps full, codes full /
+// empty. (There full / empty are a slot's, K and V by themselves.)
 template <int HD, int BITS> constexpr uint32_t pt_off_info() {
-  return pt_off_bar<HD, BITS>() + 8 * (2 * kPtLoads + 18 + kPtSteps + 2 * kPtInfo + 2 * pt_raws<HD, BITS>()) + 8;
+  return pt_off_bar<HD, BITS>() + 8 * (2 * kPtLoads + 19 + kPtSteps + 2 * kPtInfo + 2 * pt_raws<HD, BITS>()) + 8;
 }
 template <int HD, int BITS> constexpr uint32_t pt_off_beat() { return pt_off_info<HD, BITS>() + kPtInfo * 64; }  // blocks the MMA warp has come to
 // which keys of a block are there (4 words a block), which pieces of a tile of codes
 template <int HD, int BITS> constexpr uint32_t pt_off_there() { return pt_off_beat<HD, BITS>() + 16; }
-template <int HD, int BITS> constexpr uint32_t pt_off_alt() {  // tile 1's maxima and sums for tile 0
+template <int HD, int BITS> constexpr uint32_t pt_off_half() {  // one tile's maxima and sums for the other, of two items
   return pt_off_there<HD, BITS>() + (BITS ? kPtSteps * 16 + (pt_raws<HD, BITS>() * 4 + 15) / 16 * 16 : 0);
 }
-template <int HD, int BITS> constexpr uint32_t pt_smem() { return pt_off_alt<HD, BITS>() + (BITS ? 1024 : 0) + 1024; }
+template <int HD, int BITS> constexpr uint32_t pt_smem() { return pt_off_half<HD, BITS>() + (BITS ? 2048 : 0) + 1024; }
 
 // One published item (16 words)
 struct PromptItem {
@@ -122,7 +123,7 @@ struct PromptItem {
   int n[2];                // key blocks of the tiles in this part
   int tail;                // valid keys of the part's last block (128: all)
   int nbm;                 // blocks of keys: max(n[0], n[1]), or their sum where the tiles alternate; -1: no more items
-  int alt;                 // the item has rows for one tile only: both take them, tile t the blocks j = t mod 2
+  int turn;                // a cache's items: block j is for the softmax and the columns of "tile" (j + turn) mod 2
   int pad[3];
 };
 
@@ -154,11 +155,12 @@ struct PromptWindow {
   int base, before;  // first sequence; units before it
 };
 // The window's sequences, one a lane, and the units up to and including each.
+template <int BITS>
 EE_DEV int prompt_window(const PromptTcArgs& a, const PromptWindow& w, PromptSeq& s, int& nu) {
   const int lane = threadIdx.x & 31, b = w.base + lane;
   s = PromptSeq{};
   if (b < a.p.n_seq) s = prompt_seq(a.p, b);
-  nu = (s.qlen + 2 * a.tpt - 1) / (2 * a.tpt);
+  nu = (s.qlen + pt_tiles<BITS>() * a.tpt - 1) / (pt_tiles<BITS>() * a.tpt);
   int inc = nu;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -179,10 +181,10 @@ EE_DEV bool prompt_item(const PromptTcArgs& a, int idx, int units, PromptWindow&
   it.kvh = idx % per / p.splits;
   it.part = idx % p.splits;
   PromptSeq s;
-  int nu, inc = prompt_window(a, w, s, nu);
+  int nu, inc = prompt_window<BITS>(a, w, s, nu);
   while (unit < w.before && w.base > 0) {
     w.base -= 32;
-    inc = prompt_window(a, w, s, nu);
+    inc = prompt_window<BITS>(a, w, s, nu);
     w.before -= __shfl_sync(0xffffffffu, inc, 31);
   }
   inc += w.before;
@@ -193,13 +195,13 @@ EE_DEV bool prompt_item(const PromptTcArgs& a, int idx, int units, PromptWindow&
   it.qlen = __shfl_sync(0xffffffffu, s.qlen, src);
   it.k0 = __shfl_sync(0xffffffffu, s.k0, src);
   it.klen = __shfl_sync(0xffffffffu, s.klen, src);
-  it.tok = (unit - __shfl_sync(0xffffffffu, inc - nu, src)) * 2 * a.tpt;
+  it.tok = (unit - __shfl_sync(0xffffffffu, inc - nu, src)) * pt_tiles<BITS>() * a.tpt;
   int nb[2];
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     const int first = it.tok + t * a.tpt, last = min(first + a.tpt, it.qlen);
     const int kend = p.causal ? min(max(it.klen - it.qlen + last, 0), it.klen) : it.klen;
-    nb[t] = first < it.qlen ? (kend + kPtKeys - 1) / kPtKeys : 0;
+    nb[t] = t < pt_tiles<BITS>() && first < it.qlen ? (kend + kPtKeys - 1) / kPtKeys : 0;
   }
   const int all = max(nb[0], nb[1]);
   const int j0 = (int)((long long)all * it.part / p.splits), j1 = (int)((long long)all * (it.part + 1) / p.splits);
@@ -207,11 +209,6 @@ EE_DEV bool prompt_item(const PromptTcArgs& a, int idx, int units, PromptWindow&
   it.n[0] = max(min(nb[0], j1) - j0, 0);
   it.n[1] = max(min(nb[1], j1) - j0, 0);
   it.nbm = max(it.n[0], it.n[1]);
-  it.alt = BITS > 0 && it.n[1] == 0 && it.tok + a.tpt >= it.qlen && it.nbm > 1;
-  if (it.alt) {
-    it.n[0] = (it.nbm + 1) / 2;
-    it.n[1] = it.nbm / 2;
-  }
   it.tail = it.nbm > 0 ? min(it.klen - (j0 + it.nbm - 1) * kPtKeys, kPtKeys) : kPtKeys;
   return true;
 }
@@ -265,11 +262,11 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
   const uint32_t sb = (base0 + 1023u) & ~1023u;
   char* smem = smem_raw + (sb - base0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t sQ = sb, sKV = sb + 2 * TILE;
+  const uint32_t sQ = sb, sKV = sb + pt_tiles<BITS>() * TILE;
   const uint32_t b_full = sb + pt_off_bar<HD, BITS>(), b_empty = b_full + 8 * NP;
   const uint32_t b_qf = b_empty + 8 * NP, b_qe = b_qf + 8, b_s = b_qe + 8, b_p = b_s + 16, b_sf = b_p + 32, b_o = b_sf + 16;
   const uint32_t b_of = b_o + 16, b_req = b_of + 16, b_fix = b_req + 8, b_if = b_fix + 8, b_ie = b_if + 8 * kPtInfo;
-  const uint32_t b_end = b_ie + 8 * kPtInfo, b_alt = b_end + 8, b_st = b_alt + 8, b_rf = b_st + 8 * kPtSteps, b_re = b_rf + 8 * NR, off_tm = b_re + 8 * NR - sb;
+  const uint32_t b_end = b_ie + 8 * kPtInfo, b_half = b_end + 8, b_st = b_half + 16, b_rf = b_st + 8 * kPtSteps, b_re = b_rf + 8 * NR, off_tm = b_re + 8 * NR - sb;
   volatile PromptItem* ring = reinterpret_cast<volatile PromptItem*>(smem + pt_off_info<HD, BITS>());
   volatile uint32_t* beat = reinterpret_cast<volatile uint32_t*>(smem + pt_off_beat<HD, BITS>());
   const PromptArgs& p = a.p;
@@ -290,7 +287,8 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
     mbar_init(b_qf, 1);
     mbar_init(b_qe, 1);
     mbar_init(b_end, 1);
-    mbar_init(b_alt, 4);
+    mbar_init(b_half, 4);
+    mbar_init(b_half + 8, 4);
     for (int i = 0; i < kPtSteps; ++i) mbar_init(b_st + 8 * i, 4);
     *beat = 0;
     for (int t = 0; t < 2; ++t) {
@@ -450,21 +448,28 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
       // ---------------- items and loads ----------------
       bool ok = true;
       int units = 0, n = 0, nq = 0, sl = 0;  // K / V tiles and Q loads issued so far, next slot
+      int bs = 0;                            // blocks so far (cache)
       uint32_t g = 0, slot_load[NS];         // loads (barrier phases) of K / V so far, and each slot's last one
 #pragma unroll 4
-      for (int b = lane; b < p.n_seq; b += 32) units += (prompt_seq(p, b).qlen + 2 * a.tpt - 1) / (2 * a.tpt);
+      for (int b = lane; b < p.n_seq; b += 32) units += (prompt_seq(p, b).qlen + pt_tiles<BITS>() * a.tpt - 1) / (pt_tiles<BITS>() * a.tpt);
       units = __reduce_add_sync(0xffffffffu, units);
       PromptWindow window{(p.n_seq - 1) / 32 * 32, 0};
       {
         PromptSeq s;
         int nu;
-        window.before = units - __shfl_sync(0xffffffffu, prompt_window(a, window, s, nu), 31);
+        window.before = units - __shfl_sync(0xffffffffu, prompt_window<BITS>(a, window, s, nu), 31);
       }
       const uint32_t qbytes = (uint32_t)(p.group * a.tpt) * 128u * PANELS;
       for (int i = 0;; ++i) {
         const long long idx = (long long)i * gridDim.x + ((i & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
         PromptItem it{};
         const bool more = ok && idx < (long long)units * p.n_kv * p.splits && prompt_item<BITS>(a, (int)idx, units, window, it);
+        if (BITS) {  // the blocks of one item after another take turns on the tiles' softmax warps and columns
+          it.turn = bs & 1;
+          it.n[it.turn] = (it.nbm + 1) / 2;
+          it.n[1 - it.turn] = it.nbm / 2;
+          bs += it.nbm;
+        }
         if (lane == 0 && i >= kPtInfo)  // the slot's item has been read by all; if not, it stays as it is
           ok = mbar_wait(b_ie + 8 * (i % kPtInfo), (uint32_t)((i / kPtInfo - 1) & 1), a.timeout_ns);
         if (lane == 0 && ok) {
@@ -472,7 +477,7 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
           r->q0 = it.q0; r->qlen = it.qlen; r->klen = it.klen;
           r->tok = it.tok; r->kvh = it.kvh; r->part = it.part; r->key0 = it.key0;
           r->n[0] = it.n[0]; r->n[1] = it.n[1]; r->tail = it.tail;
-          r->alt = it.alt;
+          r->turn = it.turn;
           r->nbm = more ? it.nbm : -1;
           mbar_arrive(b_if + 8 * (i % kPtInfo));
           // tile w of the item (K(0) V(0) K(1) V(1) ...) into the next slot, on the load's barrier, which expects
@@ -557,17 +562,14 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
           if (it.nbm > 0) {
             int page = page_of(0), next = page_of(1);
             codes(0, 0, page);
-            // Q: its buffers are free when the last scores of the previous item are done
+            // Q: its buffer is free when the last scores of the previous item are done
             if (ok && lane == 0 && nq > 0) ok = mbar_wait(b_qe, (uint32_t)((nq - 1) & 1), a.timeout_ns);
             ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
             if (!ok) break;
             if (lane == 0) {
-              const bool two = it.n[1] > 0 && !it.alt;
-              mbar_arrive_expect_tx(b_qf, (it.n[0] > 0 ? qbytes : 0) + (two ? qbytes : 0));
-              for (int t = 0; t < 2; ++t)
-                if (t ? two : it.n[0] > 0)
-                  for (int c = 0; c < PANELS; ++c)
-                    tma_load_3d(sQ + t * TILE + c * PANEL, &mq, 64 * c, it.kvh * p.group, it.q0 + it.tok + t * a.tpt, b_qf);
+              mbar_arrive_expect_tx(b_qf, qbytes);
+              for (int c = 0; c < PANELS; ++c)
+                tma_load_3d(sQ + c * PANEL, &mq, 64 * c, it.kvh * p.group, it.q0 + it.tok, b_qf);
             }
             ++nq;
             for (int j = 0; j < it.nbm && ok; ++j) {
@@ -613,6 +615,7 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
       int sl = 0;                         // slot of the next K / V tile
       uint32_t g = 0, nq = 0, nfix = 0;   // loads of K / V, Q loads and fixed tails so far
       uint32_t nk = 0, nv = 0;            // tiles of K and of V (cache)
+      bool begun = false;                 // the item's first scores have been issued under the item before
       uint32_t np[2] = {0, 0}, no[2] = {0, 0};  // P blocks and outputs of each tile so far
       auto scores = [&](int t, int slot, int tq) {  // S_t = Q_tq K^T
         const uint64_t qd = q_desc + (uint64_t)(tq * (TILE >> 4)), kd = k_desc + (uint64_t)(slot * (TILE >> 4));
@@ -632,7 +635,7 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
         const volatile PromptItem* r = ring + i % kPtInfo;
         const int nbm = __shfl_sync(0xffffffffu, r->nbm, 0), n0 = __shfl_sync(0xffffffffu, r->n[0], 0);
         const int n1 = __shfl_sync(0xffffffffu, r->n[1], 0), tail = __shfl_sync(0xffffffffu, r->tail, 0);
-        const bool alt = BITS > 0 && __shfl_sync(0xffffffffu, r->alt, 0) != 0;
+        const int turn = BITS > 0 ? __shfl_sync(0xffffffffu, r->turn, 0) : 0;
         if (lane == 0) item_done(i);
         __syncwarp();
         if (nbm < 0) break;
@@ -660,11 +663,12 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
               if (t) ++no[1]; else ++no[0];
             }
           };
-          auto k_there = [&]() {
+          // S_t = Q K^T with the next K, whose slot is free when they are there; an item's last ones free Q
+          auto next_scores = [&](int t, bool end) {
             ok = ok && wait(b_full + 8 * (nk % KS), (nk / KS) & 1);
+            if (!ok) return;
             tc_fence_after();
-          };
-          auto k_used = [&](bool end) {  // the next K's slot is free when its scores are there; the item's last ones free Q
+            scores(t, nk % KS, 0);
             if (elect_one()) {
               umma_commit(b_empty + 8 * (nk % KS));
               if (end) umma_commit(b_qe);
@@ -672,42 +676,32 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
             __syncwarp();
             ++nk;
           };
-          ok = wait(b_qf, nq & 1);
-          ++nq;
-          // Scores of block j + 1 (of block 0 for j = -1) by tile: tiles that alternate take the other one's columns, and the
-          // scores and their softmax run before P(j) is there (P(j - 1) has been waited for, so S(j - 1) has been read)
-          for (int j = -1; j < nbm; ++j) {
-            const bool more = j + 1 < nbm;
+          if (!begun) {
+            ok = wait(b_qf, nq++ & 1);
+            next_scores(turn, nbm == 1);
+          }
+          begun = false;
+          for (int j = 0; j < nbm && ok; ++j) {
             if (lane == 0) *beat = *beat + 1;
             __syncwarp();
-            // heads of 128: P lies over S, so a tile's next scores come after its product
-            const bool early = j < 0 || alt || SEP;
-            if (more) k_there();
-            if (more && early) {
-#pragma unroll 1
-              for (int t = 0; t < 2; ++t) {
-                if (!ok || (alt ? t != ((j + 1) & 1) : j + 1 >= (t ? n1 : n0))) continue;
-                if (SEP && !alt && j >= 0) {  // S(j) is in the softmax's registers
-                  ok = wait(b_sf + 8 * t, (t ? np[1] : np[0]) & 1);
-                  tc_fence_after();
-                }
-                if (ok) scores(t, nk % KS, alt ? 0 : t);
+            // S(j + 1), or the next item's S(0), in the other tile's columns: its softmax runs before P(j) is there. (The
+            // other tile's last weights have been waited for, so its last scores have been read.)
+            const int t = (j + turn) & 1;
+            if (j + 1 < nbm) {
+              next_scores(1 - t, j + 2 == nbm);
+            } else {
+              ok = __all_sync(0xffffffffu, item_wait(i + 1));
+              const int xn = __shfl_sync(0xffffffffu, ring[(i + 1) % kPtInfo].nbm, 0);
+              if (ok && xn > 0) {
+                ok = wait(b_qf, nq++ & 1);
+                next_scores(1 - t, xn == 1);
+                begun = true;
               }
-              if (ok) k_used(j + 2 == nbm);
             }
-            if (!ok) break;
-            if (j < 0) continue;
-            ok = wait(b_full + 8 * (KS + nv % VS), (nv / VS) & 1);
+            ok = ok && wait(b_full + 8 * (KS + nv % VS), (nv / VS) & 1);
             if (!ok) break;
             tc_fence_after();
-#pragma unroll 1
-            for (int t = 0; t < 2; ++t) {
-              const int nt = t ? n1 : n0;
-              if (!ok || (alt ? t != (j & 1) : j >= nt)) continue;
-              product(t, alt ? j < 2 : j == 0, alt ? j + 2 >= nbm : j + 1 == nt);
-              if (ok && !early && j + 1 < nt) scores(t, nk % KS, t);
-            }
-            if (ok && more && !early) k_used(j + 2 == nbm);
+            product(t, j < 2, j + 2 >= nbm);
             if (!ok) break;
             if (elect_one()) umma_commit(b_empty + 8 * (KS + nv % VS));
             __syncwarp();
@@ -828,7 +822,7 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
     const uint32_t ts = tmem + 128 * t + ((uint32_t)(32 * q4) << 16), to = tmem + 256 + OC * t + ((uint32_t)(32 * q4) << 16);
     const uint32_t tp = SEP ? tmem + 384 + 64 * t + ((uint32_t)(32 * q4) << 16) : ts;
     int ns = 0, no = 0;  // score blocks and commits of O (per block when SEP, else per item) so far
-    uint32_t bs = 0, nalt = 0;  // blocks and items shared by the tiles so far (cache)
+    uint32_t bs = 0, nhalf = 0;  // blocks so far, items of more blocks than one that the tiles took turns on (cache)
     bool ok = true;
     for (int i = 0; ok; ++i) {
       ok = __all_sync(0xffffffffu, item_wait(i));
@@ -836,21 +830,35 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
       const volatile PromptItem* it = ring + i % kPtInfo;
       if (it->nbm < 0) break;
       const int nt = it->n[t], qlen = it->qlen, klen = it->klen, key0 = it->key0, nbm = it->nbm;
-      const bool alt = BITS > 0 && it->alt != 0;
-      const int tok = it->tok + (alt ? 0 : t) * a.tpt + rtok, head = it->kvh * p.group + rhead;
+      const int turn = it->turn;
+      const int tok = it->tok + (BITS ? 0 : t) * a.tpt + rtok, head = it->kvh * p.group + rhead;
       const int out_row = it->q0 + tok;
       const int part = it->part;
       __syncwarp();
       if (lane == 0) item_done(i);
       const bool mine = rtok < a.tpt && tok < qlen;
       const int lim = (p.causal ? min(klen, klen - qlen + tok + 1) : klen) - key0;  // keys of this part the row sees
+      const bool idle = BITS && !__any_sync(0xffffffffu, mine);
       float m = -INFINITY, top = -INFINITY, l = 0.f;  // top: the score at which m moves
       for (int i = 0; i < nt; ++i) {
-        const int j = alt ? 2 * i + t : i;
+        const int j = BITS ? 2 * i + ((t + turn) & 1) : i;
         ok = __all_sync(0xffffffffu, mbar_wait(b_s + 8 * t, (uint32_t)(ns & 1), a.timeout_ns));
         if (!ok) break;
         ++ns;
         tc_fence_after();
+        if (BITS && idle) {  // no row of this warp is one of the item's: whatever P holds there stays there
+          if (SEP) {
+            if (lane == 0) mbar_arrive(b_sf + 8 * t);
+            if (i > 0) ok = __all_sync(0xffffffffu, mbar_wait(b_o + 8 * t, (uint32_t)((no - 1) & 1), a.timeout_ns));
+            if (!ok) break;
+            ++no;
+          }
+          if (lane == 0) {
+            mbar_arrive(b_p + 8 * t);
+            mbar_arrive(b_p + 16 + 8 * t);
+          }
+          continue;
+        }
         uint32_t v[4][32];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, v[c]);
@@ -980,12 +988,16 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
       }
       tc_fence_after();
       const bool whole = p.splits == 1 && !p.sums;
-      if (BITS && alt && t == 1) {  // its sums and O, in the same lanes of tensor memory, are tile 0's to finish
-        *reinterpret_cast<volatile float*>(smem + pt_off_alt<HD, BITS>() + 8 * r) = m;
-        *reinterpret_cast<volatile float*>(smem + pt_off_alt<HD, BITS>() + 8 * r + 4) = l;
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(b_alt);
+      if (BITS && t != (nbm > 0 ? (nbm - 1 + turn) & 1 : 0)) {  // the other one, with the last block, finishes the rows
+        if (nt > 0) {  // this one's sums, and O in the same lanes of tensor memory, are for it to take
+          volatile float* sums = reinterpret_cast<volatile float*>(smem + pt_off_half<HD, BITS>() + 1024 * (nhalf & 1) + 8 * r);
+          sums[0] = m;
+          sums[1] = l;
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(b_half + 8 * (nhalf & 1));
+          ++nhalf;
+        }
         continue;
       }
       float own = 1.f, own1 = 0.f;  // what O (and tile 1's) is multiplied by before the division
@@ -993,13 +1005,13 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
       const long long row0 = (long long)out_row * p.n_q + head, hop = (long long)p.tq * p.n_q;
       const float2* pre_stat = reinterpret_cast<const float2*>(a.pre_stat) + row0;
       float ref = m;
-      if (BITS && alt) {
-        ok = __all_sync(0xffffffffu, mbar_wait(b_alt, (uint32_t)(nalt & 1), a.timeout_ns));
+      if (BITS && nbm > 1) {
+        ok = __all_sync(0xffffffffu, mbar_wait(b_half + 8 * (nhalf & 1), (uint32_t)(nhalf / 2 & 1), a.timeout_ns));
         if (!ok) break;
-        ++nalt;
         tc_fence_after();
-        const float m1 = *reinterpret_cast<volatile float*>(smem + pt_off_alt<HD, BITS>() + 8 * r);
-        const float l1 = *reinterpret_cast<volatile float*>(smem + pt_off_alt<HD, BITS>() + 8 * r + 4);
+        const volatile float* other = reinterpret_cast<volatile float*>(smem + pt_off_half<HD, BITS>() + 1024 * (nhalf & 1) + 8 * r);
+        const float m1 = other[0], l1 = other[1];
+        ++nhalf;
         ref = fmaxf(m, m1);
         merge = true;
         own = m == -INFINITY ? 0.f : ex2(m - ref);
@@ -1036,7 +1048,7 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
             tmem_ld32(to + 64 * c + 32 * h, o);
             if (BITS && merge) {
               uint32_t x[32];
-              tmem_ld32(to + OC + 64 * c + 32 * h, x);
+              tmem_ld32(to + (t ? 0u - OC : OC) + 64 * c + 32 * h, x);
               tmem_wait_ld();
 #pragma unroll
               for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * own + __uint_as_float(x[e]) * own1);
@@ -1048,7 +1060,7 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
               __syncwarp();
               if (lane == 0) {
                 mbar_arrive(b_of + 8 * t);
-                if (BITS && merge) mbar_arrive(b_of + 8);
+                if (BITS && merge) mbar_arrive(b_of + 8 - 8 * t);
               }
             }
           }
