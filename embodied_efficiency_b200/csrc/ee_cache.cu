@@ -12,7 +12,6 @@
 // place is looked up (a search over the offsets and one entry of the table).
 #include "ee_cache.cuh"
 #include "ee_host.h"
-#include "ee_quant.cuh"
 
 namespace ee {
 
@@ -28,14 +27,34 @@ struct CacheCopyArgs {
 
 constexpr int kCacheWarps = 4;
 
-// Codes of eight values: 8 bytes, or 4 with two codes each.
+// Divisions by Markstein's correction of a quotient with its remainder (IBM J.
+// Res. Dev. 34, 1990): q' = q + (v - q s) / s in two fused operations, rounded as
+// the division rounds -- for every 16-bit value under every 16-bit largest value,
+// all of which the tests go through.
 template <int BITS>
-EE_DEV uint2 cache_codes(const float (&f)[8], float s, uint64_t inv2) {
+EE_DEV float cache_step(float amax) {
+  constexpr float MOST = BITS == 8 ? 127.f : 7.f, INV = 1.f / MOST;
+  const float q = amax * INV;
+  return fmaxf(fmaf(fmaf(-q, MOST, amax), INV, q), 1e-8f);
+}
+// Nearest integers (ties to even) of the quotients of eight values and s: 8
+// bytes, or 4 with two codes each.
+template <int BITS>
+EE_DEV uint2 cache_codes(const uint64_t (&v)[4], float s) {
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+  inv = fmaf(fmaf(-s, inv, 1.f), inv, inv);
+  const uint64_t inv2 = both(inv), neg2 = both(-s), magic = both(12582912.f);  // 1.5 * 2^23: the sum's rounding is rint
+  uint32_t b[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint64_t q = mul2f(v[i], inv2);
+    unpack64(add2f(fma2f(fma2f(q, neg2, v[i]), inv2, q), magic), b[2 * i], b[2 * i + 1]);
+  }
   uint32_t w[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h)
-    w[h] = quant_word(pack64(__float_as_uint(f[4 * h]), __float_as_uint(f[4 * h + 1])),
-                      pack64(__float_as_uint(f[4 * h + 2]), __float_as_uint(f[4 * h + 3])), s, inv2);
+    w[h] = prmt(prmt(b[4 * h], b[4 * h + 1], 0x0040u), prmt(b[4 * h + 2], b[4 * h + 3], 0x0040u), 0x5410u);
   if (BITS == 8) return make_uint2(w[0], w[1]);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -44,104 +63,133 @@ EE_DEV uint2 cache_codes(const float (&f)[8], float s, uint64_t inv2) {
   }
   return make_uint2(prmt(w[0], w[1], 0x6420u), 0u);
 }
+// Larger magnitude of the halves of two words by themselves, NaN if either is
+template <typename T> EE_DEV uint32_t max_abs2(uint32_t a, uint32_t b);
+template <> EE_DEV uint32_t max_abs2<__nv_bfloat16>(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("{\n\t.reg .b32 x, y;\n\tabs.bf16x2 x, %1;\n\tabs.bf16x2 y, %2;\n\tmax.NaN.bf16x2 %0, x, y;\n\t}" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <> EE_DEV uint32_t max_abs2<__half>(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("{\n\t.reg .b32 x, y;\n\tabs.f16x2 x, %1;\n\tabs.f16x2 y, %2;\n\tmax.NaN.f16x2 %0, x, y;\n\t}" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
 
 template <typename T, int HD, int BITS>
 __global__ void __launch_bounds__(kCacheWarps * 32) cache_write_kernel(const __grid_constant__ CacheCopyArgs a) {
-  constexpr int CH = HD / 8, HL = 32 / CH, UN = 4;  // lanes a head, heads at once, of them in flight
+  constexpr int CH = HD / 8, HL = 32 / CH, UN = 2;  // lanes a head, heads at once, of them (K and V) in flight
+  constexpr int RB = HD * BITS / 8;
   pdl_entry();
   const int lane = threadIdx.x & 31, c = lane % CH;
   const long long tt = (long long)blockIdx.x * kCacheWarps + (threadIdx.x >> 5);
   if (tt >= a.tokens) return;
-  const int t = (int)tt, heads = 2 * a.c.n_kv;
-  long long row = -1;
-  for (int h0 = 0; h0 < heads; h0 += UN * HL) {
-    uint4 x[UN];
+  const int t = (int)tt;
+  const T* ks = reinterpret_cast<const T*>(a.k) + t * a.k_tok + (lane / CH) * a.k_head + 8 * c;
+  const T* vs = reinterpret_cast<const T*>(a.v) + t * a.v_tok + (lane / CH) * a.v_head + 8 * c;
+  long long at = -1;  // this lane's row of codes
+#pragma unroll 1
+  for (int h0 = 0; h0 < a.c.n_kv; h0 += UN * HL) {
+    uint4 x[UN][2];
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
-      const int h = h0 + u * HL + lane / CH;
-      x[u] = make_uint4(0, 0, 0, 0);
-      if (h < heads) {
-        const T* src = h < a.c.n_kv ? reinterpret_cast<const T*>(a.k) + t * a.k_tok + h * a.k_head
-                                    : reinterpret_cast<const T*>(a.v) + t * a.v_tok + (h - a.c.n_kv) * a.v_head;
-        x[u] = *reinterpret_cast<const uint4*>(src + 8 * c);
+      x[u][0] = x[u][1] = make_uint4(0, 0, 0, 0);
+      if (h0 + u * HL + lane / CH < a.c.n_kv) {
+        x[u][0] = *reinterpret_cast<const uint4*>(ks);
+        x[u][1] = *reinterpret_cast<const uint4*>(vs);
       }
+      ks += HL * a.k_head;
+      vs += HL * a.v_head;
     }
-    if (h0 == 0) {
-      row = cache_place(a.c, a.cu, cache_seq(a.cu, a.c.n_seq, t), t);
+    if (h0 == 0) {  // under the first loads
+      const long long row = cache_place(a.c, a.cu, cache_seq(a.cu, a.c.n_seq, t), t);
       if (row < 0) return;
+      at = row + ((long long)(lane / CH) << a.c.shift);
     }
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
-      const int h = h0 + u * HL + lane / CH;
-      const uint32_t xw[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
-      uint32_t mx = 0;  // 15-bit magnitudes as integers: an infinity or NaN wins
+      if (h0 + u * HL >= a.c.n_kv) break;
+      uint32_t mx[2];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) mx = __vmaxu2(mx, xw[e] & 0x7FFF7FFFu);
-      mx = max(mx & 0xFFFFu, mx >> 16);
+      for (int i = 0; i < 2; ++i)
+        mx[i] = max_abs2<T>(max_abs2<T>(x[u][i].x, x[u][i].y), max_abs2<T>(x[u][i].z, x[u][i].w));
+      uint32_t m = max_abs2<T>(prmt(mx[0], mx[1], 0x5410u), prmt(mx[0], mx[1], 0x7632u));  // K's and V's
 #pragma unroll
-      for (int o = 1; o < CH; o <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      if (h >= heads) continue;
-      const float amax = Act<T>::unpack2(mx).x;
-      const bool finite = amax <= 3.4028234e38f;
-      const float s = fmaxf(__fdiv_rn(amax, BITS == 8 ? 127.f : 7.f), 1e-8f);
-      float f[8];
+      for (int o = 1; o < CH; o <<= 1) m = max_abs2<T>(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const float2 amax = Act<T>::unpack2(m);
+      const bool have = h0 + u * HL + lane / CH < a.c.n_kv;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 p = Act<T>::unpack2(xw[e]);
-        f[2 * e] = finite ? p.x : 0.f;
-        f[2 * e + 1] = finite ? p.y : 0.f;
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t w[4] = {x[u][i].x, x[u][i].y, x[u][i].z, x[u][i].w};
+        const bool finite = (i ? amax.y : amax.x) <= 3.4028234e38f;  // false for infinities and NaN
+        const float s = cache_step<BITS>(i ? amax.y : amax.x);
+        uint64_t v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 p = Act<T>::unpack2(w[e]);
+          v[e] = pack64(__float_as_uint(p.x), __float_as_uint(p.y));
+        }
+        uint2 codes = cache_codes<BITS>(v, s);
+        if (!finite) codes = make_uint2(0, 0);
+        if (!have) continue;
+        uint8_t* dst = reinterpret_cast<uint8_t*>(i ? a.v_codes : a.k_codes) + at * RB + c * BITS;
+        if (BITS == 8) *reinterpret_cast<uint2*>(dst) = codes;
+        else *reinterpret_cast<uint32_t*>(dst) = codes.x;
+        if (c == 0) (i ? a.v_steps : a.k_steps)[at] = finite ? s : __int_as_float(0x7fffffff);
       }
-      const uint2 codes = cache_codes<BITS>(f, s, both(finite ? __frcp_rn(s) : 0.f));
-      const bool isk = h < a.c.n_kv;
-      const long long r = row + ((long long)(isk ? h : h - a.c.n_kv) << a.c.shift);
-      uint8_t* dst = reinterpret_cast<uint8_t*>(isk ? a.k_codes : a.v_codes) + r * (HD * BITS / 8) + c * BITS;
-      if (BITS == 8) *reinterpret_cast<uint2*>(dst) = codes;
-      else *reinterpret_cast<uint32_t*>(dst) = codes.x;
-      if (c == 0) (isk ? a.k_steps : a.v_steps)[r] = finite ? s : __int_as_float(0x7fffffff);
+      at += (long long)HL << a.c.shift;
     }
   }
 }
 
 template <typename T, int HD, int BITS>
 __global__ void __launch_bounds__(kCacheWarps * 32) cache_read_kernel(const __grid_constant__ CacheCopyArgs a) {
-  constexpr int CH = HD / 8, HL = 32 / CH, UN = 4;
+  constexpr int CH = HD / 8, HL = 32 / CH, UN = 2, RB = HD * BITS / 8;
   pdl_entry();
   const int lane = threadIdx.x & 31, c = lane % CH;
   const long long tt = (long long)blockIdx.x * kCacheWarps + (threadIdx.x >> 5);
   if (tt >= a.tokens) return;
-  const int t = (int)tt, heads = 2 * a.c.n_kv;
+  const int t = (int)tt;
   const long long row = cache_place(a.c, a.cu, cache_seq(a.cu, a.c.n_seq, t), t);
   if (row < 0) return;
-  for (int h0 = lane / CH; h0 < heads; h0 += UN * HL) {
-    uint2 w[UN];
-    float s[UN];
+  long long at = row + ((long long)(lane / CH) << a.c.shift);
+  T* kd = reinterpret_cast<T*>(a.k) + t * a.k_tok + (lane / CH) * a.k_head + 8 * c;
+  T* vd = reinterpret_cast<T*>(a.v) + t * a.v_tok + (lane / CH) * a.v_head + 8 * c;
+#pragma unroll 1
+  for (int h = lane / CH; h < a.c.n_kv; h += UN * HL) {
+    uint2 w[UN][2];
+    float s[UN][2];
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
-      const int h = h0 + u * HL;
-      if (h >= heads) continue;
-      const bool isk = h < a.c.n_kv;
-      const long long r = row + ((long long)(isk ? h : h - a.c.n_kv) << a.c.shift);
-      const uint8_t* src = reinterpret_cast<const uint8_t*>(isk ? a.k_codes : a.v_codes) + r * (HD * BITS / 8) + c * BITS;
-      if (BITS == 8) w[u] = *reinterpret_cast<const uint2*>(src);
-      else w[u] = make_uint2(*reinterpret_cast<const uint32_t*>(src), 0u);
-      s[u] = (isk ? a.k_steps : a.v_steps)[r];
+      if (h + u * HL >= a.c.n_kv) continue;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(i ? a.v_codes : a.k_codes) + at * RB + c * BITS;
+        if (BITS == 8) w[u][i] = *reinterpret_cast<const uint2*>(src);
+        else w[u][i] = make_uint2(*reinterpret_cast<const uint32_t*>(src), 0u);
+        s[u][i] = (i ? a.v_steps : a.k_steps)[at];
+      }
+      at += (long long)HL << a.c.shift;
     }
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
-      const int h = h0 + u * HL;
-      if (h >= heads) continue;
-      float f[8];
+      if (h + u * HL >= a.c.n_kv) continue;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        int q;  // the code, sign-extended
-        if (BITS == 8) q = (int)((e < 4 ? w[u].x : w[u].y) << (24 - 8 * (e % 4))) >> 24;
-        else q = (int)(w[u].x << (28 - 4 * e)) >> 28;
-        f[e] = (float)q * s[u];
+      for (int i = 0; i < 2; ++i) {
+        uint32_t o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {  // codes as fp16, exact
+          const uint32_t x = BITS == 8 && e > 1 ? w[u][i].y : w[u][i].x;
+          const float2 f =
+              Act<__half>::unpack2(BITS == 8 ? code_pair8<__half>(x ^ 0x80808080u, e & 1) : code_pair4<__half>(x, x >> 4, e));
+          uint32_t y0, y1;
+          unpack64(mul2f(pack64(__float_as_uint(f.x), __float_as_uint(f.y)), both(s[u][i])), y0, y1);
+          o[e] = Act<T>::pack2(__uint_as_float(y0), __uint_as_float(y1));
+        }
+        *reinterpret_cast<uint4*>(i ? vd : kd) = make_uint4(o[0], o[1], o[2], o[3]);
       }
-      T* dst = h < a.c.n_kv ? reinterpret_cast<T*>(a.k) + t * a.k_tok + h * a.k_head
-                            : reinterpret_cast<T*>(a.v) + t * a.v_tok + (h - a.c.n_kv) * a.v_head;
-      *reinterpret_cast<uint4*>(dst + 8 * c) = make_uint4(Act<T>::pack2(f[0], f[1]), Act<T>::pack2(f[2], f[3]),
-                                                          Act<T>::pack2(f[4], f[5]), Act<T>::pack2(f[6], f[7]));
+      kd += HL * a.k_head;
+      vd += HL * a.v_head;
     }
   }
 }

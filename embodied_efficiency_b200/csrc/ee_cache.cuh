@@ -10,6 +10,8 @@
 // whose page number the cache does not have, holds no key.
 #pragma once
 
+#include <type_traits>
+
 #include "ee_common.cuh"
 
 namespace ee {
@@ -35,8 +37,7 @@ EE_DEV int cache_seq(const int* cu, int n_seq, int t) {
   while (n > 1) {
     const int step = (n + 31) / 32, i = lo + lane * step;
     const unsigned below = __ballot_sync(0xffffffffu, i < lo + n && (lane == 0 || __ldg(cu + i) <= t));
-    const int hit = 31 - __clz(below);
-    const int end = lo + n;
+    const int hit = 31 - __clz(below), end = lo + n;
     lo += hit * step;
     n = min(step, end - lo);
   }
@@ -51,5 +52,23 @@ EE_DEV long long cache_place(const CacheView& c, const int* cu, int b, int t) {
   if (key < 0 || (key >> c.shift) >= c.width) return -1;
   return cache_row(c, __ldg(c.table + b * c.table_row + (key >> c.shift)), (int)(key & ((1 << c.shift) - 1)));
 }
+
+// Two signed 4-bit codes of a word, byte `p`, or two 8-bit ones of bytes 2p and
+// 2p + 1, as 16-bit values: exact, for 8 bits in bf16 a 64th of it (bf16's
+// numbers below 2^-126 take a byte as it is, times 2^-133; one multiplication by
+// 2^127 and the sum take it to where it belongs, where an exponent OR-ed above
+// it has seven bits only and takes three instructions).
+template <typename T> EE_DEV uint32_t code_pair8(uint32_t flipped, int p);  // of a word with its sign bits flipped
+template <> EE_DEV uint32_t code_pair8<__half>(uint32_t w, int p) {
+  return fma2<__half>(prmt(w, 0x64u, p ? 0x4342u : 0x4140u), 0x3C003C00u, 0xE480E480u);
+}
+template <> EE_DEV uint32_t code_pair8<__nv_bfloat16>(uint32_t w, int p) {
+  return fma2<__nv_bfloat16>(prmt(w, 0u, p ? 0x4342u : 0x4140u), 0x7F007F00u, 0xC000C000u);
+}
+template <typename T> EE_DEV uint32_t code_pair4(uint32_t w, uint32_t w_shr4, int p) {
+  return fma2<T>(nib_pair<T>(w, w_shr4, p, 0x00080008u), Act<T>::kOne2, std::is_same<T, __half>::value ? 0xE408E408u : 0xC308C308u);
+}
+// what code_pair8 leaves out
+template <typename T, int BITS> EE_DEV constexpr float code_unit() { return BITS == 8 && !std::is_same<T, __half>::value ? 64.f : 1.f; }
 
 }  // namespace ee

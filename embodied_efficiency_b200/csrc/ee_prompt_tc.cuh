@@ -219,24 +219,6 @@ EE_DEV float max3(float a, float b, float c) {
   return r;
 }
 
-// Two signed 4-bit codes of a word, byte `p`, or two 8-bit ones of bytes 2p and
-// 2p + 1, as 16-bit values: exact, for 8 bits in bf16 a 64th of it (bf16's
-// numbers below 2^-126 take a byte as it is, times 2^-133; one multiplication by
-// 2^127 and the sum take it to where it belongs, where an exponent OR-ed above
-// it has seven bits only and takes three instructions).
-template <typename T> EE_DEV uint32_t code_pair8(uint32_t flipped, int p);  // of a word with its sign bits flipped
-template <> EE_DEV uint32_t code_pair8<__half>(uint32_t w, int p) {
-  return fma2<__half>(prmt(w, 0x64u, p ? 0x4342u : 0x4140u), 0x3C003C00u, 0xE480E480u);
-}
-template <> EE_DEV uint32_t code_pair8<__nv_bfloat16>(uint32_t w, int p) {
-  return fma2<__nv_bfloat16>(prmt(w, 0u, p ? 0x4342u : 0x4140u), 0x7F007F00u, 0xC000C000u);
-}
-template <typename T> EE_DEV uint32_t code_pair4(uint32_t w, uint32_t w_shr4, int p) {
-  return fma2<T>(nib_pair<T>(w, w_shr4, p, 0x00080008u), Act<T>::kOne2, std::is_same<T, __half>::value ? 0xE408E408u : 0xC308C308u);
-}
-// what code_pair8 leaves out
-template <typename T, int BITS> EE_DEV constexpr float code_unit() { return BITS == 8 && !std::is_same<T, __half>::value ? 64.f : 1.f; }
-
 // BITS 0: K and V of 16 bits. 8 or 4: codes from a paged cache. TMA brings them
 // into a ring, 128 keys at a time; warps 10 and 11 turn them into 16-bit tiles in
 // the slots, exactly, and hand on the steps: a key's step multiplies its column

@@ -68,15 +68,12 @@ EE_DEV void norm_weights(const void* w, int w32, int at, float (&r)[8]) {
   }
 }
 
-template <typename T, int HD, bool NORM>
-__global__ void __launch_bounds__(kRotWarps * 32) rotary_kernel(const __grid_constant__ RotaryArgs a) {
-  constexpr int HALF = HD / 2, CH = HALF / 8;  // 8-pair chunks per head
-  constexpr int HL = 32 / CH;                  // heads a warp turns at once
-  constexpr int PP = HALF >= 32 ? HALF / 32 : 1;
-  pdl_entry();
+// Sines and cosines of token t's pairs 8 c .. 8 c + 7, c = lane % (hd / 16): each
+// lane evaluates hd / 64 pairs, the warp exchanges them.
+template <int HD>
+EE_DEV void rotary_angles(const RotaryArgs& a, long long t, float (&sv)[8], float (&cv)[8]) {
+  constexpr int HALF = HD / 2, CH = HALF / 8, PP = HALF >= 32 ? HALF / 32 : 1;
   const int lane = threadIdx.x & 31;
-  const long long t = (long long)blockIdx.x * kRotWarps + (threadIdx.x >> 5);
-  if (t >= a.tokens) return;
   // this lane's pairs lane * PP ..
   float sn[PP], cs[PP];
 #pragma unroll
@@ -95,7 +92,6 @@ __global__ void __launch_bounds__(kRotWarps * 32) rotary_kernel(const __grid_con
     }
   }
   const int c = lane % CH;
-  float sv[8], cv[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const int src = (8 * c + e) / PP;
@@ -107,17 +103,28 @@ __global__ void __launch_bounds__(kRotWarps * 32) rotary_kernel(const __grid_con
       cv[e] = __shfl_sync(0xffffffffu, cs[e % PP], src);
     }
   }
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kRotWarps * 32) rotary_kernel(const __grid_constant__ RotaryArgs a) {
+  constexpr int HALF = HD / 2, CH = HALF / 8;  // 8-pair chunks per head
+  constexpr int HL = 32 / CH;                  // heads a warp turns at once
+  pdl_entry();
+  const int lane = threadIdx.x & 31;
+  const long long t = (long long)blockIdx.x * kRotWarps + (threadIdx.x >> 5);
+  if (t >= a.tokens) return;
+  const int c = lane % CH;
+  float sv[8], cv[8];
+  rotary_angles<HD>(a, t, sv, cv);
   const int lo = a.interleaved ? 16 * c : 8 * c, hi = a.interleaved ? lo + 8 : lo + HALF;
-  float wl[NORM ? 8 : 1], wh[NORM ? 8 : 1];  // this lane's weights
-  // heads h0, h0 + HL, ... below `heads`; with a norm all of the queries or all of the keys, by the whole warp
-  auto turn_heads = [&](int h0, int heads, auto un) {
+  const int heads = a.n_q + a.n_kv;
+  auto turn_heads = [&](int h0, auto un) {
     constexpr int UN = decltype(un)::value;
     uint4 x[UN], y[UN];
     T* dst[UN];
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
       const int h = h0 + u * HL;
-      if (NORM) x[u] = y[u] = make_uint4(0, 0, 0, 0);
       if (h < heads) {
         const bool isq = h < a.n_q;
         const T* src = isq ? reinterpret_cast<const T*>(a.q) + t * a.q_tok + h * a.q_head
@@ -130,40 +137,10 @@ __global__ void __launch_bounds__(kRotWarps * 32) rotary_kernel(const __grid_con
     }
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
-      if (!NORM && h0 + u * HL >= heads) continue;
+      if (h0 + u * HL >= heads) continue;
       const uint32_t xw[4] = {x[u].x, x[u].y, x[u].z, x[u].w}, yw[4] = {y[u].x, y[u].y, y[u].z, y[u].w};
       uint32_t xo[4], yo[4];
-      if constexpr (NORM) {
-        float f[8], g[8], sum = 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 p = Act<T>::unpack2(xw[e]), q = Act<T>::unpack2(yw[e]);
-          f[2 * e] = p.x; f[2 * e + 1] = p.y;
-          g[2 * e] = q.x; g[2 * e + 1] = q.y;
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum = fmaf(f[e], f[e], fmaf(g[e], g[e], sum));
-#pragma unroll
-        for (int o = 1; o < CH; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (h0 + u * HL >= heads) continue;
-        const float r = rsqrtf(fmaf(sum, 1.f / HD, a.eps));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          f[e] *= r * wl[e];
-          g[e] *= r * wh[e];
-        }
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          if (a.interleaved) {
-            xo[e / 2] = Act<T>::pack2(f[e] * cv[e / 2] - f[e + 1] * sv[e / 2], f[e] * sv[e / 2] + f[e + 1] * cv[e / 2]);
-            yo[e / 2] = Act<T>::pack2(g[e] * cv[4 + e / 2] - g[e + 1] * sv[4 + e / 2],
-                                      g[e] * sv[4 + e / 2] + g[e + 1] * cv[4 + e / 2]);
-          } else {
-            xo[e / 2] = Act<T>::pack2(f[e] * cv[e] - g[e] * sv[e], f[e + 1] * cv[e + 1] - g[e + 1] * sv[e + 1]);
-            yo[e / 2] = Act<T>::pack2(f[e] * sv[e] + g[e] * cv[e], f[e + 1] * sv[e + 1] + g[e + 1] * cv[e + 1]);
-          }
-        }
-      } else      if (a.interleaved) {
+      if (a.interleaved) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float2 f = Act<T>::unpack2(xw[e]), g = Act<T>::unpack2(yw[e]);
@@ -182,18 +159,96 @@ __global__ void __launch_bounds__(kRotWarps * 32) rotary_kernel(const __grid_con
       *reinterpret_cast<uint4*>(dst[u] + hi) = make_uint4(yo[0], yo[1], yo[2], yo[3]);
     }
   };
-  if constexpr (NORM) {
+  for (int h0 = lane / CH; h0 < heads; h0 += 3 * HL) turn_heads(h0, std::integral_constant<int, 3>{});
+}
+
+// The same behind a norm of each head. Queries and keys by turns, as their
+// weights differ; a warp's pass is HL heads, UN passes in flight, with packed
+// pairs of fp32 throughout (65537 tokens, 16 + 8 heads of 64: XX us).
+template <typename T, int HD>
+__global__ void __launch_bounds__(kRotWarps * 32, 6) norm_rotary_kernel(const __grid_constant__ RotaryArgs a) {
+  constexpr int HALF = HD / 2, CH = HALF / 8, HL = 32 / CH, UN = 2;
+  pdl_entry();
+  const int lane = threadIdx.x & 31, c = lane % CH;
+  const long long t = (long long)blockIdx.x * kRotWarps + (threadIdx.x >> 5);
+  if (t >= a.tokens) return;
+  const int lo = a.interleaved ? 16 * c : 8 * c, hi = a.interleaved ? lo + 8 : lo + HALF;
+  float sv[8], cv[8];
+  bool angles = false;
+#pragma unroll 1
+  for (int part = 0; part < 2; ++part) {  // queries, keys
+    const int heads = part ? a.n_kv : a.n_q;
+    const long long head = part ? a.k_head : a.q_head, out_head = part ? a.ko_head : a.qo_head;
+    const T* src = reinterpret_cast<const T*>(part ? a.k : a.q) + t * (part ? a.k_tok : a.q_tok) + (lane / CH) * head;
+    T* dst = reinterpret_cast<T*>(part ? a.ko : a.qo) + t * (part ? a.ko_tok : a.qo_tok) + (lane / CH) * out_head;
+    float wl[8], wh[8];
+#pragma unroll 1
+    for (int h0 = 0; h0 < heads; h0 += UN * HL) {
+      uint4 x[UN], y[UN];
 #pragma unroll
-    for (int part = 0; part < 2; ++part) {  // queries, keys
-      const int first = part ? a.n_q : 0, end = part ? a.n_q + a.n_kv : a.n_q;
-      if (first == end) continue;
-      norm_weights<T>(part ? a.kw : a.qw, a.w32, lo, wl);
-      norm_weights<T>(part ? a.kw : a.qw, a.w32, hi, wh);
-      for (int h = first; h < end; h += 3 * HL) turn_heads(h + lane / CH, end, std::integral_constant<int, 3>{});
+      for (int u = 0; u < UN; ++u) {
+        x[u] = y[u] = make_uint4(0, 0, 0, 0);
+        if (h0 + u * HL + lane / CH < heads) {
+          x[u] = *reinterpret_cast<const uint4*>(src + u * HL * head + lo);
+          y[u] = *reinterpret_cast<const uint4*>(src + u * HL * head + hi);
+        }
+      }
+      if (h0 == 0) {  // under the first loads
+        norm_weights<T>(part ? a.kw : a.qw, a.w32, lo, wl);
+        norm_weights<T>(part ? a.kw : a.qw, a.w32, hi, wh);
+        if (!angles) rotary_angles<HD>(a, t, sv, cv);
+        angles = true;
+      }
+#pragma unroll
+      for (int u = 0; u < UN; ++u) {
+        if (h0 + u * HL >= heads) break;
+        const uint32_t xw[4] = {x[u].x, x[u].y, x[u].z, x[u].w}, yw[4] = {y[u].x, y[u].y, y[u].z, y[u].w};
+        uint64_t f[4], g[4], sum2 = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 p = Act<T>::unpack2(xw[e]), q = Act<T>::unpack2(yw[e]);
+          f[e] = pack64(__float_as_uint(p.x), __float_as_uint(p.y));
+          g[e] = pack64(__float_as_uint(q.x), __float_as_uint(q.y));
+          sum2 = fma2f(f[e], f[e], fma2f(g[e], g[e], sum2));
+        }
+        uint32_t s0, s1;
+        unpack64(sum2, s0, s1);
+        float sum = __uint_as_float(s0) + __uint_as_float(s1);
+#pragma unroll
+        for (int o = 1; o < CH; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const uint64_t r2 = both(rsqrtf(fmaf(sum, 1.f / HD, a.eps)));
+        uint32_t xo[4], yo[4];
+        auto pair = [](float u, float v) { return pack64(__float_as_uint(u), __float_as_uint(v)); };
+        auto round2 = [](uint64_t v) {
+          uint32_t u0, u1;
+          unpack64(v, u0, u1);
+          return Act<T>::pack2(__uint_as_float(u0), __uint_as_float(u1));
+        };
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          f[e] = mul2f(mul2f(f[e], r2), pair(wl[2 * e], wl[2 * e + 1]));
+          g[e] = mul2f(mul2f(g[e], r2), pair(wh[2 * e], wh[2 * e + 1]));
+          if (a.interleaved) {  // pairs (a, b) of one angle: (a, b) cos + (b, a) (-sin, sin)
+            uint32_t u0, u1;
+            unpack64(f[e], u0, u1);
+            xo[e] = round2(fma2f(pack64(u1, u0), pair(-sv[e], sv[e]), mul2f(f[e], both(cv[e]))));
+            unpack64(g[e], u0, u1);
+            yo[e] = round2(fma2f(pack64(u1, u0), pair(-sv[4 + e], sv[4 + e]), mul2f(g[e], both(cv[4 + e]))));
+          } else {
+            const uint64_t cs = pair(cv[2 * e], cv[2 * e + 1]), sn = pair(sv[2 * e], sv[2 * e + 1]);
+            const uint64_t ns = pair(-sv[2 * e], -sv[2 * e + 1]);
+            xo[e] = round2(fma2f(g[e], ns, mul2f(f[e], cs)));
+            yo[e] = round2(fma2f(f[e], sn, mul2f(g[e], cs)));
+          }
+        }
+        if (h0 + u * HL + lane / CH < heads) {
+          *reinterpret_cast<uint4*>(dst + u * HL * out_head + lo) = make_uint4(xo[0], xo[1], xo[2], xo[3]);
+          *reinterpret_cast<uint4*>(dst + u * HL * out_head + hi) = make_uint4(yo[0], yo[1], yo[2], yo[3]);
+        }
+      }
+      src += UN * HL * head;
+      dst += UN * HL * out_head;
     }
-  } else {
-    const int heads = a.n_q + a.n_kv;
-    for (int h0 = lane / CH; h0 < heads; h0 += 3 * HL) turn_heads(h0, heads, std::integral_constant<int, 3>{});
   }
 }
 
@@ -202,10 +257,10 @@ static int launch_rotary(const RotaryArgs& a, int hd, cudaStream_t s) {
   const unsigned grid = (unsigned)((a.tokens + kRotWarps - 1) / kRotWarps);
   cudaError_t e = cudaErrorInvalidValue;
   switch (hd) {
-    case 32: e = launch_pdl(rotary_kernel<T, 32, NORM>, dim3(grid), dim3(kRotWarps * 32), 0, s, a); break;
-    case 64: e = launch_pdl(rotary_kernel<T, 64, NORM>, dim3(grid), dim3(kRotWarps * 32), 0, s, a); break;
-    case 128: e = launch_pdl(rotary_kernel<T, 128, NORM>, dim3(grid), dim3(kRotWarps * 32), 0, s, a); break;
-    case 256: e = launch_pdl(rotary_kernel<T, 256, NORM>, dim3(grid), dim3(kRotWarps * 32), 0, s, a); break;
+    case 32: e = launch_pdl(NORM ? norm_rotary_kernel<T, 32> : rotary_kernel<T, 32>, dim3(grid), dim3(kRotWarps * 32), 0, s, a); break;
+    case 64: e = launch_pdl(NORM ? norm_rotary_kernel<T, 64> : rotary_kernel<T, 64>, dim3(grid), dim3(kRotWarps * 32), 0, s, a); break;
+    case 128: e = launch_pdl(NORM ? norm_rotary_kernel<T, 128> : rotary_kernel<T, 128>, dim3(grid), dim3(kRotWarps * 32), 0, s, a); break;
+    case 256: e = launch_pdl(NORM ? norm_rotary_kernel<T, 256> : rotary_kernel<T, 256>, dim3(grid), dim3(kRotWarps * 32), 0, s, a); break;
   }
   return e == cudaSuccess ? EE_OK : EE_ERR_LAUNCH;
 }

@@ -137,6 +137,57 @@ def test_extreme_values(cuda, bits, dtype):
     assert torch.equal(s.isnan(), ~x.float().abs().amax(-1).isfinite())
 
 
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dtype", DT)
+def test_every_largest_value(cuda, bits, dtype):
+    """Heads with each of the type's finite magnitudes as their largest, and values at and beside the borders between
+    codes under it: steps and codes are those of the true divisions."""
+    from embodied_efficiency_b200 import KVCache, cache_write
+    bitsets = torch.arange(1 << 15, dtype=torch.int32, device=cuda).to(torch.int16).view(dtype)
+    amax = bitsets[bitsets.float().isfinite()]
+    n = len(amax)
+    most = 2 ** (bits - 1) - 1
+    half = (torch.arange(63, device=cuda) % most + 0.5) / most  # borders, rounded to the type: on either side of them
+    x = (amax.float()[:, None] * torch.cat([torch.ones(1, device=cuda), half])).to(dtype)[:, None]
+    x[:, 0, 33:] *= -1
+    pages = -(-n // 256)
+    cache = KVCache.empty(pages, 1, 64, 256, bits)
+    table = torch.arange(pages, dtype=torch.int32, device=cuda)[None]
+    cache_write(cache, x, -x, offsets([n], cuda), table, torch.tensor([n], dtype=torch.int32, device=cuda))
+    c, s = quantized(x, bits)
+    assert torch.equal(codes_of(cache.k, bits).flatten(0, 2)[:n], c[:, 0])
+    assert torch.equal(codes_of(cache.v, bits).flatten(0, 2)[:n], -c[:, 0])
+    assert torch.equal(cache.k_scale.flatten()[:n], s[:, 0])
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dtype", DT)
+def test_every_quotient(cuda, bits, dtype):
+    """Every value of the type under every largest one, but for powers of two: all significands of the largest value (at
+    one exponent, and where the step is held at 1e-8), and under each all values that do not round to a code of 0."""
+    from embodied_efficiency_b200 import KVCache, cache_write
+    fi = torch.finfo(dtype)
+    sig = torch.arange(1, 2, fi.eps, device=cuda, dtype=torch.float64)  # significands
+    low = 12 if bits == 8 else 7  # a value 2^-low of the largest is below half a code
+    for scale in (1.0, 2.0 ** -21):
+        under = torch.cat([sig * 2.0 ** -e for e in range(low)] + [sig * 0])
+        pad = -len(under) % 63
+        under = torch.cat([under, under.new_zeros(pad)]).view(-1, 63) * scale
+        for part in sig.split(64):
+            top = part * scale
+            x = torch.minimum(under[None].expand(len(top), -1, -1), top[:, None, None])  # none above its largest
+            x = torch.cat([top[:, None, None].expand(-1, under.shape[0], 1), x], -1).flatten(0, 1).to(dtype)[:, None]
+            n = len(x)
+            pages = -(-n // 256)
+            cache = KVCache.empty(pages, 1, 64, 256, bits)
+            table = torch.arange(pages, dtype=torch.int32, device=cuda)[None]
+            cache_write(cache, x, -x, offsets([n], cuda), table, torch.tensor([n], dtype=torch.int32, device=cuda))
+            c, s = quantized(x, bits)
+            assert torch.equal(codes_of(cache.k, bits).flatten(0, 2)[:n], c[:, 0])
+            assert torch.equal(codes_of(cache.v, bits).flatten(0, 2)[:n], -c[:, 0])
+            assert torch.equal(cache.v_scale.flatten()[:n], s[:, 0])
+
+
 def test_what_the_device_says_is_not_trusted(cuda):
     """Page numbers, offsets and lengths outside the cache and the tensors: nothing outside is touched, rows without a
     place stay, the others are right."""
