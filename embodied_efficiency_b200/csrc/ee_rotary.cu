@@ -48,31 +48,24 @@ struct RotaryArgs {
 
 constexpr int kRotWarps = 4;
 
-// eight weights as fp32
+// four weights as fp32
 template <typename T>
-EE_DEV void norm_weights(const void* w, int w32, int at, float (&r)[8]) {
+EE_DEV void norm_weights(const void* w, int w32, int at, float (&r)[4]) {
   if (w32) {
-    const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(w) + at);
-    const float4 x = __ldg(p), y = __ldg(p + 1);
+    const float4 x = __ldg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(w) + at));
     r[0] = x.x; r[1] = x.y; r[2] = x.z; r[3] = x.w;
-    r[4] = y.x; r[5] = y.y; r[6] = y.z; r[7] = y.w;
   } else {
-    const uint4 x = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(w) + at));
-    const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 f = Act<T>::unpack2(xw[e]);
-      r[2 * e] = f.x;
-      r[2 * e + 1] = f.y;
-    }
+    const uint2 x = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const T*>(w) + at));
+    const float2 f = Act<T>::unpack2(x.x), g = Act<T>::unpack2(x.y);
+    r[0] = f.x; r[1] = f.y; r[2] = g.x; r[3] = g.y;
   }
 }
 
-// Sines and cosines of token t's pairs 8 c .. 8 c + 7, c = lane % (hd / 16): each
-// lane evaluates hd / 64 pairs, the warp exchanges them.
-template <int HD>
-EE_DEV void rotary_angles(const RotaryArgs& a, long long t, float (&sv)[8], float (&cv)[8]) {
-  constexpr int HALF = HD / 2, CH = HALF / 8, PP = HALF >= 32 ? HALF / 32 : 1;
+// Sines and cosines of token t's pairs N c .. N c + N - 1, c = lane % (hd / 2 N):
+// each lane evaluates hd / 64 pairs, the warp exchanges them.
+template <int HD, int N>
+EE_DEV void rotary_angles(const RotaryArgs& a, long long t, float (&sv)[N], float (&cv)[N]) {
+  constexpr int HALF = HD / 2, CH = HALF / N, PP = HALF >= 32 ? HALF / 32 : 1;
   const int lane = threadIdx.x & 31;
   // this lane's pairs lane * PP ..
   float sn[PP], cs[PP];
@@ -93,8 +86,8 @@ EE_DEV void rotary_angles(const RotaryArgs& a, long long t, float (&sv)[8], floa
   }
   const int c = lane % CH;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int src = (8 * c + e) / PP;
+  for (int e = 0; e < N; ++e) {
+    const int src = (N * c + e) / PP;
     if (PP == 1) {
       sv[e] = __shfl_sync(0xffffffffu, sn[0], src);
       cv[e] = __shfl_sync(0xffffffffu, cs[0], src);
@@ -115,7 +108,7 @@ __global__ void __launch_bounds__(kRotWarps * 32) rotary_kernel(const __grid_con
   if (t >= a.tokens) return;
   const int c = lane % CH;
   float sv[8], cv[8];
-  rotary_angles<HD>(a, t, sv, cv);
+  rotary_angles<HD, 8>(a, t, sv, cv);
   const int lo = a.interleaved ? 16 * c : 8 * c, hi = a.interleaved ? lo + 8 : lo + HALF;
   const int heads = a.n_q + a.n_kv;
   auto turn_heads = [&](int h0, auto un) {
@@ -163,52 +156,73 @@ __global__ void __launch_bounds__(kRotWarps * 32) rotary_kernel(const __grid_con
 }
 
 // The same behind a norm of each head. Queries and keys by turns, as their
-// weights differ; a warp's pass is HL heads, UN passes in flight, with packed
-// pairs of fp32 throughout (65537 tokens, 16 + 8 heads of 64: XX us).
+// weights differ, the weights multiplied into the turn's coefficients once for a
+// token. A lane has four pairs of a head (8-byte loads): with eight, as above,
+// the coefficients leave 20 warps an SM and 80 us where these take 69 (65537
+// tokens, 16 + 8 heads of 64; 5.8 TB/s); UN passes of HL heads are in flight.
 template <typename T, int HD>
-__global__ void __launch_bounds__(kRotWarps * 32, 6) norm_rotary_kernel(const __grid_constant__ RotaryArgs a) {
-  constexpr int HALF = HD / 2, CH = HALF / 8, HL = 32 / CH, UN = 2;
+__global__ void __launch_bounds__(kRotWarps * 32, 8) norm_rotary_kernel(const __grid_constant__ RotaryArgs a) {
+  constexpr int HALF = HD / 2, CH = HALF / 4, HL = 32 / CH, UN = 4;
   pdl_entry();
   const int lane = threadIdx.x & 31, c = lane % CH;
   const long long t = (long long)blockIdx.x * kRotWarps + (threadIdx.x >> 5);
   if (t >= a.tokens) return;
-  const int lo = a.interleaved ? 16 * c : 8 * c, hi = a.interleaved ? lo + 8 : lo + HALF;
-  float sv[8], cv[8];
+  const int lo = a.interleaved ? 8 * c : 4 * c, hi = a.interleaved ? lo + 4 : lo + HALF;
+  float sv[4], cv[4];
   bool angles = false;
+  auto pair = [](float u, float v) { return pack64(__float_as_uint(u), __float_as_uint(v)); };
 #pragma unroll 1
   for (int part = 0; part < 2; ++part) {  // queries, keys
     const int heads = part ? a.n_kv : a.n_q;
     const long long head = part ? a.k_head : a.q_head, out_head = part ? a.ko_head : a.qo_head;
     const T* src = reinterpret_cast<const T*>(part ? a.k : a.q) + t * (part ? a.k_tok : a.q_tok) + (lane / CH) * head;
     T* dst = reinterpret_cast<T*>(part ? a.ko : a.qo) + t * (part ? a.ko_tok : a.qo_tok) + (lane / CH) * out_head;
-    float wl[8], wh[8];
+    // the turn with the weights in it, for two values of x or y at once: x' = x A + x~ B, y' = y D + y~ C, where x~ is y
+    // and the other way round, or (interleaved) the neighbour
+    uint64_t A[2], B[2], C[2], D[2];
 #pragma unroll 1
     for (int h0 = 0; h0 < heads; h0 += UN * HL) {
-      uint4 x[UN], y[UN];
+      uint2 x[UN], y[UN];
 #pragma unroll
       for (int u = 0; u < UN; ++u) {
-        x[u] = y[u] = make_uint4(0, 0, 0, 0);
+        x[u] = y[u] = make_uint2(0, 0);
         if (h0 + u * HL + lane / CH < heads) {
-          x[u] = *reinterpret_cast<const uint4*>(src + u * HL * head + lo);
-          y[u] = *reinterpret_cast<const uint4*>(src + u * HL * head + hi);
+          x[u] = *reinterpret_cast<const uint2*>(src + lo);
+          y[u] = *reinterpret_cast<const uint2*>(src + hi);
         }
+        src += HL * head;
       }
       if (h0 == 0) {  // under the first loads
+        float wl[4], wh[4];
         norm_weights<T>(part ? a.kw : a.qw, a.w32, lo, wl);
         norm_weights<T>(part ? a.kw : a.qw, a.w32, hi, wh);
-        if (!angles) rotary_angles<HD>(a, t, sv, cv);
+        if (!angles) rotary_angles<HD, 4>(a, t, sv, cv);
         angles = true;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (a.interleaved) {
+            A[e] = pair(wl[2 * e] * cv[e], wl[2 * e + 1] * cv[e]);
+            B[e] = pair(-wl[2 * e + 1] * sv[e], wl[2 * e] * sv[e]);
+            D[e] = pair(wh[2 * e] * cv[2 + e], wh[2 * e + 1] * cv[2 + e]);
+            C[e] = pair(-wh[2 * e + 1] * sv[2 + e], wh[2 * e] * sv[2 + e]);
+          } else {
+            A[e] = pair(wl[2 * e] * cv[2 * e], wl[2 * e + 1] * cv[2 * e + 1]);
+            B[e] = pair(-wh[2 * e] * sv[2 * e], -wh[2 * e + 1] * sv[2 * e + 1]);
+            D[e] = pair(wh[2 * e] * cv[2 * e], wh[2 * e + 1] * cv[2 * e + 1]);
+            C[e] = pair(wl[2 * e] * sv[2 * e], wl[2 * e + 1] * sv[2 * e + 1]);
+          }
+        }
       }
 #pragma unroll
       for (int u = 0; u < UN; ++u) {
         if (h0 + u * HL >= heads) break;
-        const uint32_t xw[4] = {x[u].x, x[u].y, x[u].z, x[u].w}, yw[4] = {y[u].x, y[u].y, y[u].z, y[u].w};
-        uint64_t f[4], g[4], sum2 = 0;
+        const uint32_t xw[2] = {x[u].x, x[u].y}, yw[2] = {y[u].x, y[u].y};
+        uint64_t f[2], g[2], sum2 = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 2; ++e) {
           const float2 p = Act<T>::unpack2(xw[e]), q = Act<T>::unpack2(yw[e]);
-          f[e] = pack64(__float_as_uint(p.x), __float_as_uint(p.y));
-          g[e] = pack64(__float_as_uint(q.x), __float_as_uint(q.y));
+          f[e] = pair(p.x, p.y);
+          g[e] = pair(q.x, q.y);
           sum2 = fma2f(f[e], f[e], fma2f(g[e], g[e], sum2));
         }
         uint32_t s0, s1;
@@ -216,38 +230,43 @@ __global__ void __launch_bounds__(kRotWarps * 32, 6) norm_rotary_kernel(const __
         float sum = __uint_as_float(s0) + __uint_as_float(s1);
 #pragma unroll
         for (int o = 1; o < CH; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const uint64_t r2 = both(rsqrtf(fmaf(sum, 1.f / HD, a.eps)));
-        uint32_t xo[4], yo[4];
-        auto pair = [](float u, float v) { return pack64(__float_as_uint(u), __float_as_uint(v)); };
-        auto round2 = [](uint64_t v) {
+        float r;  // the mean is at least eps, no subnormal number
+        asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(sum, 1.f / HD, a.eps)));
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          f[e] = mul2f(f[e], both(r));
+          g[e] = mul2f(g[e], both(r));
+        }
+        uint32_t xo[2], yo[2];
+        auto turned = [&](uint64_t own, uint64_t other, uint64_t c1, uint64_t c2) {
           uint32_t u0, u1;
-          unpack64(v, u0, u1);
+          unpack64(fma2f(own, c1, mul2f(other, c2)), u0, u1);
           return Act<T>::pack2(__uint_as_float(u0), __uint_as_float(u1));
         };
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          f[e] = mul2f(mul2f(f[e], r2), pair(wl[2 * e], wl[2 * e + 1]));
-          g[e] = mul2f(mul2f(g[e], r2), pair(wh[2 * e], wh[2 * e + 1]));
-          if (a.interleaved) {  // pairs (a, b) of one angle: (a, b) cos + (b, a) (-sin, sin)
+        if (a.interleaved) {
+          auto swapped = [](uint64_t v) {
             uint32_t u0, u1;
-            unpack64(f[e], u0, u1);
-            xo[e] = round2(fma2f(pack64(u1, u0), pair(-sv[e], sv[e]), mul2f(f[e], both(cv[e]))));
-            unpack64(g[e], u0, u1);
-            yo[e] = round2(fma2f(pack64(u1, u0), pair(-sv[4 + e], sv[4 + e]), mul2f(g[e], both(cv[4 + e]))));
-          } else {
-            const uint64_t cs = pair(cv[2 * e], cv[2 * e + 1]), sn = pair(sv[2 * e], sv[2 * e + 1]);
-            const uint64_t ns = pair(-sv[2 * e], -sv[2 * e + 1]);
-            xo[e] = round2(fma2f(g[e], ns, mul2f(f[e], cs)));
-            yo[e] = round2(fma2f(f[e], sn, mul2f(g[e], cs)));
+            unpack64(v, u0, u1);
+            return pack64(u1, u0);
+          };
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            xo[e] = turned(f[e], swapped(f[e]), A[e], B[e]);
+            yo[e] = turned(g[e], swapped(g[e]), D[e], C[e]);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            xo[e] = turned(f[e], g[e], A[e], B[e]);
+            yo[e] = turned(g[e], f[e], D[e], C[e]);
           }
         }
         if (h0 + u * HL + lane / CH < heads) {
-          *reinterpret_cast<uint4*>(dst + u * HL * out_head + lo) = make_uint4(xo[0], xo[1], xo[2], xo[3]);
-          *reinterpret_cast<uint4*>(dst + u * HL * out_head + hi) = make_uint4(yo[0], yo[1], yo[2], yo[3]);
+          *reinterpret_cast<uint2*>(dst + lo) = make_uint2(xo[0], xo[1]);
+          *reinterpret_cast<uint2*>(dst + hi) = make_uint2(yo[0], yo[1]);
         }
+        dst += HL * out_head;
       }
-      src += UN * HL * head;
-      dst += UN * HL * out_head;
     }
   }
 }
