@@ -45,7 +45,7 @@ static CacheParts cache_parts(const CachePlan& p, long long tq, int n_q, int n_k
   CacheParts c{0, 0, 0};
   if (prefix_len) c.pre_splits = prompt_sums_splits(tq, prefix_len, n_q, n_kv);
   c.pre = c.pre_splits * tq * n_q;
-  if (p.nt == 0) c.own = p.splits > 1 ? p.splits * tq * n_q : 0;
+  if (p.nt == 0) c.own = p.splits > 1 || prefix_len ? p.splits * tq * n_q : 0;
   else c.own = (long long)device_sms() * plan_workers(p, hd, bits) * 2 * 8 * p.nt + (prefix_len ? tq * n_q : 0);
   return c;
 }
@@ -162,14 +162,11 @@ int ee_cache_attention(const ee_cache* cache, const void* q, int64_t q_tok, int6
   p.n_seq = n_seq;
   p.causal = causal != 0;
   p.splits = plan.splits;
-  const bool whole = plan.splits == 1;  // rows are finished where they are summed, the prefix's sums added
+  const bool whole = plan.splits == 1 && !prefix_len;  // rows are finished where they are summed
   p.sums = !whole;
   p.part = part + cp.pre * hd;
   p.stat = stat + cp.pre * 2;
   t.p = p;
-  t.pre_part = part;
-  t.pre_stat = stat;
-  t.pre_splits = whole ? cp.pre_splits : 0;
   t.tpt = 128 / p.group;
   t.status = status;
   t.timeout_ns = kCacheWaitNs;

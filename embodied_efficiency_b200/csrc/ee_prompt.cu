@@ -399,8 +399,28 @@ static size_t prompt_ws_bytes(const PromptPlan& pl, long long tq, int n_q, int h
   return (size_t)prompt_partials(pl, tq, n_q, hd) * (hd + 2) * 4;
 }
 
+// The same with a warp per (token, head), for few parts: a CTA's barriers cost
+// more than its width saves (6400 tokens, 16 heads of 128, two parts: XX us
+// where a CTA a row took 410).
+constexpr int kPrFewParts = 16;
+template <typename T, int HD>
+__global__ void __launch_bounds__(kPrJoin) prompt_combine_few_kernel(const __grid_constant__ PromptArgs a) {
+  pdl_entry();
+  const long long at = (long long)blockIdx.x * (kPrJoin / 32) + (threadIdx.x >> 5), step = (long long)a.tq * a.n_q;
+  if (at >= step) return;
+  const int tok = (int)(at / a.n_q), h = (int)(at - (long long)tok * a.n_q);
+  if (tok < __ldg(a.cu_q) || tok >= __ldg(a.cu_q + a.n_seq)) return;
+  join_row_warp<T, HD>(a.part, a.stat, a.splits, [&](long long i) { return at + i * step; },
+                       reinterpret_cast<T*>(a.out) + (long long)tok * a.o_tok + h * a.o_head);
+}
+
 template <typename T, int HD>
 static int launch_parts(const PromptArgs& a, cudaStream_t s) {
+  const long long ctas = ((long long)a.tq * a.n_q + kPrJoin / 32 - 1) / (kPrJoin / 32);
+  if (a.splits <= kPrFewParts && ctas <= 0x7fffffff)
+    return launch_pdl(prompt_combine_few_kernel<T, HD>, dim3((unsigned)ctas), dim3(kPrJoin), 0, s, a) == cudaSuccess
+               ? EE_OK
+               : EE_ERR_LAUNCH;
   return launch_pdl(prompt_combine_kernel<T, HD>, dim3((unsigned)a.tq, a.n_q), dim3(kPrJoin), 0, s, a) == cudaSuccess
              ? EE_OK
              : EE_ERR_LAUNCH;

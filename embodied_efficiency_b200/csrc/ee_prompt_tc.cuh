@@ -68,8 +68,6 @@ struct PromptTcArgs {
   unsigned long long timeout_ns;
   CacheView c;  // keys and values in a cache
   const float *k_steps, *v_steps;
-  const float *pre_part, *pre_stat;  // sums over a prefix ([pre_splits][tq][n_q]), to be added to whole rows
-  int pre_splits;
 };
 
 // registers: 384 threads launch with 168 each; the four warps of loads and MMAs
@@ -984,9 +982,6 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
       }
       float own = 1.f, own1 = 0.f;  // what O (and tile 1's) is multiplied by before the division
       bool merge = false;
-      const long long row0 = (long long)out_row * p.n_q + head, hop = (long long)p.tq * p.n_q;
-      const float2* pre_stat = reinterpret_cast<const float2*>(a.pre_stat) + row0;
-      float ref = m;
       if (BITS && nbm > 1) {
         ok = __all_sync(0xffffffffu, mbar_wait(b_half + 8 * (nhalf & 1), (uint32_t)(nhalf / 2 & 1), a.timeout_ns));
         if (!ok) break;
@@ -994,26 +989,12 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
         const volatile float* other = reinterpret_cast<volatile float*>(smem + pt_off_half<HD, BITS>() + 1024 * (nhalf & 1) + 8 * r);
         const float m1 = other[0], l1 = other[1];
         ++nhalf;
-        ref = fmaxf(m, m1);
+        const float ref = fmaxf(m, m1);
         merge = true;
         own = m == -INFINITY ? 0.f : ex2(m - ref);
         own1 = m1 == -INFINITY ? 0.f : ex2(m1 - ref);
         l = l * own + l1 * own1;
         m = ref;
-      }
-      if (BITS && a.pre_splits && mine) {
-        for (int i = 0; i < a.pre_splits; ++i) {
-          const float2 x = __ldg(pre_stat + i * hop);
-          if (x.y != 0.f) ref = fmaxf(ref, x.x);
-        }
-        const float f = m == -INFINITY ? 0.f : ex2(m - ref);
-        l *= f;
-        own *= f;
-        own1 *= f;
-        for (int i = 0; i < a.pre_splits; ++i) {
-          const float2 x = __ldg(pre_stat + i * hop);
-          if (x.y != 0.f) l += ex2(x.x - ref) * x.y;
-        }
       }
       const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees no key is zero
       const long long at = ((long long)part * p.tq + out_row) * p.n_q + head;
@@ -1043,26 +1024,6 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
               if (lane == 0) {
                 mbar_arrive(b_of + 8 * t);
                 if (BITS && merge) mbar_arrive(b_of + 8 - 8 * t);
-              }
-            }
-          }
-          if (BITS && a.pre_splits && mine) {
-            if (!merge) {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = nt > 0 ? __float_as_uint(__uint_as_float(o[e]) * own) : 0u;
-            }
-            for (int i = 0; i < a.pre_splits; ++i) {
-              const float2 x = __ldg(pre_stat + i * hop);
-              if (x.y == 0.f) continue;
-              const float f = ex2(x.x - ref);
-              const float4* src = reinterpret_cast<const float4*>(a.pre_part + (row0 + i * hop) * HD + 64 * c + 32 * h);
-#pragma unroll
-              for (int e = 0; e < 32; e += 4) {
-                const float4 y = __ldg(src + e / 4);
-                o[e] = __float_as_uint(fmaf(f, y.x, __uint_as_float(o[e])));
-                o[e + 1] = __float_as_uint(fmaf(f, y.y, __uint_as_float(o[e + 1])));
-                o[e + 2] = __float_as_uint(fmaf(f, y.z, __uint_as_float(o[e + 2])));
-                o[e + 3] = __float_as_uint(fmaf(f, y.w, __uint_as_float(o[e + 3])));
               }
             }
           }
