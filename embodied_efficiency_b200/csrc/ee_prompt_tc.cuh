@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
     }
     for (int i = 0; i < kPtInfo; ++i) {
       mbar_init(b_if + 8 * i, 1);
-      mbar_init(b_ie + 8 * i, BITS ? 13 : 10);  // 8 softmax warps, the MMA warp, the fixing warp or four decoding ones
+      mbar_init(b_ie + 8 * i, BITS ? 14 : 10);  // 8 softmax warps, the MMA warp, the fixing warp or the loading and decoding ones
     }
     mbar_fence_init();
   }
@@ -314,10 +314,20 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
   if (BITS > 0 && warp >= 12) {
     if constexpr (BITS > 0) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PtThreads<BITS>::DECODE));
-      // ---------------- codes into 16-bit tiles, 32 keys of each by a warp ----------------
-      constexpr int RB = HD * BITS / 8, CPR = RB / 16;  // 16-byte pieces of a row
-      const int quarter = warp - 12;
-      uint32_t rt = 0, count[2] = {0, 0};  // tiles of codes, of K and of V so far
+      // ---------------- codes into 16-bit tiles: 32 keys of each by a warp ----------------
+      constexpr int RB = HD * BITS / 8;                    // bytes of a row of codes
+      constexpr int PER_ROW = RB < 64 ? RB / 16 : 4;       // lanes on a row; a row of 128 bytes takes two of its pieces
+      constexpr int ROWS = 32 / PER_ROW, HALVES = RB / 16 / PER_ROW, PIECES = 32 / ROWS * HALVES;
+      constexpr int BATCH = PIECES < 4 ? PIECES : 4;       // pieces under way at once
+      const int quarter = warp - 12, row0 = 32 * quarter + lane / PER_ROW, q0 = lane % PER_ROW;
+      const uint32_t from = sb + pt_off_raw<HD, BITS>() + row0 * RB + q0 * 16;
+      uint32_t to[16 / BITS];  // where the 16-bit pieces of the lane's first piece go
+#pragma unroll
+      for (int k = 0; k < 16 / BITS; ++k) {
+        const int c = q0 * (16 / BITS) + k;
+        to[k] = sKV + (c >> 3) * PANEL + sw128(row0, c & 7);
+      }
+      uint32_t rt = 0, nk = 0, nv = 0;  // tiles of codes, of K and of V so far
       bool ok = true;
       for (int i = 0;; ++i) {
         ok = __all_sync(0xffffffffu, item_wait(i));
@@ -329,20 +339,19 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
         if (nbm < 0) break;
         for (int x = 0; x < 2 * nbm && ok; ++x) {  // K(0) K(1) V(0) K(2) V(1) ... V(nbm - 1)
           const bool isv = x == 2 * nbm - 1 || (x > 0 && (x & 1) == 0);
-          const int j = isv ? (x == 2 * nbm - 1 ? nbm - 1 : x / 2 - 1) : (x + 1) / 2;
-          const uint32_t rs = rt % NR, blk = isv ? count[1] : count[0], slots = isv ? VS : KS, slot = blk % slots;
-          const int at = (isv ? KS : 0) + slot;
+          const uint32_t rs = rt % NR, blk = isv ? nv : nk, slots = isv ? VS : KS, at = isv ? KS + blk % VS : blk % KS;
+          const int j = (x + 1) / 2;  // K's block
           ok = mbar_wait(b_rf + 8 * rs, (rt / NR) & 1, a.timeout_ns);
           // the products of the tile that used the slot before are done
           if (ok && blk >= slots) ok = mbar_wait(b_empty + 8 * at, (blk / slots - 1) & 1, a.timeout_ns);
+          float* steps = reinterpret_cast<float*>(smem + pt_off_steps<HD, BITS>() + (blk % kPtSteps) * 1024);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          const uint32_t raw = sb + pt_off_raw<HD, BITS>() + rs * pt_raw<HD, BITS>(), dst = sKV + at * TILE;
-          float* steps = reinterpret_cast<float*>(smem + pt_off_steps<HD, BITS>() + (blk % kPtSteps) * 1024);
           if (!isv) {
             const float* raw_steps = reinterpret_cast<const float*>(smem + pt_off_rawsteps<HD, BITS>() + rs * 1024);
             const uint32_t there = *reinterpret_cast<volatile uint32_t*>(smem + pt_off_there<HD, BITS>() + kPtSteps * 16 + rs * 4);
-            const int shift = min(a.c.shift, 7), key = 32 * quarter + lane;
+            const int shift = min(a.c.shift, 7);
+            const int key = 32 * quarter + lane;
             const bool have = key0 + j * kPtKeys + key < klen && (there >> (key >> shift) & 1);
             float ks = have ? raw_steps[key] : 0.f, vs = have ? raw_steps[128 + key] : 0.f;
             // a value's step that is no number must reach the rows that see it and no others: as its key's
@@ -358,46 +367,42 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(b_st + 8 * (blk % kPtSteps));
           }
-          constexpr int BATCH = CPR < 4 ? CPR : 4;  // pieces of a lane under way at once
-  #pragma unroll 1
-          for (int e0 = lane; e0 < 32 * CPR; e0 += 32 * BATCH) {
+          const uint32_t raw = from + rs * pt_raw<HD, BITS>(), dst = at * TILE;
+#pragma unroll
+          for (int e0 = 0; e0 < PIECES; e0 += BATCH) {
             uint4 x[BATCH];
-  #pragma unroll
-            for (int u = 0; u < BATCH; ++u) x[u] = lds16(raw + 32 * quarter * RB + (e0 + 32 * u) * 16);
-  #pragma unroll
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u) x[u] = lds16(raw + (e0 + u) / HALVES * (ROWS * RB) + (e0 + u) % HALVES * 64);
+#pragma unroll
             for (int u = 0; u < BATCH; ++u) {
-              const int e = e0 + 32 * u, row = 32 * quarter + e / CPR, q = e % CPR;
-              // heads of 128 in bytes: the upper half's lanes write their two pieces in the other order, so that the eight
-              // lanes of a row reach all banks
-              const int flip = HD * BITS == 1024 ? (q >> 2) & 1 : 0;
-              const uint32_t xw[4] = {flip ? x[u].z : x[u].x, flip ? x[u].w : x[u].y, flip ? x[u].x : x[u].z, flip ? x[u].y : x[u].w};
+              const int e = e0 + u;
+              const uint32_t xw[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
               uint32_t o[64 / BITS];  // pairs
-  #pragma unroll
+#pragma unroll
               for (int k = 0; k < 4; ++k) {
                 if (BITS == 8) {
                   const uint32_t f = xw[k] ^ 0x80808080u;
                   o[2 * k] = code_pair8<T>(f, 0);
                   o[2 * k + 1] = code_pair8<T>(f, 1);
                 } else {
-  #pragma unroll
+#pragma unroll
                   for (int b = 0; b < 4; ++b) o[4 * k + b] = code_pair4<T>(xw[k], xw[k] >> 4, b);
                 }
               }
               if (!VSCALE && isv) {
-                const float s = steps[128 + row];
-  #pragma unroll
+                const float s = steps[128 + row0 + e / HALVES * ROWS];
+#pragma unroll
                 for (int k = 0; k < 64 / BITS; ++k) {
                   const float2 f = Act<T>::unpack2(o[k]);
                   o[k] = Act<T>::pack2(f.x * s, f.y * s);
                 }
               }
-  #pragma unroll
-              for (int k = 0; k < 16 / BITS; ++k) {
-                const int c = q * (16 / BITS) + (HD * BITS == 1024 ? k ^ flip : k);  // 16-byte piece of the 16-bit row
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (c >> 3) * PANEL + sw128(row, c & 7)),
+#pragma unroll
+              for (int k = 0; k < 16 / BITS; ++k)
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to[k] + dst + e / HALVES * (ROWS * 128) +
+                                                                              e % HALVES * PANEL),
                              "r"(o[4 * k]), "r"(o[4 * k + 1]), "r"(o[4 * k + 2]), "r"(o[4 * k + 3])
                              : "memory");
-              }
             }
           }
           fence_proxy_async_smem();
@@ -407,14 +412,14 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
             mbar_arrive(b_full + 8 * at);
           }
           ++rt;
-          if (isv) ++count[1]; else ++count[0];
+          if (isv) ++nv; else ++nk;
         }
         if (!ok) break;
       }
       // the MMA warp's arrivals that say the tiles are used have come
       if (quarter == 0 && lane == 0) {
         for (int v = 0; v < 2; ++v) {
-          const uint32_t slots = v ? VS : KS, n = v ? count[1] : count[0];
+          const uint32_t slots = v ? VS : KS, n = v ? nv : nk;
           for (uint32_t e = n > slots ? n - slots : 0; e < n && ok; ++e)
             ok = mbar_wait(b_empty + 8 * ((v ? KS : 0) + e % slots), (e / slots) & 1, a.timeout_ns);
         }
@@ -424,8 +429,8 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
     }
   } else if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PtThreads<BITS>::REST));
-    if (warp == 8) {
-      // ---------------- items and loads ----------------
+    if (warp == (BITS ? 10 : 8)) {
+      // ---------------- items, and loads but for a cache's ----------------
       bool ok = true;
       int units = 0, n = 0, nq = 0, sl = 0;  // K / V tiles and Q loads issued so far, next slot
       int bs = 0;                            // blocks so far (cache)
@@ -451,10 +456,12 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
           bs += it.nbm;
         }
         if (lane == 0 && i >= kPtInfo)  // the slot's item has been read by all; if not, it stays as it is
-          ok = mbar_wait(b_ie + 8 * (i % kPtInfo), (uint32_t)((i / kPtInfo - 1) & 1), a.timeout_ns);
+          ok = BITS ? wait_walk(b_ie + 8 * (i % kPtInfo), (uint32_t)((i / kPtInfo - 1) & 1))
+                    : mbar_wait(b_ie + 8 * (i % kPtInfo), (uint32_t)((i / kPtInfo - 1) & 1), a.timeout_ns);
         if (lane == 0 && ok) {
           volatile PromptItem* r = ring + i % kPtInfo;
           r->q0 = it.q0; r->qlen = it.qlen; r->klen = it.klen;
+          if (BITS) r->k0 = it.k0;
           r->tok = it.tok; r->kvh = it.kvh; r->part = it.part; r->key0 = it.key0;
           r->n[0] = it.n[0]; r->n[1] = it.n[1]; r->tail = it.tail;
           r->turn = it.turn;
@@ -504,75 +511,10 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
         }
         ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
         if (!more || !ok) break;
-        if constexpr (BITS > 0) {
-          // the tiles' codes, K(0) K(1) V(0) K(2) V(1) ..., in pieces of a page; a block's steps come with its K. A lane per
-          // piece looks its page up, two blocks ahead.
-          const int shift = min(a.c.shift, 7), pieces = kPtKeys >> shift;
-          constexpr uint32_t RB = HD * BITS / 8;
-          auto page_of = [&](int j) {  // of this lane's piece of block j, -1 for none
-            const int key = it.key0 + j * kPtKeys + (lane << shift);
-            if (lane >= pieces || j >= it.nbm || key >= it.klen) return -1;
-            return __ldg(a.c.table + (long long)it.k0 * a.c.table_row + (key >> a.c.shift));
-          };
-          auto codes = [&](int w, int j, int page) {  // K (w = 0) or V of block j
-            const bool there = (unsigned)page < (unsigned)a.c.pages;
-            const uint32_t mask = __ballot_sync(0xffffffffu, there), slot = g % NR;
-            if (lane == 0 && g >= (uint32_t)NR) ok = mbar_wait(b_re + 8 * slot, (g / NR - 1) & 1, a.timeout_ns);
-            ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-            if (!ok) return;
-            const uint32_t bar = b_rf + 8 * slot, dst = sb + pt_off_raw<HD, BITS>() + slot * pt_raw<HD, BITS>();
-            const uint32_t steps = sb + pt_off_rawsteps<HD, BITS>() + slot * 1024;
-            if (lane == 0) {
-              *reinterpret_cast<volatile uint32_t*>(smem + pt_off_there<HD, BITS>() + kPtSteps * 16 + slot * 4) = mask;
-              mbar_arrive_expect_tx(bar, __popc(mask) * ((RB << shift) + (w == 0 ? 8u << shift : 0u)));
-            }
-            __syncwarp();
-            if (there) {
-              const int key = it.key0 + j * kPtKeys + (lane << shift);
-              const int row = ((page * a.c.n_kv + it.kvh) << a.c.shift) + (key & ((1 << a.c.shift) - 1));
-              tma_load_2d(dst + lane * (RB << shift), w ? &mv : &mk, 0, row, bar);
-              if (w == 0) {
-                bulk_load(steps + lane * (4 << shift), a.k_steps + row, 4 << shift, bar);
-                bulk_load(steps + 512 + lane * (4 << shift), a.v_steps + row, 4 << shift, bar);
-              }
-            }
-            __syncwarp();
-            ++g;
-          };
-          if (it.nbm > 0) {
-            int page = page_of(0), next = page_of(1);
-            codes(0, 0, page);
-            // Q: its buffer is free when the last scores of the previous item are done
-            if (ok && lane == 0 && nq > 0) ok = mbar_wait(b_qe, (uint32_t)((nq - 1) & 1), a.timeout_ns);
-            ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-            if (!ok) break;
-            if (lane == 0) {
-              mbar_arrive_expect_tx(b_qf, qbytes);
-              for (int c = 0; c < PANELS; ++c)
-                tma_load_3d(sQ + c * PANEL, &mq, 64 * c, it.kvh * p.group, it.q0 + it.tok, b_qf);
-            }
-            ++nq;
-            for (int j = 0; j < it.nbm && ok; ++j) {
-              const int after = page_of(j + 2);
-              if (j + 1 < it.nbm) codes(0, j + 1, next);
-              if (ok) codes(1, j, page);
-              page = next;
-              next = after;
-            }
-          }
-          if (!ok) break;
-        }
       }
       // everything issued lands before the CTA may exit, whatever has failed; if nothing has, it is used too, and the
       // MMA warp's arrivals that say so have come
-      if (BITS && lane == 0) {
-        bool landed = true;
-        for (uint32_t e = g > (uint32_t)NR ? g - NR : 0; e < g; ++e) landed &= mbar_wait(b_rf + 8 * (e % NR), (e / NR) & 1, kPtDrainNs);
-        if (nq > 0) landed &= mbar_wait(b_qf, (uint32_t)((nq - 1) & 1), kPtDrainNs);
-        ok = ok && landed;
-        if (ok && nq > 0) ok = mbar_wait(b_qe, (uint32_t)((nq - 1) & 1), a.timeout_ns);
-        if (!ok) atomicCAS(a.status, 0, (int)EE_ERR_TIMEOUT);
-      }
+      if (BITS && lane == 0 && !ok) atomicCAS(a.status, 0, (int)EE_ERR_TIMEOUT);
       if (BITS == 0 && lane == 0) {
         const uint32_t e0 = g > NP ? g - NP : 0;
         bool landed = true;
@@ -584,6 +526,107 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
         if (!ok) atomicCAS(a.status, 0, (int)EE_ERR_TIMEOUT);
       }
       __syncwarp();
+    } else if (BITS > 0 && warp == 8) {
+      // ---------------- loads of Q and of the tiles' codes ----------------
+      if constexpr (BITS > 0) {
+      // K(0) K(1) V(0) K(2) V(1) ..., in pieces of a page; a block's steps come with its K. A lane per piece looks its page
+      // up, two blocks and an item ahead.
+      const int shift = min(a.c.shift, 7), pieces = kPtKeys >> shift;
+      constexpr uint32_t RB = HD * BITS / 8;
+      const uint32_t qbytes = (uint32_t)(p.group * a.tpt) * 128u * PANELS;
+      uint32_t g = 0;  // tiles of codes so far
+      int nq = 0;      // loads of Q
+      bool ok = true;
+      struct At {
+        int q0, tok, kvh, k0, klen, key0, nbm;
+      };
+      auto item_at = [&](int i) {
+        At x{0, 0, 0, 0, 0, 0, -1};
+        ok = __all_sync(0xffffffffu, ok && item_wait(i));
+        if (!ok) return x;
+        const volatile PromptItem* r = ring + i % kPtInfo;
+        x = At{r->q0, r->tok, r->kvh, r->k0, r->klen, r->key0, r->nbm};
+        __syncwarp();
+        if (lane == 0) item_done(i);
+        return x;
+      };
+      auto page_of = [&](const At& x, int j) {  // of this lane's piece of block j, -1 for none
+        const int key = x.key0 + j * kPtKeys + (lane << shift);
+        if (lane >= pieces || j >= x.nbm || key >= x.klen) return -1;
+        return __ldg(a.c.table + (long long)x.k0 * a.c.table_row + (key >> a.c.shift));
+      };
+      auto codes = [&](const At& x, int w, int j, int page) {  // K (w = 0) or V of block j
+        const bool there = (unsigned)page < (unsigned)a.c.pages;
+        const uint32_t mask = __ballot_sync(0xffffffffu, there), slot = g % NR;
+        if (g >= (uint32_t)NR) ok = __all_sync(0xffffffffu, ok && mbar_wait(b_re + 8 * slot, (g / NR - 1) & 1, a.timeout_ns));
+        if (!ok) return;
+        const uint32_t bar = b_rf + 8 * slot, dst = sb + pt_off_raw<HD, BITS>() + slot * pt_raw<HD, BITS>();
+        const uint32_t steps = sb + pt_off_rawsteps<HD, BITS>() + slot * 1024;
+        if (lane == 0) {
+          *reinterpret_cast<volatile uint32_t*>(smem + pt_off_there<HD, BITS>() + kPtSteps * 16 + slot * 4) = mask;
+          mbar_arrive_expect_tx(bar, __popc(mask) * ((RB << shift) + (w == 0 ? 8u << shift : 0u)));
+        }
+        __syncwarp();
+        if (there) {
+          const int key = x.key0 + j * kPtKeys + (lane << shift);
+          const int row = ((page * a.c.n_kv + x.kvh) << a.c.shift) + (key & ((1 << a.c.shift) - 1));
+          tma_load_2d(dst + lane * (RB << shift), w ? &mv : &mk, 0, row, bar);
+          if (w == 0) {
+            bulk_load(steps + lane * (4 << shift), a.k_steps + row, 4 << shift, bar);
+            bulk_load(steps + 512 + lane * (4 << shift), a.v_steps + row, 4 << shift, bar);
+          }
+        }
+        __syncwarp();
+        ++g;
+      };
+      At it = item_at(0), nx = it;
+      int page = page_of(it, 0), next = page_of(it, 1), page2 = -1, next2 = -1;
+      for (int i = 0; ok && it.nbm >= 0; ++i) {
+        if (it.nbm == 0) {
+          nx = item_at(i + 1);
+          page2 = page_of(nx, 0);
+          next2 = page_of(nx, 1);
+        }
+        for (int j = 0; j < it.nbm && ok; ++j) {
+          if (j == 0) {
+            codes(it, 0, 0, page);
+            // Q: its buffer is free when the last scores of the previous item are done
+            if (nq > 0) ok = __all_sync(0xffffffffu, ok && mbar_wait(b_qe, (uint32_t)((nq - 1) & 1), a.timeout_ns));
+            if (!ok) break;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(b_qf, qbytes);
+              for (int c = 0; c < PANELS; ++c)
+                tma_load_3d(sQ + c * PANEL, &mq, 64 * c, it.kvh * p.group, it.q0 + it.tok, b_qf);
+            }
+            ++nq;
+          }
+          const int after = page_of(it, j + 2);
+          if (j + 1 < it.nbm) codes(it, 0, j + 1, next);
+          if (j == max(it.nbm - 2, 0)) {  // the next item's first pages, under this one's last loads
+            nx = item_at(i + 1);
+            page2 = page_of(nx, 0);
+            next2 = page_of(nx, 1);
+          }
+          if (ok) codes(it, 1, j, page);
+          page = next;
+          next = after;
+        }
+        it = nx;
+        page = page2;
+        next = next2;
+      }
+      // everything issued lands before the CTA may exit, whatever has failed; if nothing has, it is used too, and the MMA
+      // warp's arrival that says so of Q has come
+      if (lane == 0) {
+        bool landed = true;
+        for (uint32_t e = g > (uint32_t)NR ? g - NR : 0; e < g; ++e) landed &= mbar_wait(b_rf + 8 * (e % NR), (e / NR) & 1, kPtDrainNs);
+        if (nq > 0) landed &= mbar_wait(b_qf, (uint32_t)((nq - 1) & 1), kPtDrainNs);
+        ok = ok && landed;
+        if (ok && nq > 0) ok = mbar_wait(b_qe, (uint32_t)((nq - 1) & 1), a.timeout_ns);
+        if (!ok) atomicCAS(a.status, 0, (int)EE_ERR_TIMEOUT);
+      }
+      __syncwarp();
+      }
     } else if (warp == 9) {
       // ---------------- MMA issue (all lanes run the loops, see elect_one) ----------------
       // The tensor cores queue about two MMAs beyond the running one and a wait costs 100 cycles or more even when
