@@ -144,7 +144,13 @@ int ee_cache_attention(const ee_cache* cache, const void* q, int64_t q_tok, int6
     a.scale_log2 = scale_log2;
     a.k_steps = cache->k_steps; a.v_steps = cache->v_steps;
     a.part = part; a.stat = stat;
+    a.whole = cp.own - (prefix_len ? tq * n_q : 0);
     a.pre_splits = cp.pre_splits;
+    if (prefix_len) {
+      const int tpt = 128 / a.group;
+      const long long items = (tq + 2 * tpt - 1) / (2 * tpt) * n_kv * cp.pre_splits;
+      a.pre_ctas = items < 0x7fffffff ? (int)items : 0x7fffffff;
+    }
     a.status = status;
     a.timeout_ns = kCacheWaitNs;
     if (act_dtype == EE_BF16)

@@ -61,7 +61,9 @@ struct CacheAttnArgs {
   // sums of parts, [hd] each, and their maximum and weight: first of items that a border cuts, by worker ([workers][2]
   // [rows]); behind a prefix then of every whole item's rows ([tq][n_q]) and of the prefix ([pre_splits][tq][n_q])
   float *part, *stat;
+  long long whole;      // the first of the whole items' rows
   int pre_splits;       // 0: no prefix
+  int pre_ctas;         // of the kernel that sums it up
   int* status;
   unsigned long long timeout_ns;
 };
@@ -172,13 +174,20 @@ __global__ void __launch_bounds__(CaShape<HD, BITS, NT>::THREADS, 1)
     for (int i = 0; i < NS; ++i) mbar_init(full + 8 * i, 1);
     mbar_fence_init();
   }
-  pdl_entry();
+  // Behind a prefix the kernel before this one sums that up, from nothing that this one writes and for nothing that it
+  // reads; it has itself waited for everything before the call, so this one need not wait for it but before it ends (the
+  // join follows on this one).
+  if (a.pre_splits) pdl_release();
+  else pdl_entry();
   const int per = (a.c.n_seq + NTH - 1) / NTH;
   const long long total = pr_list<NTH>(a, &sh, per, a.c.n_seq, [](int, const CacheSeq&, long long) {});
   const long long share = pr_share(total, (int)gridDim.x * NWK, kCaMinSteps);
   const long long me = (long long)warp * gridDim.x + blockIdx.x;  // neighbours in the list on different SMs
   const long long first = me * share;
-  if (first >= total) return;
+  if (first >= total) {
+    pdl_wait();
+    return;
+  }
   int left = (int)(total - first < share ? total - first : share);  // steps to go
   CaAt at{};
   {
@@ -195,7 +204,10 @@ __global__ void __launch_bounds__(CaShape<HD, BITS, NT>::THREADS, 1)
       x -= steps;
       at.enter(a, at.b + 1);
     }
-    if (at.b >= a.c.n_seq) return;  // the lengths have changed meanwhile
+    if (at.b >= a.c.n_seq) {  // the lengths have changed meanwhile
+      pdl_wait();
+      return;
+    }
     const int item = (int)pr_div(x, at.per_item);
     at.step = (int)(x - (long long)item * at.per_item);
     at.r0 = item / a.c.n_kv * R;
@@ -494,8 +506,7 @@ __global__ void __launch_bounds__(CaShape<HD, BITS, NT>::THREADS, 1)
                     make_uint2(w, Act<T>::pack2(o[c + 1][j][e] * inv, o[c + 1][j][2 + e] * inv));
             }
           } else {
-            const long long workers = (long long)gridDim.x * NWK;
-            const long long slot = whole ? workers * 2 * R + (long long)(at.s.q0 + tok) * a.n_q + h
+            const long long slot = whole ? a.whole + (long long)(at.s.q0 + tok) * a.n_q + h
                                          : (me * 2 + (head ? 0 : 1)) * R + rr;  // at the share's front, or its end
 #pragma unroll
             for (int c = 0; c < CH; c += BITS == 8 ? 1 : 2) {
@@ -516,6 +527,7 @@ __global__ void __launch_bounds__(CaShape<HD, BITS, NT>::THREADS, 1)
   if (!ok && lane == 0) atomicCAS(a.status, 0, (int)EE_ERR_TIMEOUT);
   // whatever has been issued lands before the CTA ends
   for (int i = done; i < issued; ++i) mbar_wait(full + 8 * (i % NS), (uint32_t)(i / NS & 1), 1000000000ull);
+  pdl_wait();
 }
 
 // The rows whose item a border cut, rows without keys of their own, and behind a
@@ -564,10 +576,10 @@ __global__ void __launch_bounds__(kPrJoin) cache_join_kernel(const __grid_consta
     if (n == 1 && !a.pre_splits) return;  // in one share: written already
     front = w0 * share == first ? 0 : a.rows;  // else the first part is at its share's end
   }
-  const long long rows0 = (long long)most * 2 * a.rows, row = (long long)tok * a.n_q + h, hop = (long long)a.tq * a.n_q;
+  const long long row = (long long)tok * a.n_q + h, hop = (long long)a.tq * a.n_q;
   auto slot = [&](long long i) {
-    if (i >= n) return rows0 + (1 + i - n) * hop + row;  // a part of the prefix
-    if (n == 1) return rows0 + row;
+    if (i >= n) return a.whole + (1 + i - n) * hop + row;  // a part of the prefix
+    if (n == 1) return a.whole + row;
     return (w0 + i) * 2 * a.rows + (i == 0 ? front : 0) + r % a.rows;
   };
   T* out = reinterpret_cast<T*>(a.out) + (long long)tok * a.o_tok + h * a.o_head;
@@ -596,8 +608,9 @@ int launch_cache_rows(const CacheMaps& m, const CacheAttnArgs& a, cudaStream_t s
   auto fn = cache_rows_kernel<T, HD, BITS, NT>;
   static std::atomic<int> set[64];
   allow_max_smem(fn, set);
-  const int sms = device_sms(), most = sms * S::WORKERS;
-  if (launch_pdl(fn, dim3(sms), dim3(S::THREADS), S::SMEM, s, m.k, m.v, a) != cudaSuccess) return EE_ERR_LAUNCH;
+  // beside the prefix's CTAs, where they leave half of the SMs or more
+  const int sms = device_sms(), ctas = a.pre_ctas > 0 && 2 * a.pre_ctas <= sms ? sms - a.pre_ctas : sms, most = ctas * S::WORKERS;
+  if (launch_pdl(fn, dim3(ctas), dim3(S::THREADS), S::SMEM, s, m.k, m.v, a) != cudaSuccess) return EE_ERR_LAUNCH;
   // parts of a row, on average: a CTA per row from 16 on
   const long long blocks = (long long)a.tq * a.group / a.rows;
   const long long items = (blocks > a.c.n_seq ? blocks : a.c.n_seq) * a.c.n_kv;

@@ -246,11 +246,19 @@ EE_DEV uint32_t cl_count() {
 // Kernel entry under programmatic dependent launch (see ee_host.h): wait for
 // the predecessor grids (complete, memory visible), then allow the successor
 // to launch. A no-op for kernels launched without the attribute.
-EE_DEV void pdl_entry() {
+EE_DEV void pdl_wait() {
 #if EE_PDL
   asm volatile("griddepcontrol.wait;" ::: "memory");
+#endif
+}
+EE_DEV void pdl_release() {
+#if EE_PDL
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 #endif
+}
+EE_DEV void pdl_entry() {
+  pdl_wait();
+  pdl_release();
 }
 EE_DEV void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
