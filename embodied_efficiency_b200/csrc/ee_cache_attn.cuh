@@ -78,7 +78,8 @@ EE_DEV CacheSeq list_seq(const CacheAttnArgs& a, int b) {
   s.klen = min(max(__ldg(a.c.k_lens + b), 0), a.c.width << a.c.shift);
   return s;
 }
-constexpr int kCaKeys = 32, kCaMinSteps = 3;  // keys of a step; steps that are worth a worker
+constexpr int kCaKeys = 32, kCaMinSteps = 6;  // keys of a step; steps that are worth a worker (2 x 1
+                                               // token behind 30000, 4 bits: 21.4 us with 3, 19.8 with 6, 20.6 with 10)
 EE_DEV long long list_steps(const CacheAttnArgs& a, const CacheSeq& s, int& per_item) {
   per_item = (s.klen + kCaKeys - 1) / kCaKeys;
   return (((long long)s.qlen * a.group + a.rows - 1) / a.rows) * a.c.n_kv * per_item;

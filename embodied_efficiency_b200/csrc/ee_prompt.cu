@@ -399,35 +399,69 @@ static size_t prompt_ws_bytes(const PromptPlan& pl, long long tq, int n_q, int h
   return (size_t)prompt_partials(pl, tq, n_q, hd) * (hd + 2) * 4;
 }
 
-// The same with a warp per (token, head), for few parts: a CTA's barriers cost
-// more than its width saves (6400 tokens, 16 heads of 128, two parts: XX us
-// where a CTA a row took 410).
+// The same for few parts, with hd / 4 lanes a (token, head), four values a lane,
+// whose loads of four parts do not wait for the weights: a CTA's barriers cost
+// more than its width saves (6400 tokens, 16 heads of 128, two parts: 33 us where
+// a CTA a row took 410).
 constexpr int kPrFewParts = 16;
 template <typename T, int HD>
 __global__ void __launch_bounds__(kPrJoin) prompt_combine_few_kernel(const __grid_constant__ PromptArgs a) {
+  constexpr int LANES = HD / 4, UN = 4;
   pdl_entry();
-  const long long at = (long long)blockIdx.x * (kPrJoin / 32) + (threadIdx.x >> 5), step = (long long)a.tq * a.n_q;
+  const int lane = threadIdx.x % LANES;
+  const long long at = (long long)blockIdx.x * (kPrJoin / LANES) + threadIdx.x / LANES, step = (long long)a.tq * a.n_q;
   if (at >= step) return;
   const int tok = (int)(at / a.n_q), h = (int)(at - (long long)tok * a.n_q);
-  if (tok < __ldg(a.cu_q) || tok >= __ldg(a.cu_q + a.n_seq)) return;
-  join_row_warp<T, HD>(a.part, a.stat, a.splits, [&](long long i) { return at + i * step; },
-                       reinterpret_cast<T*>(a.out) + (long long)tok * a.o_tok + h * a.o_head);
+  const float2* stat = reinterpret_cast<const float2*>(a.stat) + at;
+  const float4* part = reinterpret_cast<const float4*>(a.part + at * HD) + lane;
+  float m = -INFINITY, l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < a.splits; i0 += UN) {
+    float2 st[UN];
+    float4 v[UN];
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < UN; ++i) {
+      const bool there = i0 + i < a.splits;
+      st[i] = there ? __ldg(stat + (i0 + i) * step) : make_float2(-INFINITY, 0.f);
+      v[i] = there ? __ldg(part + (i0 + i) * step * LANES) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int i = 0; i < UN; ++i) top = fmaxf(top, st[i].x);
+    const float u = top == -INFINITY ? 0.f : top, old = exp2f(m - u);
+    m = top;
+    l *= old;
+    acc = make_float4(acc.x * old, acc.y * old, acc.z * old, acc.w * old);
+#pragma unroll
+    for (int i = 0; i < UN; ++i) {
+      if (st[i].y == 0.f) continue;  // a part that has seen no key: its sums need not have been written
+      const float f = exp2f(st[i].x - u);
+      l += f * st[i].y;
+      acc.x += f * v[i].x;
+      acc.y += f * v[i].y;
+      acc.z += f * v[i].z;
+      acc.w += f * v[i].w;
+    }
+  }
+  if (tok < __ldg(a.cu_q) || tok >= __ldg(a.cu_q + a.n_seq)) return;  // rows outside the sequences stay as they were
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees no key is zero
+  *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + (long long)tok * a.o_tok + h * a.o_head + 4 * lane) =
+      make_uint2(Act<T>::pack2(acc.x * inv, acc.y * inv), Act<T>::pack2(acc.z * inv, acc.w * inv));
 }
 
 template <typename T, int HD>
-static int launch_parts(const PromptArgs& a, cudaStream_t s) {
-  const long long ctas = ((long long)a.tq * a.n_q + kPrJoin / 32 - 1) / (kPrJoin / 32);
-  if (a.splits <= kPrFewParts && ctas <= 0x7fffffff)
-    return launch_pdl(prompt_combine_few_kernel<T, HD>, dim3((unsigned)ctas), dim3(kPrJoin), 0, s, a) == cudaSuccess
-               ? EE_OK
-               : EE_ERR_LAUNCH;
-  return launch_pdl(prompt_combine_kernel<T, HD>, dim3((unsigned)a.tq, a.n_q), dim3(kPrJoin), 0, s, a) == cudaSuccess
-             ? EE_OK
-             : EE_ERR_LAUNCH;
+static int launch_parts(const PromptArgs& a, bool few, cudaStream_t s) {
+  constexpr int ROWS = kPrJoin / (HD / 4);
+  const long long ctas = ((long long)a.tq * a.n_q + ROWS - 1) / ROWS;
+  const cudaError_t e =
+      few && a.splits <= kPrFewParts && ctas <= 0x7fffffff
+          ? launch_pdl(prompt_combine_few_kernel<T, HD>, dim3((unsigned)ctas), dim3(kPrJoin), 0, s, a)
+          : launch_pdl(prompt_combine_kernel<T, HD>, dim3((unsigned)a.tq, a.n_q), dim3(kPrJoin), 0, s, a);
+  return e == cudaSuccess ? EE_OK : EE_ERR_LAUNCH;
 }
 template <typename T, int HD>
 static int launch_combine(const PromptArgs& a, cudaStream_t s) {
-  return a.splits == 1 || a.sums ? EE_OK : launch_parts<T, HD>(a, s);
+  return a.splits == 1 || a.sums ? EE_OK : launch_parts<T, HD>(a, false, s);
 }
 
 template <typename T, int HD>
@@ -522,8 +556,8 @@ int prompt_parts(long long tq, int n_seq, int n_q, int n_kv, long long keys, int
 // Joins a.splits parts of every row of a sequence.
 int launch_prompt_combine(const PromptArgs& a, int hd, int act_dtype, cudaStream_t s) {
   if (act_dtype == EE_BF16)
-    return hd == 64 ? launch_parts<__nv_bfloat16, 64>(a, s) : launch_parts<__nv_bfloat16, 128>(a, s);
-  return hd == 64 ? launch_parts<__half, 64>(a, s) : launch_parts<__half, 128>(a, s);
+    return hd == 64 ? launch_parts<__nv_bfloat16, 64>(a, true, s) : launch_parts<__nv_bfloat16, 128>(a, true, s);
+  return hd == 64 ? launch_parts<__half, 64>(a, true, s) : launch_parts<__half, 128>(a, true, s);
 }
 int launch_prompt_sums(const PromptArgs& a, int hd, int act_dtype, cudaStream_t s) {
   if (act_dtype == EE_BF16) return hd == 64 ? launch_tc<__nv_bfloat16, 64>(a, s) : launch_tc<__nv_bfloat16, 128>(a, s);
