@@ -21,6 +21,7 @@ import torch.nn.functional as F
 
 from . import _lib
 from . import fused as _fused
+from .cache import PAGE_SIZES, KVCache, cache_attention, cache_write
 from .prompt import prompt_attention
 from .wq_gemm import wq_linear
 
@@ -206,6 +207,38 @@ class PackedKV:
             cu_q = self._cu_q[n] = torch.arange(0, (b + 1) * n, n, dtype=torch.int32).to(self.cu.device)
         return cu_q
 
+    def attend(self, q: torch.Tensor, b: int, n: int) -> torch.Tensor:
+        """``n`` queries per prefix, q [b * n, heads, head_dim], each against all of its prefix."""
+        return prompt_attention(q, self.k, self.v, self.queries(b, n), self.cu, causal=False)
+
+
+class CachedKV(PackedKV):
+    """The same held as 8- or 4-bit codes: a ``KVCache``, and which of its pages (``table``) and how many keys
+    (``k_lens``) each prefix has."""
+
+    def __init__(self, cache: KVCache, table: torch.Tensor, k_lens: torch.Tensor, cu: torch.Tensor):
+        super().__init__(None, None, cu)
+        self.cache, self.table, self.k_lens = cache, table, k_lens
+
+    def attend(self, q: torch.Tensor, b: int, n: int) -> torch.Tensor:
+        return cache_attention(q, self.cache, self.queries(b, n), self.table, self.k_lens, causal=False)
+
+
+def _prefix_pages(cu: torch.Tensor, tokens: int, page_size: int):
+    """Pages one behind another for prefixes with offsets ``cu``: how many, the table and the lengths. Waits for the
+    offsets: the table's width is the host's to know."""
+    if cu.dim() != 1 or cu.dtype != torch.int32 or cu.numel() < 1:
+        raise ValueError(f"cu must be int32 offsets [batch + 1], got {cu.dtype} {tuple(cu.shape)}")
+    at = cu.cpu()
+    lens = at[1:] - at[:-1]
+    if int(at[0]) != 0 or int(at[-1]) != tokens or (lens < 0).any():
+        raise ValueError(f"cu must rise from 0 to the prefix's {tokens} rows")
+    n = (lens + page_size - 1) // page_size
+    first = n.cumsum(0) - n
+    table = first[:, None] + torch.arange(int(n.max()) if len(n) else 0)
+    table = torch.where(table < (first + n)[:, None], table, -1)
+    return int(n.sum()), table.to(torch.int32).to(cu.device), lens.to(torch.int32).to(cu.device)
+
 
 def _is_packed(prefix_kv) -> bool:
     return len(prefix_kv) > 0 and isinstance(prefix_kv[0], PackedKV)
@@ -255,6 +288,14 @@ class Block(nn.Module):
         k, v = _apply_linear(self.kv_c, prefix).chunk(2, dim=-1)
         return PackedKV(k.unflatten(-1, (self.h, self.hd)), v.unflatten(-1, (self.h, self.hd)), cu)
 
+    def precompute_kv_cached(self, prefix: torch.Tensor, cu: torch.Tensor, bits: int, page_size: int, places) -> CachedKV:
+        """The same into a cache of ``bits``-bit codes, at ``places`` from ``_prefix_pages``."""
+        kv = self.precompute_kv_packed(prefix, cu)
+        pages, table, k_lens = places
+        cache = KVCache.empty(pages, self.h, self.hd, page_size, bits, prefix.device)
+        cache_write(cache, kv.k, kv.v, cu, table, k_lens)
+        return CachedKV(cache, table, k_lens, cu)
+
     def forward(self, x: torch.Tensor, kv_c):
         """Eager GPU composition (used only where the fused launch does not apply)."""
         _lib.require_cuda(x)
@@ -271,8 +312,7 @@ class Block(nn.Module):
             x = _apply_linear(self.proj, a, residual=x)
         qc = _apply_linear(self.q_c, _apply_norm(self.nx, x))
         if isinstance(kv_c, PackedKV):
-            a = prompt_attention(qc.reshape(b * n, self.h, hd), kv_c.k, kv_c.v, kv_c.queries(b, n), kv_c.cu,
-                                 causal=False).view(b, n, d)
+            a = kv_c.attend(qc.reshape(b * n, self.h, hd), b, n).view(b, n, d)
             x = _apply_linear(self.out_c, a, residual=x)
             return _apply_linear(self.mlp[2], _apply_linear(self.mlp[0], _apply_norm(self.n2, x), gelu=True), residual=x)
         k, v = kv_c
@@ -314,12 +354,22 @@ class ActionExpert(nn.Module):
         prefix = prefix.to(self.out_norm.weight.dtype)
         return [blk.precompute_kv(prefix) for blk in self.blocks]
 
-    def encode_packed(self, prefix: torch.Tensor, cu: torch.Tensor):
+    def encode_packed(self, prefix: torch.Tensor, cu: torch.Tensor, kv_bits: int | None = None, page_size: int = 64):
         """Per-layer K/V of prefixes of different lengths: packed rows [tokens, d] and their int32 offsets
         ``cu`` [batch + 1] on the device. ``flow_sample`` and ``GraphedSampler`` take the result in place of
         ``encode``'s and run layer by layer, the cross-attention on ``prompt_attention`` (so heads of 64 or 128, in bf16
-        or fp16)."""
+        or fp16). With ``kv_bits`` 8 or 4 the K/V are held as codes in a ``KVCache`` of ``page_size`` tokens a page per
+        layer (0.53 or 0.28 of the 16-bit bytes with heads of 64, and the unused ends of last pages), the
+        cross-attention then runs on ``cache_attention``; making the table waits for ``cu`` once."""
         prefix = prefix.to(self.out_norm.weight.dtype)
+        if kv_bits is not None:
+            if kv_bits not in (8, 4):
+                raise ValueError(f"kv_bits must be 8, 4 or None, got {kv_bits}")
+            if page_size not in PAGE_SIZES:
+                raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
+            places = _prefix_pages(cu, prefix.shape[0], page_size)
+            with torch.no_grad():  # codes carry no gradient
+                return [blk.precompute_kv_cached(prefix, cu, kv_bits, page_size, places) for blk in self.blocks]
         return [blk.precompute_kv_packed(prefix, cu) for blk in self.blocks]
 
     def plan(self, batch: int, prefix_kv):

@@ -53,6 +53,7 @@ class FleetSampler:
     ``request_fn(i)`` returns request i's (prefix [1, P, d], noise [1, H, A]);
     with an ``expert``, P may differ between the requests of a chunk, whose
     prefixes are then packed without padding (``ActionExpert.encode_packed``)
+    (``kv_bits`` 8 or 4 holds every chunk's prefix K/V as codes)
     (the caller decides where requests come from; ``synth.fleet_request``
     gives the seeded synthetic fleet). With an
     ``expert`` the chunks run through ``flow_sample`` (one fused launch per
@@ -61,15 +62,19 @@ class FleetSampler:
     """
 
     def __init__(self, n_requests: int, rank: int, world: int, chunk: int = 256, n_steps: int = 10,
-                 expert=None, sample_fn: Optional[Callable] = None, device=None, graphs: bool = True):
+                 expert=None, sample_fn: Optional[Callable] = None, device=None, graphs: bool = True,
+                 kv_bits: Optional[int] = None):
         if (expert is None) == (sample_fn is None):
             raise ValueError("give exactly one of expert / sample_fn")
+        if kv_bits is not None and (expert is None or kv_bits not in (8, 4)):
+            raise ValueError(f"kv_bits must be 8 or 4, and takes an expert, got {kv_bits}")
         self.n, self.rank, self.world = n_requests, rank, world
         self.chunk, self.n_steps = chunk, n_steps
         self.lo, self.hi = shard_bounds(n_requests, rank, world)
         self.expert, self.sample_fn = expert, sample_fn
         self.device = device
         self.graphs = graphs
+        self.kv_bits = kv_bits
         self._inputs = None
         self._graphs = None
 
@@ -80,7 +85,7 @@ class FleetSampler:
         for a, b in chunk_bounds(self.lo, self.hi, self.chunk):
             reqs = [request_fn(i) for i in range(a, b)]
             lens = [r[0].shape[1] for r in reqs] if self.expert is not None else []
-            packed = len(set(lens)) > 1  # prompts of different lengths
+            packed = len(set(lens)) > 1 or self.kv_bits is not None  # prompts of different lengths, or held as codes
             pre = torch.cat([r[0][0] if packed else r[0] for r in reqs], 0)
             x0 = torch.cat([r[1] for r in reqs], 0)
             if self.device is not None:
@@ -91,7 +96,7 @@ class FleetSampler:
                 pre, x0 = pre.to(dt), x0.to(dt)
                 if packed:
                     cu = torch.tensor([0] + lens, device=pre.device).cumsum(0).to(torch.int32)
-                    kv = self.expert.encode_packed(pre, cu)
+                    kv = self.expert.encode_packed(pre, cu, self.kv_bits)
                 else:
                     kv = self.expert.encode(pre)
             staged.append((a, b, pre, x0, kv))
