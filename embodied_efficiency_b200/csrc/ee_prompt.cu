@@ -502,9 +502,9 @@ bool prompt_head_map(CUtensorMap* map, const void* base, int hd, int heads, long
 constexpr unsigned long long kPtWaitNs = 1000000000ull;
 static std::atomic<unsigned long long> g_wait_limit{kPtWaitNs};
 
-template <typename T, int HD>
-static int launch_tc(const PromptArgs& p, cudaStream_t s) {
-  auto fn = prompt_tc_kernel<T, HD>;
+template <typename T, int HD, bool JOIN = false>
+static int launch_tc(const PromptArgs& p, cudaStream_t s, const PromptMore* more = nullptr) {
+  auto fn = prompt_tc_kernel<T, HD, 0, JOIN>;
   static std::atomic<int> set[64];
   allow_max_smem(fn, set);
   const DevProps* dp = device_props();
@@ -514,6 +514,7 @@ static int launch_tc(const PromptArgs& p, cudaStream_t s) {
   a.tpt = 128 / p.group;
   a.status = gemm_status_ptr();
   a.timeout_ns = g_wait_limit.load(std::memory_order_relaxed);
+  if (JOIN) a.more = *more;
   if (!a.status) return EE_ERR_DEVICE;
   CUtensorMap mq, mk, mv;
   if (!prompt_head_map(&mq, p.q, HD, p.n_q, p.tq, p.q_head, p.q_tok, p.group, a.tpt) ||
@@ -558,6 +559,12 @@ int launch_prompt_combine(const PromptArgs& a, int hd, int act_dtype, cudaStream
   if (act_dtype == EE_BF16)
     return hd == 64 ? launch_parts<__nv_bfloat16, 64>(a, true, s) : launch_parts<__nv_bfloat16, 128>(a, true, s);
   return hd == 64 ? launch_parts<__half, 64>(a, true, s) : launch_parts<__half, 128>(a, true, s);
+}
+// The same with the rows finished: a.out gets them, with the sums in `more` added.
+int launch_prompt_more(const PromptArgs& a, const PromptMore& more, int hd, int act_dtype, cudaStream_t s) {
+  if (act_dtype == EE_BF16)
+    return hd == 64 ? launch_tc<__nv_bfloat16, 64, true>(a, s, &more) : launch_tc<__nv_bfloat16, 128, true>(a, s, &more);
+  return hd == 64 ? launch_tc<__half, 64, true>(a, s, &more) : launch_tc<__half, 128, true>(a, s, &more);
 }
 int launch_prompt_sums(const PromptArgs& a, int hd, int act_dtype, cudaStream_t s) {
   if (act_dtype == EE_BF16) return hd == 64 ? launch_tc<__nv_bfloat16, 64>(a, s) : launch_tc<__nv_bfloat16, 128>(a, s);

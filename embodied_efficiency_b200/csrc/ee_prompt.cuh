@@ -42,6 +42,14 @@ struct PromptArgs {
   float* stat;       // worker ([workers][2][16][hd]) in the kernel for few rows
 };
 
+// Sums of further keys for the rows of a call that runs as one sequence: [tq][n_q][hd], [tq][n_q][2], for the rows that
+// the offsets cu_q of n_seq sequences cover.
+struct PromptMore {
+  const float *part, *stat;
+  const int* cu_q;
+  int n_seq;
+};
+
 struct PromptSeq {
   int q0, qlen, k0, klen, blk;  // first row and length in q and in k / v; block of the sequence
 };

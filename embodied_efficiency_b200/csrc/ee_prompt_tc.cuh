@@ -68,6 +68,7 @@ struct PromptTcArgs {
   unsigned long long timeout_ns;
   CacheView c;  // keys and values in a cache
   const float *k_steps, *v_steps;
+  PromptMore more;  // JOIN
 };
 
 // registers: 384 threads launch with 168 each; the four warps of loads and MMAs
@@ -223,7 +224,10 @@ EE_DEV float max3(float a, float b, float c) {
 // of S, a value's step its column of P after the sum is taken (so the weights
 // that P V rounds to bf16 are the products). fp16 has no room for weights times
 // steps: there the values are multiplied and rounded once more, to fp16.
-template <typename T, int HD, int BITS = 0>
+//
+// JOIN: the call's rows as one sequence, and other sums of theirs are added where
+// they are finished (a.more).
+template <typename T, int HD, int BITS = 0, bool JOIN = false>
 __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
     prompt_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                      const __grid_constant__ CUtensorMap mv, const __grid_constant__ PromptTcArgs a) {
@@ -285,7 +289,11 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
     }
     mbar_fence_init();
   }
-  pdl_entry();
+  // JOIN: what is read before the rows are finished is older than the kernel this one follows, which waited for it. A
+  // CTA's first item runs beside that kernel's last ones; its end, however far, is waited for without a limit by every
+  // warp before its second item (the softmax warps: before they finish rows), so no bounded wait counts it
+  if (JOIN) pdl_release();
+  else pdl_entry();
   if (warp == 9) {
     tmem_alloc(sb + off_tm, 512);
     tmem_relinquish();
@@ -446,6 +454,7 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
       }
       const uint32_t qbytes = (uint32_t)(p.group * a.tpt) * 128u * PANELS;
       for (int i = 0;; ++i) {
+        if (JOIN && i == 1) pdl_wait();
         const long long idx = (long long)i * gridDim.x + ((i & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
         PromptItem it{};
         const bool more = ok && idx < (long long)units * p.n_kv * p.splits && prompt_item<BITS>(a, (int)idx, units, window, it);
@@ -653,6 +662,7 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
         __syncwarp();
       };
       for (int i = 0; ok; ++i) {
+        if (JOIN && i == 1) pdl_wait();
         ok = __all_sync(0xffffffffu, item_wait(i));
         if (!ok) break;
         const volatile PromptItem* r = ring + i % kPtInfo;
@@ -811,6 +821,7 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
       int n = 0, nfix = 0;
       uint32_t g = 0;
       for (int i = 0;; ++i) {
+        if (JOIN && i == 1) pdl_wait();
         bool ok = item_wait(i);
         const volatile PromptItem* r = ring + i % kPtInfo;
         const int nbm = r->nbm, tail = r->tail;
@@ -1039,17 +1050,38 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
         l = l * own + l1 * own1;
         m = ref;
       }
+      float others = 0.f;  // JOIN: what the other sums are multiplied by, and O by own
+      bool covered = mine, ours = true, theirs = false;
+      const long long more_at = (long long)out_row * p.n_q + head;
+      if (JOIN) {
+        pdl_wait();
+        covered = mine && out_row >= __ldg(a.more.cu_q) && out_row < __ldg(a.more.cu_q + a.more.n_seq);
+        const float2 st = covered ? __ldg(reinterpret_cast<const float2*>(a.more.stat) + more_at) : make_float2(-INFINITY, 0.f);
+        ours = l != 0.f;  // sums that have seen no key need not have been written
+        theirs = st.y != 0.f;
+        const float high = fmaxf(m, st.x), ref = high == -INFINITY ? 0.f : high;
+        own = ours ? ex2(m - ref) : 0.f;
+        others = theirs ? ex2(st.x - ref) : 0.f;
+        l = (ours ? l * own : 0.f) + (theirs ? st.y * others : 0.f);
+      }
       const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees no key is zero
       const long long at = ((long long)part * p.tq + out_row) * p.n_q + head;
       if (!whole && mine) *reinterpret_cast<float2*>(p.stat + 2 * at) = make_float2(m, l);
       // the element a lane's row starts at, -1 for a row that is not there
-      const long long row_at = mine ? (long long)out_row * p.o_tok + head * p.o_head : -1;
+      const long long row_at = covered ? (long long)out_row * p.o_tok + head * p.o_head : -1;
       const uint32_t stg = sb + pt_off_out<HD, BITS>() + warp * pt_stage<BITS>();
 #pragma unroll
       for (int c = 0; c < HD / 64; ++c) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t o[32];
+          float4 x4[JOIN ? 8 : 1];
+          if (JOIN) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              x4[e % (JOIN ? 8 : 1)] = theirs ? __ldg(reinterpret_cast<const float4*>(a.more.part + more_at * HD) + 16 * c + 8 * h + e)
+                                              : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
           if (nt > 0) {
             tmem_ld32(to + 64 * c + 32 * h, o);
             if (BITS && merge) {
@@ -1068,6 +1100,14 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
                 mbar_arrive(b_of + 8 * t);
                 if (BITS && merge) mbar_arrive(b_of + 8 - 8 * t);
               }
+            }
+          }
+          if (JOIN) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const float4 x = x4[e / 4 % (JOIN ? 8 : 1)];
+              const float add = e % 4 == 0 ? x.x : e % 4 == 1 ? x.y : e % 4 == 2 ? x.z : x.w;
+              o[e] = __float_as_uint((ours ? __uint_as_float(o[e]) * own : 0.f) + add * others);
             }
           }
           if (whole) {
@@ -1116,6 +1156,7 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
     }
     if (!ok && lane == 0) atomicCAS(a.status, 0, (int)EE_ERR_TIMEOUT);
   }
+  if (JOIN) pdl_wait();  // not to end before the kernel this one follows
   tc_fence_before();
   __syncthreads();  // every MMA has completed (the outputs or the MMA warp waited for them) and every TMEM read is done
   if (warp == 9) {

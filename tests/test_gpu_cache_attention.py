@@ -215,6 +215,31 @@ def test_what_the_device_says_is_not_trusted(cuda):
     assert status() == 0
 
 
+@pytest.mark.parametrize("plen", [100, 2000])
+@pytest.mark.parametrize("nq", [1, 30])
+def test_rows_outside_the_sequences_behind_a_prefix(cuda, plen, nq):
+    """Rows before the first and behind the last sequence stay as they were; captured calls repeat what eager ones give."""
+    from embodied_efficiency_b200 import cache_attention
+    n = 7
+    q, cache, _, table, kl, pre = make(cuda, torch.bfloat16, 8, 8, 2, 128, 64, [nq] * n + [5], [40 * i for i in range(n)] + [9],
+                                       8, plen)
+    table, kl = table[:n], kl[:n]
+    cu = torch.arange(n + 1, device=cuda, dtype=torch.int32) * nq + 3
+    out = cache_attention(q, cache, cu, table, kl, prefix=pre, out=torch.full_like(q, 3.0))
+    assert bool((out[:3] == 3).all()) and bool((out[3 + n * nq:] == 3).all())
+    check(out[3:3 + n * nq], q[3:3 + n * nq], cache, table, [nq] * n, [40 * i for i in range(n)], True, 128 ** -0.5, pre)
+    graph, held = torch.cuda.CUDAGraph(), torch.full_like(q, 3.0)
+    with torch.cuda.graph(graph):
+        cache_attention(q, cache, cu, table, kl, prefix=pre, out=held)
+        again = cache_attention(held, cache, cu, table, kl, prefix=pre, out=torch.empty_like(q).fill_(3.0))
+    for _ in range(3):
+        held.fill_(3.0)
+        graph.replay()
+    assert torch.equal(held, out)
+    assert torch.equal(again, cache_attention(out, cache, cu, table, kl, prefix=pre, out=torch.full_like(q, 3.0)))
+    assert status() == 0
+
+
 def test_far_pages(cuda):
     """Codes beyond 2^31 and 2^32 bytes from the cache's start."""
     from embodied_efficiency_b200 import KVCache, cache_attention, cache_write
