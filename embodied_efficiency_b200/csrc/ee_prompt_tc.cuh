@@ -94,12 +94,13 @@ template <int BITS> constexpr uint32_t pt_stage() { return BITS ? 0u : 4096u; } 
 template <int HD, int BITS> constexpr uint32_t pt_raw() { return 128u * HD * BITS / 8; }  // codes of a tile
 // tiles of codes on their way: 40 to 48 KB where they are large (with 32 KB an SM waited for them)
 template <int HD, int BITS> constexpr int pt_raws() { return !BITS ? 0 : HD * BITS == 1024 ? 3 : HD * BITS == 512 ? 5 : 6; }
-constexpr int kPtSteps = 4;  // blocks whose steps are held
+constexpr int kPtSteps = 4;  // blocks whose steps are held: of K, of V, and the powers of two that fp16 values take
+constexpr uint32_t kPtStepBytes = 3 * 128 * 4;
 template <int HD, int BITS> constexpr uint32_t pt_off_raw() { return (pt_tiles<BITS>() + pt_slots<HD, BITS>()) * pt_tile<HD>(); }
 template <int HD, int BITS> constexpr uint32_t pt_off_out() { return pt_off_raw<HD, BITS>() + pt_raws<HD, BITS>() * pt_raw<HD, BITS>(); }
 template <int HD, int BITS> constexpr uint32_t pt_off_rawsteps() { return pt_off_out<HD, BITS>() + 8 * pt_stage<BITS>(); }
 template <int HD, int BITS> constexpr uint32_t pt_off_steps() { return pt_off_rawsteps<HD, BITS>() + pt_raws<HD, BITS>() * 1024u; }
-template <int HD, int BITS> constexpr uint32_t pt_off_bar() { return pt_off_steps<HD, BITS>() + (BITS ? kPtSteps * 1024u : 0u); }
+template <int HD, int BITS> constexpr uint32_t pt_off_bar() { return pt_off_steps<HD, BITS>() + (BITS ? kPtSteps * kPtStepBytes : 0u); }
 // barriers: full / empty per load of K / V, Q full / empty, S / P (two halves) / S free / O / O free per tile, V to fix /
 // fixed, item full / empty, MMAs done after a failure; of a cache the other half's sums (twice), steps full, codes full /
 // empty. (There full / empty are a slot's, K and V by themselves.)
@@ -240,7 +241,7 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
   constexpr bool SEP = HD == 64;
   // pieces in which a block's weights are handed over (in one piece, hd 64: 501 instead of 411 us for 8192 tokens)
   constexpr int PARTS = 2;
-  constexpr bool VSCALE = BITS && !std::is_same<T, __half>::value;  // P takes the values' steps
+  constexpr bool POW2 = BITS && std::is_same<T, __half>::value;  // the values' steps are halved: P takes what a power of two leaves
   extern __shared__ __align__(1024) char smem_raw[];
   const uint32_t base0 = smem_u32(smem_raw);
   const uint32_t sb = (base0 + 1023u) & ~1023u;
@@ -352,7 +353,7 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
           ok = mbar_wait(b_rf + 8 * rs, (rt / NR) & 1, a.timeout_ns);
           // the products of the tile that used the slot before are done
           if (ok && blk >= slots) ok = mbar_wait(b_empty + 8 * at, (blk / slots - 1) & 1, a.timeout_ns);
-          float* steps = reinterpret_cast<float*>(smem + pt_off_steps<HD, BITS>() + (blk % kPtSteps) * 1024);
+          float* steps = reinterpret_cast<float*>(smem + pt_off_steps<HD, BITS>() + (blk % kPtSteps) * kPtStepBytes);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           if (!isv) {
@@ -368,6 +369,12 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
               vs = 0.f;
             }
             steps[key] = ks * (p.scale_log2 * code_unit<T, BITS>());
+            if (POW2) {  // 2^e to the values, exactly: e from -24, where fp16 ends, to 15
+              const int e = min(max(((__float_as_int(vs) >> 23) & 0xff) - 127, -24), 15);
+              const __half2 v2 = __float2half2_rn(__int_as_float((127 + e) << 23));
+              steps[256 + key] = __uint_as_float(*reinterpret_cast<const uint32_t*>(&v2));
+              vs *= __int_as_float((127 - e) << 23);
+            }
             steps[128 + key] = vs * code_unit<T, BITS>();
             const uint32_t all = __ballot_sync(0xffffffffu, have);
             if (lane == 0)
@@ -397,13 +404,10 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
                   for (int b = 0; b < 4; ++b) o[4 * k + b] = code_pair4<T>(xw[k], xw[k] >> 4, b);
                 }
               }
-              if (!VSCALE && isv) {
-                const float s = steps[128 + row0 + e / HALVES * ROWS];
+              if (POW2 && isv) {
+                const uint32_t s2 = __float_as_uint(steps[256 + row0 + e / HALVES * ROWS]);
 #pragma unroll
-                for (int k = 0; k < 64 / BITS; ++k) {
-                  const float2 f = Act<T>::unpack2(o[k]);
-                  o[k] = Act<T>::pack2(f.x * s, f.y * s);
-                }
+                for (int k = 0; k < 64 / BITS; ++k) o[k] = fma2<T>(o[k], s2, 0u);
               }
 #pragma unroll
               for (int k = 0; k < 16 / BITS; ++k)
@@ -903,7 +907,7 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
           if (lane == 0) mbar_arrive(b_sf + 8 * t);
         }
         const int left = lim - j * kPtKeys;
-        const float4* steps = reinterpret_cast<const float4*>(smem + pt_off_steps<HD, BITS>() + ((bs + j) % kPtSteps) * 1024);
+        const float4* steps = reinterpret_cast<const float4*>(smem + pt_off_steps<HD, BITS>() + ((bs + j) % kPtSteps) * kPtStepBytes);
         uint32_t there[4];
         bool gaps = false;
         if constexpr (BITS > 0) {
@@ -951,7 +955,7 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
           const float to = prompt_reference<T, 7>(mx);
           f = ex2(m - to);
           m = to;
-          top = mx + 8.f;
+          top = mx + (POW2 ? 7.f : 8.f);  // weights up to 2^15, with a factor below 2 from the values' steps 2^14 before it
         }
         const bool rescale = __any_sync(0xffffffffu, f != 1.f) && i > 0;
         if (SEP && i > 0) {  // O += P(j-1) V(j-1) is done: P may be written, O rescaled
@@ -986,7 +990,7 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
             unpack64(BITS ? add2f(x2, neg2) : fma2f(x2, sc2, neg2), y0, y1);
             float w0 = ex2(__uint_as_float(y0)), w1 = ex2(__uint_as_float(y1));
             sum[c] = add2f(sum[c], pack64(__float_as_uint(w0), __float_as_uint(w1)));
-            if (VSCALE) {
+            if (BITS) {
               if (e % 4 == 0) vs4 = steps[32 + 8 * c + e / 4];
               uint32_t u0, u1;
               unpack64(mul2f(pack64(__float_as_uint(w0), __float_as_uint(w1)),

@@ -29,8 +29,7 @@ def held(cache, table, b, n):
 def check(out, q, cache, table, q_len, k_len, causal, scale, prefix=None):
     """|out - exact| per value. With A = sum_j p_j |v_j| / sum_j p_j: the weights' rounding for the product with v gives
     2^-8 A (bf16) or 2^-16 A (fp16, rounded twice; behind a prefix and with more than 16 rows a sequence and key head
-    rounded once, 2^-11 A, and 2^-25 absolute per weight where the largest is at least 2^-1; there the values are rounded
-    to fp16 too, 2^-11 A and 2^-25 absolute), the result's rounding half a step of it; a score's error of d moves a weight by a factor e^d, twice
+    rounded once, 2^-11 A, and 2^-25 absolute per weight where the largest is at least 2^-1), the result's rounding half a step of it; a score's error of d moves a weight by a factor e^d, twice
     with the sum below it: fp32 sums of hd products, the steps' and the exponent's roundings 2^-22 of sum |q k| scale,
     and bf16 queries as fp16 2^-25 of the row's largest times sum |k|; 2^-18 A covers exp2, the sums of up to a few
     thousand weights and the merges."""
@@ -60,7 +59,7 @@ def check(out, q, cache, table, q_len, k_len, causal, scale, prefix=None):
                 if not f16:
                     d = d + qd.abs().amax(-1, keepdim=True) * kd.abs().sum(-1).amax(-1)[:, None, None] * 2 ** -25
                 d = d * scale
-            weights = 2.0 ** -8 if not f16 else (2.0 ** -10 if many else 2.0 ** -16 if prefix is None else 2.0 ** -11)
+            weights = 2.0 ** -8 if not f16 else (2.0 ** -11 if many or prefix is not None else 2.0 ** -16)
             tol = (weights * mean + fi.eps / 2 * ref.abs()) * (1 + 2 ** -6) + mean * (2 * d + 2 ** -18) + 2.0 ** -24
             if f16 and n and (many or prefix is not None):
                 tol = tol + (n if many else len(prefix[0])) * 2.0 ** -25 * vd.abs().amax(1, keepdim=True)
@@ -213,6 +212,31 @@ def test_what_the_device_says_is_not_trusted(cuda):
         kl = torch.tensor([4000, 129], dtype=torch.int32, device=cuda)
         check(cache_attention(q, cache, cu, table, kl)[:20], q[:20], cache, table, [9, 11], [128, 128], True, 0.125)
     assert status() == 0
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("hd,nq,prefix", [(64, 1, 0), (128, 1, 300), (128, 50, 0), (64, 50, 300), (64, 50, 0)])
+def test_two_roundings_at_most(cuda, dtype, bits, hd, nq, prefix):
+    """The weights' rounding for their product with the values and the result's: errors of one size that do not depend on
+    one another, sqrt(2) of the result's alone; 1.5 leaves 6 % for the fp32 steps between them."""
+    from embodied_efficiency_b200 import cache_attention
+    k_len = [nq + 40 * i for i in range(6)]
+    q, cache, cu, table, kl, pre = make(cuda, dtype, bits, 8, 4, hd, 64, [nq] * 6, k_len, 17, prefix)
+    out = cache_attention(q, cache, cu, table, kl, prefix=pre)
+    err, half = [], []
+    for b, n in enumerate(k_len):
+        kd, vd, _ = held(cache, table, b, n)
+        if prefix:
+            kd, vd = torch.cat([pre[0].double(), kd]), torch.cat([pre[1].double(), vd])
+        kd, vd = (x.transpose(0, 1).repeat_interleave(2, 0) for x in (kd, vd))
+        s = q[b * nq:(b + 1) * nq].double().transpose(0, 1) @ kd.transpose(1, 2) * hd ** -0.5
+        at = torch.arange(kd.shape[1], device=cuda)[None] - torch.arange(nq, device=cuda)[:, None]
+        ref = torch.softmax(s.masked_fill(at > n + prefix - nq, float("-inf")), -1) @ vd
+        err.append(out[b * nq:(b + 1) * nq].double().transpose(0, 1) - ref)
+        half.append(ref.to(dtype).double() - ref)
+    rms = lambda x: float(torch.cat([y.flatten() for y in x]).pow(2).mean().sqrt())
+    assert rms(err) <= 1.5 * rms(half)
 
 
 @pytest.mark.parametrize("plen", [100, 2000])
