@@ -10,6 +10,10 @@
 // warp per token: hd / 8 lanes a head, 16 bytes a lane, several heads of keys
 // and values in flight; the loads of a token's values are under way before its
 // place is looked up (a search over the offsets and one entry of the table).
+//
+// Measured: 100000 tokens of 16 heads of 128 in 8 bits written in 79 us, read in
+// 73 (5.6 and 6.0 TB/s of 6.46 a copy reaches); below some hundred tokens a
+// launch's 4 us. Several tokens a warp were slower in either direction.
 #include "ee_cache.cuh"
 #include "ee_host.h"
 

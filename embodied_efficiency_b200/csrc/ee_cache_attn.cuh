@@ -31,6 +31,11 @@
 // the values' steps have fp32's range, so they are rounded to bf16 (2^-8 each,
 // in either direction, as the 16-bit kernels' weights); for fp16 outputs a
 // second product adds what the rounding left (to 2^-16).
+//
+// HBM-bound where the call is large: 512 x 1 token behind 2048, 16 heads of 128 in
+// 8 bits 5.5 TB/s; 4 bits 3.9, where the instructions on a code count. A small
+// call is two launches (the sums, the join of rows that a border cut) of 12 us
+// between them, and the ring's latency.
 #pragma once
 
 #include <atomic>
@@ -560,23 +565,27 @@ __global__ void __launch_bounds__(kPrJoin) cache_join_kernel(const __grid_consta
     seq_first = list.before[threadIdx.x] + hit_at;
   }
   __syncthreads();
-  pdl_entry();  // by every thread, the ones that return too: this grid must not end before the one it follows
-  if (found == 0x7fffffff) return;  // rows outside the sequences stay as they were
-  const CacheSeq s = seq;
-  int steps;
-  list_steps(a, s, steps);
-  const long long share = pr_share(total, most, kCaMinSteps);
+  // what hangs on lengths and offsets alone, under the kernel before this one
+  const bool there = found != 0x7fffffff;
   const int h = MANY ? blockIdx.y : blockIdx.y * (kPrJoin / 32) + (threadIdx.x >> 5);
-  if (h >= a.n_q) return;
-  const int kvh = h / a.group, r = (tok - s.q0) * a.group + h % a.group;
+  int r = 0;
   long long w0 = 0, n = 0, front = 0;  // parts of its own: their first worker, their number, where the first's lies
-  if (steps > 0) {
-    const long long first = seq_first + (long long)(r / a.rows * a.c.n_kv + kvh) * steps;
-    w0 = pr_div(first, share);
-    n = pr_div(first + steps - 1, share) - w0 + 1;
-    if (n == 1 && !a.pre_splits) return;  // in one share: written already
-    front = w0 * share == first ? 0 : a.rows;  // else the first part is at its share's end
+  if (there && h < a.n_q) {
+    const CacheSeq s = seq;
+    int steps;
+    list_steps(a, s, steps);
+    r = (tok - s.q0) * a.group + h % a.group;
+    if (steps > 0) {
+      const long long share = pr_share(total, most, kCaMinSteps);
+      const long long first = seq_first + (long long)(r / a.rows * a.c.n_kv + h / a.group) * steps;
+      w0 = pr_div(first, share);
+      n = pr_div(first + steps - 1, share) - w0 + 1;
+      front = w0 * share == first ? 0 : a.rows;  // else the first part is at its share's end
+    }
   }
+  pdl_entry();  // by every thread, the ones that return too: this grid must not end before the one it follows
+  if (!there || h >= a.n_q) return;  // rows outside the sequences stay as they were
+  if (n == 1 && !a.pre_splits) return;  // in one share: written already
   const long long row = (long long)tok * a.n_q + h, hop = (long long)a.tq * a.n_q;
   auto slot = [&](long long i) {
     if (i >= n) return a.whole + (1 + i - n) * hop + row;  // a part of the prefix

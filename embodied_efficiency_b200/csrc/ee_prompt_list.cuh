@@ -160,8 +160,17 @@ EE_DEV void join_row_warp(const float* part, const float* stat, long long n, Slo
   float m = -INFINITY, l = 0.f, v[V] = {};
   for (long long i0 = 0; i0 < n; i0 += 32) {
     const int here = (int)(n - i0 < 32 ? n - i0 : 32);
+    float2 x[8][V / 2];
+    auto values = [&](int i) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int e = 0; e < V / 2; ++e)
+          x[k][e] = __ldg(reinterpret_cast<const float2*>(part + slot(i0 + min(i + k, here - 1)) * HD + lane * V) + e);
+    };
     const float2 st = lane < here ? __ldg(reinterpret_cast<const float2*>(stat) + slot(i0 + lane))
                                   : make_float2(-INFINITY, 0.f);
+    values(0);  // loads first: none waits for another's weight
     const float top = fmaxf(m, warp_max(st.x));
     const float u = top == -INFINITY ? 0.f : top, old = exp2f(m - u);
     m = top;
@@ -170,13 +179,8 @@ EE_DEV void join_row_warp(const float* part, const float* stat, long long n, Slo
     l = l * old + f * st.y;
 #pragma unroll
     for (int e = 0; e < V; ++e) v[e] *= old;
-    for (int i = 0; i < here; i += 8) {  // loads first: none waits for another's weight
-      float2 x[8][V / 2];
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-#pragma unroll
-        for (int e = 0; e < V / 2; ++e)
-          x[k][e] = __ldg(reinterpret_cast<const float2*>(part + slot(i0 + min(i + k, here - 1)) * HD + lane * V) + e);
+    for (int i = 0; i < here; i += 8) {
+      if (i > 0) values(i);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const float w = __shfl_sync(0xffffffffu, wt, (i + k) & 31);  // below 0 past the last part

@@ -219,15 +219,35 @@ EE_DEV float max3(float a, float b, float c) {
   return r;
 }
 
-// BITS 0: K and V of 16 bits. 8 or 4: codes from a paged cache. TMA brings them
-// into a ring, 128 keys at a time; warps 10 and 11 turn them into 16-bit tiles in
-// the slots, exactly, and hand on the steps: a key's step multiplies its column
-// of S, a value's step its column of P after the sum is taken (so the weights
-// that P V rounds to bf16 are the products). fp16 has no room for weights times
-// steps: there the values are multiplied and rounded once more, to fp16.
+// BITS 0: K and V of 16 bits. 8 or 4: codes from a paged cache, with 512 threads.
+// Warp 10 finds the items; warp 8 looks up their pages and brings codes (TMA, a
+// box per piece of a page) and steps (bulk copies) into a ring, 128 keys at a
+// time; warps 12-15 turn them into 16-bit tiles in the slots, exactly, two of K
+// and two of V, and hand on the steps. A key's step multiplies its column of S,
+// a value's its column of P after the sum is taken, so the weights that P V
+// rounds are the products: bf16 has room for them, fp16 gets the values as code
+// times a power of two, exactly, and the weights what that leaves of the step, a
+// factor below 2.
 //
-// JOIN: the call's rows as one sequence, and other sums of theirs are added where
-// they are finished (a.more).
+// There an item is one tile, as a call's sequences rarely have two (50 tokens a
+// turn): its blocks take turns on the two halves' softmax warps and columns of
+// TMEM, from where the item before stopped, so one half's softmax runs under the
+// other's products as two tiles' would; the half with the last block adds the
+// other's sums and finishes the rows. (Two tiles an item, the second empty: 240 us
+// where this takes 118; 128-row tiles with half of the rows idle cost whole
+// products either way.)
+//
+// Measured: 64 x 50 tokens behind 257 to 816, 16 heads of 128, 8 bits: 119 us;
+// 32 x 50 x 8 heads a key head behind 816 to 1632, 4 bits: 178 us, 550 TFLOP/s;
+// the same with keys and values in 16 bits: 88 and 135. With neither decoding,
+// steps nor exponentials the skeleton takes 86 and 117: what bounds it is the
+// round trip of scores, softmax and products of a lone tile, then the decoding
+// (per block 2 x 128 x 128 codes by four warps) and the steps' multiplications.
+// Not faster: K and V decoded by two warps each (118 -> 136), S read twice by
+// halves without spills (130, 200).
+//
+// JOIN: the call's rows as one sequence over 16-bit keys, and other sums of theirs
+// (a.more, left by the kernel before this one) are added where they are finished.
 template <typename T, int HD, int BITS = 0, bool JOIN = false>
 __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
     prompt_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
