@@ -587,10 +587,11 @@ __global__ void __launch_bounds__(kPrJoin) cache_join_kernel(const __grid_consta
   if (!there || h >= a.n_q) return;  // rows outside the sequences stay as they were
   if (n == 1 && !a.pre_splits) return;  // in one share: written already
   const long long row = (long long)tok * a.n_q + h, hop = (long long)a.tq * a.n_q;
+  r %= a.rows;
   auto slot = [&](long long i) {
     if (i >= n) return a.whole + (1 + i - n) * hop + row;  // a part of the prefix
     if (n == 1) return a.whole + row;
-    return (w0 + i) * 2 * a.rows + (i == 0 ? front : 0) + r % a.rows;
+    return (w0 + i) * 2 * a.rows + (i == 0 ? front : 0) + r;
   };
   T* out = reinterpret_cast<T*>(a.out) + (long long)tok * a.o_tok + h * a.o_head;
   if (MANY) join_row<T, HD>(a.part, a.stat, n + a.pre_splits, slot, out, &sh);
@@ -621,11 +622,12 @@ int launch_cache_rows(const CacheMaps& m, const CacheAttnArgs& a, cudaStream_t s
   // beside the prefix's CTAs, where they leave half of the SMs or more
   const int sms = device_sms(), ctas = a.pre_ctas > 0 && 2 * a.pre_ctas <= sms ? sms - a.pre_ctas : sms, most = ctas * S::WORKERS;
   if (launch_pdl(fn, dim3(ctas), dim3(S::THREADS), S::SMEM, s, m.k, m.v, a) != cudaSuccess) return EE_ERR_LAUNCH;
-  // parts of a row, on average: a CTA per row from 16 on
+  // parts of a row, on average: a CTA per row from 16 of its own on, or more than 32 of the prefix (64 x 16 rows with 16
+  // of them: 8 us with a CTA a row, 4 with a warp)
   const long long blocks = (long long)a.tq * a.group / a.rows;
   const long long items = (blocks > a.c.n_seq ? blocks : a.c.n_seq) * a.c.n_kv;
   const cudaError_t e =
-      most > 16 * items || a.pre_splits > 8
+      most > 16 * items || a.pre_splits > 32
           ? launch_pdl(cache_join_kernel<T, HD, true>, dim3((unsigned)a.tq, a.n_q), dim3(kPrJoin), 0, s, a, most)
           : launch_pdl(cache_join_kernel<T, HD, false>, dim3((unsigned)a.tq, (a.n_q + kPrJoin / 32 - 1) / (kPrJoin / 32)),
                        dim3(kPrJoin), 0, s, a, most);
