@@ -149,6 +149,7 @@ int ee_cache_attention(const ee_cache* cache, const void* q, int64_t q_tok, int6
     a.tq = (int)tq; a.n_q = n_q; a.group = n_q / n_kv;
     a.causal = causal != 0;
     a.rows = 8 * plan.nt;
+    a.rows_log2 = plan.nt > 1 ? 4 : 3;
     a.scale_log2 = scale_log2;
     a.k_steps = cache->k_steps; a.v_steps = cache->v_steps;
     a.part = part; a.stat = stat;

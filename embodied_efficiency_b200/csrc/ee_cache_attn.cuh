@@ -32,10 +32,13 @@
 // in either direction, as the 16-bit kernels' weights); for fp16 outputs a
 // second product adds what the rounding left (to 2^-16).
 //
-// HBM-bound where the call is large: 512 x 1 token behind 2048, 16 heads of 128 in
-// 8 bits 5.5 TB/s; 4 bits 3.9, where the instructions on a code count. A small
-// call is two launches (the sums, the join of rows that a border cut) of 12 us
-// between them, and the ring's latency.
+// HBM-bound where the call is large (64 x 1 token behind 4096, 8 key heads of 128,
+// 8 bits: 5.5 TB/s; 4 bits, where the instructions on a code count: 3.9). In
+// between, instructions: 850 a step, two warps a scheduler (64 x 1 behind 1 to
+// 1632, 16 / 4 heads of 128, 8 bits: 23.8 us where the bytes take 9.6; twelve
+// warps with rings two stages deep: 30.4 where eight took 28.7). A small call is
+// two launches, the sums and the join of rows that a border cut, and in each the
+// way through offsets, lengths and table to the codes: 9 us.
 #pragma once
 
 #include <atomic>
@@ -61,7 +64,7 @@ struct CacheAttnArgs {
   const int* cu_q;
   long long q_tok, q_head, o_tok, o_head;  // strides, elements
   int tq, n_q, group, causal;
-  int rows;             // rows of an item
+  int rows, rows_log2;  // rows of an item
   float scale_log2;     // scale * log2(e)
   // sums of parts, [hd] each, and their maximum and weight: first of items that a border cuts, by worker ([workers][2]
   // [rows]); behind a prefix then of every whole item's rows ([tq][n_q]) and of the prefix ([pre_splits][tq][n_q])
@@ -87,7 +90,7 @@ constexpr int kCaKeys = 32, kCaMinSteps = 6;  // keys of a step; steps that are 
                                                // token behind 30000, 4 bits: 21.4 us with 3, 19.8 with 6, 20.6 with 10)
 EE_DEV long long list_steps(const CacheAttnArgs& a, const CacheSeq& s, int& per_item) {
   per_item = (s.klen + kCaKeys - 1) / kCaKeys;
-  return (((long long)s.qlen * a.group + a.rows - 1) / a.rows) * a.c.n_kv * per_item;
+  return (((long long)s.qlen * a.group + a.rows - 1) >> a.rows_log2) * a.c.n_kv * per_item;
 }
 
 // How the kernel is cut: workers (warps) per CTA and stages of their rings.
@@ -104,6 +107,7 @@ struct CaShape {
   static constexpr int ROWS = 8 * NT;
 };
 
+EE_DEV void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 EE_DEV float ca_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -179,6 +183,14 @@ __global__ void __launch_bounds__(CaShape<HD, BITS, NT>::THREADS, 1)
   if (lane == 0) {
     for (int i = 0; i < NS; ++i) mbar_init(full + 8 * i, 1);
     mbar_fence_init();
+  }
+  // What a CTA's way to its first load reads, one after another (offsets and lengths, table), is brought to L2 under the
+  // kernel before this one.
+  {
+    const long long i = 32ll * ((long long)blockIdx.x * NTH + tid);
+    if (i <= a.c.n_seq) prefetch_l2(a.cu_q + i);
+    if (i < a.c.n_seq) prefetch_l2(a.c.k_lens + i);
+    if (a.c.width > 0 && i < (a.c.n_seq - 1) * a.c.table_row + a.c.width) prefetch_l2(a.c.table + i);
   }
   // Behind a prefix the kernel before this one sums that up, from nothing that this one writes and for nothing that it
   // reads; it has itself waited for everything before the call, so this one need not wait for it but before it ends (the
@@ -577,7 +589,7 @@ __global__ void __launch_bounds__(kPrJoin) cache_join_kernel(const __grid_consta
     r = (tok - s.q0) * a.group + h % a.group;
     if (steps > 0) {
       const long long share = pr_share(total, most, kCaMinSteps);
-      const long long first = seq_first + (long long)(r / a.rows * a.c.n_kv + h / a.group) * steps;
+      const long long first = seq_first + (long long)((r >> a.rows_log2) * a.c.n_kv + h / a.group) * steps;
       w0 = pr_div(first, share);
       n = pr_div(first + steps - 1, share) - w0 + 1;
       front = w0 * share == first ? 0 : a.rows;  // else the first part is at its share's end
@@ -587,7 +599,7 @@ __global__ void __launch_bounds__(kPrJoin) cache_join_kernel(const __grid_consta
   if (!there || h >= a.n_q) return;  // rows outside the sequences stay as they were
   if (n == 1 && !a.pre_splits) return;  // in one share: written already
   const long long row = (long long)tok * a.n_q + h, hop = (long long)a.tq * a.n_q;
-  r %= a.rows;
+  r &= a.rows - 1;
   auto slot = [&](long long i) {
     if (i >= n) return a.whole + (1 + i - n) * hop + row;  // a part of the prefix
     if (n == 1) return a.whole + row;
