@@ -11,9 +11,10 @@
 // and values in flight; the loads of a token's values are under way before its
 // place is looked up (a search over the offsets and one entry of the table).
 //
-// Measured: 100000 tokens of 16 heads of 128 in 8 bits written in 79 us, read in
-// 73 (5.6 and 6.0 TB/s of 6.46 a copy reaches); below some hundred tokens a
-// launch's 4 us. Several tokens a warp were slower in either direction.
+// Measured: 128 prompts of 257 to 816 tokens, 16 heads of 64, written in 8 bits in
+// 79 us (5.6 TB/s of the 6.46 that a copy reaches); 64 such prompts, heads of 128,
+// read in 73 (6.0); 64 x 1 token written in 3.5, a launch. Several tokens a warp
+// were slower in either direction.
 #include "ee_cache.cuh"
 #include "ee_host.h"
 

@@ -233,18 +233,18 @@ EE_DEV float max3(float a, float b, float c) {
 // turn): its blocks take turns on the two halves' softmax warps and columns of
 // TMEM, from where the item before stopped, so one half's softmax runs under the
 // other's products as two tiles' would; the half with the last block adds the
-// other's sums and finishes the rows. (Two tiles an item, the second empty: 240 us
-// where this takes 118; 128-row tiles with half of the rows idle cost whole
-// products either way.)
+// other's sums and finishes the rows. (Items of two tiles, the second's half at
+// the first's keys where it is empty: 150 and 207 us where this took 129 and 184
+// in the first two cases below.)
 //
-// Measured: 64 x 50 tokens behind 257 to 816, 16 heads of 128, 8 bits: 119 us;
-// 32 x 50 x 8 heads a key head behind 816 to 1632, 4 bits: 178 us, 550 TFLOP/s;
-// the same with keys and values in 16 bits: 88 and 135. With neither decoding,
-// steps nor exponentials the skeleton takes 86 and 117: what bounds it is the
-// round trip of scores, softmax and products of a lone tile, then the decoding
-// (per block 2 x 128 x 128 codes by four warps) and the steps' multiplications.
-// Not faster: K and V decoded by two warps each (118 -> 136), S read twice by
-// halves without spills (130, 200).
+// Measured, heads of 128, 8 bits: 64 x 50 tokens behind 257 to 816, 16 heads: 119
+// us; 4 x 500 to 1024 behind 1 to 4096, 16 / 4 heads: 178, 550 TFLOP/s; with keys
+// and values in 16 bits: 88 and 134. Without decoding, steps and exponentials the
+// rest takes 86 and 117: what bounds it is the round trip of scores, softmax and
+// products of a lone tile, whose 50 rows are two warps of four, then the decoding
+// (2 x 128 x 128 codes a block by four warps) and the steps' multiplications. Not
+// faster: K and V decoded by two warps each (118 -> 136), S read twice by halves,
+// without spills (118 -> 130, 179 -> 200).
 //
 // JOIN: the call's rows as one sequence over 16-bit keys, and other sums of theirs
 // (a.more, left by the kernel before this one) are added where they are finished.
