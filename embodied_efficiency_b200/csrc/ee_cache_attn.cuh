@@ -657,8 +657,9 @@ int launch_cache_tc(const CacheMaps& m, const PromptTcArgs& a, cudaStream_t s) {
   const long long items = ((long long)a.p.tq / a.tpt + a.p.n_seq) * a.p.n_kv * a.p.splits;
   if (items > 0x7fffffff) return EE_ERR_SHAPE;
   const int sms = device_sms();
-  return launch_pdl(fn, dim3((unsigned)(items < sms ? items : sms)), dim3(PtThreads<BITS>::N), pt_smem<HD, BITS>(), s, mq, m.k, m.v,
-                    a) == cudaSuccess
+  const bool keys = a.c.width > 0;  // without, any map does: none of them is loaded by
+  return launch_pdl(fn, dim3((unsigned)(items < sms ? items : sms)), dim3(PtThreads<BITS>::N), pt_smem<HD, BITS>(), s, mq,
+                    keys ? m.k : mq, keys ? m.v : mq, a) == cudaSuccess
              ? EE_OK
              : EE_ERR_LAUNCH;
 }

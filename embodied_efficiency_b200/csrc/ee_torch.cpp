@@ -1,9 +1,9 @@
 // ee_torch.cpp -- native host side of the prompt-layer operators: what a call
 // of rotary_embed, norm_rotary_embed, prompt_attention, int8_linear,
 // int8_matmul, quantize_tokens and the operators of a cache does on the host,
-// without the interpreter. A call of few
-// tokens takes the GPU 3 to 8 us; checks, allocations and argument conversion
-// in Python took 13 to 17 us around it.
+// without the interpreter. A call of few tokens takes the GPU 3 to 8
+// us; checks, allocations and argument conversion in Python took 13 to 17 us
+// around it.
 //
 // Every function here takes the usual call -- aligned, contiguous tensors of
 // the current device, no gradients, nothing to copy -- through the C ABI and
@@ -423,7 +423,7 @@ PyObject* cache_attention(PyObject*, PyObject* const* a, Py_ssize_t argc) {
   } else if (PyFloat_Check(a[7])) {
     scale = (float)PyFloat_AS_DOUBLE(a[7]);
   }
-  if (!c.need(scale > 0.f && scale < 2.0e38f)) return none();
+  if (!c.need(scale >= FLT_MIN && scale < 2.0e38f)) return none();
   const bool causal = a[6] == Py_True;
   const int64_t plen = pk ? pk->size(0) : 0;
   Tensor out;

@@ -276,6 +276,72 @@ def test_far_pages(cuda):
     cache_write(cache, x, -x, cu, table, kl)
     q = torch.randn(3, 16, hd, device=cuda).half()
     check(cache_attention(q, cache, offsets([3], cuda), table, kl), q, cache, table, [3], [600], True, hd ** -0.5)
+    q = torch.randn(70, 16, hd, device=cuda).half()
+    check(cache_attention(q, cache, offsets([70], cuda), table, kl), q, cache, table, [70], [600], True, hd ** -0.5)
+
+
+@pytest.mark.parametrize("nq", [1, 40])
+def test_no_keys_at_all(cuda, nq):
+    """A table of no pages, a cache of none: only the shared prefix is seen, or nothing."""
+    from embodied_efficiency_b200 import KVCache, cache_attention
+    q, cache, cu, table, kl, pre = make(cuda, torch.bfloat16, 8, 8, 2, 64, 32, [nq] * 3, [nq] * 3, 5, 70)
+    none = KVCache.empty(0, 2, 64, 32)
+    for c, t in ((cache, table[:, :0]), (none, table), (none, table[:, :0])):
+        assert not bool(cache_attention(q, c, cu, t, kl).any())
+        check(cache_attention(q, c, cu, t, kl, prefix=pre), q, cache, table, [nq] * 3, [0] * 3, True, 64 ** -0.5, pre)
+    assert status() == 0
+
+
+@pytest.mark.parametrize("hq,hk,nq", [(130, 1, 2), (300, 1, 1), (128, 1, 3), (256, 2, 1), (127, 1, 2)])
+def test_wide_groups(cuda, hq, hk, nq):
+    """Groups that fill or do not fit a tile of 128 rows; above, a prefix is refused."""
+    from embodied_efficiency_b200 import cache_attention
+    q_len, k_len = [nq, 1, 0, nq], [300, 1, 5, 64]
+    q, cache, cu, table, kl, pre = make(cuda, torch.bfloat16, 4, hq, hk, 64, 64, q_len, k_len, 2, 150)
+    check(cache_attention(q, cache, cu, table, kl), q, cache, table, q_len, k_len, True, 0.125)
+    if hq // hk > 128:
+        with pytest.raises(ValueError, match="128"):
+            cache_attention(q, cache, cu, table, kl, prefix=pre)
+    else:
+        check(cache_attention(q, cache, cu, table, kl, prefix=pre), q, cache, table, q_len, k_len, True, 0.125, pre)
+    assert status() == 0
+
+
+@pytest.mark.parametrize("nq", [1, 9])
+def test_thousands_of_sequences(cuda, nq):
+    from embodied_efficiency_b200 import cache_attention
+    r = random.Random(nq)
+    k_len = [r.choice([0, 1, 9, 40, 70]) for _ in range(3000)]
+    q_len = [r.choice([0, nq, nq]) for _ in k_len]
+    q, cache, cu, table, kl, pre = make(cuda, torch.bfloat16, 8, 4, 2, 64, 32, q_len, k_len, 1, 40)
+    check(cache_attention(q, cache, cu, table, kl), q, cache, table, q_len, k_len, True, 0.125)
+    check(cache_attention(q, cache, cu, table, kl, prefix=pre), q, cache, table, q_len, k_len, True, 0.125, pre)
+    assert status() == 0
+
+
+def test_calls_at_once(cuda):
+    """Calls of every kernel and order on four streams from four threads give what each gives by itself."""
+    import threading
+    from embodied_efficiency_b200 import cache_attention
+    sets = [make(cuda, torch.bfloat16, 8, 8, 2, 64, 64, [n] * 20, [n + 37 * i for i in range(20)], n, 200) for n in (1, 3, 30, 60)]
+    want = [[cache_attention(*s[:5], prefix=p) for p in (None, s[5])] for s in sets]
+    torch.cuda.synchronize()
+    bad = []
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for k in range(40):
+                s = sets[(i + k) % 4]
+                for j, p in enumerate((None, s[5])):
+                    if not torch.equal(cache_attention(*s[:5], prefix=p), want[(i + k) % 4][j]):
+                        bad.append((i, k, j))
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad and status() == 0
 
 
 def test_views_streams_and_captures(cuda):
@@ -322,6 +388,9 @@ def test_views_streams_and_captures(cuda):
     assert cache_attention(q, cache, empty, table[:0], kl[:0], out=keep) is keep and bool((keep == 2).all())
     # a table of no pages: no keys
     assert not bool(cache_attention(q, cache, cu, table[:, :0], kl).any())
+    for scale in (0.0, 1e-40, float("nan"), float("inf"), -0.1):
+        with pytest.raises(ValueError, match="scale"):
+            cache_attention(q, cache, cu, table, kl, scale=scale)
     for shared in (q[:1].expand(6, 8, 128),):
         with pytest.raises(ValueError, match="overlap"):
             cache_attention(q, cache, cu, table, kl, out=shared)
