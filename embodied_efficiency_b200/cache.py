@@ -48,6 +48,8 @@ class KVCache:
         for t, n in ((k, "k"), (v, "v"), (k_scale, "k_scale"), (v_scale, "v_scale")):
             if not t.is_contiguous() or t.data_ptr() % 16:
                 raise ValueError(f"{n} must be contiguous and on a 16-byte boundary")
+            if t.requires_grad:
+                raise ValueError(f"{n} must not ask for a gradient: the cache is written in place")
         self.device = _lib.same_device(k, v, k_scale, v_scale)
         self._tensors = (k, v, k_scale, v_scale)
         self.pages, self.kv_heads, self.page_size, self.head_dim = pages, heads, size, hd

@@ -537,7 +537,9 @@ static int launch_prompt(const PromptArgs& a, const PromptPlan& pl, int hd, cuda
 
 // The sums of all tq rows as one sequence over all tk keys, left unfinished in
 // a.part and a.stat: what a caller joins with the keys of its own. The parts of
-// the keys are those that leave no SM idle, of 512 keys or more.
+// the keys are those that leave no SM idle, of 512 keys or more (64 x 1 token
+// behind 8192 shared keys, the rows' own keys beside them: 29 us, with 256 42, with
+// 1024 33).
 int prompt_sums_splits(long long tq, long long tk, int n_q, int n_kv) {
   const int group = n_q / n_kv, tpt = 128 / group;
   const long long items = (tq + 2 * tpt - 1) / (2 * tpt) * n_kv, want = device_sms() / items, most = tk / kPtMinKeys;

@@ -56,6 +56,7 @@ def test_cache_tensors():
             ("k_scale must be", lambda: KVCache(k, v, ks.half(), vs)),
             ("v_scale must be", lambda: KVCache(k, v, ks, vs[..., :16])),
             ("v must be contiguous", lambda: KVCache(k, v.transpose(0, 1).contiguous().transpose(0, 1), ks, vs)),
+            ("k_scale must not ask", lambda: KVCache(k, v, ks.clone().requires_grad_(), vs)),
             ("bits must be", lambda: KVCache.empty(3, 2, 64, bits=3, device="cpu"))):
         with pytest.raises(ValueError, match=match):
             call()
