@@ -28,14 +28,15 @@
 // Queries go into the product as fp16, bf16 ones scaled by a power of two so
 // that the row's largest lies in [1, 2): a value more than 2^14 below it loses
 // up to 2^-25 of the largest, less than fp32 loses in the sum. The weights times
-// the values' steps have fp32's range, so they are rounded to bf16 (2^-8 each,
-// in either direction, as the 16-bit kernels' weights); for fp16 outputs a
-// second product adds what the rounding left (to 2^-16).
+// the values' steps have fp32's range, so they are rounded to bf16, and a second
+// product adds what that left (to 2^-16): without it a row of few keys is off by
+// the same half step in all its dims, 1.6 times the result's own rounding (64 x 1
+// token: 23.6 us, with it 24.4).
 //
 // HBM-bound where the call is large (64 x 1 token behind 4096, 8 key heads of 128,
 // 8 bits: 5.5 TB/s; 4 bits, where the instructions on a code count: 3.9). In
-// between, instructions: 850 a step, two warps a scheduler (64 x 1 behind 1 to
-// 1632, 16 / 4 heads of 128, 8 bits: 23.8 us where the bytes take 9.6; twelve
+// between, instructions: about 900 a step, two warps a scheduler (64 x 1 behind 1 to
+// 1632, 16 / 4 heads of 128, 8 bits: 24.5 us where the bytes take 9.6; twelve
 // warps with rings two stages deep: 30.4 where eight took 28.7). A small call is
 // two launches, the sums and the join of rows that a border cut, and in each the
 // way through offsets, lengths and table to the codes: 9 us.
@@ -169,7 +170,7 @@ __global__ void __launch_bounds__(CaShape<HD, BITS, NT>::THREADS, 1)
   using S = CaShape<HD, BITS, NT>;
   constexpr int NTH = S::THREADS, NWK = S::WORKERS, NS = S::NS, RB = S::RB, TILE = S::TILE, R = S::ROWS;
   constexpr int CH = HD / 16;  // 16-dim pieces of a head: MMAs of K Q^T, tiles of O^T
-  constexpr bool SPLIT = std::is_same<T, __half>::value;
+  constexpr bool HALF = std::is_same<T, __half>::value;
   extern __shared__ __align__(1024) char smem_raw[];
   __shared__ PrList<NTH> sh;
   __shared__ __align__(8) uint64_t bars[NWK][NS];
@@ -306,7 +307,7 @@ __global__ void __launch_bounds__(CaShape<HD, BITS, NT>::THREADS, 1)
           }
         }
         float back = a.scale_log2;
-        if (SPLIT) {
+        if (HALF) {
 #pragma unroll
           for (int c = 0; c < CH; ++c) {
             qf[j][c][0] = w[c][0];
@@ -459,10 +460,8 @@ __global__ void __launch_bounds__(CaShape<HD, BITS, NT>::THREADS, 1)
           }
           const uint32_t hi = Act<__nv_bfloat16>::pack2(w0, w1);
           pb[mt][j][i] = movmatrix(hi);
-          if (SPLIT) {
-            const float2 f = Act<__nv_bfloat16>::unpack2(hi);
-            pl[mt][j][i] = movmatrix(Act<__nv_bfloat16>::pack2(w0 - f.x, w1 - f.y));
-          }
+          const float2 f = Act<__nv_bfloat16>::unpack2(hi);
+          pl[mt][j][i] = movmatrix(Act<__nv_bfloat16>::pack2(w0 - f.x, w1 - f.y));
         }
     }
 #pragma unroll
@@ -487,7 +486,7 @@ __global__ void __launch_bounds__(CaShape<HD, BITS, NT>::THREADS, 1)
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
               mma16816<__nv_bfloat16>(o[c][j], a0, a1, a2, a3, pb[mt][j][0], pb[mt][j][1]);
-              if (SPLIT) mma16816<__nv_bfloat16>(o[c][j], a0, a1, a2, a3, pl[mt][j][0], pl[mt][j][1]);
+              mma16816<__nv_bfloat16>(o[c][j], a0, a1, a2, a3, pl[mt][j][0], pl[mt][j][1]);
             }
           }
         }
