@@ -166,7 +166,8 @@ def cache_attention(q, cache: KVCache, cu_q, table, k_lens, causal: bool = True,
     sequence's length, under the mask or on pages that the cache does not have count with weight 0, whatever is there.
     One kernel serves the whole call, chosen by the mean of queries per sequence and key head. Returns [tokens, heads,
     head_dim], new or ``out`` (which shares no memory with the inputs); rows that belong to no sequence are not
-    written. bf16 / fp16."""
+    written. Sums are fp32, of weights up to 2^8 before they are divided: values beyond 2^100 can overflow in them.
+    bf16 / fp16."""
     if out is None and type(cache) is KVCache:
         done = (_lib._native or _lib.native()).cache_attention(cache.k, cache._at, q, cu_q, table, k_lens, causal, scale,
                                                                prefix)
