@@ -110,8 +110,11 @@ template <int HD, int BITS> constexpr uint32_t pt_off_info() {
 template <int HD, int BITS> constexpr uint32_t pt_off_beat() { return pt_off_info<HD, BITS>() + kPtInfo * 64; }  // blocks the MMA warp has come to
 // which keys of a block are there (4 words a block), which pieces of a tile of codes
 template <int HD, int BITS> constexpr uint32_t pt_off_there() { return pt_off_beat<HD, BITS>() + 16; }
-template <int HD, int BITS> constexpr uint32_t pt_off_half() {  // one tile's maxima and sums for the other, of two items
+template <int HD, int BITS> constexpr uint32_t pt_off_big() {  // fp16: which values of a block leave more to the weight than a factor below 2
   return pt_off_there<HD, BITS>() + (BITS ? kPtSteps * 16 + (pt_raws<HD, BITS>() * 4 + 15) / 16 * 16 : 0);
+}
+template <int HD, int BITS> constexpr uint32_t pt_off_half() {  // one tile's maxima and sums for the other, of two items
+  return pt_off_big<HD, BITS>() + (BITS ? kPtSteps * 16 : 0);
 }
 template <int HD, int BITS> constexpr uint32_t pt_smem() { return pt_off_half<HD, BITS>() + (BITS ? 2048 : 0) + 1024; }
 
@@ -227,7 +230,8 @@ EE_DEV float max3(float a, float b, float c) {
 // a value's its column of P after the sum is taken, so the weights that P V
 // rounds are the products: bf16 has room for them, fp16 gets the values as code
 // times a power of two, exactly, and the weights what that leaves of the step, a
-// factor below 2.
+// factor below 2 (or, for values beyond fp16's largest number, the excess too: see
+// where the reference moves).
 //
 // There an item is one tile, as a call's sequences rarely have two (50 tokens a
 // turn): its blocks take turns on the two halves' softmax warps and columns of
@@ -389,16 +393,18 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
               vs = 0.f;
             }
             steps[key] = ks * (p.scale_log2 * code_unit<T, BITS>());
-            if (POW2) {  // 2^e to the values, exactly: e from -24, where fp16 ends, to 15
-              const int e = min(max(((__float_as_int(vs) >> 23) & 0xff) - 127, -24), 15);
+            if (POW2) {  // 2^e to the values, exactly: e from -24, where fp16 ends, to where its largest number holds any code
+              const int e = min(max(((__float_as_int(vs) >> 23) & 0xff) - 127, -24), BITS == 8 ? 8 : 12);
               const __half2 v2 = __float2half2_rn(__int_as_float((127 + e) << 23));
               steps[256 + key] = __uint_as_float(*reinterpret_cast<const uint32_t*>(&v2));
               vs *= __int_as_float((127 - e) << 23);
             }
             steps[128 + key] = vs * code_unit<T, BITS>();
-            const uint32_t all = __ballot_sync(0xffffffffu, have);
-            if (lane == 0)
+            const uint32_t all = __ballot_sync(0xffffffffu, have), big = POW2 ? __ballot_sync(0xffffffffu, fabsf(vs) >= 2.f) : 0u;
+            if (lane == 0) {
               *reinterpret_cast<volatile uint32_t*>(smem + pt_off_there<HD, BITS>() + (blk % kPtSteps) * 16 + quarter * 4) = all;
+              if (POW2) *reinterpret_cast<volatile uint32_t*>(smem + pt_off_big<HD, BITS>() + (blk % kPtSteps) * 16 + quarter * 4) = big;
+            }
             __syncwarp();
             if (lane == 0) mbar_arrive(b_st + 8 * (blk % kPtSteps));
           }
@@ -969,7 +975,25 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
 #pragma unroll
           for (int e = 2; e < 32; e += 2) x[c] = max3(x[c], __uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1]));
         }
-        const float mx = fmaxf(max3(x[0], x[1], x[2]), x[3]) * (BITS ? 1.f : p.scale_log2);  // a cache's steps have it in them
+        float mx = fmaxf(max3(x[0], x[1], x[2]), x[3]) * (BITS ? 1.f : p.scale_log2);  // a cache's steps have it in them
+        if (POW2) {
+          // steps beyond what the values take are the weights': the reference is the largest score with that excess in it,
+          // so that the products with them stay in fp16's range
+          const uint4 big = lds16(sb + pt_off_big<HD, BITS>() + ((bs + j) % kPtSteps) * 16);
+          if (big.x | big.y | big.z | big.w) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int e = 0; e < 32; e += 4) {
+                const float4 r = steps[32 + 8 * c + e / 4];
+                auto with = [](uint32_t s, float y) {  // y < 2^(n + 1)
+                  return __uint_as_float(s) + (float)max(((__float_as_int(y) >> 23) & 0xff) - 127, 0);
+                };
+                mx = max3(mx, with(v[c][e], r.x), with(v[c][e + 1], r.y));
+                mx = max3(mx, with(v[c][e + 2], r.z), with(v[c][e + 3], r.w));
+              }
+          }
+        }
         float f = 1.f;
         if (mx > top) {  // also from -inf, with f = 0: nothing to rescale yet
           const float to = prompt_reference<T, 7>(mx);
