@@ -387,8 +387,9 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
             const int key = 32 * quarter + lane;
             const bool have = key0 + j * kPtKeys + key < klen && (there >> (key >> shift) & 1);
             float ks = have ? raw_steps[key] : 0.f, vs = have ? raw_steps[128 + key] : 0.f;
-            // a value's step that is no number must reach the rows that see it and no others: as its key's
-            if (!(fabsf(vs) <= 3.4028234e38f)) {
+            // a value's step that is no number, or none with the unit in it, must reach the rows that see it and no others:
+            // as its key's
+            if (!(fabsf(vs * code_unit<T, BITS>()) <= 3.4028234e38f)) {
               ks = __int_as_float(0x7fffffff);
               vs = 0.f;
             }

@@ -74,3 +74,18 @@ def test_steps_that_fp16_does_not_hold(cuda, bits, hd, q_len, k_len, prefix):
     out = cache_attention(q, cache, cu, table, kl, prefix=pre)
     check_visible(out, q, cache, table, q_len, k_len, scale, pre)
     assert status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("nq", [3, 20])
+@pytest.mark.parametrize("which", ["k_scale", "v_scale"])
+def test_the_largest_steps_under_the_mask(cuda, dtype, bits, hd, nq, which):
+    """A step near fp32's largest number on one key reaches no row that does not see it."""
+    from embodied_efficiency_b200 import cache_attention
+    q, cache, cu, table, kl, _ = make(cuda, dtype, bits, 2, 1, hd, 32, [nq], [50], 4)
+    out = cache_attention(q, cache, cu, table, kl)
+    getattr(cache, which)[table[0, 1], 0, 48 - 32] = 2.0 ** 127  # key 48: not seen by queries before the last but one
+    assert torch.equal(cache_attention(q, cache, cu, table, kl)[:nq - 2], out[:nq - 2]) and bool(out.isfinite().all())
+    assert status() == 0
