@@ -66,6 +66,7 @@ size_t ee_cache_attention_workspace_bytes(int64_t tq, int32_t n_seq, int32_t n_q
                                           int32_t bits, int64_t keys, int64_t prefix_len) {
   if (tq < 1 || n_seq < 1 || n_q < 1 || n_kv < 1 || n_q % n_kv || keys < 0 || prefix_len < 0 || tq > 0x7fffff00 / n_q) return 0;
   if ((head_dim != 64 && head_dim != 128) || (bits != 8 && bits != 4)) return 0;
+  if (prefix_len && n_q / n_kv > 128) return 0;  // the call refuses it
   const CacheParts c = cache_parts(cache_plan(tq, n_seq, n_q, n_kv, keys), tq, n_q, n_kv, head_dim, bits, prefix_len);
   return (size_t)(c.own + c.pre) * (head_dim + 2) * 4;
 }

@@ -177,3 +177,14 @@ def test_abi_codes(lib):
                 (5, 1, 4, 2, 64, 16, 128, 0), (1 << 30, 1, 4, 2, 64, 8, 128, 0), (5, 1, 4, 2, 64, 8, 128, -1),
                 (5, 1, 4, 2, 64, 8, -1, 0)):
         assert need(*bad) == 0
+
+
+def test_workspace_of_calls_that_are_refused(lib):
+    """Heads that a call with a prefix does not take: no workspace, and no division by their tile's tokens."""
+    need = lib.ee_cache_attention_workspace_bytes
+    for n_q, n_kv in ((260, 2), (129, 1), (65535, 1)):
+        for tq in (1, 5, 1000):
+            for bits in (8, 4):
+                assert need(tq, 1, n_q, n_kv, 64, bits, 128, 7) == 0
+                assert need(tq, 1, n_q, n_kv, 64, bits, 128, 0) > 0
+    assert need(5, 1, 256, 2, 64, 8, 128, 7) > 0
