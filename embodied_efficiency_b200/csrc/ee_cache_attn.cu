@@ -15,8 +15,7 @@ int prompt_parts(long long tq, int n_seq, int n_q, int n_kv, long long keys, int
 int launch_prompt_sums(const PromptArgs& a, int head_dim, int act_dtype, cudaStream_t s);
 int launch_prompt_more(const PromptArgs& a, const PromptMore& more, int head_dim, int act_dtype, cudaStream_t s);
 int launch_prompt_combine(const PromptArgs& a, int head_dim, int act_dtype, cudaStream_t s);
-
-constexpr unsigned long long kCacheWaitNs = 1000000000ull;
+unsigned long long attention_wait_limit();
 
 // How a call runs, by its mean of rows (queries x group) per sequence and key
 // head: up to 8, one MMA column tile a warp; up to 16, two; above, the
@@ -162,7 +161,7 @@ int ee_cache_attention(const ee_cache* cache, const void* q, int64_t q_tok, int6
       a.pre_ctas = items < 0x7fffffff ? (int)items : 0x7fffffff;
     }
     a.status = status;
-    a.timeout_ns = kCacheWaitNs;
+    a.timeout_ns = attention_wait_limit();
     if (act_dtype == EE_BF16)
       return hd == 64 ? launch_cache_few<__nv_bfloat16, 64>(m, a, plan, cache->bits, s)
                       : launch_cache_few<__nv_bfloat16, 128>(m, a, plan, cache->bits, s);
@@ -185,7 +184,7 @@ int ee_cache_attention(const ee_cache* cache, const void* q, int64_t q_tok, int6
   t.p = p;
   t.tpt = 128 / p.group;
   t.status = status;
-  t.timeout_ns = kCacheWaitNs;
+  t.timeout_ns = attention_wait_limit();
   t.c = a.c;
   t.k_steps = cache->k_steps; t.v_steps = cache->v_steps;
   if (act_dtype == EE_BF16)

@@ -501,6 +501,7 @@ bool prompt_head_map(CUtensorMap* map, const void* base, int hd, int heads, long
 
 constexpr unsigned long long kPtWaitNs = 1000000000ull;
 static std::atomic<unsigned long long> g_wait_limit{kPtWaitNs};
+unsigned long long attention_wait_limit() { return g_wait_limit.load(std::memory_order_relaxed); }  // ee_cache_attn.cu's too
 
 template <typename T, int HD, bool JOIN = false>
 static int launch_tc(const PromptArgs& p, cudaStream_t s, const PromptMore* more = nullptr) {
@@ -513,7 +514,7 @@ static int launch_tc(const PromptArgs& p, cudaStream_t s, const PromptMore* more
   a.p = p;
   a.tpt = 128 / p.group;
   a.status = gemm_status_ptr();
-  a.timeout_ns = g_wait_limit.load(std::memory_order_relaxed);
+  a.timeout_ns = attention_wait_limit();
   if (JOIN) a.more = *more;
   if (!a.status) return EE_ERR_DEVICE;
   CUtensorMap mq, mk, mv;

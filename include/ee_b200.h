@@ -262,8 +262,8 @@ int ee_prompt_attention(const void* q, int64_t q_tok, int64_t q_head, const void
                         const int32_t* cu_q, const int32_t* cu_k, const int32_t* k_lens, int64_t tq, int64_t tk,
                         int32_t n_seq, int32_t n_q, int32_t n_kv, int32_t head_dim, int32_t causal, float scale,
                         int32_t act_dtype, void* workspace, size_t workspace_bytes, ee_stream_t stream);
-/* Limit of the waits inside the tensor-core attention kernel from the next
- * launch on, for the whole process: a wait without progress for `ns` (0: the
+/* Limit of the waits inside the attention kernels (ee_prompt_attention,
+ * ee_cache_attention) from the next launch on, for the whole process: a wait without progress for `ns` (0: the
  * default, 1 s) gives up, the launch ends with its outputs unfinished and
  * EE_ERR_TIMEOUT in the status word of ee_wq_gemm_status. */
 int ee_prompt_attention_wait_limit(uint64_t ns);
@@ -316,8 +316,9 @@ int ee_cache_read(const ee_cache* cache, void* k, int64_t k_tok, int64_t k_head,
  * 2^31 - 255. scale as for ee_prompt_attention.
  * workspace: ee_cache_attention_workspace_bytes() bytes (keys = width *
  * page_size), 16-byte aligned (may be NULL when that is 0); calls
- * that may overlap need one each. A wait that gives up after a second leaves
- * EE_ERR_TIMEOUT in the status word of ee_wq_gemm_status. */
+ * that may overlap need one each. A wait that gives up (a second, or as
+ * ee_prompt_attention_wait_limit says) leaves EE_ERR_TIMEOUT in the status word
+ * of ee_wq_gemm_status. */
 size_t ee_cache_attention_workspace_bytes(int64_t tq, int32_t n_seq, int32_t n_q, int32_t n_kv, int32_t head_dim,
                                           int32_t bits, int64_t keys, int64_t prefix_len);
 int ee_cache_attention(const ee_cache* cache, const void* q, int64_t q_tok, int64_t q_head, void* out, int64_t o_tok,
