@@ -164,7 +164,10 @@ def cache_attention(q, cache: KVCache, cu_q, table, k_lens, causal: bool = True,
     ``h // (heads // kv_heads)``; at most 128 heads a key head with a prefix. With ``causal`` a sequence's last query
     sees its last key; a query that sees no key gives zeros. ``scale`` defaults to head_dim^-0.5. Keys past a
     sequence's length, under the mask or on pages that the cache does not have count with weight 0, whatever is there.
-    One kernel serves the whole call, chosen by the mean of queries per sequence and key head. Returns [tokens, heads,
+    One kernel serves the whole call, chosen by the mean of queries per sequence and key head: a long turn among many
+    single tokens is faster in a call of its own. Lengths that the table cuts count as cut, for the mask too. For their
+    product with the values the weights keep 16 bits or more (up to 16 queries x heads a sequence and key head, no prefix)
+    or are rounded to q's type once, which about doubles the squared error that the result's rounding leaves. Returns [tokens, heads,
     head_dim], new or ``out`` (which shares no memory with the inputs); rows that belong to no sequence are not
     written. Sums are fp32, of weights up to 2^8 before they are divided: values beyond 2^100 can overflow in them.
     bf16 / fp16."""

@@ -12,9 +12,10 @@
 // place is looked up (a search over the offsets and one entry of the table).
 //
 // Measured: 128 prompts of 257 to 816 tokens, 16 heads of 64, written in 8 bits in
-// 79 us (5.6 TB/s of the 6.46 that a copy reaches); 64 such prompts, heads of 128,
-// read in 73 (6.0); 64 x 1 token written in 3.5, a launch. Several tokens a warp
-// were slower in either direction.
+// 82 us (5.4 TB/s of the 6.46 that a copy reaches); 64 such prompts, heads of 128,
+// read in 73 (6.0); 64 x 1 token written in 3.3, a launch. In 4 bits the write takes
+// what it takes in 8 (instructions a value), the read 0.92 of it. Several tokens a
+// warp were slower in either direction.
 #include "ee_cache.cuh"
 #include "ee_host.h"
 

@@ -20,7 +20,11 @@ unsigned long long attention_wait_limit();
 // How a call runs, by its mean of rows (queries x group) per sequence and key
 // head: up to 8, one MMA column tile a warp; up to 16, two; above, the
 // tensor-core kernel's 128-row tiles (64 x 50 rows behind 257..816, 16 heads of
-// 128: the kernel for few rows in 64-row items took 239 us).
+// 128: the kernel for few rows in 64-row items took 239 us). One kernel serves the
+// whole call: 63 single tokens behind 1..1632 beside one turn of 1024 tokens, 16 /
+// 4 heads of 128, take 81 us, as two calls 22 + 36; beside a turn of 200 54, as two
+// 22 + 20. Which tokens to put together is the caller's to say: the host does not
+// know the lengths.
 static CachePlan cache_plan(long long tq, int n_seq, int n_q, int n_kv, long long keys) {
   const int group = n_q / n_kv;
   const long long rows = tq * group;

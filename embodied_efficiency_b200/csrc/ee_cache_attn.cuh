@@ -35,7 +35,8 @@
 //
 // HBM-bound where the call is large (64 x 1 token behind 4096, 8 key heads of 128,
 // 8 bits: 5.5 TB/s; 4 bits, where the instructions on a code count: 3.9). In
-// between, instructions: 850 a step and the second product, two warps a scheduler (64 x 1 behind 1 to
+// between, latency: 850 instructions a step and the second product by two warps a
+// scheduler, whose issue slots are 23 % busy over the launch (64 x 1 behind 1 to
 // 1632, 16 / 4 heads of 128, 8 bits: 24.5 us where the bytes take 9.6; twelve
 // warps with rings two stages deep: 30.4 where eight took 28.7). A small call is
 // two launches, the sums and the join of rows that a border cut, and in each the

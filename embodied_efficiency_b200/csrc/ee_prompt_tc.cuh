@@ -40,7 +40,9 @@
 // may be rescaled.
 //
 // Persistent: one CTA per SM takes items c, 2G - 1 - c, 2G + c, ... of the G
-// CTAs (a snake, longest items first), and the next item's loads and first
+// CTAs (a snake, from the last sequence's last rows up: longest items first within
+// a causal prompt, but a batch's sequences in their order, whatever their lengths),
+// and the next item's loads and first
 // scores run under the current one's last products and output. Warps 0-3 and
 // 4-7: softmax and output of tile 0 and 1; warp 8: finds the items, publishes
 // them in a shared-memory ring and loads Q, K and V by TMA; warp 9: MMA issue;
@@ -231,7 +233,8 @@ EE_DEV float max3(float a, float b, float c) {
 // rounds are the products: bf16 has room for them, fp16 gets the values as code
 // times a power of two, exactly, and the weights what that leaves of the step, a
 // factor below 2 (or, for values beyond fp16's largest number, the excess too: see
-// where the reference moves).
+// where the reference moves). Weights that end below fp16's 2^-14 lose up to 2^-25
+// each beside a largest one of 2^7 or more.
 //
 // There an item is one tile, as a call's sequences rarely have two (50 tokens a
 // turn): its blocks take turns on the two halves' softmax warps and columns of
@@ -246,7 +249,13 @@ EE_DEV float max3(float a, float b, float c) {
 // and values in 16 bits: 88 and 134. Without decoding, steps and exponentials the
 // rest takes 86 and 117: what bounds it is the round trip of scores, softmax and
 // products of a lone tile, whose 50 rows are two warps of four, then the decoding
-// (2 x 128 x 128 codes a block by four warps) and the steps' multiplications. Not
+// (2 x 128 x 128 codes a block by four warps) and the steps' multiplications; and
+// the uneven end: the fullest CTA has 42 blocks where 35.2 are the mean, and 100 where
+// 81.4 are. P times the steps is rounded once, so results are off by 1.35 to 1.4
+// times a plain fp32 form's rounding (bf16: 2.2e-3 to 1.7e-3 relative), in rows of
+// few keys by one factor for all dims; a second product for what the rounding left
+// (as in ee_cache_attn.cuh) ends that and takes 139 us where this takes 120, and 217
+// where this takes 179. Not
 // faster: K and V decoded by two warps each (118 -> 136), S read twice by halves,
 // without spills (118 -> 130, 179 -> 200).
 //

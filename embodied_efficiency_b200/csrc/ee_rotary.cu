@@ -20,9 +20,10 @@
 // Measured: 65537 tokens, 16 + 8 heads of 64: 65 us, 6.2 TB/s, 0.94 of the
 // copy rate; 6528 tokens, 16 + 16 heads of 128: 17 us.
 //
-// The norm, y = w x / sqrt(mean(x^2) + eps), is taken in fp32 on the 16 values
-// that a lane holds of a head anyway, their squares summed over the head's hd /
-// 16 lanes by shuffles: one rounding, at the end, and no pass of its own.
+// The norm, y = w x / sqrt(mean(x^2) + eps), is taken in fp32 on the 8 values that
+// a lane of norm_rotary_kernel holds of a head, their squares summed over the
+// head's hd / 8 lanes by shuffles: one rounding, at the end, and no pass of its
+// own.
 #include <cfloat>
 #include <type_traits>
 
@@ -158,8 +159,9 @@ __global__ void __launch_bounds__(kRotWarps * 32) rotary_kernel(const __grid_con
 // The same behind a norm of each head. Queries and keys by turns, as their
 // weights differ, the weights multiplied into the turn's coefficients once for a
 // token. A lane has four pairs of a head (8-byte loads): with eight, as above,
-// the coefficients leave 20 warps an SM and 80 us where these take 69 (65537
-// tokens, 16 + 8 heads of 64; 5.8 TB/s); UN passes of HL heads are in flight.
+// the coefficients leave 20 warps an SM and 80 us where these took 69 (65537
+// tokens, 16 + 8 heads of 64, the same ones again and again; 75 us on tensors
+// that change from call to call, 5.4 TB/s); UN passes of HL heads are in flight.
 template <typename T, int HD>
 __global__ void __launch_bounds__(kRotWarps * 32, 8) norm_rotary_kernel(const __grid_constant__ RotaryArgs a) {
   constexpr int HALF = HD / 2, CH = HALF / 4, HL = 32 / CH, UN = 4;

@@ -360,7 +360,8 @@ class ActionExpert(nn.Module):
         ``encode``'s and run layer by layer, the cross-attention on ``prompt_attention`` (so heads of 64 or 128, in bf16
         or fp16). With ``kv_bits`` 8 or 4 the K/V are held as codes in a ``KVCache`` of ``page_size`` tokens a page per
         layer (0.53 or 0.28 of the 16-bit bytes with heads of 64, and the unused ends of last pages), the
-        cross-attention then runs on ``cache_attention``; making the table waits for ``cu`` once."""
+        cross-attention then runs on ``cache_attention``; making the table waits for ``cu`` once, and codes carry no
+        gradient, whatever ``prefix`` asks for."""
         prefix = prefix.to(self.out_norm.weight.dtype)
         if kv_bits is not None:
             if kv_bits not in (8, 4):

@@ -53,7 +53,9 @@ class FleetSampler:
     ``request_fn(i)`` returns request i's (prefix [1, P, d], noise [1, H, A]);
     with an ``expert``, P may differ between the requests of a chunk, whose
     prefixes are then packed without padding (``ActionExpert.encode_packed``)
-    (``kv_bits`` 8 or 4 holds every chunk's prefix K/V as codes)
+    (``kv_bits`` 8 or 4 holds every chunk's prefix K/V as codes, for less memory:
+    chunks then run layer by layer also where their prefixes are of one length
+    and the single launch would take them)
     (the caller decides where requests come from; ``synth.fleet_request``
     gives the seeded synthetic fleet). With an
     ``expert`` the chunks run through ``flow_sample`` (one fused launch per

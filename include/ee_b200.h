@@ -308,11 +308,12 @@ int ee_cache_read(const ee_cache* cache, void* k, int64_t k_tok, int64_t k_head,
  * [prefix_len][kv_heads][head_dim] in the act dtype that every sequence shares
  * (0: none; n_q / kv_heads at most 128 with one). Head h reads key head
  * h / (n_q / kv_heads). causal: a sequence's last query sees its last key, query
- * i keys 0 .. k_lens[b] - n + i and the prefix. A query that sees no key gives
+ * i keys 0 .. k_lens[b] - n + i (k_lens as the table cuts it) and the prefix. A query that sees no key gives
  * zeros; rows of `out` that belong to no sequence stay as they were. A key's
  * code * step counts as it is (NaN where its head held an infinity or NaN), with
- * fp32 statistics and sums; weights are rounded to 16 bits (fp16: twice) for
- * the product with the values. Strides in elements, multiples of 8. tq * n_q <
+ * fp32 statistics and sums. For the product with the values the weights are two
+ * 16-bit terms where a call has up to 16 queries x heads per sequence and key
+ * head on average, else, and over the prefix, rounded to 16 bits once. Strides in elements, multiples of 8. tq * n_q <
  * 2^31 - 255. scale as for ee_prompt_attention.
  * workspace: ee_cache_attention_workspace_bytes() bytes (keys = width *
  * page_size), 16-byte aligned (may be NULL when that is 0); calls
