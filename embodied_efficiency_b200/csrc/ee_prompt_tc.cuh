@@ -112,11 +112,11 @@ template <int HD, int BITS> constexpr uint32_t pt_off_info() {
 template <int HD, int BITS> constexpr uint32_t pt_off_beat() { return pt_off_info<HD, BITS>() + kPtInfo * 64; }  // blocks the MMA warp has come to
 // which keys of a block are there (4 words a block), which pieces of a tile of codes
 template <int HD, int BITS> constexpr uint32_t pt_off_there() { return pt_off_beat<HD, BITS>() + 16; }
-template <int HD, int BITS> constexpr uint32_t pt_off_big() {  // fp16: which values of a block leave more to the weight than a factor below 2
+template <int HD, int BITS> constexpr uint32_t pt_off_odd() {  // which values of a block leave other factors to the weight than below 2
   return pt_off_there<HD, BITS>() + (BITS ? kPtSteps * 16 + (pt_raws<HD, BITS>() * 4 + 15) / 16 * 16 : 0);
 }
 template <int HD, int BITS> constexpr uint32_t pt_off_half() {  // one tile's maxima and sums for the other, of two items
-  return pt_off_big<HD, BITS>() + (BITS ? kPtSteps * 16 : 0);
+  return pt_off_odd<HD, BITS>() + (BITS ? kPtSteps * 16 : 0);
 }
 template <int HD, int BITS> constexpr uint32_t pt_smem() { return pt_off_half<HD, BITS>() + (BITS ? 2048 : 0) + 1024; }
 
@@ -230,11 +230,15 @@ EE_DEV float max3(float a, float b, float c) {
 // time; warps 12-15 turn them into 16-bit tiles in the slots, exactly, two of K
 // and two of V, and hand on the steps. A key's step multiplies its column of S,
 // a value's its column of P after the sum is taken, so the weights that P V
-// rounds are the products: bf16 has room for them, fp16 gets the values as code
-// times a power of two, exactly, and the weights what that leaves of the step, a
-// factor below 2 (or, for values beyond fp16's largest number, the excess too: see
-// where the reference moves). Weights that end below fp16's 2^-14 lose up to 2^-25
-// each beside a largest one of 2^7 or more.
+// rounds are the products. That product is in fp16 whatever the call's type, for
+// the weights' 11 bits: the values are code times a power of two, exactly, and the
+// weights take what that leaves of the step, a factor below 2 (or, for values
+// beyond fp16's largest number and far below its smallest, the rest too: see where
+// the reference moves). In bf16 the result's rounding is eight times the weights',
+// with weights in bf16 the two together were 1.4 times it, and in rows of few keys
+// one factor for all dims; in fp16 the two are of one size. Weights that end below
+// 2^-14 lose up to 2^-25 each beside a largest one of 2^7 or more. (Weights in bf16
+// took 119 and 179 us where these take 116 and 187; two products of them, 139 and 217.)
 //
 // There an item is one tile, as a call's sequences rarely have two (50 tokens a
 // turn): its blocks take turns on the two halves' softmax warps and columns of
@@ -244,18 +248,14 @@ EE_DEV float max3(float a, float b, float c) {
 // the first's keys where it is empty: 150 and 207 us where this took 129 and 184
 // in the first two cases below.)
 //
-// Measured, heads of 128, 8 bits: 64 x 50 tokens behind 257 to 816, 16 heads: 119
-// us; 4 x 500 to 1024 behind 1 to 4096, 16 / 4 heads: 178, 550 TFLOP/s; with keys
+// Measured, heads of 128, 8 bits: 64 x 50 tokens behind 257 to 816, 16 heads: 116
+// us; 4 x 500 to 1024 behind 1 to 4096, 16 / 4 heads: 187, 525 TFLOP/s; with keys
 // and values in 16 bits: 88 and 134. Without decoding, steps and exponentials the
 // rest takes 86 and 117: what bounds it is the round trip of scores, softmax and
 // products of a lone tile, whose 50 rows are two warps of four, then the decoding
 // (2 x 128 x 128 codes a block by four warps) and the steps' multiplications; and
 // the uneven end: the fullest CTA has 42 blocks where 35.2 are the mean, and 100 where
-// 81.4 are. P times the steps is rounded once, so results are off by 1.35 to 1.4
-// times a plain fp32 form's rounding (bf16: 2.2e-3 to 1.7e-3 relative), in rows of
-// few keys by one factor for all dims; a second product for what the rounding left
-// (as in ee_cache_attn.cuh) ends that and takes 139 us where this takes 120, and 217
-// where this takes 179. Not
+// 81.4 are. Not
 // faster: K and V decoded by two warps each (118 -> 136), S read twice by halves,
 // without spills (118 -> 130, 179 -> 200).
 //
@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
   constexpr bool SEP = HD == 64;
   // pieces in which a block's weights are handed over (in one piece, hd 64: 501 instead of 411 us for 8192 tokens)
   constexpr int PARTS = 2;
-  constexpr bool POW2 = BITS && std::is_same<T, __half>::value;  // the values' steps are halved: P takes what a power of two leaves
+  using PT = typename std::conditional<BITS != 0, __half, T>::type;  // what P and V are in their product
   extern __shared__ __align__(1024) char smem_raw[];
   const uint32_t base0 = smem_u32(smem_raw);
   const uint32_t sb = (base0 + 1023u) & ~1023u;
@@ -360,7 +360,10 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
       constexpr int RB = HD * BITS / 8;                    // bytes of a row of codes
       constexpr int PER_ROW = RB < 64 ? RB / 16 : 4;       // lanes on a row; a row of 128 bytes takes two of its pieces
       constexpr int ROWS = 32 / PER_ROW, HALVES = RB / 16 / PER_ROW, PIECES = 32 / ROWS * HALVES;
-      constexpr int BATCH = PIECES < 4 ? PIECES : 4;       // pieces under way at once
+      // pieces under way at once, in a loop: unrolled whole, the two ways of decoding and the softmax do not fit the
+      // instruction cache together (bf16, heads of 128: 64 x 50 tokens 137 us, 4 x 500..1024 192; so 116 and 187; of 64
+      // with one, 99 and 167, with two 102 and 165)
+      constexpr int BATCH = PIECES < 8 ? 1 : 2;
       const int quarter = warp - 12, row0 = 32 * quarter + lane / PER_ROW, q0 = lane % PER_ROW;
       const uint32_t from = sb + pt_off_raw<HD, BITS>() + row0 * RB + q0 * 16;
       uint32_t to[16 / BITS];  // where the 16-bit pieces of the lane's first piece go
@@ -396,63 +399,70 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
             const int key = 32 * quarter + lane;
             const bool have = key0 + j * kPtKeys + key < klen && (there >> (key >> shift) & 1);
             float ks = have ? raw_steps[key] : 0.f, vs = have ? raw_steps[128 + key] : 0.f;
-            // a value's step that is no number, or none with the unit in it, must reach the rows that see it and no others:
-            // as its key's
-            if (!(fabsf(vs * code_unit<T, BITS>()) <= 3.4028234e38f)) {
+            // a value's step that is no number must reach the rows that see it and no others: as its key's
+            if (!(fabsf(vs) <= 3.4028234e38f)) {
               ks = __int_as_float(0x7fffffff);
               vs = 0.f;
             }
             steps[key] = ks * (p.scale_log2 * code_unit<T, BITS>());
-            if (POW2) {  // 2^e to the values, exactly: e from -24, where fp16 ends, to where its largest number holds any code
-              const int e = min(max(((__float_as_int(vs) >> 23) & 0xff) - 127, -24), BITS == 8 ? 8 : 12);
-              const __half2 v2 = __float2half2_rn(__int_as_float((127 + e) << 23));
-              steps[256 + key] = __uint_as_float(*reinterpret_cast<const uint32_t*>(&v2));
-              vs *= __int_as_float((127 - e) << 23);
-            }
-            steps[128 + key] = vs * code_unit<T, BITS>();
-            const uint32_t all = __ballot_sync(0xffffffffu, have), big = POW2 ? __ballot_sync(0xffffffffu, fabsf(vs) >= 2.f) : 0u;
+            // 2^e to the values, exactly: e from -24, where fp16 ends, to where its largest number holds any code
+            const int e = min(max(((__float_as_int(vs) >> 23) & 0xff) - 127, -24), BITS == 8 ? 8 : 12);
+            const __half2 v2 = __float2half2_rn(__int_as_float((127 + e) << 23));
+            vs *= __int_as_float((127 - e) << 23);
+            steps[128 + key] = vs;
+            steps[256 + key] = __uint_as_float(*reinterpret_cast<const uint32_t*>(&v2));
+            const uint32_t all = __ballot_sync(0xffffffffu, have);
+            const uint32_t odd = __ballot_sync(0xffffffffu, fabsf(vs) >= 2.f || (fabsf(vs) < 0.00390625f && vs != 0.f));
             if (lane == 0) {
               *reinterpret_cast<volatile uint32_t*>(smem + pt_off_there<HD, BITS>() + (blk % kPtSteps) * 16 + quarter * 4) = all;
-              if (POW2) *reinterpret_cast<volatile uint32_t*>(smem + pt_off_big<HD, BITS>() + (blk % kPtSteps) * 16 + quarter * 4) = big;
+              *reinterpret_cast<volatile uint32_t*>(smem + pt_off_odd<HD, BITS>() + (blk % kPtSteps) * 16 + quarter * 4) = odd;
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(b_st + 8 * (blk % kPtSteps));
           }
           const uint32_t raw = from + rs * pt_raw<HD, BITS>(), dst = at * TILE;
+          auto decode = [&](auto type, auto value) {
+            using U = decltype(type);
+#pragma unroll 1
+            for (int e0 = 0; e0 < PIECES; e0 += BATCH) {
+              uint4 x[BATCH];
 #pragma unroll
-          for (int e0 = 0; e0 < PIECES; e0 += BATCH) {
-            uint4 x[BATCH];
+              for (int u = 0; u < BATCH; ++u) x[u] = lds16(raw + (e0 + u) / HALVES * (ROWS * RB) + (e0 + u) % HALVES * 64);
+              uint32_t by[BATCH];
 #pragma unroll
-            for (int u = 0; u < BATCH; ++u) x[u] = lds16(raw + (e0 + u) / HALVES * (ROWS * RB) + (e0 + u) % HALVES * 64);
+              for (int u = 0; u < BATCH; ++u)
+                if (decltype(value)::value) by[u] = __float_as_uint(steps[256 + row0 + (e0 + u) / HALVES * ROWS]);
 #pragma unroll
-            for (int u = 0; u < BATCH; ++u) {
-              const int e = e0 + u;
-              const uint32_t xw[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
-              uint32_t o[64 / BITS];  // pairs
+              for (int u = 0; u < BATCH; ++u) {
+                const int e = e0 + u;
+                const uint32_t xw[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+                uint32_t o[64 / BITS];  // pairs
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                if (BITS == 8) {
-                  const uint32_t f = xw[k] ^ 0x80808080u;
-                  o[2 * k] = code_pair8<T>(f, 0);
-                  o[2 * k + 1] = code_pair8<T>(f, 1);
-                } else {
+                for (int k = 0; k < 4; ++k) {
+                  if (BITS == 8) {
+                    const uint32_t f = xw[k] ^ 0x80808080u;
+                    o[2 * k] = code_pair8<U>(f, 0);
+                    o[2 * k + 1] = code_pair8<U>(f, 1);
+                  } else {
 #pragma unroll
-                  for (int b = 0; b < 4; ++b) o[4 * k + b] = code_pair4<T>(xw[k], xw[k] >> 4, b);
+                    for (int b = 0; b < 4; ++b) o[4 * k + b] = code_pair4<U>(xw[k], xw[k] >> 4, b);
+                  }
                 }
-              }
-              if (POW2 && isv) {
-                const uint32_t s2 = __float_as_uint(steps[256 + row0 + e / HALVES * ROWS]);
+                if (decltype(value)::value) {
 #pragma unroll
-                for (int k = 0; k < 64 / BITS; ++k) o[k] = fma2<T>(o[k], s2, 0u);
-              }
+                  for (int k = 0; k < 64 / BITS; ++k) o[k] = fma2<U>(o[k], by[u], 0u);
+                }
 #pragma unroll
-              for (int k = 0; k < 16 / BITS; ++k)
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to[k] + dst + e / HALVES * (ROWS * 128) +
-                                                                              e % HALVES * PANEL),
-                             "r"(o[4 * k]), "r"(o[4 * k + 1]), "r"(o[4 * k + 2]), "r"(o[4 * k + 3])
-                             : "memory");
+                for (int k = 0; k < 16 / BITS; ++k)
+                  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to[k] + dst + e / HALVES * (ROWS * 128) +
+                                                                                e % HALVES * PANEL),
+                               "r"(o[4 * k]), "r"(o[4 * k + 1]), "r"(o[4 * k + 2]), "r"(o[4 * k + 3])
+                               : "memory");
+              }
             }
-          }
+          };
+          if (isv) decode(PT(), std::true_type());
+          else decode(T(), std::false_type());
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
@@ -680,7 +690,7 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
       // ---------------- MMA issue (all lanes run the loops, see elect_one) ----------------
       // The tensor cores queue about two MMAs beyond the running one and a wait costs 100 cycles or more even when
       // it is over, so the issuer's waits are few: one for V(j) and K(j + 1) together, then the weights.
-      constexpr uint32_t id_s = umma_idesc<T>(128, 128), id_o = umma_idesc<T>(128, HD) | kIdescBMajorMN;
+      constexpr uint32_t id_s = umma_idesc<T>(128, 128), id_o = umma_idesc<PT>(128, HD) | kIdescBMajorMN;
       const uint64_t q_desc = umma_desc_sw128(sQ), k_desc = umma_desc_sw128(sKV), v_desc = umma_desc_mn128(sKV, PANEL);
       auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, a.timeout_ns)); };
       bool ok = true;
@@ -986,18 +996,19 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
           for (int e = 2; e < 32; e += 2) x[c] = max3(x[c], __uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1]));
         }
         float mx = fmaxf(max3(x[0], x[1], x[2]), x[3]) * (BITS ? 1.f : p.scale_log2);  // a cache's steps have it in them
-        if (POW2) {
-          // steps beyond what the values take are the weights': the reference is the largest score with that excess in it,
+        if constexpr (BITS > 0) {
+          // steps that fp16 values do not take are the weights': the reference is the largest score with what is left in it,
           // so that the products with them stay in fp16's range
-          const uint4 big = lds16(sb + pt_off_big<HD, BITS>() + ((bs + j) % kPtSteps) * 16);
-          if (big.x | big.y | big.z | big.w) {
+          const uint4 odd = lds16(sb + pt_off_odd<HD, BITS>() + ((bs + j) % kPtSteps) * 16);
+          if (odd.x | odd.y | odd.z | odd.w) {
+            mx = -INFINITY;
 #pragma unroll
             for (int c = 0; c < 4; ++c)
 #pragma unroll
               for (int e = 0; e < 32; e += 4) {
                 const float4 r = steps[32 + 8 * c + e / 4];
-                auto with = [](uint32_t s, float y) {  // y < 2^(n + 1)
-                  return __uint_as_float(s) + (float)max(((__float_as_int(y) >> 23) & 0xff) - 127, 0);
+                auto with = [](uint32_t s, float y) {  // |y| < 2^(n + 1); a step of 0 takes little off, so that sums of weights fit fp32
+                  return __uint_as_float(s) + (float)max(((__float_as_int(y) >> 23) & 0xff) - 127, -60);
                 };
                 mx = max3(mx, with(v[c][e], r.x), with(v[c][e + 1], r.y));
                 mx = max3(mx, with(v[c][e + 2], r.z), with(v[c][e + 3], r.w));
@@ -1006,10 +1017,10 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
         }
         float f = 1.f;
         if (mx > top) {  // also from -inf, with f = 0: nothing to rescale yet
-          const float to = prompt_reference<T, 7>(mx);
+          const float to = prompt_reference<PT, 7>(mx);
           f = ex2(m - to);
           m = to;
-          top = mx + (POW2 ? 7.f : 8.f);  // weights up to 2^15, with a factor below 2 from the values' steps 2^14 before it
+          top = mx + (BITS ? 7.f : 8.f);  // weights up to 2^15, with a factor below 2 from the values' steps 2^14 before it
         }
         const bool rescale = __any_sync(0xffffffffu, f != 1.f) && i > 0;
         if (SEP && i > 0) {  // O += P(j-1) V(j-1) is done: P may be written, O rescaled
@@ -1054,7 +1065,7 @@ __global__ void __launch_bounds__(PtThreads<BITS>::N, 1)
               w0 = __uint_as_float(u0);
               w1 = __uint_as_float(u1);
             }
-            v[c >> 1][(c & 1) * 16 + e / 2] = Act<T>::pack2(w0, w1);
+            v[c >> 1][(c & 1) * 16 + e / 2] = Act<PT>::pack2(w0, w1);
           }
           if (c & 1) tmem_st32(tp + 32 * (c >> 1), v[c >> 1]);
           if (c == 3 || (PARTS == 2 && c == 1)) {

@@ -312,8 +312,8 @@ int ee_cache_read(const ee_cache* cache, void* k, int64_t k_tok, int64_t k_head,
  * zeros; rows of `out` that belong to no sequence stay as they were. A key's
  * code * step counts as it is (NaN where its head held an infinity or NaN), with
  * fp32 statistics and sums. For the product with the values the weights are two
- * 16-bit terms where a call has up to 16 queries x heads per sequence and key
- * head on average, else, and over the prefix, rounded to 16 bits once. Strides in elements, multiples of 8. tq * n_q <
+ * bf16 terms where a call has up to 16 queries x heads per sequence and key head
+ * on average, else rounded to fp16 once, and over the prefix to its type. Strides in elements, multiples of 8. tq * n_q <
  * 2^31 - 255. scale as for ee_prompt_attention.
  * workspace: ee_cache_attention_workspace_bytes() bytes (keys = width *
  * page_size), 16-byte aligned (may be NULL when that is 0); calls

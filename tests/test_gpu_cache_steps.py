@@ -89,3 +89,41 @@ def test_the_largest_steps_under_the_mask(cuda, dtype, bits, hd, nq, which):
     getattr(cache, which)[table[0, 1], 0, 48 - 32] = 2.0 ** 127  # key 48: not seen by queries before the last but one
     assert torch.equal(cache_attention(q, cache, cu, table, kl)[:nq - 2], out[:nq - 2]) and bool(out.isfinite().all())
     assert status() == 0
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("q_len", [[50, 50, 20, 30], [1, 1, 1, 1]])
+def test_steps_below_those_of_fp16(cuda, bits, hd, q_len):
+    """bf16 calls whose values are far below fp16's smallest number, a sequence's all of one size (2^-20, 2^-40 and 2^-70
+    of the usual, within 2^5 of one another), and a sequence of zeros as ``cache_write`` holds them. The weights' rounding
+    to 2^-11, and those that it takes below 2^-14: 2^-25 each beside a largest one of 2^7 or more, on values whose parts
+    that stay with them differ by up to 2^6."""
+    from embodied_efficiency_b200 import cache_attention
+    k_len = [50, 300, 131, 100]
+    q, cache, cu, table, kl, _ = make(cuda, torch.bfloat16, bits, 4, 2, hd, 32, q_len, k_len, 5)
+    for b, e in enumerate((-20, -40, -70)):
+        rows = table[b][table[b] >= 0].long()
+        cache.v_scale[rows] = cache.v_scale[rows].nan_to_num(1.0, 1.0) * 2.0 ** e
+    rows = table[3][table[3] >= 0].long()
+    cache.v[rows], cache.v_scale[rows] = 0, 1e-8
+    out = cache_attention(q, cache, cu, table, kl)
+    i = 0
+    for b, (nq, nk) in enumerate(zip(q_len, k_len)):
+        kd, vd, _ = held(cache, table, b, nk)
+        at = torch.arange(nk, device=cuda)
+        step = cache.v_scale.transpose(1, 2)[table[b].long()[at // 32], at % 32].double().T.repeat_interleave(2, 0)
+        kd, vd = (x.transpose(0, 1).repeat_interleave(2, 0) for x in (kd, vd))
+        qd = q[i:i + nq].double().transpose(0, 1)
+        seen = at[None] <= torch.arange(nq, device=cuda)[:, None] + (nk - nq)
+        p = torch.softmax((qd @ kd.transpose(1, 2) * hd ** -0.5).masked_fill(~seen, float("-inf")), -1)
+        ref, mean = p @ vd, p @ vd.abs()
+        d = (qd.abs() @ kd.abs().transpose(1, 2) * 2 ** -22).amax(-1, keepdim=True)
+        d = (d + qd.abs().amax(-1, keepdim=True) * kd.abs().sum(-1).amax(-1)[:, None, None] * 2 ** -25) * hd ** -0.5
+        small = nk * 2.0 ** -19 * (p * step[:, None]).amax(-1, keepdim=True)
+        tol = (2.0 ** -11 * mean + 2.0 ** -8 * ref.abs()) * (1 + 2 ** -6) + mean * (2 * d + 2 ** -18) + small
+        err = (out[i:i + nq].double().transpose(0, 1) - ref).abs()
+        assert bool((err <= tol).all()), (b, float((err / tol).max()))
+        assert b == 3 or bool(out[i:i + nq].any())
+        i += nq
+    assert not bool(out[sum(q_len[:3]):].any()) and status() == 0
