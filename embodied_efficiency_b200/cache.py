@@ -169,7 +169,8 @@ def cache_attention(q, cache: KVCache, cu_q, table, k_lens, causal: bool = True,
     product with the values the weights keep 16 bits (up to 16 queries x heads a sequence and key head) or 11 (above; then
     a key that counts less than 2^-32 of the row's first may count as 0), over the prefix those of q's type. Returns
     [tokens, heads, head_dim], new or ``out`` (which shares no memory with the inputs); rows that belong to no sequence are
-    not written. Sums are fp32, of weights up to 2^15 before they are divided: values beyond 2^100 can overflow in them.
+    not written. Sums are fp32, of weights up to 2^15 before they are divided: values beyond 2^100 can overflow in
+    them, values below 2^-100 be lost.
     bf16 / fp16."""
     if out is None and type(cache) is KVCache:
         done = (_lib._native or _lib.native()).cache_attention(cache.k, cache._at, q, cu_q, table, k_lens, causal, scale,
